@@ -8,10 +8,16 @@
 - ``b200_attention_softmax`` / ``B200SoftmaxSelfAttention``: the row softmax
   over materialised scores (reference: triton_attention_softmax /
   TritonSelfAttention, also exported under those names)
+- ``b200_tree_attention``, ``b200_cache_*`` / ``PagedKVCache``: attention for drafted
+  tokens (or one token) over a paged key/value cache, and the cache's page
+  operations
 """
 
 from .fused_attention import (DeviceError, b200_fused_attention, check_device_errors,  # noqa: F401
                               clear_device_errors, read_device_errors)
 from .linear import b200_linear  # noqa: F401
+from .paged_cache import (PagedKVCache, b200_cache_accept, b200_cache_append,  # noqa: F401
+                          b200_cache_compact, b200_cache_fork, b200_cache_free,
+                          b200_cache_reserve, b200_tree_attention)
 from .softmax import (B200SoftmaxSelfAttention, TritonSelfAttention,  # noqa: F401
                       b200_attention_softmax, triton_attention_softmax)

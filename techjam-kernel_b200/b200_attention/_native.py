@@ -1,5 +1,5 @@
 """ctypes binding of the C ABI in ``include/b200_attn.h``, ``include/b200_linear.h``,
-``include/b200_layernorm.h`` and ``include/b200_softmax.h``.
+``include/b200_layernorm.h``, ``include/b200_softmax.h`` and ``include/b200_paged.h``.
 
 This module is torch-free: it loads ``libb200_attention.so`` and describes the
 parameter struct.  The library is loaded from this directory only; a missing or
@@ -67,6 +67,25 @@ SOFTMAX_SYMBOLS = (
     "b200_softmax_fwd",
 )
 SOFTMAX_MAX_SEQ = 65536
+
+# Every symbol ``include/b200_paged.h`` declares.
+PAGED_SYMBOLS = (
+    "b200_cache_check",
+    "b200_cache_workspace_bytes",
+    "b200_cache_append",
+    "b200_cache_accept",
+    "b200_cache_reserve",
+    "b200_cache_fork",
+    "b200_cache_free",
+    "b200_cache_compact",
+    "b200_tree_attn_check",
+    "b200_tree_attn_workspace_bytes",
+    "b200_tree_attn_fwd",
+)
+CACHE_MAX_BATCH = 8192
+CACHE_NO_PAGES = 1
+CACHE_ROW_FULL = 2
+CACHE_BAD_ENTRY = 4
 
 LINEAR_ACT_NONE = 0
 LINEAR_ACT_GELU = 1
@@ -176,6 +195,65 @@ class SoftmaxParams(ctypes.Structure):
     ]
 
 
+class Cache(ctypes.Structure):
+    """Mirror of ``b200_cache``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("layers", ctypes.c_int64),
+        ("pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("page_table", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("slots", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("page_refs", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("error_word", ctypes.c_void_p),
+    ]
+
+
+class CacheRows(ctypes.Structure):
+    """Mirror of ``b200_cache_rows``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("counts", ctypes.c_void_p),
+    ]
+
+
+class TreeAttnParams(ctypes.Structure):
+    """Mirror of ``b200_tree_attn_params``."""
+
+    _fields_ = [
+        ("cache", Cache),
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("heads", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("o_stride", ctypes.c_int64 * 3),
+        ("mask", ctypes.c_void_p),
+        ("mask_stride", ctypes.c_int64 * 3),
+        ("draft_lens", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -223,6 +301,22 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.b200_softmax_check.argtypes = [ctypes.POINTER(SoftmaxParams)]
     lib.b200_softmax_fwd.restype = ctypes.c_int32
     lib.b200_softmax_fwd.argtypes = [ctypes.POINTER(SoftmaxParams), ctypes.c_void_p]
+    i32, i64, ptr, cache = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(Cache)
+    tree = ctypes.POINTER(TreeAttnParams)
+    for name, result, args in (
+            ("b200_cache_check", i32, [cache]),
+            ("b200_cache_workspace_bytes", i64, [cache]),
+            ("b200_cache_append", i32, [cache, ctypes.POINTER(CacheRows), ptr]),
+            ("b200_cache_accept", i32, [cache, ptr, i64, i64, ptr, ptr, ptr]),
+            ("b200_cache_reserve", i32, [cache, ptr, i64, ptr, ptr, i64, ptr]),
+            ("b200_cache_fork", i32, [cache, ptr, ptr, i64, ptr]),
+            ("b200_cache_free", i32, [cache, ptr, i64, ptr]),
+            ("b200_cache_compact", i32, [cache, ptr, ptr, i64, ptr]),
+            ("b200_tree_attn_check", i32, [tree]),
+            ("b200_tree_attn_workspace_bytes", i64, [tree]),
+            ("b200_tree_attn_fwd", i32, [tree, ptr])):
+        getattr(lib, name).restype = result
+        getattr(lib, name).argtypes = args
     return lib
 
 

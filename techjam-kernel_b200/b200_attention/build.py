@@ -1,8 +1,8 @@
 """Build the sm_100a attention library in-tree with nvcc.
 
 The shared library is torch-free: it exports the C ABI declared in
-``include/b200_attn.h``, ``include/b200_linear.h``, ``include/b200_layernorm.h``
-and ``include/b200_softmax.h``
+``include/b200_attn.h``, ``include/b200_linear.h``, ``include/b200_layernorm.h``,
+``include/b200_softmax.h`` and ``include/b200_paged.h``
 and links the CUDA runtime statically, so the same file serves the ctypes
 binding here and any other FFI host.
 """
@@ -26,8 +26,9 @@ LIB_PATH = PACKAGE_DIR / LIB_NAME
 # sets B200_ATTN_DEVERR_BOUNDS in the error word instead of faulting).
 CHECKED_LIB_PATH = PACKAGE_DIR / "libb200_attention_checked.so"
 
-SOURCES = ("attn_fwd_sm100.cu", "linear_sm100.cu", "layernorm.cu", "softmax.cu")
-HEADERS = ("sm100_ptx.cuh", "error_word.cuh", "byte_range.h")
+SOURCES = ("attn_fwd_sm100.cu", "linear_sm100.cu", "layernorm.cu", "softmax.cu",
+           "paged_cache.cu", "tree_attn.cu")
+HEADERS = ("sm100_ptx.cuh", "error_word.cuh", "byte_range.h", "paged_host.h", "tree_attn.cuh")
 
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -54,7 +55,7 @@ def _nvcc() -> str:
 def _inputs() -> list[Path]:
     files = [CSRC / s for s in SOURCES] + [CSRC / h for h in HEADERS]
     files += [INCLUDE / h for h in ("b200_attn.h", "b200_linear.h", "b200_layernorm.h",
-                                    "b200_softmax.h")]
+                                    "b200_softmax.h", "b200_paged.h")]
     return files
 
 
@@ -87,8 +88,8 @@ def build_native(force: bool = False, verbose: bool = False, checked: bool = Fal
     return out
 
 
-# The attention operator as a torch custom op (torch.ops.b200.fused_attention)
-# over the same C ABI: a C++ translation unit against torch's headers, linked
+# The attention operator and the paged-cache operators as torch custom ops
+# (torch.ops.b200.*) over the same C ABI: a C++ translation unit against torch's headers, linked
 # to libb200_attention.so found next to it ($ORIGIN).
 TORCH_OP_SOURCE = CSRC / "torch_op.cpp"
 TORCH_OP_PATH = PACKAGE_DIR / "libb200_attention_torch.so"
@@ -98,7 +99,7 @@ def _torch_op_stale() -> bool:
     if not TORCH_OP_PATH.exists():
         return True
     built = TORCH_OP_PATH.stat().st_mtime
-    deps = (TORCH_OP_SOURCE, INCLUDE / "b200_attn.h", LIB_PATH)
+    deps = (TORCH_OP_SOURCE, INCLUDE / "b200_attn.h", INCLUDE / "b200_paged.h", LIB_PATH)
     return any(f.stat().st_mtime > built for f in deps if f.exists())
 
 

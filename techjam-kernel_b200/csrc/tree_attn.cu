@@ -1,0 +1,370 @@
+// tree_attn.cu — attention for drafted tokens over a paged key/value cache:
+// entry points, and the kernel for 32-bit caches.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "b200_paged.h"
+#include "byte_range.h"
+#include "error_word.cuh"
+#include "paged_host.h"
+#include "tree_attn.cuh"
+
+namespace b200tree {
+
+namespace {
+
+// ------------------------------------------------------------ plain kernel
+// 16 rows by 64 keys a tile, fp32 multiply-adds: scores from shared memory, one
+// pass over the keys with the running maximum and sum, the products' sums in
+// registers.
+constexpr int kRows = 16, kKeys = 64, kThreads = 128;
+
+template <int DP>
+struct PlainSmem {
+  float q[kRows][DP + 4];
+  float k[kKeys][DP + 4];
+  float v[kKeys][DP];
+  float p[kRows][kKeys + 1];
+  float m[kRows], l[kRows], alpha[kRows];
+  int page[kKeys];
+  int64_t sums[kThreads / 32];
+  Start start;
+};
+
+template <int DP, int DT>
+__global__ void __launch_bounds__(kThreads) plain_kernel(const Args a) {
+  using E = Elem<DT>;
+  constexpr int kPer16 = 16 / E::kBytes;
+  extern __shared__ __align__(16) uint8_t raw[];
+  PlainSmem<DP>& sm = *reinterpret_cast<PlainSmem<DP>*>(raw);
+  b200attn::ptx::launch_dependents();
+  b200attn::ptx::grid_dependency_wait();
+  const int tid = threadIdx.x;
+  find_start<kRows, kKeys>(a, blockIdx.x, gridDim.x, sm.sums, &sm.start);
+  zero_unused_rows(a, E::kBytes);
+  const Line line(sm.start.total, gridDim.x);
+  if (blockIdx.x >= line.runs) return;
+  int64_t at = line.begin(blockIdx.x);
+  const int64_t end = line.begin(blockIdx.x + 1);
+  Place pl = sm.start.p;
+
+  constexpr int kColGroups = kThreads / DP;         // row groups of the second product
+  constexpr int kRowsPer = kRows / (kColGroups > 0 ? kColGroups : 1);
+  const int col = tid % DP, rg = tid / DP;
+  const int pieces = a.head_dim / kPer16;
+  while (at < end) {
+    // ---- one unit, from key tile pl.t on
+    const int rows = min(kRows, pl.s.drafts * a.group - pl.rt * kRows);
+    const int t0 = pl.t;
+    const int n = static_cast<int>(min(static_cast<int64_t>(pl.tiles - t0), end - at));
+    const int keys = pl.s.len + pl.s.drafts;
+    auto row_ptr = [&](const uint8_t* base, int64_t seq, int64_t head, int64_t tok, int r) {
+      const int row = pl.rt * kRows + r;
+      return base + pl.b * seq + (pl.h * a.group + row % a.group) * head + (row / a.group) * tok;
+    };
+    for (int x = tid; x < kRows * DP; x += kThreads) sm.q[x / DP][x % DP] = 0.f;
+    __syncthreads();
+    for (int x = tid; x < rows * a.head_dim; x += kThreads) {
+      const int r = x / a.head_dim, c = x - r * a.head_dim;
+      const uint8_t* src = row_ptr(a.q, a.q_seq, a.q_head, a.q_tok, r);
+      sm.q[r][c] = E::widen(reinterpret_cast<const typename E::T*>(src)[c]) * a.scale_log2;
+    }
+    if (tid < kRows) {
+      sm.m[tid] = -INFINITY;
+      sm.l[tid] = 0.f;
+    }
+    float acc[kRowsPer] = {};
+    for (int t = t0; t < t0 + n; ++t) {
+      const int k0 = t * kKeys;
+      __syncthreads();
+      if (tid < kKeys) {
+        const int key = k0 + tid;
+        int page = -1;
+        if (key < keys) {
+          page = a.table[pl.b * a.table_stride + key / a.page_size];
+          if (page < 0 || page >= a.pages) {
+            report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
+            page = -1;
+          }
+        }
+        sm.page[tid] = page;
+      }
+      __syncthreads();
+      for (int x = tid; x < kKeys * (DP / kPer16); x += kThreads) {
+        const int key = x / (DP / kPer16), c = x % (DP / kPer16);
+        const int page = sm.page[key];
+        float kv[kPer16] = {}, vv[kPer16] = {};
+        if (page >= 0 && c < pieces) {
+          const int64_t row = (k0 + key) % a.page_size;
+          const uint4 kw = *reinterpret_cast<const uint4*>(a.k + page * a.k_page + pl.h * a.k_head +
+                                                           row * a.k_row + 16 * c);
+          const uint4 vw = *reinterpret_cast<const uint4*>(a.v + page * a.v_page + pl.h * a.v_head +
+                                                           row * a.v_row + 16 * c);
+#pragma unroll
+          for (int u = 0; u < kPer16; ++u) {
+            kv[u] = E::widen(reinterpret_cast<const typename E::T*>(&kw)[u]);
+            vv[u] = E::widen(reinterpret_cast<const typename E::T*>(&vw)[u]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kPer16; ++u) {
+          sm.k[key][c * kPer16 + u] = kv[u];
+          sm.v[key][c * kPer16 + u] = vv[u];
+        }
+      }
+      __syncthreads();
+      {  // scores: this thread's key, 8 rows
+        const int key = tid & (kKeys - 1), r0 = (tid / kKeys) * (kRows / 2);
+        float s[kRows / 2] = {};
+        for (int c = 0; c < DP; c += 4) {
+          const float4 kk = *reinterpret_cast<const float4*>(&sm.k[key][c]);
+#pragma unroll
+          for (int r = 0; r < kRows / 2; ++r) {
+            const float4 qq = *reinterpret_cast<const float4*>(&sm.q[r0 + r][c]);
+            s[r] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[r]))));
+          }
+        }
+        const int j = k0 + key - pl.s.len;  // place in the draft
+#pragma unroll
+        for (int r = 0; r < kRows / 2; ++r) {
+          const int i = (pl.rt * kRows + r0 + r) / a.group;
+          const bool shown = r0 + r < rows && sm.page[key] >= 0 &&
+                             (j < 0 || (j < pl.s.drafts && sees(a, pl.b, i, j)));
+          sm.p[r0 + r][key] = shown ? s[r] : -INFINITY;
+        }
+      }
+      __syncthreads();
+      {  // softmax step: a warp takes 4 rows
+        const int lane = tid & 31, warp = tid >> 5;
+        for (int r = warp * 4; r < warp * 4 + 4; ++r) {
+          const float x0 = sm.p[r][lane], x1 = sm.p[r][lane + 32];
+          float top = fmaxf(x0, x1);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float old = sm.m[r], now = fmaxf(old, top);
+          const float base = now == -INFINITY ? 0.f : now;
+          const float p0 = exp2f(x0 - base), p1 = exp2f(x1 - base);
+          float sum = p0 + p1;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          __syncwarp();
+          sm.p[r][lane] = p0;
+          sm.p[r][lane + 32] = p1;
+          if (lane == 0) {
+            const float alpha = exp2f(old - base);
+            sm.alpha[r] = alpha;
+            sm.m[r] = now;
+            sm.l[r] = sm.l[r] * alpha + sum;
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < kRowsPer; ++r) acc[r] *= sm.alpha[rg * kRowsPer + r];
+      for (int key = 0; key < kKeys; ++key) {
+        const float vv = sm.v[key][col];
+#pragma unroll
+        for (int r = 0; r < kRowsPer; ++r) {
+          // a weight of zero leaves out its row, whatever it holds
+          const float p = sm.p[rg * kRowsPer + r][key];
+          acc[r] = fmaf(p, p == 0.f ? 0.f : vv, acc[r]);
+        }
+      }
+    }
+    __syncthreads();
+    // ---- finished, or a partial result
+    if (t0 == 0 && n == pl.tiles) {
+      if (col < a.head_dim) {
+#pragma unroll
+        for (int r = 0; r < kRowsPer; ++r) {
+          const int rr = rg * kRowsPer + r;
+          if (rr < rows) {
+            const float l = sm.l[rr];
+            uint8_t* dst = const_cast<uint8_t*>(row_ptr(a.o, a.o_seq, a.o_head, a.o_tok, rr));
+            reinterpret_cast<typename E::T*>(dst)[col] = E::round(l == 0.f ? 0.f : acc[r] / l);
+          }
+        }
+      }
+    } else {
+      float* part = a.partial + static_cast<int64_t>(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) *
+                                    (kRows * (DP + 2));
+#pragma unroll
+      for (int r = 0; r < kRowsPer; ++r) part[(rg * kRowsPer + r) * DP + col] = acc[r];
+      if (tid < kRows) {
+        part[kRows * DP + tid] = sm.m[tid];
+        part[kRows * DP + kRows + tid] = sm.l[tid];
+      }
+    }
+    if (tid == 0 && t0 + n == pl.tiles)
+      a.desc[unit_of(a, pl)] =
+          make_int2(t0 == 0 ? static_cast<int>(blockIdx.x) : line.owner(at - t0),
+                    static_cast<int>(blockIdx.x));
+    at += n;
+    if (at < end) next_unit<kRows, kKeys>(a, pl);
+    __syncthreads();
+  }
+}
+
+// -------------------------------------------------------------------- host
+using namespace b200paged;
+
+int64_t round16(int64_t n) { return (n + 15) & ~static_cast<int64_t>(15); }
+
+// Row tile, key tile and padded head dim of the kernel a call takes, and the
+// most CTAs it may run.
+struct Choice {
+  int rm, tn, dp;
+  int ctas_per_sm;
+};
+
+Choice choose(const b200_tree_attn_params* p) {
+  return Choice{kRows, kKeys, p->cache.head_dim <= 64 ? 64 : 128, p->cache.head_dim <= 64 ? 4 : 2};
+}
+
+int64_t row_tiles(const b200_tree_attn_params* p, const Choice& c) {
+  return (p->tokens * (p->heads / p->cache.kv_heads) + c.rm - 1) / c.rm;
+}
+
+constexpr int64_t kMaxRuns = 148 * 8;
+
+// CTAs of a call on a GPU of `sms` SMs: no more than there can be key tiles.
+int64_t runs_of(const b200_tree_attn_params* p, const Choice& c, int64_t sms) {
+  const int64_t keys = p->cache.slots * p->cache.page_size;
+  const double tiles = static_cast<double>(p->cache.batch * p->cache.kv_heads) *
+                       static_cast<double>(row_tiles(p, c)) *
+                       static_cast<double>((keys + c.tn - 1) / c.tn);
+  const int64_t most = sms * c.ctas_per_sm < kMaxRuns ? sms * c.ctas_per_sm : kMaxRuns;
+  return tiles < static_cast<double>(most) ? static_cast<int64_t>(tiles) : most;
+}
+
+int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
+  return round16(8 * p->cache.batch * p->cache.kv_heads * row_tiles(p, c));
+}
+
+
+template <int DP, int DT>
+int32_t run_plain(const Args& a, int runs, int64_t units, int device, cudaStream_t s) {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  std::call_once(once[device], [&] {
+    err[device] = cudaFuncSetAttribute(plain_kernel<DP, DT>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(sizeof(PlainSmem<DP>)));
+  });
+  if (err[device] != cudaSuccess) {
+    set_error(cudaGetErrorString(err[device]));
+    return B200_ATTN_ERR_LAUNCH;
+  }
+  const int32_t rc = launch(plain_kernel<DP, DT>, dim3(runs), dim3(kThreads),
+                            sizeof(PlainSmem<DP>), s, a);
+  if (rc != B200_ATTN_OK) return rc;
+  return launch(join_kernel<kRows, DP, DT>,
+                dim3(static_cast<unsigned>(units), (kRows + kJoinWarps - 1) / kJoinWarps),
+                dim3(32 * kJoinWarps), 0, s, a);
+}
+
+template <int DT>
+int32_t run_type(const Choice& c, const Args& a, int runs, int64_t units, int device,
+                 cudaStream_t s) {
+  return c.dp == 64 ? run_plain<64, DT>(a, runs, units, device, s)
+                    : run_plain<128, DT>(a, runs, units, device, s);
+}
+
+}  // namespace
+}  // namespace b200tree
+
+using namespace b200tree;
+
+extern "C" int32_t b200_tree_attn_check(const b200_tree_attn_params* p) {
+  if (!p) return B200_ATTN_ERR_INVALID_ARGUMENT;
+  const b200_cache& c = p->cache;
+  const int32_t rc = b200_cache_check(&c);
+  if (rc != B200_ATTN_OK) return rc;
+  if (!c.seq_lens || !p->q || !p->o || c.layers != 1 || p->tokens < 1 || p->heads < 1 || p->heads % c.kv_heads ||
+      p->reserved != 0)
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return B200_ATTN_ERR_INVALID_ARGUMENT;
+  // rows, units and row pieces of a call are numbered in 32 bits
+  if (p->tokens > (1 << 24) || p->heads > (1 << 16) || p->tokens * p->heads > (1ll << 25) ||
+      c.batch * p->heads * p->tokens > 0x7fffffffll)
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
+  const int64_t extent[3] = {c.batch, p->heads, p->tokens};
+  const int64_t eb = b200paged::elem_bytes(c.dtype);
+  if (!b200paged::vectors_aligned(p->q, p->q_stride, extent, 3, eb) ||
+      !b200paged::vectors_aligned(p->o, p->o_stride, extent, 3, eb) ||
+      (reinterpret_cast<uintptr_t>(p->draft_lens) & 3u))
+    return B200_ATTN_ERR_ALIGNMENT;
+  if (p->mask && (p->mask_stride[0] < 0 || p->mask_stride[1] < 0 || p->mask_stride[2] < 0))
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
+  return B200_ATTN_OK;
+}
+
+extern "C" int64_t b200_tree_attn_workspace_bytes(const b200_tree_attn_params* p) {
+  if (b200_tree_attn_check(p) != B200_ATTN_OK) return 0;
+  const Choice c = choose(p);
+  return desc_bytes(p, c) + 2 * runs_of(p, c, kMaxRuns) * 4 * c.rm * (c.dp + 2);
+}
+
+extern "C" int32_t b200_tree_attn_fwd(const b200_tree_attn_params* p, void* stream) {
+  int32_t rc = b200_tree_attn_check(p);
+  if (rc != B200_ATTN_OK) return rc;
+  if (!p->workspace || p->workspace_bytes < b200_tree_attn_workspace_bytes(p))
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(p->workspace) & 15u) return B200_ATTN_ERR_ALIGNMENT;
+  const b200_cache& c = p->cache;
+  b200paged::DeviceScope scope;
+  if ((rc = scope.enter(p->q, "q is not a device pointer")) != B200_ATTN_OK) return rc;
+  const Choice ch = choose(p);
+  const int64_t eb = b200paged::elem_bytes(c.dtype);
+  Args a{};
+  if ((rc = b200attn::resolve_error_word(c.error_word, &a.err)) != B200_ATTN_OK) return rc;
+  a.k = static_cast<const uint8_t*>(c.k);
+  a.v = static_cast<const uint8_t*>(c.v);
+  a.k_page = c.k_stride[1] * eb;
+  a.k_head = c.k_stride[2] * eb;
+  a.k_row = c.k_stride[3] * eb;
+  a.v_page = c.v_stride[1] * eb;
+  a.v_head = c.v_stride[2] * eb;
+  a.v_row = c.v_stride[3] * eb;
+  a.table = c.page_table;
+  a.table_stride = c.table_stride;
+  a.lens = c.seq_lens;
+  a.drafts = p->draft_lens;
+  a.q = static_cast<const uint8_t*>(p->q);
+  a.o = static_cast<uint8_t*>(p->o);
+  a.q_seq = p->q_stride[0] * eb;
+  a.q_head = p->q_stride[1] * eb;
+  a.q_tok = p->q_stride[2] * eb;
+  a.o_seq = p->o_stride[0] * eb;
+  a.o_head = p->o_stride[1] * eb;
+  a.o_tok = p->o_stride[2] * eb;
+  a.mask = p->mask;
+  a.m_seq = p->mask_stride[0];
+  a.m_row = p->mask_stride[1];
+  a.m_col = p->mask_stride[2];
+  a.batch = static_cast<int32_t>(c.batch);
+  a.kv_heads = static_cast<int32_t>(c.kv_heads);
+  a.group = static_cast<int32_t>(p->heads / c.kv_heads);
+  a.tokens = static_cast<int32_t>(p->tokens);
+  a.head_dim = static_cast<int32_t>(c.head_dim);
+  a.slots = static_cast<int32_t>(c.slots);
+  a.pages = static_cast<int32_t>(c.pages);
+  a.page_size = static_cast<int32_t>(c.page_size);
+  a.row_tiles = static_cast<int32_t>(row_tiles(p, ch));
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.desc = static_cast<int2*>(p->workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + desc_bytes(p, ch));
+  const int runs = static_cast<int>(runs_of(p, ch, b200paged::sm_count(scope.device)));
+  const int64_t units = c.batch * c.kv_heads * row_tiles(p, ch);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (c.dtype) {
+    case B200_ATTN_DTYPE_BF16:
+      return run_type<B200_ATTN_DTYPE_BF16>(ch, a, runs, units, scope.device, s);
+    case B200_ATTN_DTYPE_FP16:
+      return run_type<B200_ATTN_DTYPE_FP16>(ch, a, runs, units, scope.device, s);
+    default:
+      return run_type<B200_ATTN_DTYPE_FP32>(ch, a, runs, units, scope.device, s);
+  }
+}

@@ -10,6 +10,7 @@
 #include "error_word.cuh"
 #include "paged_host.h"
 #include "tree_attn.cuh"
+#include "tree_attn_rows.cuh"
 
 namespace b200tree {
 
@@ -214,13 +215,18 @@ int64_t round16(int64_t n) { return (n + 15) & ~static_cast<int64_t>(15); }
 
 // Row tile, key tile and padded head dim of the kernel a call takes, and the
 // most CTAs it may run.
+enum Kernel { kPlain, kFewRows };
 struct Choice {
+  Kernel kernel;
   int rm, tn, dp;
   int ctas_per_sm;
 };
 
 Choice choose(const b200_tree_attn_params* p) {
-  return Choice{kRows, kKeys, p->cache.head_dim <= 64 ? 64 : 128, p->cache.head_dim <= 64 ? 4 : 2};
+  const int dp = p->cache.head_dim <= 64 ? 64 : 128;
+  if (p->cache.dtype == B200_ATTN_DTYPE_FP32) return Choice{kPlain, kRows, kKeys, dp, dp == 64 ? 4 : 2};
+  const int64_t rows = p->tokens * (p->heads / p->cache.kv_heads);
+  return Choice{kFewRows, rows <= 16 ? 16 : 32, kRowTile, dp, 1};
 }
 
 int64_t row_tiles(const b200_tree_attn_params* p, const Choice& c) {
@@ -244,32 +250,48 @@ int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
 }
 
 
-template <int DP, int DT>
-int32_t run_plain(const Args& a, int runs, int64_t units, int device, cudaStream_t s) {
+// One kernel over the runs, one that joins the units that were cut.
+template <int RM, int DP, int DT>
+int32_t run_pair(void (*kernel)(Args), int threads, int smem, const Args& a, int runs, int64_t units,
+                 int device, cudaStream_t s) {
   static std::once_flag once[kMaxDevices];
   static cudaError_t err[kMaxDevices];
   std::call_once(once[device], [&] {
-    err[device] = cudaFuncSetAttribute(plain_kernel<DP, DT>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(sizeof(PlainSmem<DP>)));
+    err[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (err[device] != cudaSuccess) {
     set_error(cudaGetErrorString(err[device]));
     return B200_ATTN_ERR_LAUNCH;
   }
-  const int32_t rc = launch(plain_kernel<DP, DT>, dim3(runs), dim3(kThreads),
-                            sizeof(PlainSmem<DP>), s, a);
+  const int32_t rc = launch(kernel, dim3(runs), dim3(threads), smem, s, a);
   if (rc != B200_ATTN_OK) return rc;
-  return launch(join_kernel<kRows, DP, DT>,
-                dim3(static_cast<unsigned>(units), (kRows + kJoinWarps - 1) / kJoinWarps),
+  return launch(join_kernel<RM, DP, DT>,
+                dim3(static_cast<unsigned>(units), (RM + kJoinWarps - 1) / kJoinWarps),
                 dim3(32 * kJoinWarps), 0, s, a);
+}
+
+template <int DP, int DT>
+int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int device,
+                  cudaStream_t s) {
+  if constexpr (DT == B200_ATTN_DTYPE_FP32) {
+    return run_pair<kRows, DP, DT>(plain_kernel<DP, DT>, kThreads, sizeof(PlainSmem<DP>), a, runs,
+                                   units, device, s);
+  } else {
+    using One = RowShape<1, DP>;
+    using Two = RowShape<2, DP>;
+    if (c.rm == 16)
+      return run_pair<16, DP, DT>(rows_kernel<One, DT>, kRowThreads, One::kSmemBytes, a, runs,
+                                  units, device, s);
+    return run_pair<32, DP, DT>(rows_kernel<Two, DT>, kRowThreads, Two::kSmemBytes, a, runs, units,
+                                device, s);
+  }
 }
 
 template <int DT>
 int32_t run_type(const Choice& c, const Args& a, int runs, int64_t units, int device,
                  cudaStream_t s) {
-  return c.dp == 64 ? run_plain<64, DT>(a, runs, units, device, s)
-                    : run_plain<128, DT>(a, runs, units, device, s);
+  return c.dp == 64 ? run_width<64, DT>(c, a, runs, units, device, s)
+                    : run_width<128, DT>(c, a, runs, units, device, s);
 }
 
 }  // namespace
@@ -296,6 +318,10 @@ extern "C" int32_t b200_tree_attn_check(const b200_tree_attn_params* p) {
       !b200paged::vectors_aligned(p->o, p->o_stride, extent, 3, eb) ||
       (reinterpret_cast<uintptr_t>(p->draft_lens) & 3u))
     return B200_ATTN_ERR_ALIGNMENT;
+  // so are the key tiles of one CTA
+  if (static_cast<double>(c.batch * p->heads * p->tokens) *
+          static_cast<double>(c.slots * c.page_size) > 1e14)
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
   if (p->mask && (p->mask_stride[0] < 0 || p->mask_stride[1] < 0 || p->mask_stride[2] < 0))
     return B200_ATTN_ERR_INVALID_ARGUMENT;
   return B200_ATTN_OK;

@@ -27,7 +27,7 @@ LIB_PATH = PACKAGE_DIR / LIB_NAME
 CHECKED_LIB_PATH = PACKAGE_DIR / "libb200_attention_checked.so"
 
 SOURCES = ("attn_fwd_sm100.cu", "linear_sm100.cu", "layernorm.cu", "softmax.cu",
-           "paged_cache.cu", "tree_attn.cu")
+           "paged_cache.cu", "tree_attn.cu", "tree_attn_sm100.cu")
 HEADERS = ("sm100_ptx.cuh", "error_word.cuh", "byte_range.h", "paged_host.h", "tree_attn.cuh",
            "tree_attn_rows.cuh")
 

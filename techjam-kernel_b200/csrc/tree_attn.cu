@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const Args a) {
   b200attn::ptx::grid_dependency_wait();
   const int tid = threadIdx.x;
   find_start<kRows, kKeys>(a, blockIdx.x, gridDim.x, sm.sums, &sm.start);
-  zero_unused_rows(a, E::kBytes);
+  zero_unused_rows(a, E::kBytes, kThreads);
   const Line line(sm.start.total, gridDim.x);
   if (blockIdx.x >= line.runs) return;
   int64_t at = line.begin(blockIdx.x);
@@ -215,17 +215,29 @@ int64_t round16(int64_t n) { return (n + 15) & ~static_cast<int64_t>(15); }
 
 // Row tile, key tile and padded head dim of the kernel a call takes, and the
 // most CTAs it may run.
-enum Kernel { kPlain, kFewRows };
+enum Kernel { kPlain, kFewRows, kManyRows };
 struct Choice {
   Kernel kernel;
   int rm, tn, dp;
   int ctas_per_sm;
 };
 
+// The pools can be gathered by tensor maps: boxes of 8 rows or more, and
+// strides that move.
+bool gather_boxes(const b200_cache& c) {
+  if (box_rows_of(c.page_size) < 8) return false;
+  const int64_t extent[4] = {1, c.pages, c.kv_heads, c.page_size};
+  for (int d = 1; d < 4; ++d)
+    if (extent[d] > 1 && (c.k_stride[d] <= 0 || c.v_stride[d] <= 0)) return false;
+  return true;
+}
+
 Choice choose(const b200_tree_attn_params* p) {
   const int dp = p->cache.head_dim <= 64 ? 64 : 128;
   if (p->cache.dtype == B200_ATTN_DTYPE_FP32) return Choice{kPlain, kRows, kKeys, dp, dp == 64 ? 4 : 2};
   const int64_t rows = p->tokens * (p->heads / p->cache.kv_heads);
+  if (rows > 32 && gather_boxes(p->cache))
+    return Choice{kManyRows, rows <= 128 ? 128 : 256, 128, dp, 1};
   return Choice{kFewRows, rows <= 16 ? 16 : 32, kRowTile, dp, 1};
 }
 
@@ -250,10 +262,16 @@ int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
 }
 
 
-// One kernel over the runs, one that joins the units that were cut.
 template <int RM, int DP, int DT>
-int32_t run_pair(void (*kernel)(Args), int threads, int smem, const Args& a, int runs, int64_t units,
-                 int device, cudaStream_t s) {
+int32_t run_join(const Args& a, int64_t units, cudaStream_t s) {
+  return launch(join_kernel<RM, DP, DT>,
+                dim3(static_cast<unsigned>(units), (RM + kJoinWarps - 1) / kJoinWarps),
+                dim3(32 * kJoinWarps), 0, s, a);
+}
+
+template <int RM, int DP, int DT>
+int32_t run_one(void (*kernel)(Args), int threads, int smem, const Args& a, int runs, int device,
+                cudaStream_t s) {
   static std::once_flag once[kMaxDevices];
   static cudaError_t err[kMaxDevices];
   std::call_once(once[device], [&] {
@@ -263,27 +281,36 @@ int32_t run_pair(void (*kernel)(Args), int threads, int smem, const Args& a, int
     set_error(cudaGetErrorString(err[device]));
     return B200_ATTN_ERR_LAUNCH;
   }
-  const int32_t rc = launch(kernel, dim3(runs), dim3(threads), smem, s, a);
-  if (rc != B200_ATTN_OK) return rc;
-  return launch(join_kernel<RM, DP, DT>,
-                dim3(static_cast<unsigned>(units), (RM + kJoinWarps - 1) / kJoinWarps),
-                dim3(32 * kJoinWarps), 0, s, a);
+  return launch(kernel, dim3(runs), dim3(threads), smem, s, a);
 }
 
+// One kernel over the runs, one that joins the units that were cut.
 template <int DP, int DT>
 int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int device,
                   cudaStream_t s) {
+  int32_t rc;
   if constexpr (DT == B200_ATTN_DTYPE_FP32) {
-    return run_pair<kRows, DP, DT>(plain_kernel<DP, DT>, kThreads, sizeof(PlainSmem<DP>), a, runs,
-                                   units, device, s);
+    rc = run_one<16, DP, DT>(plain_kernel<DP, DT>, kThreads, sizeof(PlainSmem<DP>), a, runs, device,
+                             s);
+    return rc != B200_ATTN_OK ? rc : run_join<kRows, DP, DT>(a, units, s);
   } else {
     using One = RowShape<1, DP>;
     using Two = RowShape<2, DP>;
-    if (c.rm == 16)
-      return run_pair<16, DP, DT>(rows_kernel<One, DT>, kRowThreads, One::kSmemBytes, a, runs,
-                                  units, device, s);
-    return run_pair<32, DP, DT>(rows_kernel<Two, DT>, kRowThreads, Two::kSmemBytes, a, runs, units,
-                                device, s);
+    if (c.kernel == kManyRows)
+      rc = launch_tiles(c.rm, c.dp, DT, a, runs, device, s);
+    else if (c.rm == 16)
+      rc = run_one<16, DP, DT>(rows_kernel<One, DT>, kRowThreads, One::kSmemBytes, a, runs, device,
+                               s);
+    else
+      rc = run_one<32, DP, DT>(rows_kernel<Two, DT>, kRowThreads, Two::kSmemBytes, a, runs, device,
+                               s);
+    if (rc != B200_ATTN_OK) return rc;
+    switch (c.rm) {
+      case 16: return run_join<16, DP, DT>(a, units, s);
+      case 32: return run_join<32, DP, DT>(a, units, s);
+      case 128: return run_join<128, DP, DT>(a, units, s);
+      default: return run_join<256, DP, DT>(a, units, s);
+    }
   }
 }
 

@@ -187,13 +187,14 @@ __device__ __forceinline__ void find_start(const Args& a, int64_t run, int64_t r
 
 // The drafted tokens i >= n_b of the sequences that this CTA looks after get
 // zero rows (sequences without drafted tokens have no unit at all).
-__device__ __forceinline__ void zero_unused_rows(const Args& a, int elem_bytes) {
+// `threads`: the first threads of the CTA, which call this.
+__device__ __forceinline__ void zero_unused_rows(const Args& a, int elem_bytes, int threads) {
   const int heads = a.kv_heads * a.group;
   const int pieces = a.head_dim * elem_bytes / 16;
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
     const Seq s = seq_of(a, b);
     const int n = (a.tokens - s.drafts) * heads * pieces;
-    for (int x = threadIdx.x; x < n; x += blockDim.x) {
+    for (int x = threadIdx.x; x < n; x += threads) {
       const int row = x / pieces;
       const int i = s.drafts + row / heads;
       uint8_t* dst = a.o + b * a.o_seq + (row % heads) * a.o_head + i * a.o_tok;
@@ -278,5 +279,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Args a) {
   for (int x = 0; x < kCols; ++x)
     if (lane + 32 * x < a.head_dim) dst[lane + 32 * x] = E::round(acc[x] * inv);
 }
+
+// Host side of tree_attn_sm100.cu: the row tiles of 128 or 256, and the largest
+// power of two up to 128 that divides a page (the kernel takes 8 and more).
+int32_t launch_tiles(int rm, int dp, int dtype, const Args& a, int runs, int device,
+                     cudaStream_t s);
+int box_rows_of(int64_t page_size);
 
 }  // namespace b200tree

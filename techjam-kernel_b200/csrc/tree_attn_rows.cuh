@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const Args a) {
   find_start<RM, kRowTile>(a, blockIdx.x, gridDim.x, sums, start);
   const Line line(start->total, gridDim.x);
   if (blockIdx.x >= line.runs) {
-    zero_unused_rows(a, 2);
+    zero_unused_rows(a, 2, kRowThreads);
     return;
   }
   int64_t at = line.begin(blockIdx.x);
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const Args a) {
   };
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s) issue();
-  zero_unused_rows(a, 2);
+  zero_unused_rows(a, 2, kRowThreads);
 
   // ------------------------------------------------------------- queries
   constexpr int kQPieces = RM * S::kPieces / kRowThreads > 0 ? RM * S::kPieces / kRowThreads : 1;

@@ -1,0 +1,790 @@
+// tree_attn_sm100.cu — drafted-token attention for many rows (more than 32 a
+// key head), 16-bit caches, on the fifth-generation tensor cores: wide trees,
+// and pieces of prompts over a cache.
+//
+// A CTA owns one run of the line of key tiles (tree_attn.cuh).  Twelve warps:
+//   warps 0-3, 4-7  two softmax groups, one thread per row = one TMEM lane
+//   warp 8          TMA producer: K and V tiles of 128 keys into a ring
+//   warp 9          tcgen05 issuer of the scores, owner of the tensor memory
+//   warp 10         tcgen05 issuer of the weighted values (warp 11 idle)
+// The last four warps hand registers to the softmax groups, whose threads hold a
+// row of 128 scores: 384 x 168 at launch = 256 x 216 + 128 x 72.
+// Tensor memory: S (128 columns, shared) | P0 P1 (64 each) | O0 O1 (DP each).
+// With up to 128 rows (kTwo false) both groups hold the same rows and take the
+// key tiles in turn, each with its own maximum, sum and output sums, joined in
+// tensor memory at the end of the unit: the scores of the next tile are formed
+// while this one's are exponentiated, although there is only one row tile.
+// With up to 256 rows (kTwo) each group has its own 128 rows and every key tile
+// serves both, so a key is read once for 256 rows.
+// A key tile is gathered from its pages by boxes of gcd(page_size, 128) rows,
+// one box a lane of the producer; a box past the last key reads page number
+// `pages`, which is out of range and arrives as zeros.  The ring runs on over
+// unit borders.
+// Every wait is bounded (about a second); when one runs out, the CTA reports it in
+// the error word, waits (bounded) for its own copies and products, frees its
+// tensor memory and returns.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <cstdint>
+#include <mutex>
+
+#include "paged_host.h"
+#include "tree_attn.cuh"
+
+namespace b200tree {
+namespace {
+
+namespace ptx = b200attn::ptx;
+
+constexpr int kThreads = 384;
+constexpr int kSoftmaxThreads = 256;
+constexpr int kLoadWarp = 8, kQkWarp = 9, kPvWarp = 10;
+constexpr int kTile = 128;  // keys of a tile, rows of a row tile
+constexpr uint32_t kTmemCols = 512;
+constexpr uint64_t kWaitNs = 1000000000ull;
+constexpr float kRescale = 8.0f;  // output sums are rescaled when the maximum grew by 2^8
+constexpr int kIssuerSpin = 4096;  // polls of an issuer before its suspending wait
+
+template <int DP_, bool kTwo_>
+struct TileShape {
+  static constexpr int DP = DP_;
+  static constexpr bool kTwo = kTwo_;
+  static constexpr int RM = kTwo ? 256 : 128;
+  static constexpr int kChunks = DP / 64;                  // 128-byte swizzle blocks of a row
+  static constexpr int kChunkBytes = kTile * 128;
+  static constexpr int kTileBytes = kChunks * kChunkBytes;  // a Q, K or V tile
+  static constexpr int kPieces = DP / 8;                   // 16-byte pieces of a row
+  static constexpr int kQTiles = kTwo ? 2 : 1;
+  static constexpr int kSlots = DP == 128 ? (kTwo ? 5 : 6) : (kTwo ? 10 : 12);
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffRing = kQTiles * kTileBytes;
+  static constexpr int kOffSums = kOffRing + kSlots * kTileBytes;
+  static constexpr int kOffStart = kOffSums + 8 * 12;  // one sum a warp
+  static constexpr int kOffBar = kOffStart + 48;
+  static constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kSlots,
+                       kBarSFull = kBarEmpty + kSlots, kBarSFree = kBarSFull + 2,
+                       kBarPFull = kBarSFree + 2, kBarPvDone = kBarPFull + 2,
+                       kBarDrain = kBarPvDone + 2, kBars = kBarDrain + 1;
+  static constexpr int kOffMisc = kOffBar + 8 * kBars;
+  static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
+  static_assert(kSmemBytes <= 232448, "exceeds the shared memory of a block");
+  static constexpr uint32_t kColP = 128, kColO = 256;
+  static_assert(kColO + 2 * DP <= kTmemCols, "exceeds the tensor memory");
+};
+
+__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                       int32_t* err) {
+  const uint64_t t0 = ptx::globaltimer_ns();
+  while (true) {
+#pragma unroll 1
+    for (int k = 0; k < 32; ++k)
+      if (ptx::mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (ptx::globaltimer_ns() - t0 > kWaitNs) {
+      *abort_flag = 1u;
+      report_error(err, B200_ATTN_DEVERR_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity,
+                                         volatile uint32_t* abort_flag, int32_t* err) {
+  return ptx::mbar_try_wait(bar, parity) || wait_slow(bar, parity, abort_flag, err);
+}
+
+__device__ __forceinline__ bool issuer_wait(uint32_t bar, uint32_t parity,
+                                            volatile uint32_t* abort_flag, int32_t* err) {
+#pragma unroll 1
+  for (int k = 0; k < kIssuerSpin; ++k)
+    if (ptx::mbar_test_wait(bar, parity)) return true;
+  return wait_bar(bar, parity, abort_flag, err);
+}
+
+// By every lane; the result is the same for the warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity,
+                                          volatile uint32_t* abort_flag, int32_t* err) {
+  const bool all = __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, err));
+  if (!all) *abort_flag = 1u;
+  return all;
+}
+
+__device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
+  ptx::tc_fence_before();
+  __syncwarp();
+  if (lane == 0) ptx::mbar_arrive(bar);
+}
+
+// Two tensor-memory columns of this thread's lane.
+__device__ __forceinline__ void st_pair(uint32_t addr, uint32_t x, uint32_t y) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void ld_pair(uint32_t addr, uint32_t& x, uint32_t& y) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];"
+               : "=r"(x), "=r"(y)
+               : "r"(addr));
+}
+
+// Waits (bounded) for a barrier without regard to the abort flag.
+__device__ __forceinline__ void settle(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = ptx::globaltimer_ns();
+  while (!ptx::mbar_try_wait(bar, parity) && ptx::globaltimer_ns() - t0 < kWaitNs) {
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (DT == B200_ATTN_DTYPE_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (DT == B200_ATTN_DTYPE_BF16)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t kExp = DT == B200_ATTN_DTYPE_BF16 ? 0x7f807f80u : 0x7c007c00u;
+  return __vcmpeq2(w & kExp, kExp);
+}
+
+template <class S, int DT>
+__global__ void __launch_bounds__(kThreads, 1)
+    tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                 const Args a, const int32_t box_rows) {
+  constexpr int DP = S::DP, NS = S::kSlots, RM = S::RM;
+  constexpr bool kTwo = S::kTwo, kBF16 = DT == B200_ATTN_DTYPE_BF16;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = ptx::smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Start* start = reinterpret_cast<Start*>(smem + S::kOffStart);
+  // misc[0] tensor memory base, [1] abort flag, [2] last segment with a value that is not finite
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem + S::kOffMisc);
+  volatile uint32_t* abort_flag = misc + 1;
+  auto bar = [&](int i) { return sbase + S::kOffBar + 8u * static_cast<uint32_t>(i); };
+
+  ptx::launch_dependents();
+  if (threadIdx.x == 0) {
+    misc[1] = 0u;
+    misc[2] = 0u;
+    ptx::mbar_init(bar(S::kBarQ), 8);
+    for (int s = 0; s < NS; ++s) {
+      ptx::mbar_init(bar(S::kBarFull + s), 1);
+      ptx::mbar_init(bar(S::kBarEmpty + s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(bar(S::kBarSFull + i), 1);
+      ptx::mbar_init(bar(S::kBarSFree + i), 4);
+      ptx::mbar_init(bar(S::kBarPFull + i), 4);
+      ptx::mbar_init(bar(S::kBarPvDone + i), 1);
+    }
+    ptx::mbar_init(bar(S::kBarDrain), 2);
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+    ptx::tma_prefetch_desc(&tm_k);
+    ptx::tma_prefetch_desc(&tm_v);
+  }
+  ptx::grid_dependency_wait();
+  find_start<RM, kTile>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem + S::kOffSums),
+                        start);
+  const Line line(start->total, gridDim.x);
+  if (blockIdx.x >= line.runs) {
+    zero_unused_rows(a, 2, kThreads);
+    return;
+  }
+  if (warp == kQkWarp) {
+    ptx::tmem_alloc(sbase + S::kOffMisc, kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = misc[0];
+  const int64_t begin = line.begin(blockIdx.x), end = line.begin(blockIdx.x + 1);
+  Place pl = start->p;
+
+  // Tiles of the segment that starts at line position `at`, and of those the
+  // ones of softmax group i.
+  auto seg_tiles = [&](int64_t at) {
+    return static_cast<int>(min(static_cast<int64_t>(pl.tiles - pl.t), end - at));
+  };
+  auto unit_rows = [&](const Place& p) { return min(RM, p.s.drafts * a.group - p.rt * RM); };
+  // group i takes tile j of a segment
+  auto takes = [&](int i, int j, int rows) {
+    return kTwo ? (i == 0 || rows > kTile) : (j & 1) == i;
+  };
+
+  if (warp >= kLoadWarp) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------ TMA producer
+    const int boxes = kTile / box_rows;
+    const int u = lane % boxes, chunk = lane / boxes;
+    const bool mine = chunk < S::kChunks;
+    const uint32_t part = chunk * S::kChunkBytes + u * box_rows * 128;
+    const uint32_t size = static_cast<uint32_t>(a.page_size);
+    int page = 0, row = 0;
+    auto look_up = [&]() {
+      const int key = pl.t * kTile + u * box_rows;
+      page = a.pages;
+      row = 0;
+      if (mine && key < pl.s.len + pl.s.drafts) {
+        const uint32_t slot = static_cast<uint32_t>(key) / size;
+        page = __ldg(a.table + pl.b * a.table_stride + slot);
+        row = static_cast<int>(static_cast<uint32_t>(key) - slot * size);
+      }
+    };
+    look_up();
+    uint32_t load = 0;
+    bool ok = true;
+    for (int64_t at = begin; ok && at < end; ++at) {
+      if (page < 0 || page > a.pages || (page == a.pages && mine &&
+                                         pl.t * kTile + u * box_rows < pl.s.len + pl.s.drafts)) {
+        report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
+        page = a.pages;
+      }
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t s = load % NS;
+        if (!warp_wait(bar(S::kBarEmpty + s), ((load / NS) & 1u) ^ 1u, abort_flag, a.err)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) ptx::mbar_arrive_expect_tx(bar(S::kBarFull + s), S::kTileBytes);
+        __syncwarp();
+        if (mine)
+          ptx::tma_load_4d(sbase + S::kOffRing + s * S::kTileBytes + part, kv ? &tm_v : &tm_k,
+                           bar(S::kBarFull + s), 64 * chunk, row, pl.h, page);
+        ++load;
+      }
+      if (ok && at + 1 < end) {
+        if (++pl.t == pl.tiles) next_unit<RM, kTile>(a, pl);
+        look_up();
+      }
+    }
+    if (!ok) {
+      // copies in flight land before the shared memory goes
+      for (uint32_t x = load > NS ? load - NS : 0u; x < load; ++x)
+        settle(bar(S::kBarFull + x % NS), (x / NS) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == kQkWarp) {
+    // -------------------------------------------------- scores S = Q K^T
+    if (lane == 0) {
+      constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, kTile, false);
+      uint32_t tile = 0, seg = 0, made[2] = {0u, 0u};
+      int prev = -1;
+      bool ok = true;
+      for (int64_t at = begin; ok && at < end; ++seg) {
+        const int n = seg_tiles(at), rows = unit_rows(pl);
+        ok = wait_bar(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
+        for (int j = 0; ok && j < n; ++j, ++tile) {
+          const uint32_t load = 2u * tile, s = load % NS;
+          ok = wait_bar(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!ok || !takes(i, j, rows)) continue;
+            // the scores before these have been copied to registers
+            if (prev >= 0 && !issuer_wait(bar(S::kBarSFree + prev), (made[prev] - 1u) & 1u,
+                                          abort_flag, a.err)) {
+              ok = false;
+              continue;
+            }
+            ptx::tc_fence_after();
+            const uint32_t qa = sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes;
+            const uint32_t ka = sbase + S::kOffRing + s * S::kTileBytes;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * S::kChunkBytes + (kk & 3) * 32;
+              ptx::tc_mma_ss(tmem, ptx::smem_desc_sw128(qa + off, 16, 1024),
+                             ptx::smem_desc_sw128(ka + off, 16, 1024), id, kk > 0 ? 1u : 0u);
+            }
+            ptx::tc_commit(bar(S::kBarSFull + i));
+            ++made[i];
+            prev = i;
+          }
+          if (ok) ptx::tc_commit(bar(S::kBarEmpty + s));
+        }
+        at += n;
+        pl.t += n;
+        if (at < end) next_unit<RM, kTile>(a, pl);
+      }
+      ptx::tc_commit(bar(S::kBarDrain));
+      settle(bar(S::kBarDrain), 0);
+    }
+    __syncwarp();
+  } else if (warp == kPvWarp) {
+    // ------------------------------------------------------- O_i += P_i V
+    if (lane == 0) {
+      constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, DP, true);
+      uint32_t tile = 0, made[2] = {0u, 0u};
+      bool ok = true;
+      for (int64_t at = begin; ok && at < end;) {
+        const int n = seg_tiles(at), rows = unit_rows(pl);
+        bool fresh[2] = {true, true};
+        for (int j = 0; ok && j < n; ++j, ++tile) {
+          const uint32_t load = 2u * tile + 1u, s = load % NS;
+          ok = wait_bar(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err);
+          const uint32_t va = sbase + S::kOffRing + s * S::kTileBytes;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!ok || !takes(i, j, rows)) continue;
+            if (!issuer_wait(bar(S::kBarPFull + i), made[i] & 1u, abort_flag, a.err)) {
+              ok = false;
+              continue;
+            }
+            ptx::tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + S::kColP + 64 * i + kk * 8,
+                             ptx::smem_desc_sw128(va + kk * 2048, S::kChunkBytes, 1024), id,
+                             (!fresh[i] || kk > 0) ? 1u : 0u);
+            ptx::tc_commit(bar(S::kBarPvDone + i));
+            fresh[i] = false;
+            ++made[i];
+          }
+          if (ok) ptx::tc_commit(bar(S::kBarEmpty + s));
+        }
+        at += n;
+        pl.t += n;
+        if (at < end) next_unit<RM, kTile>(a, pl);
+      }
+      ptx::tc_commit(bar(S::kBarDrain));
+      settle(bar(S::kBarDrain), 0);
+    }
+    __syncwarp();
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // ------------------------------------------------------------ softmax
+    const int i = warp >> 2, quad = warp & 3, rl = quad * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t tS = tmem + lanes, tP = tS + S::kColP + 64 * i, tO = tS + S::kColO;
+    const int pieces = a.head_dim / 8;
+    const uint32_t size = static_cast<uint32_t>(a.page_size);
+    // this thread's part of the queries: its row of its row tile; where both groups
+    // hold the same rows, half of it each
+    constexpr int kMine = kTwo ? S::kPieces : S::kPieces / 2;
+    const int p0 = kTwo ? 0 : i * kMine;
+    const int row0 = kTwo ? i * kTile : 0;  // first row of this group in the unit
+    uint4 qreg[kMine];
+    auto fetch_q = [&](const Place& p) {
+      const bool have = row0 + rl < unit_rows(p);
+      const int row = p.rt * RM + row0 + rl, tok = row / a.group;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          a.q + p.b * a.q_seq + (p.h * a.group + row - tok * a.group) * a.q_head + tok * a.q_tok);
+#pragma unroll
+      for (int x = 0; x < kMine; ++x) {
+        qreg[x] = make_uint4(0u, 0u, 0u, 0u);
+        if (have && p0 + x < pieces) qreg[x] = __ldg(src + p0 + x);
+      }
+    };
+    auto store_q = [&]() {
+      const uint32_t base = sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes + rl * 128;
+#pragma unroll
+      for (int x = 0; x < kMine; ++x) {
+        const int p = p0 + x;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                         base + (p >> 3) * S::kChunkBytes + (((p & 7) ^ (rl & 7)) << 4)),
+                     "r"(qreg[x].x), "r"(qreg[x].y), "r"(qreg[x].z), "r"(qreg[x].w)
+                     : "memory");
+      }
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(S::kBarQ));
+    };
+    fetch_q(pl);
+    store_q();
+    zero_unused_rows(a, 2, kSoftmaxThreads);
+
+    uint32_t tile = 0, seg = 0, cnt = 0;  // tiles of the run, segments, tiles of this group
+    bool ok = true;
+    for (int64_t at = begin; ok && at < end; ++seg) {
+      const int n = seg_tiles(at), rows = unit_rows(pl), t0 = pl.t;
+      const int len = pl.s.len, keys = len + pl.s.drafts;
+      const int first_row = pl.rt * RM + row0 + quad * 32;  // of this warp
+      const bool idle = row0 + quad * 32 >= rows;           // the warp's rows are padding
+      const int my_tok = min((first_row + lane) / a.group, a.tokens - 1);
+      auto clean = [&](int j, int k0) {
+        if (kTwo && i != 0) return true;
+        // Values past the last key become 0 (their rows may hold anything, and
+        // 0 x infinity would reach the sums), and so do elements of drafted
+        // values that are not finite: those are added below to the rows that
+        // see them.  In kTwo the second group's product of this tile is
+        // issued after this group's, which waits for this.
+        const uint32_t load = 2u * (tile + j) + 1u, s = load % NS;
+        if (!warp_wait(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err)) {
+          return false;
+        }
+        const int r0 = max(0, len - k0);
+        bool odd = false;
+        for (int x = quad * 32 + lane; x < (kTile - r0) * S::kPieces; x += kTile) {
+          const int r = r0 + x / S::kPieces, pc = x % S::kPieces;
+          const uint32_t ad = sbase + S::kOffRing + s * S::kTileBytes + (pc >> 3) * S::kChunkBytes +
+                              r * 128 + ((pc & 7) << 4);
+          uint32_t w[4] = {0u, 0u, 0u, 0u};
+          bool put = k0 + r >= keys;
+          if (!put) {
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(ad)
+                         : "memory");
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const uint32_t f = not_finite<DT>(w[y]);
+              put |= f != 0u;
+              w[y] &= ~f;
+            }
+            odd |= put;
+          }
+          if (put)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ad), "r"(w[0]),
+                         "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+        }
+        if (odd) misc[2] = seg + 1u;
+        ptx::fence_proxy_async_smem();
+        return true;
+      };
+      float m_run = -INFINITY, l_run = 0.f;
+      int done = 0;
+      for (int j = 0; j < n; ++j) {
+        if (!takes(i, j, rows)) continue;
+        if (!warp_wait(bar(S::kBarSFull + i), cnt & 1u, abort_flag, a.err)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const int k0 = (t0 + j) * kTile;
+        if (idle) {  // nothing to compute, but the barriers count this warp
+          warp_arrive(bar(S::kBarSFree + i), lane);
+          ok = cnt == 0 || warp_wait(bar(S::kBarPvDone + i), (cnt - 1u) & 1u, abort_flag, a.err);
+          if (ok && k0 + kTile > len) ok = clean(j, k0);
+          if (!ok) break;
+          warp_arrive(bar(S::kBarPFull + i), lane);
+          ++cnt;
+          continue;
+        }
+        uint32_t sr[kTile];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          ptx::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * c]));
+        ptx::tmem_wait_ld();
+        warp_arrive(bar(S::kBarSFree + i), lane);
+        if (k0 + kTile > len) {
+          // drafted tokens and places past the last key: one word of 32 keys at a
+          // time, the lanes reading a token's mask row together
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int key = k0 + 32 * q;
+            uint32_t word = 0u;
+            if (key + 32 <= len) {
+              word = ~0u;
+            } else if (key < keys) {
+              const int d = key + lane - len;
+              const int tok0 = first_row / a.group;
+              const int tok1 = min((first_row + 31) / a.group, a.tokens - 1);
+              for (int tok = tok0; tok <= tok1; ++tok) {
+                const bool shown = d < 0 || (d < pl.s.drafts && sees(a, pl.b, tok, d));
+                const uint32_t w = __ballot_sync(0xffffffffu, shown);
+                if (tok == my_tok) word = w;
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!((word >> k) & 1u)) sr[32 * q + k] = __float_as_uint(-INFINITY);
+          }
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < kTile; k += 4) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) top[y] = fmaxf(top[y], __uint_as_float(sr[k + y]));
+        }
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+        const bool resc = mx > m_run + kRescale || (m_run == -INFINITY && mx > m_run);
+        const float m_new = resc ? mx : m_run;
+        const float alpha = resc ? ptx::ex2_approx(m_run - m_new) : 1.f;
+        m_run = m_new;
+        l_run *= alpha;
+        uint32_t pk[kTile / 2];
+        const float neg = m_run == -INFINITY ? 0.f : -m_run;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < kTile / 2; ++e) {
+          const float x = ptx::ex2_approx(fmaf(__uint_as_float(sr[2 * e]), a.scale_log2, neg));
+          const float y = ptx::ex2_approx(fmaf(__uint_as_float(sr[2 * e + 1]), a.scale_log2, neg));
+          // the sum is taken of the rounded weights, which the product uses
+          pk[e] = pack2<DT>(x, y);
+          const float2 r = unpack2<DT>(pk[e]);
+          sum[2 * (e & 1)] += r.x;
+          sum[2 * (e & 1) + 1] += r.y;
+        }
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // P_i was last read by the product before this one
+        if (cnt > 0) {
+          if (!warp_wait(bar(S::kBarPvDone + i), (cnt - 1u) & 1u, abort_flag, a.err)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+        }
+        if (done > 0 && __any_sync(0xffffffffu, resc)) {
+#pragma unroll
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32b_x32(tO + DP * i + 32 * c, o);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            ptx::tmem_st_32x32b_x32(tO + DP * i + 32 * c, o);
+          }
+        }
+        ptx::tmem_st_32x32b_x32(tP, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
+        ptx::tmem_st_32x32b_x32(tP + 32, *reinterpret_cast<uint32_t(*)[32]>(&pk[32]));
+        ptx::tmem_wait_st();
+        if (k0 + kTile > len && !clean(j, k0)) {
+          ok = false;
+          break;
+        }
+        warp_arrive(bar(S::kBarPFull + i), lane);
+        ++cnt;
+        ++done;
+      }
+      if (ok && cnt > 0) ok = warp_wait(bar(S::kBarPvDone + i), (cnt - 1u) & 1u, abort_flag, a.err);
+      // ---------------------------------------------------- end of a segment
+      if (!kTwo && ok) {
+        // the other group reads this row's maximum and sum where P_i was
+        st_pair(tP, __float_as_uint(m_run), __float_as_uint(l_run));
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+      }
+      ok = ptx::named_barrier_and(1, kSoftmaxThreads, ok);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const Place unit = pl;
+      const bool first = t0 == 0, last = t0 + n == pl.tiles;
+      const int64_t unit_begin = at - t0;
+      const bool any_odd = misc[2] == seg + 1u;
+      at += n;
+      tile += n;
+      if (at < end) {
+        next_unit<RM, kTile>(a, pl);
+        fetch_q(pl);  // on its way while the results are written
+      }
+      // weights of the groups' sums in this thread's row
+      float top = m_run, total = l_run, w[2] = {1.f, 1.f};
+      if constexpr (!kTwo) {
+        uint32_t om, ol;
+        ld_pair(tS + S::kColP + 64 * (1 - i), om, ol);
+        ptx::tmem_wait_ld();
+        const float m_other = __uint_as_float(om);
+        top = fmaxf(m_run, m_other);
+        const float mine_w = m_run == -INFINITY ? 0.f : ptx::ex2_approx(m_run - top);
+        const float other_w = m_other == -INFINITY ? 0.f : ptx::ex2_approx(m_other - top);
+        total = mine_w * l_run + other_w * __uint_as_float(ol);
+        w[0] = i == 0 ? mine_w : other_w;
+        w[1] = i == 0 ? other_w : mine_w;
+      }
+      const bool mine = row0 + rl < rows;
+      const bool finish = first && last;
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      const int row = unit.rt * RM + row0 + rl, tok = min(row / a.group, a.tokens - 1);
+      uint8_t* out = a.o + unit.b * a.o_seq + (unit.h * a.group + row % a.group) * a.o_head +
+                     tok * a.o_tok;
+      float* part = a.partial +
+                    static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * (RM * (DP + 2));
+      if (!idle) {
+        // kTwo: all columns of the own rows; else half the columns of the shared ones
+        constexpr int kSpan = kTwo ? DP : DP / 2;
+#pragma unroll
+        for (int c = 0; c < kSpan / 32; ++c) {
+          const int col = (kTwo ? 0 : i * kSpan) + 32 * c;
+          uint32_t o[32];
+          float acc[32];
+          if constexpr (kTwo) {
+            ptx::tmem_ld_32x32b_x32(tO + DP * i + col, o);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[e] = __uint_as_float(o[e]);
+          } else {
+            ptx::tmem_ld_32x32b_x32(tO + col, o);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[e] = w[0] * __uint_as_float(o[e]);
+            if (n > 1) {
+              ptx::tmem_ld_32x32b_x32(tO + DP + col, o);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) acc[e] += w[1] * __uint_as_float(o[e]);
+            }
+          }
+          if (any_odd && mine) {
+            // this segment's drafted values that are not finite, for rows that see them
+            const int d1 = min(unit.s.drafts, (t0 + n) * kTile - len);
+            for (int d = max(0, t0 * kTile - len); d < d1; ++d) {
+              if (!sees(a, unit.b, tok, d)) continue;
+              const uint32_t key = len + d, slot = key / size;
+              const int pg = a.table[unit.b * a.table_stride + slot];
+              if (pg < 0 || pg >= a.pages) continue;
+              const uint32_t* v = reinterpret_cast<const uint32_t*>(
+                  a.v + pg * a.v_page + unit.h * a.v_head +
+                  static_cast<int64_t>(key - slot * size) * a.v_row + 2 * col);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                if (col + 2 * e >= a.head_dim) continue;
+                const uint32_t x = v[e], f = not_finite<DT>(x);
+                const float2 y = unpack2<DT>(x);
+                if (f & 0xffffu) acc[2 * e] += y.x;
+                if (f >> 16) acc[2 * e + 1] += y.y;
+              }
+            }
+          }
+          if (finish) {
+            if (mine) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (col + 8 * e < a.head_dim)
+                  *reinterpret_cast<uint4*>(out + 2 * (col + 8 * e)) = make_uint4(
+                      pack2<DT>(acc[8 * e] * inv, acc[8 * e + 1] * inv),
+                      pack2<DT>(acc[8 * e + 2] * inv, acc[8 * e + 3] * inv),
+                      pack2<DT>(acc[8 * e + 4] * inv, acc[8 * e + 5] * inv),
+                      pack2<DT>(acc[8 * e + 6] * inv, acc[8 * e + 7] * inv));
+            }
+          } else if (mine) {
+            float* dst = part + (row0 + rl) * DP + col;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              *reinterpret_cast<float2*>(dst + e) = make_float2(acc[e], acc[e + 1]);
+          }
+        }
+      }
+      if (!finish && mine && (kTwo || i == 0)) {
+        part[RM * DP + row0 + rl] = top;
+        part[RM * DP + RM + row0 + rl] = total;
+      }
+      if (threadIdx.x == 0 && last)
+        a.desc[unit_of(a, unit)] =
+            make_int2(first ? static_cast<int>(blockIdx.x) : line.owner(unit_begin),
+                      static_cast<int>(blockIdx.x));
+      // the sums and the queries of this unit have been read
+      ptx::tc_fence_before();
+      ptx::named_barrier_sync(1, kSoftmaxThreads);
+      if (at < end) store_q();
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == kQkWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// -------------------------------------------------------------------- host
+using namespace b200paged;
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// Map {head_dim, page_size, kv_heads, pages} of a pool, boxes of {64, box_rows, 1, 1}.
+int32_t encode_pool(CUtensorMap* map, const uint8_t* base, int64_t row, int64_t head, int64_t page,
+                    const Args& a, int dtype, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled entry point unavailable");
+    return B200_ATTN_ERR_LAUNCH;
+  }
+  // strides of dimensions with one entry never move the address
+  const int64_t any = a.head_dim * 16;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.page_size),
+                        static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.page_size > 1 ? row : any),
+                           static_cast<cuuint64_t>(a.kv_heads > 1 ? head : any),
+                           static_cast<cuuint64_t>(a.pages > 1 ? page : any)};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(map, dtype == B200_ATTN_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+         4, const_cast<uint8_t*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed");
+    return B200_ATTN_ERR_LAUNCH;
+  }
+  return B200_ATTN_OK;
+}
+
+template <class S, int DT>
+int32_t launch_shape(const CUtensorMap& k, const CUtensorMap& v, const Args& a, int box_rows,
+                     int runs, int device, cudaStream_t s) {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  auto kernel = tiles_kernel<S, DT>;
+  std::call_once(once[device], [&] {
+    err[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       S::kSmemBytes);
+  });
+  if (err[device] != cudaSuccess) {
+    set_error(cudaGetErrorString(err[device]));
+    return B200_ATTN_ERR_LAUNCH;
+  }
+  return launch(kernel, dim3(runs), dim3(kThreads), S::kSmemBytes, s, k, v, a, box_rows);
+}
+
+template <int DP, int DT>
+int32_t launch_rows(bool two, const CUtensorMap& k, const CUtensorMap& v, const Args& a,
+                    int box_rows, int runs, int device, cudaStream_t s) {
+  return two ? launch_shape<TileShape<DP, true>, DT>(k, v, a, box_rows, runs, device, s)
+             : launch_shape<TileShape<DP, false>, DT>(k, v, a, box_rows, runs, device, s);
+}
+
+}  // namespace
+
+int box_rows_of(int64_t page_size) {
+  int g = 1;
+  while (g < kTile && page_size % (2 * g) == 0) g *= 2;
+  return g;
+}
+
+int32_t launch_tiles(int rm, int dp, int dtype, const Args& a, int runs, int device,
+                     cudaStream_t s) {
+  const int g = box_rows_of(a.page_size);
+  CUtensorMap k, v;
+  int32_t rc = encode_pool(&k, a.k, a.k_row, a.k_head, a.k_page, a, dtype, g);
+  if (rc == B200_ATTN_OK) rc = encode_pool(&v, a.v, a.v_row, a.v_head, a.v_page, a, dtype, g);
+  if (rc != B200_ATTN_OK) return rc;
+  const bool two = rm == 256;
+  if (dtype == B200_ATTN_DTYPE_BF16)
+    return dp == 64 ? launch_rows<64, B200_ATTN_DTYPE_BF16>(two, k, v, a, g, runs, device, s)
+                    : launch_rows<128, B200_ATTN_DTYPE_BF16>(two, k, v, a, g, runs, device, s);
+  return dp == 64 ? launch_rows<64, B200_ATTN_DTYPE_FP16>(two, k, v, a, g, runs, device, s)
+                  : launch_rows<128, B200_ATTN_DTYPE_FP16>(two, k, v, a, g, runs, device, s);
+}
+
+}  // namespace b200tree

@@ -35,7 +35,7 @@ struct PlainSmem {
 };
 
 template <int DP, int DT>
-__global__ void __launch_bounds__(kThreads) plain_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__ Args a) {
   using E = Elem<DT>;
   constexpr int kPer16 = 16 / E::kBytes;
   extern __shared__ __align__(16) uint8_t raw[];

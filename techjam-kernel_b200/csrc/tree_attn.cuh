@@ -208,6 +208,43 @@ __device__ __forceinline__ bool sees(const Args& a, int b, int i, int j) {
   return a.mask ? a.mask[b * a.m_seq + i * a.m_row + j * a.m_col] != 0 : j <= i;
 }
 
+// Bit x: whether drafted token i of sequence b (of `drafts`) sees place d0 + x of the
+// draft.  Places before the draft are committed tokens, which it sees.  A row of
+// mask bytes is read as the aligned words that hold it, all at once: a byte at a
+// time, each waiting for its load, these reads took longer than the tile's products.
+__device__ __forceinline__ uint32_t seen_word(const Args& a, int b, int i, int d0, int drafts) {
+  uint32_t word = 0u;
+  int n = drafts - d0;  // bits of the word that lie in the draft or before it
+  if (!a.mask) {
+    n = min(n, i + 1 - d0);
+    word = ~0u;
+  } else {
+    const uint8_t* row = a.mask + b * a.m_seq + i * a.m_row;
+    if (a.m_col == 1) {
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(row), hi = lo + drafts;
+      const uintptr_t at = lo + d0, base = at & ~static_cast<uintptr_t>(3);
+      const uint32_t shift = 8u * static_cast<uint32_t>(at & 3u);
+      uint32_t w[9];
+#pragma unroll
+      for (int x = 0; x < 9; ++x) {
+        const uintptr_t p = base + 4 * x;
+        w[x] = p + 4 > lo && p < hi ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
+      }
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const uint32_t v = __vcmpne4(__funnelshift_r(w[x], w[x + 1], shift), 0u) & 0x01010101u;
+        word |= ((v * 0x10204080u) >> 28) << (4 * x);  // the four bytes' low bits side by side
+      }
+    } else {
+#pragma unroll 8
+      for (int x = 0; x < 32; ++x)
+        if (d0 + x >= 0 && x < n && row[(d0 + x) * a.m_col]) word |= 1u << x;
+    }
+    if (d0 < 0) word |= d0 <= -32 ? ~0u : (1u << -d0) - 1u;
+  }
+  return n >= 32 ? word : (n <= 0 ? 0u : word & ((1u << n) - 1u));
+}
+
 template <int DT>
 struct Elem;
 template <>
@@ -237,7 +274,7 @@ struct Elem<B200_ATTN_DTYPE_FP32> {
 constexpr int kJoinWarps = 8;
 
 template <int RM, int DP, int DT>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Args a) {
   using E = Elem<DT>;
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();

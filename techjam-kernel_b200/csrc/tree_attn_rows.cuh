@@ -106,7 +106,7 @@ struct RowShape {
 };
 
 template <class S, int DT>
-__global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const Args a) {
+__global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_constant__ Args a) {
   constexpr int RM = S::RM, DP = S::DP, MT = S::MT, NS = S::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sbase = b200attn::ptx::smem_u32(smem);

@@ -2,18 +2,20 @@
 // key head), 16-bit caches, on the fifth-generation tensor cores: wide trees,
 // and pieces of prompts over a cache.
 //
-// A CTA owns one run of the line of key tiles (tree_attn.cuh).  Twelve warps:
+// A CTA owns one run of the line of key tiles (tree_attn.cuh).  Eleven warps:
 //   warps 0-3, 4-7  two softmax groups, one thread per row = one TMEM lane
 //   warp 8          TMA producer: K and V tiles of 128 keys into a ring
 //   warp 9          tcgen05 issuer of the scores, owner of the tensor memory
-//   warp 10         tcgen05 issuer of the weighted values (warp 11 idle)
-// The last four warps hand registers to the softmax groups, whose threads hold a
-// row of 128 scores: 384 x 168 at launch = 256 x 216 + 128 x 72.
-// Tensor memory: S (128 columns, shared) | P0 P1 (64 each) | O0 O1 (DP each).
+//   warp 10         tcgen05 issuer of the weighted values
+// Tensor memory: S (128 columns, shared) | P0 P1 (64 each) | O0 O1 (DP each).  A
+// group copies its scores to registers at once, so the next scores are formed
+// while it exponentiates; weights that lie over their scores instead, which
+// would leave S to each group, made every product wait for the one before it
+// (measured 5400 cycles a tile of 256 rows).
 // With up to 128 rows (kTwo false) both groups hold the same rows and take the
 // key tiles in turn, each with its own maximum, sum and output sums, joined in
-// tensor memory at the end of the unit: the scores of the next tile are formed
-// while this one's are exponentiated, although there is only one row tile.
+// tensor memory at the end of the unit: the tensor cores work for one group while
+// the other exponentiates, although there is only one row tile.
 // With up to 256 rows (kTwo) each group has its own 128 rows and every key tile
 // serves both, so a key is read once for 256 rows.
 // A key tile is gathered from its pages by boxes of gcd(page_size, 128) rows,
@@ -38,7 +40,7 @@ namespace {
 
 namespace ptx = b200attn::ptx;
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 352;
 constexpr int kSoftmaxThreads = 256;
 constexpr int kLoadWarp = 8, kQkWarp = 9, kPvWarp = 10;
 constexpr int kTile = 128;  // keys of a tile, rows of a row tile
@@ -64,17 +66,21 @@ struct TileShape {
   static constexpr int kOffStart = kOffSums + 8 * 12;  // one sum a warp
   static constexpr int kOffBar = kOffStart + 48;
   static constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kSlots,
-                       kBarSFull = kBarEmpty + kSlots, kBarSFree = kBarSFull + 2,
-                       kBarPFull = kBarSFree + 2, kBarPvDone = kBarPFull + 2,
-                       kBarDrain = kBarPvDone + 2, kBars = kBarDrain + 1;
+                       kBarScores = kBarEmpty + kSlots, kBarRead = kBarScores + 2,
+                       kBarWeights = kBarRead + 2, kBarSums = kBarWeights + 2,
+                       kBarDrain = kBarSums + 2, kBars = kBarDrain + 1;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of a block");
   static constexpr uint32_t kColP = 128, kColO = 256;
+  // Numbers of the loads, in the order of their use: the scores lead the values by a
+  // tile, K0 K1 V0 K2 V1 ... (the place of the key tile past the last stays empty).
+  __device__ static uint32_t load_k(uint32_t t) { return t ? 2 * t - 1 : 0u; }
+  __device__ static uint32_t load_v(uint32_t t) { return 2 * t + 2; }
   static_assert(kColO + 2 * DP <= kTmemCols, "exceeds the tensor memory");
 };
 
-__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
                                        int32_t* err) {
   const uint64_t t0 = ptx::globaltimer_ns();
   while (true) {
@@ -117,6 +123,24 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
   if (lane == 0) ptx::mbar_arrive(bar);
 }
 
+// 16 tensor-memory columns of this thread's lane.
+__device__ __forceinline__ void st_x16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void ld_x16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
 // Two tensor-memory columns of this thread's lane.
 __device__ __forceinline__ void st_pair(uint32_t addr, uint32_t x, uint32_t y) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y)
@@ -158,10 +182,17 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   return __vcmpeq2(w & kExp, kExp);
 }
 
+// Scores whose bit is not set become -inf.
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t word) {
+#pragma unroll
+  for (int k = 0; k < 32; ++k)
+    if (!((word >> k) & 1u)) s[k] = __float_as_uint(-INFINITY);
+}
+
 template <class S, int DT>
 __global__ void __launch_bounds__(kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                 const Args a, const int32_t box_rows) {
+                 const __grid_constant__ Args a, const int32_t box_rows) {
   constexpr int DP = S::DP, NS = S::kSlots, RM = S::RM;
   constexpr bool kTwo = S::kTwo, kBF16 = DT == B200_ATTN_DTYPE_BF16;
   extern __shared__ uint8_t raw[];
@@ -185,10 +216,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(bar(S::kBarEmpty + s), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(bar(S::kBarSFull + i), 1);
-      ptx::mbar_init(bar(S::kBarSFree + i), 4);
-      ptx::mbar_init(bar(S::kBarPFull + i), 4);
-      ptx::mbar_init(bar(S::kBarPvDone + i), 1);
+      ptx::mbar_init(bar(S::kBarScores + i), 1);
+      ptx::mbar_init(bar(S::kBarRead + i), 4);
+      ptx::mbar_init(bar(S::kBarWeights + i), 4);
+      ptx::mbar_init(bar(S::kBarSums + i), 1);
     }
     ptx::mbar_init(bar(S::kBarDrain), 2);
     ptx::fence_mbar_init();
@@ -226,8 +257,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     return kTwo ? (i == 0 || rows > kTile) : (j & 1) == i;
   };
 
-  if (warp >= kLoadWarp) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == kLoadWarp) {
     // ------------------------------------------------------ TMA producer
     const int boxes = kTile / box_rows;
@@ -235,47 +264,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool mine = chunk < S::kChunks;
     const uint32_t part = chunk * S::kChunkBytes + u * box_rows * 128;
     const uint32_t size = static_cast<uint32_t>(a.page_size);
-    int page = 0, row = 0;
+    struct Box {
+      int page, row, head;
+    };
     auto look_up = [&]() {
       const int key = pl.t * kTile + u * box_rows;
-      page = a.pages;
-      row = 0;
+      Box x{a.pages, 0, pl.h};
       if (mine && key < pl.s.len + pl.s.drafts) {
         const uint32_t slot = static_cast<uint32_t>(key) / size;
-        page = __ldg(a.table + pl.b * a.table_stride + slot);
-        row = static_cast<int>(static_cast<uint32_t>(key) - slot * size);
+        x.page = __ldg(a.table + pl.b * a.table_stride + slot);
+        x.row = static_cast<int>(static_cast<uint32_t>(key) - slot * size);
+        if (x.page >= a.pages) x.page = -1;
       }
+      return x;
     };
-    look_up();
-    uint32_t load = 0;
-    bool ok = true;
-    for (int64_t at = begin; ok && at < end; ++at) {
-      if (page < 0 || page > a.pages || (page == a.pages && mine &&
-                                         pl.t * kTile + u * box_rows < pl.s.len + pl.s.drafts)) {
+    auto load = [&](uint32_t number, const CUtensorMap* map, Box x) {
+      const uint32_t s = number % NS;
+      if (!warp_wait(bar(S::kBarEmpty + s), ((number / NS) & 1u) ^ 1u, abort_flag, a.err))
+        return false;
+      if (x.page < 0) {
         report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
-        page = a.pages;
+        x.page = a.pages;
       }
-      for (int kv = 0; kv < 2; ++kv) {
-        const uint32_t s = load % NS;
-        if (!warp_wait(bar(S::kBarEmpty + s), ((load / NS) & 1u) ^ 1u, abort_flag, a.err)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) ptx::mbar_arrive_expect_tx(bar(S::kBarFull + s), S::kTileBytes);
-        __syncwarp();
-        if (mine)
-          ptx::tma_load_4d(sbase + S::kOffRing + s * S::kTileBytes + part, kv ? &tm_v : &tm_k,
-                           bar(S::kBarFull + s), 64 * chunk, row, pl.h, page);
-        ++load;
+      if (lane == 0) ptx::mbar_arrive_expect_tx(bar(S::kBarFull + s), S::kTileBytes);
+      __syncwarp();
+      if (mine)
+        ptx::tma_load_4d(sbase + S::kOffRing + s * S::kTileBytes + part, map, bar(S::kBarFull + s),
+                         64 * chunk, x.row, x.head, x.page);
+      return true;
+    };
+    // The page numbers of a tile are read while the loads before it are issued, and
+    // serve its keys and, two loads later, its values.
+    const uint32_t tiles = static_cast<uint32_t>(end - begin);
+    Box next = look_up(), before[2] = {next, next};  // of tiles t, and t - 2, t - 1
+    uint32_t issued = 0;                             // one past the last load issued
+    bool ok = true;
+    for (uint32_t t = 0; ok && t < tiles + 2; ++t) {
+      const Box now = next;
+      if (t >= 2) {
+        ok = load(S::load_v(t - 2), &tm_v, before[0]);
+        if (ok) issued = S::load_v(t - 2) + 1;
       }
-      if (ok && at + 1 < end) {
+      before[0] = before[1];
+      before[1] = now;
+      if (!ok || t >= tiles) continue;
+      ok = load(S::load_k(t), &tm_k, now);
+      if (ok) issued = S::load_k(t) + 1;
+      if (ok && t + 1 < tiles) {
         if (++pl.t == pl.tiles) next_unit<RM, kTile>(a, pl);
-        look_up();
+        next = look_up();
       }
     }
     if (!ok) {
       // copies in flight land before the shared memory goes
-      for (uint32_t x = load > NS ? load - NS : 0u; x < load; ++x)
+      for (uint32_t x = issued > NS ? issued - NS : 0u; x < issued; ++x)
         settle(bar(S::kBarFull + x % NS), (x / NS) & 1u);
     }
     __syncwarp();
@@ -290,13 +332,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = seg_tiles(at), rows = unit_rows(pl);
         ok = wait_bar(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
         for (int j = 0; ok && j < n; ++j, ++tile) {
-          const uint32_t load = 2u * tile, s = load % NS;
-          ok = wait_bar(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err);
+          const uint32_t number = S::load_k(tile), s = number % NS;
+          ok = issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (!ok || !takes(i, j, rows)) continue;
             // the scores before these have been copied to registers
-            if (prev >= 0 && !issuer_wait(bar(S::kBarSFree + prev), (made[prev] - 1u) & 1u,
+            if (prev >= 0 && !issuer_wait(bar(S::kBarRead + prev), (made[prev] - 1u) & 1u,
                                           abort_flag, a.err)) {
               ok = false;
               continue;
@@ -310,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               ptx::tc_mma_ss(tmem, ptx::smem_desc_sw128(qa + off, 16, 1024),
                              ptx::smem_desc_sw128(ka + off, 16, 1024), id, kk > 0 ? 1u : 0u);
             }
-            ptx::tc_commit(bar(S::kBarSFull + i));
+            ptx::tc_commit(bar(S::kBarScores + i));
             ++made[i];
             prev = i;
           }
@@ -334,13 +376,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = seg_tiles(at), rows = unit_rows(pl);
         bool fresh[2] = {true, true};
         for (int j = 0; ok && j < n; ++j, ++tile) {
-          const uint32_t load = 2u * tile + 1u, s = load % NS;
-          ok = wait_bar(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err);
+          const uint32_t number = S::load_v(tile), s = number % NS;
+          ok = issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
           const uint32_t va = sbase + S::kOffRing + s * S::kTileBytes;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (!ok || !takes(i, j, rows)) continue;
-            if (!issuer_wait(bar(S::kBarPFull + i), made[i] & 1u, abort_flag, a.err)) {
+            if (!issuer_wait(bar(S::kBarWeights + i), made[i] & 1u, abort_flag, a.err)) {
               ok = false;
               continue;
             }
@@ -350,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + S::kColP + 64 * i + kk * 8,
                              ptx::smem_desc_sw128(va + kk * 2048, S::kChunkBytes, 1024), id,
                              (!fresh[i] || kk > 0) ? 1u : 0u);
-            ptx::tc_commit(bar(S::kBarPvDone + i));
+            ptx::tc_commit(bar(S::kBarSums + i));
             fresh[i] = false;
             ++made[i];
           }
@@ -364,9 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       settle(bar(S::kBarDrain), 0);
     }
     __syncwarp();
-  }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------------------ softmax
     const int i = warp >> 2, quad = warp & 3, rl = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
@@ -378,9 +418,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kMine = kTwo ? S::kPieces : S::kPieces / 2;
     const int p0 = kTwo ? 0 : i * kMine;
     const int row0 = kTwo ? i * kTile : 0;  // first row of this group in the unit
-    uint4 qreg[kMine];
-    auto fetch_q = [&](const Place& p) {
-      const bool have = row0 + rl < unit_rows(p);
+    auto fetch_q = [&](const Place& p, bool more, uint4 (&qreg)[kMine]) {
+      const bool have = more && row0 + rl < unit_rows(p);
       const int row = p.rt * RM + row0 + rl, tok = row / a.group;
       const uint4* src = reinterpret_cast<const uint4*>(
           a.q + p.b * a.q_seq + (p.h * a.group + row - tok * a.group) * a.q_head + tok * a.q_tok);
@@ -390,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (have && p0 + x < pieces) qreg[x] = __ldg(src + p0 + x);
       }
     };
-    auto store_q = [&]() {
+    auto store_q = [&](const uint4 (&qreg)[kMine]) {
       const uint32_t base = sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes + rl * 128;
 #pragma unroll
       for (int x = 0; x < kMine; ++x) {
@@ -404,8 +443,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(S::kBarQ));
     };
-    fetch_q(pl);
-    store_q();
+    {
+      uint4 qreg[kMine];
+      fetch_q(pl, true, qreg);
+      store_q(qreg);
+    }
     zero_unused_rows(a, 2, kSoftmaxThreads);
 
     uint32_t tile = 0, seg = 0, cnt = 0;  // tiles of the run, segments, tiles of this group
@@ -423,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // values that are not finite: those are added below to the rows that
         // see them.  In kTwo the second group's product of this tile is
         // issued after this group's, which waits for this.
-        const uint32_t load = 2u * (tile + j) + 1u, s = load % NS;
+        const uint32_t load = S::load_v(tile + j), s = load % NS;
         if (!warp_wait(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err)) {
           return false;
         }
@@ -461,18 +503,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       int done = 0;
       for (int j = 0; j < n; ++j) {
         if (!takes(i, j, rows)) continue;
-        if (!warp_wait(bar(S::kBarSFull + i), cnt & 1u, abort_flag, a.err)) {
+        if (!warp_wait(bar(S::kBarScores + i), cnt & 1u, abort_flag, a.err)) {
           ok = false;
           break;
         }
         ptx::tc_fence_after();
         const int k0 = (t0 + j) * kTile;
         if (idle) {  // nothing to compute, but the barriers count this warp
-          warp_arrive(bar(S::kBarSFree + i), lane);
-          ok = cnt == 0 || warp_wait(bar(S::kBarPvDone + i), (cnt - 1u) & 1u, abort_flag, a.err);
+          warp_arrive(bar(S::kBarRead + i), lane);
+          ok = cnt == 0 || warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
           if (ok && k0 + kTile > len) ok = clean(j, k0);
           if (!ok) break;
-          warp_arrive(bar(S::kBarPFull + i), lane);
+          warp_arrive(bar(S::kBarWeights + i), lane);
           ++cnt;
           continue;
         }
@@ -481,91 +523,79 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 4; ++c)
           ptx::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * c]));
         ptx::tmem_wait_ld();
-        warp_arrive(bar(S::kBarSFree + i), lane);
-        if (k0 + kTile > len) {
-          // drafted tokens and places past the last key: one word of 32 keys at a
-          // time, the lanes reading a token's mask row together
+        warp_arrive(bar(S::kBarRead + i), lane);
+        // a bit for each key that this row sees
+        const bool partly = k0 + kTile > len;  // drafted tokens, or places past the last key
+        if (partly) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int key = k0 + 32 * q;
-            uint32_t word = 0u;
-            if (key + 32 <= len) {
-              word = ~0u;
-            } else if (key < keys) {
-              const int d = key + lane - len;
-              const int tok0 = first_row / a.group;
-              const int tok1 = min((first_row + 31) / a.group, a.tokens - 1);
-              for (int tok = tok0; tok <= tok1; ++tok) {
-                const bool shown = d < 0 || (d < pl.s.drafts && sees(a, pl.b, tok, d));
-                const uint32_t w = __ballot_sync(0xffffffffu, shown);
-                if (tok == my_tok) word = w;
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (!((word >> k) & 1u)) sr[32 * q + k] = __float_as_uint(-INFINITY);
+            const int d = k0 + 32 * q - len;
+            if (d > -32)
+              hide(*reinterpret_cast<uint32_t(*)[32]>(&sr[32 * q]),
+                   seen_word(a, pl.b, my_tok, d, pl.s.drafts));
           }
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < kTile; k += 4) {
-#pragma unroll
-          for (int y = 0; y < 4; ++y) top[y] = fmaxf(top[y], __uint_as_float(sr[k + y]));
-        }
+        for (int k = 0; k < kTile; ++k) top[k & 3] = fmaxf(top[k & 3], __uint_as_float(sr[k]));
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
         const bool resc = mx > m_run + kRescale || (m_run == -INFINITY && mx > m_run);
         const float m_new = resc ? mx : m_run;
         const float alpha = resc ? ptx::ex2_approx(m_run - m_new) : 1.f;
         m_run = m_new;
         l_run *= alpha;
-        uint32_t pk[kTile / 2];
-        const float neg = m_run == -INFINITY ? 0.f : -m_run;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < kTile / 2; ++e) {
-          const float x = ptx::ex2_approx(fmaf(__uint_as_float(sr[2 * e]), a.scale_log2, neg));
-          const float y = ptx::ex2_approx(fmaf(__uint_as_float(sr[2 * e + 1]), a.scale_log2, neg));
-          // the sum is taken of the rounded weights, which the product uses
-          pk[e] = pack2<DT>(x, y);
-          const float2 r = unpack2<DT>(pk[e]);
-          sum[2 * (e & 1)] += r.x;
-          sum[2 * (e & 1) + 1] += r.y;
-        }
-        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        // P_i was last read by the product before this one
+        // P_i was last read by the product before this one, which also left O_i at rest
         if (cnt > 0) {
-          if (!warp_wait(bar(S::kBarPvDone + i), (cnt - 1u) & 1u, abort_flag, a.err)) {
+          if (!warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err)) {
             ok = false;
             break;
           }
           ptx::tc_fence_after();
         }
         if (done > 0 && __any_sync(0xffffffffu, resc)) {
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x32(tO + DP * i + 32 * c, o);
+#pragma unroll 1
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t o[16];
+            ld_x16(tO + DP * i + 16 * c, o);
             ptx::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            ptx::tmem_st_32x32b_x32(tO + DP * i + 32 * c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            st_x16(tO + DP * i + 16 * c, o);
           }
         }
-        ptx::tmem_st_32x32b_x32(tP, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
-        ptx::tmem_st_32x32b_x32(tP + 32, *reinterpret_cast<uint32_t(*)[32]>(&pk[32]));
+        const float neg = m_run == -INFINITY ? 0.f : -m_run;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // pieces of 32 keys, so that few registers are new
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int k = 32 * c + 2 * e;
+            const float x = ptx::ex2_approx(fmaf(__uint_as_float(sr[k]), a.scale_log2, neg));
+            const float y = ptx::ex2_approx(fmaf(__uint_as_float(sr[k + 1]), a.scale_log2, neg));
+            // the sum is taken of the rounded weights, which the product uses
+            pk[e] = pack2<DT>(x, y);
+            const float2 r = unpack2<DT>(pk[e]);
+            sum[2 * (e & 1)] += r.x;
+            sum[2 * (e & 1) + 1] += r.y;
+          }
+          st_x16(tP + 16 * c, pk);
+        }
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         ptx::tmem_wait_st();
-        if (k0 + kTile > len && !clean(j, k0)) {
+        if (partly && !clean(j, k0)) {
           ok = false;
           break;
         }
-        warp_arrive(bar(S::kBarPFull + i), lane);
+        warp_arrive(bar(S::kBarWeights + i), lane);
         ++cnt;
         ++done;
       }
-      if (ok && cnt > 0) ok = warp_wait(bar(S::kBarPvDone + i), (cnt - 1u) & 1u, abort_flag, a.err);
+      if (ok && cnt > 0) ok = warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
       // ---------------------------------------------------- end of a segment
       if (!kTwo && ok) {
         // the other group reads this row's maximum and sum where P_i was
+        ptx::tc_fence_after();
         st_pair(tP, __float_as_uint(m_run), __float_as_uint(l_run));
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
@@ -579,10 +609,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool any_odd = misc[2] == seg + 1u;
       at += n;
       tile += n;
-      if (at < end) {
-        next_unit<RM, kTile>(a, pl);
-        fetch_q(pl);  // on its way while the results are written
-      }
+      if (at < end) next_unit<RM, kTile>(a, pl);
+      uint4 qreg[kMine];  // the next queries, on their way while the results are written
+      fetch_q(pl, at < end, qreg);
       // weights of the groups' sums in this thread's row
       float top = m_run, total = l_run, w[2] = {1.f, 1.f};
       if constexpr (!kTwo) {
@@ -681,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the sums and the queries of this unit have been read
       ptx::tc_fence_before();
       ptx::named_barrier_sync(1, kSoftmaxThreads);
-      if (at < end) store_q();
+      if (at < end) store_q(qreg);
     }
   }
 

@@ -21,6 +21,7 @@ namespace {
 // pass over the keys with the running maximum and sum, the products' sums in
 // registers.
 constexpr int kRows = 16, kKeys = 64, kThreads = 128;
+using PlainGrid = Grid<kRows, kKeys, 1>;
 
 template <int DP>
 struct PlainSmem {
@@ -31,7 +32,7 @@ struct PlainSmem {
   float m[kRows], l[kRows], alpha[kRows];
   int page[kKeys];
   int64_t sums[kThreads / 32];
-  Start start;
+  Run run;
 };
 
 template <int DP, int DT>
@@ -43,23 +44,20 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
   const int tid = threadIdx.x;
-  find_start<kRows, kKeys>(a, blockIdx.x, gridDim.x, sm.sums, &sm.start);
+  find_run<PlainGrid>(a, blockIdx.x, gridDim.x, sm.sums, &sm.run);
   zero_unused_rows(a, E::kBytes, kThreads);
-  const Line line(sm.start.total, gridDim.x);
-  if (blockIdx.x >= line.runs) return;
-  int64_t at = line.begin(blockIdx.x);
-  const int64_t end = line.begin(blockIdx.x + 1);
-  Place pl = sm.start.p;
+  const Run& run = sm.run;
+  Place pl = run.p;
 
   constexpr int kColGroups = kThreads / DP;         // row groups of the second product
   constexpr int kRowsPer = kRows / (kColGroups > 0 ? kColGroups : 1);
   const int col = tid % DP, rg = tid / DP;
   const int pieces = a.head_dim / kPer16;
-  while (at < end) {
+  while (!run.done(pl)) {
     // ---- one unit, from key tile pl.t on
     const int rows = min(kRows, pl.s.drafts * a.group - pl.rt * kRows);
     const int t0 = pl.t;
-    const int n = static_cast<int>(min(static_cast<int64_t>(pl.tiles - t0), end - at));
+    const int n = run.tiles(pl);
     const int keys = pl.s.len + pl.s.drafts;
     auto row_ptr = [&](const uint8_t* base, int64_t seq, int64_t head, int64_t tok, int r) {
       const int row = pl.rt * kRows + r;
@@ -200,10 +198,10 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
     }
     if (tid == 0 && t0 + n == pl.tiles)
       a.desc[unit_of(a, pl)] =
-          make_int2(t0 == 0 ? static_cast<int>(blockIdx.x) : line.owner(at - t0),
+          make_int2(t0 == 0 ? static_cast<int>(blockIdx.x) : run.first_run,
                     static_cast<int>(blockIdx.x));
-    at += n;
-    if (at < end) next_unit<kRows, kKeys>(a, pl);
+    pl.t += n;
+    if (pl.t == pl.tiles) next_unit<PlainGrid>(a, pl);
     __syncthreads();
   }
 }
@@ -263,10 +261,17 @@ int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
 
 
 template <int RM, int DP, int DT>
-int32_t run_join(const Args& a, int64_t units, cudaStream_t s) {
-  return launch(join_kernel<RM, DP, DT>,
-                dim3(static_cast<unsigned>(units), (RM + kJoinWarps - 1) / kJoinWarps),
+int32_t run_join_rows(const Args& a, int64_t units, cudaStream_t s) {
+  return launch(join_rows_kernel<RM, DP, DT>, dim3(static_cast<unsigned>(units), RM / 4),
                 dim3(32 * kJoinWarps), 0, s, a);
+}
+
+template <int RM, int DP, int DT>
+int32_t run_join_columns(const Args& a, int64_t units, cudaStream_t s) {
+  // few units: the blocks that share a unit's rows share its columns too
+  const unsigned shares = units * (RM / 32) < 300 ? DP / 32 : 1;
+  return launch(join_columns_kernel<RM, DP, DT>,
+                dim3(static_cast<unsigned>(units), RM / 32, shares), dim3(32 * kJoinWarps), 0, s, a);
 }
 
 template <int RM, int DP, int DT>
@@ -292,7 +297,7 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
   if constexpr (DT == B200_ATTN_DTYPE_FP32) {
     rc = run_one<16, DP, DT>(plain_kernel<DP, DT>, kThreads, sizeof(PlainSmem<DP>), a, runs, device,
                              s);
-    return rc != B200_ATTN_OK ? rc : run_join<kRows, DP, DT>(a, units, s);
+    return rc != B200_ATTN_OK ? rc : run_join_rows<kRows, DP, DT>(a, units, s);
   } else {
     using One = RowShape<1, DP>;
     using Two = RowShape<2, DP>;
@@ -306,10 +311,10 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
                                s);
     if (rc != B200_ATTN_OK) return rc;
     switch (c.rm) {
-      case 16: return run_join<16, DP, DT>(a, units, s);
-      case 32: return run_join<32, DP, DT>(a, units, s);
-      case 128: return run_join<128, DP, DT>(a, units, s);
-      default: return run_join<256, DP, DT>(a, units, s);
+      case 16: return run_join_rows<16, DP, DT>(a, units, s);
+      case 32: return run_join_rows<32, DP, DT>(a, units, s);
+      case 128: return run_join_columns<128, DP, DT>(a, units, s);
+      default: return run_join_columns<256, DP, DT>(a, units, s);
     }
   }
 }

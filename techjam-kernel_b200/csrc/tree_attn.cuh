@@ -8,7 +8,8 @@
 // in the order (sequence, key head, row tile, key tile), form one line that is
 // cut into equal runs, one for each CTA, whatever the lengths of the
 // sequences are: one long sequence fills the GPU and a ragged batch has no
-// tail.  A unit that lies inside one run is finished there; one that is cut
+// tail.  What a unit costs beside its tiles (queries in, results out) is counted as
+// EX tiles ahead of its first.  A unit that lies inside one run is finished there; one that is cut
 // leaves partial results (unnormalised sums, row maximum, row sum) that a second
 // kernel joins in the order of the runs, so the result does not depend on timing.
 #pragma once
@@ -69,38 +70,44 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b) {
   return s;
 }
 
-template <int RM, int TN>
-struct Shape {
+// RM rows and TN keys a tile, EX tiles' worth of work beside a unit's tiles.
+template <int RM_, int TN_, int EX_>
+struct Grid {
+  static constexpr int RM = RM_, TN = TN_, EX = EX_;
   __device__ static int key_tiles(const Seq& s) {
     return s.drafts > 0 ? (s.len + s.drafts + TN - 1) / TN : 0;
   }
   __device__ static int row_tiles(const Args& a, const Seq& s) {
     return (s.drafts * a.group + RM - 1) / RM;
   }
+  // places of a sequence in the line
+  __device__ static int64_t places(const Args& a, const Seq& s) {
+    const int t = key_tiles(s);
+    return t == 0 ? 0 : static_cast<int64_t>(t + EX) * row_tiles(a, s) * a.kv_heads;
+  }
 };
 
-// A place in the line of tiles: a key tile of a unit.
+// A key tile of a unit.
 struct Place {
   int b, h, rt, t;     // sequence, key head, row tile, key tile
   int tiles, rts;      // key tiles and row tiles of the sequence
   Seq s;
 };
 
-template <int RM, int TN>
+template <class G>
 __device__ __forceinline__ void enter_seq(const Args& a, Place& p) {
   // the first sequence from p.b on with work; p.b == batch at the end
-  p.tiles = 0;
   while (p.b < a.batch) {
     p.s = seq_of(a, p.b);
-    p.tiles = Shape<RM, TN>::key_tiles(p.s);
-    p.rts = Shape<RM, TN>::row_tiles(a, p.s);
+    p.tiles = G::key_tiles(p.s);
+    p.rts = G::row_tiles(a, p.s);
     if (p.tiles > 0) break;
     ++p.b;
   }
 }
 
-// One unit further.
-template <int RM, int TN>
+// The first tile of the unit after p's.
+template <class G>
 __device__ __forceinline__ void next_unit(const Args& a, Place& p) {
   p.t = 0;
   if (++p.rt < p.rts) return;
@@ -108,46 +115,42 @@ __device__ __forceinline__ void next_unit(const Args& a, Place& p) {
   if (++p.h < a.kv_heads) return;
   p.h = 0;
   ++p.b;
-  enter_seq<RM, TN>(a, p);
+  enter_seq<G>(a, p);
 }
 
 __device__ __forceinline__ int unit_of(const Args& a, const Place& p) {
   return (p.b * a.kv_heads + p.h) * a.row_tiles + p.rt;
 }
 
-// The line of tiles: `total` of them over the CTAs, run c has tiles
-// [begin(c), begin(c + 1)).  No run is empty: with fewer tiles than CTAs the last
-// CTAs have none.
-struct Line {
-  int64_t total;
-  int64_t runs;
-  __device__ Line(int64_t tiles, int64_t ctas) : total(tiles), runs(min(tiles, ctas)) {}
-  __device__ int64_t begin(int64_t c) const { return c * total / runs; }
-  // the run that tile t lies in: the last c with begin(c) <= t
-  __device__ int owner(int64_t t) const { return static_cast<int>(((t + 1) * runs - 1) / total); }
-};
-
-// Start of this CTA's run.  Every thread sums the tiles of its share of the
-// sequences, a scan finds the total, and the thread whose share holds the run's
-// first tile walks to it.  `sums` is scratch for blockDim.x / 32 + 1 values;
-// `out` receives the place.  Ends with a barrier.
-struct Start {
+// A CTA's run: from place `p` up to, not including, tile et of unit (eb, eh, ert).
+// first_run: the run that holds the first tile of p's unit.
+struct Run {
   Place p;
-  int64_t total;
+  int eb, eh, ert, et;
+  int first_run;
+
+  __device__ __forceinline__ bool ends_in(const Place& x) const {
+    return x.b == eb && x.h == eh && x.rt == ert;
+  }
+  __device__ __forceinline__ bool done(const Place& x) const { return ends_in(x) && x.t >= et; }
+  // tiles of the run from x on in x's unit
+  __device__ __forceinline__ int tiles(const Place& x) const {
+    return (ends_in(x) ? et : x.tiles) - x.t;
+  }
 };
 
-template <int RM, int TN>
-__device__ __forceinline__ void find_start(const Args& a, int64_t run, int64_t runs, int64_t* sums,
-                                           Start* out) {
+// Finds this CTA's run.  Every thread counts the places of its share of the
+// sequences, a scan finds the total, and the threads whose shares hold the run's
+// first place and the next run's walk to them.  `sums`: scratch of one value a warp.
+// Ends with a barrier; *out is in shared memory.
+template <class G>
+__device__ __forceinline__ void find_run(const Args& a, int64_t run, int64_t ctas, int64_t* sums,
+                                         Run* out) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.batch + nt - 1) / nt;
   const int b0 = min(a.batch, tid * each), b1 = min(a.batch, b0 + each);
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Seq s = seq_of(a, b);
-    mine += static_cast<int64_t>(Shape<RM, TN>::key_tiles(s)) * Shape<RM, TN>::row_tiles(a, s) *
-            a.kv_heads;
-  }
+  for (int b = b0; b < b1; ++b) mine += G::places(a, seq_of(a, b));
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -161,26 +164,43 @@ __device__ __forceinline__ void find_start(const Args& a, int64_t run, int64_t r
     if (w < warp) before += sums[w];
     total += sums[w];
   }
-  const Line line(total, runs);
-  if (tid == 0) out->total = total;
-  const int64_t first = run < line.runs ? line.begin(run) : total;
-  if (mine > 0 && first >= before && first < before + mine) {
-    int64_t left = first - before;
-    Place p{};
-    for (int b = b0; b < b1; ++b) {
-      p.b = b;
-      p.s = seq_of(a, b);
-      p.tiles = Shape<RM, TN>::key_tiles(p.s);
-      p.rts = Shape<RM, TN>::row_tiles(a, p.s);
-      const int64_t all = static_cast<int64_t>(p.tiles) * p.rts * a.kv_heads;
-      if (left < all) break;
-      left -= all;
+  // runs [c total / runs, (c + 1) total / runs): none is empty of places
+  const int64_t runs = min(total, ctas);
+  for (int end = 0; end < 2; ++end) {
+    const int64_t at = run + end < runs ? (run + end) * total / runs : total;
+    Place p{a.batch, 0, 0, 0, 0, 0, {0, 0}};
+    int first_run = 0;
+    if (at == total) {
+      if (tid != 0) continue;
+    } else {
+      if (mine == 0 || at < before || at >= before + mine) continue;
+      int64_t left = at - before;
+      for (p.b = b0; p.b < b1; ++p.b) {
+        p.s = seq_of(a, p.b);
+        const int64_t all = G::places(a, p.s);
+        if (left < all) break;
+        left -= all;
+      }
+      p.tiles = G::key_tiles(p.s);
+      p.rts = G::row_tiles(a, p.s);
+      const int span = p.tiles + G::EX;
+      const int x = static_cast<int>(left % span);
+      const int u = static_cast<int>(left / span);
+      p.t = max(0, x - G::EX);
+      p.rt = u % p.rts;
+      p.h = u / p.rts;
+      // the last run that begins at or before the unit's first tile
+      first_run = static_cast<int>(((at - x + G::EX + 1) * runs - 1) / total);
     }
-    p.t = static_cast<int>(left % p.tiles);
-    const int u = static_cast<int>(left / p.tiles);
-    p.rt = u % p.rts;
-    p.h = u / p.rts;
-    out->p = p;
+    if (end == 0) {
+      out->p = p;
+      out->first_run = first_run;
+    } else {
+      out->eb = p.b;
+      out->eh = p.h;
+      out->ert = p.rt;
+      out->et = p.t;
+    }
   }
   __syncthreads();
 }
@@ -269,52 +289,168 @@ struct Elem<B200_ATTN_DTYPE_FP32> {
   __device__ static T round(float x) { return x; }
 };
 
-// Joins the partial results of cut units: a warp takes one row, its lanes the
-// columns, and adds the runs' sums in order, weighted by 2^(m - top).
+// Joins the partial results of cut units.  The warps of a block share the runs of a
+// unit, so that all of them are read at once, each with its own maximum and sums;
+// then they join in shared memory.  The runs of a warp and the warps are taken in
+// order: the result does not depend on timing.
 constexpr int kJoinWarps = 8;
 
+struct Joint {
+  int2 runs;   // first and last run of the unit
+  int row0;    // first row of the block in the unit
+  int rows;    // rows of the unit
+  int b, h, rt;
+};
+
+template <int RM>
+__device__ __forceinline__ bool joint_of(const Args& a, int row0, Joint* j) {
+  const int unit = blockIdx.x, bh = unit / a.row_tiles;
+  j->rt = unit % a.row_tiles;
+  j->b = bh / a.kv_heads;
+  j->h = bh % a.kv_heads;
+  j->row0 = row0;
+  const int drafts = a.drafts ? a.drafts[j->b] : a.tokens;
+  j->rows = min(RM, drafts * a.group - j->rt * RM);
+  if (row0 >= j->rows || drafts > a.tokens) return false;
+  j->runs = a.desc[unit];
+  return j->runs.x < j->runs.y;
+}
+
+// The partial result of run c: the unit's first run kept it in its second place (the
+// unit began there), the others in their first.
+template <int RM, int DP>
+__device__ __forceinline__ const float* part_of(const Args& a, const Joint& j, int c) {
+  return a.partial + static_cast<int64_t>(2 * c + (c == j.runs.x)) * (RM * (DP + 2));
+}
+
+__device__ __forceinline__ uint8_t* out_row(const Args& a, const Joint& j, int r, int rm) {
+  const int row = j.rt * rm + r, tok = row / a.group;
+  return a.o + j.b * a.o_seq + (j.h * a.group + row - tok * a.group) * a.o_head + tok * a.o_tok;
+}
+
+// Row by row: partial sums [RM][DP], a block takes 4 rows, a lane DP / 32 columns.
 template <int RM, int DP, int DT>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_rows_kernel(const __grid_constant__ Args a) {
   using E = Elem<DT>;
+  constexpr int kCols = DP / 32;
+  __shared__ float sums[kJoinWarps][4][DP];
+  __shared__ float tops[kJoinWarps][4], totals[kJoinWarps][4];
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
-  const int unit = blockIdx.x;
-  const int rt = unit % a.row_tiles, bh = unit / a.row_tiles;
-  const int b = bh / a.kv_heads, h = bh % a.kv_heads;
-  const int drafts = a.drafts ? a.drafts[b] : a.tokens;
-  const int rows = min(RM, drafts * a.group - rt * RM);
-  const int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
-  if (r >= rows || drafts > a.tokens) return;
-  const int2 d = a.desc[unit];
-  if (d.x >= d.y) return;
-  const int lane = threadIdx.x & 31;
-  constexpr int kSlot = RM * (DP + 2);
-  // the first run holds the unit's first tile (second slot of the run), the
-  // others begin inside the unit (first slot)
-  auto slot = [&](int c) { return a.partial + static_cast<int64_t>(2 * c + (c == d.x)) * kSlot; };
-  float top = -INFINITY;
-  for (int c = d.x + lane; c <= d.y; c += 32) top = fmaxf(top, slot(c)[RM * DP + r]);
+  Joint j;
+  if (!joint_of<RM>(a, 4 * blockIdx.y, &j)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float top[4], total[4], acc[4][kCols];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.f : top;
-  constexpr int kCols = DP / 32;
-  float acc[kCols] = {};
-  float total = 0.f;
-#pragma unroll 4
-  for (int c = d.x; c <= d.y; ++c) {
-    const float* p = slot(c);
-    const float w = exp2f(p[RM * DP + r] - base);
-    total += w * p[RM * DP + RM + r];
+  for (int r = 0; r < 4; ++r) {
+    top[r] = -INFINITY;
+    total[r] = 0.f;
 #pragma unroll
-    for (int x = 0; x < kCols; ++x) acc[x] += w * p[r * DP + lane + 32 * x];
+    for (int x = 0; x < kCols; ++x) acc[r][x] = 0.f;
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  const int row = rt * RM + r;
-  typename E::T* dst = reinterpret_cast<typename E::T*>(
-      a.o + b * a.o_seq + (h * a.group + row % a.group) * a.o_head + (row / a.group) * a.o_tok);
+  for (int c = j.runs.x + warp; c <= j.runs.y; c += kJoinWarps) {
+    const float* p = part_of<RM, DP>(a, j, c);
 #pragma unroll
-  for (int x = 0; x < kCols; ++x)
-    if (lane + 32 * x < a.head_dim) dst[lane + 32 * x] = E::round(acc[x] * inv);
+    for (int r = 0; r < 4; ++r) {
+      const int row = min(j.row0 + r, j.rows - 1);
+      float v[kCols];
+#pragma unroll
+      for (int x = 0; x < kCols; ++x) v[x] = p[row * DP + lane + 32 * x];
+      const float m = p[RM * DP + row], l = p[RM * DP + RM + row];
+      const float now = fmaxf(top[r], m), base = now == -INFINITY ? 0.f : now;
+      const float keep = exp2f(top[r] - base), w = exp2f(m - base);
+      top[r] = now;
+      total[r] = total[r] * keep + w * l;
+#pragma unroll
+      for (int x = 0; x < kCols; ++x) acc[r][x] = acc[r][x] * keep + w * v[x];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (lane == 0) {
+      tops[warp][r] = top[r];
+      totals[warp][r] = total[r];
+    }
+#pragma unroll
+    for (int x = 0; x < kCols; ++x) sums[warp][r][lane + 32 * x] = acc[r][x];
+  }
+  __syncthreads();
+  for (int y = threadIdx.x; y < 4 * DP; y += 32 * kJoinWarps) {
+    const int r = y / DP, col = y % DP;
+    if (j.row0 + r >= j.rows || col >= a.head_dim) continue;
+    float best = -INFINITY, sum = 0.f, all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) best = fmaxf(best, tops[w][r]);
+    const float base = best == -INFINITY ? 0.f : best;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float f = exp2f(tops[w][r] - base);
+      sum += f * sums[w][r][col];
+      all += f * totals[w][r];
+    }
+    reinterpret_cast<typename E::T*>(out_row(a, j, j.row0 + r, RM))[col] =
+        E::round(all == 0.f ? 0.f * sum : sum / all);
+  }
+}
+
+// Column by column: partial sums [DP][RM], a block takes 32 rows, a lane one of them,
+// and 32 columns at a time; gridDim.z blocks share the columns.
+template <int RM, int DP, int DT>
+__global__ void __launch_bounds__(32 * kJoinWarps)
+    join_columns_kernel(const __grid_constant__ Args a) {
+  using E = Elem<DT>;
+  __shared__ float sums[kJoinWarps][32][33];
+  __shared__ float tops[kJoinWarps][32], totals[kJoinWarps][32];
+  b200attn::ptx::launch_dependents();
+  b200attn::ptx::grid_dependency_wait();
+  Joint j;
+  if (!joint_of<RM>(a, 32 * blockIdx.y, &j)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = min(j.row0 + lane, j.rows - 1);
+  for (int c0 = 32 * blockIdx.z; c0 < DP; c0 += 32 * gridDim.z) {
+    float top = -INFINITY, total = 0.f, acc[32];
+#pragma unroll
+    for (int x = 0; x < 32; ++x) acc[x] = 0.f;
+    for (int c = j.runs.x + warp; c <= j.runs.y; c += kJoinWarps) {
+      const float* p = part_of<RM, DP>(a, j, c);
+      float v[32];
+#pragma unroll
+      for (int x = 0; x < 32; ++x) v[x] = p[(c0 + x) * RM + row];
+      const float m = p[RM * DP + row], l = p[RM * DP + RM + row];
+      const float now = fmaxf(top, m), base = now == -INFINITY ? 0.f : now;
+      const float keep = exp2f(top - base), w = exp2f(m - base);
+      top = now;
+      total = total * keep + w * l;
+#pragma unroll
+      for (int x = 0; x < 32; ++x) acc[x] = acc[x] * keep + w * v[x];
+    }
+    tops[warp][lane] = top;
+    totals[warp][lane] = total;
+#pragma unroll
+    for (int x = 0; x < 32; ++x) sums[warp][lane][x] = acc[x];
+    __syncthreads();
+    // a thread finishes 4 columns of a row
+    const int r = threadIdx.x >> 3, x0 = 4 * (threadIdx.x & 7);
+    if (j.row0 + r < j.rows && c0 + x0 < a.head_dim) {
+      float best = -INFINITY, all = 0.f, sum[4] = {};
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) best = fmaxf(best, tops[w][r]);
+      const float base = best == -INFINITY ? 0.f : best;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = exp2f(tops[w][r] - base);
+        all += f * totals[w][r];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum[x] += f * sums[w][r][x0 + x];
+      }
+      const float inv = all == 0.f ? 0.f : 1.f / all;
+      typename E::T* dst =
+          reinterpret_cast<typename E::T*>(out_row(a, j, j.row0 + r, RM)) + c0 + x0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) dst[x] = E::round(sum[x] * inv);
+    }
+    __syncthreads();
+  }
 }
 
 // Host side of tree_attn_sm100.cu: the row tiles of 128 or 256, and the largest

@@ -103,6 +103,7 @@ struct RowShape {
   static constexpr int kOffMisc = kOffStat + 4 * 2 * kRowWarps * RM;
   static constexpr int kSmemBytes = kOffMisc + 256;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of a block");
+  using G = Grid<RM, kRowTile, 1>;
 };
 
 template <class S, int DT>
@@ -113,19 +114,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   float* join = reinterpret_cast<float*>(smem + S::kOffJoin);
   float* stat = reinterpret_cast<float*>(smem + S::kOffStat);  // [warp][{max, sum}][RM]
   int64_t* sums = reinterpret_cast<int64_t*>(smem + S::kOffMisc);
-  Start* start = reinterpret_cast<Start*>(smem + S::kOffMisc + 80);
+  Run* found = reinterpret_cast<Run*>(smem + S::kOffMisc + 80);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
-  find_start<RM, kRowTile>(a, blockIdx.x, gridDim.x, sums, start);
-  const Line line(start->total, gridDim.x);
-  if (blockIdx.x >= line.runs) {
-    zero_unused_rows(a, 2, kRowThreads);
-    return;
-  }
-  int64_t at = line.begin(blockIdx.x);
-  const int64_t end = line.begin(blockIdx.x + 1);
-  int left = static_cast<int>(end - at);  // tiles whose loads are still to be issued
+  find_run<typename S::G>(a, blockIdx.x, gridDim.x, sums, found);
+  const Run& run = *found;
 
   const int pieces = a.head_dim / 8;
   const uint32_t ring = sbase + warp * (NS * 2 * S::kBlockBytes);
@@ -134,7 +128,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
 
   // ------------------------------------------------------------- loads
   // The place of the next tile to load; its page numbers are read one tile ahead.
-  Place ld = start->p;
+  Place ld = run.p;
+  bool more = !run.done(ld);  // tiles are still to be loaded
   int page = -1, page_row = 0, ld_keys = 0;
   auto look_up = [&]() {
     const int key = ld.t * kRowTile + warp * kRowKeys + (whole ? 0 : (lane & 15));
@@ -147,11 +142,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       page_row = static_cast<int>(static_cast<uint32_t>(key) - slot * size);
     }
   };
-  look_up();
+  if (more) look_up();
   int stage = 0;  // stage the next loads go to
   auto issue = [&]() {
-    if (left > 0) {
-      --left;
+    if (more) {
       if (page >= a.pages || (page < 0 && (whole ? 0 : (lane & 15)) < ld_keys)) {
         report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
         page = -1;
@@ -176,10 +170,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
         cp_async16(dst + off, ks, ok ? 16u : 0u);
         cp_async16(dst + S::kBlockBytes + off, vs, ok ? 16u : 0u);
       }
-      if (left > 0) {
-        if (++ld.t == ld.tiles) next_unit<RM, kRowTile>(a, ld);
-        look_up();
-      }
+      if (++ld.t == ld.tiles) next_unit<typename S::G>(a, ld);
+      more = !run.done(ld);
+      if (more) look_up();
     }
     cp_async_commit();
     stage = stage + 1 == NS ? 0 : stage + 1;
@@ -217,17 +210,19 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
     }
   };
 
-  Place pl = start->p;
-  fetch_q(pl);
-  store_q();
+  Place pl = run.p;
+  if (!run.done(pl)) {
+    fetch_q(pl);
+    store_q();
+  }
   __syncthreads();
   int use = 0;  // stage of the tile at hand
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // row and column pair of this lane in a product
   const int mat = lane >> 3, mrow = lane & 7;    // matrix and row this lane addresses
 
-  while (at < end) {
+  while (!run.done(pl)) {
     const int t0 = pl.t;
-    const int n = static_cast<int>(min(static_cast<int64_t>(pl.tiles - t0), end - at));
+    const int n = run.tiles(pl);
     const int keys = pl.s.len + pl.s.drafts;
     float o[MT][DP / 8][4];
     float m[MT][2], l[MT][2];
@@ -391,12 +386,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
     // ------------------------------------------- join the warps' results
     const Place done = pl;
     const bool first = t0 == 0, last = t0 + n == pl.tiles;
-    const int64_t unit_begin = at - t0;
-    at += n;
-    if (at < end) {
-      next_unit<RM, kRowTile>(a, pl);
-      fetch_q(pl);  // on its way while the results are joined
-    }
+    pl.t += n;
+    if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
+    const bool again = !run.done(pl);
+    if (again) fetch_q(pl);  // on its way while the results are joined
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -491,9 +484,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       part[RM * DP + RM + r] = total;
     }
     if (tid == 0 && last)
-      a.desc[unit_of(a, done)] = make_int2(
-          first ? static_cast<int>(blockIdx.x) : line.owner(unit_begin), static_cast<int>(blockIdx.x));
-    if (at < end) store_q();  // the queries' fragments are in registers, or read between the barriers
+      a.desc[unit_of(a, done)] =
+          make_int2(first ? static_cast<int>(blockIdx.x) : run.first_run, static_cast<int>(blockIdx.x));
+    if (again) store_q();  // the queries' fragments are in registers, or read between the barriers
     __syncthreads();
   }
 }

@@ -63,8 +63,10 @@ struct TileShape {
   static constexpr int kOffQ = 0;
   static constexpr int kOffRing = kQTiles * kTileBytes;
   static constexpr int kOffSums = kOffRing + kSlots * kTileBytes;
-  static constexpr int kOffStart = kOffSums + 8 * 12;  // one sum a warp
-  static constexpr int kOffBar = kOffStart + 48;
+  static constexpr int kOffRun = kOffSums + 8 * 12;  // one sum a warp
+  static constexpr int kOffBar = kOffRun + 64;
+  static_assert(sizeof(Run) <= 64, "a run's place");
+  using G = Grid<RM, kTile, 2>;
   static constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kSlots,
                        kBarScores = kBarEmpty + kSlots, kBarRead = kBarScores + 2,
                        kBarWeights = kBarRead + 2, kBarSums = kBarWeights + 2,
@@ -159,6 +161,27 @@ __device__ __forceinline__ void settle(uint32_t bar, uint32_t parity) {
   }
 }
 
+// Largest of three; (x, y) = (a, b) * m + c; (x, y) += (a, b): two lanes an instruction.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c) {
+  asm("{\n\t.reg .b64 p, q, r, s;\n\t"
+      "mov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %4};\n\tmov.b64 r, {%5, %5};\n\t"
+      "fma.rn.f32x2 s, p, q, r;\n\tmov.b64 {%0, %1}, s;\n\t}"
+      : "=f"(x), "=f"(y)
+      : "f"(a), "f"(b), "f"(m), "f"(c));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 p, q, s;\n\t"
+      "mov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\t"
+      "add.rn.f32x2 s, p, q;\n\tmov.b64 {%0, %1}, s;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (DT == B200_ATTN_DTYPE_BF16) {
@@ -200,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                              ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = ptx::smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Start* start = reinterpret_cast<Start*>(smem + S::kOffStart);
+  Run* found = reinterpret_cast<Run*>(smem + S::kOffRun);
   // misc[0] tensor memory base, [1] abort flag, [2] last segment with a value that is not finite
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem + S::kOffMisc);
   volatile uint32_t* abort_flag = misc + 1;
@@ -210,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     misc[1] = 0u;
     misc[2] = 0u;
-    ptx::mbar_init(bar(S::kBarQ), 8);
+    ptx::mbar_init(bar(S::kBarQ), kTwo ? 8 : 4);
     for (int s = 0; s < NS; ++s) {
       ptx::mbar_init(bar(S::kBarFull + s), 1);
       ptx::mbar_init(bar(S::kBarEmpty + s), 1);
@@ -228,10 +251,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::tma_prefetch_desc(&tm_v);
   }
   ptx::grid_dependency_wait();
-  find_start<RM, kTile>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem + S::kOffSums),
-                        start);
-  const Line line(start->total, gridDim.x);
-  if (blockIdx.x >= line.runs) {
+  find_run<typename S::G>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem + S::kOffSums),
+                          found);
+  const Run& run = *found;
+  Place pl = run.p;
+  if (run.done(pl)) {
     zero_unused_rows(a, 2, kThreads);
     return;
   }
@@ -243,14 +267,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = misc[0];
-  const int64_t begin = line.begin(blockIdx.x), end = line.begin(blockIdx.x + 1);
-  Place pl = start->p;
-
-  // Tiles of the segment that starts at line position `at`, and of those the
-  // ones of softmax group i.
-  auto seg_tiles = [&](int64_t at) {
-    return static_cast<int>(min(static_cast<int64_t>(pl.tiles - pl.t), end - at));
-  };
   auto unit_rows = [&](const Place& p) { return min(RM, p.s.drafts * a.group - p.rt * RM); };
   // group i takes tile j of a segment
   auto takes = [&](int i, int j, int rows) {
@@ -295,11 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // The page numbers of a tile are read while the loads before it are issued, and
     // serve its keys and, two loads later, its values.
-    const uint32_t tiles = static_cast<uint32_t>(end - begin);
     Box next = look_up(), before[2] = {next, next};  // of tiles t, and t - 2, t - 1
     uint32_t issued = 0;                             // one past the last load issued
     bool ok = true;
-    for (uint32_t t = 0; ok && t < tiles + 2; ++t) {
+    int rest = 2;  // rounds after the last keys, for the last values
+    for (uint32_t t = 0; ok && rest > 0; ++t) {
       const Box now = next;
       if (t >= 2) {
         ok = load(S::load_v(t - 2), &tm_v, before[0]);
@@ -307,13 +323,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       before[0] = before[1];
       before[1] = now;
-      if (!ok || t >= tiles) continue;
-      ok = load(S::load_k(t), &tm_k, now);
-      if (ok) issued = S::load_k(t) + 1;
-      if (ok && t + 1 < tiles) {
-        if (++pl.t == pl.tiles) next_unit<RM, kTile>(a, pl);
-        next = look_up();
+      if (run.done(pl)) {
+        --rest;
+        continue;
       }
+      ok = ok && load(S::load_k(t), &tm_k, now);
+      if (ok) issued = S::load_k(t) + 1;
+      if (++pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
+      if (!run.done(pl)) next = look_up();
     }
     if (!ok) {
       // copies in flight land before the shared memory goes
@@ -328,8 +345,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t tile = 0, seg = 0, made[2] = {0u, 0u};
       int prev = -1;
       bool ok = true;
-      for (int64_t at = begin; ok && at < end; ++seg) {
-        const int n = seg_tiles(at), rows = unit_rows(pl);
+      for (; ok && !run.done(pl); ++seg) {
+        const int n = run.tiles(pl), rows = unit_rows(pl);
         ok = wait_bar(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
         for (int j = 0; ok && j < n; ++j, ++tile) {
           const uint32_t number = S::load_k(tile), s = number % NS;
@@ -358,9 +375,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (ok) ptx::tc_commit(bar(S::kBarEmpty + s));
         }
-        at += n;
         pl.t += n;
-        if (at < end) next_unit<RM, kTile>(a, pl);
+        if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
       }
       ptx::tc_commit(bar(S::kBarDrain));
       settle(bar(S::kBarDrain), 0);
@@ -372,8 +388,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, DP, true);
       uint32_t tile = 0, made[2] = {0u, 0u};
       bool ok = true;
-      for (int64_t at = begin; ok && at < end;) {
-        const int n = seg_tiles(at), rows = unit_rows(pl);
+      while (ok && !run.done(pl)) {
+        const int n = run.tiles(pl), rows = unit_rows(pl);
         bool fresh[2] = {true, true};
         for (int j = 0; ok && j < n; ++j, ++tile) {
           const uint32_t number = S::load_v(tile), s = number % NS;
@@ -398,9 +414,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (ok) ptx::tc_commit(bar(S::kBarEmpty + s));
         }
-        at += n;
         pl.t += n;
-        if (at < end) next_unit<RM, kTile>(a, pl);
+        if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
       }
       ptx::tc_commit(bar(S::kBarDrain));
       settle(bar(S::kBarDrain), 0);
@@ -413,47 +428,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tS = tmem + lanes, tP = tS + S::kColP + 64 * i, tO = tS + S::kColO;
     const int pieces = a.head_dim / 8;
     const uint32_t size = static_cast<uint32_t>(a.page_size);
-    // this thread's part of the queries: its row of its row tile; where both groups
-    // hold the same rows, half of it each
-    constexpr int kMine = kTwo ? S::kPieces : S::kPieces / 2;
-    const int p0 = kTwo ? 0 : i * kMine;
+    // The queries of a unit, 16 bytes a lane and whole rows at a time, straight to shared
+    // memory.  With kTwo a group brings its own rows; else the group of the segment's
+    // last tile brings all of them, since all scores before its own are complete.
+    constexpr int kAt = 32 / S::kPieces;    // rows at a time
     const int row0 = kTwo ? i * kTile : 0;  // first row of this group in the unit
-    auto fetch_q = [&](const Place& p, bool more, uint4 (&qreg)[kMine]) {
-      const bool have = more && row0 + rl < unit_rows(p);
-      const int row = p.rt * RM + row0 + rl, tok = row / a.group;
-      const uint4* src = reinterpret_cast<const uint4*>(
-          a.q + p.b * a.q_seq + (p.h * a.group + row - tok * a.group) * a.q_head + tok * a.q_tok);
-#pragma unroll
-      for (int x = 0; x < kMine; ++x) {
-        qreg[x] = make_uint4(0u, 0u, 0u, 0u);
-        if (have && p0 + x < pieces) qreg[x] = __ldg(src + p0 + x);
-      }
-    };
-    auto store_q = [&](const uint4 (&qreg)[kMine]) {
-      const uint32_t base = sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes + rl * 128;
-#pragma unroll
-      for (int x = 0; x < kMine; ++x) {
-        const int p = p0 + x;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                         base + (p >> 3) * S::kChunkBytes + (((p & 7) ^ (rl & 7)) << 4)),
-                     "r"(qreg[x].x), "r"(qreg[x].y), "r"(qreg[x].z), "r"(qreg[x].w)
+    const int q_piece = lane % S::kPieces;
+    auto bring_q = [&](const Place& p) {
+      const int rows = unit_rows(p);
+#pragma unroll 4
+      for (int x = 0; x < 32 / kAt; ++x) {
+        const int r = quad * 32 + x * kAt + lane / S::kPieces;
+        const int row = p.rt * RM + row0 + r, tok = row / a.group;
+        const bool have = row0 + r < rows && q_piece < pieces;
+        const uint8_t* src = a.q;
+        if (have)
+          src += p.b * a.q_seq + (p.h * a.group + row - tok * a.group) * a.q_head + tok * a.q_tok +
+                 16 * q_piece;
+        const uint32_t dst = sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes +
+                             (q_piece >> 3) * S::kChunkBytes + r * 128 +
+                             (((q_piece & 7) ^ (r & 7)) << 4);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                     "r"(have ? 16u : 0u)
                      : "memory");
       }
+    };
+    auto q_is_there = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
       ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(S::kBarQ));
     };
-    {
-      uint4 qreg[kMine];
-      fetch_q(pl, true, qreg);
-      store_q(qreg);
+    if (kTwo || i == 0) {
+      bring_q(pl);
+      q_is_there();
     }
     zero_unused_rows(a, 2, kSoftmaxThreads);
 
+    constexpr int kStep = kTwo ? 1 : 2;  // from a group's tile to its next
     uint32_t tile = 0, seg = 0, cnt = 0;  // tiles of the run, segments, tiles of this group
     bool ok = true;
-    for (int64_t at = begin; ok && at < end; ++seg) {
-      const int n = seg_tiles(at), rows = unit_rows(pl), t0 = pl.t;
+    for (; ok && !run.done(pl); ++seg) {
+      const int n = run.tiles(pl), rows = unit_rows(pl), t0 = pl.t;
       const int len = pl.s.len, keys = len + pl.s.drafts;
       const int first_row = pl.rt * RM + row0 + quad * 32;  // of this warp
       const bool idle = row0 + quad * 32 >= rows;           // the warp's rows are padding
@@ -499,8 +515,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::fence_proxy_async_smem();
         return true;
       };
+      // drafts of up to 64 tokens: this row's mask, read before it is needed
+      uint64_t seen = 0u;
+      if (a.tokens <= 64 && !idle && (t0 + n) * kTile > len)
+        seen = seen_word(a, pl.b, my_tok, 0, pl.s.drafts) |
+               static_cast<uint64_t>(a.tokens > 32 ? seen_word(a, pl.b, my_tok, 32, pl.s.drafts) : 0u)
+                   << 32;
       float m_run = -INFINITY, l_run = 0.f;
       int done = 0;
+      // The next unit; its queries are on their way while the last tile is worked on,
+      // and its scores while this unit's results are written.
+      Place unit = pl;
+      bool brings = false;
+      auto look_ahead = [&]() {
+        pl.t += n;
+        if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
+        brings = !run.done(pl) && (kTwo || ((n - 1) & 1) == i);
+        if (brings) bring_q(pl);
+      };
       for (int j = 0; j < n; ++j) {
         if (!takes(i, j, rows)) continue;
         if (!warp_wait(bar(S::kBarScores + i), cnt & 1u, abort_flag, a.err)) {
@@ -511,6 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int k0 = (t0 + j) * kTile;
         if (idle) {  // nothing to compute, but the barriers count this warp
           warp_arrive(bar(S::kBarRead + i), lane);
+          if (j + kStep >= n) look_ahead();
           ok = cnt == 0 || warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
           if (ok && k0 + kTile > len) ok = clean(j, k0);
           if (!ok) break;
@@ -524,20 +557,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * c]));
         ptx::tmem_wait_ld();
         warp_arrive(bar(S::kBarRead + i), lane);
+        if (j + kStep >= n) look_ahead();
         // a bit for each key that this row sees
         const bool partly = k0 + kTile > len;  // drafted tokens, or places past the last key
         if (partly) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int d = k0 + 32 * q - len;
-            if (d > -32)
-              hide(*reinterpret_cast<uint32_t(*)[32]>(&sr[32 * q]),
-                   seen_word(a, pl.b, my_tok, d, pl.s.drafts));
+            if (d <= -32) continue;
+            uint32_t word;
+            if (a.tokens <= 64)
+              word = d >= 64 ? 0u
+                             : static_cast<uint32_t>(d < 0 ? seen << -d | ((1u << -d) - 1u) : seen >> d);
+            else
+              word = seen_word(a, unit.b, my_tok, d, unit.s.drafts);
+            hide(*reinterpret_cast<uint32_t(*)[32]>(&sr[32 * q]), word);
           }
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < kTile; ++k) top[k & 3] = fmaxf(top[k & 3], __uint_as_float(sr[k]));
+        for (int k = 0; k < kTile; k += 2)
+          top[(k >> 1) & 3] =
+              max3(top[(k >> 1) & 3], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
         const bool resc = mx > m_run + kRescale || (m_run == -INFINITY && mx > m_run);
         const float m_new = resc ? mx : m_run;
@@ -571,13 +612,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int k = 32 * c + 2 * e;
-            const float x = ptx::ex2_approx(fmaf(__uint_as_float(sr[k]), a.scale_log2, neg));
-            const float y = ptx::ex2_approx(fmaf(__uint_as_float(sr[k + 1]), a.scale_log2, neg));
-            // the sum is taken of the rounded weights, which the product uses
+            float x, y;
+            fma2(x, y, __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]), a.scale_log2, neg);
+            x = ptx::ex2_approx(x);
+            y = ptx::ex2_approx(y);
+            add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], x, y);
             pk[e] = pack2<DT>(x, y);
-            const float2 r = unpack2<DT>(pk[e]);
-            sum[2 * (e & 1)] += r.x;
-            sum[2 * (e & 1) + 1] += r.y;
           }
           st_x16(tP + 16 * c, pk);
         }
@@ -591,6 +631,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++cnt;
         ++done;
       }
+      if (ok && (kTwo ? !takes(i, 0, rows) : i >= n)) {
+        // The group had no tile here.  It must not count twice towards one unit's
+        // queries, so it waits until this unit's are complete.
+        ok = warp_wait(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
+        look_ahead();
+      }
+      if (brings) q_is_there();
       if (ok && cnt > 0) ok = warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
       // ---------------------------------------------------- end of a segment
       if (!kTwo && ok) {
@@ -600,18 +647,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
       }
-      ok = ptx::named_barrier_and(1, kSoftmaxThreads, ok);
+      if constexpr (!kTwo) ok = ptx::named_barrier_and(1, kSoftmaxThreads, ok);
       if (!ok) break;
       ptx::tc_fence_after();
-      const Place unit = pl;
-      const bool first = t0 == 0, last = t0 + n == pl.tiles;
-      const int64_t unit_begin = at - t0;
+      const bool first = t0 == 0, last = t0 + n == unit.tiles;
       const bool any_odd = misc[2] == seg + 1u;
-      at += n;
       tile += n;
-      if (at < end) next_unit<RM, kTile>(a, pl);
-      uint4 qreg[kMine];  // the next queries, on their way while the results are written
-      fetch_q(pl, at < end, qreg);
       // weights of the groups' sums in this thread's row
       float top = m_run, total = l_run, w[2] = {1.f, 1.f};
       if constexpr (!kTwo) {
@@ -629,7 +670,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mine = row0 + rl < rows;
       const bool finish = first && last;
       const float inv = total == 0.f ? 0.f : 1.f / total;
-      const int row = unit.rt * RM + row0 + rl, tok = min(row / a.group, a.tokens - 1);
+      const int tok = my_tok;
+      const int row = unit.rt * RM + row0 + rl;
       uint8_t* out = a.o + unit.b * a.o_seq + (unit.h * a.group + row % a.group) * a.o_head +
                      tok * a.o_tok;
       float* part = a.partial +
@@ -691,11 +733,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                       pack2<DT>(acc[8 * e + 4] * inv, acc[8 * e + 5] * inv),
                       pack2<DT>(acc[8 * e + 6] * inv, acc[8 * e + 7] * inv));
             }
-          } else if (mine) {
-            float* dst = part + (row0 + rl) * DP + col;
+          } else {
+            // a column of rows at a time
 #pragma unroll
-            for (int e = 0; e < 32; e += 2)
-              *reinterpret_cast<float2*>(dst + e) = make_float2(acc[e], acc[e + 1]);
+            for (int e = 0; e < 32; ++e) part[(col + e) * RM + row0 + rl] = acc[e];
           }
         }
       }
@@ -705,12 +746,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (threadIdx.x == 0 && last)
         a.desc[unit_of(a, unit)] =
-            make_int2(first ? static_cast<int>(blockIdx.x) : line.owner(unit_begin),
+            make_int2(first ? static_cast<int>(blockIdx.x) : run.first_run,
                       static_cast<int>(blockIdx.x));
-      // the sums and the queries of this unit have been read
+      // both groups' sums have been read by both
       ptx::tc_fence_before();
-      ptx::named_barrier_sync(1, kSoftmaxThreads);
-      if (at < end) store_q(qreg);
+      if constexpr (!kTwo) ptx::named_barrier_sync(1, kSoftmaxThreads);
     }
   }
 

@@ -204,6 +204,8 @@ def test_large_pool_offsets():
 def test_bad_pages_and_lengths_are_reported_and_skipped(dtype, T):
     args = make([40, 60], T, 2, 2, 64, 16, dtype)
     q, k, v, table, lens = (t.cuda() for t in args)
+    want, size, grow = attention64(*args)
+    bound = attention_bound(dtype, want, size, grow, 64, 60 + T)
     for broken in ("page", "missing", "length", "drafts"):
         t, n = table.clone(), lens.clone()
         drafts = None
@@ -222,5 +224,5 @@ def test_bad_pages_and_lengths_are_reported_and_skipped(dtype, T):
                 b200_tree_attention(q, k, v, table, lens)
         finally:
             clear_device_errors(q.device)
-        whole = b200_tree_attention(q, k, v, table, lens)
-        assert torch.equal(got[1], whole[1]), broken
+        # the other sequence is unharmed (its keys may be cut differently, so not bit for bit)
+        assert ((got[1].cpu().double() - want[1]).abs() <= bound[1]).all(), broken

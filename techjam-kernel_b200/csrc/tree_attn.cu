@@ -211,36 +211,46 @@ using namespace b200paged;
 
 int64_t round16(int64_t n) { return (n + 15) & ~static_cast<int64_t>(15); }
 
-// Row tile, key tile and padded head dim of the kernel a call takes, and the
-// most CTAs it may run.
+// The kernel a call takes, its row tile (`rm` places, `rows` of them used), key tile and
+// padded head dim, and the most CTAs it may run on an SM.
 enum Kernel { kPlain, kFewRows, kManyRows };
 struct Choice {
   Kernel kernel;
-  int rm, tn, dp;
+  int rm, rows, tn, dp;
   int ctas_per_sm;
 };
 
-// The pools can be gathered by tensor maps: boxes of 8 rows or more, and
-// strides that move.
-bool gather_boxes(const b200_cache& c) {
+// Queries and pools can be read through tensor maps: page boxes of 8 rows or more,
+// and strides that move.
+bool by_tensor_maps(const b200_tree_attn_params* p) {
+  const b200_cache& c = p->cache;
   if (box_rows_of(c.page_size) < 8) return false;
   const int64_t extent[4] = {1, c.pages, c.kv_heads, c.page_size};
   for (int d = 1; d < 4; ++d)
     if (extent[d] > 1 && (c.k_stride[d] <= 0 || c.v_stride[d] <= 0)) return false;
+  const int64_t q_extent[3] = {c.batch, p->heads, p->tokens};
+  for (int d = 0; d < 3; ++d)
+    if (q_extent[d] > 1 && p->q_stride[d] <= 0) return false;
   return true;
 }
 
 Choice choose(const b200_tree_attn_params* p) {
   const int dp = p->cache.head_dim <= 64 ? 64 : 128;
-  if (p->cache.dtype == B200_ATTN_DTYPE_FP32) return Choice{kPlain, kRows, kKeys, dp, dp == 64 ? 4 : 2};
+  if (p->cache.dtype == B200_ATTN_DTYPE_FP32) return Choice{kPlain, kRows, kRows, kKeys, dp, dp == 64 ? 4 : 2};
   const int64_t rows = p->tokens * (p->heads / p->cache.kv_heads);
-  if (rows > 32 && gather_boxes(p->cache))
-    return Choice{kManyRows, rows <= 128 ? 128 : 256, 128, dp, 1};
-  return Choice{kFewRows, rows <= 16 ? 16 : 32, kRowTile, dp, 1};
+  const int64_t group = p->heads / p->cache.kv_heads;
+  if (rows > 32 && group <= 128 && by_tensor_maps(p)) {
+    // whole tokens to a tile of 128 places
+    const int tile = static_cast<int>(128 / group * group);
+    if (rows <= tile) return Choice{kManyRows, 128, tile, 128, dp, 1};
+    return Choice{kManyRows, 256, 2 * tile, 128, dp, 1};
+  }
+  const int rm = rows <= 16 ? 16 : 32;
+  return Choice{kFewRows, rm, rm, kRowTile, dp, 1};
 }
 
 int64_t row_tiles(const b200_tree_attn_params* p, const Choice& c) {
-  return (p->tokens * (p->heads / p->cache.kv_heads) + c.rm - 1) / c.rm;
+  return (p->tokens * (p->heads / p->cache.kv_heads) + c.rows - 1) / c.rows;
 }
 
 constexpr int64_t kMaxRuns = 148 * 8;
@@ -302,7 +312,7 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
     using One = RowShape<1, DP>;
     using Two = RowShape<2, DP>;
     if (c.kernel == kManyRows)
-      rc = launch_tiles(c.rm, c.dp, DT, a, runs, device, s);
+      rc = launch_tiles(c.rm, c.dp, DT, a, a.kv_heads * a.group, runs, device, s);
     else if (c.rm == 16)
       rc = run_one<16, DP, DT>(rows_kernel<One, DT>, kRowThreads, One::kSmemBytes, a, runs, device,
                                s);
@@ -410,6 +420,7 @@ extern "C" int32_t b200_tree_attn_fwd(const b200_tree_attn_params* p, void* stre
   a.slots = static_cast<int32_t>(c.slots);
   a.pages = static_cast<int32_t>(c.pages);
   a.page_size = static_cast<int32_t>(c.page_size);
+  a.unit_rows = ch.rows;
   a.row_tiles = static_cast<int32_t>(row_tiles(p, ch));
   a.scale_log2 = p->scale * 1.4426950408889634f;
   a.desc = static_cast<int2*>(p->workspace);

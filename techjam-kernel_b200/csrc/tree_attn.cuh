@@ -3,7 +3,7 @@
 //
 // Work.  The rows of one (sequence, key head) are its drafted tokens times the
 // query heads of the key head, row r = token * group + head in group.  They are
-// cut into row tiles of RM rows; a unit is one row tile of one (sequence, key
+// cut into row tiles of up to RM rows; a unit is one row tile of one (sequence, key
 // head), and reads the sequence's keys in tiles of TN.  All tiles of all units,
 // in the order (sequence, key head, row tile, key tile), form one line that is
 // cut into equal runs, one for each CTA, whatever the lengths of the
@@ -44,6 +44,7 @@ struct Args {
   int64_t m_seq, m_row, m_col;
   int32_t batch, kv_heads, group, tokens, head_dim;
   int32_t slots, pages, page_size;
+  int32_t unit_rows;  // rows of a row tile (whole tokens for the kernel of many rows)
   int32_t row_tiles;  // of a full draft: the stride of unit numbers
   float scale_log2;
   int2* desc;       // [batch * kv_heads * row_tiles] first and last run of a unit
@@ -78,7 +79,7 @@ struct Grid {
     return s.drafts > 0 ? (s.len + s.drafts + TN - 1) / TN : 0;
   }
   __device__ static int row_tiles(const Args& a, const Seq& s) {
-    return (s.drafts * a.group + RM - 1) / RM;
+    return (s.drafts * a.group + a.unit_rows - 1) / a.unit_rows;
   }
   // places of a sequence in the line
   __device__ static int64_t places(const Args& a, const Seq& s) {
@@ -302,7 +303,6 @@ struct Joint {
   int b, h, rt;
 };
 
-template <int RM>
 __device__ __forceinline__ bool joint_of(const Args& a, int row0, Joint* j) {
   const int unit = blockIdx.x, bh = unit / a.row_tiles;
   j->rt = unit % a.row_tiles;
@@ -310,7 +310,7 @@ __device__ __forceinline__ bool joint_of(const Args& a, int row0, Joint* j) {
   j->h = bh % a.kv_heads;
   j->row0 = row0;
   const int drafts = a.drafts ? a.drafts[j->b] : a.tokens;
-  j->rows = min(RM, drafts * a.group - j->rt * RM);
+  j->rows = min(a.unit_rows, drafts * a.group - j->rt * a.unit_rows);
   if (row0 >= j->rows || drafts > a.tokens) return false;
   j->runs = a.desc[unit];
   return j->runs.x < j->runs.y;
@@ -323,8 +323,8 @@ __device__ __forceinline__ const float* part_of(const Args& a, const Joint& j, i
   return a.partial + static_cast<int64_t>(2 * c + (c == j.runs.x)) * (RM * (DP + 2));
 }
 
-__device__ __forceinline__ uint8_t* out_row(const Args& a, const Joint& j, int r, int rm) {
-  const int row = j.rt * rm + r, tok = row / a.group;
+__device__ __forceinline__ uint8_t* out_row(const Args& a, const Joint& j, int r) {
+  const int row = j.rt * a.unit_rows + r, tok = row / a.group;
   return a.o + j.b * a.o_seq + (j.h * a.group + row - tok * a.group) * a.o_head + tok * a.o_tok;
 }
 
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_rows_kernel(const __grid
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
   Joint j;
-  if (!joint_of<RM>(a, 4 * blockIdx.y, &j)) return;
+  if (!joint_of(a, 4 * blockIdx.y, &j)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float top[4], total[4], acc[4][kCols];
 #pragma unroll
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_rows_kernel(const __grid
       sum += f * sums[w][r][col];
       all += f * totals[w][r];
     }
-    reinterpret_cast<typename E::T*>(out_row(a, j, j.row0 + r, RM))[col] =
+    reinterpret_cast<typename E::T*>(out_row(a, j, j.row0 + r))[col] =
         E::round(all == 0.f ? 0.f * sum : sum / all);
   }
 }
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
   Joint j;
-  if (!joint_of<RM>(a, 32 * blockIdx.y, &j)) return;
+  if (!joint_of(a, 32 * blockIdx.y, &j)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = min(j.row0 + lane, j.rows - 1);
   for (int c0 = 32 * blockIdx.z; c0 < DP; c0 += 32 * gridDim.z) {
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
       }
       const float inv = all == 0.f ? 0.f : 1.f / all;
       typename E::T* dst =
-          reinterpret_cast<typename E::T*>(out_row(a, j, j.row0 + r, RM)) + c0 + x0;
+          reinterpret_cast<typename E::T*>(out_row(a, j, j.row0 + r)) + c0 + x0;
 #pragma unroll
       for (int x = 0; x < 4; ++x) dst[x] = E::round(sum[x] * inv);
     }
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 
 // Host side of tree_attn_sm100.cu: the row tiles of 128 or 256, and the largest
 // power of two up to 128 that divides a page (the kernel takes 8 and more).
-int32_t launch_tiles(int rm, int dp, int dtype, const Args& a, int runs, int device,
+int32_t launch_tiles(int rm, int dp, int dtype, const Args& a, int heads, int runs, int device,
                      cudaStream_t s);
 int box_rows_of(int64_t page_size);
 

@@ -2,11 +2,15 @@
 // key head), 16-bit caches, on the fifth-generation tensor cores: wide trees,
 // and pieces of prompts over a cache.
 //
-// A CTA owns one run of the line of key tiles (tree_attn.cuh).  Eleven warps:
+// A CTA owns one run of the line of key tiles (tree_attn.cuh).  Twelve warps:
 //   warps 0-3, 4-7  two softmax groups, one thread per row = one TMEM lane
 //   warp 8          TMA producer: K and V tiles of 128 keys into a ring
 //   warp 9          tcgen05 issuer of the scores, owner of the tensor memory
 //   warp 10         tcgen05 issuer of the weighted values
+//   warp 11         TMA producer of the queries, as soon as the scores of the unit
+//                   before are complete
+// A thread of a softmax group holds a row of 128 scores, which leaves few registers:
+// what is needed of the unit only at its ends lies in shared memory.
 // Tensor memory: S (128 columns, shared) | P0 P1 (64 each) | O0 O1 (DP each).  A
 // group copies its scores to registers at once, so the next scores are formed
 // while it exponentiates; weights that lie over their scores instead, which
@@ -40,9 +44,9 @@ namespace {
 
 namespace ptx = b200attn::ptx;
 
-constexpr int kThreads = 352;
+constexpr int kThreads = 384;
 constexpr int kSoftmaxThreads = 256;
-constexpr int kLoadWarp = 8, kQkWarp = 9, kPvWarp = 10;
+constexpr int kLoadWarp = 8, kQkWarp = 9, kPvWarp = 10, kQWarp = 11;
 constexpr int kTile = 128;  // keys of a tile, rows of a row tile
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitNs = 1000000000ull;
@@ -64,10 +68,12 @@ struct TileShape {
   static constexpr int kOffRing = kQTiles * kTileBytes;
   static constexpr int kOffSums = kOffRing + kSlots * kTileBytes;
   static constexpr int kOffRun = kOffSums + 8 * 12;  // one sum a warp
-  static constexpr int kOffBar = kOffRun + 64;
+  static constexpr int kOffPlace = kOffRun + 64;  // one a softmax warp
+  static constexpr int kOffBar = kOffPlace + 8 * 32;
+  static_assert(sizeof(Place) == 32, "eight numbers");
   static_assert(sizeof(Run) <= 64, "a run's place");
   using G = Grid<RM, kTile, 2>;
-  static constexpr int kBarQ = 0, kBarFull = 1, kBarEmpty = kBarFull + kSlots,
+  static constexpr int kBarQ = 0, kBarQRead = 1, kBarFull = 2, kBarEmpty = kBarFull + kSlots,
                        kBarScores = kBarEmpty + kSlots, kBarRead = kBarScores + 2,
                        kBarWeights = kBarRead + 2, kBarSums = kBarWeights + 2,
                        kBarDrain = kBarSums + 2, kBars = kBarDrain + 1;
@@ -214,7 +220,8 @@ __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t word) {
 
 template <class S, int DT>
 __global__ void __launch_bounds__(kThreads, 1)
-    tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+    tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ CUtensorMap tm_v,
                  const __grid_constant__ Args a, const int32_t box_rows) {
   constexpr int DP = S::DP, NS = S::kSlots, RM = S::RM;
   constexpr bool kTwo = S::kTwo, kBF16 = DT == B200_ATTN_DTYPE_BF16;
@@ -233,7 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     misc[1] = 0u;
     misc[2] = 0u;
-    ptx::mbar_init(bar(S::kBarQ), kTwo ? 8 : 4);
+    ptx::mbar_init(bar(S::kBarQ), 1);
+    ptx::mbar_init(bar(S::kBarQRead), 1);
     for (int s = 0; s < NS; ++s) {
       ptx::mbar_init(bar(S::kBarFull + s), 1);
       ptx::mbar_init(bar(S::kBarEmpty + s), 1);
@@ -247,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::mbar_init(bar(S::kBarDrain), 2);
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_smem();
+    ptx::tma_prefetch_desc(&tm_q);
     ptx::tma_prefetch_desc(&tm_k);
     ptx::tma_prefetch_desc(&tm_v);
   }
@@ -267,10 +276,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = misc[0];
-  auto unit_rows = [&](const Place& p) { return min(RM, p.s.drafts * a.group - p.rt * RM); };
+  // rows of a unit, and of those one group's share
+  auto unit_rows = [&](const Place& p) {
+    return min(a.unit_rows, p.s.drafts * a.group - p.rt * a.unit_rows);
+  };
+  const int share = kTwo ? a.unit_rows >> 1 : a.unit_rows;
   // group i takes tile j of a segment
   auto takes = [&](int i, int j, int rows) {
-    return kTwo ? (i == 0 || rows > kTile) : (j & 1) == i;
+    return kTwo ? (i == 0 || rows > share) : (j & 1) == i;
+  };
+
+  auto next_segment = [&](Place& p) {
+    p.t += run.tiles(p);
+    if (p.t == p.tiles) next_unit<typename S::G>(a, p);
   };
 
   if (warp == kLoadWarp) {
@@ -375,11 +393,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (ok) ptx::tc_commit(bar(S::kBarEmpty + s));
         }
+        ptx::tc_commit(bar(S::kBarQRead));
         pl.t += n;
         if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
       }
       ptx::tc_commit(bar(S::kBarDrain));
       settle(bar(S::kBarDrain), 0);
+    }
+    __syncwarp();
+  } else if (warp == kQWarp) {
+    // ------------------------------------------------------------- queries
+    // Row r of a row tile is head r % group of token r / group: a box of whole tokens.
+    if (lane == 0) {
+      const int tokens = share / a.group;
+      const uint32_t bytes = static_cast<uint32_t>(share) * 128u * S::kChunks;
+      uint32_t seg = 0;
+      bool ok = true;
+      for (; ok && !run.done(pl); ++seg) {
+        ok = seg == 0 || wait_bar(bar(S::kBarQRead), (seg - 1u) & 1u, abort_flag, a.err);
+        if (!ok) break;
+        const int tiles = kTwo && unit_rows(pl) > share ? 2 : 1;
+        ptx::mbar_arrive_expect_tx(bar(S::kBarQ), tiles * bytes);
+        for (int i = 0; i < tiles; ++i)
+#pragma unroll
+          for (int c = 0; c < S::kChunks; ++c)
+            ptx::tma_load_4d(sbase + S::kOffQ + i * S::kTileBytes + c * S::kChunkBytes, &tm_q,
+                             bar(S::kBarQ), 64 * c, pl.h * a.group,
+                             pl.rt * (a.unit_rows / a.group) + i * tokens, pl.b);
+        next_segment(pl);
+      }
+      if (!ok && seg > 0) settle(bar(S::kBarQ), (seg - 1u) & 1u);
     }
     __syncwarp();
   } else if (warp == kPvWarp) {
@@ -426,68 +469,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int i = warp >> 2, quad = warp & 3, rl = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t tS = tmem + lanes, tP = tS + S::kColP + 64 * i, tO = tS + S::kColO;
-    const int pieces = a.head_dim / 8;
-    const uint32_t size = static_cast<uint32_t>(a.page_size);
-    // The queries of a unit, 16 bytes a lane and whole rows at a time, straight to shared
-    // memory.  With kTwo a group brings its own rows; else the group of the segment's
-    // last tile brings all of them, since all scores before its own are complete.
-    constexpr int kAt = 32 / S::kPieces;    // rows at a time
-    const int row0 = kTwo ? i * kTile : 0;  // first row of this group in the unit
-    const int q_piece = lane % S::kPieces;
-    auto bring_q = [&](const Place& p) {
-      const int rows = unit_rows(p);
-#pragma unroll 4
-      for (int x = 0; x < 32 / kAt; ++x) {
-        const int r = quad * 32 + x * kAt + lane / S::kPieces;
-        const int row = p.rt * RM + row0 + r, tok = row / a.group;
-        const bool have = row0 + r < rows && q_piece < pieces;
-        const uint8_t* src = a.q;
-        if (have)
-          src += p.b * a.q_seq + (p.h * a.group + row - tok * a.group) * a.q_head + tok * a.q_tok +
-                 16 * q_piece;
-        const uint32_t dst = sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes +
-                             (q_piece >> 3) * S::kChunkBytes + r * 128 +
-                             (((q_piece & 7) ^ (r & 7)) << 4);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                     "r"(have ? 16u : 0u)
-                     : "memory");
-      }
-    };
-    auto q_is_there = [&]() {
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(S::kBarQ));
-    };
-    if (kTwo || i == 0) {
-      bring_q(pl);
-      q_is_there();
-    }
+    const int row0 = i * (kTwo ? share : 0);  // first row of this group in the unit
+    Place* where = reinterpret_cast<Place*>(smem + S::kOffPlace) + warp;
+    if (lane == 0) *where = pl;
+    __syncwarp();
     zero_unused_rows(a, 2, kSoftmaxThreads);
 
-    constexpr int kStep = kTwo ? 1 : 2;  // from a group's tile to its next
     uint32_t tile = 0, seg = 0, cnt = 0;  // tiles of the run, segments, tiles of this group
     bool ok = true;
-    for (; ok && !run.done(pl); ++seg) {
-      const int n = run.tiles(pl), rows = unit_rows(pl), t0 = pl.t;
-      const int len = pl.s.len, keys = len + pl.s.drafts;
-      const int first_row = pl.rt * RM + row0 + quad * 32;  // of this warp
-      const bool idle = row0 + quad * 32 >= rows;           // the warp's rows are padding
-      const int my_tok = min((first_row + lane) / a.group, a.tokens - 1);
+    for (; ok && !run.done(*where); ++seg) {
+      const int n = run.tiles(*where), rows = unit_rows(*where), t0 = where->t, len = where->s.len;
+      const bool idle = row0 + quad * 32 >= rows || quad * 32 >= share;  // padding rows only
+      // Values past the last key become 0 (their rows may hold anything, and 0 x
+      // infinity would reach the sums), and so do elements of drafted values that
+      // are not finite: those are added below to the rows that see them.  In kTwo
+      // the second group's product of a tile is issued after the first's, which
+      // waits for this.
       auto clean = [&](int j, int k0) {
         if (kTwo && i != 0) return true;
-        // Values past the last key become 0 (their rows may hold anything, and
-        // 0 x infinity would reach the sums), and so do elements of drafted
-        // values that are not finite: those are added below to the rows that
-        // see them.  In kTwo the second group's product of this tile is
-        // issued after this group's, which waits for this.
+        const int keys = len + where->s.drafts;
         const uint32_t load = S::load_v(tile + j), s = load % NS;
-        if (!warp_wait(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err)) {
-          return false;
-        }
+        if (!warp_wait(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err)) return false;
         const int r0 = max(0, len - k0);
         bool odd = false;
-        for (int x = quad * 32 + lane; x < (kTile - r0) * S::kPieces; x += kTile) {
+        for (int x = rl; x < (kTile - r0) * S::kPieces; x += kTile) {
           const int r = r0 + x / S::kPieces, pc = x % S::kPieces;
           const uint32_t ad = sbase + S::kOffRing + s * S::kTileBytes + (pc >> 3) * S::kChunkBytes +
                               r * 128 + ((pc & 7) << 4);
@@ -515,24 +520,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::fence_proxy_async_smem();
         return true;
       };
-      // drafts of up to 64 tokens: this row's mask, read before it is needed
-      uint64_t seen = 0u;
-      if (a.tokens <= 64 && !idle && (t0 + n) * kTile > len)
-        seen = seen_word(a, pl.b, my_tok, 0, pl.s.drafts) |
-               static_cast<uint64_t>(a.tokens > 32 ? seen_word(a, pl.b, my_tok, 32, pl.s.drafts) : 0u)
-                   << 32;
       float m_run = -INFINITY, l_run = 0.f;
       int done = 0;
-      // The next unit; its queries are on their way while the last tile is worked on,
-      // and its scores while this unit's results are written.
-      Place unit = pl;
-      bool brings = false;
-      auto look_ahead = [&]() {
-        pl.t += n;
-        if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
-        brings = !run.done(pl) && (kTwo || ((n - 1) & 1) == i);
-        if (brings) bring_q(pl);
-      };
       for (int j = 0; j < n; ++j) {
         if (!takes(i, j, rows)) continue;
         if (!warp_wait(bar(S::kBarScores + i), cnt & 1u, abort_flag, a.err)) {
@@ -541,15 +530,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ptx::tc_fence_after();
         const int k0 = (t0 + j) * kTile;
+        const bool partly = k0 + kTile > len;  // drafted tokens, or places past the last key
         if (idle) {  // nothing to compute, but the barriers count this warp
           warp_arrive(bar(S::kBarRead + i), lane);
-          if (j + kStep >= n) look_ahead();
           ok = cnt == 0 || warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
-          if (ok && k0 + kTile > len) ok = clean(j, k0);
+          if (ok && partly) ok = clean(j, k0);
           if (!ok) break;
           warp_arrive(bar(S::kBarWeights + i), lane);
           ++cnt;
           continue;
+        }
+        // a bit for each key that this row sees
+        uint32_t words[4] = {~0u, ~0u, ~0u, ~0u};
+        if (partly) {
+          const int tok = min((where->rt * a.unit_rows + row0 + rl) / a.group, a.tokens - 1);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int d = k0 + 32 * q - len;
+            if (d > -32) words[q] = seen_word(a, where->b, tok, d, where->s.drafts);
+          }
         }
         uint32_t sr[kTile];
 #pragma unroll
@@ -557,22 +556,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * c]));
         ptx::tmem_wait_ld();
         warp_arrive(bar(S::kBarRead + i), lane);
-        if (j + kStep >= n) look_ahead();
-        // a bit for each key that this row sees
-        const bool partly = k0 + kTile > len;  // drafted tokens, or places past the last key
         if (partly) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int d = k0 + 32 * q - len;
-            if (d <= -32) continue;
-            uint32_t word;
-            if (a.tokens <= 64)
-              word = d >= 64 ? 0u
-                             : static_cast<uint32_t>(d < 0 ? seen << -d | ((1u << -d) - 1u) : seen >> d);
-            else
-              word = seen_word(a, unit.b, my_tok, d, unit.s.drafts);
-            hide(*reinterpret_cast<uint32_t(*)[32]>(&sr[32 * q]), word);
-          }
+          for (int q = 0; q < 4; ++q)
+            hide(*reinterpret_cast<uint32_t(*)[32]>(&sr[32 * q]), words[q]);
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -631,14 +618,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++cnt;
         ++done;
       }
-      if (ok && (kTwo ? !takes(i, 0, rows) : i >= n)) {
-        // The group had no tile here.  It must not count twice towards one unit's
-        // queries, so it waits until this unit's are complete.
-        ok = warp_wait(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
-        look_ahead();
+      const Place unit = *where;
+      __syncwarp();
+      if (lane == 0) {
+        Place next = unit;
+        next_segment(next);
+        *where = next;
       }
-      if (brings) q_is_there();
       if (ok && cnt > 0) ok = warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
+      __syncwarp();
       // ---------------------------------------------------- end of a segment
       if (!kTwo && ok) {
         // the other group reads this row's maximum and sum where P_i was
@@ -667,11 +655,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         w[0] = i == 0 ? mine_w : other_w;
         w[1] = i == 0 ? other_w : mine_w;
       }
-      const bool mine = row0 + rl < rows;
+      const bool mine = rl < share && row0 + rl < rows;
+      const int row = unit.rt * a.unit_rows + row0 + rl, tok = min(row / a.group, a.tokens - 1);
+      const uint32_t size = static_cast<uint32_t>(a.page_size);
       const bool finish = first && last;
       const float inv = total == 0.f ? 0.f : 1.f / total;
-      const int tok = my_tok;
-      const int row = unit.rt * RM + row0 + rl;
       uint8_t* out = a.o + unit.b * a.o_seq + (unit.h * a.group + row % a.group) * a.o_head +
                      tok * a.o_tok;
       float* part = a.partial +
@@ -809,9 +797,40 @@ int32_t encode_pool(CUtensorMap* map, const uint8_t* base, int64_t row, int64_t 
   return B200_ATTN_OK;
 }
 
+// Map {head_dim, heads, tokens, batch} of the queries, boxes of {64, group, tokens, 1}.
+int32_t encode_q(CUtensorMap* map, const Args& a, int heads, int tokens, int dtype) {
+  auto fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled entry point unavailable");
+    return B200_ATTN_ERR_LAUNCH;
+  }
+  const int64_t any = a.head_dim * 16;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(a.tokens), static_cast<cuuint64_t>(a.batch)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(heads > 1 ? a.q_head : any),
+                           static_cast<cuuint64_t>(a.tokens > 1 ? a.q_tok : any),
+                           static_cast<cuuint64_t>(a.batch > 1 ? a.q_seq : any)};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(tokens), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(map, dtype == B200_ATTN_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+         4, const_cast<uint8_t*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed");
+    return B200_ATTN_ERR_LAUNCH;
+  }
+  return B200_ATTN_OK;
+}
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
 template <class S, int DT>
-int32_t launch_shape(const CUtensorMap& k, const CUtensorMap& v, const Args& a, int box_rows,
-                     int runs, int device, cudaStream_t s) {
+int32_t launch_shape(const Maps& m, const Args& a, int box_rows, int runs, int device, cudaStream_t s) {
   static std::once_flag once[kMaxDevices];
   static cudaError_t err[kMaxDevices];
   auto kernel = tiles_kernel<S, DT>;
@@ -823,14 +842,14 @@ int32_t launch_shape(const CUtensorMap& k, const CUtensorMap& v, const Args& a, 
     set_error(cudaGetErrorString(err[device]));
     return B200_ATTN_ERR_LAUNCH;
   }
-  return launch(kernel, dim3(runs), dim3(kThreads), S::kSmemBytes, s, k, v, a, box_rows);
+  return launch(kernel, dim3(runs), dim3(kThreads), S::kSmemBytes, s, m.q, m.k, m.v, a, box_rows);
 }
 
 template <int DP, int DT>
-int32_t launch_rows(bool two, const CUtensorMap& k, const CUtensorMap& v, const Args& a,
-                    int box_rows, int runs, int device, cudaStream_t s) {
-  return two ? launch_shape<TileShape<DP, true>, DT>(k, v, a, box_rows, runs, device, s)
-             : launch_shape<TileShape<DP, false>, DT>(k, v, a, box_rows, runs, device, s);
+int32_t launch_rows(bool two, const Maps& m, const Args& a, int box_rows, int runs, int device,
+                    cudaStream_t s) {
+  return two ? launch_shape<TileShape<DP, true>, DT>(m, a, box_rows, runs, device, s)
+             : launch_shape<TileShape<DP, false>, DT>(m, a, box_rows, runs, device, s);
 }
 
 }  // namespace
@@ -841,19 +860,22 @@ int box_rows_of(int64_t page_size) {
   return g;
 }
 
-int32_t launch_tiles(int rm, int dp, int dtype, const Args& a, int runs, int device,
+int32_t launch_tiles(int rm, int dp, int dtype, const Args& a, int heads, int runs, int device,
                      cudaStream_t s) {
   const int g = box_rows_of(a.page_size);
-  CUtensorMap k, v;
-  int32_t rc = encode_pool(&k, a.k, a.k_row, a.k_head, a.k_page, a, dtype, g);
-  if (rc == B200_ATTN_OK) rc = encode_pool(&v, a.v, a.v_row, a.v_head, a.v_page, a, dtype, g);
-  if (rc != B200_ATTN_OK) return rc;
   const bool two = rm == 256;
+  Maps m;
+  int32_t rc = encode_q(&m.q, a, heads, a.unit_rows / a.group / (two ? 2 : 1), dtype);
+  if (rc == B200_ATTN_OK)
+    rc = encode_pool(&m.k, a.k, a.k_row, a.k_head, a.k_page, a, dtype, g);
+  if (rc == B200_ATTN_OK)
+    rc = encode_pool(&m.v, a.v, a.v_row, a.v_head, a.v_page, a, dtype, g);
+  if (rc != B200_ATTN_OK) return rc;
   if (dtype == B200_ATTN_DTYPE_BF16)
-    return dp == 64 ? launch_rows<64, B200_ATTN_DTYPE_BF16>(two, k, v, a, g, runs, device, s)
-                    : launch_rows<128, B200_ATTN_DTYPE_BF16>(two, k, v, a, g, runs, device, s);
-  return dp == 64 ? launch_rows<64, B200_ATTN_DTYPE_FP16>(two, k, v, a, g, runs, device, s)
-                  : launch_rows<128, B200_ATTN_DTYPE_FP16>(two, k, v, a, g, runs, device, s);
+    return dp == 64 ? launch_rows<64, B200_ATTN_DTYPE_BF16>(two, m, a, g, runs, device, s)
+                    : launch_rows<128, B200_ATTN_DTYPE_BF16>(two, m, a, g, runs, device, s);
+  return dp == 64 ? launch_rows<64, B200_ATTN_DTYPE_FP16>(two, m, a, g, runs, device, s)
+                  : launch_rows<128, B200_ATTN_DTYPE_FP16>(two, m, a, g, runs, device, s);
 }
 
 }  // namespace b200tree

@@ -6,9 +6,10 @@
 //   warps 0-3, 4-7  two softmax groups, one thread per row = one TMEM lane
 //   warp 8          TMA producer: K and V tiles of 128 keys into a ring
 //   warp 9          tcgen05 issuer of the scores, owner of the tensor memory
-//   warp 10         tcgen05 issuer of the weighted values
+//   warp 10         tcgen05 issuer of the weighted values; it also makes the values of
+//                   a unit's last tile fit for the product
 //   warp 11         TMA producer of the queries, as soon as the scores of the unit
-//                   before are complete
+//                   before are complete, and packer of the tree masks
 // A thread of a softmax group holds a row of 128 scores, which leaves few registers:
 // what is needed of the unit only at its ends lies in shared memory.
 // Tensor memory: S (128 columns, shared) | P0 P1 (64 each) | O0 O1 (DP each).  A
@@ -51,6 +52,7 @@ constexpr int kTile = 128;  // keys of a tile, rows of a row tile
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr float kRescale = 8.0f;  // output sums are rescaled when the maximum grew by 2^8
+constexpr int kSeen = 64;  // tokens of a draft whose masks fit a word of 64 bits each
 constexpr int kIssuerSpin = 4096;  // polls of an issuer before its suspending wait
 
 template <int DP_, bool kTwo_>
@@ -69,7 +71,8 @@ struct TileShape {
   static constexpr int kOffSums = kOffRing + kSlots * kTileBytes;
   static constexpr int kOffRun = kOffSums + 8 * 12;  // one sum a warp
   static constexpr int kOffPlace = kOffRun + 64;  // one a softmax warp
-  static constexpr int kOffBar = kOffPlace + 8 * 32;
+  static constexpr int kOffSeen = kOffPlace + 8 * 32;  // [2][kSeen] masks of a unit's tokens
+  static constexpr int kOffBar = kOffSeen + 2 * 8 * kSeen;
   static_assert(sizeof(Place) == 32, "eight numbers");
   static_assert(sizeof(Run) <= 64, "a run's place");
   using G = Grid<RM, kTile, 2>;
@@ -232,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Run* found = reinterpret_cast<Run*>(smem + S::kOffRun);
   // misc[0] tensor memory base, [1] abort flag, [2] last segment with a value that is not finite
+  uint64_t* seen = reinterpret_cast<uint64_t*>(smem + S::kOffSeen);
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem + S::kOffMisc);
   volatile uint32_t* abort_flag = misc + 1;
   auto bar = [&](int i) { return sbase + S::kOffBar + 8u * static_cast<uint32_t>(i); };
@@ -240,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     misc[1] = 0u;
     misc[2] = 0u;
-    ptx::mbar_init(bar(S::kBarQ), 1);
+    ptx::mbar_init(bar(S::kBarQ), 2);
     ptx::mbar_init(bar(S::kBarQRead), 1);
     for (int s = 0; s < NS; ++s) {
       ptx::mbar_init(bar(S::kBarFull + s), 1);
@@ -404,62 +408,103 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kQWarp) {
     // ------------------------------------------------------------- queries
     // Row r of a row tile is head r % group of token r / group: a box of whole tokens.
-    if (lane == 0) {
-      const int tokens = share / a.group;
-      const uint32_t bytes = static_cast<uint32_t>(share) * 128u * S::kChunks;
-      uint32_t seg = 0;
-      bool ok = true;
-      for (; ok && !run.done(pl); ++seg) {
-        ok = seg == 0 || wait_bar(bar(S::kBarQRead), (seg - 1u) & 1u, abort_flag, a.err);
-        if (!ok) break;
+    const int tokens = share / a.group;
+    const uint32_t bytes = static_cast<uint32_t>(share) * 128u * S::kChunks;
+    uint32_t seg = 0;
+    bool ok = true;
+    for (; ok && !run.done(pl); ++seg) {
+      ok = seg == 0 || warp_wait(bar(S::kBarQRead), (seg - 1u) & 1u, abort_flag, a.err);
+      if (!ok) break;
+      const int first = pl.rt * (a.unit_rows / a.group);  // token
+      if (lane == 0) {
         const int tiles = kTwo && unit_rows(pl) > share ? 2 : 1;
         ptx::mbar_arrive_expect_tx(bar(S::kBarQ), tiles * bytes);
         for (int i = 0; i < tiles; ++i)
 #pragma unroll
           for (int c = 0; c < S::kChunks; ++c)
             ptx::tma_load_4d(sbase + S::kOffQ + i * S::kTileBytes + c * S::kChunkBytes, &tm_q,
-                             bar(S::kBarQ), 64 * c, pl.h * a.group,
-                             pl.rt * (a.unit_rows / a.group) + i * tokens, pl.b);
-        next_segment(pl);
+                             bar(S::kBarQ), 64 * c, pl.h * a.group, first + i * tokens, pl.b);
       }
-      if (!ok && seg > 0) settle(bar(S::kBarQ), (seg - 1u) & 1u);
+      if (a.tokens <= kSeen) {
+        // one row tile holds all tokens; a bit for each drafted token that a token sees
+        for (int tok = lane; tok < a.tokens; tok += 32) {
+          const uint32_t lo = seen_word(a, pl.b, tok, 0, pl.s.drafts);
+          const uint32_t hi = a.tokens > 32 ? seen_word(a, pl.b, tok, 32, pl.s.drafts) : 0u;
+          seen[(seg & 1u) * kSeen + tok] = static_cast<uint64_t>(hi) << 32 | lo;
+        }
+        __syncwarp();
+      }
+      if (lane == 0) ptx::mbar_arrive(bar(S::kBarQ));
+      next_segment(pl);
     }
+    if (!ok && seg > 0) settle(bar(S::kBarQ), (seg - 1u) & 1u);
     __syncwarp();
   } else if (warp == kPvWarp) {
     // ------------------------------------------------------- O_i += P_i V
-    if (lane == 0) {
-      constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, DP, true);
-      uint32_t tile = 0, made[2] = {0u, 0u};
-      bool ok = true;
-      while (ok && !run.done(pl)) {
-        const int n = run.tiles(pl), rows = unit_rows(pl);
-        bool fresh[2] = {true, true};
-        for (int j = 0; ok && j < n; ++j, ++tile) {
-          const uint32_t number = S::load_v(tile), s = number % NS;
-          ok = issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
-          const uint32_t va = sbase + S::kOffRing + s * S::kTileBytes;
+    constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, DP, true);
+    uint32_t tile = 0, seg = 0, made[2] = {0u, 0u};
+    bool ok = true;
+    for (; ok && !run.done(pl); ++seg) {
+      const int n = run.tiles(pl), rows = unit_rows(pl), len = pl.s.len;
+      bool fresh[2] = {true, true};
+      for (int j = 0; ok && j < n; ++j, ++tile) {
+        const uint32_t number = S::load_v(tile), s = number % NS;
+        ok = warp_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
+        const uint32_t va = sbase + S::kOffRing + s * S::kTileBytes;
+        const int k0 = (pl.t + j) * kTile;
+        if (ok && k0 + kTile > len) {
+          // Values past the last key become 0 (their rows may hold anything, and 0 x
+          // infinity would reach the sums), and so do elements of drafted values that
+          // are not finite: the softmax groups add those to the rows that see them.
+          const int r0 = max(0, len - k0), r1 = len + pl.s.drafts - k0;
+          bool odd = false;
+#pragma unroll 4
+          for (int x = lane; x < (kTile - r0) * S::kPieces; x += 32) {
+            const int r = r0 + x / S::kPieces, pc = x % S::kPieces;
+            const uint32_t ad = va + (pc >> 3) * S::kChunkBytes + r * 128 + ((pc & 7) << 4);
+            uint32_t w[4], any = 0u;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(ad));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (!ok || !takes(i, j, rows)) continue;
-            if (!issuer_wait(bar(S::kBarWeights + i), made[i] & 1u, abort_flag, a.err)) {
-              ok = false;
-              continue;
+            for (int y = 0; y < 4; ++y) {
+              const uint32_t f = r < r1 ? not_finite<DT>(w[y]) : ~0u;
+              any |= f;
+              w[y] &= ~f;
             }
-            ptx::tc_fence_after();
+            odd |= any != 0u && r < r1;
+            if (any)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ad), "r"(w[0]),
+                           "r"(w[1]), "r"(w[2]), "r"(w[3])
+                           : "memory");
+          }
+          if (odd) misc[2] = seg + 1u;
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!ok || !takes(i, j, rows)) continue;
+          ok = __all_sync(0xffffffffu, issuer_wait(bar(S::kBarWeights + i), made[i] & 1u, abort_flag,
+                                                   a.err));
+          if (!ok) continue;
+          ptx::tc_fence_after();
+          if (lane == 0) {
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; ++kk)
               ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + S::kColP + 64 * i + kk * 8,
                              ptx::smem_desc_sw128(va + kk * 2048, S::kChunkBytes, 1024), id,
                              (!fresh[i] || kk > 0) ? 1u : 0u);
             ptx::tc_commit(bar(S::kBarSums + i));
-            fresh[i] = false;
-            ++made[i];
           }
-          if (ok) ptx::tc_commit(bar(S::kBarEmpty + s));
+          fresh[i] = false;
+          ++made[i];
         }
-        pl.t += n;
-        if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
+        if (ok && lane == 0) ptx::tc_commit(bar(S::kBarEmpty + s));
       }
+      next_segment(pl);
+    }
+    if (lane == 0) {
       ptx::tc_commit(bar(S::kBarDrain));
       settle(bar(S::kBarDrain), 0);
     }
@@ -475,51 +520,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     zero_unused_rows(a, 2, kSoftmaxThreads);
 
-    uint32_t tile = 0, seg = 0, cnt = 0;  // tiles of the run, segments, tiles of this group
+    uint32_t seg = 0, cnt = 0;  // segments of the run, tiles of this group
     bool ok = true;
     for (; ok && !run.done(*where); ++seg) {
       const int n = run.tiles(*where), rows = unit_rows(*where), t0 = where->t, len = where->s.len;
       const bool idle = row0 + quad * 32 >= rows || quad * 32 >= share;  // padding rows only
-      // Values past the last key become 0 (their rows may hold anything, and 0 x
-      // infinity would reach the sums), and so do elements of drafted values that
-      // are not finite: those are added below to the rows that see them.  In kTwo
-      // the second group's product of a tile is issued after the first's, which
-      // waits for this.
-      auto clean = [&](int j, int k0) {
-        if (kTwo && i != 0) return true;
-        const int keys = len + where->s.drafts;
-        const uint32_t load = S::load_v(tile + j), s = load % NS;
-        if (!warp_wait(bar(S::kBarFull + s), (load / NS) & 1u, abort_flag, a.err)) return false;
-        const int r0 = max(0, len - k0);
-        bool odd = false;
-        for (int x = rl; x < (kTile - r0) * S::kPieces; x += kTile) {
-          const int r = r0 + x / S::kPieces, pc = x % S::kPieces;
-          const uint32_t ad = sbase + S::kOffRing + s * S::kTileBytes + (pc >> 3) * S::kChunkBytes +
-                              r * 128 + ((pc & 7) << 4);
-          uint32_t w[4] = {0u, 0u, 0u, 0u};
-          bool put = k0 + r >= keys;
-          if (!put) {
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                         : "r"(ad)
-                         : "memory");
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint32_t f = not_finite<DT>(w[y]);
-              put |= f != 0u;
-              w[y] &= ~f;
-            }
-            odd |= put;
-          }
-          if (put)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ad), "r"(w[0]),
-                         "r"(w[1]), "r"(w[2]), "r"(w[3])
-                         : "memory");
-        }
-        if (odd) misc[2] = seg + 1u;
-        ptx::fence_proxy_async_smem();
-        return true;
-      };
       float m_run = -INFINITY, l_run = 0.f;
       int done = 0;
       for (int j = 0; j < n; ++j) {
@@ -534,7 +539,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (idle) {  // nothing to compute, but the barriers count this warp
           warp_arrive(bar(S::kBarRead + i), lane);
           ok = cnt == 0 || warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
-          if (ok && partly) ok = clean(j, k0);
           if (!ok) break;
           warp_arrive(bar(S::kBarWeights + i), lane);
           ++cnt;
@@ -544,10 +548,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t words[4] = {~0u, ~0u, ~0u, ~0u};
         if (partly) {
           const int tok = min((where->rt * a.unit_rows + row0 + rl) / a.group, a.tokens - 1);
+          const uint64_t bits = a.tokens <= kSeen ? seen[(seg & 1u) * kSeen + tok] : 0u;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int d = k0 + 32 * q - len;
-            if (d > -32) words[q] = seen_word(a, where->b, tok, d, where->s.drafts);
+            if (d <= -32) continue;
+            if (a.tokens <= kSeen)
+              words[q] = d >= 64 ? 0u
+                                 : static_cast<uint32_t>(d < 0 ? bits << -d | ((1u << -d) - 1u) : bits >> d);
+            else
+              words[q] = seen_word(a, where->b, tok, d, where->s.drafts);
           }
         }
         uint32_t sr[kTile];
@@ -610,10 +620,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         ptx::tmem_wait_st();
-        if (partly && !clean(j, k0)) {
-          ok = false;
-          break;
-        }
         warp_arrive(bar(S::kBarWeights + i), lane);
         ++cnt;
         ++done;
@@ -640,7 +646,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::tc_fence_after();
       const bool first = t0 == 0, last = t0 + n == unit.tiles;
       const bool any_odd = misc[2] == seg + 1u;
-      tile += n;
       // weights of the groups' sums in this thread's row
       float top = m_run, total = l_run, w[2] = {1.f, 1.f};
       if constexpr (!kTwo) {

@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
   constexpr int kRowsPer = kRows / (kColGroups > 0 ? kColGroups : 1);
   const int col = tid % DP, rg = tid / DP;
   const int pieces = a.head_dim / kPer16;
+#pragma unroll 1
   while (!run.done(pl)) {
     // ---- one unit, from key tile pl.t on
     const int rows = min(kRows, pl.s.drafts * a.group - pl.rt * kRows);
@@ -75,6 +76,7 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
       sm.l[tid] = 0.f;
     }
     float acc[kRowsPer] = {};
+#pragma unroll 1
     for (int t = t0; t < t0 + n; ++t) {
       const int k0 = t * kKeys;
       __syncthreads();

@@ -98,6 +98,7 @@ struct Place {
 template <class G>
 __device__ __forceinline__ void enter_seq(const Args& a, Place& p) {
   // the first sequence from p.b on with work; p.b == batch at the end
+#pragma unroll 1
   while (p.b < a.batch) {
     p.s = seq_of(a, p.b);
     p.tiles = G::key_tiles(p.s);
@@ -108,8 +109,11 @@ __device__ __forceinline__ void enter_seq(const Args& a, Place& p) {
 }
 
 // The first tile of the unit after p's.
+// Not inlined, like the other parts that run once a unit: with them in line at each
+// use the kernel was 188 KB of code, and the instruction fetches of the parts that run
+// seldom took longer than their work.
 template <class G>
-__device__ __forceinline__ void next_unit(const Args& a, Place& p) {
+__device__ __noinline__ void next_unit(const Args& a, Place& p) {
   p.t = 0;
   if (++p.rt < p.rts) return;
   p.rt = 0;
@@ -145,12 +149,13 @@ struct Run {
 // first place and the next run's walk to them.  `sums`: scratch of one value a warp.
 // Ends with a barrier; *out is in shared memory.
 template <class G>
-__device__ __forceinline__ void find_run(const Args& a, int64_t run, int64_t ctas, int64_t* sums,
+__device__ __noinline__ void find_run(const Args& a, int64_t run, int64_t ctas, int64_t* sums,
                                          Run* out) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.batch + nt - 1) / nt;
   const int b0 = min(a.batch, tid * each), b1 = min(a.batch, b0 + each);
   int64_t mine = 0;
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) mine += G::places(a, seq_of(a, b));
   int64_t incl = mine;
 #pragma unroll
@@ -161,12 +166,14 @@ __device__ __forceinline__ void find_run(const Args& a, int64_t run, int64_t cta
   if (lane == 31) sums[warp] = incl;
   __syncthreads();
   int64_t before = incl - mine, total = 0;
+#pragma unroll 1
   for (int w = 0; w < nt >> 5; ++w) {
     if (w < warp) before += sums[w];
     total += sums[w];
   }
   // runs [c total / runs, (c + 1) total / runs): none is empty of places
   const int64_t runs = min(total, ctas);
+#pragma unroll 1
   for (int end = 0; end < 2; ++end) {
     const int64_t at = run + end < runs ? (run + end) * total / runs : total;
     Place p{a.batch, 0, 0, 0, 0, 0, {0, 0}};
@@ -176,6 +183,7 @@ __device__ __forceinline__ void find_run(const Args& a, int64_t run, int64_t cta
     } else {
       if (mine == 0 || at < before || at >= before + mine) continue;
       int64_t left = at - before;
+#pragma unroll 1
       for (p.b = b0; p.b < b1; ++p.b) {
         p.s = seq_of(a, p.b);
         const int64_t all = G::places(a, p.s);
@@ -209,12 +217,14 @@ __device__ __forceinline__ void find_run(const Args& a, int64_t run, int64_t cta
 // The drafted tokens i >= n_b of the sequences that this CTA looks after get
 // zero rows (sequences without drafted tokens have no unit at all).
 // `threads`: the first threads of the CTA, which call this.
-__device__ __forceinline__ void zero_unused_rows(const Args& a, int elem_bytes, int threads) {
+static __device__ __noinline__ void zero_unused_rows(const Args& a, int elem_bytes, int threads) {
   const int heads = a.kv_heads * a.group;
   const int pieces = a.head_dim * elem_bytes / 16;
+#pragma unroll 1
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
     const Seq s = seq_of(a, b);
     const int n = (a.tokens - s.drafts) * heads * pieces;
+#pragma unroll 1
     for (int x = threadIdx.x; x < n; x += threads) {
       const int row = x / pieces;
       const int i = s.drafts + row / heads;
@@ -233,7 +243,7 @@ __device__ __forceinline__ bool sees(const Args& a, int b, int i, int j) {
 // draft.  Places before the draft are committed tokens, which it sees.  A row of
 // mask bytes is read as the aligned words that hold it, all at once: a byte at a
 // time, each waiting for its load, these reads took longer than the tile's products.
-__device__ __forceinline__ uint32_t seen_word(const Args& a, int b, int i, int d0, int drafts) {
+static __device__ __noinline__ uint32_t seen_word(const Args& a, int b, int i, int d0, int drafts) {
   uint32_t word = 0u;
   int n = drafts - d0;  // bits of the word that lie in the draft or before it
   if (!a.mask) {

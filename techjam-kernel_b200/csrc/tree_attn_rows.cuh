@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // row and column pair of this lane in a product
   const int mat = lane >> 3, mrow = lane & 7;    // matrix and row this lane addresses
 
+#pragma unroll 1
   while (!run.done(pl)) {
     const int t0 = pl.t;
     const int n = run.tiles(pl);
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
     }
     bool odd = false;  // a drafted token's value was not finite
 
+#pragma unroll 1
     for (int t = t0; t < t0 + n; ++t) {
       issue();
       cp_async_wait<NS - 1>();

@@ -76,7 +76,7 @@ struct TileShape {
   static_assert(sizeof(Place) == 32, "eight numbers");
   static_assert(sizeof(Run) <= 64, "a run's place");
   using G = Grid<RM, kTile, 2>;
-  static constexpr int kBarQ = 0, kBarQRead = 1, kBarFull = 2, kBarEmpty = kBarFull + kSlots,
+  static constexpr int kBarQ = 0, kBarQRead = 1, kBarSeen = 2, kBarFull = 3, kBarEmpty = kBarFull + kSlots,
                        kBarScores = kBarEmpty + kSlots, kBarRead = kBarScores + 2,
                        kBarWeights = kBarRead + 2, kBarSums = kBarWeights + 2,
                        kBarDrain = kBarSums + 2, kBars = kBarDrain + 1;
@@ -221,6 +221,34 @@ __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t word) {
     if (!((word >> k) & 1u)) s[k] = __float_as_uint(-INFINITY);
 }
 
+// Adds to a finished row (`out`) or its partial sums (`part`, columns `pitch` apart) the
+// values of drafted tokens d0..d1 that are not finite and that the row's token sees.
+// They were left out of the product, where a weight of zero would not hide them.
+template <int DT>
+__device__ __noinline__ void add_odd(const Args& a, const Place& unit, int tok, int d0, int d1,
+                                     int col0, int col1, uint16_t* out, float* part, int pitch) {
+  using E = Elem<DT>;
+  const uint32_t size = static_cast<uint32_t>(a.page_size);
+  for (int d = max(0, d0); d < min(unit.s.drafts, d1); ++d) {
+    if (!sees(a, unit.b, tok, d)) continue;
+    const uint32_t key = unit.s.len + d, slot = key / size;
+    const int pg = a.table[unit.b * a.table_stride + slot];
+    if (pg < 0 || pg >= a.pages) continue;
+    const typename E::T* v = reinterpret_cast<const typename E::T*>(
+        a.v + pg * a.v_page + unit.h * a.v_head + static_cast<int64_t>(key - slot * size) * a.v_row);
+    for (int c = col0; c < col1; ++c) {
+      const float x = E::widen(v[c]);
+      if (isfinite(x)) continue;
+      if (out) {
+        typename E::T* o = reinterpret_cast<typename E::T*>(out) + c;
+        *o = E::round(E::widen(*o) + x);
+      } else {
+        part[c * pitch] += x;
+      }
+    }
+  }
+}
+
 template <class S, int DT>
 __global__ void __launch_bounds__(kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -244,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     misc[1] = 0u;
     misc[2] = 0u;
-    ptx::mbar_init(bar(S::kBarQ), 2);
+    ptx::mbar_init(bar(S::kBarQ), 1);
+    ptx::mbar_init(bar(S::kBarSeen), 1);
     ptx::mbar_init(bar(S::kBarQRead), 1);
     for (int s = 0; s < NS; ++s) {
       ptx::mbar_init(bar(S::kBarFull + s), 1);
@@ -337,6 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t issued = 0;                             // one past the last load issued
     bool ok = true;
     int rest = 2;  // rounds after the last keys, for the last values
+#pragma unroll 1
     for (uint32_t t = 0; ok && rest > 0; ++t) {
       const Box now = next;
       if (t >= 2) {
@@ -364,35 +394,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------- scores S = Q K^T
     if (lane == 0) {
       constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, kTile, false);
-      uint32_t tile = 0, seg = 0, made[2] = {0u, 0u};
+      uint32_t tile = 0, seg = 0;
+      uint32_t made = 0u;  // bit i: parity of the number of scores made for group i
       int prev = -1;
       bool ok = true;
+#pragma unroll 1
       for (; ok && !run.done(pl); ++seg) {
         const int n = run.tiles(pl), rows = unit_rows(pl);
         ok = wait_bar(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
+        bool packed = false;
+#pragma unroll 1
         for (int j = 0; ok && j < n; ++j, ++tile) {
+          // the masks are there before the scores that need them
+          if (!packed && (j == n - 1 || (pl.t + j + 1) * kTile > pl.s.len)) {
+            ok = wait_bar(bar(S::kBarSeen), seg & 1u, abort_flag, a.err);
+            packed = true;
+          }
           const uint32_t number = S::load_k(tile), s = number % NS;
-          ok = issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
-#pragma unroll
+          ok = ok && issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
+#pragma unroll 1
           for (int i = 0; i < 2; ++i) {
             if (!ok || !takes(i, j, rows)) continue;
             // the scores before these have been copied to registers
-            if (prev >= 0 && !issuer_wait(bar(S::kBarRead + prev), (made[prev] - 1u) & 1u,
+            if (prev >= 0 && !issuer_wait(bar(S::kBarRead + prev), ((made >> prev) & 1u) ^ 1u,
                                           abort_flag, a.err)) {
               ok = false;
               continue;
             }
             ptx::tc_fence_after();
-            const uint32_t qa = sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes;
-            const uint32_t ka = sbase + S::kOffRing + s * S::kTileBytes;
+            const uint64_t qd = ptx::smem_desc_sw128(
+                sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes, 16, 1024);
+            const uint64_t kd =
+                ptx::smem_desc_sw128(sbase + S::kOffRing + s * S::kTileBytes, 16, 1024);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * S::kChunkBytes + (kk & 3) * 32;
-              ptx::tc_mma_ss(tmem, ptx::smem_desc_sw128(qa + off, 16, 1024),
-                             ptx::smem_desc_sw128(ka + off, 16, 1024), id, kk > 0 ? 1u : 0u);
+              const uint32_t off = ((kk >> 2) * S::kChunkBytes + (kk & 3) * 32) >> 4;
+              ptx::tc_mma_ss(tmem, qd + off, kd + off, id, kk > 0 ? 1u : 0u);
             }
             ptx::tc_commit(bar(S::kBarScores + i));
-            ++made[i];
+            made ^= 1u << i;
             prev = i;
           }
           if (ok) ptx::tc_commit(bar(S::kBarEmpty + s));
@@ -412,6 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t bytes = static_cast<uint32_t>(share) * 128u * S::kChunks;
     uint32_t seg = 0;
     bool ok = true;
+#pragma unroll 1
     for (; ok && !run.done(pl); ++seg) {
       ok = seg == 0 || warp_wait(bar(S::kBarQRead), (seg - 1u) & 1u, abort_flag, a.err);
       if (!ok) break;
@@ -426,7 +467,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                              bar(S::kBarQ), 64 * c, pl.h * a.group, first + i * tokens, pl.b);
       }
       if (a.tokens <= kSeen) {
-        // one row tile holds all tokens; a bit for each drafted token that a token sees
+        // a bit for each drafted token that a token sees
+#pragma unroll 1
         for (int tok = lane; tok < a.tokens; tok += 32) {
           const uint32_t lo = seen_word(a, pl.b, tok, 0, pl.s.drafts);
           const uint32_t hi = a.tokens > 32 ? seen_word(a, pl.b, tok, 32, pl.s.drafts) : 0u;
@@ -434,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
-      if (lane == 0) ptx::mbar_arrive(bar(S::kBarQ));
+      if (lane == 0) ptx::mbar_arrive(bar(S::kBarSeen));
       next_segment(pl);
     }
     if (!ok && seg > 0) settle(bar(S::kBarQ), (seg - 1u) & 1u);
@@ -442,11 +484,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kPvWarp) {
     // ------------------------------------------------------- O_i += P_i V
     constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, DP, true);
-    uint32_t tile = 0, seg = 0, made[2] = {0u, 0u};
+    uint32_t tile = 0, seg = 0;
+    uint32_t made = 0u;  // bit i: parity of the number of products made for group i
     bool ok = true;
+#pragma unroll 1
     for (; ok && !run.done(pl); ++seg) {
       const int n = run.tiles(pl), rows = unit_rows(pl), len = pl.s.len;
-      bool fresh[2] = {true, true};
+      uint32_t begun = 0u;  // bit i: O_i holds a product of this segment
+#pragma unroll 1
       for (int j = 0; ok && j < n; ++j, ++tile) {
         const uint32_t number = S::load_v(tile), s = number % NS;
         ok = warp_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
@@ -456,49 +501,68 @@ __global__ void __launch_bounds__(kThreads, 1)
           // Values past the last key become 0 (their rows may hold anything, and 0 x
           // infinity would reach the sums), and so do elements of drafted values that
           // are not finite: the softmax groups add those to the rows that see them.
-          const int r0 = max(0, len - k0), r1 = len + pl.s.drafts - k0;
+          const int r0 = max(0, len - k0), r1 = min(kTile, len + pl.s.drafts - k0);
+          auto piece = [&](int x) {  // shared-memory address of piece x of the tile's rows
+            const int pc = x % S::kPieces;
+            return va + (pc >> 3) * S::kChunkBytes + (x / S::kPieces) * 128 + ((pc & 7) << 4);
+          };
+          auto put = [&](int x, uint32_t (&w)[4]) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece(x)), "r"(w[0]),
+                         "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+          };
           bool odd = false;
-#pragma unroll 4
-          for (int x = lane; x < (kTile - r0) * S::kPieces; x += 32) {
-            const int r = r0 + x / S::kPieces, pc = x % S::kPieces;
-            const uint32_t ad = va + (pc >> 3) * S::kChunkBytes + r * 128 + ((pc & 7) << 4);
-            uint32_t w[4], any = 0u;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                         : "r"(ad));
+#pragma unroll 1
+          for (int x0 = r0 * S::kPieces; x0 < r1 * S::kPieces; x0 += 32 * 8) {
+            uint32_t w[8][4], any = 0u;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint32_t f = r < r1 ? not_finite<DT>(w[y]) : ~0u;
-              any |= f;
-              w[y] &= ~f;
+            for (int u = 0; u < 8; ++u) {
+              const int x = x0 + 32 * u + lane;
+              w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
+              if (x < r1 * S::kPieces)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3])
+                             : "r"(piece(x)));
             }
-            odd |= any != 0u && r < r1;
-            if (any)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ad), "r"(w[0]),
-                           "r"(w[1]), "r"(w[2]), "r"(w[3])
-                           : "memory");
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) any |= not_finite<DT>(w[u][y]);
+            if (any) {
+              odd = true;
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const int x = x0 + 32 * u + lane;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) w[u][y] &= ~not_finite<DT>(w[u][y]);
+                if (x < r1 * S::kPieces) put(x, w[u]);
+              }
+            }
           }
+          uint32_t zero[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1
+          for (int x = r1 * S::kPieces + lane; x < kTile * S::kPieces; x += 32) put(x, zero);
           if (odd) misc[2] = seg + 1u;
           ptx::fence_proxy_async_smem();
           __syncwarp();
         }
-#pragma unroll
+        const uint64_t vd = ptx::smem_desc_sw128(va, S::kChunkBytes, 1024);
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (!ok || !takes(i, j, rows)) continue;
-          ok = __all_sync(0xffffffffu, issuer_wait(bar(S::kBarWeights + i), made[i] & 1u, abort_flag,
-                                                   a.err));
+          ok = __all_sync(0xffffffffu, issuer_wait(bar(S::kBarWeights + i), (made >> i) & 1u,
+                                                   abort_flag, a.err));
           if (!ok) continue;
           ptx::tc_fence_after();
           if (lane == 0) {
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; ++kk)
               ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + S::kColP + 64 * i + kk * 8,
-                             ptx::smem_desc_sw128(va + kk * 2048, S::kChunkBytes, 1024), id,
-                             (!fresh[i] || kk > 0) ? 1u : 0u);
+                             vd + kk * (2048 >> 4), id, (((begun >> i) & 1u) || kk > 0) ? 1u : 0u);
             ptx::tc_commit(bar(S::kBarSums + i));
           }
-          fresh[i] = false;
-          ++made[i];
+          begun |= 1u << i;
+          made ^= 1u << i;
         }
         if (ok && lane == 0) ptx::tc_commit(bar(S::kBarEmpty + s));
       }
@@ -522,11 +586,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     uint32_t seg = 0, cnt = 0;  // segments of the run, tiles of this group
     bool ok = true;
+#pragma unroll 1
     for (; ok && !run.done(*where); ++seg) {
       const int n = run.tiles(*where), rows = unit_rows(*where), t0 = where->t, len = where->s.len;
       const bool idle = row0 + quad * 32 >= rows || quad * 32 >= share;  // padding rows only
       float m_run = -INFINITY, l_run = 0.f;
       int done = 0;
+#pragma unroll 1
       for (int j = 0; j < n; ++j) {
         if (!takes(i, j, rows)) continue;
         if (!warp_wait(bar(S::kBarScores + i), cnt & 1u, abort_flag, a.err)) {
@@ -662,7 +728,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const bool mine = rl < share && row0 + rl < rows;
       const int row = unit.rt * a.unit_rows + row0 + rl, tok = min(row / a.group, a.tokens - 1);
-      const uint32_t size = static_cast<uint32_t>(a.page_size);
       const bool finish = first && last;
       const float inv = total == 0.f ? 0.f : 1.f / total;
       uint8_t* out = a.o + unit.b * a.o_seq + (unit.h * a.group + row % a.group) * a.o_head +
@@ -672,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!idle) {
         // kTwo: all columns of the own rows; else half the columns of the shared ones
         constexpr int kSpan = kTwo ? DP : DP / 2;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kSpan / 32; ++c) {
           const int col = (kTwo ? 0 : i * kSpan) + 32 * c;
           uint32_t o[32];
@@ -692,27 +757,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               ptx::tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) acc[e] += w[1] * __uint_as_float(o[e]);
-            }
-          }
-          if (any_odd && mine) {
-            // this segment's drafted values that are not finite, for rows that see them
-            const int d1 = min(unit.s.drafts, (t0 + n) * kTile - len);
-            for (int d = max(0, t0 * kTile - len); d < d1; ++d) {
-              if (!sees(a, unit.b, tok, d)) continue;
-              const uint32_t key = len + d, slot = key / size;
-              const int pg = a.table[unit.b * a.table_stride + slot];
-              if (pg < 0 || pg >= a.pages) continue;
-              const uint32_t* v = reinterpret_cast<const uint32_t*>(
-                  a.v + pg * a.v_page + unit.h * a.v_head +
-                  static_cast<int64_t>(key - slot * size) * a.v_row + 2 * col);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                if (col + 2 * e >= a.head_dim) continue;
-                const uint32_t x = v[e], f = not_finite<DT>(x);
-                const float2 y = unpack2<DT>(x);
-                if (f & 0xffffu) acc[2 * e] += y.x;
-                if (f >> 16) acc[2 * e + 1] += y.y;
-              }
             }
           }
           if (finish) {
@@ -736,6 +780,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!finish && mine && (kTwo || i == 0)) {
         part[RM * DP + row0 + rl] = top;
         part[RM * DP + RM + row0 + rl] = total;
+      }
+      if (any_odd && mine) {
+        const int col0 = kTwo ? 0 : i * (DP / 2), col1 = min(a.head_dim, kTwo ? DP : col0 + DP / 2);
+        add_odd<DT>(a, unit, tok, t0 * kTile - len, (t0 + n) * kTile - len, col0, col1,
+                    finish ? reinterpret_cast<uint16_t*>(out) : nullptr, part + row0 + rl, RM);
       }
       if (threadIdx.x == 0 && last)
         a.desc[unit_of(a, unit)] =

@@ -31,7 +31,7 @@ struct PlainSmem {
   float p[kRows][kKeys + 1];
   float m[kRows], l[kRows], alpha[kRows];
   int page[kKeys];
-  int64_t sums[kThreads / 32];
+  uint32_t sums[kThreads / 32];
   Run run;
 };
 
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
           make_int2(t0 == 0 ? static_cast<int>(blockIdx.x) : run.first_run,
                     static_cast<int>(blockIdx.x));
     pl.t += n;
-    if (pl.t == pl.tiles) next_unit<PlainGrid>(a, pl);
+    if (pl.t == pl.tiles) pl = next_unit<PlainGrid>(a, pl);
     __syncthreads();
   }
 }
@@ -362,9 +362,10 @@ extern "C" int32_t b200_tree_attn_check(const b200_tree_attn_params* p) {
       !b200paged::vectors_aligned(p->o, p->o_stride, extent, 3, eb) ||
       (reinterpret_cast<uintptr_t>(p->draft_lens) & 3u))
     return B200_ATTN_ERR_ALIGNMENT;
-  // so are the key tiles of one CTA
-  if (static_cast<double>(c.batch * p->heads * p->tokens) *
-          static_cast<double>(c.slots * c.page_size) > 1e14)
+  // so are all key tiles of a call
+  const Choice ch = choose(p);
+  if (static_cast<double>(c.batch * c.kv_heads * row_tiles(p, ch)) *
+          static_cast<double>(c.slots * c.page_size / ch.tn + 4) > 2e9)
     return B200_ATTN_ERR_INVALID_ARGUMENT;
   if (p->mask && (p->mask_stride[0] < 0 || p->mask_stride[1] < 0 || p->mask_stride[2] < 0))
     return B200_ATTN_ERR_INVALID_ARGUMENT;

@@ -72,19 +72,20 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b) {
 }
 
 // RM rows and TN keys a tile, EX tiles' worth of work beside a unit's tiles.
-template <int RM_, int TN_, int EX_>
+template <int RM_, int TN_, uint32_t EX_>
 struct Grid {
-  static constexpr int RM = RM_, TN = TN_, EX = EX_;
+  static constexpr int RM = RM_, TN = TN_;
+  static constexpr uint32_t EX = EX_;
   __device__ static int key_tiles(const Seq& s) {
     return s.drafts > 0 ? (s.len + s.drafts + TN - 1) / TN : 0;
   }
   __device__ static int row_tiles(const Args& a, const Seq& s) {
     return (s.drafts * a.group + a.unit_rows - 1) / a.unit_rows;
   }
-  // places of a sequence in the line
-  __device__ static int64_t places(const Args& a, const Seq& s) {
+  // places of a sequence in the line (all sequences' together fit 31 bits)
+  __device__ static uint32_t places(const Args& a, const Seq& s) {
     const int t = key_tiles(s);
-    return t == 0 ? 0 : static_cast<int64_t>(t + EX) * row_tiles(a, s) * a.kv_heads;
+    return t == 0 ? 0u : (t + EX) * row_tiles(a, s) * a.kv_heads;
   }
 };
 
@@ -108,19 +109,19 @@ __device__ __forceinline__ void enter_seq(const Args& a, Place& p) {
   }
 }
 
-// The first tile of the unit after p's.
-// Not inlined, like the other parts that run once a unit: with them in line at each
-// use the kernel was 188 KB of code, and the instruction fetches of the parts that run
-// seldom took longer than their work.
+// The first tile of the unit after p's.  Not inlined, like the other parts that run
+// once a unit: with them in line at each use the kernels were up to 188 KB of code, and
+// fetching the instructions of what runs seldom took longer than its work.
 template <class G>
-__device__ __noinline__ void next_unit(const Args& a, Place& p) {
+__device__ __noinline__ Place next_unit(const Args& a, Place p) {
   p.t = 0;
-  if (++p.rt < p.rts) return;
+  if (++p.rt < p.rts) return p;
   p.rt = 0;
-  if (++p.h < a.kv_heads) return;
+  if (++p.h < a.kv_heads) return p;
   p.h = 0;
   ++p.b;
   enter_seq<G>(a, p);
+  return p;
 }
 
 __device__ __forceinline__ int unit_of(const Args& a, const Place& p) {
@@ -149,57 +150,57 @@ struct Run {
 // first place and the next run's walk to them.  `sums`: scratch of one value a warp.
 // Ends with a barrier; *out is in shared memory.
 template <class G>
-__device__ __noinline__ void find_run(const Args& a, int64_t run, int64_t ctas, int64_t* sums,
-                                         Run* out) {
+__device__ __noinline__ void find_run(const Args& a, uint32_t run, uint32_t ctas, uint32_t* sums,
+                                      Run* out) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.batch + nt - 1) / nt;
   const int b0 = min(a.batch, tid * each), b1 = min(a.batch, b0 + each);
-  int64_t mine = 0;
+  uint32_t mine = 0;
 #pragma unroll 1
   for (int b = b0; b < b1; ++b) mine += G::places(a, seq_of(a, b));
-  int64_t incl = mine;
+  uint32_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
+    const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += t;
   }
   if (lane == 31) sums[warp] = incl;
   __syncthreads();
-  int64_t before = incl - mine, total = 0;
+  uint32_t before = incl - mine, total = 0;
 #pragma unroll 1
   for (int w = 0; w < nt >> 5; ++w) {
     if (w < warp) before += sums[w];
     total += sums[w];
   }
-  // runs [c total / runs, (c + 1) total / runs): none is empty of places
-  const int64_t runs = min(total, ctas);
+  // `more` runs of q + 1 places, then runs of q: none is empty of places
+  const uint32_t runs = min(total, ctas), q = runs ? total / runs : 0u, more = total - q * runs;
 #pragma unroll 1
-  for (int end = 0; end < 2; ++end) {
-    const int64_t at = run + end < runs ? (run + end) * total / runs : total;
+  for (uint32_t end = 0; end < 2; ++end) {
+    const uint32_t c = run + end;
+    const uint32_t at = c < runs ? c * q + min(c, more) : total;
     Place p{a.batch, 0, 0, 0, 0, 0, {0, 0}};
     int first_run = 0;
     if (at == total) {
       if (tid != 0) continue;
     } else {
-      if (mine == 0 || at < before || at >= before + mine) continue;
-      int64_t left = at - before;
+      if (at < before || at >= before + mine) continue;
+      uint32_t left = at - before;
 #pragma unroll 1
       for (p.b = b0; p.b < b1; ++p.b) {
         p.s = seq_of(a, p.b);
-        const int64_t all = G::places(a, p.s);
+        const uint32_t all = G::places(a, p.s);
         if (left < all) break;
         left -= all;
       }
       p.tiles = G::key_tiles(p.s);
       p.rts = G::row_tiles(a, p.s);
-      const int span = p.tiles + G::EX;
-      const int x = static_cast<int>(left % span);
-      const int u = static_cast<int>(left / span);
-      p.t = max(0, x - G::EX);
-      p.rt = u % p.rts;
-      p.h = u / p.rts;
-      // the last run that begins at or before the unit's first tile
-      first_run = static_cast<int>(((at - x + G::EX + 1) * runs - 1) / total);
+      const uint32_t span = p.tiles + G::EX, u = left / span, x = left - u * span;
+      p.t = x > G::EX ? static_cast<int>(x - G::EX) : 0;
+      p.h = static_cast<int>(u) / p.rts;
+      p.rt = static_cast<int>(u) - p.h * p.rts;
+      // the run that the unit's first tile lies in
+      const uint32_t tile = at - x + G::EX, long_runs = more * (q + 1);
+      first_run = static_cast<int>(tile < long_runs ? tile / (q + 1) : more + (tile - long_runs) / q);
     }
     if (end == 0) {
       out->p = p;
@@ -299,6 +300,34 @@ struct Elem<B200_ATTN_DTYPE_FP32> {
   __device__ static float widen(T x) { return x; }
   __device__ static T round(float x) { return x; }
 };
+
+// Adds to a finished row (`out`) or its partial sums (`part`, columns `pitch` apart) the
+// values of drafted tokens d0..d1 that are not finite and that the row's token sees.
+// They were left out of the product, where a weight of zero would not hide them.
+template <int DT>
+__device__ __noinline__ void add_odd(const Args& a, int b, int h, Seq s, int tok, int d0, int d1,
+                                     int col0, int col1, uint16_t* out, float* part, int pitch) {
+  using E = Elem<DT>;
+  const uint32_t size = static_cast<uint32_t>(a.page_size);
+  for (int d = max(0, d0); d < min(s.drafts, d1); ++d) {
+    if (!sees(a, b, tok, d)) continue;
+    const uint32_t key = s.len + d, slot = key / size;
+    const int pg = a.table[b * a.table_stride + slot];
+    if (pg < 0 || pg >= a.pages) continue;
+    const typename E::T* v = reinterpret_cast<const typename E::T*>(
+        a.v + pg * a.v_page + h * a.v_head + static_cast<int64_t>(key - slot * size) * a.v_row);
+    for (int c = col0; c < col1; ++c) {
+      const float x = E::widen(v[c]);
+      if (isfinite(x)) continue;
+      if (out) {
+        typename E::T* o = reinterpret_cast<typename E::T*>(out) + c;
+        *o = E::round(E::widen(*o) + x);
+      } else {
+        part[c * pitch] += x;
+      }
+    }
+  }
+}
 
 // Joins the partial results of cut units.  The warps of a block share the runs of a
 // unit, so that all of them are read at once, each with its own maximum and sums;

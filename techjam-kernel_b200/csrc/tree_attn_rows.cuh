@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   const uint32_t sbase = b200attn::ptx::smem_u32(smem);
   float* join = reinterpret_cast<float*>(smem + S::kOffJoin);
   float* stat = reinterpret_cast<float*>(smem + S::kOffStat);  // [warp][{max, sum}][RM]
-  int64_t* sums = reinterpret_cast<int64_t*>(smem + S::kOffMisc);
+  uint32_t* sums = reinterpret_cast<uint32_t*>(smem + S::kOffMisc);
   Run* found = reinterpret_cast<Run*>(smem + S::kOffMisc + 80);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   b200attn::ptx::launch_dependents();
@@ -170,14 +170,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
         cp_async16(dst + off, ks, ok ? 16u : 0u);
         cp_async16(dst + S::kBlockBytes + off, vs, ok ? 16u : 0u);
       }
-      if (++ld.t == ld.tiles) next_unit<typename S::G>(a, ld);
+      if (++ld.t == ld.tiles) ld = next_unit<typename S::G>(a, ld);
       more = !run.done(ld);
       if (more) look_up();
     }
     cp_async_commit();
     stage = stage + 1 == NS ? 0 : stage + 1;
   };
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < NS - 1; ++s) issue();
   zero_unused_rows(a, 2, kRowThreads);
 
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
     const Place done = pl;
     const bool first = t0 == 0, last = t0 + n == pl.tiles;
     pl.t += n;
-    if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
+    if (pl.t == pl.tiles) pl = next_unit<typename S::G>(a, pl);
     const bool again = !run.done(pl);
     if (again) fetch_q(pl);  // on its way while the results are joined
 #pragma unroll
@@ -457,23 +457,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
         acc.x += v.x;
         acc.y += v.y;
       }
-      if (any_odd && r < rows) {
-        // this run's drafted values that are not finite, for the rows that see them
-        const int j1 = min(done.s.drafts, (t0 + n) * kRowTile - done.s.len);
-        for (int j = max(0, t0 * kRowTile - done.s.len); j < j1; ++j) {
-          if (c0 + c >= a.head_dim || !sees(a, done.b, tok, j)) continue;
-          const uint32_t key = done.s.len + j, slot = key / size;
-          const int pg = a.table[done.b * a.table_stride + slot];
-          if (pg < 0 || pg >= a.pages) continue;
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(
-              a.v + pg * a.v_page + done.h * a.v_head +
-              static_cast<int64_t>(key - slot * size) * a.v_row + 2 * (c0 + c));
-          const uint32_t f = non_finite<DT>(w);
-          const float2 v = unpack_pair<DT>(w);
-          if (f & 0xffffu) acc.x += v.x;
-          if (f >> 16) acc.y += v.y;
-        }
-      }
       if (finish) {
         if (r < rows && c0 + c < a.head_dim)
           *reinterpret_cast<uint32_t*>(out + 2 * (c0 + c)) = pack_pair<DT>(acc.x * inv, acc.y * inv);
@@ -481,6 +464,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
         *reinterpret_cast<float2*>(part + r * DP + c0 + c) = acc;
       }
     }
+    if (any_odd && r < rows)
+      for (int c0 = c; c0 < DP; c0 += S::kCols)
+        add_odd<DT>(a, done.b, done.h, done.s, tok, t0 * kRowTile - done.s.len,
+                    (t0 + n) * kRowTile - done.s.len, c0, min(a.head_dim, c0 + kEach),
+                    finish ? reinterpret_cast<uint16_t*>(out) : nullptr, part + r * DP, 1);
     if (!finish && c == 0) {
       part[RM * DP + r] = top;
       part[RM * DP + RM + r] = total;

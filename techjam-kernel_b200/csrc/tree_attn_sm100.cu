@@ -221,34 +221,6 @@ __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t word) {
     if (!((word >> k) & 1u)) s[k] = __float_as_uint(-INFINITY);
 }
 
-// Adds to a finished row (`out`) or its partial sums (`part`, columns `pitch` apart) the
-// values of drafted tokens d0..d1 that are not finite and that the row's token sees.
-// They were left out of the product, where a weight of zero would not hide them.
-template <int DT>
-__device__ __noinline__ void add_odd(const Args& a, const Place& unit, int tok, int d0, int d1,
-                                     int col0, int col1, uint16_t* out, float* part, int pitch) {
-  using E = Elem<DT>;
-  const uint32_t size = static_cast<uint32_t>(a.page_size);
-  for (int d = max(0, d0); d < min(unit.s.drafts, d1); ++d) {
-    if (!sees(a, unit.b, tok, d)) continue;
-    const uint32_t key = unit.s.len + d, slot = key / size;
-    const int pg = a.table[unit.b * a.table_stride + slot];
-    if (pg < 0 || pg >= a.pages) continue;
-    const typename E::T* v = reinterpret_cast<const typename E::T*>(
-        a.v + pg * a.v_page + unit.h * a.v_head + static_cast<int64_t>(key - slot * size) * a.v_row);
-    for (int c = col0; c < col1; ++c) {
-      const float x = E::widen(v[c]);
-      if (isfinite(x)) continue;
-      if (out) {
-        typename E::T* o = reinterpret_cast<typename E::T*>(out) + c;
-        *o = E::round(E::widen(*o) + x);
-      } else {
-        part[c * pitch] += x;
-      }
-    }
-  }
-}
-
 template <class S, int DT>
 __global__ void __launch_bounds__(kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -293,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::tma_prefetch_desc(&tm_v);
   }
   ptx::grid_dependency_wait();
-  find_run<typename S::G>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem + S::kOffSums),
+  find_run<typename S::G>(a, blockIdx.x, gridDim.x, reinterpret_cast<uint32_t*>(smem + S::kOffSums),
                           found);
   const Run& run = *found;
   Place pl = run.p;
@@ -321,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   auto next_segment = [&](Place& p) {
     p.t += run.tiles(p);
-    if (p.t == p.tiles) next_unit<typename S::G>(a, p);
+    if (p.t == p.tiles) p = next_unit<typename S::G>(a, p);
   };
 
   if (warp == kLoadWarp) {
@@ -381,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ok = ok && load(S::load_k(t), &tm_k, now);
       if (ok) issued = S::load_k(t) + 1;
-      if (++pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
+      if (++pl.t == pl.tiles) pl = next_unit<typename S::G>(a, pl);
       if (!run.done(pl)) next = look_up();
     }
     if (!ok) {
@@ -439,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ptx::tc_commit(bar(S::kBarQRead));
         pl.t += n;
-        if (pl.t == pl.tiles) next_unit<typename S::G>(a, pl);
+        if (pl.t == pl.tiles) pl = next_unit<typename S::G>(a, pl);
       }
       ptx::tc_commit(bar(S::kBarDrain));
       settle(bar(S::kBarDrain), 0);
@@ -783,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (any_odd && mine) {
         const int col0 = kTwo ? 0 : i * (DP / 2), col1 = min(a.head_dim, kTwo ? DP : col0 + DP / 2);
-        add_odd<DT>(a, unit, tok, t0 * kTile - len, (t0 + n) * kTile - len, col0, col1,
+        add_odd<DT>(a, unit.b, unit.h, unit.s, tok, t0 * kTile - len, (t0 + n) * kTile - len, col0, col1,
                     finish ? reinterpret_cast<uint16_t*>(out) : nullptr, part + row0 + rl, RM);
       }
       if (threadIdx.x == 0 && last)

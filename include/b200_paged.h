@@ -142,7 +142,14 @@ typedef struct b200_tree_attn_params {
   int32_t reserved;       /* 0 */
   void* workspace;        /* b200_tree_attn_workspace_bytes(p) bytes, 16-byte aligned */
   int64_t workspace_bytes;
+  /* Optional B200_TREE_ATTN_COUNTERS int32 in device memory, zero before the first
+   * call and left zero by every call, for calls that do not overlap in time (one
+   * stream's): a call of few rows then joins its partial results in the same kernel
+   * instead of a second one. */
+  int32_t* counters;
 } b200_tree_attn_params;
+
+#define B200_TREE_ATTN_COUNTERS 1024
 
 B200_ATTN_API int32_t b200_tree_attn_check(const b200_tree_attn_params* p);
 B200_ATTN_API int64_t b200_tree_attn_workspace_bytes(const b200_tree_attn_params* p);

@@ -251,6 +251,7 @@ class TreeAttnParams(ctypes.Structure):
         ("reserved", ctypes.c_int32),
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_int64),
+        ("counters", ctypes.c_void_p),
     ]
 
 

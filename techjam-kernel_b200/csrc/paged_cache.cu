@@ -221,6 +221,71 @@ struct Scratch {
   uint32_t* flags;   // [ceil(batch * slots / 32) + 32]
 };
 
+// ------------------------------------------------------------------- moves
+// Warps take (move, layer, K or V, head) segments in turn; a segment's rows are
+// contiguous pieces of 16 bytes, and a lane keeps kUnroll of them in flight.
+constexpr int kUnroll = 4;
+
+// By warp `warp` of `warps`.
+__device__ __forceinline__ void move_rows(const Pool& c, const Scratch& w, int count, int warp,
+                                          int warps) {
+  const int lane = threadIdx.x & 31;
+  const int per_move = c.layers * 2 * c.heads;
+  const int64_t items = static_cast<int64_t>(count) * per_move;
+  for (int64_t it = warp; it < items; it += warps) {
+    const int i = static_cast<int>(it / per_move);
+    const int rest = static_cast<int>(it - static_cast<int64_t>(i) * per_move);
+    const int h = rest % c.heads, lv = rest / c.heads;
+    const int layer = lv >> 1;
+    const bool value = lv & 1;
+    const Move m = w.moves[i];
+    uint8_t* base = value ? c.v + layer * c.v_layer + h * c.v_head
+                          : c.k + layer * c.k_layer + h * c.k_head;
+    const int64_t page_bytes = value ? c.v_page : c.k_page;
+    const int64_t row_bytes = value ? c.v_row : c.k_row;
+    const uint8_t* src = base + m.src * page_bytes;
+    uint8_t* dst = base + m.dst * page_bytes;
+    const int pieces = m.rows * c.chunks;
+    for (int x0 = lane; x0 < pieces; x0 += 32 * kUnroll) {
+      uint4 a[kUnroll];
+      int64_t off[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int x = x0 + 32 * u;
+        const int row = x / c.chunks;
+        off[u] = row * row_bytes + 16 * (x - row * c.chunks);
+        if (x < pieces) a[u] = __ldcs(reinterpret_cast<const uint4*>(src + off[u]));
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (x0 + 32 * u < pieces) *reinterpret_cast<uint4*>(dst + off[u]) = a[u];
+    }
+  }
+}
+
+// Table entries follow the moved pages.  By thread `at` of `threads`.
+__device__ __forceinline__ void remap_table(const Pool& c, const Scratch& w, int held, int64_t at,
+                                            int64_t threads) {
+  const int64_t entries = static_cast<int64_t>(c.batch) * c.slots;
+  for (int64_t e = at; e < entries; e += threads) {
+    int32_t* t = &c.table[(e / c.slots) * c.table_stride + e % c.slots];
+    const int p = *t;
+    if (p >= c.pages) report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
+    else if (p >= held && c.refs[p] == 0) *t = w.list[p];
+  }
+}
+
+template <bool kRemap>
+__global__ void __launch_bounds__(kCopyThreads) move_kernel(const Pool c, const Scratch w) {
+  b200attn::ptx::launch_dependents();
+  b200attn::ptx::grid_dependency_wait();
+  const int warps = kCopyThreads / 32;
+  move_rows(c, w, w.count[0], blockIdx.x * warps + (threadIdx.x >> 5), gridDim.x * warps);
+  if constexpr (kRemap)
+    remap_table(c, w, w.count[1], static_cast<int64_t>(blockIdx.x) * kCopyThreads + threadIdx.x,
+                static_cast<int64_t>(gridDim.x) * kCopyThreads);
+}
+
 // ----------------------------------------------------------------- reserve
 // One CTA.  The slots that the batch writes are numbered in (sequence, slot)
 // order; pass 1 flags those that need a page, pass 2 lists as many free pages,
@@ -228,7 +293,7 @@ struct Scratch {
 // counts before the whole request is known to fit.
 __global__ void __launch_bounds__(kPlanThreads)
     reserve_plan_kernel(const Pool c, const int32_t* tokens, int64_t uniform, int32_t* status,
-                        const Scratch w) {
+                        const Scratch w, const bool moves_here) {
   extern __shared__ int32_t first_of[];  // [batch + 1] slots wanted before sequence b
   __shared__ int part[33];
   __shared__ int bad, carry, copies;
@@ -350,7 +415,8 @@ __global__ void __launch_bounds__(kPlanThreads)
     }
   }
   __syncthreads();
-  if (tid == 0) w.count[0] = copies;
+  if (moves_here) move_rows(c, w, copies, tid >> 5, kPlanThreads / 32);
+  else if (tid == 0) w.count[0] = copies;
 }
 
 // ----------------------------------------------------------------- compact
@@ -358,7 +424,7 @@ __global__ void __launch_bounds__(kPlanThreads)
 // the held pages at or past n (ascending), so sources and destinations never
 // meet and every page moves at most once.
 __global__ void __launch_bounds__(kPlanThreads)
-    compact_plan_kernel(const Pool c, int32_t* live, const Scratch w) {
+    compact_plan_kernel(const Pool c, int32_t* live, const Scratch w, const bool moves_here) {
   __shared__ int part[33];
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
@@ -404,62 +470,10 @@ __global__ void __launch_bounds__(kPlanThreads)
     w.count[1] = held;
     *live = held;
   }
-}
-
-// ------------------------------------------------------------- move kernel
-// Warps take (move, layer, K or V, head) segments in turn; a segment's rows are
-// contiguous pieces of 16 bytes, and a lane keeps kUnroll of them in flight.
-constexpr int kUnroll = 4;
-
-template <bool kRemap>
-__global__ void __launch_bounds__(kCopyThreads) move_kernel(const Pool c, const Scratch w) {
-  b200attn::ptx::launch_dependents();
-  b200attn::ptx::grid_dependency_wait();
-  const int count = w.count[0];
-  const int lane = threadIdx.x & 31;
-  const int warps = kCopyThreads / 32;
-  const int per_move = c.layers * 2 * c.heads;
-  const int64_t items = static_cast<int64_t>(count) * per_move;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * warps + (threadIdx.x >> 5); it < items;
-       it += static_cast<int64_t>(gridDim.x) * warps) {
-    const int i = static_cast<int>(it / per_move);
-    const int rest = static_cast<int>(it - static_cast<int64_t>(i) * per_move);
-    const int h = rest % c.heads, lv = rest / c.heads;
-    const int layer = lv >> 1;
-    const bool value = lv & 1;
-    const Move m = w.moves[i];
-    uint8_t* base = value ? c.v + layer * c.v_layer + h * c.v_head
-                          : c.k + layer * c.k_layer + h * c.k_head;
-    const int64_t page_bytes = value ? c.v_page : c.k_page;
-    const int64_t row_bytes = value ? c.v_row : c.k_row;
-    const uint8_t* src = base + m.src * page_bytes;
-    uint8_t* dst = base + m.dst * page_bytes;
-    const int pieces = m.rows * c.chunks;
-    for (int x0 = lane; x0 < pieces; x0 += 32 * kUnroll) {
-      uint4 a[kUnroll];
-      int64_t off[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int x = x0 + 32 * u;
-        const int row = x / c.chunks;
-        off[u] = row * row_bytes + 16 * (x - row * c.chunks);
-        if (x < pieces) a[u] = __ldcs(reinterpret_cast<const uint4*>(src + off[u]));
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (x0 + 32 * u < pieces) *reinterpret_cast<uint4*>(dst + off[u]) = a[u];
-    }
-  }
-  if constexpr (kRemap) {
-    const int held = w.count[1];
-    const int64_t entries = static_cast<int64_t>(c.batch) * c.slots;
-    for (int64_t e = static_cast<int64_t>(blockIdx.x) * kCopyThreads + threadIdx.x; e < entries;
-         e += static_cast<int64_t>(gridDim.x) * kCopyThreads) {
-      int32_t* t = &c.table[(e / c.slots) * c.table_stride + e % c.slots];
-      const int p = *t;
-      if (p >= c.pages) report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
-      else if (p >= held && c.refs[p] == 0) *t = w.list[p];
-    }
+  if (moves_here) {
+    __syncthreads();
+    move_rows(c, w, holes, tid >> 5, kPlanThreads / 32);
+    remap_table(c, w, held, tid, kPlanThreads);
   }
 }
 
@@ -584,6 +598,11 @@ int32_t check_table(const b200_cache* c) {
   return B200_ATTN_OK;
 }
 
+// Bytes of one page's keys and values in all layers.
+int64_t page_bytes(const b200_cache* c) {
+  return 2 * c->layers * c->kv_heads * c->page_size * c->head_dim * elem_bytes(c->dtype);
+}
+
 int32_t check_scratch(const b200_cache* c, const void* ws, int64_t bytes) {
   if (!ws || bytes < b200_cache_workspace_bytes(c)) return B200_ATTN_ERR_INVALID_ARGUMENT;
   return (reinterpret_cast<uintptr_t>(ws) & 15u) ? B200_ATTN_ERR_ALIGNMENT : B200_ATTN_OK;
@@ -597,6 +616,9 @@ ByteRange span(const void* base, const int64_t* stride, const int64_t* extent, i
   const uintptr_t lo = reinterpret_cast<uintptr_t>(base);
   return ByteRange{lo, lo + static_cast<uintptr_t>(last * eb)};
 }
+
+// Up to so many bytes are moved by the planning CTA itself: a second launch takes longer.
+constexpr int64_t kMovesHere = 1 << 20;
 
 unsigned move_grid(int device, int64_t items) {
   const int64_t most = 8ll * sm_count(device);
@@ -714,10 +736,12 @@ extern "C" int32_t b200_cache_reserve(const b200_cache* c, const int32_t* tokens
   if ((rc = resolve_error_word(c->error_word, &p.err)) != B200_ATTN_OK) return rc;
   const Scratch w = scratch_of(c, workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  rc = launch(reserve_plan_kernel, dim3(1), dim3(kPlanThreads),
-              sizeof(int32_t) * static_cast<size_t>(c->batch + 1), s, p, tokens, uniform, status, w);
-  if (rc != B200_ATTN_OK) return rc;
   // at most one page of a sequence is copied
+  const bool here = c->batch * page_bytes(c) <= kMovesHere;
+  rc = launch(reserve_plan_kernel, dim3(1), dim3(kPlanThreads),
+              sizeof(int32_t) * static_cast<size_t>(c->batch + 1), s, p, tokens, uniform, status, w,
+              here);
+  if (rc != B200_ATTN_OK || here) return rc;
   return launch(move_kernel<false>, dim3(move_grid(scope.device, c->batch * c->layers * 2 * c->kv_heads)),
                 dim3(kCopyThreads), 0, s, p, w);
 }
@@ -770,8 +794,10 @@ extern "C" int32_t b200_cache_compact(const b200_cache* c, int32_t* live, void* 
   if ((rc = resolve_error_word(c->error_word, &p.err)) != B200_ATTN_OK) return rc;
   const Scratch w = scratch_of(c, workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  rc = launch(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, live, w);
-  if (rc != B200_ATTN_OK) return rc;
+  // at most every second page moves
+  const bool here = c->pages / 2 * page_bytes(c) <= kMovesHere;
+  rc = launch(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, live, w, here);
+  if (rc != B200_ATTN_OK || here) return rc;
   return launch(move_kernel<true>, dim3(move_grid(scope.device, c->pages * c->layers * 2 * c->kv_heads)),
                 dim3(kCopyThreads), 0, s, p, w);
 }

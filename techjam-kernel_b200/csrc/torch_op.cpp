@@ -13,11 +13,15 @@
 // packing; the kernel, its tensor maps and its checks are the C library's.
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
 #include <cmath>
+#include <map>
+#include <mutex>
 #include <optional>
+#include <utility>
 
 #include "b200_attn.h"
 #include "b200_paged.h"
@@ -345,6 +349,27 @@ at::Tensor cache_compact(const at::Tensor& k, const at::Tensor& v, const at::Ten
   return live;
 }
 
+// Zeroed counters of a stream's calls (b200_tree_attn_params::counters), kept for the
+// process.  None while a graph is captured: a replay may run beside calls on the stream
+// that captured it.
+int32_t* counters_of(cudaStream_t stream, const at::Tensor& like) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &status) != cudaSuccess ||
+      status != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  static std::mutex mu;
+  static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();
+  std::lock_guard<std::mutex> lock(mu);
+  at::Tensor& t = (*kept)[{like.device().index(), stream}];
+  if (!t.defined()) {
+    const c10::InferenceMode off(false);
+    t = at::zeros({B200_TREE_ATTN_COUNTERS}, like.options().dtype(at::kInt));
+  }
+  return static_cast<int32_t*>(t.data_ptr());
+}
+
 at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                           const at::Tensor& table, const at::Tensor& lens, const OptTensor& mask,
                           const OptTensor& draft_lens, std::optional<double> scale,
@@ -409,7 +434,9 @@ at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Te
     ws = scratch(p.workspace_bytes, q);
     p.workspace = ws.data_ptr();
   }
-  raise_code("b200_tree_attn_fwd", b200_tree_attn_fwd(&p, stream_of(q)));
+  const cudaStream_t stream = stream_of(q);
+  p.counters = counters_of(stream, q);
+  raise_code("b200_tree_attn_fwd", b200_tree_attn_fwd(&p, stream));
   return result;
 }
 

@@ -198,10 +198,21 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
         part[kRows * DP + kRows + tid] = sm.l[tid];
       }
     }
-    if (tid == 0 && t0 + n == pl.tiles)
-      a.desc[unit_of(a, pl)] =
-          make_int2(t0 == 0 ? static_cast<int>(blockIdx.x) : run.first_run,
-                    static_cast<int>(blockIdx.x));
+    const bool first = t0 == 0, last = t0 + n == pl.tiles;
+    if (!(first && last)) {
+      const int from = run.ends_in(pl) ? run.end_first : (first ? blockIdx.x : run.first_run);
+      const int to = run.ends_in(pl) ? run.end_last : blockIdx.x;
+      if (a.counters) {
+        static_assert(sizeof(JoinSmem<DP, kThreads / 32>) <= sizeof(sm.k), "joins in place");
+        join_if_last<kRows, DP, DT, kThreads / 32>(
+            a, pl.b, pl.h, pl.rt, rows, from, to,
+            reinterpret_cast<JoinSmem<DP, kThreads / 32>*>(&sm.k[0][0]));
+      } else if (tid == 0 && last) {
+        a.desc[unit_of(a, pl)] = make_int2(from, to);
+      }
+    } else if (tid == 0 && !a.counters) {
+      a.desc[unit_of(a, pl)] = make_int2(0, 0);
+    }
     pl.t += n;
     if (pl.t == pl.tiles) pl = next_unit<PlainGrid>(a, pl);
     __syncthreads();
@@ -255,6 +266,10 @@ int64_t row_tiles(const b200_tree_attn_params* p, const Choice& c) {
   return (p->tokens * (p->heads / p->cache.kv_heads) + c.rows - 1) / c.rows;
 }
 
+int64_t units_of(const b200_tree_attn_params* p, const Choice& c) {
+  return p->cache.batch * p->cache.kv_heads * row_tiles(p, c);
+}
+
 constexpr int64_t kMaxRuns = 148 * 8;
 
 // CTAs of a call on a GPU of `sms` SMs: no more than there can be key tiles.
@@ -272,10 +287,10 @@ int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
 }
 
 
-template <int RM, int DP, int DT>
+template <int RM, int DP, int DT, int WARPS>
 int32_t run_join_rows(const Args& a, int64_t units, cudaStream_t s) {
-  return launch(join_rows_kernel<RM, DP, DT>, dim3(static_cast<unsigned>(units), RM / 4),
-                dim3(32 * kJoinWarps), 0, s, a);
+  return launch(join_rows_kernel<RM, DP, DT, WARPS>, dim3(static_cast<unsigned>(units), RM / 4),
+                dim3(32 * WARPS), 0, s, a);
 }
 
 template <int RM, int DP, int DT>
@@ -301,7 +316,8 @@ int32_t run_one(void (*kernel)(Args), int threads, int smem, const Args& a, int 
   return launch(kernel, dim3(runs), dim3(threads), smem, s, a);
 }
 
-// One kernel over the runs, one that joins the units that were cut.
+// One kernel over the runs, and where it does not join the units that were cut, one that
+// does.
 template <int DP, int DT>
 int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int device,
                   cudaStream_t s) {
@@ -309,7 +325,7 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
   if constexpr (DT == B200_ATTN_DTYPE_FP32) {
     rc = run_one<16, DP, DT>(plain_kernel<DP, DT>, kThreads, sizeof(PlainSmem<DP>), a, runs, device,
                              s);
-    return rc != B200_ATTN_OK ? rc : run_join_rows<kRows, DP, DT>(a, units, s);
+    return rc != B200_ATTN_OK || a.counters ? rc : run_join_rows<kRows, DP, DT, kThreads / 32>(a, units, s);
   } else {
     using One = RowShape<1, DP>;
     using Two = RowShape<2, DP>;
@@ -321,10 +337,10 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
     else
       rc = run_one<32, DP, DT>(rows_kernel<Two, DT>, kRowThreads, Two::kSmemBytes, a, runs, device,
                                s);
-    if (rc != B200_ATTN_OK) return rc;
+    if (rc != B200_ATTN_OK || a.counters) return rc;
     switch (c.rm) {
-      case 16: return run_join_rows<16, DP, DT>(a, units, s);
-      case 32: return run_join_rows<32, DP, DT>(a, units, s);
+      case 16: return run_join_rows<16, DP, DT, kRowWarps>(a, units, s);
+      case 32: return run_join_rows<32, DP, DT, kRowWarps>(a, units, s);
       case 128: return run_join_columns<128, DP, DT>(a, units, s);
       default: return run_join_columns<256, DP, DT>(a, units, s);
     }
@@ -360,7 +376,7 @@ extern "C" int32_t b200_tree_attn_check(const b200_tree_attn_params* p) {
   const int64_t eb = b200paged::elem_bytes(c.dtype);
   if (!b200paged::vectors_aligned(p->q, p->q_stride, extent, 3, eb) ||
       !b200paged::vectors_aligned(p->o, p->o_stride, extent, 3, eb) ||
-      (reinterpret_cast<uintptr_t>(p->draft_lens) & 3u))
+      ((reinterpret_cast<uintptr_t>(p->draft_lens) | reinterpret_cast<uintptr_t>(p->counters)) & 3u))
     return B200_ATTN_ERR_ALIGNMENT;
   // so are all key tiles of a call
   const Choice ch = choose(p);
@@ -428,8 +444,9 @@ extern "C" int32_t b200_tree_attn_fwd(const b200_tree_attn_params* p, void* stre
   a.scale_log2 = p->scale * 1.4426950408889634f;
   a.desc = static_cast<int2*>(p->workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + desc_bytes(p, ch));
+  if (ch.kernel != kManyRows && units_of(p, ch) <= B200_TREE_ATTN_COUNTERS) a.counters = p->counters;
   const int runs = static_cast<int>(runs_of(p, ch, b200paged::sm_count(scope.device)));
-  const int64_t units = c.batch * c.kv_heads * row_tiles(p, ch);
+  const int64_t units = units_of(p, ch);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (c.dtype) {
     case B200_ATTN_DTYPE_BF16:

@@ -48,6 +48,7 @@ struct Args {
   int32_t row_tiles;  // of a full draft: the stride of unit numbers
   float scale_log2;
   int2* desc;       // [batch * kv_heads * row_tiles] first and last run of a unit
+  int32_t* counters;  // null, or one a unit, zero between calls
   float* partial;   // [2 * runs] x {sums [RM][DP], maximum [RM], sum [RM]}
   int32_t* err;
 };
@@ -129,11 +130,12 @@ __device__ __forceinline__ int unit_of(const Args& a, const Place& p) {
 }
 
 // A CTA's run: from place `p` up to, not including, tile et of unit (eb, eh, ert).
-// first_run: the run that holds the first tile of p's unit.
+// first_run: the run that holds the first tile of p's unit; end_first, end_last: the
+// runs that hold the first and the last tile of the unit that the run ends in.
 struct Run {
   Place p;
   int eb, eh, ert, et;
-  int first_run;
+  int first_run, end_first, end_last;
 
   __device__ __forceinline__ bool ends_in(const Place& x) const {
     return x.b == eb && x.h == eh && x.rt == ert;
@@ -179,7 +181,7 @@ __device__ __noinline__ void find_run(const Args& a, uint32_t run, uint32_t ctas
     const uint32_t c = run + end;
     const uint32_t at = c < runs ? c * q + min(c, more) : total;
     Place p{a.batch, 0, 0, 0, 0, 0, {0, 0}};
-    int first_run = 0;
+    int first_run = 0, last_run = 0;
     if (at == total) {
       if (tid != 0) continue;
     } else {
@@ -198,9 +200,11 @@ __device__ __noinline__ void find_run(const Args& a, uint32_t run, uint32_t ctas
       p.t = x > G::EX ? static_cast<int>(x - G::EX) : 0;
       p.h = static_cast<int>(u) / p.rts;
       p.rt = static_cast<int>(u) - p.h * p.rts;
-      // the run that the unit's first tile lies in
-      const uint32_t tile = at - x + G::EX, long_runs = more * (q + 1);
-      first_run = static_cast<int>(tile < long_runs ? tile / (q + 1) : more + (tile - long_runs) / q);
+      // the runs that the unit's first and last tile lie in
+      const uint32_t long_runs = more * (q + 1);
+      const uint32_t head = at - x + G::EX, tail = at - x + span - 1;
+      first_run = static_cast<int>(head < long_runs ? head / (q + 1) : more + (head - long_runs) / q);
+      last_run = static_cast<int>(tail < long_runs ? tail / (q + 1) : more + (tail - long_runs) / q);
     }
     if (end == 0) {
       out->p = p;
@@ -210,6 +214,8 @@ __device__ __noinline__ void find_run(const Args& a, uint32_t run, uint32_t ctas
       out->eh = p.h;
       out->ert = p.rt;
       out->et = p.t;
+      out->end_first = first_run;
+      out->end_last = last_run;
     }
   }
   __syncthreads();
@@ -367,17 +373,19 @@ __device__ __forceinline__ uint8_t* out_row(const Args& a, const Joint& j, int r
   return a.o + j.b * a.o_seq + (j.h * a.group + row - tok * a.group) * a.o_head + tok * a.o_tok;
 }
 
-// Row by row: partial sums [RM][DP], a block takes 4 rows, a lane DP / 32 columns.
-template <int RM, int DP, int DT>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_rows_kernel(const __grid_constant__ Args a) {
+// Row by row, partial sums [RM][DP]: 4 rows of a unit by the WARPS warps of a block, a
+// lane taking DP / 32 columns.  Reads past L1: other CTAs of this kernel may have
+// written the partial results.
+template <int DP, int WARPS>
+struct JoinSmem {
+  float sums[WARPS][4][DP];
+  float tops[WARPS][4], totals[WARPS][4];
+};
+
+template <int RM, int DP, int DT, int WARPS>
+__device__ __noinline__ void join_four(const Args& a, Joint j, JoinSmem<DP, WARPS>* sm) {
   using E = Elem<DT>;
   constexpr int kCols = DP / 32;
-  __shared__ float sums[kJoinWarps][4][DP];
-  __shared__ float tops[kJoinWarps][4], totals[kJoinWarps][4];
-  b200attn::ptx::launch_dependents();
-  b200attn::ptx::grid_dependency_wait();
-  Joint j;
-  if (!joint_of(a, 4 * blockIdx.y, &j)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float top[4], total[4], acc[4][kCols];
 #pragma unroll
@@ -387,49 +395,87 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_rows_kernel(const __grid
 #pragma unroll
     for (int x = 0; x < kCols; ++x) acc[r][x] = 0.f;
   }
-  for (int c = j.runs.x + warp; c <= j.runs.y; c += kJoinWarps) {
+#pragma unroll 1
+  for (int c = j.runs.x + warp; c <= j.runs.y; c += WARPS) {
     const float* p = part_of<RM, DP>(a, j, c);
+    float v[4][kCols], m[4], l[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = min(j.row0 + r, j.rows - 1);
-      float v[kCols];
 #pragma unroll
-      for (int x = 0; x < kCols; ++x) v[x] = p[row * DP + lane + 32 * x];
-      const float m = p[RM * DP + row], l = p[RM * DP + RM + row];
-      const float now = fmaxf(top[r], m), base = now == -INFINITY ? 0.f : now;
-      const float keep = exp2f(top[r] - base), w = exp2f(m - base);
+      for (int x = 0; x < kCols; ++x) v[r][x] = __ldcg(p + row * DP + lane + 32 * x);
+      m[r] = __ldcg(p + RM * DP + row);
+      l[r] = __ldcg(p + RM * DP + RM + row);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float now = fmaxf(top[r], m[r]), base = now == -INFINITY ? 0.f : now;
+      const float keep = exp2f(top[r] - base), w = exp2f(m[r] - base);
       top[r] = now;
-      total[r] = total[r] * keep + w * l;
+      total[r] = total[r] * keep + w * l[r];
 #pragma unroll
-      for (int x = 0; x < kCols; ++x) acc[r][x] = acc[r][x] * keep + w * v[x];
+      for (int x = 0; x < kCols; ++x) acc[r][x] = acc[r][x] * keep + w * v[r][x];
     }
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     if (lane == 0) {
-      tops[warp][r] = top[r];
-      totals[warp][r] = total[r];
+      sm->tops[warp][r] = top[r];
+      sm->totals[warp][r] = total[r];
     }
 #pragma unroll
-    for (int x = 0; x < kCols; ++x) sums[warp][r][lane + 32 * x] = acc[r][x];
+    for (int x = 0; x < kCols; ++x) sm->sums[warp][r][lane + 32 * x] = acc[r][x];
   }
   __syncthreads();
-  for (int y = threadIdx.x; y < 4 * DP; y += 32 * kJoinWarps) {
+#pragma unroll 1
+  for (int y = threadIdx.x; y < 4 * DP; y += 32 * WARPS) {
     const int r = y / DP, col = y % DP;
     if (j.row0 + r >= j.rows || col >= a.head_dim) continue;
     float best = -INFINITY, sum = 0.f, all = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) best = fmaxf(best, tops[w][r]);
+    for (int w = 0; w < WARPS; ++w) best = fmaxf(best, sm->tops[w][r]);
     const float base = best == -INFINITY ? 0.f : best;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      const float f = exp2f(tops[w][r] - base);
-      sum += f * sums[w][r][col];
-      all += f * totals[w][r];
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = exp2f(sm->tops[w][r] - base);
+      sum += f * sm->sums[w][r][col];
+      all += f * sm->totals[w][r];
     }
     reinterpret_cast<typename E::T*>(out_row(a, j, j.row0 + r))[col] =
         E::round(all == 0.f ? 0.f * sum : sum / all);
   }
+  __syncthreads();
+}
+
+// WARPS as in the kernel that left the partial results: the same sums in the same order,
+// wherever they are joined.
+template <int RM, int DP, int DT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) join_rows_kernel(const __grid_constant__ Args a) {
+  __shared__ JoinSmem<DP, WARPS> sm;
+  b200attn::ptx::launch_dependents();
+  b200attn::ptx::grid_dependency_wait();
+  Joint j;
+  if (joint_of(a, 4 * blockIdx.y, &j)) join_four<RM, DP, DT, WARPS>(a, j, &sm);
+}
+
+// The same within the kernel that left the partial results: the last of a unit's runs to
+// arrive joins them all.  By all threads of a CTA, after it has written its own.
+template <int RM, int DP, int DT, int WARPS>
+__device__ __noinline__ void join_if_last(const Args& a, int b, int h, int rt, int rows, int first,
+                                          int last, JoinSmem<DP, WARPS>* sm) {
+  __threadfence();
+  __syncthreads();
+  int32_t* counter = &a.counters[(b * a.kv_heads + h) * a.row_tiles + rt];
+  bool mine = false;
+  if (threadIdx.x == 0) {
+    mine = atomicAdd(counter, 1) == last - first;
+    if (mine) *counter = 0;
+  }
+  if (!__syncthreads_or(mine)) return;
+  __threadfence();
+  Joint j{make_int2(first, last), 0, rows, b, h, rt};
+#pragma unroll 1
+  for (; j.row0 < rows; j.row0 += 4) join_four<RM, DP, DT, WARPS>(a, j, sm);
 }
 
 // Column by column: partial sums [DP][RM], a block takes 32 rows, a lane one of them,

@@ -103,7 +103,8 @@ struct RowShape {
   static constexpr int kOffMisc = kOffStat + 4 * 2 * kRowWarps * RM;
   static constexpr int kSmemBytes = kOffMisc + 256;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of a block");
-  using G = Grid<RM, kRowTile, 1>;
+  using G = Grid<RM, kRowTile, 2>;
+  static_assert(sizeof(JoinSmem<DP, kRowWarps>) <= 4 * kRowWarps * RM * kJoinPitch, "joins in place");
 };
 
 template <class S, int DT>
@@ -473,9 +474,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       part[RM * DP + r] = top;
       part[RM * DP + RM + r] = total;
     }
-    if (tid == 0 && last)
-      a.desc[unit_of(a, done)] =
-          make_int2(first ? static_cast<int>(blockIdx.x) : run.first_run, static_cast<int>(blockIdx.x));
+    if (!finish) {
+      const int from = run.ends_in(done) ? run.end_first : (first ? blockIdx.x : run.first_run);
+      const int to = run.ends_in(done) ? run.end_last : blockIdx.x;
+      if (a.counters)
+        join_if_last<RM, DP, DT, kRowWarps>(a, done.b, done.h, done.rt, rows, from, to,
+                                            reinterpret_cast<JoinSmem<DP, kRowWarps>*>(join));
+      else if (tid == 0 && last)
+        a.desc[unit_of(a, done)] = make_int2(from, to);
+    } else if (tid == 0 && !a.counters) {
+      a.desc[unit_of(a, done)] = make_int2(0, 0);
+    }
     if (again) store_q();  // the queries' fragments are in registers, or read between the barriers
     __syncthreads();
   }

@@ -30,7 +30,7 @@ struct PlainSmem {
   float v[kKeys][DP];
   float p[kRows][kKeys + 1];
   float m[kRows], l[kRows], alpha[kRows];
-  int page[kKeys];
+  bool live[kKeys];  // the key is there
   uint32_t sums[kThreads / 32];
   Run run;
 };
@@ -64,12 +64,16 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
       const int row = pl.rt * kRows + r;
       return base + pl.b * seq + (pl.h * a.group + row % a.group) * head + (row / a.group) * tok;
     };
-    for (int x = tid; x < kRows * DP; x += kThreads) sm.q[x / DP][x % DP] = 0.f;
-    __syncthreads();
-    for (int x = tid; x < rows * a.head_dim; x += kThreads) {
-      const int r = x / a.head_dim, c = x - r * a.head_dim;
-      const uint8_t* src = row_ptr(a.q, a.q_seq, a.q_head, a.q_tok, r);
-      sm.q[r][c] = E::widen(reinterpret_cast<const typename E::T*>(src)[c]) * a.scale_log2;
+#pragma unroll 4
+    for (int x = tid; x < kRows * (DP / kPer16); x += kThreads) {
+      const int r = x / (DP / kPer16), c = x % (DP / kPer16);
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows && c < pieces)
+        w = __ldg(reinterpret_cast<const uint4*>(row_ptr(a.q, a.q_seq, a.q_head, a.q_tok, r)) + c);
+#pragma unroll
+      for (int e = 0; e < kPer16; ++e)
+        sm.q[r][c * kPer16 + e] =
+            E::widen(reinterpret_cast<const typename E::T*>(&w)[e]) * a.scale_log2;
     }
     if (tid < kRows) {
       sm.m[tid] = -INFINITY;
@@ -80,39 +84,46 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
     for (int t = t0; t < t0 + n; ++t) {
       const int k0 = t * kKeys;
       __syncthreads();
-      if (tid < kKeys) {
-        const int key = k0 + tid;
-        int page = -1;
-        if (key < keys) {
-          page = a.table[pl.b * a.table_stride + key / a.page_size];
-          if (page < 0 || page >= a.pages) {
-            report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
-            page = -1;
-          }
-        }
-        sm.page[tid] = page;
-      }
-      __syncthreads();
-      for (int x = tid; x < kKeys * (DP / kPer16); x += kThreads) {
-        const int key = x / (DP / kPer16), c = x % (DP / kPer16);
-        const int page = sm.page[key];
-        float kv[kPer16] = {}, vv[kPer16] = {};
-        if (page >= 0 && c < pieces) {
-          const int64_t row = (k0 + key) % a.page_size;
-          const uint4 kw = *reinterpret_cast<const uint4*>(a.k + page * a.k_page + pl.h * a.k_head +
-                                                           row * a.k_row + 16 * c);
-          const uint4 vw = *reinterpret_cast<const uint4*>(a.v + page * a.v_page + pl.h * a.v_head +
-                                                           row * a.v_row + 16 * c);
+      // keys and values, a thread 4 pieces of 16 bytes of each at a time: page numbers,
+      // then rows, are all read before any is used
+      constexpr int kRowPieces = DP / kPer16, kBatch = 4;
+#pragma unroll 1
+      for (int x0 = tid; x0 < kKeys * kRowPieces; x0 += kBatch * kThreads) {
+        int page[kBatch];
+        uint4 kw[kBatch], vw[kBatch];
 #pragma unroll
-          for (int u = 0; u < kPer16; ++u) {
-            kv[u] = E::widen(reinterpret_cast<const typename E::T*>(&kw)[u]);
-            vv[u] = E::widen(reinterpret_cast<const typename E::T*>(&vw)[u]);
+        for (int u = 0; u < kBatch; ++u) {
+          const int key = (x0 + u * kThreads) / kRowPieces;
+          page[u] = -1;
+          if (k0 + key < keys) {
+            page[u] = __ldg(a.table + pl.b * a.table_stride + (k0 + key) / a.page_size);
+            if (page[u] < 0 || page[u] >= a.pages) {
+              report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
+              page[u] = -1;
+            }
           }
         }
 #pragma unroll
-        for (int u = 0; u < kPer16; ++u) {
-          sm.k[key][c * kPer16 + u] = kv[u];
-          sm.v[key][c * kPer16 + u] = vv[u];
+        for (int u = 0; u < kBatch; ++u) {
+          const int x = x0 + u * kThreads, key = x / kRowPieces, c = x % kRowPieces;
+          kw[u] = vw[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (page[u] >= 0 && c < pieces) {
+            const int64_t row = (k0 + key) % a.page_size;
+            kw[u] = *reinterpret_cast<const uint4*>(a.k + page[u] * a.k_page + pl.h * a.k_head +
+                                                    row * a.k_row + 16 * c);
+            vw[u] = *reinterpret_cast<const uint4*>(a.v + page[u] * a.v_page + pl.h * a.v_head +
+                                                    row * a.v_row + 16 * c);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int x = x0 + u * kThreads, key = x / kRowPieces, c = x % kRowPieces;
+          if (c == 0) sm.live[key] = page[u] >= 0;
+#pragma unroll
+          for (int e = 0; e < kPer16; ++e) {
+            sm.k[key][c * kPer16 + e] = E::widen(reinterpret_cast<const typename E::T*>(&kw[u])[e]);
+            sm.v[key][c * kPer16 + e] = E::widen(reinterpret_cast<const typename E::T*>(&vw[u])[e]);
+          }
         }
       }
       __syncthreads();
@@ -131,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
 #pragma unroll
         for (int r = 0; r < kRows / 2; ++r) {
           const int i = (pl.rt * kRows + r0 + r) / a.group;
-          const bool shown = r0 + r < rows && sm.page[key] >= 0 &&
+          const bool shown = r0 + r < rows && sm.live[key] &&
                              (j < 0 || (j < pl.s.drafts && sees(a, pl.b, i, j)));
           sm.p[r0 + r][key] = shown ? s[r] : -INFINITY;
         }

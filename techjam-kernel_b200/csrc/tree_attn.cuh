@@ -147,7 +147,52 @@ struct Run {
   }
 };
 
-// Finds this CTA's run.  Every thread counts the places of its share of the
+// Run boundaries: `more` runs of q + 1 places, then runs of q; none is empty of places.
+struct Cuts {
+  uint32_t total, runs, q, more;
+  __device__ Cuts(uint32_t places, uint32_t ctas) : total(places), runs(min(places, ctas)) {
+    q = runs ? total / runs : 0u;
+    more = total - q * runs;
+  }
+  __device__ uint32_t begin(uint32_t c) const { return c < runs ? c * q + min(c, more) : total; }
+  __device__ int owner(uint32_t place) const {
+    const uint32_t head = more * (q + 1);
+    return static_cast<int>(place < head ? place / (q + 1) : more + (place - head) / q);
+  }
+};
+
+// Writes the run's first (end = false) or one-past-last place `at`, which lies `left`
+// places into the work of sequence b.
+template <class G>
+__device__ __forceinline__ void put_place(const Args& a, const Cuts& cuts, bool end, int b,
+                                          const Seq& s, uint32_t at, uint32_t left, Run* out) {
+  Place p{b, 0, 0, 0, 0, 0, s};
+  int first_run = 0, last_run = 0;
+  if (b < a.batch) {
+    p.tiles = G::key_tiles(s);
+    p.rts = G::row_tiles(a, s);
+    const uint32_t span = p.tiles + G::EX, u = left / span, x = left - u * span;
+    p.t = x > G::EX ? static_cast<int>(x - G::EX) : 0;
+    p.h = static_cast<int>(u) / p.rts;
+    p.rt = static_cast<int>(u) - p.h * p.rts;
+    // the runs that the unit's first and last tile lie in
+    first_run = cuts.owner(at - x + G::EX);
+    last_run = cuts.owner(at - x + span - 1);
+  }
+  if (!end) {
+    out->p = p;
+    out->first_run = first_run;
+  } else {
+    out->eb = p.b;
+    out->eh = p.h;
+    out->ert = p.rt;
+    out->et = p.t;
+    out->end_first = first_run;
+    out->end_last = last_run;
+  }
+}
+
+// find_run: this CTA's run.  Every thread counts the places of its share of the
 // sequences, a scan finds the total, and the threads whose shares hold the run's
 // first place and the next run's walk to them.  `sums`: scratch of one value a warp.
 // Ends with a barrier; *out is in shared memory.
@@ -155,67 +200,56 @@ template <class G>
 __device__ __noinline__ void find_run(const Args& a, uint32_t run, uint32_t ctas, uint32_t* sums,
                                       Run* out) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
-  const int each = (a.batch + nt - 1) / nt;
+  const bool one = a.batch <= 32;  // a lane a sequence: one warp finds the run by itself
+  if (one && warp > 0) {
+    __syncthreads();
+    return;
+  }
+  const int each = one ? 1 : (a.batch + nt - 1) / nt;
   const int b0 = min(a.batch, tid * each), b1 = min(a.batch, b0 + each);
   uint32_t mine = 0;
+  Seq s{0, 0};
 #pragma unroll 1
-  for (int b = b0; b < b1; ++b) mine += G::places(a, seq_of(a, b));
+  for (int b = b0; b < b1; ++b) {
+    s = seq_of(a, b);
+    mine += G::places(a, s);
+  }
   uint32_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += t;
   }
-  if (lane == 31) sums[warp] = incl;
-  __syncthreads();
-  uint32_t before = incl - mine, total = 0;
+  uint32_t before = incl - mine, total = __shfl_sync(0xffffffffu, incl, 31);
+  if (!one) {
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    total = 0;
 #pragma unroll 1
-  for (int w = 0; w < nt >> 5; ++w) {
-    if (w < warp) before += sums[w];
-    total += sums[w];
+    for (int w = 0; w < nt >> 5; ++w) {
+      if (w < warp) before += sums[w];
+      total += sums[w];
+    }
   }
-  // `more` runs of q + 1 places, then runs of q: none is empty of places
-  const uint32_t runs = min(total, ctas), q = runs ? total / runs : 0u, more = total - q * runs;
+  const Cuts cuts(total, ctas);
 #pragma unroll 1
   for (uint32_t end = 0; end < 2; ++end) {
-    const uint32_t c = run + end;
-    const uint32_t at = c < runs ? c * q + min(c, more) : total;
-    Place p{a.batch, 0, 0, 0, 0, 0, {0, 0}};
-    int first_run = 0, last_run = 0;
+    const uint32_t at = cuts.begin(run + end);
     if (at == total) {
-      if (tid != 0) continue;
-    } else {
-      if (at < before || at >= before + mine) continue;
+      if (tid == 0) put_place<G>(a, cuts, end, a.batch, Seq{0, 0}, 0, 0, out);
+    } else if (at >= before && at < before + mine) {
       uint32_t left = at - before;
+      int b = b0;
+      if (each > 1) {
 #pragma unroll 1
-      for (p.b = b0; p.b < b1; ++p.b) {
-        p.s = seq_of(a, p.b);
-        const uint32_t all = G::places(a, p.s);
-        if (left < all) break;
-        left -= all;
+        for (; b < b1; ++b) {
+          s = seq_of(a, b);
+          const uint32_t all = G::places(a, s);
+          if (left < all) break;
+          left -= all;
+        }
       }
-      p.tiles = G::key_tiles(p.s);
-      p.rts = G::row_tiles(a, p.s);
-      const uint32_t span = p.tiles + G::EX, u = left / span, x = left - u * span;
-      p.t = x > G::EX ? static_cast<int>(x - G::EX) : 0;
-      p.h = static_cast<int>(u) / p.rts;
-      p.rt = static_cast<int>(u) - p.h * p.rts;
-      // the runs that the unit's first and last tile lie in
-      const uint32_t long_runs = more * (q + 1);
-      const uint32_t head = at - x + G::EX, tail = at - x + span - 1;
-      first_run = static_cast<int>(head < long_runs ? head / (q + 1) : more + (head - long_runs) / q);
-      last_run = static_cast<int>(tail < long_runs ? tail / (q + 1) : more + (tail - long_runs) / q);
-    }
-    if (end == 0) {
-      out->p = p;
-      out->first_run = first_run;
-    } else {
-      out->eb = p.b;
-      out->eh = p.h;
-      out->ert = p.rt;
-      out->et = p.t;
-      out->end_first = first_run;
-      out->end_last = last_run;
+      put_place<G>(a, cuts, end, b, s, at, left, out);
     }
   }
   __syncthreads();

@@ -12,6 +12,8 @@
 // warps of this one join their results in shared memory.
 #pragma once
 
+#include <type_traits>
+
 #include "tree_attn.cuh"
 
 namespace b200tree {
@@ -418,61 +420,74 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
         scale[i][hh] = top == -INFINITY ? 0.f : b200attn::ptx::ex2_approx(m[i][hh] - top);
       }
     const int rows = min(RM, done.s.drafts * a.group - done.rt * RM);
-    // thread -> one row and kEach columns of the columns at hand
-    constexpr int kEach = RM * S::kCols / kRowThreads;
-    static_assert(kEach == 2, "two columns a thread");
-    const int r = tid / (S::kCols / kEach), c = (tid % (S::kCols / kEach)) * kEach;
-    float top = -INFINITY, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, stat[2 * w * RM + r]);
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) {
-      const float mw = stat[2 * w * RM + r];
-      if (mw != -INFINITY)
-        total += stat[(2 * w + 1) * RM + r] * b200attn::ptx::ex2_approx(mw - top);
-    }
     float* part = a.partial + static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * (RM * (DP + 2));
     const bool finish = first && last;
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    const int row = done.rt * RM + r, tok = row / a.group;
-    uint8_t* out = a.o + done.b * a.o_seq + (done.h * a.group + row - tok * a.group) * a.o_head +
-                   tok * a.o_tok;
+    // The warps' sums go through shared memory, `cols` columns at a time; a thread adds two
+    // columns of a row.  Up to 8 rows (a token of 8 query heads): twice the columns of half
+    // the rows.
+    auto join_columns = [&](auto row_count, auto col_count) {
+      constexpr int kR = decltype(row_count)::value, kC = decltype(col_count)::value;
+      constexpr int kPitch = kC + 4;
+      static_assert(kR * kC == 2 * kRowThreads, "two columns a thread");
+      static_assert(kR * kPitch <= RM * S::kJoinPitch, "in place");
+      const int r = tid / (kC / 2), c = (tid % (kC / 2)) * 2;
+      float top = -INFINITY, total = 0.f;
 #pragma unroll
-    for (int c0 = 0; c0 < DP; c0 += S::kCols) {
-      if (c0) __syncthreads();
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int x = 0; x < S::kCols / 8; ++x) {
-          float* d = join + (warp * RM + 16 * i + g) * S::kJoinPitch + 8 * x + t2;
-          const float* src = o[i][c0 / 8 + x];
-          *reinterpret_cast<float2*>(d) = make_float2(src[0] * scale[i][0], src[1] * scale[i][0]);
-          *reinterpret_cast<float2*>(d + 8 * S::kJoinPitch) =
-              make_float2(src[2] * scale[i][1], src[3] * scale[i][1]);
-        }
-      __syncthreads();
-      float2 acc = make_float2(0.f, 0.f);
+      for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, stat[2 * w * RM + r]);
 #pragma unroll
       for (int w = 0; w < kRowWarps; ++w) {
-        const float2 v = *reinterpret_cast<const float2*>(join + (w * RM + r) * S::kJoinPitch + c);
-        acc.x += v.x;
-        acc.y += v.y;
+        const float mw = stat[2 * w * RM + r];
+        if (mw != -INFINITY)
+          total += stat[(2 * w + 1) * RM + r] * b200attn::ptx::ex2_approx(mw - top);
       }
-      if (finish) {
-        if (r < rows && c0 + c < a.head_dim)
-          *reinterpret_cast<uint32_t*>(out + 2 * (c0 + c)) = pack_pair<DT>(acc.x * inv, acc.y * inv);
-      } else {
-        *reinterpret_cast<float2*>(part + r * DP + c0 + c) = acc;
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      const int row = done.rt * RM + r, tok = row / a.group;
+      uint8_t* out = a.o + done.b * a.o_seq + (done.h * a.group + row - tok * a.group) * a.o_head +
+                     tok * a.o_tok;
+#pragma unroll
+      for (int c0 = 0; c0 < DP; c0 += kC) {
+        if (c0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < (kR > 16 ? MT : 1); ++i)
+#pragma unroll
+          for (int x = 0; x < kC / 8; ++x) {
+            float* d = join + (warp * kR + 16 * i + g) * kPitch + 8 * x + t2;
+            const float* src = o[i][c0 / 8 + x];
+            *reinterpret_cast<float2*>(d) = make_float2(src[0] * scale[i][0], src[1] * scale[i][0]);
+            if (kR > 8)
+              *reinterpret_cast<float2*>(d + 8 * kPitch) =
+                  make_float2(src[2] * scale[i][1], src[3] * scale[i][1]);
+          }
+        __syncthreads();
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) {
+          const float2 v = *reinterpret_cast<const float2*>(join + (w * kR + r) * kPitch + c);
+          acc.x += v.x;
+          acc.y += v.y;
+        }
+        if (finish) {
+          if (r < rows && c0 + c < a.head_dim)
+            *reinterpret_cast<uint32_t*>(out + 2 * (c0 + c)) = pack_pair<DT>(acc.x * inv, acc.y * inv);
+        } else {
+          *reinterpret_cast<float2*>(part + r * DP + c0 + c) = acc;
+        }
       }
-    }
-    if (any_odd && r < rows)
-      for (int c0 = c; c0 < DP; c0 += S::kCols)
-        add_odd<DT>(a, done.b, done.h, done.s, tok, t0 * kRowTile - done.s.len,
-                    (t0 + n) * kRowTile - done.s.len, c0, min(a.head_dim, c0 + kEach),
-                    finish ? reinterpret_cast<uint16_t*>(out) : nullptr, part + r * DP, 1);
-    if (!finish && c == 0) {
-      part[RM * DP + r] = top;
-      part[RM * DP + RM + r] = total;
+      if (any_odd && r < rows)
+        for (int c0 = c; c0 < DP; c0 += kC)
+          add_odd<DT>(a, done.b, done.h, done.s, tok, t0 * kRowTile - done.s.len,
+                      (t0 + n) * kRowTile - done.s.len, c0, min(a.head_dim, c0 + 2),
+                      finish ? reinterpret_cast<uint16_t*>(out) : nullptr, part + r * DP, 1);
+      if (!finish && c == 0) {
+        part[RM * DP + r] = top;
+        part[RM * DP + RM + r] = total;
+      }
+    };
+    if (MT == 1 && rows <= 8) {
+      if constexpr (MT == 1)
+        join_columns(std::integral_constant<int, 8>{}, std::integral_constant<int, 64>{});
+    } else {
+      join_columns(std::integral_constant<int, RM>{}, std::integral_constant<int, S::kCols>{});
     }
     if (!finish) {
       const int from = run.ends_in(done) ? run.end_first : (first ? blockIdx.x : run.first_run);

@@ -34,6 +34,7 @@ from .attention_dispatch import (AttentionMode, AttentionModelSpec, AttentionRun
                                  select_attention_stack_plan)
 from .fused_attention import b200_fused_attention
 from .linear import b200_linear, linear_supported
+from .paged_cache import PagedKVCache
 
 _DTYPE_NAMES = {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32"}
 
@@ -139,6 +140,23 @@ class B200FusedSelfAttention(nn.Module):
         context = b200_fused_attention(q, k, v, valid_token_mask, causal, self.scale,
                                        output_bshd=True)
         return context.view(batch, seq_len, self.d_model)
+
+    def cached_context(self, x: torch.Tensor, cache: PagedKVCache, layer: int,
+                       tree_mask: Optional[torch.Tensor] = None,
+                       draft_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention context [B, T, d] of drafted tokens ``x`` over ``cache``, before
+        ``out_proj``: their keys and values are written behind the committed tokens of
+        ``layer`` (whose pages ``cache.reserve`` has provided), and each sees the committed
+        tokens and those drafted ones that ``tree_mask`` shows it (without it, those up
+        to itself).  Inference only."""
+        batch, tokens, _ = x.shape
+        weight, bias = self._stacked_qkv()
+        qkv = torch.nn.functional.linear(x, weight, bias).view(
+            batch, tokens, 3, self.num_heads, self.head_dim)
+        q, k, v = (qkv[:, :, t].transpose(1, 2) for t in range(3))
+        cache.append(layer, k, v, draft_lens)
+        context = cache.attend(layer, q, tree_mask, draft_lens, self.scale, output_bshd=True)
+        return context.view(batch, tokens, self.d_model)
 
     def _plan_mode(self, x: torch.Tensor, causal: bool) -> AttentionMode:
         needs_autograd = torch.is_grad_enabled() and (

@@ -26,6 +26,9 @@ An optional
 token embedding in front serves the end-to-end configuration (vocabulary 32000,
 uniform random token ids); the reference model itself starts from hidden
 states, so parity is defined from the hidden states onward.
+
+``Decoder.cached_forward`` answers token by token over a paged key/value cache
+(``PagedKVCache``): a prompt, the next token, or a tree of drafted tokens.
 """
 
 from __future__ import annotations
@@ -41,6 +44,7 @@ from .attention_dispatch import AttentionModelSpec
 from .layernorm import b200_add_layer_norm, b200_layer_norm, layer_norm_supported
 from .linear import b200_linear, linear_supported
 from .modules import B200FusedSelfAttention
+from .paged_cache import PagedKVCache
 
 
 @dataclass(frozen=True)
@@ -121,6 +125,23 @@ class DecoderBlock(nn.Module):
         return b200_linear(g, self.ffn_out.weight, self.ffn_out.bias, residual=x1,
                            row_mask=valid_token_mask, masked_rows="zero"), None
 
+    def cached_forward(self, x: torch.Tensor, cache: PagedKVCache, layer: int,
+                       tree_mask: Optional[torch.Tensor] = None,
+                       draft_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The block over drafted tokens [B, T, d] whose context lies in ``cache``
+        (``B200FusedSelfAttention.cached_context``)."""
+        if self._fusable(x):
+            h = b200_layer_norm(x, self.norm1.weight, self.norm1.bias, self.norm1.eps)
+            context = self.attention.cached_context(h, cache, layer, tree_mask, draft_lens)
+            out = self.attention.out_proj
+            x = b200_linear(context, out.weight, out.bias, residual=x)
+            h = b200_layer_norm(x, self.norm2.weight, self.norm2.bias, self.norm2.eps)
+            h = b200_linear(h, self.ffn_in.weight, self.ffn_in.bias, activation="gelu")
+            return b200_linear(h, self.ffn_out.weight, self.ffn_out.bias, residual=x)
+        context = self.attention.cached_context(self.norm1(x), cache, layer, tree_mask, draft_lens)
+        x = x + self.attention.out_proj(context)
+        return x + self.ffn_out(F.gelu(self.ffn_in(self.norm2(x)), approximate="none"))
+
     def _fusable(self, x: torch.Tensor) -> bool:
         """The block's LayerNorms and linear layers fit the fused kernels for
         input ``x`` (inference on 16-bit CUDA tensors, sizes multiples of 8)."""
@@ -170,6 +191,35 @@ class Decoder(nn.Module):
         if valid_token_mask is not None:
             x = x.masked_fill(~valid_token_mask[..., None], 0)
         return x
+
+    def new_cache(self, batch: int, max_tokens: int, page_size: int = 64,
+                  pages: Optional[int] = None) -> PagedKVCache:
+        """An empty paged cache for ``batch`` sequences of up to ``max_tokens`` committed
+        and drafted tokens (``pages`` in the pool; by default enough for all of them)."""
+        slots = -(-max_tokens // page_size)
+        weight = self.final_norm.weight
+        return PagedKVCache(self.config.num_layers, pages if pages is not None else batch * slots,
+                            self.config.num_heads, page_size,
+                            self.config.d_model // self.config.num_heads, batch, slots,
+                            dtype=weight.dtype, device=weight.device)
+
+    def cached_forward(self, x: torch.Tensor, cache: PagedKVCache,
+                       tree_mask: Optional[torch.Tensor] = None,
+                       draft_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Final hidden states [B, T, d] of drafted tokens ``x`` (hidden states, or token ids
+        [B, T]): a prompt (a chain), the next token, or a tree of drafted tokens.  A step is
+        ``cache.reserve(T)``, this call, and ``cache.accept(paths, counts)`` for the tokens
+        that are kept.  Causal models only; inference only."""
+        if not self.config.causal:
+            raise ValueError("a cache serves causal models only")
+        if self.embed is not None and not torch.is_floating_point(x):
+            x = self.embed(x)
+        for i, layer in enumerate(self.layers):
+            x = layer.cached_forward(x, cache, i, tree_mask, draft_lens)
+        fn = self.final_norm
+        if x.dtype != torch.float32 and layer_norm_supported(x, fn.weight):
+            return b200_layer_norm(x, fn.weight, fn.bias, fn.eps)
+        return fn(x)
 
     def _forward_layers(self, x, valid_token_mask):
         for layer in self.layers:

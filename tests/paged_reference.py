@@ -42,11 +42,13 @@ def attention64(q, k_pages, v_pages, table, lens, mask=None, drafts=None, scale=
 def attention_bound(dtype, out, size, grow, head_dim, keys):
     """How far the kernels' output may be from the 64-bit one, element by element.
 
-    With u half a unit in the last place of the type and w = 2^-24: a score is a
-    sum of head_dim products, off by at most head_dim w grow, so a weight by that
-    and a few w for the exponential; normalising doubles it.  16-bit weights are
-    rounded once (u each, and as much in their sum).  Sums over the keys add keys
-    w.  The output is rounded once (half a smallest subnormal at least)."""
+    With 2u the largest relative error of one rounding to the type, and w = 2^-24: a
+    score is a sum of head_dim products, off by at most head_dim w grow, so a weight by
+    that and a few w for the exponential; normalising doubles it.  Sums over the keys add
+    keys w.  16-bit weights are rounded, so is the output: 3u of the size of the sum in
+    all, which is one and a half times the largest error of one rounding (the
+    weights' errors are independent, and do not all point one way).  Half a smallest
+    subnormal at least."""
     u = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12, torch.float32: 2.0 ** -24}[dtype]
     tiny = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -24, torch.float32: 0.0}[dtype]
     w = 2.0 ** -24

@@ -129,6 +129,39 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   const uint32_t size = static_cast<uint32_t>(a.page_size);
   const bool whole = a.page_size % kRowKeys == 0;  // a block lies in one page
 
+  // ------------------------------------------------------------- queries
+  constexpr int kQPieces = RM * S::kPieces / kRowThreads > 0 ? RM * S::kPieces / kRowThreads : 1;
+  uint4 qreg[kQPieces];
+  auto fetch_q = [&](const Place& p) {
+    const int rows = min(RM, p.s.drafts * a.group - p.rt * RM);
+#pragma unroll
+    for (int u = 0; u < kQPieces; ++u) {
+      const int x = tid + u * kRowThreads;
+      const int r = x / S::kPieces, piece = x % S::kPieces;
+      qreg[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows && piece < pieces) {
+        const int row = p.rt * RM + r, i = row / a.group;
+        qreg[u] = *reinterpret_cast<const uint4*>(
+            a.q + p.b * a.q_seq + (p.h * a.group + row - i * a.group) * a.q_head + i * a.q_tok +
+            16 * piece);
+      }
+    }
+  };
+  auto store_q = [&]() {
+#pragma unroll
+    for (int u = 0; u < kQPieces; ++u) {
+      const int x = tid + u * kRowThreads;
+      const int r = x / S::kPieces, piece = x % S::kPieces;
+      if (r < RM)
+        *reinterpret_cast<uint4*>(smem + S::kOffQ + r * S::kRowBytes + ((piece ^ (r & 7)) << 4)) =
+            qreg[u];
+    }
+  };
+
+  Place pl = run.p;
+  const bool any = !run.done(pl);
+  if (any) fetch_q(pl);
+
   // ------------------------------------------------------------- loads
   // The place of the next tile to load; its page numbers are read one tile ahead.
   Place ld = run.p;
@@ -182,42 +215,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   };
 #pragma unroll 1
   for (int s = 0; s < NS - 1; ++s) issue();
-  zero_unused_rows(a, 2, kRowThreads);
 
-  // ------------------------------------------------------------- queries
-  constexpr int kQPieces = RM * S::kPieces / kRowThreads > 0 ? RM * S::kPieces / kRowThreads : 1;
-  uint4 qreg[kQPieces];
-  auto fetch_q = [&](const Place& p) {
-    const int rows = min(RM, p.s.drafts * a.group - p.rt * RM);
-#pragma unroll
-    for (int u = 0; u < kQPieces; ++u) {
-      const int x = tid + u * kRowThreads;
-      const int r = x / S::kPieces, piece = x % S::kPieces;
-      qreg[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows && piece < pieces) {
-        const int row = p.rt * RM + r, i = row / a.group;
-        qreg[u] = *reinterpret_cast<const uint4*>(
-            a.q + p.b * a.q_seq + (p.h * a.group + row - i * a.group) * a.q_head + i * a.q_tok +
-            16 * piece);
-      }
-    }
-  };
-  auto store_q = [&]() {
-#pragma unroll
-    for (int u = 0; u < kQPieces; ++u) {
-      const int x = tid + u * kRowThreads;
-      const int r = x / S::kPieces, piece = x % S::kPieces;
-      if (r < RM)
-        *reinterpret_cast<uint4*>(smem + S::kOffQ + r * S::kRowBytes + ((piece ^ (r & 7)) << 4)) =
-            qreg[u];
-    }
-  };
-
-  Place pl = run.p;
-  if (!run.done(pl)) {
-    fetch_q(pl);
-    store_q();
-  }
+  if (any) store_q();
   __syncthreads();
   int use = 0;  // stage of the tile at hand
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // row and column pair of this lane in a product
@@ -503,6 +502,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
     if (again) store_q();  // the queries' fragments are in registers, or read between the barriers
     __syncthreads();
   }
+  zero_unused_rows(a, 2, kRowThreads);
 }
 
 }  // namespace b200tree

@@ -223,7 +223,9 @@ struct Scratch {
 
 // ------------------------------------------------------------------- moves
 // Warps take (move, layer, K or V, head) segments in turn; a segment's rows are
-// contiguous pieces of 16 bytes, and a lane keeps kUnroll of them in flight.
+// contiguous pieces of 16 bytes, and a lane keeps kUnroll of them in flight.  Stored as
+// streaming: nothing reads the rows soon (copies of 224 part-filled pages in 32 layers,
+// 451 MB: 74 us against 87 us with plain stores; 8 pieces in flight 100 us, 2: 95 us).
 constexpr int kUnroll = 4;
 
 // By warp `warp` of `warps`.
@@ -258,7 +260,7 @@ __device__ __forceinline__ void move_rows(const Pool& c, const Scratch& w, int c
       }
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
-        if (x0 + 32 * u < pieces) *reinterpret_cast<uint4*>(dst + off[u]) = a[u];
+        if (x0 + 32 * u < pieces) __stcs(reinterpret_cast<uint4*>(dst + off[u]), a[u]);
     }
   }
 }

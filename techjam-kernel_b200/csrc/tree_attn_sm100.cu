@@ -75,7 +75,7 @@ struct TileShape {
   static constexpr int kOffBar = kOffSeen + 2 * 8 * kSeen;
   static_assert(sizeof(Place) == 32, "eight numbers");
   static_assert(sizeof(Run) <= 64, "a run's place");
-  using G = Grid<RM, kTile, 2>;
+  using G = Grid<RM, kTile, 4>;
   static constexpr int kBarQ = 0, kBarQRead = 1, kBarSeen = 2, kBarFull = 3, kBarEmpty = kBarFull + kSlots,
                        kBarScores = kBarEmpty + kSlots, kBarRead = kBarScores + 2,
                        kBarWeights = kBarRead + 2, kBarSums = kBarWeights + 2,

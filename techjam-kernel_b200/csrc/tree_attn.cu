@@ -338,10 +338,13 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
                              s);
     return rc != B200_ATTN_OK || a.counters ? rc : run_join_rows<kRows, DP, DT, kThreads / 32>(a, units, s);
   } else {
-    using One = RowShape<1, DP>;
-    using Two = RowShape<2, DP>;
+    using Few = RowShape<1, true, DP>;
+    using One = RowShape<1, false, DP>;
+    using Two = RowShape<2, false, DP>;
     if (c.kernel == kManyRows)
       rc = launch_tiles(c.rm, c.dp, DT, a, a.kv_heads * a.group, runs, device, s);
+    else if (a.tokens * a.group <= 8)
+      rc = run_one<8, DP, DT>(rows_kernel<Few, DT>, kRowThreads, Few::kSmemBytes, a, runs, device, s);
     else if (c.rm == 16)
       rc = run_one<16, DP, DT>(rows_kernel<One, DT>, kRowThreads, One::kSmemBytes, a, runs, device,
                                s);

@@ -88,10 +88,14 @@ __device__ __forceinline__ uint32_t non_finite(uint32_t w) {
   return __vcmpeq2(w & kExp, kExp);
 }
 
-// Shape of an instance: MT row tiles of 16, head dim padded to DP.
-template <int MT_, int DP_>
+// Shape of an instance: MT row tiles of 16 (FEW: up to 8 rows of one tile, whose other half
+// is left out of the softmax), head dim padded to DP.
+template <int MT_, bool FEW_, int DP_>
 struct RowShape {
   static constexpr int MT = MT_, DP = DP_, RM = 16 * MT_;
+  static constexpr bool FEW = FEW_;
+  static constexpr int kHalves = FEW ? 1 : 2;  // halves of 8 rows of a tile
+  static_assert(!FEW || MT == 1, "up to 8 rows");
   static constexpr int kRowBytes = 2 * DP;
   static constexpr int kPieces = kRowBytes / 16;
   static constexpr int kBlockBytes = kRowKeys * kRowBytes;     // one warp's keys or values
@@ -180,6 +184,15 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   };
   if (more) look_up();
   int stage = 0;  // stage the next loads go to
+  constexpr int kRowsAt = 32 / S::kPieces;  // rows a warp loads at a time
+  constexpr int kPlaces = 8 / kRowsAt;
+  const int piece = lane % S::kPieces, r0 = lane / S::kPieces;
+  uint32_t place[kPlaces];  // of this lane's piece in its rows among 8
+#pragma unroll
+  for (int i = 0; i < kPlaces; ++i) {
+    const int r = r0 + i * kRowsAt;
+    place[i] = r * S::kRowBytes + ((piece ^ r) << 4);
+  }
   auto issue = [&]() {
     if (more) {
       if (page >= a.pages || (page < 0 && (whole ? 0 : (lane & 15)) < ld_keys)) {
@@ -188,9 +201,22 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       }
       const uint32_t dst = ring + stage * (2 * S::kBlockBytes);
       const int64_t head_k = ld.h * a.k_head, head_v = ld.h * a.v_head;
-      constexpr int kRowsAt = 32 / S::kPieces;  // rows a warp loads at a time
-      const int piece = lane % S::kPieces, r0 = lane / S::kPieces;
+      if (whole && page >= 0 && ld_keys >= kRowKeys && a.head_dim == DP) {
+        // a whole block of one page
+        const int64_t at = page_row + r0;
+        const uint8_t* ks = a.k + page * a.k_page + head_k + at * a.k_row + 16 * piece;
+        const uint8_t* vs = a.v + page * a.v_page + head_v + at * a.v_row + 16 * piece;
 #pragma unroll
+        for (int i = 0; i < kRowKeys / kRowsAt; ++i) {
+          // rows 8 apart have the same swizzle
+          const uint32_t off = dst + place[i % kPlaces] + (i / kPlaces) * (8 * S::kRowBytes);
+          cp_async16(off, ks, 16u);
+          cp_async16(off + S::kBlockBytes, vs, 16u);
+          ks += kRowsAt * a.k_row;
+          vs += kRowsAt * a.v_row;
+        }
+      } else
+#pragma unroll 1
       for (int i = 0; i < kRowKeys / kRowsAt; ++i) {
         const int r = r0 + i * kRowsAt;
         const int pg = whole ? page : __shfl_sync(0xffffffffu, page, r);
@@ -257,18 +283,21 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       const int k0 = t * kRowTile + warp * kRowKeys;
       if (k0 < keys) {
         float s[MT][2][4];
+        float s2[2][4];  // one row tile: the odd steps' sums, for shorter chains of products
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int x = 0; x < 2; ++x) {
+          s2[x][0] = s2[x][1] = s2[x][2] = s2[x][3] = 0.f;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) s[i][x][0] = s[i][x][1] = s[i][x][2] = s[i][x][3] = 0.f;
+          for (int i = 0; i < MT; ++i) s[i][x][0] = s[i][x][1] = s[i][x][2] = s[i][x][3] = 0.f;
+        }
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           uint32_t b[4];
           const int r = (mat >> 1) * 8 + mrow;
           ldmatrix_x4(b, kb + r * S::kRowBytes + (((2 * kk + (mat & 1)) ^ (r & 7)) << 4));
           if constexpr (MT == 1) {
-            mma16816<DT>(s[0][0], qf[kk], b[0], b[1]);
-            mma16816<DT>(s[0][1], qf[kk], b[2], b[3]);
+            mma16816<DT>(kk & 1 ? s2[0] : s[0][0], qf[kk], b[0], b[1]);
+            mma16816<DT>(kk & 1 ? s2[1] : s[0][1], qf[kk], b[2], b[3]);
           } else {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -279,12 +308,18 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
             }
           }
         }
+        if constexpr (MT == 1) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 2 * S::kHalves; ++e) s[0][x][e] += s2[x][e];
+        }
         if (k0 + kRowKeys > pl.s.len) {
           // drafted tokens, or past the last key
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 2 * S::kHalves; ++e) {
               const int row = pl.rt * RM + 16 * i + g + (e >> 1) * 8;
               const int tok = min(row / a.group, a.tokens - 1);
 #pragma unroll
@@ -328,7 +363,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
+          for (int hh = 0; hh < S::kHalves; ++hh) {
             float top = fmaxf(fmaxf(s[i][0][2 * hh], s[i][0][2 * hh + 1]),
                               fmaxf(s[i][1][2 * hh], s[i][1][2 * hh + 1]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -341,35 +376,39 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
-            l[i][0] *= alpha[i][0];
-            l[i][1] *= alpha[i][1];
 #pragma unroll
-            for (int x = 0; x < DP / 8; ++x) {
-              o[i][x][0] *= alpha[i][0];
-              o[i][x][1] *= alpha[i][0];
-              o[i][x][2] *= alpha[i][1];
-              o[i][x][3] *= alpha[i][1];
+            for (int hh = 0; hh < S::kHalves; ++hh) {
+              l[i][hh] *= alpha[i][hh];
+#pragma unroll
+              for (int x = 0; x < DP / 8; ++x) {
+                o[i][x][2 * hh] *= alpha[i][hh];
+                o[i][x][2 * hh + 1] *= alpha[i][hh];
+              }
             }
           }
         }
         uint32_t pf[MT][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const float b0 = m[i][0] == -INFINITY ? 0.f : m[i][0];
-          const float b1 = m[i][1] == -INFINITY ? 0.f : m[i][1];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float p0 = b200attn::ptx::ex2_approx(fmaf(s[i][x][0], a.scale_log2, -b0));
-            const float p1 = b200attn::ptx::ex2_approx(fmaf(s[i][x][1], a.scale_log2, -b0));
-            const float p2 = b200attn::ptx::ex2_approx(fmaf(s[i][x][2], a.scale_log2, -b1));
-            const float p3 = b200attn::ptx::ex2_approx(fmaf(s[i][x][3], a.scale_log2, -b1));
-            // weights are rounded to the element type for the product; their sum is
-            // taken of the rounded ones, so a row of few keys stays exact
-            pf[i][2 * x] = pack_pair<DT>(p0, p1);
-            pf[i][2 * x + 1] = pack_pair<DT>(p2, p3);
-            const float2 r0 = unpack_pair<DT>(pf[i][2 * x]), r1 = unpack_pair<DT>(pf[i][2 * x + 1]);
-            l[i][0] += r0.x + r0.y;
-            l[i][1] += r1.x + r1.y;
+          for (int hh = 0; hh < 2; ++hh) {
+            if (hh >= S::kHalves) {
+              pf[i][1] = pf[i][3] = 0u;
+              break;
+            }
+            const float base = m[i][hh] == -INFINITY ? 0.f : m[i][hh];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float p0 = b200attn::ptx::ex2_approx(fmaf(s[i][x][2 * hh], a.scale_log2, -base));
+              const float p1 =
+                  b200attn::ptx::ex2_approx(fmaf(s[i][x][2 * hh + 1], a.scale_log2, -base));
+              // weights are rounded to the element type for the product; their sum is
+              // taken of the rounded ones, so a row of few keys stays exact
+              const uint32_t w = pack_pair<DT>(p0, p1);
+              const float2 r = unpack_pair<DT>(w);
+              pf[i][2 * x + hh] = w;
+              l[i][hh] += r.x + r.y;
+            }
           }
         }
 #pragma unroll
@@ -482,9 +521,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
         part[RM * DP + RM + r] = total;
       }
     };
-    if (MT == 1 && rows <= 8) {
-      if constexpr (MT == 1)
-        join_columns(std::integral_constant<int, 8>{}, std::integral_constant<int, 64>{});
+    if constexpr (S::FEW) {
+      join_columns(std::integral_constant<int, 8>{}, std::integral_constant<int, 64>{});
     } else {
       join_columns(std::integral_constant<int, RM>{}, std::integral_constant<int, S::kCols>{});
     }

@@ -20,7 +20,9 @@ namespace {
 // 16 rows by 64 keys a tile, fp32 multiply-adds: scores from shared memory, one
 // pass over the keys with the running maximum and sum, the products' sums in
 // registers.
-constexpr int kRows = 16, kKeys = 64, kThreads = 128;
+constexpr int kRows = 16, kKeys = 64, kThreads = 256;
+constexpr int kScoreRows = kRows * kKeys / kThreads;  // rows of a thread's key
+constexpr int kWarpRows = kRows * 32 / kThreads;      // rows of a warp in the softmax step
 using PlainGrid = Grid<kRows, kKeys, 1>;
 
 template <int DP>
@@ -127,20 +129,20 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
         }
       }
       __syncthreads();
-      {  // scores: this thread's key, 8 rows
-        const int key = tid & (kKeys - 1), r0 = (tid / kKeys) * (kRows / 2);
-        float s[kRows / 2] = {};
+      {  // scores: this thread's key, some rows
+        const int key = tid & (kKeys - 1), r0 = (tid / kKeys) * kScoreRows;
+        float s[kScoreRows] = {};
         for (int c = 0; c < DP; c += 4) {
           const float4 kk = *reinterpret_cast<const float4*>(&sm.k[key][c]);
 #pragma unroll
-          for (int r = 0; r < kRows / 2; ++r) {
+          for (int r = 0; r < kScoreRows; ++r) {
             const float4 qq = *reinterpret_cast<const float4*>(&sm.q[r0 + r][c]);
             s[r] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[r]))));
           }
         }
         const int j = k0 + key - pl.s.len;  // place in the draft
 #pragma unroll
-        for (int r = 0; r < kRows / 2; ++r) {
+        for (int r = 0; r < kScoreRows; ++r) {
           const int i = (pl.rt * kRows + r0 + r) / a.group;
           const bool shown = r0 + r < rows && sm.live[key] &&
                              (j < 0 || (j < pl.s.drafts && sees(a, pl.b, i, j)));
@@ -148,9 +150,10 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
         }
       }
       __syncthreads();
-      {  // softmax step: a warp takes 4 rows
+      {  // softmax step
         const int lane = tid & 31, warp = tid >> 5;
-        for (int r = warp * 4; r < warp * 4 + 4; ++r) {
+#pragma unroll
+        for (int r = warp * kWarpRows; r < warp * kWarpRows + kWarpRows; ++r) {
           const float x0 = sm.p[r][lane], x1 = sm.p[r][lane + 32];
           float top = fmaxf(x0, x1);
 #pragma unroll
@@ -175,6 +178,7 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
       __syncthreads();
 #pragma unroll
       for (int r = 0; r < kRowsPer; ++r) acc[r] *= sm.alpha[rg * kRowsPer + r];
+#pragma unroll 8
       for (int key = 0; key < kKeys; ++key) {
         const float vv = sm.v[key][col];
 #pragma unroll

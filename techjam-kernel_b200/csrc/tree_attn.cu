@@ -248,11 +248,11 @@ struct Choice {
   int ctas_per_sm;
 };
 
-// Queries and pools can be read through tensor maps: page boxes of 8 rows or more,
-// and strides that move.
-bool by_tensor_maps(const b200_tree_attn_params* p) {
+// Queries and pools can be read through tensor maps: page boxes of `box_rows` or more (8 at
+// least), and strides that move.
+bool by_tensor_maps(const b200_tree_attn_params* p, int box_rows) {
   const b200_cache& c = p->cache;
-  if (box_rows_of(c.page_size) < 8) return false;
+  if (box_rows_of(c.page_size) < box_rows) return false;
   const int64_t extent[4] = {1, c.pages, c.kv_heads, c.page_size};
   for (int d = 1; d < 4; ++d)
     if (extent[d] > 1 && (c.k_stride[d] <= 0 || c.v_stride[d] <= 0)) return false;
@@ -267,7 +267,11 @@ Choice choose(const b200_tree_attn_params* p) {
   if (p->cache.dtype == B200_ATTN_DTYPE_FP32) return Choice{kPlain, kRows, kRows, kKeys, dp, dp == 64 ? 4 : 2};
   const int64_t rows = p->tokens * (p->heads / p->cache.kv_heads);
   const int64_t group = p->heads / p->cache.kv_heads;
-  if (rows > 32 && group <= 128 && by_tensor_maps(p)) {
+  // More than 16 rows: the tcgen05 kernel, unless its boxes would be small, where each box
+  // costs more than its bytes: 32 rows over 131001 keys take 100 us with boxes of 64 keys,
+  // 141 us with boxes of 16; the few-row kernel 128 us with either.  Up to 16 rows the
+  // few-row kernel reads at the rate of memory (16 rows: 100 us, 4 rows: 92 us).
+  if (rows > 16 && group <= 128 && by_tensor_maps(p, rows > 32 ? 8 : 32)) {
     // whole tokens to a tile of 128 places
     const int tile = static_cast<int>(128 / group * group);
     if (rows <= tile) return Choice{kManyRows, 128, tile, 128, dp, 1};
@@ -304,7 +308,7 @@ int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
 
 template <int RM, int DP, int DT, int WARPS>
 int32_t run_join_rows(const Args& a, int64_t units, cudaStream_t s) {
-  return launch(join_rows_kernel<RM, DP, DT, WARPS>, dim3(static_cast<unsigned>(units), RM / 4),
+  return launch(join_rows_kernel<RM, DP, DT, WARPS>, dim3(static_cast<unsigned>(units)),
                 dim3(32 * WARPS), 0, s, a);
 }
 

@@ -407,8 +407,8 @@ __device__ __forceinline__ uint8_t* out_row(const Args& a, const Joint& j, int r
   return a.o + j.b * a.o_seq + (j.h * a.group + row - tok * a.group) * a.o_head + tok * a.o_tok;
 }
 
-// Row by row, partial sums [RM][DP]: 4 rows of a unit by the WARPS warps of a block, a
-// lane taking DP / 32 columns.  Reads past L1: other CTAs of this kernel may have
+// Row by row, partial sums [RM][DP], a lane taking DP / 32 columns.  Up to 4 rows: the WARPS
+// warps of a block share the runs and join in shared memory.  Reads past L1: other CTAs of this kernel may have
 // written the partial results.
 template <int DP, int WARPS>
 struct JoinSmem {
@@ -481,15 +481,69 @@ __device__ __noinline__ void join_four(const Args& a, Joint j, JoinSmem<DP, WARP
   __syncthreads();
 }
 
-// WARPS as in the kernel that left the partial results: the same sums in the same order,
-// wherever they are joined.
+// More rows: each warp takes RM / WARPS of them over all runs, without shared memory.
+template <int RM, int DP, int DT, int WARPS>
+__device__ __noinline__ void join_many(const Args& a, Joint j) {
+  using E = Elem<DT>;
+  constexpr int kCols = DP / 32, kN = RM / WARPS;
+  const int lane = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * kN;
+  if (r0 >= j.rows) return;
+  float top[kN], total[kN], acc[kN][kCols];
+#pragma unroll
+  for (int r = 0; r < kN; ++r) {
+    top[r] = -INFINITY;
+    total[r] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kCols; ++x) acc[r][x] = 0.f;
+  }
+#pragma unroll 2
+  for (int c = j.runs.x; c <= j.runs.y; ++c) {
+    const float* p = part_of<RM, DP>(a, j, c);
+    float v[kN][kCols], m[kN], l[kN];
+#pragma unroll
+    for (int r = 0; r < kN; ++r) {
+#pragma unroll
+      for (int x = 0; x < kCols; ++x) v[r][x] = __ldcg(p + (r0 + r) * DP + lane + 32 * x);
+      m[r] = __ldcg(p + RM * DP + r0 + r);
+      l[r] = __ldcg(p + RM * DP + RM + r0 + r);
+    }
+#pragma unroll
+    for (int r = 0; r < kN; ++r) {
+      const float now = fmaxf(top[r], m[r]), base = now == -INFINITY ? 0.f : now;
+      const float keep = exp2f(top[r] - base), w = exp2f(m[r] - base);
+      top[r] = now;
+      total[r] = total[r] * keep + w * l[r];
+#pragma unroll
+      for (int x = 0; x < kCols; ++x) acc[r][x] = acc[r][x] * keep + w * v[r][x];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kN; ++r) {
+    if (r0 + r >= j.rows) break;
+    typename E::T* out = reinterpret_cast<typename E::T*>(out_row(a, j, r0 + r));
+#pragma unroll
+    for (int x = 0; x < kCols; ++x)
+      if (lane + 32 * x < a.head_dim)
+        out[lane + 32 * x] =
+            E::round(total[r] == 0.f ? 0.f * acc[r][x] : acc[r][x] / total[r]);
+  }
+}
+
+template <int RM, int DP, int DT, int WARPS>
+__device__ __forceinline__ void join_unit(const Args& a, const Joint& j, JoinSmem<DP, WARPS>* sm) {
+  if (j.rows <= 4) join_four<RM, DP, DT, WARPS>(a, j, sm);
+  else join_many<RM, DP, DT, WARPS>(a, j);
+}
+
+// A block a unit.  WARPS as in the kernel that left the partial results: the same sums in
+// the same order, wherever they are joined.
 template <int RM, int DP, int DT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) join_rows_kernel(const __grid_constant__ Args a) {
   __shared__ JoinSmem<DP, WARPS> sm;
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
   Joint j;
-  if (joint_of(a, 4 * blockIdx.y, &j)) join_four<RM, DP, DT, WARPS>(a, j, &sm);
+  if (joint_of(a, 0, &j)) join_unit<RM, DP, DT, WARPS>(a, j, &sm);
 }
 
 // The same within the kernel that left the partial results: the last of a unit's runs to
@@ -507,9 +561,7 @@ __device__ __noinline__ void join_if_last(const Args& a, int b, int h, int rt, i
   }
   if (!__syncthreads_or(mine)) return;
   __threadfence();
-  Joint j{make_int2(first, last), 0, rows, b, h, rt};
-#pragma unroll 1
-  for (; j.row0 < rows; j.row0 += 4) join_four<RM, DP, DT, WARPS>(a, j, sm);
+  join_unit<RM, DP, DT, WARPS>(a, Joint{make_int2(first, last), 0, rows, b, h, rt}, sm);
 }
 
 // Column by column: partial sums [DP][RM], a block takes 32 rows, a lane one of them,

@@ -277,8 +277,9 @@ Choice choose(const b200_tree_attn_params* p) {
     if (rows <= tile) return Choice{kManyRows, 128, tile, 128, dp, 1};
     return Choice{kManyRows, 256, 2 * tile, 128, dp, 1};
   }
-  const int rm = rows <= 16 ? 16 : 32;
-  return Choice{kFewRows, rm, rm, kRowTile, dp, 1};
+  // (the shapes do not depend on the head dim)
+  if (rows <= 16) return Choice{kFewRows, 16, 16, RowShape<1, false, 64>::kTile, dp, RowShape<1, false, 64>::kCtas};
+  return Choice{kFewRows, 32, 32, RowShape<2, false, 64>::kTile, dp, 1};
 }
 
 int64_t row_tiles(const b200_tree_attn_params* p, const Choice& c) {
@@ -352,17 +353,17 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
     if (c.kernel == kManyRows)
       rc = launch_tiles(c.rm, c.dp, DT, a, a.kv_heads * a.group, runs, device, s);
     else if (a.tokens * a.group <= 8)
-      rc = run_one<8, DP, DT>(rows_kernel<Few, DT>, kRowThreads, Few::kSmemBytes, a, runs, device, s);
+      rc = run_one<8, DP, DT>(rows_kernel<Few, DT>, Few::kThreads, Few::kSmemBytes, a, runs, device, s);
     else if (c.rm == 16)
-      rc = run_one<16, DP, DT>(rows_kernel<One, DT>, kRowThreads, One::kSmemBytes, a, runs, device,
+      rc = run_one<16, DP, DT>(rows_kernel<One, DT>, One::kThreads, One::kSmemBytes, a, runs, device,
                                s);
     else
-      rc = run_one<32, DP, DT>(rows_kernel<Two, DT>, kRowThreads, Two::kSmemBytes, a, runs, device,
+      rc = run_one<32, DP, DT>(rows_kernel<Two, DT>, Two::kThreads, Two::kSmemBytes, a, runs, device,
                                s);
     if (rc != B200_ATTN_OK || a.counters) return rc;
     switch (c.rm) {
-      case 16: return run_join_rows<16, DP, DT, kRowWarps>(a, units, s);
-      case 32: return run_join_rows<32, DP, DT, kRowWarps>(a, units, s);
+      case 16: return run_join_rows<16, DP, DT, One::kWarps>(a, units, s);
+      case 32: return run_join_rows<32, DP, DT, Two::kWarps>(a, units, s);
       case 128: return run_join_columns<128, DP, DT>(a, units, s);
       default: return run_join_columns<256, DP, DT>(a, units, s);
     }

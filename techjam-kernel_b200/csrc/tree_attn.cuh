@@ -429,7 +429,7 @@ __device__ __noinline__ void join_four(const Args& a, Joint j, JoinSmem<DP, WARP
 #pragma unroll
     for (int x = 0; x < kCols; ++x) acc[r][x] = 0.f;
   }
-#pragma unroll 1
+#pragma unroll 3
   for (int c = j.runs.x + warp; c <= j.runs.y; c += WARPS) {
     const float* p = part_of<RM, DP>(a, j, c);
     float v[4][kCols], m[4], l[4];
@@ -496,7 +496,7 @@ __device__ __noinline__ void join_many(const Args& a, Joint j) {
 #pragma unroll
     for (int x = 0; x < kCols; ++x) acc[r][x] = 0.f;
   }
-#pragma unroll 2
+#pragma unroll 4
   for (int c = j.runs.x; c <= j.runs.y; ++c) {
     const float* p = part_of<RM, DP>(a, j, c);
     float v[kN][kCols], m[kN], l[kN];

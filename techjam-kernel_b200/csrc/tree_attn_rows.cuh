@@ -18,10 +18,7 @@
 
 namespace b200tree {
 
-constexpr int kRowWarps = 8;
-constexpr int kRowThreads = 32 * kRowWarps;
-constexpr int kRowKeys = 16;                      // keys of a warp's block
-constexpr int kRowTile = kRowWarps * kRowKeys;    // keys of a tile
+constexpr int kRowKeys = 16;  // keys of a warp's block
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
@@ -94,27 +91,33 @@ template <int MT_, bool FEW_, int DP_>
 struct RowShape {
   static constexpr int MT = MT_, DP = DP_, RM = 16 * MT_;
   static constexpr bool FEW = FEW_;
+  // One row tile: two CTAs of 4 warps on an SM, so that one reads while the other joins;
+  // two row tiles need the SM for one CTA of 8.
+  static constexpr int kWarps = MT == 1 ? 4 : 8, kThreads = 32 * kWarps;
+  static constexpr int kCtas = 8 / kWarps;          // on an SM
+  static constexpr int kTile = kWarps * kRowKeys;   // keys of a tile
   static constexpr int kHalves = FEW ? 1 : 2;  // halves of 8 rows of a tile
   static_assert(!FEW || MT == 1, "up to 8 rows");
   static constexpr int kRowBytes = 2 * DP;
   static constexpr int kPieces = kRowBytes / 16;
   static constexpr int kBlockBytes = kRowKeys * kRowBytes;     // one warp's keys or values
   static constexpr int kStages = DP == 128 ? 3 : 6;            // 192 KB of loads in flight
-  static constexpr int kRingBytes = kRowWarps * kStages * 2 * kBlockBytes;
-  static constexpr int kCols = MT == 1 ? 32 : 16;              // columns joined at a time
+  static constexpr int kRingBytes = kWarps * kStages * 2 * kBlockBytes;
+  static constexpr int kEach = MT == 1 ? 4 : 2;                // columns of a thread in a join
+  static constexpr int kCols = kEach * kThreads / RM;          // columns joined at a time
   static constexpr int kJoinPitch = kCols + 4;
   static constexpr int kOffQ = kRingBytes;
   static constexpr int kOffJoin = kOffQ + RM * kRowBytes;
-  static constexpr int kOffStat = kOffJoin + 4 * kRowWarps * RM * kJoinPitch;
-  static constexpr int kOffMisc = kOffStat + 4 * 2 * kRowWarps * RM;
+  static constexpr int kOffStat = kOffJoin + 4 * kWarps * RM * kJoinPitch;
+  static constexpr int kOffMisc = kOffStat + 4 * 2 * kWarps * RM;
   static constexpr int kSmemBytes = kOffMisc + 256;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of a block");
-  using G = Grid<RM, kRowTile, 2>;
-  static_assert(sizeof(JoinSmem<DP, kRowWarps>) <= 4 * kRowWarps * RM * kJoinPitch, "joins in place");
+  using G = Grid<RM, kTile, 2>;
+  static_assert(sizeof(JoinSmem<DP, kWarps>) <= 4 * kWarps * RM * kJoinPitch, "joins in place");
 };
 
 template <class S, int DT>
-__global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(S::kThreads, S::kCtas) rows_kernel(const __grid_constant__ Args a) {
   constexpr int RM = S::RM, DP = S::DP, MT = S::MT, NS = S::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sbase = b200attn::ptx::smem_u32(smem);
@@ -134,13 +137,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   const bool whole = a.page_size % kRowKeys == 0;  // a block lies in one page
 
   // ------------------------------------------------------------- queries
-  constexpr int kQPieces = RM * S::kPieces / kRowThreads > 0 ? RM * S::kPieces / kRowThreads : 1;
+  constexpr int kQPieces = RM * S::kPieces / S::kThreads > 0 ? RM * S::kPieces / S::kThreads : 1;
   uint4 qreg[kQPieces];
   auto fetch_q = [&](const Place& p) {
     const int rows = min(RM, p.s.drafts * a.group - p.rt * RM);
 #pragma unroll
     for (int u = 0; u < kQPieces; ++u) {
-      const int x = tid + u * kRowThreads;
+      const int x = tid + u * S::kThreads;
       const int r = x / S::kPieces, piece = x % S::kPieces;
       qreg[u] = make_uint4(0u, 0u, 0u, 0u);
       if (r < rows && piece < pieces) {
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   auto store_q = [&]() {
 #pragma unroll
     for (int u = 0; u < kQPieces; ++u) {
-      const int x = tid + u * kRowThreads;
+      const int x = tid + u * S::kThreads;
       const int r = x / S::kPieces, piece = x % S::kPieces;
       if (r < RM)
         *reinterpret_cast<uint4*>(smem + S::kOffQ + r * S::kRowBytes + ((piece ^ (r & 7)) << 4)) =
@@ -172,8 +175,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   bool more = !run.done(ld);  // tiles are still to be loaded
   int page = -1, page_row = 0, ld_keys = 0;
   auto look_up = [&]() {
-    const int key = ld.t * kRowTile + warp * kRowKeys + (whole ? 0 : (lane & 15));
-    ld_keys = ld.s.len + ld.s.drafts - (ld.t * kRowTile + warp * kRowKeys);
+    const int key = ld.t * S::kTile + warp * kRowKeys + (whole ? 0 : (lane & 15));
+    ld_keys = ld.s.len + ld.s.drafts - (ld.t * S::kTile + warp * kRowKeys);
     page = -1;
     page_row = 0;
     if (key < ld.s.len + ld.s.drafts) {
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       __syncwarp();
       const uint32_t kb = ring + use * (2 * S::kBlockBytes), vb = kb + S::kBlockBytes;
       use = use + 1 == NS ? 0 : use + 1;
-      const int k0 = t * kRowTile + warp * kRowKeys;
+      const int k0 = t * S::kTile + warp * kRowKeys;
       if (k0 < keys) {
         float s[MT][2][4];
         float s2[2][4];  // one row tile: the odd steps' sums, for shorter chains of products
@@ -453,27 +456,27 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       for (int hh = 0; hh < 2; ++hh) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w)
+        for (int w = 0; w < S::kWarps; ++w)
           top = fmaxf(top, stat[2 * w * RM + 16 * i + 8 * hh + g]);
         scale[i][hh] = top == -INFINITY ? 0.f : b200attn::ptx::ex2_approx(m[i][hh] - top);
       }
     const int rows = min(RM, done.s.drafts * a.group - done.rt * RM);
     float* part = a.partial + static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * (RM * (DP + 2));
     const bool finish = first && last;
-    // The warps' sums go through shared memory, `cols` columns at a time; a thread adds two
-    // columns of a row.  Up to 8 rows (a token of 8 query heads): twice the columns of half
+    // The warps' sums go through shared memory, some columns at a time; a thread adds
+    // kEach columns of a row.  Up to 8 rows (a token of 8 query heads): twice the columns of half
     // the rows.
     auto join_columns = [&](auto row_count, auto col_count) {
       constexpr int kR = decltype(row_count)::value, kC = decltype(col_count)::value;
       constexpr int kPitch = kC + 4;
-      static_assert(kR * kC == 2 * kRowThreads, "two columns a thread");
+      static_assert(kR * kC == S::kEach * S::kThreads, "kEach columns a thread");
       static_assert(kR * kPitch <= RM * S::kJoinPitch, "in place");
-      const int r = tid / (kC / 2), c = (tid % (kC / 2)) * 2;
+      const int r = tid / (kC / S::kEach), c = (tid % (kC / S::kEach)) * S::kEach;
       float top = -INFINITY, total = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, stat[2 * w * RM + r]);
+      for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, stat[2 * w * RM + r]);
 #pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) {
+      for (int w = 0; w < S::kWarps; ++w) {
         const float mw = stat[2 * w * RM + r];
         if (mw != -INFINITY)
           total += stat[(2 * w + 1) * RM + r] * b200attn::ptx::ex2_approx(mw - top);
@@ -497,24 +500,31 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
                   make_float2(src[2] * scale[i][1], src[3] * scale[i][1]);
           }
         __syncthreads();
-        float2 acc = make_float2(0.f, 0.f);
+        float2 acc[S::kEach / 2];
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) {
-          const float2 v = *reinterpret_cast<const float2*>(join + (w * kR + r) * kPitch + c);
-          acc.x += v.x;
-          acc.y += v.y;
-        }
-        if (finish) {
-          if (r < rows && c0 + c < a.head_dim)
-            *reinterpret_cast<uint32_t*>(out + 2 * (c0 + c)) = pack_pair<DT>(acc.x * inv, acc.y * inv);
-        } else {
-          *reinterpret_cast<float2*>(part + r * DP + c0 + c) = acc;
+        for (int e = 0; e < S::kEach / 2; ++e) acc[e] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < S::kWarps; ++w)
+#pragma unroll
+          for (int e = 0; e < S::kEach / 2; ++e) {
+            const float2 v =
+                *reinterpret_cast<const float2*>(join + (w * kR + r) * kPitch + c + 2 * e);
+            acc[e].x += v.x;
+            acc[e].y += v.y;
+          }
+#pragma unroll
+        for (int e = 0; e < S::kEach / 2; ++e) {
+          if (!finish)
+            *reinterpret_cast<float2*>(part + r * DP + c0 + c + 2 * e) = acc[e];
+          else if (r < rows && c0 + c < a.head_dim)
+            *reinterpret_cast<uint32_t*>(out + 2 * (c0 + c + 2 * e)) =
+                pack_pair<DT>(acc[e].x * inv, acc[e].y * inv);
         }
       }
       if (any_odd && r < rows)
         for (int c0 = c; c0 < DP; c0 += kC)
-          add_odd<DT>(a, done.b, done.h, done.s, tok, t0 * kRowTile - done.s.len,
-                      (t0 + n) * kRowTile - done.s.len, c0, min(a.head_dim, c0 + 2),
+          add_odd<DT>(a, done.b, done.h, done.s, tok, t0 * S::kTile - done.s.len,
+                      (t0 + n) * S::kTile - done.s.len, c0, min(a.head_dim, c0 + S::kEach),
                       finish ? reinterpret_cast<uint16_t*>(out) : nullptr, part + r * DP, 1);
       if (!finish && c == 0) {
         part[RM * DP + r] = top;
@@ -530,8 +540,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       const int from = run.ends_in(done) ? run.end_first : (first ? blockIdx.x : run.first_run);
       const int to = run.ends_in(done) ? run.end_last : blockIdx.x;
       if (a.counters)
-        join_if_last<RM, DP, DT, kRowWarps>(a, done.b, done.h, done.rt, rows, from, to,
-                                            reinterpret_cast<JoinSmem<DP, kRowWarps>*>(join));
+        join_if_last<RM, DP, DT, S::kWarps>(a, done.b, done.h, done.rt, rows, from, to,
+                                            reinterpret_cast<JoinSmem<DP, S::kWarps>*>(join));
       else if (tid == 0 && last)
         a.desc[unit_of(a, done)] = make_int2(from, to);
     } else if (tid == 0 && !a.counters) {
@@ -540,7 +550,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
     if (again) store_q();  // the queries' fragments are in registers, or read between the barriers
     __syncthreads();
   }
-  zero_unused_rows(a, 2, kRowThreads);
+  zero_unused_rows(a, 2, S::kThreads);
 }
 
 }  // namespace b200tree

@@ -225,6 +225,13 @@ __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t word) {
     if (!((word >> k) & 1u)) s[k] = __float_as_uint(-INFINITY);
 }
 
+// Bits 15 and 31: whether the halves of a word are not finite (adding one to an exponent
+// of all ones carries into the sign's place).
+template <int DT>
+__device__ __forceinline__ uint32_t exponent_carry(uint32_t w) {
+  return (w & 0x7fff7fffu) + (DT == B200_ATTN_DTYPE_BF16 ? 0x00800080u : 0x04000400u);
+}
+
 template <class S, int DT>
 __global__ void __launch_bounds__(kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -478,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // infinity would reach the sums), and so do elements of drafted values that
           // are not finite: the softmax groups add those to the rows that see them.
           const int r0 = max(0, len - k0), r1 = min(kTile, len + pl.s.drafts - k0);
+          const int r2 = min(kTile, (r1 + box_rows - 1) & -box_rows);  // later boxes are zero
           auto piece = [&](int x) {  // shared-memory address of piece x of the tile's rows
             const int pc = x % S::kPieces;
             return va + (pc >> 3) * S::kChunkBytes + (x / S::kPieces) * 128 + ((pc & 7) << 4);
@@ -503,8 +511,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int u = 0; u < 8; ++u)
 #pragma unroll
-              for (int y = 0; y < 4; ++y) any |= not_finite<DT>(w[u][y]);
-            if (any) {
+              for (int y = 0; y < 4; ++y) any |= exponent_carry<DT>(w[u][y]);
+            if (any & 0x80008000u) {
               odd = true;
 #pragma unroll
               for (int u = 0; u < 8; ++u) {
@@ -517,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           uint32_t zero[4] = {0u, 0u, 0u, 0u};
 #pragma unroll 1
-          for (int x = r1 * S::kPieces + lane; x < kTile * S::kPieces; x += 32) put(x, zero);
+          for (int x = r1 * S::kPieces + lane; x < r2 * S::kPieces; x += 32) put(x, zero);
           if (odd) misc[2] = seg + 1u;
           ptx::fence_proxy_async_smem();
           __syncwarp();

@@ -12,6 +12,8 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -38,7 +40,6 @@ NVCC_FLAGS = (
     "-lineinfo",
     "-Xcompiler", "-fPIC",
     "-Xcompiler", "-fvisibility=hidden",
-    "-shared",
 )
 
 
@@ -75,16 +76,26 @@ def build_native(force: bool = False, verbose: bool = False, checked: bool = Fal
         return out
     tmp = out.with_suffix(".so.tmp")
     defines = ["-DB200_ATTN_CHECKED=1"] if checked else []
-    cmd = [_nvcc(), *NVCC_FLAGS, *defines, f"-I{INCLUDE}", f"-I{CSRC}",
-           *[str(CSRC / s) for s in SOURCES], "-o", str(tmp)]
+    nvcc = _nvcc()
+
+    def run(args: list[str]) -> str:
+        cmd = [nvcc, *NVCC_FLAGS, *defines, *args]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+            print(" ".join(cmd))
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stderr[-8000:]}")
+        return proc.stderr
+
+    # one nvcc a source, side by side, then the link
+    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(len(SOURCES)) as pool:
+        objs = [str(Path(objects) / f"{s}.o") for s in SOURCES]
+        told = list(pool.map(lambda so: run([f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(CSRC / so[0]),
+                                             "-o", so[1]]), zip(SOURCES, objs)))
+        told.append(run(["-shared", *objs, "-o", str(tmp)]))
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd))
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stderr[-8000:]}")
-    if verbose and proc.stderr:
-        print(proc.stderr)
+        print("".join(told))
     os.replace(tmp, out)
     return out
 

@@ -66,7 +66,10 @@ struct Rows {
 
 // One thread moves one 16-byte piece of one token's key and value row in up to
 // kLayerGroup layers: the page is looked up once, and up to 2 x kLayerGroup
-// loads are in flight before the stores.
+// loads are in flight before the stores.  Bound by HBM: 64 sequences of 16 tokens in
+// 32 layers (268 MB read and written) take 45 us, the rate of a plain copy of as many
+// bytes (44 us).  Groups of 2 or 8 layers, token-major order and streaming stores were
+// all within 3 % or slower.
 constexpr int kLayerGroup = 4;
 
 __global__ void __launch_bounds__(kCopyThreads) append_kernel(const Pool c, const Rows r) {
@@ -115,7 +118,8 @@ __global__ void __launch_bounds__(kCopyThreads) append_kernel(const Pool c, cons
 // One thread owns one 16-byte column of one (layer, K or V, sequence, head) and
 // moves it along the path in order.  paths increases strictly, so paths[j] >= j:
 // a row is overwritten only by the move of an earlier or the same step, whose
-// batch of loads was complete before its stores.
+// batch of loads was complete before its stores.  Paths of up to 16 rows in 64 sequences
+// and 32 layers: 16 us, of which the launch and the chain path -> page -> row are most.
 constexpr int kPathBatch = 8;
 
 __global__ void __launch_bounds__(kCopyThreads)
@@ -225,7 +229,9 @@ struct Scratch {
 // Warps take (move, layer, K or V, head) segments in turn; a segment's rows are
 // contiguous pieces of 16 bytes, and a lane keeps kUnroll of them in flight.  Stored as
 // streaming: nothing reads the rows soon (copies of 224 part-filled pages in 32 layers,
-// 451 MB: 74 us against 87 us with plain stores; 8 pieces in flight 100 us, 2: 95 us).
+// 451 MB: 74 us = 6.1 TB/s against 87 us with plain stores; 8 pieces in flight 100 us, 2:
+// 95 us).  Bound by HBM; compacting 186 whole pages of 32 layers, 780 MB, takes 112 us with
+// its plan, part of it out of L2.
 constexpr int kUnroll = 4;
 
 // By warp `warp` of `warps`.
@@ -422,6 +428,9 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // ----------------------------------------------------------------- compact
+// Small calls are bound by the launch and by the plan's chain of passes: with moves of up to
+// 1 MiB done by the planning CTA itself a call is one launch (a pool of 38 pages: 3.4 us
+// behind the call before it).
 // One CTA plans: n pages are held; the free pages before n (ascending) receive
 // the held pages at or past n (ascending), so sources and destinations never
 // meet and every page moves at most once.

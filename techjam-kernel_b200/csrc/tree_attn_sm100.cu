@@ -132,20 +132,32 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity,
   return ptx::mbar_try_wait(bar, parity) || wait_slow(bar, parity, abort_flag, err);
 }
 
-__device__ __forceinline__ bool issuer_wait(uint32_t bar, uint32_t parity,
-                                            volatile uint32_t* abort_flag, int32_t* err) {
-#pragma unroll 1
-  for (int k = 0; k < kIssuerSpin; ++k)
-    if (ptx::mbar_test_wait(bar, parity)) return true;
-  return wait_bar(bar, parity, abort_flag, err);
-}
-
 // By every lane; the result is the same for the warp.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity,
                                           volatile uint32_t* abort_flag, int32_t* err) {
   const bool all = __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, err));
   if (!all) *abort_flag = 1u;
   return all;
+}
+
+// The same, spinning at first: for the issuers, on whom all others wait.
+__device__ __forceinline__ bool issuer_wait(uint32_t bar, uint32_t parity,
+                                            volatile uint32_t* abort_flag, int32_t* err) {
+#pragma unroll 1
+  for (int k = 0; k < kIssuerSpin; ++k)
+    if (__all_sync(0xffffffffu, ptx::mbar_test_wait(bar, parity))) return true;
+  return warp_wait(bar, parity, abort_flag, err);
+}
+
+// The lane of a converged warp that issues.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t mine;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(mine));
+  return mine != 0;
 }
 
 __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
@@ -391,55 +403,59 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kQkWarp) {
     // -------------------------------------------------- scores S = Q K^T
-    if (lane == 0) {
-      constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, kTile, false);
-      uint32_t tile = 0, seg = 0;
-      uint32_t made = 0u;  // bit i: parity of the number of scores made for group i
-      int prev = -1;
-      bool ok = true;
+    // By the whole warp, one lane of which issues: in control flow that is the same for the
+    // warp the operands' descriptors stay in uniform registers.
+    constexpr uint32_t id = ptx::idesc_f16(kBF16, kTile, kTile, false);
+    uint32_t tile = 0, seg = 0;
+    uint32_t made = 0u;  // bit i: parity of the number of scores made for group i
+    int prev = -1;
+    bool ok = true;
 #pragma unroll 1
-      for (; ok && !run.done(pl); ++seg) {
-        const int n = run.tiles(pl), rows = unit_rows(pl);
-        ok = wait_bar(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
-        bool packed = false;
+    for (; ok; ++seg) {
+      const int n = __shfl_sync(0xffffffffu, run.tiles(pl), 0);
+      if (n <= 0) break;
+      const bool second = !kTwo || __shfl_sync(0xffffffffu, unit_rows(pl), 0) > share;
+      // the first tile that needs the masks
+      const int masked = __shfl_sync(0xffffffffu, min(n - 1, max(0, pl.s.len / kTile - pl.t)), 0);
+      ok = warp_wait(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
 #pragma unroll 1
-        for (int j = 0; ok && j < n; ++j, ++tile) {
-          // the masks are there before the scores that need them
-          if (!packed && (j == n - 1 || (pl.t + j + 1) * kTile > pl.s.len)) {
-            ok = wait_bar(bar(S::kBarSeen), seg & 1u, abort_flag, a.err);
-            packed = true;
-          }
-          const uint32_t number = S::load_k(tile), s = number % NS;
-          ok = ok && issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
+      for (int j = 0; ok && j < n; ++j, ++tile) {
+        // the masks are there before the scores that need them
+        if (j == masked) ok = warp_wait(bar(S::kBarSeen), seg & 1u, abort_flag, a.err);
+        const uint32_t number = S::load_k(tile), s = number % NS;
+        ok = ok && issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
 #pragma unroll 1
-          for (int i = 0; i < 2; ++i) {
-            if (!ok || !takes(i, j, rows)) continue;
-            // the scores before these have been copied to registers
-            if (prev >= 0 && !issuer_wait(bar(S::kBarRead + prev), ((made >> prev) & 1u) ^ 1u,
-                                          abort_flag, a.err)) {
-              ok = false;
-              continue;
-            }
-            ptx::tc_fence_after();
-            const uint64_t qd = ptx::smem_desc_sw128(
-                sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes, 16, 1024);
-            const uint64_t kd =
-                ptx::smem_desc_sw128(sbase + S::kOffRing + s * S::kTileBytes, 16, 1024);
+        for (int i = 0; i < 2; ++i) {
+          if (!ok || (kTwo ? (i == 1 && !second) : (j & 1) != i)) continue;
+          // the scores before these have been copied to registers
+          ok = prev < 0 ||
+               issuer_wait(bar(S::kBarRead + prev), ((made >> prev) & 1u) ^ 1u, abort_flag, a.err);
+          if (!ok) continue;
+          ptx::tc_fence_after();
+          const uint64_t qd = ptx::smem_desc_sw128(
+              sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes, 16, 1024);
+          const uint64_t kd =
+              ptx::smem_desc_sw128(sbase + S::kOffRing + s * S::kTileBytes, 16, 1024);
+          if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
               const uint32_t off = ((kk >> 2) * S::kChunkBytes + (kk & 3) * 32) >> 4;
               ptx::tc_mma_ss(tmem, qd + off, kd + off, id, kk > 0 ? 1u : 0u);
             }
             ptx::tc_commit(bar(S::kBarScores + i));
-            made ^= 1u << i;
-            prev = i;
           }
-          if (ok) ptx::tc_commit(bar(S::kBarEmpty + s));
+          __syncwarp();
+          made ^= 1u << i;
+          prev = i;
         }
-        ptx::tc_commit(bar(S::kBarQRead));
-        pl.t += n;
-        if (pl.t == pl.tiles) pl = next_unit<typename S::G>(a, pl);
+        if (ok && elect_one()) ptx::tc_commit(bar(S::kBarEmpty + s));
+        __syncwarp();
       }
+      if (elect_one()) ptx::tc_commit(bar(S::kBarQRead));
+      __syncwarp();
+      next_segment(pl);
+    }
+    if (elect_one()) {
       ptx::tc_commit(bar(S::kBarDrain));
       settle(bar(S::kBarDrain), 0);
     }
@@ -487,8 +503,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t made = 0u;  // bit i: parity of the number of products made for group i
     bool ok = true;
 #pragma unroll 1
-    for (; ok && !run.done(pl); ++seg) {
-      const int n = run.tiles(pl), rows = unit_rows(pl), len = pl.s.len;
+    for (; ok; ++seg) {
+      const int n = __shfl_sync(0xffffffffu, run.tiles(pl), 0);
+      if (n <= 0) break;
+      const int rows = __shfl_sync(0xffffffffu, unit_rows(pl), 0), len = pl.s.len;
       uint32_t begun = 0u;  // bit i: O_i holds a product of this segment
 #pragma unroll 1
       for (int j = 0; ok && j < n; ++j, ++tile) {
@@ -550,25 +568,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (!ok || !takes(i, j, rows)) continue;
-          ok = __all_sync(0xffffffffu, issuer_wait(bar(S::kBarWeights + i), (made >> i) & 1u,
-                                                   abort_flag, a.err));
+          ok = issuer_wait(bar(S::kBarWeights + i), (made >> i) & 1u, abort_flag, a.err);
           if (!ok) continue;
           ptx::tc_fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; ++kk)
               ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + S::kColP + 64 * i + kk * 8,
                              vd + kk * (2048 >> 4), id, (((begun >> i) & 1u) || kk > 0) ? 1u : 0u);
             ptx::tc_commit(bar(S::kBarSums + i));
           }
+          __syncwarp();
           begun |= 1u << i;
           made ^= 1u << i;
         }
-        if (ok && lane == 0) ptx::tc_commit(bar(S::kBarEmpty + s));
+        if (ok && elect_one()) ptx::tc_commit(bar(S::kBarEmpty + s));
+        __syncwarp();
       }
       next_segment(pl);
     }
-    if (lane == 0) {
+    if (elect_one()) {
       ptx::tc_commit(bar(S::kBarDrain));
       settle(bar(S::kBarDrain), 0);
     }

@@ -732,7 +732,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       ptx::tc_fence_after();
       const bool first = t0 == 0, last = t0 + n == unit.tiles;
-      const bool any_odd = misc[2] == seg + 1u;
+      // (a later segment's may have been noted already: then add_odd looks, and finds none)
+      const bool any_odd = misc[2] > seg;
       // weights of the groups' sums in this thread's row
       float top = m_run, total = l_run, w[2] = {1.f, 1.f};
       if constexpr (!kTwo) {

@@ -135,6 +135,25 @@ def test_hidden_draft_rows_may_hold_anything(dtype, T, group, bad):
     assert not torch.isfinite(got[:, :, 3, ::3]).any()
 
 
+@pytest.mark.parametrize("T,group", [(4, 2), (20, 4), (64, 4)])
+def test_infinite_values_of_many_short_sequences(T, group):
+    """Several units of one key tile to a CTA, each with an infinite value in its draft."""
+    gen = torch.Generator().manual_seed(5)
+    lens = [(7 * b) % 50 for b in range(40)]
+    args = make(lens, T, 16, group, 64, 32, BF16, seed=6)
+    q, k, v, table, _ = args
+    mask = torch.stack([random_tree(T, gen) for _ in lens])
+    for b, n in enumerate(lens):
+        v[int(table[b, (n + 3) // 32]), :, (n + 3) % 32, ::3] = float("inf")
+    got = b200_tree_attention(*(t.cuda() for t in args), mask.cuda()).cpu()
+    for b in range(len(lens)):
+        sees = mask[b, :, 3]
+        assert torch.isfinite(got[b][:, ~sees]).all()
+        assert (got[b][:, sees][..., ::3] == float("inf")).all()
+        rest = torch.arange(64) % 3 != 0
+        assert torch.isfinite(got[b][:, sees][..., rest]).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("T,group", [(3, 2), (40, 3)])
 def test_strides_and_layouts(dtype, T, group):

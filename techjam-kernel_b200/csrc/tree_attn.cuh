@@ -564,13 +564,52 @@ __device__ __noinline__ void join_if_last(const Args& a, int b, int h, int rt, i
   join_unit<RM, DP, DT, WARPS>(a, Joint{make_int2(first, last), 0, rows, b, h, rt}, sm);
 }
 
-// Column by column: partial sums [DP][RM], a block takes 32 rows, a lane one of them,
-// and 32 columns at a time; gridDim.z blocks share the columns.
-template <int RM, int DP, int DT>
+// Column by column: partial sums [DP][RM], a block takes 32 rows, a lane one of them.
+// A unit of up to kFewRuns runs, as in batches: each warp joins DP / 8 columns over all
+// runs by itself.  Longer ones: the warps share the runs and join kJoinCols columns at a time
+// in shared memory; gridDim.z blocks share the columns.  Few units: SPREAD, with more reads
+// in flight in a warp; many units: fewer registers, and so more warps.
+constexpr int kFewRuns = 4, kJoinCols = 16;
+
+// Folds the runs c, c + step ... into the columns from c0 on of a row; U runs are read at once.
+template <int RM, int DP, int U, int N>
+__device__ __forceinline__ void fold_runs(const Args& a, const Joint& j, int c, int step, int c0,
+                                          int row, float& top, float& total, float (&acc)[N]) {
+  top = -INFINITY;
+  total = 0.f;
+#pragma unroll
+  for (int x = 0; x < N; ++x) acc[x] = 0.f;
+#pragma unroll 1
+  for (; c <= j.runs.y; c += U * step) {
+    float v[U][N], m[U], l[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + u * step > j.runs.y) continue;
+      const float* p = part_of<RM, DP>(a, j, c + u * step) + row;
+#pragma unroll
+      for (int x = 0; x < N; ++x) v[u][x] = p[(c0 + x) * RM];
+      m[u] = p[RM * DP];
+      l[u] = p[RM * DP + RM];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + u * step > j.runs.y) continue;
+      const float now = fmaxf(top, m[u]), base = now == -INFINITY ? 0.f : now;
+      const float keep = exp2f(top - base), w = exp2f(m[u] - base);
+      top = now;
+      total = total * keep + w * l[u];
+#pragma unroll
+      for (int x = 0; x < N; ++x) acc[x] = acc[x] * keep + w * v[u][x];
+    }
+  }
+}
+
+template <int RM, int DP, int DT, bool SPREAD>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     join_columns_kernel(const __grid_constant__ Args a) {
   using E = Elem<DT>;
-  __shared__ float sums[kJoinWarps][32][33];
+  using T = typename E::T;
+  __shared__ float sums[kJoinWarps][32][kJoinCols + 1];
   __shared__ float tops[kJoinWarps][32], totals[kJoinWarps][32];
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
@@ -578,32 +617,41 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   if (!joint_of(a, 32 * blockIdx.y, &j)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = min(j.row0 + lane, j.rows - 1);
-  for (int c0 = 32 * blockIdx.z; c0 < DP; c0 += 32 * gridDim.z) {
-    float top = -INFINITY, total = 0.f, acc[32];
+  float top, total;
+  if (j.runs.y - j.runs.x < kFewRuns) {
+    constexpr int kN = DP / kJoinWarps;
+    const int c0 = kN * warp;
+    if (blockIdx.z > 0 || c0 >= a.head_dim) return;
+    float acc[kN];
+    fold_runs<RM, DP, SPREAD ? 2 : 1>(a, j, j.runs.x, 1, c0, row, top, total, acc);
+    if (j.row0 + lane >= j.rows) return;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    T* dst = reinterpret_cast<T*>(out_row(a, j, row)) + c0;
 #pragma unroll
-    for (int x = 0; x < 32; ++x) acc[x] = 0.f;
-    for (int c = j.runs.x + warp; c <= j.runs.y; c += kJoinWarps) {
-      const float* p = part_of<RM, DP>(a, j, c);
-      float v[32];
+    for (int x = 0; x < kN; x += 8) {
+      if (c0 + x >= a.head_dim) break;
+      union {
+        T e[8];
+        uint4 w;
+      } o;
 #pragma unroll
-      for (int x = 0; x < 32; ++x) v[x] = p[(c0 + x) * RM + row];
-      const float m = p[RM * DP + row], l = p[RM * DP + RM + row];
-      const float now = fmaxf(top, m), base = now == -INFINITY ? 0.f : now;
-      const float keep = exp2f(top - base), w = exp2f(m - base);
-      top = now;
-      total = total * keep + w * l;
-#pragma unroll
-      for (int x = 0; x < 32; ++x) acc[x] = acc[x] * keep + w * v[x];
+      for (int y = 0; y < 8; ++y) o.e[y] = E::round(acc[x + y] * inv);
+      *reinterpret_cast<uint4*>(dst + x) = o.w;
     }
+    return;
+  }
+  for (int c0 = kJoinCols * blockIdx.z; c0 < a.head_dim; c0 += kJoinCols * gridDim.z) {
+    float acc[kJoinCols];
+    fold_runs<RM, DP, SPREAD ? 3 : 1>(a, j, j.runs.x + warp, kJoinWarps, c0, row, top, total, acc);
     tops[warp][lane] = top;
     totals[warp][lane] = total;
 #pragma unroll
-    for (int x = 0; x < 32; ++x) sums[warp][lane][x] = acc[x];
+    for (int x = 0; x < kJoinCols; ++x) sums[warp][lane][x] = acc[x];
     __syncthreads();
-    // a thread finishes 4 columns of a row
-    const int r = threadIdx.x >> 3, x0 = 4 * (threadIdx.x & 7);
+    // a thread finishes 2 columns of a row
+    const int r = threadIdx.x >> 3, x0 = 2 * (threadIdx.x & 7);
     if (j.row0 + r < j.rows && c0 + x0 < a.head_dim) {
-      float best = -INFINITY, all = 0.f, sum[4] = {};
+      float best = -INFINITY, all = 0.f, sum[2] = {};
 #pragma unroll
       for (int w = 0; w < kJoinWarps; ++w) best = fmaxf(best, tops[w][r]);
       const float base = best == -INFINITY ? 0.f : best;
@@ -612,13 +660,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
         const float f = exp2f(tops[w][r] - base);
         all += f * totals[w][r];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sum[x] += f * sums[w][r][x0 + x];
+        for (int x = 0; x < 2; ++x) sum[x] += f * sums[w][r][x0 + x];
       }
       const float inv = all == 0.f ? 0.f : 1.f / all;
-      typename E::T* dst =
-          reinterpret_cast<typename E::T*>(out_row(a, j, j.row0 + r)) + c0 + x0;
+      T* dst = reinterpret_cast<T*>(out_row(a, j, j.row0 + r)) + c0 + x0;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) dst[x] = E::round(sum[x] * inv);
+      for (int x = 0; x < 2; ++x) dst[x] = E::round(sum[x] * inv);
     }
     __syncthreads();
   }

@@ -569,7 +569,7 @@ __device__ __noinline__ void join_if_last(const Args& a, int b, int h, int rt, i
 // runs by itself.  Longer ones: the warps share the runs and join kJoinCols columns at a time
 // in shared memory; gridDim.z blocks share the columns.  Few units: SPREAD, with more reads
 // in flight in a warp; many units: fewer registers, and so more warps.
-constexpr int kFewRuns = 4, kJoinCols = 16;
+constexpr int kFewRuns = 12, kJoinCols = 16;
 
 // Folds the runs c, c + step ... into the columns from c0 on of a row; U runs are read at once.
 template <int RM, int DP, int U, int N>

@@ -5,18 +5,19 @@
 // The mathematics is that of the kernel for few rows: one pass over the keys with a
 // running maximum and sum.  What bounds it: R rows do 4 R D operations for the 4 D
 // bytes of a key and value, so from about 260 rows the tensor cores, below it
-// HBM.  Measured (bf16, D 128): 32 sequences of 2 to 6 thousand keys, 8 key heads, 256
-// rows, 638 MB and 153 GFLOP: 202 us in short runs (757 TFLOP/s, 45 % of the
-// tensor cores' measured rate and half of the memory's), 228 us back to back, where
+// HBM.  Measured (bf16, D 128): 32 sequences of 1 to 8 thousand keys, 8 key heads, 256
+// rows, 638 MB and 153 GFLOP: 181 us in short runs (845 TFLOP/s, half of the
+// tensor cores' measured rate and of the memory's), 217 us back to back, where
 // the board's power limit lowers the clock; DRAM reads are the
-// cache's bytes exactly.  A key tile of 256 rows takes about 4100 cycles: the two
-// products of scores 1050 cycles each, those of the values 600, and each softmax group's
-// exponentials (128 a thread) between them; tensor pipe and exponential unit are each
-// active 45 % of the time.  32 rows over 131001 keys: 537 MB, 99 us, 5.4 TB/s.  Short
-// contexts (8 sequences of 300 tokens, 63 rows a head, fp16: 29 us against 6 us of
-// bytes) are bound by the ends of a unit (queries in, results out: about 10 us
-// each, overlapped only in part) and by boxes of 16 rows at about 165 cycles a box.
-// Scores of half a tile (64 keys) in buffers of their own: 260 us against 228 us.
+// cache's bytes exactly.  A key tile of 256 rows takes about 4000 cycles, in which a softmax
+// group waits for its scores (570 cycles of products and 300 to be seen), copies them (400),
+// exponentiates (128 a thread, 3000 cycles with its waits) and hands over the weights;
+// tensor pipe and exponential unit are each active under half of the time.
+// 64 rows over 131001 keys: 537 MB, 97 us, 5.5 TB/s.  Short
+// contexts (5 sequences of 601 to 5003 keys, 63 rows a head, fp16, pages of 48: 28 us against
+// 6 us of bytes) are bound by the ends of a unit (queries in, results out) and by boxes
+// of 16 rows at about 165 cycles a box.
+// Scores of half a tile (64 keys) in buffers of their own: 260 us against 228 us then.
 //
 // A CTA owns one run of the line of key tiles (tree_attn.cuh).  Twelve warps:
 //   warps 0-3, 4-7  two softmax groups, one thread per row = one TMEM lane

@@ -712,7 +712,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++cnt;
         ++done;
       }
+      // while the last product runs: where the row's results go
       const Place unit = *where;
+      const bool first = t0 == 0, last = t0 + n == unit.tiles, finish = first && last;
+      const bool mine = rl < share && row0 + rl < rows;
+      const int row = unit.rt * a.unit_rows + row0 + rl, tok = min(row / a.group, a.tokens - 1);
+      uint8_t* out = a.o + unit.b * a.o_seq + (unit.h * a.group + row % a.group) * a.o_head +
+                     tok * a.o_tok;
+      float* part = a.partial +
+                    static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * (RM * (DP + 2));
       __syncwarp();
       if (lane == 0) {
         Place next = unit;
@@ -732,7 +740,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (!kTwo) ok = ptx::named_barrier_and(1, kSoftmaxThreads, ok);
       if (!ok) break;
       ptx::tc_fence_after();
-      const bool first = t0 == 0, last = t0 + n == unit.tiles;
       // (a later segment's may have been noted already: then add_odd looks, and finds none)
       const bool any_odd = misc[2] > seg;
       // weights of the groups' sums in this thread's row
@@ -749,14 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         w[0] = i == 0 ? mine_w : other_w;
         w[1] = i == 0 ? other_w : mine_w;
       }
-      const bool mine = rl < share && row0 + rl < rows;
-      const int row = unit.rt * a.unit_rows + row0 + rl, tok = min(row / a.group, a.tokens - 1);
-      const bool finish = first && last;
       const float inv = total == 0.f ? 0.f : 1.f / total;
-      uint8_t* out = a.o + unit.b * a.o_seq + (unit.h * a.group + row % a.group) * a.o_head +
-                     tok * a.o_tok;
-      float* part = a.partial +
-                    static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * (RM * (DP + 2));
       if (!idle) {
         // kTwo: all columns of the own rows; else half the columns of the shared ones
         constexpr int kSpan = kTwo ? DP : DP / 2;

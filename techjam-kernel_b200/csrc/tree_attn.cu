@@ -271,10 +271,15 @@ Choice choose(const b200_tree_attn_params* p) {
   const int64_t rows = p->tokens * (p->heads / p->cache.kv_heads);
   const int64_t group = p->heads / p->cache.kv_heads;
   // More than 16 rows: the tcgen05 kernel, unless its boxes would be small, where each box
-  // costs more than its bytes: 32 rows over 131001 keys take 100 us with boxes of 64 keys,
-  // 141 us with boxes of 16; the few-row kernel 128 us with either.  Up to 16 rows the
-  // few-row kernel reads at the rate of memory (16 rows: 100 us, 4 rows: 92 us).
-  if (rows > 16 && group <= 128 && by_tensor_maps(p, rows > 32 ? 8 : 32)) {
+  // costs more than its bytes: 32 rows over 131001 keys take 97 us with boxes of 64 keys,
+  // 141 us with boxes of 16; the few-row kernel 128 us with either.  Where the slots hold
+  // short contexts only, the ends of units weigh more, and there the tcgen05 kernel is ahead
+  // with boxes of 16 too (64 sequences of up to 400 tokens, 32 rows: 47 us against 62 us; 16
+  // of up to 3000: 50 us with either; 32 of up to 8000: 186 us against 168 us).
+  // Up to 16 rows the few-row kernel reads at the rate of memory (16 rows: 100 us, 4
+  // rows: 92 us).
+  const int64_t least = rows > 32 ? 8 : p->cache.slots * p->cache.page_size <= 2048 ? 16 : 32;
+  if (rows > 16 && group <= 128 && by_tensor_maps(p, least)) {
     // whole tokens to a tile of 128 places
     const int tile = static_cast<int>(128 / group * group);
     if (rows <= tile) return Choice{kManyRows, 128, tile, 128, dp, 1};

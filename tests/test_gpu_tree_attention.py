@@ -79,6 +79,25 @@ def test_page_sizes(dtype, page):
     check(args, random_tree(9, torch.Generator().manual_seed(page)))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [40, 72, 128])
+@pytest.mark.parametrize("T,group", [(17, 1), (8, 4)])
+def test_a_wider_table_changes_nothing(dtype, D, T, group):
+    """Slots for more than 2048 keys change the kernel for 17 to 32 rows: both are within the
+    bound of the same values, so within two of each other."""
+    gen = torch.Generator().manual_seed(D)
+    q, k, v, table, lens = make([0, 20, 190, 333], T, 2, group, D, 16, dtype, seed=D + T)
+    mask = torch.stack([random_tree(T, gen) for _ in range(4)])
+    wide = torch.full((4, 130), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    want, size, grow = attention64(q, k, v, table, lens, mask)
+    bound = attention_bound(dtype, want, size, grow, D, 333 + T)
+    got = [b200_tree_attention(q.cuda(), k.cuda(), v.cuda(), t.cuda(), lens.cuda(), mask.cuda())
+           for t in (table, wide)]
+    assert read_device_errors(got[0].device) == 0
+    assert ((got[0].cpu().double() - got[1].cpu().double()).abs() <= 2 * bound).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("T,group,kv_heads", [(33, 1, 2), (16, 4, 1), (31, 3, 1), (64, 2, 1), (65, 4, 1),
                                               (130, 1, 1)])

@@ -144,8 +144,8 @@ typedef struct b200_tree_attn_params {
   int64_t workspace_bytes;
   /* Optional B200_TREE_ATTN_COUNTERS int32 in device memory, zero before the first
    * call and left zero by every call, for calls that do not overlap in time (one
-   * stream's): a call of few rows then joins its partial results in the same kernel
-   * instead of a second one. */
+   * stream's): most calls of few rows then join their partial results in the same
+   * kernel instead of a second one. */
   int32_t* counters;
 } b200_tree_attn_params;
 

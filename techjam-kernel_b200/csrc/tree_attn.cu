@@ -276,7 +276,7 @@ Choice choose(const b200_tree_attn_params* p) {
   // short contexts only, the ends of units weigh more, and there the tcgen05 kernel is ahead
   // with boxes of 16 too (64 sequences of up to 400 tokens, 32 rows: 47 us against 62 us; 16
   // of up to 3000: 50 us with either; 32 of up to 8000: 186 us against 168 us).
-  // Up to 16 rows the few-row kernel reads at the rate of memory (16 rows: 100 us, 4
+  // Up to 16 rows the few-row kernel reads near the rate of memory (16 rows: 103 us, 4
   // rows: 92 us).
   const int64_t least = rows > 32 ? 8 : p->cache.slots * p->cache.page_size <= 2048 ? 16 : 32;
   if (rows > 16 && group <= 128 && by_tensor_maps(p, least)) {
@@ -300,6 +300,16 @@ int64_t units_of(const b200_tree_attn_params* p, const Choice& c) {
 
 constexpr int64_t kMaxRuns = 148 * 8;
 
+// Whether the cut units of few rows get a join kernel of their own although the attention
+// kernel could join them: a long context of several rows leaves many partial results to the one
+// CTA that would (one sequence, 16 rows: 33.8 us against 23.4 us at 4000 keys, 19.6 against 18.6
+// at 1000, 112 against 103 at 131001; 4 sequences of 4000: 26.4 against 24.2).  For short contexts the second launch costs
+// more (500 keys, 8 rows: 15.0 us against 17.0 us).
+bool join_apart(const b200_tree_attn_params* p, const Choice& c, int64_t runs, int64_t units) {
+  return c.kernel != kManyRows && p->tokens * (p->heads / p->cache.kv_heads) > 4 &&
+         p->cache.slots * p->cache.page_size >= 12 * c.tn && runs >= 8 * units;
+}
+
 // CTAs of a call on a GPU of `sms` SMs: no more than there can be key tiles.
 int64_t runs_of(const b200_tree_attn_params* p, const Choice& c, int64_t sms) {
   const int64_t keys = p->cache.slots * p->cache.page_size;
@@ -316,7 +326,10 @@ int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
 
 
 template <int RM, int DP, int DT, int WARPS>
-int32_t run_join_rows(const Args& a, int64_t units, cudaStream_t s) {
+int32_t run_join_rows(const Args& a, int64_t units, bool spread, cudaStream_t s) {
+  if (spread)
+    return launch(join_spread_kernel<RM, DP, DT>, dim3(static_cast<unsigned>(units), RM / 4),
+                  dim3(32 * kJoinWarps), 0, s, a);
   return launch(join_rows_kernel<RM, DP, DT, WARPS>, dim3(static_cast<unsigned>(units)),
                 dim3(32 * WARPS), 0, s, a);
 }
@@ -348,13 +361,13 @@ int32_t run_one(void (*kernel)(Args), int threads, int smem, const Args& a, int 
 // One kernel over the runs, and where it does not join the units that were cut, one that
 // does.
 template <int DP, int DT>
-int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int device,
+int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, bool spread, int device,
                   cudaStream_t s) {
   int32_t rc;
   if constexpr (DT == B200_ATTN_DTYPE_FP32) {
     rc = run_one<16, DP, DT>(plain_kernel<DP, DT>, kThreads, sizeof(PlainSmem<DP>), a, runs, device,
                              s);
-    return rc != B200_ATTN_OK || a.counters ? rc : run_join_rows<kRows, DP, DT, kThreads / 32>(a, units, s);
+    return rc != B200_ATTN_OK || a.counters ? rc : run_join_rows<kRows, DP, DT, kThreads / 32>(a, units, spread, s);
   } else {
     using Few = RowShape<1, true, DP>;
     using One = RowShape<1, false, DP>;
@@ -371,8 +384,8 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
                                s);
     if (rc != B200_ATTN_OK || a.counters) return rc;
     switch (c.rm) {
-      case 16: return run_join_rows<16, DP, DT, One::kWarps>(a, units, s);
-      case 32: return run_join_rows<32, DP, DT, Two::kWarps>(a, units, s);
+      case 16: return run_join_rows<16, DP, DT, One::kWarps>(a, units, spread, s);
+      case 32: return run_join_rows<32, DP, DT, Two::kWarps>(a, units, spread, s);
       case 128: return run_join_columns<128, DP, DT>(a, units, s);
       default: return run_join_columns<256, DP, DT>(a, units, s);
     }
@@ -380,10 +393,10 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, int d
 }
 
 template <int DT>
-int32_t run_type(const Choice& c, const Args& a, int runs, int64_t units, int device,
+int32_t run_type(const Choice& c, const Args& a, int runs, int64_t units, bool spread, int device,
                  cudaStream_t s) {
-  return c.dp == 64 ? run_width<64, DT>(c, a, runs, units, device, s)
-                    : run_width<128, DT>(c, a, runs, units, device, s);
+  return c.dp == 64 ? run_width<64, DT>(c, a, runs, units, spread, device, s)
+                    : run_width<128, DT>(c, a, runs, units, spread, device, s);
 }
 
 }  // namespace
@@ -476,16 +489,17 @@ extern "C" int32_t b200_tree_attn_fwd(const b200_tree_attn_params* p, void* stre
   a.scale_log2 = p->scale * 1.4426950408889634f;
   a.desc = static_cast<int2*>(p->workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + desc_bytes(p, ch));
-  if (ch.kernel != kManyRows && units_of(p, ch) <= B200_TREE_ATTN_COUNTERS) a.counters = p->counters;
   const int runs = static_cast<int>(runs_of(p, ch, b200paged::sm_count(scope.device)));
   const int64_t units = units_of(p, ch);
+  const bool spread = join_apart(p, ch, runs, units);
+  if (ch.kernel != kManyRows && !spread && units <= B200_TREE_ATTN_COUNTERS) a.counters = p->counters;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (c.dtype) {
     case B200_ATTN_DTYPE_BF16:
-      return run_type<B200_ATTN_DTYPE_BF16>(ch, a, runs, units, scope.device, s);
+      return run_type<B200_ATTN_DTYPE_BF16>(ch, a, runs, units, spread, scope.device, s);
     case B200_ATTN_DTYPE_FP16:
-      return run_type<B200_ATTN_DTYPE_FP16>(ch, a, runs, units, scope.device, s);
+      return run_type<B200_ATTN_DTYPE_FP16>(ch, a, runs, units, spread, scope.device, s);
     default:
-      return run_type<B200_ATTN_DTYPE_FP32>(ch, a, runs, units, scope.device, s);
+      return run_type<B200_ATTN_DTYPE_FP32>(ch, a, runs, units, spread, scope.device, s);
   }
 }

@@ -16,7 +16,7 @@
 // a warp is enough here: on 64 sequences of up to 16 thousand keys (8 rows) the tensor
 // pipe is active 18 % of the time, and the fifth-generation one has no tile below 64 rows.
 // Measured (bf16, D 128, 8 key heads): those 64 sequences, 1.07 GB, 172 us = 6.2 TB/s, 96 %
-// of the rate of a plain copy; 16 rows over 131001 keys, 537 MB, 99 us in short runs, of
+// of the rate of a plain copy; 16 rows over 131001 keys, 537 MB, 103 us, of
 // which about 10 are the joins of the units cut over 37 CTAs each; one token over 1000 keys
 // 13 us, which is the launch, one chain of dependent loads (length, table, keys) and
 // the join.  Prefetching the next blocks into L2 by bulk instructions instead of a deep ring:

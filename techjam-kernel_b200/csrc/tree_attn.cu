@@ -270,15 +270,17 @@ Choice choose(const b200_tree_attn_params* p) {
   if (p->cache.dtype == B200_ATTN_DTYPE_FP32) return Choice{kPlain, kRows, kRows, kKeys, dp, dp == 64 ? 4 : 2};
   const int64_t rows = p->tokens * (p->heads / p->cache.kv_heads);
   const int64_t group = p->heads / p->cache.kv_heads;
-  // More than 16 rows: the tcgen05 kernel, unless its boxes would be small, where each box
-  // costs more than its bytes: 32 rows over 131001 keys take 97 us with boxes of 64 keys,
-  // 141 us with boxes of 16; the few-row kernel 128 us with either.  Where the slots hold
-  // short contexts only, the ends of units weigh more, and there the tcgen05 kernel is ahead
-  // with boxes of 16 too (64 sequences of up to 400 tokens, 32 rows: 47 us against 62 us; 16
-  // of up to 3000: 50 us with either; 32 of up to 8000: 186 us against 168 us).
+  // More than 16 rows: the tcgen05 kernel, unless its boxes would be so small that issuing
+  // them takes longer than their bytes.  Up to 32 rows, D 128: ahead of the few-row kernel
+  // with boxes of 8 keys already (131001 keys: 143 us against 166 us; 64 sequences of 3000 to
+  // 8000 keys: 333 against 444; of up to 400: 51 against 64).  D 64: behind with boxes of
+  // 16 (64 sequences of 3000 to 8000: 258 us against 222 us), but not where the slots hold
+  // short contexts only, whose ends of units weigh more (64 of up to 400: 45 us against 46
+  // us with boxes of 8).
   // Up to 16 rows the few-row kernel reads near the rate of memory (16 rows: 103 us, 4
   // rows: 92 us).
-  const int64_t least = rows > 32 ? 8 : p->cache.slots * p->cache.page_size <= 2048 ? 16 : 32;
+  const bool eight = rows > 32 || dp == 128 || p->cache.slots * p->cache.page_size <= 2048;
+  const int least = eight ? 8 : 32;
   if (rows > 16 && group <= 128 && by_tensor_maps(p, least)) {
     // whole tokens to a tile of 128 places
     const int tile = static_cast<int>(128 / group * group);

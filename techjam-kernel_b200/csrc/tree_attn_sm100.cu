@@ -15,8 +15,8 @@
 // tensor pipe and exponential unit are each active under half of the time.
 // 64 rows over 131001 keys: 537 MB, 97 us, 5.5 TB/s.  Short
 // contexts (5 sequences of 601 to 5003 keys, 63 rows a head, fp16, pages of 48: 28 us against
-// 6 us of bytes) are bound by the ends of a unit (queries in, results out) and by boxes
-// of 16 rows at about 165 cycles a box.
+// 6 us of bytes) are bound by the ends of a unit (queries in, results out) and by
+// issuing boxes of 16 rows.
 // Scores of half a tile (64 keys) in buffers of their own: 260 us against 228 us then.
 //
 // A CTA owns one run of the line of key tiles (tree_attn.cuh).  Twelve warps:
@@ -365,11 +365,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
         x.page = a.pages;
       }
-      if (lane == 0) ptx::mbar_arrive_expect_tx(bar(S::kBarFull + s), S::kTileBytes);
+      const uint32_t at = sbase + S::kOffRing + s * S::kTileBytes;
+      const uint32_t full = bar(S::kBarFull + s);
+      if (elect_one()) ptx::mbar_arrive_expect_tx(full, S::kTileBytes);
       __syncwarp();
-      if (mine)
-        ptx::tma_load_4d(sbase + S::kOffRing + s * S::kTileBytes + part, map, bar(S::kBarFull + s),
-                         64 * chunk, x.row, x.head, x.page);
+      if (S::kChunks == 1 || boxes <= 2) {
+        if (mine)
+          ptx::tma_load_4d(at + part, map, full, 64 * chunk, x.row, x.head, x.page);
+        return true;
+      }
+      // Many small boxes: one lane issues them all, four boxes of both halves of a row
+      // at a time from uniform registers; with a lane each the producer, not the memory,
+      // set the pace (64 rows over 131001 keys in pages of 16: 141 us against 116 us;
+      // large boxes and D = 64: 1 to 3 % the other way).
+      const int head = __shfl_sync(0xffffffffu, x.head, 0);
+#pragma unroll 1
+      for (int i = 0; i < boxes; i += 4) {
+        int row[4], page[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          row[y] = __shfl_sync(0xffffffffu, x.row, i + y);
+          page[y] = __shfl_sync(0xffffffffu, x.page, i + y);
+        }
+        if (elect_one()) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+              ptx::tma_load_4d(at + c * S::kChunkBytes + (i + y) * box_rows * 128, map, full, 64 * c,
+                               row[y], head, page[y]);
+        }
+        __syncwarp();
+      }
       return true;
     };
     // The page numbers of a tile are read while the loads before it are issued, and

@@ -83,8 +83,8 @@ def test_page_sizes(dtype, page):
 @pytest.mark.parametrize("D", [40, 72, 128])
 @pytest.mark.parametrize("T,group", [(17, 1), (8, 4)])
 def test_a_wider_table_changes_nothing(dtype, D, T, group):
-    """Slots for more than 2048 keys change the kernel for 17 to 32 rows: both are within the
-    bound of the same values, so within two of each other."""
+    """Slots for more than 2048 keys change the kernel for 17 to 32 rows of narrow heads: both are
+    within the bound of the same values, so within two of each other."""
     gen = torch.Generator().manual_seed(D)
     q, k, v, table, lens = make([0, 20, 190, 333], T, 2, group, D, 16, dtype, seed=D + T)
     mask = torch.stack([random_tree(T, gen) for _ in range(4)])
@@ -94,6 +94,30 @@ def test_a_wider_table_changes_nothing(dtype, D, T, group):
     bound = attention_bound(dtype, want, size, grow, D, 333 + T)
     got = [b200_tree_attention(q.cuda(), k.cuda(), v.cuda(), t.cuda(), lens.cuda(), mask.cuda())
            for t in (table, wide)]
+    assert read_device_errors(got[0].device) == 0
+    assert ((got[0].cpu().double() - got[1].cpu().double()).abs() <= 2 * bound).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [40, 72, 128])
+@pytest.mark.parametrize("T,group", [(17, 1), (8, 4), (25, 3)])
+def test_the_page_size_changes_nothing(dtype, D, T, group):
+    """Odd pages go to the kernel of few rows in several row tiles, pages of 16 to that of
+    many rows: both are within the bound of the same values, so within two of each other."""
+    gen = torch.Generator().manual_seed(D)
+    lens_of = [0, 20, 190, 333]
+    q, k, v, table, lens = make(lens_of, T, 2, group, D, 16, dtype, seed=D + T + 1)
+    mask = torch.stack([random_tree(T, gen) for _ in range(4)])
+    other = make(lens_of, T, 2, group, D, 7, dtype, seed=D + T + 1)
+    for b, n in enumerate(lens_of):
+        for t in range(n + T):
+            here, there = table[b, t // 16], other[3][b, t // 7]
+            other[1][there, :, t % 7] = k[here, :, t % 16]
+            other[2][there, :, t % 7] = v[here, :, t % 16]
+    want, size, grow = attention64(q, k, v, table, lens, mask)
+    bound = attention_bound(dtype, want, size, grow, D, 333 + T)
+    got = [b200_tree_attention(q.cuda(), *(x.cuda() for x in c), lens.cuda(), mask.cuda())
+           for c in ((k, v, table), other[1:4])]
     assert read_device_errors(got[0].device) == 0
     assert ((got[0].cpu().double() - got[1].cpu().double()).abs() <= 2 * bound).all()
 

@@ -6,8 +6,8 @@
 // running maximum and sum.  What bounds it: R rows do 4 R D operations for the 4 D
 // bytes of a key and value, so from about 260 rows the tensor cores, below it
 // HBM.  Measured (bf16, D 128): 32 sequences of 1 to 8 thousand keys, 8 key heads, 256
-// rows, 638 MB and 153 GFLOP: 181 us in short runs (845 TFLOP/s, half of the
-// tensor cores' measured rate and of the memory's), 217 us back to back, where
+// rows, 638 MB and 153 GFLOP: 183 us in short runs (836 TFLOP/s, half of the
+// tensor cores' measured rate and of the memory's), 209 us back to back, where
 // the board's power limit lowers the clock; DRAM reads are the
 // cache's bytes exactly.  A key tile of 256 rows takes about 4000 cycles, in which a softmax
 // group waits for its scores (570 cycles of products and 300 to be seen), copies them (400),

@@ -820,8 +820,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                       pack2<DT>(acc[8 * e + 4] * inv, acc[8 * e + 5] * inv),
                       pack2<DT>(acc[8 * e + 6] * inv, acc[8 * e + 7] * inv));
             }
-          } else {
-            // a column of rows at a time
+          } else if (mine) {
+            // A column of rows at a time.  Own rows only: where the head group does not divide
+            // 128 a group's share is less than its 128 lanes, and the places of the lanes past
+            // it are the other group's first rows.
 #pragma unroll
             for (int e = 0; e < 32; ++e) part[(col + e) * RM + row0 + rl] = acc[e];
           }

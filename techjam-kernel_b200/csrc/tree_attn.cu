@@ -492,6 +492,7 @@ extern "C" int32_t b200_tree_attn_fwd(const b200_tree_attn_params* p, void* stre
   a.desc = static_cast<int2*>(p->workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + desc_bytes(p, ch));
   const int runs = static_cast<int>(runs_of(p, ch, b200paged::sm_count(scope.device)));
+  a.runs = runs;
   const int64_t units = units_of(p, ch);
   const bool spread = join_apart(p, ch, runs, units);
   if (ch.kernel != kManyRows && !spread && units <= B200_TREE_ATTN_COUNTERS) a.counters = p->counters;

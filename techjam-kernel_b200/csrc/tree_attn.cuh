@@ -48,6 +48,7 @@ struct Args {
   int32_t row_tiles;  // of a full draft: the stride of unit numbers
   float scale_log2;
   int2* desc;       // [batch * kv_heads * row_tiles] first and last run of a unit
+  int32_t runs;     // CTAs of the attention kernel
   int32_t* counters;  // null, or one a unit, zero between calls
   float* partial;   // [2 * runs] x {sums [RM][DP], maximum [RM], sum [RM]}
   int32_t* err;
@@ -58,17 +59,22 @@ struct Seq {
   int32_t len, drafts;
 };
 
+// Without a report; false: out of range, and the sequence has no unit.
+__device__ __forceinline__ bool read_seq(const Args& a, int b, Seq* s) {
+  s->len = a.lens[b];
+  s->drafts = a.drafts ? a.drafts[b] : a.tokens;
+  const int64_t room = static_cast<int64_t>(a.slots) * a.page_size;
+  if (s->len >= 0 && s->drafts >= 0 && s->drafts <= a.tokens &&
+      (s->drafts == 0 || static_cast<int64_t>(s->len) + s->drafts <= room))
+    return true;
+  s->len = 0;
+  s->drafts = 0;
+  return false;
+}
+
 __device__ __forceinline__ Seq seq_of(const Args& a, int b) {
   Seq s;
-  s.len = a.lens[b];
-  s.drafts = a.drafts ? a.drafts[b] : a.tokens;
-  const int64_t room = static_cast<int64_t>(a.slots) * a.page_size;
-  if (s.len < 0 || s.drafts < 0 || s.drafts > a.tokens ||
-      (s.drafts > 0 && static_cast<int64_t>(s.len) + s.drafts > room)) {
-    report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
-    s.len = 0;
-    s.drafts = 0;
-  }
+  if (!read_seq(a, b, &s)) report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
   return s;
 }
 
@@ -382,17 +388,20 @@ struct Joint {
   int b, h, rt;
 };
 
+// False: nothing to join.  Units of sequences that were left out have no entry, and a CTA
+// whose wait ran out leaves its units without one: what the workspace held before is not
+// taken for a range of runs.
 __device__ __forceinline__ bool joint_of(const Args& a, int row0, Joint* j) {
   const int unit = blockIdx.x, bh = unit / a.row_tiles;
   j->rt = unit % a.row_tiles;
   j->b = bh / a.kv_heads;
   j->h = bh % a.kv_heads;
   j->row0 = row0;
-  const int drafts = a.drafts ? a.drafts[j->b] : a.tokens;
-  j->rows = min(a.unit_rows, drafts * a.group - j->rt * a.unit_rows);
-  if (row0 >= j->rows || drafts > a.tokens) return false;
   j->runs = a.desc[unit];
-  return j->runs.x < j->runs.y;
+  Seq s;
+  read_seq(a, j->b, &s);
+  j->rows = min(a.unit_rows, s.drafts * a.group - j->rt * a.unit_rows);
+  return row0 < j->rows && j->runs.x >= 0 && j->runs.x < j->runs.y && j->runs.y < a.runs;
 }
 
 // The partial result of run c: the unit's first run kept it in its second place (the

@@ -87,7 +87,11 @@ __global__ void __launch_bounds__(kCopyThreads) append_kernel(const Pool c, cons
   const int x = static_cast<int>(rest) - h * c.chunks;
   if (r.counts && j >= r.counts[b]) return;
   const int len = c.lens[b];
-  const uint32_t at = static_cast<uint32_t>(len) + j;  // a negative length lands past all slots
+  if (len < 0) {  // len + j would wrap round to the first tokens
+    report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
+    return;
+  }
+  const uint32_t at = static_cast<uint32_t>(len) + j;
   const uint32_t slot = at / static_cast<uint32_t>(c.page_size);
   const int page = page_at(c, b, slot);
   if (page < 0) return;

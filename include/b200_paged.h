@@ -73,7 +73,8 @@ typedef struct b200_cache_rows {
   int64_t tokens;        /* rows given for each sequence */
   int64_t k_stride[4];   /* layer, sequence, head, token: elements */
   int64_t v_stride[4];
-  const int32_t* counts; /* optional [batch]: rows of each sequence that are written */
+  const int32_t* counts; /* optional [batch]: rows of each sequence that are written, 0..tokens
+                            (a sequence with another number is skipped and reported) */
 } b200_cache_rows;
 
 /* Host-only validation of the cache description.  Makes no CUDA call. */

@@ -85,9 +85,11 @@ __global__ void __launch_bounds__(kCopyThreads) append_kernel(const Pool c, cons
   rest -= j * per_tok;
   const int h = static_cast<int>(rest / static_cast<uint32_t>(c.chunks));
   const int x = static_cast<int>(rest) - h * c.chunks;
-  if (r.counts && j >= r.counts[b]) return;
+  const int count = r.counts ? r.counts[b] : r.tokens;
   const int len = c.lens[b];
-  if (len < 0) {  // len + j would wrap round to the first tokens
+  const bool given = count >= 0 && count <= r.tokens;
+  if (given && j >= count) return;
+  if (!given || len < 0) {  // (len + j would wrap round to the first tokens)
     report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
     return;
   }

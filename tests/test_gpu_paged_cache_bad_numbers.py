@@ -45,3 +45,15 @@ def test_append_skips_negative_lengths(dtype, negative):
     m.append(k_new, v_new, [0, 0, 9])
     m.lens[2] = 0
     m.check(c.k_pages, c.v_pages, c.page_table, c.seq_lens, c.page_refs)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("counts", [(6, -1, 2), (1 << 30, -(1 << 31), 5), (6, 7, 0)])
+def test_append_skips_counts_of_rows_that_were_not_given(dtype, counts):
+    c = filled(2, 20, 2, 4, 16, 3, 4, dtype)
+    assert int(c.reserve(12)) == 0
+    m = model_of(c)
+    k_new, v_new = rows_of(c, 5, 2)
+    reported(c, lambda: b200_cache_append(k_new, v_new, c.k_pages, c.v_pages, c.page_table, c.seq_lens, i32(counts)))
+    m.append(k_new, v_new, [0, 0, counts[2]])
+    m.check(c.k_pages, c.v_pages, c.page_table, c.seq_lens, c.page_refs)

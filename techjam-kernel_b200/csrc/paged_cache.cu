@@ -142,7 +142,8 @@ __global__ void __launch_bounds__(kCopyThreads)
   const int x = static_cast<int>(rest) - h * c.chunks;
   const int len = c.lens[b];
   int n = counts[b];
-  if (n < 0 || n > width || len < 0) {
+  const int64_t room = static_cast<int64_t>(c.slots) * c.page_size;
+  if (n < 0 || n > width || len < 0 || (n > 0 && static_cast<int64_t>(len) + n > room)) {
     report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
     n = 0;
   }

@@ -57,3 +57,19 @@ def test_append_skips_counts_of_rows_that_were_not_given(dtype, counts):
     reported(c, lambda: b200_cache_append(k_new, v_new, c.k_pages, c.v_pages, c.page_table, c.seq_lens, i32(counts)))
     m.append(k_new, v_new, [0, 0, counts[2]])
     m.check(c.k_pages, c.v_pages, c.page_table, c.seq_lens, c.page_refs)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("paths", [[0, 1, 2, 3], [1, 2, 3, 4]])
+def test_accept_does_not_grow_a_sequence_past_its_slots(dtype, paths):
+    """The length stays as it is, and no row moves; a sequence may fill its slots exactly."""
+    c = filled(2, 20, 2, 4, 16, 4, 4, dtype)
+    assert int(c.reserve(16)) == 0
+    c.seq_lens.copy_(i32([14, 16, 2, 12 if paths[0] == 0 else 11]))
+    m = model_of(c)
+    counts = i32([3, 1, 2, 4])
+    got = reported(c, lambda: b200_cache_accept(c.k_pages, c.v_pages, c.page_table, c.seq_lens,
+                                                i32([paths] * 4), counts))
+    want = m.accept([paths] * 4, [0, 0, 2, 4])
+    assert got.tolist() == want.tolist()
+    m.check(c.k_pages, c.v_pages, c.page_table, c.seq_lens, c.page_refs)

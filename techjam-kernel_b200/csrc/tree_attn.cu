@@ -300,7 +300,10 @@ int64_t units_of(const b200_tree_attn_params* p, const Choice& c) {
   return p->cache.batch * p->cache.kv_heads * row_tiles(p, c);
 }
 
-constexpr int64_t kMaxRuns = 148 * 8;
+// Most SMs that a call runs on.  Workspaces are sized on the host for as many, without asking
+// a device: more than the 148 of a B200, and every one counts (256 rows of 128 columns: 42.6 MB
+// for 160 SMs).
+constexpr int64_t kMaxSms = 160;
 
 // Whether the cut units of few rows get a join kernel of their own although the attention
 // kernel could join them: a long context of several rows leaves many partial results to the one
@@ -318,7 +321,7 @@ int64_t runs_of(const b200_tree_attn_params* p, const Choice& c, int64_t sms) {
   const double tiles = static_cast<double>(p->cache.batch * p->cache.kv_heads) *
                        static_cast<double>(row_tiles(p, c)) *
                        static_cast<double>((keys + c.tn - 1) / c.tn);
-  const int64_t most = sms * c.ctas_per_sm < kMaxRuns ? sms * c.ctas_per_sm : kMaxRuns;
+  const int64_t most = (sms < kMaxSms ? sms : kMaxSms) * c.ctas_per_sm;
   return tiles < static_cast<double>(most) ? static_cast<int64_t>(tiles) : most;
 }
 
@@ -438,7 +441,7 @@ extern "C" int32_t b200_tree_attn_check(const b200_tree_attn_params* p) {
 extern "C" int64_t b200_tree_attn_workspace_bytes(const b200_tree_attn_params* p) {
   if (b200_tree_attn_check(p) != B200_ATTN_OK) return 0;
   const Choice c = choose(p);
-  return desc_bytes(p, c) + 2 * runs_of(p, c, kMaxRuns) * 4 * c.rm * (c.dp + 2);
+  return desc_bytes(p, c) + 2 * runs_of(p, c, kMaxSms) * 4 * c.rm * (c.dp + 2);
 }
 
 extern "C" int32_t b200_tree_attn_fwd(const b200_tree_attn_params* p, void* stream) {

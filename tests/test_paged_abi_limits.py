@@ -1,0 +1,30 @@
+"""Sizes, limits and overlaps that the C entries of the paged cache look at on the host (no GPU
+needed: nothing here is launched)."""
+
+import ctypes
+
+import pytest
+
+from b200_attention import _native
+from test_paged_abi import INVALID, OK, attn, cache, lib  # noqa: F401 (lib is a fixture)
+
+
+@pytest.mark.parametrize("batch,slots,page,heads,group,D,tokens,rows", [
+    (32, 128, 64, 8, 4, 128, 64, 256),
+    (1, 2048, 64, 8, 4, 128, 64, 256),
+    (1, 2048, 64, 8, 4, 128, 16, 128),
+    (64, 512, 16, 8, 4, 128, 1, 16),
+    (5, 512, 7, 16, 1, 64, 30, 32),
+])
+def test_workspace_is_that_of_the_runs_of_one_gpu(lib, batch, slots, page, heads, group, D, tokens, rows):  # noqa: F811
+    """Two partial results of up to 256 rows for each CTA, on 160 SMs at most (two CTAs an SM
+    for up to 16 rows), and 8 bytes a unit."""
+    row, head = D, page * D
+    kw = dict(batch=batch, slots=slots, table_stride=slots, page_size=page, kv_heads=heads, head_dim=D, pages=4096,
+              k_stride=(0, heads * head, head, row), v_stride=(0, heads * head, head, row))
+    t = attn(cache_kw=kw, heads=heads * group, tokens=tokens,
+             q_stride=(heads * group * tokens * D, tokens * D, D), o_stride=(heads * group * tokens * D, tokens * D, D))
+    size = lib.b200_tree_attn_workspace_bytes(ctypes.byref(t))
+    ctas = 160 * (2 if rows == 16 else 1)
+    units = batch * heads * -(-tokens * group // rows)
+    assert 0 < size <= 2 * ctas * 4 * rows * (D + 2) + 8 * units + 16

@@ -606,8 +606,9 @@ int32_t check_table(const b200_cache* c) {
   if (c->batch < 1 || c->batch > B200_CACHE_MAX_BATCH || c->slots < 1 || c->slots > (1ll << 24) ||
       c->pages < 1 || c->pages > (1ll << 30) || c->page_size < 1 || c->page_size > (1ll << 20))
     return B200_ATTN_ERR_INVALID_ARGUMENT;
-  // token positions and slot numbers fit 32 bits
-  if (c->slots * c->page_size > 0x3fffffffll || c->batch * c->slots > 0x7fffffffll)
+  // token positions and slot numbers fit 32 bits, the latter up to the end of the planning
+  // CTA's last round over them
+  if (c->slots * c->page_size > 0x3fffffffll || c->batch * c->slots > 0x7fffffffll - kPlanThreads)
     return B200_ATTN_ERR_INVALID_ARGUMENT;
   if (c->batch > 1 && c->table_stride < c->slots) return B200_ATTN_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(c->page_table) | reinterpret_cast<uintptr_t>(c->seq_lens) |

@@ -28,3 +28,14 @@ def test_workspace_is_that_of_the_runs_of_one_gpu(lib, batch, slots, page, heads
     ctas = 160 * (2 if rows == 16 else 1)
     units = batch * heads * -(-tokens * group // rows)
     assert 0 < size <= 2 * ctas * 4 * rows * (D + 2) + 8 * units + 16
+
+
+def test_the_table_has_room_for_the_numbering_of_its_slots(lib):  # noqa: F811
+    """The planning CTA steps over the slots wanted in rounds of 1024, in 32 bits: the end of
+    the last round has to be below 2^31."""
+    def check(batch, slots):
+        return lib.b200_cache_check(ctypes.byref(cache(batch=batch, slots=slots, table_stride=slots, page_size=1)))
+
+    assert 8192 * 262143 + 1024 < 1 << 31 and check(8192, 262143) == OK
+    assert 7282 * 294903 == (1 << 31) - 2 and check(7282, 294903) == INVALID
+    assert check(1, 1 << 24) == OK

@@ -656,6 +656,8 @@ extern "C" int32_t b200_cache_check(const b200_cache* c) {
   if (!c->k || !c->v || c->layers < 1 || c->layers > (1 << 15) || c->kv_heads < 1 ||
       c->kv_heads > (1 << 16))
     return B200_ATTN_ERR_INVALID_ARGUMENT;
+  // so are the pieces of a page in all layers that a move is cut into
+  if (2 * c->layers * c->kv_heads > 0x7fffffffll) return B200_ATTN_ERR_INVALID_ARGUMENT;
   if (!known_dtype(c->dtype) || c->head_dim < 8 || c->head_dim > 128 || c->head_dim % 8)
     return B200_ATTN_ERR_UNSUPPORTED;
   const int64_t extent[4] = {c->layers, c->pages, c->kv_heads, c->page_size};

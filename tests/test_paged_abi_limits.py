@@ -39,3 +39,14 @@ def test_the_table_has_room_for_the_numbering_of_its_slots(lib):  # noqa: F811
     assert 8192 * 262143 + 1024 < 1 << 31 and check(8192, 262143) == OK
     assert 7282 * 294903 == (1 << 31) - 2 and check(7282, 294903) == INVALID
     assert check(1, 1 << 24) == OK
+
+
+def test_rows_of_a_page_in_all_layers_are_numbered_in_32_bits(lib):  # noqa: F811
+    """Page moves number a page's (layer, keys or values, head) pieces in 32 bits."""
+    def check(layers, heads):
+        strides = (8 * heads, 8 * heads, 8, 8)
+        return lib.b200_cache_check(ctypes.byref(cache(layers=layers, kv_heads=heads, page_size=1, head_dim=8,
+                                                       k_stride=strides, v_stride=strides)))
+
+    assert check(1 << 15, (1 << 15) - 1) == OK
+    assert check(1 << 15, 1 << 15) == INVALID and check(1 << 15, 1 << 16) == INVALID

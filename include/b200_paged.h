@@ -90,9 +90,9 @@ B200_ATTN_API int32_t b200_cache_append(const b200_cache* c, const b200_cache_ro
 
 /* Keep counts[b] of the drafted tokens of sequence b: token seq_lens[b] + j
  * becomes the drafted token paths[b][j] (strictly increasing in j), in all
- * layers; new_lens[b] = seq_lens[b] + counts[b] (new_lens is not seq_lens).  A
- * sequence whose count is not in 0..width, or would not fit its slots, keeps its
- * length and is reported. */
+ * layers; new_lens[b] = seq_lens[b] + counts[b] (new_lens overlaps neither
+ * seq_lens nor the table, paths or counts).  A sequence whose count is not in
+ * 0..width, or would not fit its slots, keeps its length and is reported. */
 B200_ATTN_API int32_t b200_cache_accept(const b200_cache* c, const int32_t* paths, int64_t width,
                                         int64_t path_stride, const int32_t* counts,
                                         int32_t* new_lens, void* stream);

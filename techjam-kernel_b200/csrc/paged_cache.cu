@@ -20,6 +20,7 @@
 namespace b200paged {
 
 using b200attn::ByteRange;
+using b200attn::rows_range;
 using b200attn::report_error;
 
 namespace {
@@ -729,6 +730,13 @@ extern "C" int32_t b200_cache_accept(const b200_cache* c, const int32_t* paths, 
   if ((reinterpret_cast<uintptr_t>(paths) | reinterpret_cast<uintptr_t>(counts) |
        reinterpret_cast<uintptr_t>(new_lens)) & 3u)
     return B200_ATTN_ERR_ALIGNMENT;
+  // the new lengths must not lie where other blocks of the kernel still read
+  const ByteRange out = rows_range(new_lens, 1, c->batch, 0, 4);
+  if (out.overlaps(rows_range(c->seq_lens, 1, c->batch, 0, 4)) ||
+      out.overlaps(rows_range(counts, 1, c->batch, 0, 4)) ||
+      out.overlaps(rows_range(paths, c->batch, width, path_stride, 4)) ||
+      out.overlaps(rows_range(c->page_table, c->batch, c->slots, c->table_stride, 4)))
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
   DeviceScope scope;
   if ((rc = scope.enter(c->k, "the pools are not device memory")) != B200_ATTN_OK) return rc;
   Pool p = pool_of(c);

@@ -50,3 +50,17 @@ def test_rows_of_a_page_in_all_layers_are_numbered_in_32_bits(lib):  # noqa: F81
 
     assert check(1 << 15, (1 << 15) - 1) == OK
     assert check(1 << 15, 1 << 15) == INVALID and check(1 << 15, 1 << 16) == INVALID
+
+
+@pytest.mark.parametrize("out,code", [
+    (0x30000000 + 8, INVALID),    # the lengths
+    (0x30000000 - 8, INVALID),
+    (0x700 + 8, INVALID),         # the counts
+    (0x600 + 60, INVALID),        # the last entries of the paths
+    (0x20000000 + 92, INVALID),   # the page table
+])
+def test_accept_refuses_new_lengths_over_what_it_reads(lib, out, code):  # noqa: F811
+    """Blocks of one sequence read while those of another write."""
+    p = ctypes.c_void_p
+    got = lib.b200_cache_accept(ctypes.byref(cache()), p(0x600), 5, 6, p(0x700), p(out), None)
+    assert got == code

@@ -133,7 +133,7 @@ B200_ATTN_API int32_t b200_cache_compact(const b200_cache* c, int32_t* live, voi
 typedef struct b200_tree_attn_params {
   b200_cache cache;
   const void* q; /* [batch, heads, tokens, head_dim] */
-  void* o;
+  void* o;       /* may be q, element for element; overlaps no other input */
   int64_t heads;
   int64_t tokens;
   int64_t q_stride[3]; /* batch, head, token: elements; head_dim contiguous */

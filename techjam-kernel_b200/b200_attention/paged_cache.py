@@ -138,7 +138,8 @@ def b200_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
 
     bfloat16 and float16 products run on the tensor cores, float32 in fp32;
     maximum, sum and output sums are fp32 and the output is rounded once.  Returns
-    ``[B, H, T, D]``, or ``[B, T, H, D]`` with ``output_bshd``; ``out`` may supply it."""
+    ``[B, H, T, D]``, or ``[B, T, H, D]`` with ``output_bshd``; ``out`` may supply it; it
+    may be ``q`` itself, and shares no memory with another argument."""
     return _call("tree_attention", q.device, q, k_pages, v_pages, page_table, seq_lens, tree_mask,
                  draft_lens, scale, output_bshd, out)
 

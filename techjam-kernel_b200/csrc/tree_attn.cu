@@ -292,6 +292,35 @@ Choice choose(const b200_tree_attn_params* p) {
   return Choice{kFewRows, 32, 32, RowShape<2, false, 64>::kTile, dp, 1};
 }
 
+// Whether the output can share bytes with what the call reads, or with itself.  In the place
+// of the queries, element for element, it may: a unit's rows are written when all its CTAs have
+// read its queries.
+bool output_collides(const b200_tree_attn_params* p) {
+  using b200attn::may_overlap;
+  using b200attn::stretches_of;
+  const b200_cache& c = p->cache;
+  const int64_t eb = elem_bytes(c.dtype);
+  const int64_t rows[3] = {c.batch, p->heads, p->tokens};
+  const int64_t pool[3] = {c.pages, c.kv_heads, c.page_size};
+  bool in_place = p->q == p->o;
+  for (int d = 0; d < 3; ++d) {
+    if (rows[d] <= 1) continue;
+    if (p->o_stride[d] == 0) return true;
+    in_place = in_place && p->o_stride[d] == p->q_stride[d];
+  }
+  const auto o = stretches_of(p->o, p->o_stride, rows, 3, c.head_dim, eb);
+  if (!in_place && may_overlap(o, stretches_of(p->q, p->q_stride, rows, 3, c.head_dim, eb)))
+    return true;
+  if (may_overlap(o, stretches_of(c.k, c.k_stride + 1, pool, 3, c.head_dim, eb)) ||
+      may_overlap(o, stretches_of(c.v, c.v_stride + 1, pool, 3, c.head_dim, eb)) ||
+      may_overlap(o, stretches_of(c.page_table, &c.table_stride, &c.batch, 1, c.slots, 4)) ||
+      may_overlap(o, stretches_of(c.seq_lens, nullptr, nullptr, 0, c.batch, 4)))
+    return true;
+  const int64_t marks[3] = {c.batch, p->tokens, p->tokens};
+  return (p->mask && may_overlap(o, stretches_of(p->mask, p->mask_stride, marks, 3, 1, 1))) ||
+         (p->draft_lens && may_overlap(o, stretches_of(p->draft_lens, nullptr, nullptr, 0, c.batch, 4)));
+}
+
 int64_t row_tiles(const b200_tree_attn_params* p, const Choice& c) {
   return (p->tokens * (p->heads / p->cache.kv_heads) + c.rows - 1) / c.rows;
 }
@@ -435,6 +464,7 @@ extern "C" int32_t b200_tree_attn_check(const b200_tree_attn_params* p) {
     return B200_ATTN_ERR_INVALID_ARGUMENT;
   if (p->mask && (p->mask_stride[0] < 0 || p->mask_stride[1] < 0 || p->mask_stride[2] < 0))
     return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (output_collides(p)) return B200_ATTN_ERR_INVALID_ARGUMENT;
   return B200_ATTN_OK;
 }
 

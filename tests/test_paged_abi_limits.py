@@ -64,3 +64,53 @@ def test_accept_refuses_new_lengths_over_what_it_reads(lib, out, code):  # noqa:
     p = ctypes.c_void_p
     got = lib.b200_cache_accept(ctypes.byref(cache()), p(0x600), 5, 6, p(0x700), p(out), None)
     assert got == code
+
+
+def rows_at(q, o, q_stride, o_stride, **kw):
+    return attn(q=q, o=o, q_stride=q_stride, o_stride=o_stride, **kw)
+
+
+# attn(): 3 sequences, 8 heads, 5 tokens, D 64; a token of all heads is 1024 bytes
+HEAD_MAJOR, TOKEN_MAJOR = (8 * 5 * 64, 5 * 64, 64), (8 * 5 * 64, 64, 8 * 64)
+HALVES = (2 * 8 * 5 * 64, 64, 2 * 8 * 64)  # token-major, as one of two in a tensor
+SIZE = 3 * 8 * 5 * 64 * 2
+
+
+@pytest.mark.parametrize("q,o,qs,os,code", [
+    (0x70000000, 0x70000000, HEAD_MAJOR, HEAD_MAJOR, OK),        # in place, element for element
+    (0x70000000, 0x70000000, TOKEN_MAJOR, TOKEN_MAJOR, OK),
+    (0x70000000, 0x70000000, TOKEN_MAJOR, HEAD_MAJOR, INVALID),  # in place in another order
+    (0x70000000, 0x70000000 + 128, HEAD_MAJOR, HEAD_MAJOR, INVALID),
+    (0x70000000, 0x70000000 + SIZE - 16, HEAD_MAJOR, HEAD_MAJOR, INVALID),
+    (0x70000000, 0x70000000 + SIZE, HEAD_MAJOR, HEAD_MAJOR, OK),
+    (0x70000000 + SIZE, 0x70000000, HEAD_MAJOR, HEAD_MAJOR, OK),
+    (0x70000000, 0x70000000 + 1024, HALVES, HALVES, OK),         # side by side in one tensor
+    (0x70000000 + 1024, 0x70000000, HALVES, HALVES, OK),
+    (0x70000000, 0x70000000 + 1008, HALVES, HALVES, INVALID),
+    (0x70000000, 0x70000000 + 1040, HALVES, HALVES, INVALID),
+    (0x70000000, 0x70000000 + 1024, HALVES, HEAD_MAJOR, INVALID),
+    (0x70000000, 0x10000000 + 2048, HEAD_MAJOR, HEAD_MAJOR, INVALID),   # in the keys
+    (0x70000000, 0x100000000 - 128, HEAD_MAJOR, HEAD_MAJOR, INVALID),   # into the values
+    (0x70000000, 0x20000000 - SIZE + 16, HEAD_MAJOR, HEAD_MAJOR, INVALID),  # into the table
+    (0x70000000, 0x30000000 - SIZE + 16, HEAD_MAJOR, HEAD_MAJOR, INVALID),  # into the lengths
+    (0x70000000, 0x80000000, HEAD_MAJOR, (0, 5 * 64, 64), INVALID),     # one row for all sequences
+])
+def test_output_may_not_lie_over_the_inputs(lib, q, o, qs, os, code):  # noqa: F811
+    assert lib.b200_tree_attn_check(ctypes.byref(rows_at(q, o, qs, os))) == code
+
+
+def test_output_may_not_lie_over_the_mask_or_the_draft_lengths(lib):  # noqa: F811
+    mask = dict(mask=0x80000000 + 64, mask_stride=(0, 5, 1))
+    for kw, code in ((mask, INVALID), (dict(mask, mask=0x80000000 - 25), OK), (dict(mask, mask=0x80000000 - 24), INVALID),
+                     (dict(draft_lens=0x80000000 + SIZE), OK), (dict(draft_lens=0x80000000 + SIZE - 4), INVALID)):
+        assert lib.b200_tree_attn_check(ctypes.byref(attn(**kw))) == code
+
+
+def test_output_beside_the_pools_of_one_tensor(lib):  # noqa: F811
+    """Keys, values and an output in the same rows of one tensor do not overlap."""
+    # a row of 3 x 64 elements: keys, values, output; pages of 16 rows, 4 heads
+    kw = dict(k=0x10000000, v=0x10000080, k_stride=(0, 4 * 16 * 192, 16 * 192, 192),
+              v_stride=(0, 4 * 16 * 192, 16 * 192, 192))
+    strides = (8 * 5 * 192, 5 * 192, 192)
+    assert lib.b200_tree_attn_check(ctypes.byref(attn(cache_kw=kw, o=0x10000100, o_stride=strides))) == OK
+    assert lib.b200_tree_attn_check(ctypes.byref(attn(cache_kw=kw, o=0x10000080, o_stride=strides))) == INVALID

@@ -19,6 +19,7 @@ work in place on the tensors given, so a step can be captured in a CUDA graph.
 Results do not depend on execution order: free pages are given out lowest
 number first, in (sequence, slot) order.
 
+Inference only: tensors that ask for gradients are refused.
 Shapes, types and devices are checked on the host (``ValueError`` / ``TypeError``).
 Page numbers, lengths and sequence numbers lie on the device; a bad one skips its
 access there and is reported like every device error of this package (the next

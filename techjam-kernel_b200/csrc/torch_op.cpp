@@ -227,6 +227,8 @@ b200_cache cache_view(const at::Tensor& k, const at::Tensor& v, const at::Tensor
   TORCH_CHECK_VALUE(k.stride(d + 3) == 1 && v.stride(d + 3) == 1,
                     "the pools must have a contiguous last dimension");
   TORCH_CHECK_VALUE(k.numel() > 0, "the pools must not be empty");
+  TORCH_CHECK_VALUE(!(c10::GradMode::is_enabled() && (k.requires_grad() || v.requires_grad())),
+                    "the paged cache is inference-only (autograd requested)");
   TORCH_CHECK_VALUE(!refs.has_value() || c.pages == k.size(d), "page_refs must have one count for "
                     "each of the ", k.size(d), " pages, got ", c.pages);
   TORCH_CHECK_VALUE(k.size(d + 3) % 8 == 0 && k.size(d + 3) <= 128, "head_dim ", k.size(d + 3),

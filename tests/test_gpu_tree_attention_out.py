@@ -42,3 +42,26 @@ def test_not_over_other_inputs():
                          (q, v.view(-1)[-q.numel():].view(q.shape)), (q, other[:1, :, :4].expand(2, 4, 4, 64))):
         with pytest.raises(ValueError):
             b200_tree_attention(queries, k, v, table, lens, out=out)
+
+
+def test_gradients_through_a_cache_are_refused():
+    """Of queries, pools and rows alike: the result would have none."""
+    from b200_attention import b200_cache_accept, b200_cache_append, b200_cache_compact, b200_cache_reserve
+
+    q, k, v, table, lens = (t.cuda() for t in make([40, 50], 1, 2, 2, 64, 16, torch.bfloat16))
+    refs = torch.ones(k.shape[0], dtype=torch.int32, device="cuda")
+    rows = torch.randn(2, 2, 1, 64, device="cuda").bfloat16()
+    one = torch.ones(2, dtype=torch.int32, device="cuda")
+    for kk, vv in ((k.clone().requires_grad_(), v), (k, v.clone().requires_grad_())):
+        for call in (lambda: b200_tree_attention(q, kk, vv, table, lens),
+                     lambda: b200_cache_append(rows, rows, kk, vv, table, lens),
+                     lambda: b200_cache_accept(kk, vv, table, lens, torch.zeros_like(table[:, :1]), one),
+                     lambda: b200_cache_reserve(kk, vv, table, lens, refs, 0),
+                     lambda: b200_cache_compact(kk, vv, table.clone(), refs.clone())):
+            with pytest.raises(ValueError, match="inference-only"):
+                call()
+        with torch.no_grad():
+            b200_tree_attention(q, kk, vv, table, lens)
+    with pytest.raises(ValueError, match="inference-only"):
+        b200_cache_append(rows.requires_grad_(), rows.detach(), k, v, table, lens)
+    assert read_device_errors(q.device) == 0

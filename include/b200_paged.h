@@ -107,7 +107,7 @@ B200_ATTN_API int32_t b200_cache_reserve(const b200_cache* c, const int32_t* tok
 
 /* Sequence dst[i] lets go of its pages and shares those of src[i] that cover its
  * committed tokens.  No dst may be another's dst or any src (such an entry is
- * skipped and reported). */
+ * skipped and reported, as is one whose src has a length that does not fit its slots). */
 B200_ATTN_API int32_t b200_cache_fork(const b200_cache* c, const int32_t* src, const int32_t* dst,
                                       int64_t n, void* stream);
 

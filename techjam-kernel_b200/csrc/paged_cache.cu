@@ -508,12 +508,13 @@ __global__ void __launch_bounds__(kCopyThreads)
   bool ok = s >= 0 && s < c.batch && d >= 0 && d < c.batch;
   for (int j = threadIdx.x; j < n; j += kCopyThreads)
     if (src[j] == d || (dst[j] == d && j != i)) ok = false;
+  const int len = ok ? c.lens[s] : 0;
+  if (len < 0 || len > static_cast<int64_t>(c.slots) * c.page_size) ok = false;
   ok = __syncthreads_and(ok);
   if (!ok) {
     if (threadIdx.x == 0) report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
     return;
   }
-  const int len = c.lens[s];
   for (int m = threadIdx.x; m < c.slots; m += kCopyThreads) {
     int32_t* to = &c.table[static_cast<int64_t>(d) * c.table_stride + m];
     const int old = *to;

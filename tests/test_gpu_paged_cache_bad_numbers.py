@@ -73,3 +73,14 @@ def test_accept_does_not_grow_a_sequence_past_its_slots(dtype, paths):
     want = m.accept([paths] * 4, [0, 0, 2, 4])
     assert got.tolist() == want.tolist()
     m.check(c.k_pages, c.v_pages, c.page_table, c.seq_lens, c.page_refs)
+
+
+@pytest.mark.parametrize("length", [-1, 17, (1 << 31) - 1])
+def test_fork_does_not_hand_on_a_bad_length(length):
+    c = filled(1, 20, 1, 4, 16, 4, 4, torch.bfloat16)
+    assert int(c.reserve(6)) == 0
+    c.seq_lens.copy_(i32([length, 6, 5, 5]))
+    m = model_of(c)
+    reported(c, lambda: c.fork(i32([0, 1]), i32([2, 3])))
+    m.fork([1], [3])
+    m.check(c.k_pages, c.v_pages, c.page_table, c.seq_lens, c.page_refs)

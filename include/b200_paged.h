@@ -84,7 +84,9 @@ B200_ATTN_API int32_t b200_cache_check(const b200_cache* c);
 B200_ATTN_API int64_t b200_cache_workspace_bytes(const b200_cache* c);
 
 /* Write row j of `rows` as token seq_lens[b] + j of every sequence b.  The
- * slots must hold pages (b200_cache_reserve). */
+ * slots must hold pages of the sequence's own (b200_cache_reserve with status 0:
+ * a page that is still shared is written for all that hold it).  Tokens without
+ * a page, past the slots or of a negative length are skipped and reported. */
 B200_ATTN_API int32_t b200_cache_append(const b200_cache* c, const b200_cache_rows* rows,
                                         void* stream);
 
@@ -126,8 +128,14 @@ B200_ATTN_API int32_t b200_cache_compact(const b200_cache* c, int32_t* live, voi
  * n_b (n_b = draft_lens ? draft_lens[b] : tokens) whose mask byte (b, i, j) is
  * set; without a mask, those with j <= i.  A tree is given by its ancestor
  * mask (each token sees its ancestors and itself).
- *   o_i = sum_p softmax_p(scale * q_i . k_p) v_p,  in fp32, rounded once.
- * Rows that see nothing, and rows i >= n_b, are zero.  Head h reads key head
+ *   o_i = sum_p softmax_p(scale * q_i . k_p) v_p.
+ * Scores, maxima, sums of weights and sums of values are fp32, and the output is
+ * rounded once.  With 16-bit caches the weights, relative to the largest so far,
+ * are rounded to the element type for the product with the values, as the tensor
+ * cores take them, and their sum is taken of the rounded ones; with fp32 caches
+ * they are not rounded.
+ * Rows that see nothing, rows i >= n_b, and all rows of a sequence whose length or
+ * draft does not fit its slots or the call (which is reported) are zero.  Head h reads key head
  * h / (heads / kv_heads).  `cache` describes one layer (layers = 1).
  */
 typedef struct b200_tree_attn_params {

@@ -137,8 +137,11 @@ def b200_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     attention forward gives NaN for rows that see nothing, as torch's softmax does;
     here such rows are padding).
 
-    bfloat16 and float16 products run on the tensor cores, float32 in fp32;
-    maximum, sum and output sums are fp32 and the output is rounded once.  Returns
+    bfloat16 and float16 products run on the tensor cores, float32 in fp32.
+    Scores, maximum, sum and output sums are fp32 and the output is rounded once; the
+    softmax weights of the 16-bit types are rounded to the type for the product with the
+    values, and summed as rounded.  A call under graph capture keeps no counters between
+    launches, so cut units of few rows are joined by a second kernel there.  Returns
     ``[B, H, T, D]``, or ``[B, T, H, D]`` with ``output_bshd``; ``out`` may supply it; it
     may be ``q`` itself, and shares no memory with another argument."""
     return _call("tree_attention", q.device, q, k_pages, v_pages, page_table, seq_lens, tree_mask,

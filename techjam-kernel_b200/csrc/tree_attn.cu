@@ -20,9 +20,9 @@ namespace {
 // 16 rows by 64 keys a tile, fp32 multiply-adds: scores from shared memory, one
 // pass over the keys with the running maximum and sum, the products' sums in
 // registers.  fp32 caches are for checking a model, not for serving it: the products stay
-// exact fp32 and each tile's loads, scores and sums follow one another.  A tree of 5 tokens
-// over 3 sequences of up to 1025 keys, 4 heads of 32, takes 16 us, most of it the launch
-// and the chain of loads; its 0.6 MB would take 0.1 us.
+// exact fp32 and each tile's loads, scores and sums follow one another.  Trees of up to 5
+// tokens over 3 sequences of up to 700 keys, 4 key heads of 3, D 40, take 15.6 us, most of it
+// the launch and the chain of loads; their 0.56 MB would take 0.09 us.
 constexpr int kRows = 16, kKeys = 64, kThreads = 256;
 constexpr int kScoreRows = kRows * kKeys / kThreads;  // rows of a thread's key
 constexpr int kWarpRows = kRows * 32 / kThreads;      // rows of a warp in the softmax step
@@ -278,7 +278,7 @@ Choice choose(const b200_tree_attn_params* p) {
   // short contexts only, whose ends of units weigh more (64 of up to 400: 45 us against 46
   // us with boxes of 8).
   // Up to 16 rows the few-row kernel reads near the rate of memory (16 rows: 103 us, 4
-  // rows: 92 us).
+  // rows: 97 us).
   const bool eight = rows > 32 || dp == 128 || p->cache.slots * p->cache.page_size <= 2048;
   const int least = eight ? 8 : 32;
   if (rows > 16 && group <= 128 && by_tensor_maps(p, least)) {

@@ -10,8 +10,9 @@
 // sequences are: one long sequence fills the GPU and a ragged batch has no
 // tail.  What a unit costs beside its tiles (queries in, results out) is counted as
 // EX tiles ahead of its first.  A unit that lies inside one run is finished there; one that is cut
-// leaves partial results (unnormalised sums, row maximum, row sum) that a second
-// kernel joins in the order of the runs, so the result does not depend on timing.
+// leaves partial results (unnormalised sums, row maximum, row sum), which are joined in
+// the order of the runs, so the result does not depend on timing: by the last of its
+// runs to arrive where the kernel of few rows has counters, else by a second kernel.
 #pragma once
 
 #include <cuda_bf16.h>

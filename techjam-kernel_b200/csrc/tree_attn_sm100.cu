@@ -6,16 +6,15 @@
 // running maximum and sum.  What bounds it: R rows do 4 R D operations for the 4 D
 // bytes of a key and value, so from about 260 rows the tensor cores, below it
 // HBM.  Measured (bf16, D 128): 32 sequences of 1 to 8 thousand keys, 8 key heads, 256
-// rows, 638 MB and 153 GFLOP: 183 us in short runs (836 TFLOP/s, half of the
-// tensor cores' measured rate and of the memory's), 209 us back to back, where
-// the board's power limit lowers the clock; DRAM reads are the
-// cache's bytes exactly.  A key tile of 256 rows takes about 4000 cycles, in which a softmax
+// rows, 638 MB and 153 GFLOP: 212 us in a stream of calls (718 TFLOP/s and 3.0 TB/s, 43 and
+// 46 % of the measured rates), where the board's power limit lowers the clock, and 177 us in
+// runs too short for that; DRAM reads are the cache's bytes exactly.  A key tile of 256 rows takes about 4000 cycles, in which a softmax
 // group waits for its scores (570 cycles of products and 300 to be seen), copies them (400),
 // exponentiates (128 a thread, 3000 cycles with its waits) and hands over the weights;
 // tensor pipe and exponential unit are each active under half of the time.
-// 64 rows over 131001 keys: 537 MB, 97 us, 5.5 TB/s.  Short
-// contexts (5 sequences of 601 to 5003 keys, 63 rows a head, fp16, pages of 48: 28 us against
-// 6 us of bytes) are bound by the ends of a unit (queries in, results out) and by
+// 64 rows over 131001 keys: 537 MB, 111 us in a stream of calls, 4.8 TB/s (96 us in short
+// runs).  Short contexts (5 sequences of 601 to 5003 keys, 63 rows a head, fp16, pages of 48:
+// 28 us against 6 us of bytes) are bound by the ends of a unit (queries in, results out) and by
 // issuing boxes of 16 rows.
 // Scores of half a tile (64 keys) in buffers of their own: 260 us against 228 us then.
 //

@@ -9,8 +9,9 @@
   over materialised scores (reference: triton_attention_softmax /
   TritonSelfAttention, also exported under those names)
 - ``b200_tree_attention``, ``b200_cache_*`` / ``PagedKVCache``: attention for drafted
-  tokens (or one token) over a paged key/value cache, and the cache's page
-  operations
+  tokens (or one token) over a paged key/value cache of 16 or 32 bits or of 4, and the
+  cache's page operations
+- ``b200_verify_drafts``: which drafted tokens the target keeps, and the next one
 """
 
 from .fused_attention import (DeviceError, b200_fused_attention, check_device_errors,  # noqa: F401
@@ -18,6 +19,7 @@ from .fused_attention import (DeviceError, b200_fused_attention, check_device_er
 from .linear import b200_linear  # noqa: F401
 from .paged_cache import (PagedKVCache, b200_cache_accept, b200_cache_append,  # noqa: F401
                           b200_cache_compact, b200_cache_fork, b200_cache_free,
-                          b200_cache_reserve, b200_tree_attention)
+                          b200_cache_read, b200_cache_reserve, b200_tree_attention)
 from .softmax import (B200SoftmaxSelfAttention, TritonSelfAttention,  # noqa: F401
                       b200_attention_softmax, triton_attention_softmax)
+from .verify import b200_verify_drafts  # noqa: F401

@@ -1,5 +1,6 @@
 """ctypes binding of the C ABI in ``include/b200_attn.h``, ``include/b200_linear.h``,
-``include/b200_layernorm.h``, ``include/b200_softmax.h`` and ``include/b200_paged.h``.
+``include/b200_layernorm.h``, ``include/b200_softmax.h``, ``include/b200_paged.h``,
+``include/b200_cache4.h`` and ``include/b200_verify.h``.
 
 This module is torch-free: it loads ``libb200_attention.so`` and describes the
 parameter struct.  The library is loaded from this directory only; a missing or
@@ -82,6 +83,23 @@ PAGED_SYMBOLS = (
     "b200_tree_attn_workspace_bytes",
     "b200_tree_attn_fwd",
 )
+# Every symbol ``include/b200_cache4.h`` declares.
+CACHE4_SYMBOLS = (
+    "b200_cache4_row_bytes",
+    "b200_cache4_append",
+    "b200_cache4_read",
+    "b200_cache4_attn_check",
+    "b200_cache4_attn_workspace_bytes",
+    "b200_cache4_attn_fwd",
+)
+
+# Every symbol ``include/b200_verify.h`` declares.
+VERIFY_SYMBOLS = (
+    "b200_verify_check",
+    "b200_verify_drafts",
+)
+VERIFY_MAX_NODES = 1024
+VERIFY_MAX_VOCAB = 1 << 24
 CACHE_MAX_BATCH = 8192
 CACHE_NO_PAGES = 1
 CACHE_ROW_FULL = 2
@@ -255,6 +273,36 @@ class TreeAttnParams(ctypes.Structure):
     ]
 
 
+class VerifyParams(ctypes.Structure):
+    """Mirror of ``b200_verify_params``."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("logits_stride", ctypes.c_int64 * 2),
+        ("draft_probs", ctypes.c_void_p),
+        ("draft_stride", ctypes.c_int64 * 2),
+        ("tokens", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("uniforms", ctypes.c_void_p),
+        ("uniform_stride", ctypes.c_int64),
+        ("parents", ctypes.c_void_p),
+        ("parent_stride", ctypes.c_int64),
+        ("draft_lens", ctypes.c_void_p),
+        ("paths", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("next", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("nodes", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("temperature", ctypes.c_double),
+        ("dtype", ctypes.c_int32),
+        ("draft_dtype", ctypes.c_int32),
+        ("wide_tokens", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("error_word", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -315,7 +363,15 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
             ("b200_cache_compact", i32, [cache, ptr, ptr, i64, ptr]),
             ("b200_tree_attn_check", i32, [tree]),
             ("b200_tree_attn_workspace_bytes", i64, [tree]),
-            ("b200_tree_attn_fwd", i32, [tree, ptr])):
+            ("b200_tree_attn_fwd", i32, [tree, ptr]),
+            ("b200_cache4_row_bytes", i32, [i64]),
+            ("b200_cache4_append", i32, [cache, i64, i32, ctypes.POINTER(CacheRows), ptr]),
+            ("b200_cache4_read", i32, [cache, i64, i32, ctypes.POINTER(CacheRows), ptr]),
+            ("b200_cache4_attn_check", i32, [tree, i64, i32]),
+            ("b200_cache4_attn_workspace_bytes", i64, [tree, i64, i32]),
+            ("b200_cache4_attn_fwd", i32, [tree, i64, i32, ptr]),
+            ("b200_verify_check", i32, [ctypes.POINTER(VerifyParams)]),
+            ("b200_verify_drafts", i32, [ctypes.POINTER(VerifyParams), ptr])):
         getattr(lib, name).restype = result
         getattr(lib, name).argtypes = args
     return lib

@@ -2,8 +2,8 @@
 
 The shared library is torch-free: it exports the C ABI declared in
 ``include/b200_attn.h``, ``include/b200_linear.h``, ``include/b200_layernorm.h``,
-``include/b200_softmax.h`` and ``include/b200_paged.h``
-and links the CUDA runtime statically, so the same file serves the ctypes
+``include/b200_softmax.h``, ``include/b200_paged.h``, ``include/b200_cache4.h`` and
+``include/b200_verify.h`` and links the CUDA runtime statically, so the same file serves the ctypes
 binding here and any other FFI host.
 """
 
@@ -29,9 +29,10 @@ LIB_PATH = PACKAGE_DIR / LIB_NAME
 CHECKED_LIB_PATH = PACKAGE_DIR / "libb200_attention_checked.so"
 
 SOURCES = ("attn_fwd_sm100.cu", "linear_sm100.cu", "layernorm.cu", "softmax.cu",
-           "paged_cache.cu", "tree_attn.cu", "tree_attn_sm100.cu")
+           "paged_cache.cu", "tree_attn.cu", "tree_attn_sm100.cu", "cache4.cu", "tree_attn4.cu",
+           "verify.cu")
 HEADERS = ("sm100_ptx.cuh", "error_word.cuh", "byte_range.h", "paged_host.h", "tree_attn.cuh",
-           "tree_attn_rows.cuh")
+           "tree_attn_host.cuh", "tree_attn_rows.cuh")
 
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -57,7 +58,8 @@ def _nvcc() -> str:
 def _inputs() -> list[Path]:
     files = [CSRC / s for s in SOURCES] + [CSRC / h for h in HEADERS]
     files += [INCLUDE / h for h in ("b200_attn.h", "b200_linear.h", "b200_layernorm.h",
-                                    "b200_softmax.h", "b200_paged.h")]
+                                    "b200_softmax.h", "b200_paged.h", "b200_cache4.h",
+                                    "b200_verify.h")]
     return files
 
 
@@ -111,7 +113,8 @@ def _torch_op_stale() -> bool:
     if not TORCH_OP_PATH.exists():
         return True
     built = TORCH_OP_PATH.stat().st_mtime
-    deps = (TORCH_OP_SOURCE, INCLUDE / "b200_attn.h", INCLUDE / "b200_paged.h", LIB_PATH)
+    deps = (TORCH_OP_SOURCE, INCLUDE / "b200_attn.h", INCLUDE / "b200_paged.h",
+            INCLUDE / "b200_cache4.h", INCLUDE / "b200_verify.h", LIB_PATH)
     return any(f.stat().st_mtime > built for f in deps if f.exists())
 
 

@@ -10,6 +10,12 @@ first dimension), and its bookkeeping in device memory:
   tree of them) lie directly behind the committed ones until they are accepted;
 * ``page_refs`` int32 ``[pages]``: how many sequences hold a page (0: free).
 
+Pools of uint8 hold the cache in 4 bits (``include/b200_cache4.h``): a row of 48 bytes
+(``head_dim`` up to 64) or 80 (up to 128) stands for a vector in four groups, each number
+``low + step * code``.  ``b200_cache_append`` rounds vectors into such rows,
+``b200_tree_attention`` reads them, ``b200_cache_read`` gives the numbers back, and the page
+operations move the rows as they are.
+
 One decode step is ``b200_cache_reserve`` (pages for the tokens to come, copy on
 write), for every layer ``b200_cache_append`` and ``b200_tree_attention``, and
 ``b200_cache_accept`` (keep the accepted path).  ``b200_cache_fork``,
@@ -28,7 +34,7 @@ launch raises ``DeviceError``).  ``PagedKVCache`` keeps the tensors together.
 
 from __future__ import annotations
 
-from typing import Optional, Union
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -65,9 +71,27 @@ def b200_cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.T
                       draft_lens: Optional[torch.Tensor] = None) -> None:
     """Write ``k_new``/``v_new`` ``[(layers,) batch, kv_heads, tokens, head_dim]`` (any
     strides, last dimension contiguous) as tokens ``seq_lens[b] + j`` of each
-    sequence; with ``draft_lens`` int32 ``[batch]`` only rows ``j < draft_lens[b]``."""
+    sequence; with ``draft_lens`` int32 ``[batch]`` only rows ``j < draft_lens[b]``.
+
+    Into a 4-bit cache (uint8 pools) go vectors of bfloat16, float16 or float32: each quarter
+    of a vector padded to 64 or 128 has a ``low``, the bfloat16 number at or below its smallest, a
+    ``step``, that at or above a fifteenth of the way from it to the largest, and codes
+    ``(x - low) / step`` rounded to nearest, ties to even.  A number is off by half a step at
+    most; a group that holds an infinity or NaN reads as NaN."""
     _call("cache_append", k_pages.device, k_new, v_new, k_pages, v_pages, page_table, seq_lens,
           draft_lens)
+
+
+def b200_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    starts: torch.Tensor, tokens: int, head_dim: int,
+                    dtype: torch.dtype = torch.bfloat16,
+                    counts: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that a 4-bit cache holds for tokens ``starts[b] + j``, ``j <
+    tokens`` (``starts`` int32 ``[batch]``), as ``dtype`` tensors ``[(layers,) batch, kv_heads,
+    tokens, head_dim]``, each number rounded once.  With ``counts`` int32 ``[batch]`` only rows
+    ``j < counts[b]`` are read, and the others are zero."""
+    return _call("cache_read", k_pages.device, k_pages, v_pages, page_table, starts, tokens,
+                 head_dim, dtype, counts)
 
 
 def b200_cache_accept(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -141,7 +165,12 @@ def b200_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     Scores, maximum, sum and output sums are fp32 and the output is rounded once; the
     softmax weights of the 16-bit types are rounded to the type for the product with the
     values, and summed as rounded.  A call under graph capture keeps no counters between
-    launches, so cut units of few rows are joined by a second kernel there.  Returns
+    launches, so cut units of few rows are joined by a second kernel there.
+
+    Over a 4-bit cache (uint8 pools ``[pages, kv_heads, page_size, row bytes]``) ``q`` is
+    bfloat16 or float16.  Products with the codes are exact in fp32 sums, steps and lows are
+    applied in fp32; a weight times the step of its value is rounded to fp16 for the product
+    with the codes (relative to the largest such step), the sum of weights is not.  Returns
     ``[B, H, T, D]``, or ``[B, T, H, D]`` with ``output_bshd``; ``out`` may supply it; it
     may be ``q`` itself, and shares no memory with another argument."""
     return _call("tree_attention", q.device, q, k_pages, v_pages, page_table, seq_lens, tree_mask,
@@ -150,7 +179,8 @@ def b200_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
 
 class PagedKVCache:
     """The tensors of a paged cache, all pages free and all sequences empty, and the
-    page operations on them."""
+    page operations on them.  With ``bits=4`` the pools hold 4-bit rows, and ``dtype`` is that of
+    the vectors that go in and out."""
 
     NO_PAGES = _native.CACHE_NO_PAGES
     ROW_FULL = _native.CACHE_ROW_FULL
@@ -158,13 +188,21 @@ class PagedKVCache:
 
     def __init__(self, layers: int, pages: int, kv_heads: int, page_size: int, head_dim: int,
                  batch: int, slots: int, *, dtype: torch.dtype = torch.bfloat16,
-                 device: Union[str, torch.device] = "cuda") -> None:
+                 device: Union[str, torch.device] = "cuda", bits: Optional[int] = None) -> None:
         shape = (layers, pages, kv_heads, page_size, head_dim)
         if min(shape) < 1 or batch < 1 or slots < 1:
             raise ValueError(f"a cache needs positive sizes, got {shape}, batch {batch}, "
                              f"slots {slots}")
-        self.k_pages = torch.zeros(shape, dtype=dtype, device=device)
-        self.v_pages = torch.zeros(shape, dtype=dtype, device=device)
+        if bits not in (None, 4):
+            raise ValueError(f"bits must be 4, or None for pages of {dtype}, got {bits}")
+        self.head_dim, self.dtype, stored = head_dim, dtype, dtype
+        if bits == 4:
+            if head_dim % 8 or head_dim > 128:
+                raise ValueError(f"head_dim {head_dim} is outside the kernel envelope of a 4-bit "
+                                 "cache (multiples of 8 up to 128)")
+            shape, stored = (*shape[:-1], 48 if head_dim <= 64 else 80), torch.uint8
+        self.k_pages = torch.zeros(shape, dtype=stored, device=device)
+        self.v_pages = torch.zeros(shape, dtype=stored, device=device)
         ints = dict(dtype=torch.int32, device=device)
         self.page_table = torch.full((batch, slots), -1, **ints)
         self.seq_lens = torch.zeros(batch, **ints)
@@ -188,6 +226,12 @@ class PagedKVCache:
                output_bshd: bool = False) -> torch.Tensor:
         return b200_tree_attention(q, self.k_pages[layer], self.v_pages[layer], self.page_table,
                                    self.seq_lens, tree_mask, draft_lens, scale, output_bshd)
+
+    def read(self, layer: int, starts: torch.Tensor, tokens: int,
+             counts: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``b200_cache_read`` of one layer (4-bit caches)."""
+        return b200_cache_read(self.k_pages[layer], self.v_pages[layer], self.page_table, starts,
+                               tokens, self.head_dim, self.dtype, counts)
 
     def accept(self, paths: torch.Tensor, counts: torch.Tensor) -> None:
         self.seq_lens.copy_(b200_cache_accept(self.k_pages, self.v_pages, self.page_table,

@@ -193,15 +193,16 @@ class Decoder(nn.Module):
         return x
 
     def new_cache(self, batch: int, max_tokens: int, page_size: int = 64,
-                  pages: Optional[int] = None) -> PagedKVCache:
+                  pages: Optional[int] = None, bits: Optional[int] = None) -> PagedKVCache:
         """An empty paged cache for ``batch`` sequences of up to ``max_tokens`` committed
-        and drafted tokens (``pages`` in the pool; by default enough for all of them)."""
+        and drafted tokens (``pages`` in the pool; by default enough for all of them), of the
+        model's type, or with ``bits=4`` held in 4 bits."""
         slots = -(-max_tokens // page_size)
         weight = self.final_norm.weight
         return PagedKVCache(self.config.num_layers, pages if pages is not None else batch * slots,
                             self.config.num_heads, page_size,
                             self.config.d_model // self.config.num_heads, batch, slots,
-                            dtype=weight.dtype, device=weight.device)
+                            dtype=weight.dtype, device=weight.device, bits=bits)
 
     def cached_forward(self, x: torch.Tensor, cache: PagedKVCache,
                        tree_mask: Optional[torch.Tensor] = None,

@@ -1,5 +1,5 @@
-// torch_op.cpp — the attention operator and the paged-cache operators as torch
-// custom ops over the C ABI.
+// torch_op.cpp — the attention operator, the paged-cache operators and the check of
+// drafted tokens as torch custom ops over the C ABI.
 //
 // torch.ops.b200.fused_attention keeps the argument meaning, checks and
 // exception types of the reference operator triton_fused_attention
@@ -21,10 +21,14 @@
 #include <map>
 #include <mutex>
 #include <optional>
+#include <tuple>
 #include <utility>
+#include <vector>
 
 #include "b200_attn.h"
+#include "b200_cache4.h"
 #include "b200_paged.h"
+#include "b200_verify.h"
 
 namespace {
 
@@ -208,7 +212,8 @@ b200_cache table_view(const at::Tensor& table, const OptTensor& lens, const OptT
 }
 
 // The whole cache; pools are [layers, pages, kv_heads, page_size, head_dim] or,
-// of one layer, [pages, kv_heads, page_size, head_dim].
+// of one layer, [pages, kv_heads, page_size, head_dim].  Pools of uint8 hold rows of 4-bit numbers
+// (b200_cache4.h) and are described as 16-bit ones of half as many elements.
 b200_cache cache_view(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
                       const OptTensor& lens, const OptTensor& refs, int64_t error_word) {
   TORCH_CHECK_VALUE(k.dim() == 4 || k.dim() == 5,
@@ -218,9 +223,12 @@ b200_cache cache_view(const at::Tensor& k, const at::Tensor& v, const at::Tensor
                     k.sizes(), " and ", v.sizes());
   TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type(),
                    "k_pages and v_pages must have the same dtype");
-  const int32_t dt = dtype_code(k.scalar_type());
-  TORCH_CHECK_TYPE(dt >= 0, "k_pages must be bfloat16, float16 or float32, got ", k.scalar_type());
+  const bool coded = k.scalar_type() == at::kByte;
+  const int32_t dt = coded ? B200_ATTN_DTYPE_BF16 : dtype_code(k.scalar_type());
+  TORCH_CHECK_TYPE(dt >= 0, "k_pages must be bfloat16, float16 or float32, or uint8 for a 4-bit "
+                   "cache, got ", k.scalar_type());
   const int64_t d = k.dim() - 4;  // of the page dimension
+  const int64_t each = coded ? 2 : 1;  // elements of the pools to one of the description
   b200_cache c = table_view(table, lens, refs, k.size(d + 2), error_word);
   TORCH_CHECK_VALUE(k.device() == table.device() && v.device() == table.device(),
                     "the pools and the page table must be on the same device");
@@ -231,17 +239,27 @@ b200_cache cache_view(const at::Tensor& k, const at::Tensor& v, const at::Tensor
                     "the paged cache is inference-only (autograd requested)");
   TORCH_CHECK_VALUE(!refs.has_value() || c.pages == k.size(d), "page_refs must have one count for "
                     "each of the ", k.size(d), " pages, got ", c.pages);
-  TORCH_CHECK_VALUE(k.size(d + 3) % 8 == 0 && k.size(d + 3) <= 128, "head_dim ", k.size(d + 3),
-                    " is outside the kernel envelope (multiples of 8 up to 128)");
+  if (coded) {
+    TORCH_CHECK_VALUE(k.size(d + 3) == b200_cache4_row_bytes(64) ||
+                          k.size(d + 3) == b200_cache4_row_bytes(128),
+                      "rows of a 4-bit cache have ", b200_cache4_row_bytes(64), " bytes (head_dim up "
+                      "to 64) or ", b200_cache4_row_bytes(128), " (up to 128), got ", k.size(d + 3));
+    for (int64_t i = 0; i < d + 3; ++i)
+      TORCH_CHECK_VALUE(k.size(i) == 1 || (k.stride(i) % 16 == 0 && v.stride(i) % 16 == 0),
+                        "the strides of a 4-bit cache must be multiples of 16 bytes");
+  } else {
+    TORCH_CHECK_VALUE(k.size(d + 3) % 8 == 0 && k.size(d + 3) <= 128, "head_dim ", k.size(d + 3),
+                      " is outside the kernel envelope (multiples of 8 up to 128)");
+  }
   c.k = k.data_ptr();
   c.v = v.data_ptr();
   c.layers = d ? k.size(0) : 1;
   c.pages = k.size(d);
   c.kv_heads = k.size(d + 1);
-  c.head_dim = k.size(d + 3);
+  c.head_dim = k.size(d + 3) / each;
   for (int64_t i = 0; i < 4; ++i) {
-    c.k_stride[i] = i == 0 && !d ? 0 : k.stride(d + i - 1);
-    c.v_stride[i] = i == 0 && !d ? 0 : v.stride(d + i - 1);
+    c.k_stride[i] = i == 0 && !d ? 0 : k.stride(d + i - 1) / each;
+    c.v_stride[i] = i == 0 && !d ? 0 : v.stride(d + i - 1) / each;
   }
   c.dtype = dt;
   return c;
@@ -255,6 +273,25 @@ at::Tensor scratch(int64_t bytes, const at::Tensor& like) {
   return at::empty({bytes}, like.options().dtype(at::kByte));
 }
 
+// The head dim of vectors that go into rows of a 4-bit cache, checked against them.
+void check_coded(const b200_cache& c, int64_t head_dim, const char* whose) {
+  const int64_t bytes = b200_cache4_row_bytes(head_dim);
+  TORCH_CHECK_VALUE(bytes > 0, "head_dim ", head_dim,
+                    " is outside the kernel envelope (multiples of 8 up to 128)");
+  TORCH_CHECK_VALUE(bytes == 2 * c.head_dim, whose, " has head_dim ", head_dim, ", whose rows have ",
+                    bytes, " bytes in a 4-bit cache; the pools' have ", 2 * c.head_dim);
+}
+
+void fill_rows(b200_cache_rows* r, const at::Tensor& k, const at::Tensor& v, int64_t d) {
+  r->k = k.data_ptr();
+  r->v = v.data_ptr();
+  r->tokens = k.size(d + 2);
+  for (int64_t i = 0; i < 4; ++i) {
+    r->k_stride[i] = i == 0 && !d ? 0 : k.stride(d + i - 1);
+    r->v_stride[i] = i == 0 && !d ? 0 : v.stride(d + i - 1);
+  }
+}
+
 void cache_append(const at::Tensor& k_new, const at::Tensor& v_new, const at::Tensor& k,
                   const at::Tensor& v, const at::Tensor& table, const at::Tensor& lens,
                   const OptTensor& counts, int64_t error_word) {
@@ -263,12 +300,22 @@ void cache_append(const at::Tensor& k_new, const at::Tensor& v_new, const at::Te
   TORCH_CHECK_VALUE(k_new.dim() == k.dim() && v_new.sizes() == k_new.sizes(),
                     "k_new and v_new must have shape [(layers,) batch, kv_heads, tokens, "
                     "head_dim] like the pools; got ", k_new.sizes(), " and ", v_new.sizes());
+  const bool coded = k.scalar_type() == at::kByte;
+  const int64_t head_dim = k_new.size(d + 3);
+  if (coded) check_coded(c, head_dim, "k_new");
   TORCH_CHECK_VALUE((!d || k_new.size(0) == c.layers) && k_new.size(d) == c.batch &&
-                        k_new.size(d + 1) == c.kv_heads && k_new.size(d + 3) == c.head_dim,
+                        k_new.size(d + 1) == c.kv_heads && (coded || head_dim == c.head_dim),
                     "k_new must have shape [(", c.layers, ",) ", c.batch, ", ", c.kv_heads,
-                    ", tokens, ", c.head_dim, "], got ", k_new.sizes());
-  TORCH_CHECK_TYPE(k_new.scalar_type() == k.scalar_type() && v_new.scalar_type() == k.scalar_type(),
-                   "k_new and v_new must have the pools' dtype ", k.scalar_type());
+                    ", tokens, ", coded ? head_dim : c.head_dim, "], got ", k_new.sizes());
+  const int32_t dt = dtype_code(k_new.scalar_type());
+  if (coded) {
+    TORCH_CHECK_TYPE(dt >= 0 && v_new.scalar_type() == k_new.scalar_type(),
+                     "k_new and v_new must both be bfloat16, float16 or float32, got ",
+                     k_new.scalar_type(), " and ", v_new.scalar_type());
+  } else {
+    TORCH_CHECK_TYPE(k_new.scalar_type() == k.scalar_type() && v_new.scalar_type() == k.scalar_type(),
+                     "k_new and v_new must have the pools' dtype ", k.scalar_type());
+  }
   TORCH_CHECK_VALUE(k_new.device() == k.device() && v_new.device() == k.device(),
                     "k_new and v_new must be on the cache's device");
   TORCH_CHECK_VALUE(k_new.stride(d + 3) == 1 && v_new.stride(d + 3) == 1,
@@ -277,16 +324,36 @@ void cache_append(const at::Tensor& k_new, const at::Tensor& v_new, const at::Te
                       (k_new.requires_grad() || v_new.requires_grad())),
                     "the paged cache is inference-only (autograd requested)");
   b200_cache_rows r{};
-  r.k = k_new.data_ptr();
-  r.v = v_new.data_ptr();
-  r.tokens = k_new.size(d + 2);
-  for (int64_t i = 0; i < 4; ++i) {
-    r.k_stride[i] = i == 0 && !d ? 0 : k_new.stride(d + i - 1);
-    r.v_stride[i] = i == 0 && !d ? 0 : v_new.stride(d + i - 1);
-  }
+  fill_rows(&r, k_new, v_new, d);
   if (counts.has_value()) r.counts = ints(*counts, "draft_lens", {c.batch}, k.device());
   if (r.tokens == 0) return;
-  raise_code("b200_cache_append", b200_cache_append(&c, &r, stream_of(k)));
+  if (coded)
+    raise_code("b200_cache4_append", b200_cache4_append(&c, head_dim, dt, &r, stream_of(k)));
+  else
+    raise_code("b200_cache_append", b200_cache_append(&c, &r, stream_of(k)));
+}
+
+std::tuple<at::Tensor, at::Tensor> cache_read(const at::Tensor& k, const at::Tensor& v,
+                                              const at::Tensor& table, const at::Tensor& starts,
+                                              int64_t tokens, int64_t head_dim, at::ScalarType dtype,
+                                              const OptTensor& counts, int64_t error_word) {
+  TORCH_CHECK_TYPE(k.scalar_type() == at::kByte, "b200_cache_read reads 4-bit caches (uint8 pools), "
+                   "got ", k.scalar_type());
+  const b200_cache c = cache_view(k, v, table, starts, std::nullopt, error_word);
+  check_coded(c, head_dim, "the call");
+  const int32_t dt = dtype_code(dtype);
+  TORCH_CHECK_TYPE(dt >= 0, "dtype must be bfloat16, float16 or float32, got ", dtype);
+  TORCH_CHECK_VALUE(tokens >= 0, "tokens must not be negative");
+  const int64_t d = k.dim() - 4;
+  std::vector<int64_t> shape{c.batch, c.kv_heads, tokens, head_dim};
+  if (d) shape.insert(shape.begin(), c.layers);
+  at::Tensor k_out = at::empty(shape, k.options().dtype(dtype)), v_out = at::empty_like(k_out);
+  b200_cache_rows r{};
+  fill_rows(&r, k_out, v_out, d);
+  if (counts.has_value()) r.counts = ints(*counts, "counts", {c.batch}, k.device());
+  if (tokens > 0)
+    raise_code("b200_cache4_read", b200_cache4_read(&c, head_dim, dt, &r, stream_of(k)));
+  return {k_out, v_out};
 }
 
 at::Tensor cache_accept(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
@@ -383,11 +450,21 @@ at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Te
   p.cache = cache_view(k, v, table, lens, std::nullopt, error_word);
   const int64_t B = q.size(0), H = q.size(1), T = q.size(2), D = q.size(3);
   TORCH_CHECK_VALUE(B == p.cache.batch, "q has ", B, " sequences, page_table ", p.cache.batch);
-  TORCH_CHECK_VALUE(D == p.cache.head_dim, "q has head_dim ", D, ", the pools ", p.cache.head_dim);
+  const bool coded = k.scalar_type() == at::kByte;
+  if (coded) {
+    check_coded(p.cache, D, "q");
+  } else {
+    TORCH_CHECK_VALUE(D == p.cache.head_dim, "q has head_dim ", D, ", the pools ", p.cache.head_dim);
+  }
   TORCH_CHECK_VALUE(H >= 1 && H % p.cache.kv_heads == 0, "q's heads (", H,
                     ") must be a multiple of the pools' (", p.cache.kv_heads, ")");
-  TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type(), "q must have the pools' dtype ",
-                   k.scalar_type(), ", got ", q.scalar_type());
+  if (coded) {
+    TORCH_CHECK_TYPE(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf,
+                     "q must be bfloat16 or float16 over a 4-bit cache, got ", q.scalar_type());
+  } else {
+    TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type(), "q must have the pools' dtype ",
+                     k.scalar_type(), ", got ", q.scalar_type());
+  }
   TORCH_CHECK_VALUE(q.device() == k.device(), "q must be on the cache's device");
   TORCH_CHECK_VALUE(q.stride(3) == 1, "q must have a contiguous last dimension");
   TORCH_CHECK_VALUE(!(c10::GradMode::is_enabled() && q.requires_grad()),
@@ -430,7 +507,9 @@ at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Te
   fill_strides(p.q_stride, q);
   fill_strides(p.o_stride, o);
   p.scale = static_cast<float>(sc);
-  p.workspace_bytes = b200_tree_attn_workspace_bytes(&p);
+  const int32_t dt = dtype_code(q.scalar_type());
+  p.workspace_bytes = coded ? b200_cache4_attn_workspace_bytes(&p, D, dt)
+                            : b200_tree_attn_workspace_bytes(&p);
   at::Tensor ws;
   if (p.workspace_bytes > 0) {
     ws = scratch(p.workspace_bytes, q);
@@ -438,8 +517,96 @@ at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Te
   }
   const cudaStream_t stream = stream_of(q);
   p.counters = counters_of(stream, q);
-  raise_code("b200_tree_attn_fwd", b200_tree_attn_fwd(&p, stream));
+  if (coded)
+    raise_code("b200_cache4_attn_fwd", b200_cache4_attn_fwd(&p, D, dt, stream));
+  else
+    raise_code("b200_tree_attn_fwd", b200_tree_attn_fwd(&p, stream));
   return result;
+}
+
+// ------------------------------------------------------------ drafted tokens
+std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(
+    const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& uniforms,
+    const OptTensor& draft_probs, const OptTensor& parents, const OptTensor& draft_lens,
+    double temperature, int64_t error_word) {
+  TORCH_CHECK_VALUE(logits.dim() == 3, "logits must have shape [B, T, V], got ", logits.sizes());
+  TORCH_CHECK_VALUE(logits.is_cuda(), "b200_verify_drafts runs on CUDA tensors only");
+  const int64_t B = logits.size(0), T = logits.size(1), V = logits.size(2);
+  TORCH_CHECK_VALUE(B >= 1 && B <= 65535, "logits must have 1 to 65535 sequences, got ", B);
+  TORCH_CHECK_VALUE(T >= 1 && T <= B200_VERIFY_MAX_NODES, "logits must have 1 to ",
+                    B200_VERIFY_MAX_NODES, " nodes, got ", T);
+  TORCH_CHECK_VALUE(V >= 1 && V <= B200_VERIFY_MAX_VOCAB, "logits must have 1 to ",
+                    B200_VERIFY_MAX_VOCAB, " tokens, got ", V);
+  b200_verify_params p{};
+  p.dtype = dtype_code(logits.scalar_type());
+  TORCH_CHECK_TYPE(p.dtype >= 0, "logits must be bfloat16, float16 or float32, got ",
+                   logits.scalar_type());
+  TORCH_CHECK_VALUE(V == 1 || logits.stride(2) == 1, "logits must have a contiguous last dimension");
+  TORCH_CHECK_TYPE(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt,
+                   "tokens must have dtype torch.int64 or torch.int32, got ", tokens.scalar_type());
+  TORCH_CHECK_TYPE(uniforms.scalar_type() == at::kFloat, "uniforms must have dtype torch.float32, "
+                   "got ", uniforms.scalar_type());
+  for (const at::Tensor* t : {&tokens, &uniforms}) {
+    const char* name = t == &tokens ? "tokens" : "uniforms";
+    TORCH_CHECK_VALUE(t->dim() == 2 && t->size(0) == B && t->size(1) == T, name,
+                      " must have shape [", B, ", ", T, "], got ", t->sizes());
+    TORCH_CHECK_VALUE(T == 1 || t->stride(1) == 1, name, " must have a contiguous last dimension");
+    TORCH_CHECK_VALUE(t->device() == logits.device(), name, " must be on the logits' device");
+  }
+  TORCH_CHECK_VALUE(temperature >= 0.0 && std::isfinite(temperature),
+                    "temperature must be a finite number of 0 or more, got ", temperature);
+  TORCH_CHECK_VALUE(!(c10::GradMode::is_enabled() &&
+                      (logits.requires_grad() || uniforms.requires_grad() ||
+                       (draft_probs.has_value() && draft_probs->requires_grad()))),
+                    "b200_verify_drafts is inference-only (autograd requested)");
+  if (draft_probs.has_value()) {
+    const at::Tensor& q = *draft_probs;
+    TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == B && q.size(1) == T - 1 && q.size(2) == V,
+                      "draft_probs must have shape [", B, ", ", T - 1, ", ", V, "], got ", q.sizes());
+    p.draft_dtype = dtype_code(q.scalar_type());
+    TORCH_CHECK_TYPE(p.draft_dtype >= 0, "draft_probs must be bfloat16, float16 or float32, got ",
+                     q.scalar_type());
+    TORCH_CHECK_VALUE(V == 1 || q.stride(2) == 1,
+                      "draft_probs must have a contiguous last dimension");
+    TORCH_CHECK_VALUE(q.device() == logits.device(), "draft_probs must be on the logits' device");
+    if (T > 1) p.draft_probs = q.data_ptr();
+    p.draft_stride[0] = q.stride(0);
+    p.draft_stride[1] = q.stride(1);
+  }
+  if (parents.has_value()) {
+    const at::Tensor& t = *parents;
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, "parents must have dtype torch.int32, got ",
+                     t.scalar_type());
+    const bool shared = t.dim() == 1;
+    TORCH_CHECK_VALUE((shared || (t.dim() == 2 && t.size(0) == B)) && t.size(-1) == T,
+                      "parents must have shape [", T, "] or [", B, ", ", T, "], got ", t.sizes());
+    TORCH_CHECK_VALUE(T == 1 || t.stride(-1) == 1, "parents must have a contiguous last dimension");
+    TORCH_CHECK_VALUE(t.device() == logits.device(), "parents must be on the logits' device");
+    p.parents = static_cast<const int32_t*>(t.data_ptr());
+    p.parent_stride = shared ? 0 : t.stride(0);
+  }
+  if (draft_lens.has_value()) p.draft_lens = ints(*draft_lens, "draft_lens", {B}, logits.device());
+  at::Tensor paths = at::empty({B, T}, logits.options().dtype(at::kInt));
+  at::Tensor counts = at::empty({B}, logits.options().dtype(at::kInt));
+  at::Tensor next = at::empty({B}, logits.options().dtype(at::kLong));
+  p.logits = logits.data_ptr();
+  p.logits_stride[0] = logits.stride(0);
+  p.logits_stride[1] = logits.stride(1);
+  p.tokens = tokens.data_ptr();
+  p.token_stride = tokens.stride(0);
+  p.wide_tokens = tokens.scalar_type() == at::kLong;
+  p.uniforms = static_cast<const float*>(uniforms.data_ptr());
+  p.uniform_stride = uniforms.stride(0);
+  p.paths = static_cast<int32_t*>(paths.data_ptr());
+  p.counts = static_cast<int32_t*>(counts.data_ptr());
+  p.next = static_cast<int64_t*>(next.data_ptr());
+  p.batch = B;
+  p.nodes = T;
+  p.vocab = V;
+  p.temperature = temperature;
+  p.error_word = reinterpret_cast<int32_t*>(static_cast<intptr_t>(error_word));
+  raise_code("b200_verify_drafts", b200_verify_drafts(&p, stream_of(logits)));
+  return {paths, counts, next};
 }
 
 }  // namespace
@@ -449,6 +616,15 @@ TORCH_LIBRARY(b200, m) {
       "cache_append(Tensor k_new, Tensor v_new, Tensor(a!) k_pages, Tensor(b!) v_pages, "
       "Tensor page_table, Tensor seq_lens, Tensor? draft_lens, int error_word) -> ()",
       &cache_append);
+  m.def(
+      "cache_read(Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor starts, int tokens, "
+      "int head_dim, ScalarType dtype, Tensor? counts, int error_word) -> (Tensor, Tensor)",
+      &cache_read);
+  m.def(
+      "verify_drafts(Tensor logits, Tensor tokens, Tensor uniforms, Tensor? draft_probs, "
+      "Tensor? parents, Tensor? draft_lens, float temperature, int error_word) -> "
+      "(Tensor, Tensor, Tensor)",
+      &verify_drafts);
   m.def(
       "cache_accept(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor seq_lens, "
       "Tensor paths, Tensor counts, int error_word) -> Tensor",

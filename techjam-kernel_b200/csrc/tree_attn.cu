@@ -10,6 +10,7 @@
 #include "error_word.cuh"
 #include "paged_host.h"
 #include "tree_attn.cuh"
+#include "tree_attn_host.cuh"
 #include "tree_attn_rows.cuh"
 
 namespace b200tree {
@@ -240,8 +241,6 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(const __grid_constant__
 // -------------------------------------------------------------------- host
 using namespace b200paged;
 
-int64_t round16(int64_t n) { return (n + 15) & ~static_cast<int64_t>(15); }
-
 // The kernel a call takes, its row tile (`rm` places, `rows` of them used), key tile and
 // padded head dim, and the most CTAs it may run on an SM.
 enum Kernel { kPlain, kFewRows, kManyRows };
@@ -292,35 +291,6 @@ Choice choose(const b200_tree_attn_params* p) {
   return Choice{kFewRows, 32, 32, RowShape<2, false, 64>::kTile, dp, 1};
 }
 
-// Whether the output can share bytes with what the call reads, or with itself.  In the place
-// of the queries, element for element, it may: a unit's rows are written when all its CTAs have
-// read its queries.
-bool output_collides(const b200_tree_attn_params* p) {
-  using b200attn::may_overlap;
-  using b200attn::stretches_of;
-  const b200_cache& c = p->cache;
-  const int64_t eb = elem_bytes(c.dtype);
-  const int64_t rows[3] = {c.batch, p->heads, p->tokens};
-  const int64_t pool[3] = {c.pages, c.kv_heads, c.page_size};
-  bool in_place = p->q == p->o;
-  for (int d = 0; d < 3; ++d) {
-    if (rows[d] <= 1) continue;
-    if (p->o_stride[d] == 0) return true;
-    in_place = in_place && p->o_stride[d] == p->q_stride[d];
-  }
-  const auto o = stretches_of(p->o, p->o_stride, rows, 3, c.head_dim, eb);
-  if (!in_place && may_overlap(o, stretches_of(p->q, p->q_stride, rows, 3, c.head_dim, eb)))
-    return true;
-  if (may_overlap(o, stretches_of(c.k, c.k_stride + 1, pool, 3, c.head_dim, eb)) ||
-      may_overlap(o, stretches_of(c.v, c.v_stride + 1, pool, 3, c.head_dim, eb)) ||
-      may_overlap(o, stretches_of(c.page_table, &c.table_stride, &c.batch, 1, c.slots, 4)) ||
-      may_overlap(o, stretches_of(c.seq_lens, nullptr, nullptr, 0, c.batch, 4)))
-    return true;
-  const int64_t marks[3] = {c.batch, p->tokens, p->tokens};
-  return (p->mask && may_overlap(o, stretches_of(p->mask, p->mask_stride, marks, 3, 1, 1))) ||
-         (p->draft_lens && may_overlap(o, stretches_of(p->draft_lens, nullptr, nullptr, 0, c.batch, 4)));
-}
-
 int64_t row_tiles(const b200_tree_attn_params* p, const Choice& c) {
   return (p->tokens * (p->heads / p->cache.kv_heads) + c.rows - 1) / c.rows;
 }
@@ -328,11 +298,6 @@ int64_t row_tiles(const b200_tree_attn_params* p, const Choice& c) {
 int64_t units_of(const b200_tree_attn_params* p, const Choice& c) {
   return p->cache.batch * p->cache.kv_heads * row_tiles(p, c);
 }
-
-// Most SMs that a call runs on.  Workspaces are sized on the host for as many, without asking
-// a device: more than the 148 of a B200, and every one counts (256 rows of 128 columns: 42.6 MB
-// for 160 SMs).
-constexpr int64_t kMaxSms = 160;
 
 // Whether the cut units of few rows get a join kernel of their own although the attention
 // kernel could join them: a long context of several rows leaves many partial results to the one
@@ -359,15 +324,6 @@ int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
 }
 
 
-template <int RM, int DP, int DT, int WARPS>
-int32_t run_join_rows(const Args& a, int64_t units, bool spread, cudaStream_t s) {
-  if (spread)
-    return launch(join_spread_kernel<RM, DP, DT>, dim3(static_cast<unsigned>(units), RM / 4),
-                  dim3(32 * kJoinWarps), 0, s, a);
-  return launch(join_rows_kernel<RM, DP, DT, WARPS>, dim3(static_cast<unsigned>(units)),
-                dim3(32 * WARPS), 0, s, a);
-}
-
 template <int RM, int DP, int DT>
 int32_t run_join_columns(const Args& a, int64_t units, cudaStream_t s) {
   // few units: the blocks that share a unit's rows share its columns too
@@ -377,21 +333,6 @@ int32_t run_join_columns(const Args& a, int64_t units, cudaStream_t s) {
                 dim3(32 * kJoinWarps), 0, s, a);
 }
 
-template <int RM, int DP, int DT>
-int32_t run_one(void (*kernel)(Args), int threads, int smem, const Args& a, int runs, int device,
-                cudaStream_t s) {
-  static std::once_flag once[kMaxDevices];
-  static cudaError_t err[kMaxDevices];
-  std::call_once(once[device], [&] {
-    err[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  });
-  if (err[device] != cudaSuccess) {
-    set_error(cudaGetErrorString(err[device]));
-    return B200_ATTN_ERR_LAUNCH;
-  }
-  return launch(kernel, dim3(runs), dim3(threads), smem, s, a);
-}
-
 // One kernel over the runs, and where it does not join the units that were cut, one that
 // does.
 template <int DP, int DT>
@@ -399,8 +340,7 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, bool 
                   cudaStream_t s) {
   int32_t rc;
   if constexpr (DT == B200_ATTN_DTYPE_FP32) {
-    rc = run_one<16, DP, DT>(plain_kernel<DP, DT>, kThreads, sizeof(PlainSmem<DP>), a, runs, device,
-                             s);
+    rc = run_one<plain_kernel<DP, DT>>(kThreads, sizeof(PlainSmem<DP>), a, runs, device, s);
     return rc != B200_ATTN_OK || a.counters ? rc : run_join_rows<kRows, DP, DT, kThreads / 32>(a, units, spread, s);
   } else {
     using Few = RowShape<1, true, DP>;
@@ -409,13 +349,11 @@ int32_t run_width(const Choice& c, const Args& a, int runs, int64_t units, bool 
     if (c.kernel == kManyRows)
       rc = launch_tiles(c.rm, c.dp, DT, a, a.kv_heads * a.group, runs, device, s);
     else if (a.tokens * a.group <= 8)
-      rc = run_one<8, DP, DT>(rows_kernel<Few, DT>, Few::kThreads, Few::kSmemBytes, a, runs, device, s);
+      rc = run_one<rows_kernel<Few, DT>>(Few::kThreads, Few::kSmemBytes, a, runs, device, s);
     else if (c.rm == 16)
-      rc = run_one<16, DP, DT>(rows_kernel<One, DT>, One::kThreads, One::kSmemBytes, a, runs, device,
-                               s);
+      rc = run_one<rows_kernel<One, DT>>(One::kThreads, One::kSmemBytes, a, runs, device, s);
     else
-      rc = run_one<32, DP, DT>(rows_kernel<Two, DT>, Two::kThreads, Two::kSmemBytes, a, runs, device,
-                               s);
+      rc = run_one<rows_kernel<Two, DT>>(Two::kThreads, Two::kSmemBytes, a, runs, device, s);
     if (rc != B200_ATTN_OK || a.counters) return rc;
     switch (c.rm) {
       case 16: return run_join_rows<16, DP, DT, One::kWarps>(a, units, spread, s);
@@ -464,7 +402,7 @@ extern "C" int32_t b200_tree_attn_check(const b200_tree_attn_params* p) {
     return B200_ATTN_ERR_INVALID_ARGUMENT;
   if (p->mask && (p->mask_stride[0] < 0 || p->mask_stride[1] < 0 || p->mask_stride[2] < 0))
     return B200_ATTN_ERR_INVALID_ARGUMENT;
-  if (output_collides(p)) return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (output_collides(p, c.head_dim, eb)) return B200_ATTN_ERR_INVALID_ARGUMENT;
   return B200_ATTN_OK;
 }
 
@@ -487,38 +425,7 @@ extern "C" int32_t b200_tree_attn_fwd(const b200_tree_attn_params* p, void* stre
   const int64_t eb = b200paged::elem_bytes(c.dtype);
   Args a{};
   if ((rc = b200attn::resolve_error_word(c.error_word, &a.err)) != B200_ATTN_OK) return rc;
-  a.k = static_cast<const uint8_t*>(c.k);
-  a.v = static_cast<const uint8_t*>(c.v);
-  a.k_page = c.k_stride[1] * eb;
-  a.k_head = c.k_stride[2] * eb;
-  a.k_row = c.k_stride[3] * eb;
-  a.v_page = c.v_stride[1] * eb;
-  a.v_head = c.v_stride[2] * eb;
-  a.v_row = c.v_stride[3] * eb;
-  a.table = c.page_table;
-  a.table_stride = c.table_stride;
-  a.lens = c.seq_lens;
-  a.drafts = p->draft_lens;
-  a.q = static_cast<const uint8_t*>(p->q);
-  a.o = static_cast<uint8_t*>(p->o);
-  a.q_seq = p->q_stride[0] * eb;
-  a.q_head = p->q_stride[1] * eb;
-  a.q_tok = p->q_stride[2] * eb;
-  a.o_seq = p->o_stride[0] * eb;
-  a.o_head = p->o_stride[1] * eb;
-  a.o_tok = p->o_stride[2] * eb;
-  a.mask = p->mask;
-  a.m_seq = p->mask_stride[0];
-  a.m_row = p->mask_stride[1];
-  a.m_col = p->mask_stride[2];
-  a.batch = static_cast<int32_t>(c.batch);
-  a.kv_heads = static_cast<int32_t>(c.kv_heads);
-  a.group = static_cast<int32_t>(p->heads / c.kv_heads);
-  a.tokens = static_cast<int32_t>(p->tokens);
-  a.head_dim = static_cast<int32_t>(c.head_dim);
-  a.slots = static_cast<int32_t>(c.slots);
-  a.pages = static_cast<int32_t>(c.pages);
-  a.page_size = static_cast<int32_t>(c.page_size);
+  fill_args(p, eb, eb, c.head_dim, &a);
   a.unit_rows = ch.rows;
   a.row_tiles = static_cast<int32_t>(row_tiles(p, ch));
   a.scale_log2 = p->scale * 1.4426950408889634f;

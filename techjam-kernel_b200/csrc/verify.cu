@@ -1,0 +1,630 @@
+// verify.cu — the check of drafted tokens against the target's probabilities
+// (definition: b200_verify.h).
+//
+// A cluster of CTAs walks the tree of one sequence.  Only the rows of the nodes on the path
+// are read, each by all CTAs of the cluster, a contiguous share a warp; the CTAs
+// exchange their sums through distributed shared memory and all take the same decisions.  A
+// step down the tree is one pass over a row (maximum and sum of exponentials, fp32).  Refused
+// drafts with probabilities take further passes over the row of the target and that of
+// the drafter, which lie in L2 by then: the sum again in 64 bits, and the sum of what is left
+// after each refusal.  The last pass's sums, a warp each, say in which share the next token lies;
+// it is divided among the warps of its CTA once more, and one warp scans the part.
+// Exponentials and sums that the next token hangs on are 64-bit: among 32000 cumulated
+// weights a sum that is off by 1e-8 would pick a neighbour once in some thousand draws.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "b200_verify.h"
+#include "byte_range.h"
+#include "error_word.cuh"
+#include "paged_host.h"
+#include "sm100_ptx.cuh"
+#include "tree_attn.cuh"
+
+namespace b200verify {
+
+using b200attn::report_error;
+using b200tree::Elem;
+
+namespace {
+
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kMaxCluster = 8;
+constexpr int kMaxNodes = B200_VERIFY_MAX_NODES;
+constexpr uint32_t kAll = 0xffffffffu;
+
+struct Args {
+  const uint8_t* logits;
+  int64_t l_seq, l_node;  // bytes
+  const uint8_t* probs;   // null: drafts count as certain
+  int64_t q_seq, q_node;
+  const uint8_t* tokens;
+  int64_t t_seq;  // elements
+  const float* uniforms;
+  int64_t u_seq;
+  const int32_t* parents;  // null: a chain
+  int64_t p_seq;
+  const int32_t* lens;
+  int32_t* paths;
+  int32_t* counts;
+  int64_t* next;
+  double inv_temp;  // 0: the largest logit
+  int32_t nodes, vocab, share;  // share: numbers of a warp, a multiple of 4
+  int32_t probs_type, wide_tokens;
+  bool probs_vec;
+  int32_t* err;
+};
+
+struct Exchange {  // what a CTA tells the others
+  double sum;
+  float top;
+  int32_t at;  // of the largest number
+  int32_t bad;
+};
+
+struct Smem {
+  Exchange told[2][kMaxCluster];
+  Exchange warp[kWarps];
+  double warp_sum[kWarps];
+  double part_sum[kWarps];
+  double z[kMaxNodes];        // sums of what was left after each refusal at a node
+  int32_t parent[kMaxNodes];
+  int32_t token[kMaxNodes];   // -1: out of range
+  float uniform[kMaxNodes];
+  float logit[kMaxNodes];     // the target's for the node's token, in its parent's row
+  float prob[kMaxNodes];      // the drafter's
+  int32_t refused[kMaxNodes]; // tokens refused at this node that have no weight any more
+  int32_t path[kMaxNodes];
+};
+
+// Four numbers of a row from number v on; `vec`: by one load where all four are there.
+template <int DT, class T = typename Elem<DT>::T>
+__device__ __forceinline__ void load4(const uint8_t* row, int v, int end, bool vec, float fill,
+                                      float (&x)[4]) {
+  const T* p = reinterpret_cast<const T*>(row) + v;
+  if (vec && v + 4 <= end) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 w = __ldg(reinterpret_cast<const float4*>(p));
+      x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+    } else {
+      union {
+        uint2 w;
+        T e[4];
+      } u;
+      u.w = __ldg(reinterpret_cast<const uint2*>(p));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = Elem<DT>::widen(u.e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v + i < end ? Elem<DT>::widen(p[i]) : fill;
+  }
+}
+
+__device__ __forceinline__ float as_prob(float q) { return q > 0.f ? q : 0.f; }
+
+__device__ __forceinline__ void probs4(const Args& a, const uint8_t* row, int v, int end,
+                                       float (&q)[4]) {
+  if (a.probs_type == B200_ATTN_DTYPE_FP32)
+    load4<B200_ATTN_DTYPE_FP32>(row, v, end, a.probs_vec, 0.f, q);
+  else if (a.probs_type == B200_ATTN_DTYPE_BF16)
+    load4<B200_ATTN_DTYPE_BF16>(row, v, end, a.probs_vec, 0.f, q);
+  else
+    load4<B200_ATTN_DTYPE_FP16>(row, v, end, a.probs_vec, 0.f, q);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = as_prob(q[i]);
+}
+
+__device__ __forceinline__ float one_prob(const Args& a, const uint8_t* row, int v) {
+  if (a.probs_type == B200_ATTN_DTYPE_FP32) return as_prob(reinterpret_cast<const float*>(row)[v]);
+  if (a.probs_type == B200_ATTN_DTYPE_BF16)
+    return as_prob(__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[v]));
+  return as_prob(__half2float(reinterpret_cast<const __half*>(row)[v]));
+}
+
+// What is known of the node that the path has reached.
+struct Node {
+  const uint8_t* row;
+  const uint8_t* probs;
+  float top;       // largest logit
+  double sum;      // of exp((l - top) / T): of fp32 exponentials, until it is needed in 64 bits
+  bool exact;      // sum is the 64-bit one
+  int refusals;    // sums in z, or tokens in `refused`
+};
+
+__device__ __forceinline__ double weight(const Args& a, float l, float top) {
+  return exp((static_cast<double>(l) - static_cast<double>(top)) * a.inv_temp);
+}
+
+// The weight that is left of `e` after the node's refusals, with the drafter's q.
+__device__ __forceinline__ double left_of(const Smem& sm, const Node& n, int level, double e,
+                                          double q) {
+  double y = e;
+  if (level > 0) {
+    y = fmax(y / n.sum - q, 0.0);
+    for (int j = 1; j < level; ++j) y = fmax(y / sm.z[j - 1] - q, 0.0);
+  }
+  return y;
+}
+
+// Four such weights from number v on.
+template <int DT>
+__device__ __forceinline__ void weights4(const Args& a, const Smem& sm, const Node& n, int level,
+                                         int v, int end, bool vec, double (&y)[4]) {
+  float l[4], q[4] = {0.f, 0.f, 0.f, 0.f};
+  load4<DT>(n.row, v, end, vec, -INFINITY, l);
+  if (level > 0) probs4(a, n.probs, v, end, q);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    double e = l[i] == -INFINITY ? 0.0 : weight(a, l[i], n.top);
+    if (!a.probs)
+      for (int j = 0; j < n.refusals; ++j)
+        if (sm.refused[j] == v + i) e = 0.0;
+    y[i] = left_of(sm, n, level, e, q[i]);
+  }
+}
+
+__device__ __forceinline__ double warp_total(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
+  return x;
+}
+
+// Tells `mine` (thread 0's) to every CTA of the cluster; by all threads of all CTAs.  Two
+// slots in turn: a CTA writes a slot again when all have passed the barrier after reading it.
+__device__ __forceinline__ void tell(Smem& sm, int& turn, const Exchange& mine, uint32_t rank,
+                                     uint32_t ctas) {
+  turn ^= 1;
+  if (threadIdx.x < ctas) {
+    const uint32_t at = b200attn::ptx::mapa_shared(
+        b200attn::ptx::smem_u32(&sm.told[turn][rank]), threadIdx.x);
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(mine.sum) : "memory");
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(mine.top) : "memory");
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + 12), "r"(mine.at) : "memory");
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + 16), "r"(mine.bad) : "memory");
+  }
+  b200attn::ptx::cluster_sync();
+}
+
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_constant__ Args a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t ctas = gridDim.x, rank = blockIdx.x;  // one cluster a sequence
+  const int64_t b = blockIdx.y;
+  b200attn::ptx::launch_dependents();
+  b200attn::ptx::grid_dependency_wait();
+
+  int n = a.lens ? a.lens[b] : a.nodes;
+  if (n < 0 || n > a.nodes) {
+    if (tid == 0 && rank == 0) report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
+    n = 0;
+  }
+  const uint8_t* logits = a.logits + b * a.l_seq;
+  const uint8_t* probs = a.probs ? a.probs + b * a.q_seq : nullptr;
+  for (int i = tid; i < n; i += kThreads) {
+    int parent = a.parents ? a.parents[b * a.p_seq + i] : i - 1;
+    sm.uniform[i] = a.uniforms[b * a.u_seq + i];
+    if (i == 0) {
+      sm.parent[0] = -1;
+      continue;
+    }
+    const int64_t t = a.wide_tokens ? reinterpret_cast<const int64_t*>(a.tokens)[b * a.t_seq + i]
+                                    : reinterpret_cast<const int32_t*>(a.tokens)[b * a.t_seq + i];
+    const bool known = t >= 0 && t < a.vocab;
+    if (parent < -1 || parent >= i || !known) {
+      if (rank == 0) report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
+      parent = -1;
+    }
+    sm.parent[i] = parent;
+    sm.token[i] = static_cast<int>(t);
+    if (parent >= 0) {
+      const uint8_t* row = logits + parent * a.l_node;
+      sm.logit[i] = Elem<DT>::widen(reinterpret_cast<const typename Elem<DT>::T*>(row)[t]);
+      if (probs) sm.prob[i] = one_prob(a, probs + parent * a.q_node, static_cast<int>(t));
+    }
+  }
+  // every CTA of the cluster runs: its shared memory may be written
+  b200attn::ptx::cluster_sync();
+
+  const int begin = min(static_cast<int64_t>(a.vocab),
+                        static_cast<int64_t>(rank * kWarps + warp) * a.share);
+  const int end = min(static_cast<int64_t>(a.vocab), begin + static_cast<int64_t>(a.share));
+  int turn = 0, length = 0, at = 0;
+  int64_t next = -1;
+  bool teller = rank == 0;  // this CTA writes the next token
+  Node node{};
+
+  // Sums the weights that are left after `level` refusals: sm.warp_sum a warp of this CTA, told[turn] a
+  // CTA, and in all.
+  auto total_of = [&](int level) {
+    double s = 0.0;
+    for (int v = begin + 4 * lane; v < end; v += 128) {
+      double y[4];
+      weights4<DT>(a, sm, node, level, v, end, VEC, y);
+      s += (y[0] + y[1]) + (y[2] + y[3]);
+    }
+    s = warp_total(s);
+    __syncthreads();
+    if (lane == 0) sm.warp_sum[warp] = s;
+    __syncthreads();
+    Exchange mine{0.0, 0.f, 0, 0};
+    for (int w = 0; w < kWarps; ++w) mine.sum += sm.warp_sum[w];
+    tell(sm, turn, mine, rank, ctas);
+    double total = 0.0;
+    for (uint32_t c = 0; c < ctas; ++c) total += sm.told[turn][c].sum;
+    return total;
+  };
+
+  while (n > 0) {
+    // ------------------------------------- a node: its largest logit and its sum
+    if (tid == 0 && rank == 0) sm.path[length] = at;
+    ++length;
+    node.row = logits + at * a.l_node;
+    node.probs = probs ? probs + at * a.q_node : nullptr;
+    node.exact = false;
+    node.refusals = 0;
+    float top = -INFINITY, sum = 0.f;
+    int where = 0;
+    bool bad = false;
+    const float to_log2 = static_cast<float>(a.inv_temp * 1.4426950408889634);
+    for (int v = begin + 4 * lane; v < end; v += 4 * 128) {
+      float l[4][4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (v + 128 * u < end) {
+          load4<DT>(node.row, v + 128 * u, end, VEC, -INFINITY, l[u]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l[u][i] = -INFINITY;
+        }
+      }
+      float big = top;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          bad |= !(l[u][i] < INFINITY);
+          if (l[u][i] > big) {
+            big = l[u][i];
+            where = v + 128 * u + i;
+          }
+        }
+      if (big == -INFINITY) continue;
+      sum *= exp2f((top - big) * to_log2);
+      top = big;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += exp2f((l[u][i] - big) * to_log2);
+    }
+    Exchange mine{sum, top, where, bad ? 1 : 0};
+    auto take = [&](Exchange& x, const Exchange& y) {  // y lies behind or before x
+      const float big = fmaxf(x.top, y.top);
+      if (y.top > x.top || (y.top == x.top && y.at < x.at)) x.at = y.at;
+      if (big > -INFINITY)
+        x.sum = x.sum * exp2f((x.top - big) * to_log2) + y.sum * exp2f((y.top - big) * to_log2);
+      x.top = big;
+      x.bad |= y.bad;
+    };
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      Exchange y;
+      y.sum = __shfl_xor_sync(kAll, mine.sum, o);
+      y.top = __shfl_xor_sync(kAll, mine.top, o);
+      y.at = __shfl_xor_sync(kAll, mine.at, o);
+      y.bad = __shfl_xor_sync(kAll, mine.bad, o);
+      take(mine, y);
+    }
+    __syncthreads();
+    if (lane == 0) sm.warp[warp] = mine;
+    __syncthreads();
+    mine = sm.warp[0];
+    for (int w = 1; w < kWarps; ++w) take(mine, sm.warp[w]);
+    tell(sm, turn, mine, rank, ctas);
+    mine = sm.told[turn][0];
+    for (uint32_t c = 1; c < ctas; ++c) take(mine, sm.told[turn][c]);
+    node.top = mine.top;
+    node.sum = mine.sum;
+    const bool none = mine.bad || mine.top == -INFINITY;  // no distribution
+    if (none) break;
+
+    // --------------------------------------------------- its children in order
+    int kept = -1;
+    double gone = 0.0;   // weight of the refused tokens, where drafts count as certain
+    bool summed = false; // warp_sum and told hold what is left now
+    double left = 0.0;   // its sum
+    for (int i0 = at + 1; i0 < n && kept < 0; i0 += 32) {
+      uint32_t mask = __ballot_sync(kAll, i0 + lane < n && sm.parent[i0 + lane] == at);
+      while (mask != 0u && kept < 0) {
+        const int c = i0 + __ffs(mask) - 1;
+        mask &= mask - 1;
+        if (a.inv_temp == 0.0) {
+          if (sm.token[c] == mine.at && sm.uniform[c] < 1.f) kept = c;
+          continue;
+        }
+        const double e = sm.logit[c] == -INFINITY ? 0.0 : weight(a, sm.logit[c], node.top);
+        const double u = static_cast<double>(sm.uniform[c]);
+        if (!probs) {
+          bool again = false;
+          for (int j = 0; j < node.refusals; ++j) again |= sm.refused[j] == sm.token[c];
+          if (again) continue;
+          if (u * (node.sum - gone) < e) {
+            kept = c;
+            continue;
+          }
+          if (node.sum - gone - e > 0.0) {  // something is left without it
+            gone += e;
+            __syncthreads();
+            if (tid == 0) sm.refused[node.refusals] = sm.token[c];
+            __syncthreads();
+            ++node.refusals;
+          }
+          continue;
+        }
+        const double q = static_cast<double>(sm.prob[c]);
+        const double y = left_of(sm, node, node.refusals, e, q);
+        const double of = node.refusals > 0 ? sm.z[node.refusals - 1] : node.sum;
+        if (u * q * of < y) {
+          kept = c;
+          continue;
+        }
+        if (!node.exact) {
+          node.sum = total_of(0);
+          node.exact = true;
+        }
+        const double rest = total_of(node.refusals + 1);
+        summed = rest > 0.0;
+        if (summed) {
+          left = rest;
+          __syncthreads();
+          if (tid == 0) sm.z[node.refusals] = rest;
+          __syncthreads();
+          ++node.refusals;
+        }
+      }
+    }
+    if (kept >= 0) {
+      at = kept;
+      continue;
+    }
+    // ------------------------------------------------------- the next token
+    if (a.inv_temp == 0.0) {
+      next = mine.at;
+      break;
+    }
+    const int level = probs ? node.refusals : 0;
+    if (!summed) left = total_of(level);
+    if (!(left > 0.0)) {  // only by the rounding of the row's sum: refusals leave something
+      next = mine.at;
+      break;
+    }
+    const double goal = static_cast<double>(sm.uniform[0]) * left;
+    // the CTA, then the warp, then the part of its share that the goal lies in: the first
+    // whose end is past it, or else the last with any weight
+    double before = 0.0;
+    auto find = [&](auto sums, int count) {
+      double cum = before, from = before;
+      int best = -1;
+      for (int i = 0; i < count; ++i) {
+        const double s = sums(i);
+        if (s > 0.0) {
+          best = i;
+          from = cum;
+          if (cum + s > goal) break;
+        }
+        cum += s;
+      }
+      before = from;
+      return best;
+    };
+    const int cta = find([&](int i) { return sm.told[turn][i].sum; }, static_cast<int>(ctas));
+    teller = cta == static_cast<int>(rank);
+    if (!teller) break;
+    const int owner = find([&](int i) { return sm.warp_sum[i]; }, kWarps);
+    const int part = (a.share / 4 + kWarps - 1) / kWarps * 4;
+    const int from = min(static_cast<int64_t>(a.vocab),
+                         static_cast<int64_t>(rank * kWarps + owner) * a.share);
+    const int to = min(static_cast<int64_t>(a.vocab), from + static_cast<int64_t>(a.share));
+    {
+      double s = 0.0;
+      const int stop = min(to, from + (warp + 1) * part);
+      for (int v = from + warp * part + 4 * lane; v < stop; v += 128) {
+        double y[4];
+        weights4<DT>(a, sm, node, level, v, stop, VEC, y);
+        s += (y[0] + y[1]) + (y[2] + y[3]);
+      }
+      s = warp_total(s);
+      if (lane == 0) sm.part_sum[warp] = s;
+      __syncthreads();
+    }
+    const int which = find([&](int i) { return sm.part_sum[i]; }, kWarps);
+    if (warp == 0) {
+      const int stop = min(to, from + (which + 1) * part);
+      int found = -1, last = -1;
+      for (int v0 = from + which * part; v0 < stop && found < 0; v0 += 128) {
+        const int v = v0 + 4 * lane;
+        double y[4] = {0.0, 0.0, 0.0, 0.0};
+        if (v < stop) weights4<DT>(a, sm, node, level, v, stop, VEC, y);
+        double mine4 = (y[0] + y[1]) + (y[2] + y[3]), cum = mine4;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double t = __shfl_up_sync(kAll, cum, o);
+          if (lane >= o) cum += t;
+        }
+        const double all = __shfl_sync(kAll, cum, 31);
+        double run = before + (cum - mine4);
+        int first = -1, some = -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          run += y[i];
+          if (y[i] > 0.0) {
+            some = v + i;
+            if (first < 0 && run > goal) first = v + i;
+          }
+        }
+        const uint32_t hit = __ballot_sync(kAll, first >= 0), any = __ballot_sync(kAll, some >= 0);
+        if (hit) found = __shfl_sync(kAll, first, __ffs(hit) - 1);
+        if (any) last = __shfl_sync(kAll, some, 31 - __clz(any));
+        before += all;
+      }
+      next = found >= 0 ? found : last;
+    }
+    break;
+  }
+  // ---------------------------------------------------------------- results
+  if (rank == 0) {
+    __syncthreads();
+    for (int i = tid; i < a.nodes; i += kThreads)
+      a.paths[b * a.nodes + i] = i < length ? sm.path[i] : -1;
+    if (tid == 0) a.counts[b] = length;
+  }
+  if (teller && tid == 0) a.next[b] = next;
+}
+
+// -------------------------------------------------------------------- host
+using namespace b200paged;
+
+int32_t launch_cluster(void (*kernel)(Args), const Args& a, unsigned ctas, int64_t batch,
+                       cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas, static_cast<unsigned>(batch));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error(cudaGetErrorString(e));
+    return B200_ATTN_ERR_LAUNCH;
+  }
+  count_launch();
+  return B200_ATTN_OK;
+}
+static_assert(sizeof(Smem) <= 48 * 1024, "no opt-in needed");
+
+// Rows of four numbers can be read by one load.
+bool by_fours(const void* base, const int64_t* stride, const int64_t* extent, int64_t eb) {
+  if (reinterpret_cast<uintptr_t>(base) % (4 * eb)) return false;
+  for (int d = 0; d < 2; ++d)
+    if (extent[d] > 1 && stride[d] % 4) return false;
+  return true;
+}
+
+template <int DT>
+int32_t run(const Args& a, bool vec, unsigned ctas, int64_t batch, cudaStream_t s) {
+  return launch_cluster(vec ? verify_kernel<DT, true> : verify_kernel<DT, false>, a, ctas, batch, s);
+}
+
+}  // namespace
+}  // namespace b200verify
+
+using namespace b200verify;
+
+extern "C" int32_t b200_verify_check(const b200_verify_params* p) {
+  using b200attn::may_overlap;
+  using b200attn::stretches_of;
+  if (!p || !p->logits || !p->tokens || !p->uniforms || !p->paths || !p->counts || !p->next ||
+      p->reserved != 0 || (p->wide_tokens & ~1))
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (p->batch < 1 || p->batch > 65535 || p->nodes < 1 || p->nodes > B200_VERIFY_MAX_NODES ||
+      p->vocab < 1 || p->vocab > B200_VERIFY_MAX_VOCAB)
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (!(p->temperature >= 0.0) || !std::isfinite(p->temperature) ||
+      (p->temperature > 0.0 && !std::isfinite(1.0 / p->temperature)))
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (!known_dtype(p->dtype) || (p->draft_probs && !known_dtype(p->draft_dtype)))
+    return B200_ATTN_ERR_UNSUPPORTED;
+  const int64_t eb = elem_bytes(p->dtype), qb = elem_bytes(p->draft_dtype);
+  const int64_t tb = p->wide_tokens ? 8 : 4;
+  const int64_t extent[2] = {p->batch, p->nodes}, rows[2] = {p->batch, p->nodes - 1};
+  for (int d = 0; d < 2; ++d)
+    if ((extent[d] > 1 && p->logits_stride[d] < 0) ||
+        (p->draft_probs && rows[d] > 1 && p->draft_stride[d] < 0))
+      return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (p->batch > 1 && (p->token_stride < 0 || p->uniform_stride < 0 || p->parent_stride < 0))
+    return B200_ATTN_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(p->logits) % eb ||
+      (p->draft_probs && reinterpret_cast<uintptr_t>(p->draft_probs) % qb) ||
+      reinterpret_cast<uintptr_t>(p->tokens) % tb || (reinterpret_cast<uintptr_t>(p->next) & 7u) ||
+      ((reinterpret_cast<uintptr_t>(p->uniforms) | reinterpret_cast<uintptr_t>(p->parents) |
+        reinterpret_cast<uintptr_t>(p->draft_lens) | reinterpret_cast<uintptr_t>(p->paths) |
+        reinterpret_cast<uintptr_t>(p->counts)) & 3u))
+    return B200_ATTN_ERR_ALIGNMENT;
+  // no output shares a byte with an input or another output
+  const b200attn::Stretches outs[3] = {
+      stretches_of(p->paths, nullptr, nullptr, 0, p->batch * p->nodes, 4),
+      stretches_of(p->counts, nullptr, nullptr, 0, p->batch, 4),
+      stretches_of(p->next, nullptr, nullptr, 0, p->batch, 8)};
+  for (int i = 0; i < 3; ++i) {
+    const auto& o = outs[i];
+    for (int j = 0; j < i; ++j)
+      if (may_overlap(o, outs[j])) return B200_ATTN_ERR_INVALID_ARGUMENT;
+    if (may_overlap(o, stretches_of(p->logits, p->logits_stride, extent, 2, p->vocab, eb)) ||
+        (p->draft_probs && p->nodes > 1 &&
+         may_overlap(o, stretches_of(p->draft_probs, p->draft_stride, rows, 2, p->vocab, qb))) ||
+        may_overlap(o, stretches_of(p->tokens, &p->token_stride, &p->batch, 1, p->nodes, tb)) ||
+        may_overlap(o, stretches_of(p->uniforms, &p->uniform_stride, &p->batch, 1, p->nodes, 4)) ||
+        (p->parents &&
+         may_overlap(o, stretches_of(p->parents, &p->parent_stride, &p->batch, 1, p->nodes, 4))) ||
+        (p->draft_lens && may_overlap(o, stretches_of(p->draft_lens, nullptr, nullptr, 0, p->batch, 4))))
+      return B200_ATTN_ERR_INVALID_ARGUMENT;
+  }
+  return B200_ATTN_OK;
+}
+
+extern "C" int32_t b200_verify_drafts(const b200_verify_params* p, void* stream) {
+  int32_t rc = b200_verify_check(p);
+  if (rc != B200_ATTN_OK) return rc;
+  b200paged::DeviceScope scope;
+  if ((rc = scope.enter(p->logits, "logits are not device memory")) != B200_ATTN_OK) return rc;
+  Args a{};
+  if ((rc = b200attn::resolve_error_word(p->error_word, &a.err)) != B200_ATTN_OK) return rc;
+  const int64_t eb = elem_bytes(p->dtype), qb = elem_bytes(p->draft_dtype);
+  const int64_t extent[2] = {p->batch, p->nodes}, rows[2] = {p->batch, p->nodes - 1};
+  a.logits = static_cast<const uint8_t*>(p->logits);
+  a.l_seq = p->logits_stride[0] * eb;
+  a.l_node = p->logits_stride[1] * eb;
+  if (p->draft_probs && p->temperature > 0.0) {
+    a.probs = static_cast<const uint8_t*>(p->draft_probs);
+    a.q_seq = p->draft_stride[0] * qb;
+    a.q_node = p->draft_stride[1] * qb;
+    a.probs_type = p->draft_dtype;
+    a.probs_vec = by_fours(p->draft_probs, p->draft_stride, rows, qb);
+  }
+  a.tokens = static_cast<const uint8_t*>(p->tokens);
+  a.t_seq = p->token_stride;
+  a.uniforms = p->uniforms;
+  a.u_seq = p->uniform_stride;
+  a.parents = p->parents;
+  a.p_seq = p->parent_stride;
+  a.lens = p->draft_lens;
+  a.paths = p->paths;
+  a.counts = p->counts;
+  a.next = p->next;
+  a.inv_temp = p->temperature > 0.0 ? 1.0 / p->temperature : 0.0;
+  a.nodes = static_cast<int32_t>(p->nodes);
+  a.vocab = static_cast<int32_t>(p->vocab);
+  a.wide_tokens = p->wide_tokens;
+  const unsigned ctas = p->vocab > 16384 ? 8 : (p->vocab > 4096 ? 4 : 1);
+  const int64_t warps = static_cast<int64_t>(ctas) * kWarps;
+  a.share = static_cast<int32_t>((p->vocab + 4 * warps - 1) / (4 * warps) * 4);
+  const bool vec = by_fours(p->logits, p->logits_stride, extent, eb);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (p->dtype) {
+    case B200_ATTN_DTYPE_BF16: return run<B200_ATTN_DTYPE_BF16>(a, vec, ctas, p->batch, s);
+    case B200_ATTN_DTYPE_FP16: return run<B200_ATTN_DTYPE_FP16>(a, vec, ctas, p->batch, s);
+    default: return run<B200_ATTN_DTYPE_FP32>(a, vec, ctas, p->batch, s);
+  }
+}

@@ -46,9 +46,6 @@ struct Shape4 {
   static constexpr int kHalves = FEW ? 1 : 2;
   static constexpr int kCodes = DP / 2, kRowBytes = kCodes + 16;
   static constexpr int kPieces = kRowBytes / 16;
-  // A block's keys: codes, then what follows them (lanes read four rows' codes at once); its
-  // values: whole rows.  No read of either meets a bank twice.
-  static constexpr int kKeyMeta = kRowKeys * kCodes;
   static constexpr int kBlockBytes = kRowKeys * kRowBytes;
   static constexpr int kStages = DP == 128 ? 5 : 8;
   static constexpr int kRingBytes = kWarps * kStages * 2 * kBlockBytes;
@@ -157,58 +154,61 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   Place ld = run.p;
   bool more = !run.done(ld);
   int page = -1, page_row = 0, ld_keys = 0;
+  const uint32_t inv_size = 0xffffffffu / size + 1u;  // 0 for size 1
   auto look_up = [&]() {
     const int key = ld.t * S::kTile + warp * kRowKeys + (whole ? 0 : (lane & 15));
     ld_keys = ld.s.len + ld.s.drafts - (ld.t * S::kTile + warp * kRowKeys);
     page = -1;
     page_row = 0;
     if (key < ld.s.len + ld.s.drafts) {
-      const uint32_t slot = static_cast<uint32_t>(key) / size;
+      // key / size or one more: key is below 2^30
+      uint32_t slot = size == 1u ? key : __umulhi(key, inv_size);
+      page_row = key - static_cast<int>(slot * size);
+      if (page_row < 0) {
+        --slot;
+        page_row += static_cast<int>(size);
+      }
       page = __ldg(a.table + ld.b * a.table_stride + slot);
-      page_row = static_cast<int>(static_cast<uint32_t>(key) - slot * size);
     }
   };
   if (more) look_up();
   int stage = 0;  // stage the next loads go to
-  // this lane's 16-byte pieces of a block: row, byte in the row, place in the stage
-  constexpr int kLoads = 2 * kRowKeys * S::kPieces / 32;
-  constexpr int kHalfPieces = kRowKeys * S::kPieces;
-  static_assert(2 * kRowKeys * S::kPieces % 32 == 0, "whole warps of pieces");
+  // Rows side by side: a block's keys and values are 2 kPieces / 32 loads of 16 bytes a lane, of
+  // which the middle one takes the end of the keys and the beginning of the values.
+  const bool tight = whole && a.k_row == S::kRowBytes && a.v_row == S::kRowBytes;
+  constexpr int kKeyLoads = S::kBlockBytes / 512, kRest = S::kBlockBytes % 512;
+  static_assert(kRest == 256, "half a load of 16 bytes a lane");
   auto issue = [&]() {
     if (more) {
       if (page >= a.pages || (page < 0 && (whole ? 0 : (lane & 15)) < ld_keys)) {
         report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
         page = -1;
       }
-      const uint32_t dst = ring + stage * (2 * S::kBlockBytes);
-      const uint8_t* kb = a.k + ld.h * a.k_head;
-      const uint8_t* vb = a.v + ld.h * a.v_head;
-      if (whole && page >= 0) {
-        kb += page * a.k_page + page_row * a.k_row;
-        vb += page * a.v_page + page_row * a.v_row;
-      }
+      const uint32_t dst = ring + stage * (2 * S::kBlockBytes) + 16 * lane;
+      if (tight && page >= 0 && ld_keys >= kRowKeys) {
+        const uint8_t* ks = a.k + ld.h * a.k_head + page * a.k_page + page_row * S::kRowBytes + 16 * lane;
+        const uint8_t* vs = a.v + ld.h * a.v_head + page * a.v_page + page_row * S::kRowBytes + 16 * lane;
 #pragma unroll
-      for (int u = 0; u < kLoads; ++u) {
-        const int x = lane + 32 * u;
-        const bool value = x >= kHalfPieces;
-        const int y = value ? x - kHalfPieces : x;
-        const int r = y / S::kPieces, piece = y - r * S::kPieces;
-        int pg = page;
-        int64_t at = r;
-        if (!whole) {
-          pg = __shfl_sync(0xffffffffu, page, r);
-          at = __shfl_sync(0xffffffffu, page_row, r);
+        for (int u = 0; u < kKeyLoads; ++u) cp_async16(dst + 512 * u, ks + 512 * u, 16u);
+        cp_async16(dst + 512 * kKeyLoads, lane < 16 ? ks + 512 * kKeyLoads : vs - kRest, 16u);
+#pragma unroll
+        for (int u = 0; u < kKeyLoads; ++u)
+          cp_async16(dst + 512 * (kKeyLoads + 1) + 512 * u, vs + kRest + 512 * u, 16u);
+      } else {
+#pragma unroll 1
+        for (int x = lane; x < 2 * S::kBlockBytes / 16; x += 32) {
+          const bool value = x >= S::kBlockBytes / 16;
+          const int y = value ? x - S::kBlockBytes / 16 : x;
+          const int r = y / S::kPieces, piece = y - r * S::kPieces;
+          const int pg = whole ? page : __shfl_sync(0xffffffffu, page, r);
+          const int64_t at = whole ? page_row + r : __shfl_sync(0xffffffffu, page_row, r);
+          const uint8_t* src = value ? a.v : a.k;
+          const bool ok = pg >= 0 && r < ld_keys;
+          if (ok)
+            src += value ? ld.h * a.v_head + pg * a.v_page + at * a.v_row + 16 * piece
+                         : ld.h * a.k_head + pg * a.k_page + at * a.k_row + 16 * piece;
+          cp_async16(dst - 16 * lane + 16 * x, src, ok ? 16u : 0u);
         }
-        const bool ok = pg >= 0 && r < ld_keys;
-        const uint8_t* src = value ? vb : kb;
-        if (ok) {
-          src += at * (value ? a.v_row : a.k_row) + 16 * piece;
-          if (!whole) src += pg * (value ? a.v_page : a.k_page);
-        }
-        const uint32_t off =
-            value ? S::kBlockBytes + r * S::kRowBytes + 16 * piece
-                  : (piece < S::kPieces - 1 ? r * S::kCodes + 16 * piece : S::kKeyMeta + 16 * r);
-        cp_async16(dst + off, src, ok ? 16u : 0u);
       }
       if (++ld.t == ld.tiles) ld = next_unit<typename S::G>(a, ld);
       more = !run.done(ld);
@@ -297,13 +297,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       to_log2[hh] = a.scale_log2 * 0x1p24f * __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
     }
 
-    float o[4 * NG][4];  // columns of step products, of group g and place i: o[NG g + i]
-    float ol[2][4];      // this lane's keys' sums of weight times low
+    // Sums of the step products, transposed: rows of the product are numbers (places i and i + 1
+    // of group g, for columns r8 of the value's row), its columns the unit's rows.
+    float o[S::kHalves][2 * NG][4];
+    float ol[2][4];  // this lane's keys' sums of weight times low
     float m[2], l[2];
 #pragma unroll
-    for (int x = 0; x < 4 * NG; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+    for (int hh = 0; hh < S::kHalves; ++hh) {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
+      for (int x = 0; x < 2 * NG; ++x)
+        o[hh][x][0] = o[hh][x][1] = o[hh][x][2] = o[hh][x][3] = 0.f;
       m[hh] = -INFINITY;
       l[hh] = 0.f;
 #pragma unroll
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         float s[2][4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t row = 8 * x + r8, at = kb + row * S::kCodes + c4 * (S::kCodes / 4);
+          const uint32_t row = kb + (8 * x + r8) * S::kRowBytes, at = row + c4 * (S::kCodes / 4);
           uint32_t w[NG];
           if constexpr (NG == 4) {
             const uint4 v = lds128(at);
@@ -340,12 +343,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           uint32_t low;
           asm volatile("{\n.reg .u16 h;\nld.shared.u16 h, [%1];\nmov.b32 %0, {h, h};\n}"
                        : "=r"(low)
-                       : "r"(kb + S::kKeyMeta + 16 * row + 8 + 2 * c4)
+                       : "r"(row + S::kCodes + 8 + 2 * c4)
                        : "memory");
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
           mma16816<B200_ATTN_DTYPE_BF16>(acc, qs, low, low);
-          const uint32_t meta = kb + S::kKeyMeta + 16 * (8 * x + 2 * c4);
-          const uint2 s0 = lds64(meta), s1 = lds64(meta + 16);  // steps of the lane's two keys
+          const uint32_t meta = kb + (8 * x + 2 * c4) * S::kRowBytes + S::kCodes;
+          const uint2 s0 = lds64(meta), s1 = lds64(meta + S::kRowBytes);  // steps of the lane's two keys
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             float p[4];
@@ -432,18 +435,23 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           step_up = __uint_as_float((268u - top_step) << 23);
 #pragma unroll
           for (int hh = 0; hh < S::kHalves; ++hh) {
-            const float f0 = alpha[hh] * d0;
             l[hh] *= alpha[hh];
 #pragma unroll
             for (int g = 0; g < 4; ++g) ol[hh][g] *= alpha[hh];
+            // rows 2 c4 and 2 c4 + 1, whose factors lie in the lanes of those rows
+            const float f = alpha[hh] * d0;
+            const float f0 = __shfl_sync(0xffffffffu, f, 8 * c4);
+            const float f1 = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
 #pragma unroll
-            for (int x = 0; x < 4 * NG; ++x) {
-              o[x][2 * hh] = o[x][2 * hh] * f0 * d1;
-              o[x][2 * hh + 1] = o[x][2 * hh + 1] * f0 * d1;
+            for (int x = 0; x < 2 * NG; ++x) {
+              o[hh][x][0] = o[hh][x][0] * f0 * d1;
+              o[hh][x][1] = o[hh][x][1] * f1 * d1;
+              o[hh][x][2] = o[hh][x][2] * f0 * d1;
+              o[hh][x][3] = o[hh][x][3] * f1 * d1;
             }
           }
         }
-        float p[2][4];
+        float p[2][4], pu[2][4];  // weights, and times the steps' factor
 #pragma unroll
         for (int hh = 0; hh < S::kHalves; ++hh) {
           const float base = m[hh] == -INFINITY ? 0.f : m[hh];
@@ -454,6 +462,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
               p[x][2 * hh + e] =
                   b200attn::ptx::ex2_approx(fmaf(s[x][2 * hh + e], to_log2[hh], -base));
               l[hh] += p[x][2 * hh + e];
+              pu[x][2 * hh + e] = p[x][2 * hh + e] * step_up;
             }
         }
         // ------------------------------------------------------- values
@@ -475,16 +484,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t sw = g < 2 ? meta[i].x : meta[i].y, lo = g < 2 ? meta[i].z : meta[i].w;
-            st[i] = (g & 1 ? high_half(sw) : low_half(sw)) * step_up;
+            st[i] = g & 1 ? high_half(sw) : low_half(sw);
             lw[i] = g & 1 ? high_half(lo) : low_half(lo);
           }
-          uint32_t pf[4] = {0u, 0u, 0u, 0u};
+          uint32_t pf[S::kHalves][2];
 #pragma unroll
           for (int hh = 0; hh < S::kHalves; ++hh)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              pf[2 * x + hh] = pack_pair<B200_ATTN_DTYPE_FP16>(p[x][2 * hh] * st[2 * x],
-                                                               p[x][2 * hh + 1] * st[2 * x + 1]);
+              pf[hh][x] = pack_pair<B200_ATTN_DTYPE_FP16>(pu[x][2 * hh] * st[2 * x],
+                                                          pu[x][2 * hh + 1] * st[2 * x + 1]);
               ol[hh][g] = fmaf(p[x][2 * hh], lw[2 * x], ol[hh][g]);
               ol[hh][g] = fmaf(p[x][2 * hh + 1], lw[2 * x + 1], ol[hh][g]);
             }
@@ -492,20 +501,18 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           const int word = NG == 4 ? g / 2 : 0, half = NG == 4 ? g & 1 : g / 2;
           uint32_t v0 = __byte_perm(w[0][word], w[1][word], half ? 0x7632 : 0x5410);
           uint32_t v1 = __byte_perm(w[2][word], w[3][word], half ? 0x7632 : 0x5410);
-          if constexpr (NG == 4) {
-            mma_f16(o[4 * g], pf, v0 & kLow, v1 & kLow, o[4 * g][0], o[4 * g][1], o[4 * g][2], o[4 * g][3]);
-            mma_f16(o[4 * g + 1], pf, v0 & kHigh, v1 & kHigh, o[4 * g + 1][0], o[4 * g + 1][1], o[4 * g + 1][2], o[4 * g + 1][3]);
+          if (NG == 2 && (g & 1)) {
             v0 >>= 8;
             v1 >>= 8;
-            mma_f16(o[4 * g + 2], pf, v0 & kLow, v1 & kLow, o[4 * g + 2][0], o[4 * g + 2][1], o[4 * g + 2][2], o[4 * g + 2][3]);
-            mma_f16(o[4 * g + 3], pf, v0 & kHigh, v1 & kHigh, o[4 * g + 3][0], o[4 * g + 3][1], o[4 * g + 3][2], o[4 * g + 3][3]);
-          } else {
-            if (g & 1) {
-              v0 >>= 8;
-              v1 >>= 8;
+          }
+#pragma unroll
+          for (int y = 0; y < NG / 2; ++y) {
+            const uint32_t vf[4] = {(v0 >> 8 * y) & kLow, (v0 >> 8 * y) & kHigh,
+                                    (v1 >> 8 * y) & kLow, (v1 >> 8 * y) & kHigh};
+#pragma unroll
+            for (int hh = 0; hh < S::kHalves; ++hh) {
+              mma16816<B200_ATTN_DTYPE_FP16>(o[hh][NG / 2 * g + y], vf, pf[hh][0], pf[hh][1]);
             }
-            mma_f16(o[2 * g], pf, v0 & kLow, v1 & kLow, o[2 * g][0], o[2 * g][1], o[2 * g][2], o[2 * g][3]);
-            mma_f16(o[2 * g + 1], pf, v0 & kHigh, v1 & kHigh, o[2 * g + 1][0], o[2 * g + 1][1], o[2 * g + 1][2], o[2 * g + 1][3]);
           }
         }
       }
@@ -536,13 +543,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       }
     }
     const bool any_odd = __syncthreads_or(odd);
-    float scale[2];
+    // of row r8, and of rows 2 c4 and 2 c4 + 1
+    float scale[2], scale_c[2][2];
 #pragma unroll
     for (int hh = 0; hh < S::kHalves; ++hh) {
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, stat[2 * w * RM + 8 * hh + r8]);
       scale[hh] = top == -INFINITY ? 0.f : b200attn::ptx::ex2_approx(m[hh] - top);
+      scale_c[hh][0] = __shfl_sync(0xffffffffu, scale[hh], 8 * c4) * unit0;
+      scale_c[hh][1] = __shfl_sync(0xffffffffu, scale[hh], 8 * c4 + 4) * unit0;
     }
     float* part = a.partial + static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * (RM * (DP + 2));
     const bool finish = first && last;
@@ -563,22 +573,26 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
     for (int c0 = 0; c0 < DP; c0 += kC) {
       if (c0) __syncthreads();
-      // a lane holds 2 NG columns of a group side by side: places i of columns 2 c4, 2 c4 + 1
+      // numbers DP / 4 g + NG r8 + i of rows 2 c4 and 2 c4 + 1, whose lows' sums lie in the lanes
+      // of those rows
 #pragma unroll
       for (int g = c0 / (DP / 4); g < (c0 + kC) / (DP / 4); ++g)
 #pragma unroll
         for (int hh = 0; hh < S::kHalves; ++hh) {
-          float* d = join + (warp * S::kJoinRows + 8 * hh + r8) * kPitch + DP / 4 * g - c0 + 2 * NG * c4;
-          float v[2 * NG];
+          float* d = join + (warp * S::kJoinRows + 8 * hh + 2 * c4) * kPitch + DP / 4 * g - c0 + NG * r8;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int e = 0; e < 2; ++e) {
+            const float low = __shfl_sync(0xffffffffu, ol[hh][g] * scale[hh], 8 * c4 + 4 * e);
+            float v[NG];
 #pragma unroll
             for (int i = 0; i < NG; ++i)
-              v[NG * e + i] = (o[NG * g + i][2 * hh + e] * unit0 * (i & 1 ? unit1 * 0.0625f : unit1) +
-                               ol[hh][g]) * scale[hh];
-#pragma unroll
-          for (int i = 0; i < 2 * NG; i += 4)
-            *reinterpret_cast<float4*>(d + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+              v[i] = fmaf(o[hh][NG / 2 * g + i / 2][2 * (i & 1) + e] * scale_c[hh][e],
+                          i & 1 ? unit1 * 0.0625f : unit1, low);
+            if constexpr (NG == 4)
+              *reinterpret_cast<float4*>(d + e * kPitch) = make_float4(v[0], v[1], v[2], v[3]);
+            else
+              *reinterpret_cast<float2*>(d + e * kPitch) = make_float2(v[0], v[1]);
+          }
         }
       __syncthreads();
       float acc[kEach];

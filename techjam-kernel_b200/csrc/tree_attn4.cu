@@ -18,7 +18,7 @@
 // from two rows, two byte permutes.
 //
 // As in the kernel of 16-bit caches (tree_attn_rows.cuh) the warps of a CTA share a key tile,
-// 16 keys each, and fetch them into rings of their own.
+// 32 keys each, and fetch them into rings of their own.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -41,16 +41,18 @@ template <bool FEW_, int DP_>
 struct Shape4 {
   static constexpr bool FEW = FEW_;
   static constexpr int DP = DP_, RM = 16;
-  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kCtas = 3;
-  static constexpr int kTile = kWarps * kRowKeys;
+  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kCtas = FEW ? 3 : 2;  // CTAs of an SM
+  static constexpr int kParts = 2, kKeys = kParts * kRowKeys;  // keys of a warp's block
+  static constexpr int kTile = kWarps * kKeys;
   static constexpr int kHalves = FEW ? 1 : 2;
   static constexpr int kCodes = DP / 2, kRowBytes = kCodes + 16;
   static constexpr int kPieces = kRowBytes / 16;
-  static constexpr int kBlockBytes = kRowKeys * kRowBytes;
-  static constexpr int kStages = DP == 128 ? 5 : 8;
-  static constexpr int kRingBytes = kWarps * kStages * 2 * kBlockBytes;
+  static constexpr int kPartBytes = kRowKeys * kRowBytes;  // 16 keys, or values
+  static constexpr int kBlockBytes = kParts * 2 * kPartBytes;
+  static constexpr int kStages = (DP == 128 ? 3 : 4) + (FEW ? 0 : 1);
+  static constexpr int kRingBytes = kWarps * kStages * kBlockBytes;
   static constexpr int kJoinRows = FEW ? 8 : 16;
-  static constexpr int kJoinCols = DP < 1024 / kJoinRows ? DP : 1024 / kJoinRows;
+  static constexpr int kJoinCols = 512 / kJoinRows;
   static constexpr int kEach = kJoinRows * kJoinCols / kThreads;  // columns of a thread in a join
   static constexpr int kJoinPitch = kJoinCols + 4;
   static constexpr int kOffJoin = kRingBytes;
@@ -59,7 +61,7 @@ struct Shape4 {
   static constexpr int kOffMisc = kOffStat + 4 * 2 * kWarps * RM;
   static constexpr int kSmemBytes = kOffMisc + 256;
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "exceeds the shared memory of an SM");
-  using G = Grid<RM, kTile, 2>;
+  using G = Grid<RM, kTile, 1>;
   static_assert(sizeof(JoinSmem<DP, kWarps>) <= kJoinBytes, "joins in place");
 };
 
@@ -92,11 +94,40 @@ __device__ __forceinline__ uint4 lds128(uint32_t ad) {
 }
 __device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// A 16-bit number of shared memory in both halves.
+__device__ __forceinline__ uint32_t twice16(uint32_t ad) {
+  uint32_t v;
+  asm volatile("{\n.reg .u16 h;\nld.shared.u16 h, [%1];\nmov.b32 %0, {h, h};\n}"
+               : "=r"(v)
+               : "r"(ad)
+               : "memory");
+  return v;
+}
+// The transpose of an 8 x 8 matrix of 16-bit numbers, of which each lane has two of a row.
+__device__ __forceinline__ uint32_t turned(uint32_t w) {
+  uint32_t v;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(v) : "r"(w));
+  return v;
+}
 // The larger bf16 of each half; a NaN counts as nothing.
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
+}
+
+// Packed fp32 pairs (sm_100 .f32x2): each lane rounds like the scalar operation.
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mov.b64 d, {%0, %1};\n\tfma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1) {
+  asm("{\n\t.reg .b64 a, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 d, {%0, %1};\n\t"
+      "mul.rn.f32x2 d, d, a;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(a0), "f"(a1));
 }
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
@@ -131,7 +162,7 @@ __device__ __noinline__ void add_odd4(const Args& a, int b, int h, Seq s, int to
 template <class S, int DT>
 __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     rows4_kernel(const __grid_constant__ Args a) {
-  constexpr int RM = S::RM, DP = S::DP, NS = S::kStages, NG = DP / 32;
+  constexpr int RM = S::RM, DP = S::DP, NS = S::kStages, NG = DP / 32, NT = S::kHalves;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sbase = b200attn::ptx::smem_u32(smem);
   float* join = reinterpret_cast<float*>(smem + S::kOffJoin);
@@ -139,15 +170,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   uint32_t* sums = reinterpret_cast<uint32_t*>(smem + S::kOffMisc);
   Run* found = reinterpret_cast<Run*>(smem + S::kOffMisc + 80);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r8 = lane >> 2, c4 = lane & 3;  // row and column pair of this lane in a product
+  const int r8 = lane >> 2, c4 = lane & 3;  // row, and half the column, of this lane in a product
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
   find_run<typename S::G>(a, blockIdx.x, gridDim.x, sums, found);
   const Run& run = *found;
 
-  const uint32_t ring = sbase + warp * (NS * 2 * S::kBlockBytes);
+  const uint32_t ring = sbase + warp * (NS * S::kBlockBytes);
   const uint32_t size = static_cast<uint32_t>(a.page_size);
-  const bool whole = a.page_size % kRowKeys == 0;  // a block lies in one page
+  const bool whole = a.page_size % kRowKeys == 0;  // 16 keys lie in one page
 
   // ------------------------------------------------------------- loads
   // The place of the next tile to load; its page numbers are read one tile ahead.
@@ -155,9 +186,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   bool more = !run.done(ld);
   int page = -1, page_row = 0, ld_keys = 0;
   const uint32_t inv_size = 0xffffffffu / size + 1u;  // 0 for size 1
-  auto look_up = [&]() {
-    const int key = ld.t * S::kTile + warp * kRowKeys + (whole ? 0 : (lane & 15));
-    ld_keys = ld.s.len + ld.s.drafts - (ld.t * S::kTile + warp * kRowKeys);
+  auto look_up = [&]() {  // a lane a key, or where 16 keys share a page, the first of them
+    const int first = ld.t * S::kTile + warp * S::kKeys;
+    const int key = first + (whole ? lane & 16 : lane);
+    ld_keys = ld.s.len + ld.s.drafts - first;
     page = -1;
     page_row = 0;
     if (key < ld.s.len + ld.s.drafts) {
@@ -173,37 +205,45 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   };
   if (more) look_up();
   int stage = 0;  // stage the next loads go to
-  // Rows side by side: a block's keys and values are 2 kPieces / 32 loads of 16 bytes a lane, of
-  // which the middle one takes the end of the keys and the beginning of the values.
+  // Rows side by side: 16 keys and their values are 5 (or 3) loads of 16 bytes a lane, of which the
+  // middle one takes the end of the keys and the beginning of the values.
   const bool tight = whole && a.k_row == S::kRowBytes && a.v_row == S::kRowBytes;
-  constexpr int kKeyLoads = S::kBlockBytes / 512, kRest = S::kBlockBytes % 512;
+  constexpr int kKeyLoads = S::kPartBytes / 512, kRest = S::kPartBytes % 512;
   static_assert(kRest == 256, "half a load of 16 bytes a lane");
   auto issue = [&]() {
     if (more) {
-      if (page >= a.pages || (page < 0 && (whole ? 0 : (lane & 15)) < ld_keys)) {
+      if (page >= a.pages || (page < 0 && (whole ? lane & 16 : lane) < ld_keys)) {
         report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
         page = -1;
       }
-      const uint32_t dst = ring + stage * (2 * S::kBlockBytes) + 16 * lane;
-      if (tight && page >= 0 && ld_keys >= kRowKeys) {
-        const uint8_t* ks = a.k + ld.h * a.k_head + page * a.k_page + page_row * S::kRowBytes + 16 * lane;
-        const uint8_t* vs = a.v + ld.h * a.v_head + page * a.v_page + page_row * S::kRowBytes + 16 * lane;
+      const uint32_t dst = ring + stage * S::kBlockBytes + 16 * lane;
+      if (tight && ld_keys >= S::kKeys && __all_sync(0xffffffffu, page >= 0)) {
 #pragma unroll
-        for (int u = 0; u < kKeyLoads; ++u) cp_async16(dst + 512 * u, ks + 512 * u, 16u);
-        cp_async16(dst + 512 * kKeyLoads, lane < 16 ? ks + 512 * kKeyLoads : vs - kRest, 16u);
+        for (int h = 0; h < S::kParts; ++h) {
+          const int64_t pg = __shfl_sync(0xffffffffu, page, 16 * h);
+          const int at = __shfl_sync(0xffffffffu, page_row, 16 * h) * S::kRowBytes + 16 * lane;
+          const uint8_t* ks = a.k + ld.h * a.k_head + pg * a.k_page + at;
+          const uint8_t* vs = a.v + ld.h * a.v_head + pg * a.v_page + at;
+          const uint32_t to = dst + h * (2 * S::kPartBytes);
 #pragma unroll
-        for (int u = 0; u < kKeyLoads; ++u)
-          cp_async16(dst + 512 * (kKeyLoads + 1) + 512 * u, vs + kRest + 512 * u, 16u);
+          for (int u = 0; u < kKeyLoads; ++u) cp_async16(to + 512 * u, ks + 512 * u, 16u);
+          cp_async16(to + 512 * kKeyLoads, lane < 16 ? ks + 512 * kKeyLoads : vs - kRest, 16u);
+#pragma unroll
+          for (int u = 0; u < kKeyLoads; ++u)
+            cp_async16(to + 512 * (kKeyLoads + 1) + 512 * u, vs + kRest + 512 * u, 16u);
+        }
       } else {
 #pragma unroll 1
-        for (int x = lane; x < 2 * S::kBlockBytes / 16; x += 32) {
-          const bool value = x >= S::kBlockBytes / 16;
-          const int y = value ? x - S::kBlockBytes / 16 : x;
+        for (int x = lane; x < S::kBlockBytes / 16; x += 32) {
+          const int h = x / (S::kPartBytes / 8), z = x - h * (S::kPartBytes / 8);
+          const bool value = z >= S::kPartBytes / 16;
+          const int y = value ? z - S::kPartBytes / 16 : z;
           const int r = y / S::kPieces, piece = y - r * S::kPieces;
-          const int pg = whole ? page : __shfl_sync(0xffffffffu, page, r);
-          const int64_t at = whole ? page_row + r : __shfl_sync(0xffffffffu, page_row, r);
+          const int from = 16 * h + (whole ? 0 : r);
+          const int pg = __shfl_sync(0xffffffffu, page, from);
+          const int64_t at = __shfl_sync(0xffffffffu, page_row, from) + (whole ? r : 0);
           const uint8_t* src = value ? a.v : a.k;
-          const bool ok = pg >= 0 && r < ld_keys;
+          const bool ok = pg >= 0 && 16 * h + r < ld_keys;
           if (ok)
             src += value ? ld.h * a.v_head + pg * a.v_page + at * a.v_row + 16 * piece
                          : ld.h * a.k_head + pg * a.k_page + at * a.k_row + 16 * piece;
@@ -233,14 +273,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     // ----------------------------------------------------------- queries
     // Row r8 (and r8 + 8) as fp16 operands, times the power of two that brings the row's
     // largest number to 2^13..2^14; the pairs that meet the codes' high half bytes, by 1/16 more.
-    uint32_t qf[DP / 16][4];
-    uint32_t qs[4];   // the sums of the four groups, in three bf16 numbers
-    float to_log2[2];  // from the products' unit to that of the exponents
+    uint32_t qf[NT][DP / 16][2];
+    uint32_t qs[NT][2];   // the sums of the four groups, in three bf16 numbers
+    float to_log2[NT][2];  // from the products' unit to that of the exponents: rows 2 c4, 2 c4 + 1
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
+    for (int nt = 0; nt < NT; ++nt) {
       float x[DP / 16][4];
-      const int r = r8 + 8 * hh;
-      const bool live = hh < S::kHalves && r < rows;
+      const int r = r8 + 8 * nt;
       const int row = pl.rt * RM + r, tok = row / a.group;
       const uint8_t* src = a.q + pl.b * a.q_seq +
                            (pl.h * a.group + row - tok * a.group) * a.q_head + tok * a.q_tok;
@@ -251,7 +290,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         uint32_t w[NG];
 #pragma unroll
         for (int i = 0; i < NG; ++i) w[i] = 0u;
-        if (live && d < a.head_dim) {
+        if (r < rows && d < a.head_dim) {
           if constexpr (NG == 4) {
             const uint4 v = *reinterpret_cast<const uint4*>(src + 2 * d);
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
@@ -277,8 +316,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       const float up = __uint_as_float(static_cast<uint32_t>(267 - e) << 23);  // 2^(13 - exponent)
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
-        qf[i][hh] = pack_pair<B200_ATTN_DTYPE_FP16>(x[i][0] * up, x[i][1] * up);
-        qf[i][2 + hh] =
+        qf[nt][i][0] = pack_pair<B200_ATTN_DTYPE_FP16>(x[i][0] * up, x[i][1] * up);
+        qf[nt][i][1] =
             pack_pair<B200_ATTN_DTYPE_FP16>(x[i][2] * up * 0.0625f, x[i][3] * up * 0.0625f);
       }
       float mine = 0.f;  // the sum of group c4, in the unit of the products
@@ -291,26 +330,29 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       const uint32_t hi = pack_pair<B200_ATTN_DTYPE_BF16>(mine, 0.f);
       const float rest = mine - low_half(hi);
       const uint32_t mid = pack_pair<B200_ATTN_DTYPE_BF16>(rest, 0.f);
-      const uint32_t lo = pack_pair<B200_ATTN_DTYPE_BF16>(rest - low_half(mid), 0.f);
-      qs[hh] = hi | mid << 16;
-      qs[2 + hh] = lo;
-      to_log2[hh] = a.scale_log2 * 0x1p24f * __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
+      qs[nt][0] = hi | mid << 16;
+      qs[nt][1] = pack_pair<B200_ATTN_DTYPE_BF16>(rest - low_half(mid), 0.f);
+      const float f = a.scale_log2 * 0x1p24f * __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
+      to_log2[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c4);
+      to_log2[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
     }
 
-    // Sums of the step products, transposed: rows of the product are numbers (places i and i + 1
-    // of group g, for columns r8 of the value's row), its columns the unit's rows.
-    float o[S::kHalves][2 * NG][4];
-    float ol[2][4];  // this lane's keys' sums of weight times low
-    float m[2], l[2];
+    // All products have keys, or the numbers of a value, as their rows and the unit's rows as their
+    // columns: a lane has rows 2 c4 and 2 c4 + 1 of each eight (the second index, or two of
+    // four).  o: sums of the step products, of places i and i + 1 of group g and column r8 of the
+    // value's row; ol: this lane's keys' sums of weight times low; m, l: maximum and sum.
+    float o[NT][2 * NG][4];
+    float2 ol[NT][4];
+    float m[NT][2], l[NT][2];
 #pragma unroll
-    for (int hh = 0; hh < S::kHalves; ++hh) {
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int x = 0; x < 2 * NG; ++x)
-        o[hh][x][0] = o[hh][x][1] = o[hh][x][2] = o[hh][x][3] = 0.f;
-      m[hh] = -INFINITY;
-      l[hh] = 0.f;
+        o[nt][x][0] = o[nt][x][1] = o[nt][x][2] = o[nt][x][3] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) ol[hh][g] = 0.f;
+      for (int g = 0; g < 4; ++g) ol[nt][g] = make_float2(0.f, 0.f);
     }
     // Steps are multiplied by 2^(141 - top), which keeps them, and the weights times them,
     // below 2^15; top is the exponent of the largest so far (2^-100 at least).
@@ -323,110 +365,132 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       issue();
       cp_async_wait<NS - 1>();
       __syncwarp();
-      const uint32_t kb = ring + use * (2 * S::kBlockBytes), vb = kb + S::kBlockBytes;
+      const uint32_t block = ring + use * S::kBlockBytes;
       use = use + 1 == NS ? 0 : use + 1;
-      const int k0 = t * S::kTile + warp * kRowKeys;
+      const int k0 = t * S::kTile + warp * S::kKeys;
       if (k0 < keys) {
         // ------------------------------------------------------- scores
-        float s[2][4];
+        // keys r8 (elements 0, 1) and r8 + 8 (2, 3) of each 16
+        float s[S::kParts][NT][4];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t row = kb + (8 * x + r8) * S::kRowBytes, at = row + c4 * (S::kCodes / 4);
-          uint32_t w[NG];
+        for (int h = 0; h < S::kParts; ++h) {
+          const uint32_t row0 = block + h * (2 * S::kPartBytes) + r8 * S::kRowBytes;
+          const uint32_t row1 = row0 + 8 * S::kRowBytes;
+          uint32_t w0[NG], w1[NG];
           if constexpr (NG == 4) {
-            const uint4 v = lds128(at);
-            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+            const uint4 u = lds128(row0 + c4 * (S::kCodes / 4)), v = lds128(row1 + c4 * (S::kCodes / 4));
+            w0[0] = u.x, w0[1] = u.y, w0[2] = u.z, w0[3] = u.w;
+            w1[0] = v.x, w1[1] = v.y, w1[2] = v.z, w1[3] = v.w;
           } else {
-            const uint2 v = lds64(at);
-            w[0] = v.x, w[1] = v.y;
+            const uint2 u = lds64(row0 + c4 * (S::kCodes / 4)), v = lds64(row1 + c4 * (S::kCodes / 4));
+            w0[0] = u.x, w0[1] = u.y;
+            w1[0] = v.x, w1[1] = v.y;
           }
-          uint32_t low;
-          asm volatile("{\n.reg .u16 h;\nld.shared.u16 h, [%1];\nmov.b32 %0, {h, h};\n}"
-                       : "=r"(low)
-                       : "r"(row + S::kCodes + 8 + 2 * c4)
-                       : "memory");
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16816<B200_ATTN_DTYPE_BF16>(acc, qs, low, low);
-          const uint32_t meta = kb + (8 * x + 2 * c4) * S::kRowBytes + S::kCodes;
-          const uint2 s0 = lds64(meta), s1 = lds64(meta + S::kRowBytes);  // steps of the lane's two keys
+          const uint2 s0 = lds64(row0 + S::kCodes), s1 = lds64(row1 + S::kCodes);
+          const uint32_t low0 = twice16(row0 + S::kCodes + 8 + 2 * c4);
+          const uint32_t low1 = twice16(row1 + S::kCodes + 8 + 2 * c4);
+          const uint32_t lows[4] = {low0, low1, low0, low1};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            s[h][nt][0] = s[h][nt][1] = s[h][nt][2] = s[h][nt][3] = 0.f;
+            mma16816<B200_ATTN_DTYPE_BF16>(s[h][nt], lows, qs[nt][0], qs[nt][1]);
+          }
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            float p[4];
-            if constexpr (NG == 4) {
-              mma_f16(p, qf[2 * g], w[g] & kLow, w[g] & kHigh, 0.f, 0.f, 0.f, 0.f);
-              const uint32_t v = w[g] >> 8;
-              mma_f16(p, qf[2 * g + 1], v & kLow, v & kHigh, p[0], p[1], p[2], p[3]);
-            } else {
-              const uint32_t v = g & 1 ? w[g / 2] >> 8 : w[g / 2];
-              mma_f16(p, qf[g], v & kLow, v & kHigh, 0.f, 0.f, 0.f, 0.f);
+            float p[NT][4];
+#pragma unroll
+            for (int y = 0; y < NG / 2; ++y) {
+              const int step = NG / 2 * g + y, word = step / 2, shift = 8 * (step & 1);
+              const uint32_t u = w0[word] >> shift, v = w1[word] >> shift;
+              const uint32_t kf[4] = {u & kLow, v & kLow, u & kHigh, v & kHigh};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if (y == 0)
+                  mma_f16(p[nt], kf, qf[nt][step][0], qf[nt][step][1], 0.f, 0.f, 0.f, 0.f);
+                else
+                  mma16816<B200_ATTN_DTYPE_FP16>(p[nt], kf, qf[nt][step][0], qf[nt][step][1]);
+              }
             }
             const uint32_t a0 = g < 2 ? s0.x : s0.y, a1 = g < 2 ? s1.x : s1.y;
             const float f0 = g & 1 ? high_half(a0) : low_half(a0);
             const float f1 = g & 1 ? high_half(a1) : low_half(a1);
-            acc[0] = fmaf(f0, p[0], acc[0]);
-            acc[1] = fmaf(f1, p[1], acc[1]);
-            if constexpr (!S::FEW) {
-              acc[2] = fmaf(f0, p[2], acc[2]);
-              acc[3] = fmaf(f1, p[3], acc[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              fma2(s[h][nt][0], s[h][nt][1], f0, f0, p[nt][0], p[nt][1]);
+              fma2(s[h][nt][2], s[h][nt][3], f1, f1, p[nt][2], p[nt][3]);
             }
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[x][e] = acc[e];
         }
-        // steps and lows of the values of the lane's keys 2 c4, 2 c4 + 1, and 8 further
-        uint4 meta[4];
+        if (k0 + S::kKeys > pl.s.len) {  // drafted tokens, or past the last key
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          meta[i] = lds128(vb + (8 * (i >> 1) + 2 * c4 + (i & 1)) * S::kRowBytes + S::kCodes);
-        if (k0 + kRowKeys > pl.s.len) {
-          // drafted tokens, or past the last key
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2 * S::kHalves; ++e) {
-            const int row = pl.rt * RM + r8 + (e >> 1) * 8;
-            const int tok = min(row / a.group, a.tokens - 1);
+            for (int e = 0; e < 2; ++e) {
+              const int row = pl.rt * RM + 8 * nt + 2 * c4 + e;
+              const int tok = min(row / a.group, a.tokens - 1);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int j = k0 + 8 * x + 2 * c4 + (e & 1) - pl.s.len;
-              if (j >= 0 && (j >= pl.s.drafts || !sees(a, pl.b, tok, j))) s[x][e] = -INFINITY;
+              for (int h = 0; h < S::kParts; ++h)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  const int j = k0 + 16 * h + 8 * y + r8 - pl.s.len;
+                  if (j >= 0 && (j >= pl.s.drafts || !sees(a, pl.b, tok, j)))
+                    s[h][nt][2 * y + e] = -INFINITY;
+                }
             }
-          }
-          // A hidden value must not reach a row as 0 x NaN: it becomes 0 here and is added
-          // below to the rows that see it.
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (k0 + 8 * (i >> 1) + 2 * c4 + (i & 1) < pl.s.len) continue;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&meta[i]);
+          // A hidden value must not reach a row as 0 x NaN: steps and lows that are not finite become 0
+          // here, and are added below to the rows that see them.  A lane a key.
+          if (k0 + lane >= pl.s.len) {
+            const uint32_t at = block + (lane / 16) * (2 * S::kPartBytes) + S::kPartBytes +
+                                (lane & 15) * S::kRowBytes + S::kCodes;
+            uint4 v = lds128(at);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+            uint32_t any = 0u;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const uint32_t f = non_finite<B200_ATTN_DTYPE_BF16>(w[y]);
-              odd |= f != 0u;
+              any |= f;
               w[y] &= ~f;
             }
+            if (any) {
+              odd = true;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
+                           "r"(w[2]), "r"(w[3])
+                           : "memory");
+            }
           }
+          __syncwarp();
         }
         // ------------------------------------------------------ softmax
         // running maximum and largest step; the sums so far are rescaled only where one grew
-        uint32_t big = max_bf16x2(max_bf16x2(max_bf16x2(meta[0].x, meta[0].y), max_bf16x2(meta[1].x, meta[1].y)),
-                                  max_bf16x2(max_bf16x2(meta[2].x, meta[2].y), max_bf16x2(meta[3].x, meta[3].y)));
-        big = max_bf16x2(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = max_bf16x2(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        uint32_t e0 = (big >> 7) & 0xffu, e1 = big >> 23;
-        e0 = e0 == 255u ? 0u : e0;  // all of them NaN
-        e1 = e1 == 255u ? 0u : e1;
-        const uint32_t now_step = max(top_step, max(e0, e1));
-        bool grew = now_step > top_step;
-        float alpha[2] = {1.f, 1.f};
-#pragma unroll
-        for (int hh = 0; hh < S::kHalves; ++hh) {
-          float top = fmaxf(fmaxf(s[0][2 * hh], s[0][2 * hh + 1]),
-                            fmaxf(s[1][2 * hh], s[1][2 * hh + 1]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float now = fmaxf(m[hh], top * to_log2[hh]);
-          grew |= now > m[hh];
-          alpha[hh] = now == -INFINITY ? 1.f : b200attn::ptx::ex2_approx(m[hh] - now);
-          m[hh] = now;
+        uint32_t big = 0u;  // of the values of the keys of a lane's row, a lane two keys
+        {
+          const uint32_t at = block + S::kPartBytes + (lane & 15) * S::kRowBytes + S::kCodes;
+          const uint2 u = lds64(at), v = lds64(at + 2 * S::kPartBytes);
+          big = max_bf16x2(max_bf16x2(u.x, u.y), max_bf16x2(v.x, v.y));
+          big = max_bf16x2(big, big >> 16);
+          // a NaN counts as nothing, also where there is nothing else
+          big = (big & 0x7fffu) > 0x7f80u ? 0u : big & 0xffffu;
+          big = __reduce_max_sync(0xffffffffu, big);
         }
+        const uint32_t now_step = max(top_step, big >> 7);
+        bool grew = now_step > top_step;
+        float alpha[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+            for (int h = 1; h < S::kParts; ++h)
+              top = fmaxf(top, fmaxf(s[h][nt][e], s[h][nt][2 + e]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1)
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float now = fmaxf(m[nt][e], top * to_log2[nt][e]);
+            grew |= now > m[nt][e];
+            alpha[nt][e] = now == -INFINITY ? 1.f : b200attn::ptx::ex2_approx(m[nt][e] - now);
+            m[nt][e] = now;
+          }
         if (__any_sync(0xffffffffu, grew)) {
           // 2^(top_step - now_step), in two factors: they may lie 254 apart
           const float d0 = __uint_as_float((127u - (now_step - top_step) / 2) << 23);
@@ -434,84 +498,94 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           top_step = now_step;
           step_up = __uint_as_float((268u - top_step) << 23);
 #pragma unroll
-          for (int hh = 0; hh < S::kHalves; ++hh) {
-            l[hh] *= alpha[hh];
+          for (int nt = 0; nt < NT; ++nt) {
+            const float f0 = alpha[nt][0], f1 = alpha[nt][1];
+            mul2(l[nt][0], l[nt][1], f0, f1);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) ol[hh][g] *= alpha[hh];
-            // rows 2 c4 and 2 c4 + 1, whose factors lie in the lanes of those rows
-            const float f = alpha[hh] * d0;
-            const float f0 = __shfl_sync(0xffffffffu, f, 8 * c4);
-            const float f1 = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
+            for (int g = 0; g < 4; ++g) mul2(ol[nt][g].x, ol[nt][g].y, f0, f1);
 #pragma unroll
-            for (int x = 0; x < 2 * NG; ++x) {
-              o[hh][x][0] = o[hh][x][0] * f0 * d1;
-              o[hh][x][1] = o[hh][x][1] * f1 * d1;
-              o[hh][x][2] = o[hh][x][2] * f0 * d1;
-              o[hh][x][3] = o[hh][x][3] * f1 * d1;
-            }
+            for (int x = 0; x < 2 * NG; ++x)
+#pragma unroll
+              for (int y = 0; y < 4; y += 2) {
+                mul2(o[nt][x][y], o[nt][x][y + 1], f0 * d0, f1 * d0);
+                mul2(o[nt][x][y], o[nt][x][y + 1], d1, d1);
+              }
           }
         }
-        float p[2][4], pu[2][4];  // weights, and times the steps' factor
 #pragma unroll
-        for (int hh = 0; hh < S::kHalves; ++hh) {
-          const float base = m[hh] == -INFINITY ? 0.f : m[hh];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int e = 0; e < 2; ++e) {
+            const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              p[x][2 * hh + e] =
-                  b200attn::ptx::ex2_approx(fmaf(s[x][2 * hh + e], to_log2[hh], -base));
-              l[hh] += p[x][2 * hh + e];
-              pu[x][2 * hh + e] = p[x][2 * hh + e] * step_up;
-            }
-        }
+            for (int h = 0; h < S::kParts; ++h)
+#pragma unroll
+              for (int y = 0; y < 4; y += 2) {
+                s[h][nt][y + e] =
+                    b200attn::ptx::ex2_approx(fmaf(s[h][nt][y + e], to_log2[nt][e], -base));
+                l[nt][e] += s[h][nt][y + e];
+              }
+          }
         // ------------------------------------------------------- values
-        uint32_t w[4][NG / 2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t at =
-              vb + (8 * (i >> 1) + 2 * c4 + (i & 1)) * S::kRowBytes + r8 * (S::kCodes / 8);
-          if constexpr (NG == 4) {
-            const uint2 v = lds64(at);
-            w[i][0] = v.x, w[i][1] = v.y;
-          } else {
-            w[i][0] = lds32(at);
-          }
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float st[4], lw[4];
+        for (int h = 0; h < S::kParts; ++h) {
+          const uint32_t vb = block + h * (2 * S::kPartBytes) + S::kPartBytes;
+          // codes of keys 2 c4, 2 c4 + 1, and 8 further; steps and lows of keys r8 and r8 + 8
+          uint32_t w[4][NG / 2];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t sw = g < 2 ? meta[i].x : meta[i].y, lo = g < 2 ? meta[i].z : meta[i].w;
-            st[i] = g & 1 ? high_half(sw) : low_half(sw);
-            lw[i] = g & 1 ? high_half(lo) : low_half(lo);
-          }
-          uint32_t pf[S::kHalves][2];
-#pragma unroll
-          for (int hh = 0; hh < S::kHalves; ++hh)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              pf[hh][x] = pack_pair<B200_ATTN_DTYPE_FP16>(pu[x][2 * hh] * st[2 * x],
-                                                          pu[x][2 * hh + 1] * st[2 * x + 1]);
-              ol[hh][g] = fmaf(p[x][2 * hh], lw[2 * x], ol[hh][g]);
-              ol[hh][g] = fmaf(p[x][2 * hh + 1], lw[2 * x + 1], ol[hh][g]);
+            const uint32_t at = vb + (8 * (i >> 1) + 2 * c4 + (i & 1)) * S::kRowBytes + r8 * (S::kCodes / 8);
+            if constexpr (NG == 4) {
+              const uint2 v = lds64(at);
+              w[i][0] = v.x, w[i][1] = v.y;
+            } else {
+              w[i][0] = lds32(at);
             }
-          // the half words of the group, of two keys each
-          const int word = NG == 4 ? g / 2 : 0, half = NG == 4 ? g & 1 : g / 2;
-          uint32_t v0 = __byte_perm(w[0][word], w[1][word], half ? 0x7632 : 0x5410);
-          uint32_t v1 = __byte_perm(w[2][word], w[3][word], half ? 0x7632 : 0x5410);
-          if (NG == 2 && (g & 1)) {
-            v0 >>= 8;
-            v1 >>= 8;
           }
+          const uint4 m0 = lds128(vb + r8 * S::kRowBytes + S::kCodes);
+          const uint4 m1 = lds128(vb + (r8 + 8) * S::kRowBytes + S::kCodes);
+          float pu[NT][4];  // weights times the steps' factor
 #pragma unroll
-          for (int y = 0; y < NG / 2; ++y) {
-            const uint32_t vf[4] = {(v0 >> 8 * y) & kLow, (v0 >> 8 * y) & kHigh,
-                                    (v1 >> 8 * y) & kLow, (v1 >> 8 * y) & kHigh};
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int hh = 0; hh < S::kHalves; ++hh) {
-              mma16816<B200_ATTN_DTYPE_FP16>(o[hh][NG / 2 * g + y], vf, pf[hh][0], pf[hh][1]);
+            for (int y = 0; y < 4; y += 2) {
+              pu[nt][y] = s[h][nt][y], pu[nt][y + 1] = s[h][nt][y + 1];
+              mul2(pu[nt][y], pu[nt][y + 1], step_up, step_up);
+            }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t sw0 = g < 2 ? m0.x : m0.y, sw1 = g < 2 ? m1.x : m1.y;
+            const uint32_t lw0 = g < 2 ? m0.z : m0.w, lw1 = g < 2 ? m1.z : m1.w;
+            const float st0 = g & 1 ? high_half(sw0) : low_half(sw0);
+            const float st1 = g & 1 ? high_half(sw1) : low_half(sw1);
+            const float lo0 = g & 1 ? high_half(lw0) : low_half(lw0);
+            const float lo1 = g & 1 ? high_half(lw1) : low_half(lw1);
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float y[4] = {pu[nt][0], pu[nt][1], pu[nt][2], pu[nt][3]};
+              mul2(y[0], y[1], st0, st0);
+              mul2(y[2], y[3], st1, st1);
+              pf[nt][0] = turned(pack_pair<B200_ATTN_DTYPE_FP16>(y[0], y[1]));
+              pf[nt][1] = turned(pack_pair<B200_ATTN_DTYPE_FP16>(y[2], y[3]));
+              fma2(ol[nt][g].x, ol[nt][g].y, s[h][nt][0], s[h][nt][1], lo0, lo0);
+              fma2(ol[nt][g].x, ol[nt][g].y, s[h][nt][2], s[h][nt][3], lo1, lo1);
+            }
+            // the half words of the group, of two keys each
+            const int word = NG == 4 ? g / 2 : 0, half = NG == 4 ? g & 1 : g / 2;
+            uint32_t v0 = __byte_perm(w[0][word], w[1][word], half ? 0x7632 : 0x5410);
+            uint32_t v1 = __byte_perm(w[2][word], w[3][word], half ? 0x7632 : 0x5410);
+            if (NG == 2 && (g & 1)) {
+              v0 >>= 8;
+              v1 >>= 8;
+            }
+#pragma unroll
+            for (int y = 0; y < NG / 2; ++y) {
+              const uint32_t vf[4] = {(v0 >> 8 * y) & kLow, (v0 >> 8 * y) & kHigh,
+                                      (v1 >> 8 * y) & kLow, (v1 >> 8 * y) & kHigh};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816<B200_ATTN_DTYPE_FP16>(o[nt][NG / 2 * g + y], vf, pf[nt][0], pf[nt][1]);
             }
           }
         }
@@ -528,32 +602,36 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     const float unit0 = __uint_as_float((127u + top_step / 2) << 23);
     const float unit1 = __uint_as_float((127u + (top_step + 1) / 2 - 141u + 24u) << 23);
 #pragma unroll
-    for (int hh = 0; hh < S::kHalves; ++hh) {
-      float v = l[hh];
-      v += __shfl_xor_sync(0xffffffffu, v, 1);
-      v += __shfl_xor_sync(0xffffffffu, v, 2);
-      if (c4 == 0) {
-        stat[(2 * warp) * RM + 8 * hh + r8] = m[hh];
-        stat[(2 * warp + 1) * RM + 8 * hh + r8] = v;
-      }
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        ol[hh][g] += __shfl_xor_sync(0xffffffffu, ol[hh][g], 1);
-        ol[hh][g] += __shfl_xor_sync(0xffffffffu, ol[hh][g], 2);
+      for (int x = 4; x < 32; x <<= 1) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          ol[nt][g].x += __shfl_xor_sync(0xffffffffu, ol[nt][g].x, x);
+          ol[nt][g].y += __shfl_xor_sync(0xffffffffu, ol[nt][g].y, x);
+        }
+      }
+      if (r8 == 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          stat[(2 * warp) * RM + 8 * nt + 2 * c4 + e] = m[nt][e];
+          stat[(2 * warp + 1) * RM + 8 * nt + 2 * c4 + e] = l[nt][e];
+        }
       }
     }
     const bool any_odd = __syncthreads_or(odd);
-    // of row r8, and of rows 2 c4 and 2 c4 + 1
-    float scale[2], scale_c[2][2];
+    float scale[NT][2];
 #pragma unroll
-    for (int hh = 0; hh < S::kHalves; ++hh) {
-      float top = -INFINITY;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, stat[2 * w * RM + 8 * hh + r8]);
-      scale[hh] = top == -INFINITY ? 0.f : b200attn::ptx::ex2_approx(m[hh] - top);
-      scale_c[hh][0] = __shfl_sync(0xffffffffu, scale[hh], 8 * c4) * unit0;
-      scale_c[hh][1] = __shfl_sync(0xffffffffu, scale[hh], 8 * c4 + 4) * unit0;
-    }
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, stat[2 * w * RM + 8 * nt + 2 * c4 + e]);
+        scale[nt][e] = top == -INFINITY ? 0.f : b200attn::ptx::ex2_approx(m[nt][e] - top);
+      }
     float* part = a.partial + static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * (RM * (DP + 2));
     const bool finish = first && last;
     constexpr int kC = S::kJoinCols, kPitch = S::kJoinPitch, kEach = S::kEach;
@@ -573,27 +651,25 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
     for (int c0 = 0; c0 < DP; c0 += kC) {
       if (c0) __syncthreads();
-      // numbers DP / 4 g + NG r8 + i of rows 2 c4 and 2 c4 + 1, whose lows' sums lie in the lanes
-      // of those rows
+      // numbers DP / 4 g + NG r8 + i of rows 2 c4 and 2 c4 + 1
 #pragma unroll
       for (int g = c0 / (DP / 4); g < (c0 + kC) / (DP / 4); ++g)
 #pragma unroll
-        for (int hh = 0; hh < S::kHalves; ++hh) {
-          float* d = join + (warp * S::kJoinRows + 8 * hh + 2 * c4) * kPitch + DP / 4 * g - c0 + NG * r8;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float low = __shfl_sync(0xffffffffu, ol[hh][g] * scale[hh], 8 * c4 + 4 * e);
+            float* d = join + (warp * S::kJoinRows + 8 * nt + 2 * c4 + e) * kPitch + DP / 4 * g - c0 + NG * r8;
+            const float low = (e ? ol[nt][g].y : ol[nt][g].x) * scale[nt][e];
             float v[NG];
 #pragma unroll
             for (int i = 0; i < NG; ++i)
-              v[i] = fmaf(o[hh][NG / 2 * g + i / 2][2 * (i & 1) + e] * scale_c[hh][e],
+              v[i] = fmaf(o[nt][NG / 2 * g + i / 2][2 * (i & 1) + e] * (scale[nt][e] * unit0),
                           i & 1 ? unit1 * 0.0625f : unit1, low);
             if constexpr (NG == 4)
-              *reinterpret_cast<float4*>(d + e * kPitch) = make_float4(v[0], v[1], v[2], v[3]);
+              *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
             else
-              *reinterpret_cast<float2*>(d + e * kPitch) = make_float2(v[0], v[1]);
+              *reinterpret_cast<float2*>(d) = make_float2(v[0], v[1]);
           }
-        }
       __syncthreads();
       float acc[kEach];
 #pragma unroll
@@ -648,8 +724,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 // -------------------------------------------------------------------- host
 using namespace b200paged;
 
-using AnyShape = Shape4<false, 128>;  // tiles and CTAs do not depend on the instance
-static_assert(AnyShape::kTile == Shape4<true, 64>::kTile && AnyShape::kCtas == Shape4<true, 64>::kCtas,
+using AnyShape = Shape4<false, 128>;  // row and key tiles do not depend on the instance
+static_assert(AnyShape::kTile == Shape4<true, 64>::kTile && AnyShape::RM == Shape4<true, 64>::RM,
               "one division of the work");
 
 int64_t rows_of(const b200_tree_attn_params* p) { return p->tokens * (p->heads / p->cache.kv_heads); }
@@ -666,7 +742,8 @@ int64_t runs_of(const b200_tree_attn_params* p, int64_t sms) {
   const int64_t keys = p->cache.slots * p->cache.page_size;
   const double tiles = static_cast<double>(units_of(p)) *
                        static_cast<double>((keys + AnyShape::kTile - 1) / AnyShape::kTile);
-  const int64_t most = (sms < kMaxSms ? sms : kMaxSms) * AnyShape::kCtas;
+  const int64_t most = (sms < kMaxSms ? sms : kMaxSms) *
+                       (rows_of(p) <= 8 ? Shape4<true, 128>::kCtas : Shape4<false, 128>::kCtas);
   return tiles < static_cast<double>(most) ? static_cast<int64_t>(tiles) : most;
 }
 

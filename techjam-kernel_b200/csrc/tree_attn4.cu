@@ -41,7 +41,7 @@ template <bool FEW_, int DP_>
 struct Shape4 {
   static constexpr bool FEW = FEW_;
   static constexpr int DP = DP_, RM = 16;
-  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kCtas = FEW ? 3 : 2;  // CTAs of an SM
+  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kCtas = !FEW ? 2 : (DP_ == 128 ? 3 : 4);  // CTAs of an SM
   static constexpr int kParts = 2, kKeys = kParts * kRowKeys;  // keys of a warp's block
   static constexpr int kTile = kWarps * kKeys;
   static constexpr int kHalves = FEW ? 1 : 2;
@@ -49,7 +49,7 @@ struct Shape4 {
   static constexpr int kPieces = kRowBytes / 16;
   static constexpr int kPartBytes = kRowKeys * kRowBytes;  // 16 keys, or values
   static constexpr int kBlockBytes = kParts * 2 * kPartBytes;
-  static constexpr int kStages = (DP == 128 ? 3 : 4) + (FEW ? 0 : 1);
+  static constexpr int kStages = DP == 128 ? (FEW ? 3 : 4) : (FEW ? 3 : 5);
   static constexpr int kRingBytes = kWarps * kStages * kBlockBytes;
   static constexpr int kJoinRows = FEW ? 8 : 16;
   static constexpr int kJoinCols = 512 / kJoinRows;
@@ -58,7 +58,8 @@ struct Shape4 {
   static constexpr int kOffJoin = kRingBytes;
   static constexpr int kJoinBytes = 4 * kWarps * kJoinRows * kJoinPitch;
   static constexpr int kOffStat = kOffJoin + kJoinBytes;
-  static constexpr int kOffMisc = kOffStat + 4 * 2 * kWarps * RM;
+  static constexpr int kOffPlaces = kOffStat + 4 * 2 * kWarps * RM;  // of the warps' loads
+  static constexpr int kOffMisc = kOffPlaces + kWarps * sizeof(Place);
   static constexpr int kSmemBytes = kOffMisc + 256;
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "exceeds the shared memory of an SM");
   using G = Grid<RM, kTile, 1>;
@@ -116,20 +117,6 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// Packed fp32 pairs (sm_100 .f32x2): each lane rounds like the scalar operation.
-__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mov.b64 d, {%0, %1};\n\tfma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "+f"(d0), "+f"(d1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1) {
-  asm("{\n\t.reg .b64 a, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 d, {%0, %1};\n\t"
-      "mul.rn.f32x2 d, d, a;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "+f"(d0), "+f"(d1)
-      : "f"(a0), "f"(a1));
-}
-
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 
 // Adds NaN to the numbers of a finished row (`out`) or its partial sums (`part`) whose group
@@ -181,18 +168,32 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   const bool whole = a.page_size % kRowKeys == 0;  // 16 keys lie in one page
 
   // ------------------------------------------------------------- loads
-  // The place of the next tile to load; its page numbers are read one tile ahead.
-  Place ld = run.p;
-  bool more = !run.done(ld);
-  int page = -1, page_row = 0, ld_keys = 0;
+  // The warp's next block to load: its first key, the sequence's keys, blocks left in the unit, and
+  // where the unit's page numbers and pools begin.  Page numbers are read one block ahead.  The
+  // unit itself is in shared memory (`at`), for when it ends.
+  Place* at = reinterpret_cast<Place*>(smem + S::kOffPlaces) + warp;
+  int ld_key = 0, ld_total = 0, ld_left = 0;
+  const int32_t* ld_table = a.table;
+  const uint8_t *ld_k = a.k, *ld_v = a.v;
+  auto enter = [&](const Place& p) {
+    __syncwarp();
+    if (lane == 0) *at = p;
+    __syncwarp();
+    ld_left = run.done(p) ? 0 : run.tiles(p);
+    ld_key = p.t * S::kTile + warp * S::kKeys;
+    ld_total = p.s.len + p.s.drafts;
+    ld_table = a.table + p.b * a.table_stride;
+    ld_k = a.k + p.h * a.k_head;
+    ld_v = a.v + p.h * a.v_head;
+  };
+  enter(run.p);
+  int page = -1, page_row = 0;
   const uint32_t inv_size = 0xffffffffu / size + 1u;  // 0 for size 1
   auto look_up = [&]() {  // a lane a key, or where 16 keys share a page, the first of them
-    const int first = ld.t * S::kTile + warp * S::kKeys;
-    const int key = first + (whole ? lane & 16 : lane);
-    ld_keys = ld.s.len + ld.s.drafts - first;
+    const int key = ld_key + (whole ? lane & 16 : lane);
     page = -1;
     page_row = 0;
-    if (key < ld.s.len + ld.s.drafts) {
+    if (key < ld_total) {
       // key / size or one more: key is below 2^30
       uint32_t slot = size == 1u ? key : __umulhi(key, inv_size);
       page_row = key - static_cast<int>(slot * size);
@@ -200,10 +201,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         --slot;
         page_row += static_cast<int>(size);
       }
-      page = __ldg(a.table + ld.b * a.table_stride + slot);
+      page = __ldg(ld_table + slot);
     }
   };
-  if (more) look_up();
+  if (ld_left > 0) look_up();
   int stage = 0;  // stage the next loads go to
   // Rows side by side: 16 keys and their values are 5 (or 3) loads of 16 bytes a lane, of which the
   // middle one takes the end of the keys and the beginning of the values.
@@ -211,19 +212,17 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   constexpr int kKeyLoads = S::kPartBytes / 512, kRest = S::kPartBytes % 512;
   static_assert(kRest == 256, "half a load of 16 bytes a lane");
   auto issue = [&]() {
-    if (more) {
-      if (page >= a.pages || (page < 0 && (whole ? lane & 16 : lane) < ld_keys)) {
-        report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
-        page = -1;
-      }
+    if (ld_left > 0) {
+      const int ld_keys = ld_total - ld_key;
       const uint32_t dst = ring + stage * S::kBlockBytes + 16 * lane;
-      if (tight && ld_keys >= S::kKeys && __all_sync(0xffffffffu, page >= 0)) {
+      if (tight && __all_sync(0xffffffffu, ld_keys >= S::kKeys && static_cast<uint32_t>(page) <
+                                                                      static_cast<uint32_t>(a.pages))) {
 #pragma unroll
         for (int h = 0; h < S::kParts; ++h) {
           const int64_t pg = __shfl_sync(0xffffffffu, page, 16 * h);
-          const int at = __shfl_sync(0xffffffffu, page_row, 16 * h) * S::kRowBytes + 16 * lane;
-          const uint8_t* ks = a.k + ld.h * a.k_head + pg * a.k_page + at;
-          const uint8_t* vs = a.v + ld.h * a.v_head + pg * a.v_page + at;
+          const int in = __shfl_sync(0xffffffffu, page_row, 16 * h) * S::kRowBytes + 16 * lane;
+          const uint8_t* ks = ld_k + pg * a.k_page + in;
+          const uint8_t* vs = ld_v + pg * a.v_page + in;
           const uint32_t to = dst + h * (2 * S::kPartBytes);
 #pragma unroll
           for (int u = 0; u < kKeyLoads; ++u) cp_async16(to + 512 * u, ks + 512 * u, 16u);
@@ -233,6 +232,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             cp_async16(to + 512 * (kKeyLoads + 1) + 512 * u, vs + kRest + 512 * u, 16u);
         }
       } else {
+        if (page >= a.pages || (page < 0 && (whole ? lane & 16 : lane) < ld_keys)) {
+          report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
+          page = -1;
+        }
 #pragma unroll 1
         for (int x = lane; x < S::kBlockBytes / 16; x += 32) {
           const int h = x / (S::kPartBytes / 8), z = x - h * (S::kPartBytes / 8);
@@ -241,18 +244,23 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           const int r = y / S::kPieces, piece = y - r * S::kPieces;
           const int from = 16 * h + (whole ? 0 : r);
           const int pg = __shfl_sync(0xffffffffu, page, from);
-          const int64_t at = __shfl_sync(0xffffffffu, page_row, from) + (whole ? r : 0);
-          const uint8_t* src = value ? a.v : a.k;
+          const int64_t in = __shfl_sync(0xffffffffu, page_row, from) + (whole ? r : 0);
+          const uint8_t* src = value ? ld_v : ld_k;
           const bool ok = pg >= 0 && 16 * h + r < ld_keys;
           if (ok)
-            src += value ? ld.h * a.v_head + pg * a.v_page + at * a.v_row + 16 * piece
-                         : ld.h * a.k_head + pg * a.k_page + at * a.k_row + 16 * piece;
+            src += value ? pg * a.v_page + in * a.v_row + 16 * piece
+                         : pg * a.k_page + in * a.k_row + 16 * piece;
           cp_async16(dst - 16 * lane + 16 * x, src, ok ? 16u : 0u);
         }
       }
-      if (++ld.t == ld.tiles) ld = next_unit<typename S::G>(a, ld);
-      more = !run.done(ld);
-      if (more) look_up();
+      ld_key += S::kTile;
+      if (--ld_left == 0) {
+        Place p = *at;
+        p.t += run.tiles(p);
+        if (p.t == p.tiles) p = next_unit<typename S::G>(a, p);
+        enter(p);
+      }
+      if (ld_left > 0) look_up();
     }
     cp_async_commit();
     stage = stage + 1 == NS ? 0 : stage + 1;
@@ -354,10 +362,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
       for (int g = 0; g < 4; ++g) ol[nt][g] = make_float2(0.f, 0.f);
     }
-    // Steps are multiplied by 2^(141 - top), which keeps them, and the weights times them,
-    // below 2^15; top is the exponent of the largest so far (2^-100 at least).
-    uint32_t top_step = 27u;
-    float step_up = __uint_as_float((268u - 27u) << 23);
+    // Steps are multiplied by 2^(137 - top), which keeps them below 2^11, and weights, up to 2^4,
+    // times them below 2^15; top is the exponent of the largest so far (2^-100 at least).
+    uint32_t top_step = 27u, most_step = 27u << 7 | 0x7fu;  // the latter as bf16 bits
+    float step_up = __uint_as_float((264u - 27u) << 23);
     bool odd = false;  // a drafted token's step or low was not finite
 
 #pragma unroll 1
@@ -416,8 +424,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             const float f1 = g & 1 ? high_half(a1) : low_half(a1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              fma2(s[h][nt][0], s[h][nt][1], f0, f0, p[nt][0], p[nt][1]);
-              fma2(s[h][nt][2], s[h][nt][3], f1, f1, p[nt][2], p[nt][3]);
+              s[h][nt][0] = fmaf(f0, p[nt][0], s[h][nt][0]);
+              s[h][nt][1] = fmaf(f0, p[nt][1], s[h][nt][1]);
+              s[h][nt][2] = fmaf(f1, p[nt][2], s[h][nt][2]);
+              s[h][nt][3] = fmaf(f1, p[nt][3], s[h][nt][3]);
             }
           }
         }
@@ -461,55 +471,62 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           __syncwarp();
         }
         // ------------------------------------------------------ softmax
-        // running maximum and largest step; the sums so far are rescaled only where one grew
-        uint32_t big = 0u;  // of the values of the keys of a lane's row, a lane two keys
+        // The maximum and the largest step that weights and steps are taken relative to follow the
+        // true ones only where a score is over 2^4 times, or a step is above them: of 18 blocks of
+        // random keys about two, where every new maximum would rescale the sums in ten.
+        uint32_t big;  // steps of two keys' values
+        bool grew = false;
         {
           const uint32_t at = block + S::kPartBytes + (lane & 15) * S::kRowBytes + S::kCodes;
           const uint2 u = lds64(at), v = lds64(at + 2 * S::kPartBytes);
           big = max_bf16x2(max_bf16x2(u.x, u.y), max_bf16x2(v.x, v.y));
-          big = max_bf16x2(big, big >> 16);
-          // a NaN counts as nothing, also where there is nothing else
-          big = (big & 0x7fffu) > 0x7f80u ? 0u : big & 0xffffu;
-          big = __reduce_max_sync(0xffffffffu, big);
+          grew = (big >> 16) > most_step || (big & 0xffffu) > most_step;
         }
-        const uint32_t now_step = max(top_step, big >> 7);
-        bool grew = now_step > top_step;
-        float alpha[NT][2];
+        float top[NT][2];  // of the lane's keys
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+            float x = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
-            for (int h = 1; h < S::kParts; ++h)
-              top = fmaxf(top, fmaxf(s[h][nt][e], s[h][nt][2 + e]));
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1)
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float now = fmaxf(m[nt][e], top * to_log2[nt][e]);
-            grew |= now > m[nt][e];
-            alpha[nt][e] = now == -INFINITY ? 1.f : b200attn::ptx::ex2_approx(m[nt][e] - now);
-            m[nt][e] = now;
+            for (int h = 1; h < S::kParts; ++h) x = fmaxf(x, fmaxf(s[h][nt][e], s[h][nt][2 + e]));
+            top[nt][e] = x * to_log2[nt][e];
+            grew |= top[nt][e] > m[nt][e] + 4.f;
           }
         if (__any_sync(0xffffffffu, grew)) {
+          // a NaN counts as nothing, also where there is nothing else
+          const uint32_t lo = big & 0xffffu, hi = big >> 16;
+          const uint32_t most = __reduce_max_sync(
+              0xffffffffu, max((lo & 0x7fffu) > 0x7f80u ? 0u : lo, (hi & 0x7fffu) > 0x7f80u ? 0u : hi));
+          const uint32_t now_step = max(top_step, most >> 7);
           // 2^(top_step - now_step), in two factors: they may lie 254 apart
           const float d0 = __uint_as_float((127u - (now_step - top_step) / 2) << 23);
           const float d1 = __uint_as_float((127u - (now_step - top_step + 1) / 2) << 23);
           top_step = now_step;
-          step_up = __uint_as_float((268u - top_step) << 23);
+          most_step = top_step << 7 | 0x7fu;
+          step_up = __uint_as_float((264u - top_step) << 23);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float f0 = alpha[nt][0], f1 = alpha[nt][1];
-            mul2(l[nt][0], l[nt][1], f0, f1);
+            float f[2];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) mul2(ol[nt][g].x, ol[nt][g].y, f0, f1);
+            for (int e = 0; e < 2; ++e) {
+              float x = top[nt][e];
+#pragma unroll
+              for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
+              const float now = fmaxf(m[nt][e], x);
+              f[e] = now == -INFINITY ? 1.f : b200attn::ptx::ex2_approx(m[nt][e] - now);
+              m[nt][e] = now;
+              l[nt][e] *= f[e];
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              ol[nt][g].x *= f[0];
+              ol[nt][g].y *= f[1];
+            }
 #pragma unroll
             for (int x = 0; x < 2 * NG; ++x)
 #pragma unroll
-              for (int y = 0; y < 4; y += 2) {
-                mul2(o[nt][x][y], o[nt][x][y + 1], f0 * d0, f1 * d0);
-                mul2(o[nt][x][y], o[nt][x][y + 1], d1, d1);
-              }
+              for (int y = 0; y < 4; ++y) o[nt][x][y] = o[nt][x][y] * (f[y & 1] * d0) * d1;
           }
         }
 #pragma unroll
@@ -548,10 +565,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int y = 0; y < 4; y += 2) {
-              pu[nt][y] = s[h][nt][y], pu[nt][y + 1] = s[h][nt][y + 1];
-              mul2(pu[nt][y], pu[nt][y + 1], step_up, step_up);
-            }
+            for (int y = 0; y < 4; ++y) pu[nt][y] = s[h][nt][y] * step_up;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const uint32_t sw0 = g < 2 ? m0.x : m0.y, sw1 = g < 2 ? m1.x : m1.y;
@@ -563,13 +577,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             uint32_t pf[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              float y[4] = {pu[nt][0], pu[nt][1], pu[nt][2], pu[nt][3]};
-              mul2(y[0], y[1], st0, st0);
-              mul2(y[2], y[3], st1, st1);
-              pf[nt][0] = turned(pack_pair<B200_ATTN_DTYPE_FP16>(y[0], y[1]));
-              pf[nt][1] = turned(pack_pair<B200_ATTN_DTYPE_FP16>(y[2], y[3]));
-              fma2(ol[nt][g].x, ol[nt][g].y, s[h][nt][0], s[h][nt][1], lo0, lo0);
-              fma2(ol[nt][g].x, ol[nt][g].y, s[h][nt][2], s[h][nt][3], lo1, lo1);
+              pf[nt][0] = turned(pack_pair<B200_ATTN_DTYPE_FP16>(pu[nt][0] * st0, pu[nt][1] * st0));
+              pf[nt][1] = turned(pack_pair<B200_ATTN_DTYPE_FP16>(pu[nt][2] * st1, pu[nt][3] * st1));
+              ol[nt][g].x = fmaf(s[h][nt][0], lo0, fmaf(s[h][nt][2], lo1, ol[nt][g].x));
+              ol[nt][g].y = fmaf(s[h][nt][1], lo0, fmaf(s[h][nt][3], lo1, ol[nt][g].y));
             }
             // the half words of the group, of two keys each
             const int word = NG == 4 ? g / 2 : 0, half = NG == 4 ? g & 1 : g / 2;
@@ -600,7 +611,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     if (pl.t == pl.tiles) pl = next_unit<typename S::G>(a, pl);
     // the steps' factor and the codes' 2^-24 leave the sums (in two factors)
     const float unit0 = __uint_as_float((127u + top_step / 2) << 23);
-    const float unit1 = __uint_as_float((127u + (top_step + 1) / 2 - 141u + 24u) << 23);
+    const float unit1 = __uint_as_float((127u + (top_step + 1) / 2 - 137u + 24u) << 23);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -739,11 +750,14 @@ int64_t units_of(const b200_tree_attn_params* p) {
 }
 
 int64_t runs_of(const b200_tree_attn_params* p, int64_t sms) {
+  const bool narrow = p->cache.head_dim == 24;  // rows of 48 bytes
   const int64_t keys = p->cache.slots * p->cache.page_size;
   const double tiles = static_cast<double>(units_of(p)) *
                        static_cast<double>((keys + AnyShape::kTile - 1) / AnyShape::kTile);
   const int64_t most = (sms < kMaxSms ? sms : kMaxSms) *
-                       (rows_of(p) <= 8 ? Shape4<true, 128>::kCtas : Shape4<false, 128>::kCtas);
+                       (rows_of(p) > 8 ? AnyShape::kCtas
+                        : narrow      ? Shape4<true, 64>::kCtas
+                                      : Shape4<true, 128>::kCtas);
   return tiles < static_cast<double>(most) ? static_cast<int64_t>(tiles) : most;
 }
 

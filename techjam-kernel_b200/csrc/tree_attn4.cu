@@ -59,50 +59,40 @@ struct Shape4 {
   static constexpr int kJoinBytes = 4 * kWarps * kJoinRows * kJoinPitch;
   static constexpr int kOffStat = kOffJoin + kJoinBytes;
   static constexpr int kOffPlaces = kOffStat + 4 * 2 * kWarps * RM;  // of the warps' loads
-  static constexpr int kOffMisc = kOffPlaces + kWarps * sizeof(Place);
+  static constexpr int kOffBars = kOffPlaces + kWarps * sizeof(Place);  // a barrier a block
+  static constexpr int kOffMisc = kOffBars + 8 * kWarps * kStages;
   static constexpr int kSmemBytes = kOffMisc + 256;
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "exceeds the shared memory of an SM");
   using G = Grid<RM, kTile, 1>;
   static_assert(sizeof(JoinSmem<DP, kWarps>) <= kJoinBytes, "joins in place");
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                        uint32_t b1, float c0, float c1, float c2, float c3) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%10, %11, %12, %13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
-        "f"(c3));
+// Products m16n8k16 without side effects, which the compiler may move: d = a b + c.
+template <int DT>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                    float c0, float c1, float c2, float c3) {
+  if constexpr (DT == B200_ATTN_DTYPE_BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
+          "f"(c3));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
+          "f"(c3));
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t ad) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(ad) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t ad) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(ad) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t ad) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(ad)
-               : "memory");
-  return v;
+template <class T>
+__device__ __forceinline__ T lds(const uint8_t* at) {
+  return *reinterpret_cast<const T*>(at);
 }
 __device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 // A 16-bit number of shared memory in both halves.
-__device__ __forceinline__ uint32_t twice16(uint32_t ad) {
-  uint32_t v;
-  asm volatile("{\n.reg .u16 h;\nld.shared.u16 h, [%1];\nmov.b32 %0, {h, h};\n}"
-               : "=r"(v)
-               : "r"(ad)
-               : "memory");
-  return v;
+__device__ __forceinline__ uint32_t twice16(const uint8_t* at) {
+  return __byte_perm(lds<uint16_t>(at), 0u, 0x1010);
 }
 // The transpose of an 8 x 8 matrix of 16-bit numbers, of which each lane has two of a row.
 __device__ __forceinline__ uint32_t turned(uint32_t w) {
@@ -115,6 +105,27 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
+}
+
+// `bytes` (a multiple of 16) of global memory to shared memory; counted by barrier `bar`.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const uint8_t* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+// Waits for a block's copies, a second at most; false (reported) when they did not come.  By
+// whole warps.
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int32_t* err) {
+  const uint64_t t0 = b200attn::ptx::globaltimer_ns();
+  bool ok;
+  do {
+    ok = b200attn::ptx::mbar_try_wait(bar, parity);
+  } while (!ok && b200attn::ptx::globaltimer_ns() - t0 < 1000000000ull);
+  ok = __all_sync(0xffffffffu, ok);
+  if (!ok) report_error(err, B200_ATTN_DEVERR_WAIT_TIMEOUT);
+  return ok;
 }
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
@@ -163,7 +174,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   find_run<typename S::G>(a, blockIdx.x, gridDim.x, sums, found);
   const Run& run = *found;
 
+  uint8_t* blocks = smem + warp * (NS * S::kBlockBytes);  // this warp's ring
   const uint32_t ring = sbase + warp * (NS * S::kBlockBytes);
+  const uint32_t bars = sbase + S::kOffBars + 8 * NS * warp;
   const uint32_t size = static_cast<uint32_t>(a.page_size);
   const bool whole = a.page_size % kRowKeys == 0;  // 16 keys lie in one page
 
@@ -206,51 +219,41 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   };
   if (ld_left > 0) look_up();
   int stage = 0;  // stage the next loads go to
-  // Rows side by side: 16 keys and their values are 5 (or 3) loads of 16 bytes a lane, of which the
-  // middle one takes the end of the keys and the beginning of the values.
+  bool dead = false;  // a wait ran out
   const bool tight = whole && a.k_row == S::kRowBytes && a.v_row == S::kRowBytes;
-  constexpr int kKeyLoads = S::kPartBytes / 512, kRest = S::kPartBytes % 512;
-  static_assert(kRest == 256, "half a load of 16 bytes a lane");
   auto issue = [&]() {
-    if (ld_left > 0) {
+    if (ld_left > 0 && !dead) {
       const int ld_keys = ld_total - ld_key;
-      const uint32_t dst = ring + stage * S::kBlockBytes + 16 * lane;
+      const uint32_t bar = bars + 8 * stage;
+      const uint32_t dst = ring + stage * S::kBlockBytes + (lane / 16) * (2 * S::kPartBytes);
       if (tight && __all_sync(0xffffffffu, ld_keys >= S::kKeys && static_cast<uint32_t>(page) <
                                                                       static_cast<uint32_t>(a.pages))) {
-#pragma unroll
-        for (int h = 0; h < S::kParts; ++h) {
-          const int64_t pg = __shfl_sync(0xffffffffu, page, 16 * h);
-          const int in = __shfl_sync(0xffffffffu, page_row, 16 * h) * S::kRowBytes + 16 * lane;
-          const uint8_t* ks = ld_k + pg * a.k_page + in;
-          const uint8_t* vs = ld_v + pg * a.v_page + in;
-          const uint32_t to = dst + h * (2 * S::kPartBytes);
-#pragma unroll
-          for (int u = 0; u < kKeyLoads; ++u) cp_async16(to + 512 * u, ks + 512 * u, 16u);
-          cp_async16(to + 512 * kKeyLoads, lane < 16 ? ks + 512 * kKeyLoads : vs - kRest, 16u);
-#pragma unroll
-          for (int u = 0; u < kKeyLoads; ++u)
-            cp_async16(to + 512 * (kKeyLoads + 1) + 512 * u, vs + kRest + 512 * u, 16u);
+        // 16 keys that lie side by side, and their values, in one copy each
+        if (lane == 0) b200attn::ptx::mbar_arrive_expect_tx(bar, S::kBlockBytes);
+        if ((lane & 15) == 0) {
+          const int in = page_row * S::kRowBytes;
+          bulk_copy(dst, ld_k + page * a.k_page + in, S::kPartBytes, bar);
+          bulk_copy(dst + S::kPartBytes, ld_v + page * a.v_page + in, S::kPartBytes, bar);
         }
       } else {
-        if (page >= a.pages || (page < 0 && (whole ? lane & 16 : lane) < ld_keys)) {
+        // a lane a key
+        bool there = lane < ld_keys;
+        if (there && (page < 0 || page >= a.pages)) {
           report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
-          page = -1;
+          there = false;
+          for (int x = 0; x < 2 * S::kPieces; ++x)  // a row without a page is zero
+            *reinterpret_cast<uint4*>(blocks + stage * S::kBlockBytes + (lane / 16) * (2 * S::kPartBytes) +
+                                      (x / S::kPieces) * S::kPartBytes + (lane & 15) * S::kRowBytes +
+                                      16 * (x % S::kPieces)) = make_uint4(0u, 0u, 0u, 0u);
+          b200attn::ptx::fence_proxy_async_smem();
         }
-#pragma unroll 1
-        for (int x = lane; x < S::kBlockBytes / 16; x += 32) {
-          const int h = x / (S::kPartBytes / 8), z = x - h * (S::kPartBytes / 8);
-          const bool value = z >= S::kPartBytes / 16;
-          const int y = value ? z - S::kPartBytes / 16 : z;
-          const int r = y / S::kPieces, piece = y - r * S::kPieces;
-          const int from = 16 * h + (whole ? 0 : r);
-          const int pg = __shfl_sync(0xffffffffu, page, from);
-          const int64_t in = __shfl_sync(0xffffffffu, page_row, from) + (whole ? r : 0);
-          const uint8_t* src = value ? ld_v : ld_k;
-          const bool ok = pg >= 0 && 16 * h + r < ld_keys;
-          if (ok)
-            src += value ? pg * a.v_page + in * a.v_row + 16 * piece
-                         : pg * a.k_page + in * a.k_row + 16 * piece;
-          cp_async16(dst - 16 * lane + 16 * x, src, ok ? 16u : 0u);
+        const uint32_t rows = __popc(__ballot_sync(0xffffffffu, there));
+        if (lane == 0) b200attn::ptx::mbar_arrive_expect_tx(bar, rows * 2 * S::kRowBytes);
+        if (there) {
+          const int64_t in = page_row + (whole ? lane & 15 : 0);
+          const uint32_t to = dst + (lane & 15) * S::kRowBytes;
+          bulk_copy(to, ld_k + page * a.k_page + in * a.k_row, S::kRowBytes, bar);
+          bulk_copy(to + S::kPartBytes, ld_v + page * a.v_page + in * a.v_row, S::kRowBytes, bar);
         }
       }
       ld_key += S::kTile;
@@ -261,15 +264,19 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         enter(p);
       }
       if (ld_left > 0) look_up();
+      stage = stage + 1 == NS ? 0 : stage + 1;
     }
-    cp_async_commit();
-    stage = stage + 1 == NS ? 0 : stage + 1;
   };
+  if (lane == 0)
+    for (int x = 0; x < NS; ++x) b200attn::ptx::mbar_init(bars + 8 * x, 1);
+  b200attn::ptx::fence_mbar_init();
+  __syncwarp();
 #pragma unroll 1
-  for (int s = 0; s < NS - 1; ++s) issue();
+  for (int x = 0; x < NS - 1; ++x) issue();
 
   Place pl = run.p;
-  int use = 0;  // stage of the tile at hand
+  int use = 0;          // stage of the block at hand
+  uint32_t parity = 0;  // of its barrier
 
 #pragma unroll 1
   while (!run.done(pl)) {
@@ -371,10 +378,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll 1
     for (int t = t0; t < t0 + n; ++t) {
       issue();
-      cp_async_wait<NS - 1>();
-      __syncwarp();
-      const uint32_t block = ring + use * S::kBlockBytes;
-      use = use + 1 == NS ? 0 : use + 1;
+      if (!dead && !__all_sync(0xffffffffu, b200attn::ptx::mbar_try_wait(bars + 8 * use, parity)))
+        dead = !wait_long(bars + 8 * use, parity, a.err);
+      if (dead) break;
+      uint8_t* block = blocks + use * S::kBlockBytes;
+      if (++use == NS) {
+        use = 0;
+        parity ^= 1u;
+      }
       const int k0 = t * S::kTile + warp * S::kKeys;
       if (k0 < keys) {
         // ------------------------------------------------------- scores
@@ -382,26 +393,25 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         float s[S::kParts][NT][4];
 #pragma unroll
         for (int h = 0; h < S::kParts; ++h) {
-          const uint32_t row0 = block + h * (2 * S::kPartBytes) + r8 * S::kRowBytes;
-          const uint32_t row1 = row0 + 8 * S::kRowBytes;
+          const uint8_t* row0 = block + h * (2 * S::kPartBytes) + r8 * S::kRowBytes;
+          const uint8_t* row1 = row0 + 8 * S::kRowBytes;
           uint32_t w0[NG], w1[NG];
           if constexpr (NG == 4) {
-            const uint4 u = lds128(row0 + c4 * (S::kCodes / 4)), v = lds128(row1 + c4 * (S::kCodes / 4));
+            const uint4 u = lds<uint4>(row0 + c4 * (S::kCodes / 4)), v = lds<uint4>(row1 + c4 * (S::kCodes / 4));
             w0[0] = u.x, w0[1] = u.y, w0[2] = u.z, w0[3] = u.w;
             w1[0] = v.x, w1[1] = v.y, w1[2] = v.z, w1[3] = v.w;
           } else {
-            const uint2 u = lds64(row0 + c4 * (S::kCodes / 4)), v = lds64(row1 + c4 * (S::kCodes / 4));
+            const uint2 u = lds<uint2>(row0 + c4 * (S::kCodes / 4)), v = lds<uint2>(row1 + c4 * (S::kCodes / 4));
             w0[0] = u.x, w0[1] = u.y;
             w1[0] = v.x, w1[1] = v.y;
           }
-          const uint2 s0 = lds64(row0 + S::kCodes), s1 = lds64(row1 + S::kCodes);
+          const uint2 s0 = lds<uint2>(row0 + S::kCodes), s1 = lds<uint2>(row1 + S::kCodes);
           const uint32_t low0 = twice16(row0 + S::kCodes + 8 + 2 * c4);
           const uint32_t low1 = twice16(row1 + S::kCodes + 8 + 2 * c4);
           const uint32_t lows[4] = {low0, low1, low0, low1};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            s[h][nt][0] = s[h][nt][1] = s[h][nt][2] = s[h][nt][3] = 0.f;
-            mma16816<B200_ATTN_DTYPE_BF16>(s[h][nt], lows, qs[nt][0], qs[nt][1]);
+            mma<B200_ATTN_DTYPE_BF16>(s[h][nt], lows, qs[nt][0], qs[nt][1], 0.f, 0.f, 0.f, 0.f);
           }
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
@@ -413,10 +423,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
               const uint32_t kf[4] = {u & kLow, v & kLow, u & kHigh, v & kHigh};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                if (y == 0)
-                  mma_f16(p[nt], kf, qf[nt][step][0], qf[nt][step][1], 0.f, 0.f, 0.f, 0.f);
-                else
-                  mma16816<B200_ATTN_DTYPE_FP16>(p[nt], kf, qf[nt][step][0], qf[nt][step][1]);
+                {
+                const bool on = y > 0;
+                mma<B200_ATTN_DTYPE_FP16>(p[nt], kf, qf[nt][step][0], qf[nt][step][1],
+                                          on ? p[nt][0] : 0.f, on ? p[nt][1] : 0.f,
+                                          on ? p[nt][2] : 0.f, on ? p[nt][3] : 0.f);
+              }
               }
             }
             const uint32_t a0 = g < 2 ? s0.x : s0.y, a1 = g < 2 ? s1.x : s1.y;
@@ -448,24 +460,25 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
                 }
             }
           // A hidden value must not reach a row as 0 x NaN: steps and lows that are not finite become 0
-          // here, and are added below to the rows that see them.  A lane a key.
+          // here, and are added below to the rows that see them.  A lane a key.  Behind the last
+          // key lies what an earlier block left, which counts as 0 too.
           if (k0 + lane >= pl.s.len) {
-            const uint32_t at = block + (lane / 16) * (2 * S::kPartBytes) + S::kPartBytes +
+            uint8_t* at = block + (lane / 16) * (2 * S::kPartBytes) + S::kPartBytes +
                                 (lane & 15) * S::kRowBytes + S::kCodes;
-            uint4 v = lds128(at);
+            uint4 v = lds<uint4>(at);
             uint32_t* w = reinterpret_cast<uint32_t*>(&v);
             uint32_t any = 0u;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const uint32_t f = non_finite<B200_ATTN_DTYPE_BF16>(w[y]);
+              const uint32_t f =
+                  k0 + lane < keys ? non_finite<B200_ATTN_DTYPE_BF16>(w[y]) : 0xffffffffu;
               any |= f;
               w[y] &= ~f;
             }
             if (any) {
-              odd = true;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
-                           "r"(w[2]), "r"(w[3])
-                           : "memory");
+              odd |= k0 + lane < keys;
+              *reinterpret_cast<uint4*>(at) = v;
+              b200attn::ptx::fence_proxy_async_smem();  // the next copy lands here
             }
           }
           __syncwarp();
@@ -477,8 +490,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         uint32_t big;  // steps of two keys' values
         bool grew = false;
         {
-          const uint32_t at = block + S::kPartBytes + (lane & 15) * S::kRowBytes + S::kCodes;
-          const uint2 u = lds64(at), v = lds64(at + 2 * S::kPartBytes);
+          uint8_t* at = block + S::kPartBytes + (lane & 15) * S::kRowBytes + S::kCodes;
+          const uint2 u = lds<uint2>(at), v = lds<uint2>(at + 2 * S::kPartBytes);
           big = max_bf16x2(max_bf16x2(u.x, u.y), max_bf16x2(v.x, v.y));
           grew = (big >> 16) > most_step || (big & 0xffffu) > most_step;
         }
@@ -546,21 +559,21 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         // ------------------------------------------------------- values
 #pragma unroll
         for (int h = 0; h < S::kParts; ++h) {
-          const uint32_t vb = block + h * (2 * S::kPartBytes) + S::kPartBytes;
+          const uint8_t* vb = block + h * (2 * S::kPartBytes) + S::kPartBytes;
           // codes of keys 2 c4, 2 c4 + 1, and 8 further; steps and lows of keys r8 and r8 + 8
           uint32_t w[4][NG / 2];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t at = vb + (8 * (i >> 1) + 2 * c4 + (i & 1)) * S::kRowBytes + r8 * (S::kCodes / 8);
+            const uint8_t* at = vb + (8 * (i >> 1) + 2 * c4 + (i & 1)) * S::kRowBytes + r8 * (S::kCodes / 8);
             if constexpr (NG == 4) {
-              const uint2 v = lds64(at);
+              const uint2 v = lds<uint2>(at);
               w[i][0] = v.x, w[i][1] = v.y;
             } else {
-              w[i][0] = lds32(at);
+              w[i][0] = lds<uint32_t>(at);
             }
           }
-          const uint4 m0 = lds128(vb + r8 * S::kRowBytes + S::kCodes);
-          const uint4 m1 = lds128(vb + (r8 + 8) * S::kRowBytes + S::kCodes);
+          const uint4 m0 = lds<uint4>(vb + r8 * S::kRowBytes + S::kCodes);
+          const uint4 m1 = lds<uint4>(vb + (r8 + 8) * S::kRowBytes + S::kCodes);
           float pu[NT][4];  // weights times the steps' factor
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -595,8 +608,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
               const uint32_t vf[4] = {(v0 >> 8 * y) & kLow, (v0 >> 8 * y) & kHigh,
                                       (v1 >> 8 * y) & kLow, (v1 >> 8 * y) & kHigh};
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816<B200_ATTN_DTYPE_FP16>(o[nt][NG / 2 * g + y], vf, pf[nt][0], pf[nt][1]);
+              for (int nt = 0; nt < NT; ++nt) {
+                float(&d)[4] = o[nt][NG / 2 * g + y];
+                mma<B200_ATTN_DTYPE_FP16>(d, vf, pf[nt][0], pf[nt][1], d[0], d[1], d[2], d[3]);
+              }
             }
           }
         }
@@ -730,6 +745,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     __syncthreads();
   }
   zero_unused_rows(a, 2, S::kThreads);
+  if (dead)  // its copies may be on their way still
+    for (int x = 0; x < NS; ++x) wait_long(bars + 8 * x, (x >= use) == (parity != 0u), nullptr);
 }
 
 // -------------------------------------------------------------------- host

@@ -41,7 +41,7 @@ template <bool FEW_, int DP_>
 struct Shape4 {
   static constexpr bool FEW = FEW_;
   static constexpr int DP = DP_, RM = 16;
-  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kCtas = !FEW ? 2 : (DP_ == 128 ? 3 : 4);  // CTAs of an SM
+  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kCtas = !FEW ? 2 : 4;  // CTAs of an SM
   static constexpr int kParts = 2, kKeys = kParts * kRowKeys;  // keys of a warp's block
   static constexpr int kTile = kWarps * kKeys;
   static constexpr int kHalves = FEW ? 1 : 2;
@@ -49,7 +49,7 @@ struct Shape4 {
   static constexpr int kPieces = kRowBytes / 16;
   static constexpr int kPartBytes = kRowKeys * kRowBytes;  // 16 keys, or values
   static constexpr int kBlockBytes = kParts * 2 * kPartBytes;
-  static constexpr int kStages = DP == 128 ? (FEW ? 3 : 4) : (FEW ? 3 : 5);
+  static constexpr int kStages = DP == 128 ? (FEW ? 2 : 4) : (FEW ? 3 : 5);
   static constexpr int kRingBytes = kWarps * kStages * kBlockBytes;
   static constexpr int kJoinRows = FEW ? 8 : 16;
   static constexpr int kJoinCols = 512 / kJoinRows;
@@ -58,8 +58,8 @@ struct Shape4 {
   static constexpr int kOffJoin = kRingBytes;
   static constexpr int kJoinBytes = 4 * kWarps * kJoinRows * kJoinPitch;
   static constexpr int kOffStat = kOffJoin + kJoinBytes;
-  static constexpr int kOffPlaces = kOffStat + 4 * 2 * kWarps * RM;  // of the warps' loads
-  static constexpr int kOffBars = kOffPlaces + kWarps * sizeof(Place);  // a barrier a block
+  static constexpr int kOffPlaces = kOffStat + 4 * 2 * kWarps * RM;  // of the warps' loads, and two units
+  static constexpr int kOffBars = kOffPlaces + (kWarps + 2) * sizeof(Place);  // a barrier a block
   static constexpr int kOffMisc = kOffBars + 8 * kWarps * kStages;
   static constexpr int kSmemBytes = kOffMisc + 256;
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "exceeds the shared memory of an SM");
@@ -181,23 +181,17 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   const bool whole = a.page_size % kRowKeys == 0;  // 16 keys lie in one page
 
   // ------------------------------------------------------------- loads
-  // The warp's next block to load: its first key, the sequence's keys, blocks left in the unit, and
-  // where the unit's page numbers and pools begin.  Page numbers are read one block ahead.  The
-  // unit itself is in shared memory (`at`), for when it ends.
+  // The warp's next block to load: its first key and the blocks left in the unit, which itself is in
+  // shared memory (`at`): registers are what limits the warps on an SM.  Page numbers are read
+  // one block ahead.
   Place* at = reinterpret_cast<Place*>(smem + S::kOffPlaces) + warp;
-  int ld_key = 0, ld_total = 0, ld_left = 0;
-  const int32_t* ld_table = a.table;
-  const uint8_t *ld_k = a.k, *ld_v = a.v;
+  int ld_key = 0, ld_left = 0;
   auto enter = [&](const Place& p) {
     __syncwarp();
     if (lane == 0) *at = p;
     __syncwarp();
     ld_left = run.done(p) ? 0 : run.tiles(p);
     ld_key = p.t * S::kTile + warp * S::kKeys;
-    ld_total = p.s.len + p.s.drafts;
-    ld_table = a.table + p.b * a.table_stride;
-    ld_k = a.k + p.h * a.k_head;
-    ld_v = a.v + p.h * a.v_head;
   };
   enter(run.p);
   int page = -1, page_row = 0;
@@ -206,7 +200,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     const int key = ld_key + (whole ? lane & 16 : lane);
     page = -1;
     page_row = 0;
-    if (key < ld_total) {
+    if (key < at->s.len + at->s.drafts) {
       // key / size or one more: key is below 2^30
       uint32_t slot = size == 1u ? key : __umulhi(key, inv_size);
       page_row = key - static_cast<int>(slot * size);
@@ -214,7 +208,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
         --slot;
         page_row += static_cast<int>(size);
       }
-      page = __ldg(ld_table + slot);
+      page = __ldg(a.table + at->b * a.table_stride + slot);
     }
   };
   if (ld_left > 0) look_up();
@@ -223,7 +217,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   const bool tight = whole && a.k_row == S::kRowBytes && a.v_row == S::kRowBytes;
   auto issue = [&]() {
     if (ld_left > 0 && !dead) {
-      const int ld_keys = ld_total - ld_key;
+      const int ld_keys = at->s.len + at->s.drafts - ld_key;
+      const uint8_t* ld_k = a.k + at->h * a.k_head;
+      const uint8_t* ld_v = a.v + at->h * a.v_head;
       const uint32_t bar = bars + 8 * stage;
       const uint32_t dst = ring + stage * S::kBlockBytes + (lane / 16) * (2 * S::kPartBytes);
       if (tight && __all_sync(0xffffffffu, ld_keys >= S::kKeys && static_cast<uint32_t>(page) <
@@ -274,15 +270,20 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll 1
   for (int x = 0; x < NS - 1; ++x) issue();
 
-  Place pl = run.p;
+  // the CTA's unit, and the one after it
+  Place* units = reinterpret_cast<Place*>(smem + S::kOffPlaces) + S::kWarps;
+  if (tid == 0) units[0] = run.p;
+  __syncthreads();
+  int flip = 0;
   int use = 0;          // stage of the block at hand
   uint32_t parity = 0;  // of its barrier
 
 #pragma unroll 1
-  while (!run.done(pl)) {
+  while (!run.done(units[flip])) {
+    const Place& pl = units[flip];
     const int t0 = pl.t;
     const int n = run.tiles(pl);
-    const int keys = pl.s.len + pl.s.drafts;
+    const int len = pl.s.len, keys = len + pl.s.drafts;
     const int rows = min(RM, pl.s.drafts * a.group - pl.rt * RM);
 
     // ----------------------------------------------------------- queries
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             }
           }
         }
-        if (k0 + S::kKeys > pl.s.len) {  // drafted tokens, or past the last key
+        if (k0 + S::kKeys > len) {  // drafted tokens, or past the last key
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
               for (int h = 0; h < S::kParts; ++h)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                  const int j = k0 + 16 * h + 8 * y + r8 - pl.s.len;
+                  const int j = k0 + 16 * h + 8 * y + r8 - len;
                   if (j >= 0 && (j >= pl.s.drafts || !sees(a, pl.b, tok, j)))
                     s[h][nt][2 * y + e] = -INFINITY;
                 }
@@ -462,7 +463,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           // A hidden value must not reach a row as 0 x NaN: steps and lows that are not finite become 0
           // here, and are added below to the rows that see them.  A lane a key.  Behind the last
           // key lies what an earlier block left, which counts as 0 too.
-          if (k0 + lane >= pl.s.len) {
+          if (k0 + lane >= len) {
             uint8_t* at = block + (lane / 16) * (2 * S::kPartBytes) + S::kPartBytes +
                                 (lane & 15) * S::kRowBytes + S::kCodes;
             uint4 v = lds<uint4>(at);
@@ -620,10 +621,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     }
 
     // ------------------------------------------- join the warps' results
-    const Place done = pl;
+    const Place& done = pl;
     const bool first = t0 == 0, last = t0 + n == pl.tiles;
-    pl.t += n;
-    if (pl.t == pl.tiles) pl = next_unit<typename S::G>(a, pl);
+    flip ^= 1;
+    if (tid == 0) {
+      Place p = pl;
+      p.t += n;
+      if (p.t == p.tiles) p = next_unit<typename S::G>(a, p);
+      units[flip] = p;
+    }
     // the steps' factor and the codes' 2^-24 leave the sums (in two factors)
     const float unit0 = __uint_as_float((127u + top_step / 2) << 23);
     const float unit1 = __uint_as_float((127u + (top_step + 1) / 2 - 137u + 24u) << 23);

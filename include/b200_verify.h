@@ -25,7 +25,7 @@
  * without a distribution (a NaN or +infinity, or nothing above -infinity), whose children
  * are not kept.  Draft probabilities below 0 and NaN count as 0.
  *
- * Sums are 64-bit; the test of a first child takes the row's sum of fp32 exponentials.
+ * Exponentials and sums are 64-bit.
  * Results do not depend on execution order.  A token id out of range, a parent that
  * does not come before its child and a draft length out of range are reported in the error
  * word (B200_ATTN_DEVERR_BOUNDS): such a node is not kept, such a sequence counts as empty.

@@ -4,13 +4,18 @@
 // A cluster of CTAs walks the tree of one sequence.  Only the rows of the nodes on the path
 // are read, each by all CTAs of the cluster, a contiguous share a warp; the CTAs
 // exchange their sums through distributed shared memory and all take the same decisions.  A
-// step down the tree is one pass over a row (maximum and sum of exponentials, fp32).  Refused
-// drafts with probabilities take further passes over the row of the target and that of
-// the drafter, which lie in L2 by then: the sum again in 64 bits, and the sum of what is left
-// after each refusal.  The last pass's sums, a warp each, say in which share the next token lies;
-// it is divided among the warps of its CTA once more, and one warp scans the part.
-// Exponentials and sums that the next token hangs on are 64-bit: among 32000 cumulated
-// weights a sum that is off by 1e-8 would pick a neighbour once in some thousand draws.
+// step down the tree is one pass over a row: the sum of e^(l / T).  What is left after k refusals of
+// drafts with probabilities q, each time normalised, is
+//   max(p - t_k q, 0) / F(t_k),  F(t) = sum of max(p - t q, 0),  t_1 = 1,  t_(k+1) = t_k + F(t_k),
+// (max(y / Z - q, 0) of y = max(a p - b q, 0) is max(a / Z p - (b / Z + 1) q, 0)): a refusal takes
+// one more pass over the row of the target, which lies in L2 by then, and that of the drafter,
+// whatever was refused before it.  The last pass's sums, a warp each, say in which share
+// the next token lies; it is divided among the warps of its CTA once more, and one warp
+// scans the part.
+// Exponentials and sums are 64-bit: among 32000 cumulated weights a sum that is off by 1e-8
+// would pick a neighbour once in some thousand draws.  The exponentials need no maximum
+// beforehand: e^(l / T) does not leave the range of 64 bits unless |l / T| is over 600, and such
+// a row is summed again relative to its maximum.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -58,19 +63,18 @@ struct Args {
 
 struct Exchange {  // what a CTA tells the others
   double sum;
-  float top;
-  int32_t at;  // of the largest number
+  float top;   // largest number
+  int32_t at;  // its place
   int32_t bad;
 };
 
 struct Smem {
   Exchange told[2][kMaxCluster];
   Exchange warp[kWarps];
-  double warp_sum[kWarps];
   double part_sum[kWarps];
-  double z[kMaxNodes];        // sums of what was left after each refusal at a node
+  double power[64];           // 2^(j / 64)
   int32_t parent[kMaxNodes];
-  int32_t token[kMaxNodes];   // -1: out of range
+  int32_t token[kMaxNodes];
   float uniform[kMaxNodes];
   float logit[kMaxNodes];     // the target's for the node's token, in its parent's row
   float prob[kMaxNodes];      // the drafter's
@@ -123,60 +127,154 @@ __device__ __forceinline__ float one_prob(const Args& a, const uint8_t* row, int
   return as_prob(__half2float(reinterpret_cast<const __half*>(row)[v]));
 }
 
-// What is known of the node that the path has reached.
+// The node that the path has reached.  Number v has the weight max(scale e^((l - top) / T) - t q, 0),
+// or 0 where it is one of `refused`.
 struct Node {
   const uint8_t* row;
   const uint8_t* probs;
-  float top;       // largest logit
-  double sum;      // of exp((l - top) / T): of fp32 exponentials, until it is needed in 64 bits
-  bool exact;      // sum is the 64-bit one
-  int refusals;    // sums in z, or tokens in `refused`
+  double top, scale, t;
+  int refused;
 };
 
-__device__ __forceinline__ double weight(const Args& a, float l, float top) {
-  return exp((static_cast<double>(l) - static_cast<double>(top)) * a.inv_temp);
+// e^z for z up to 700, and 0 below -700: 2^(k / 64) from a table times a polynomial for the rest
+// (Tang, "Table-driven implementation of the exponential function in IEEE floating-point
+// arithmetic", 1989).  |r| <= ln 2 / 128: the first term left out is below 4e-14 of the result, and
+// r is off by 1e-13 at most.
+__device__ __forceinline__ double exp_of(const double* power, double z) {
+  constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are the integer
+  const double t = fma(z, 92.332482616893656877, kRound);  // 64 / ln 2
+  const int k = __double2loint(t);
+  const double r = fma(t - kRound, -0.010830424696249145, z);  // ln 2 / 64
+  double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+  p = fma(r, p, 0.5);
+  p = fma(r * r, p, r);
+  const double w = power[k & 63];
+  const double y = fma(w, p, w);
+  return z > -700.0 ? __hiloint2double(__double2hiint(y) + ((k >> 6) << 20), __double2loint(y)) : 0.0;
 }
 
-// The weight that is left of `e` after the node's refusals, with the drafter's q.
-__device__ __forceinline__ double left_of(const Smem& sm, const Node& n, int level, double e,
-                                          double q) {
-  double y = e;
-  if (level > 0) {
-    y = fmax(y / n.sum - q, 0.0);
-    for (int j = 1; j < level; ++j) y = fmax(y / sm.z[j - 1] - q, 0.0);
-  }
-  return y;
+__device__ __forceinline__ double weight(const Args& a, const Smem& sm, float l, double top) {
+  return exp_of(sm.power, fma(static_cast<double>(l), a.inv_temp, -top));
 }
 
-// Four such weights from number v on.
-template <int DT>
-__device__ __forceinline__ void weights4(const Args& a, const Smem& sm, const Node& n, int level,
-                                         int v, int end, bool vec, double (&y)[4]) {
-  float l[4], q[4] = {0.f, 0.f, 0.f, 0.f};
-  load4<DT>(n.row, v, end, vec, -INFINITY, l);
-  if (level > 0) probs4(a, n.probs, v, end, q);
+// The weights of four numbers from v on.
+__device__ __forceinline__ void weights4(const Args& a, const Smem& sm, const Node& n, int v,
+                                         const float (&l)[4], const float (&q)[4], double (&y)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    double e = l[i] == -INFINITY ? 0.0 : weight(a, l[i], n.top);
-    if (!a.probs)
-      for (int j = 0; j < n.refusals; ++j)
-        if (sm.refused[j] == v + i) e = 0.0;
-    y[i] = left_of(sm, n, level, e, q[i]);
+  for (int i = 0; i < 4; ++i)
+    y[i] = fmax(fma(weight(a, sm, l[i], n.top), n.scale, -n.t * static_cast<double>(q[i])), 0.0);
+  for (int j = 0; j < n.refused; ++j) {
+    const uint32_t x = static_cast<uint32_t>(sm.refused[j] - v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (x == i) y[i] = 0.0;
   }
 }
 
-__device__ __forceinline__ double warp_total(double x) {
+template <class T>
+__device__ __forceinline__ T warp_total(T x) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
   return x;
 }
 
-// Tells `mine` (thread 0's) to every CTA of the cluster; by all threads of all CTAs.  Two
-// slots in turn: a CTA writes a slot again when all have passed the barrier after reading it.
-__device__ __forceinline__ void tell(Smem& sm, int& turn, const Exchange& mine, uint32_t rank,
-                                     uint32_t ctas) {
-  turn ^= 1;
+// A row's first pass, of numbers [begin, end) by a warp: the sum of e^((l - top) / T), the largest logit and
+// its place, and whether one is NaN or +infinity.
+template <int DT, bool VEC>
+__device__ __noinline__ Exchange first_pass(const Args& a, const Smem& sm, const uint8_t* row,
+                                            double top, int begin, int end) {
+  constexpr int kDeep = 4;  // loads in flight
+  const int lane = threadIdx.x & 31;
+  Exchange x{0.0, -INFINITY, 0x7fffffff, 0};
+  double sum[2] = {0.0, 0.0};
+  for (int v = begin + 4 * lane; v < end; v += 128 * kDeep) {
+    float l[kDeep][4];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      if (v + 128 * u < end) {
+        load4<DT>(row, v + 128 * u, end, VEC, -INFINITY, l[u]);
+      } else {
+        l[u][0] = l[u][1] = l[u][2] = l[u][3] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x.bad |= !(l[u][i] < INFINITY);
+        if (l[u][i] > x.top) {
+          x.top = l[u][i];
+          x.at = v + 128 * u + i;
+        }
+      }
+    if (a.inv_temp != 0.0) {
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i & 1] += weight(a, sm, l[u][i], top);
+    }
+  }
+  x.sum = warp_total(sum[0] + sum[1]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float high = __shfl_xor_sync(kAll, x.top, o);
+    const int at = __shfl_xor_sync(kAll, x.at, o);
+    if (high > x.top || (high == x.top && at < x.at)) {
+      x.top = high;
+      x.at = at;
+    }
+  }
+  x.bad = __any_sync(kAll, x.bad);
+  return x;
+}
+
+// The sum of the weights of numbers [begin, end), by a warp.
+template <int DT, bool VEC>
+__device__ __noinline__ double sum_pass(const Args& a, const Smem& sm, const Node& n, int begin,
+                                        int end) {
+  constexpr int kDeep = 2;  // loads in flight
+  double sum[2] = {0.0, 0.0};
+  for (int v = begin + 4 * (threadIdx.x & 31); v < end; v += 128 * kDeep) {
+    float l[kDeep][4], q[kDeep][4];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[u][i] = -INFINITY, q[u][i] = 0.f;
+      if (v + 128 * u < end) {
+        load4<DT>(n.row, v + 128 * u, end, VEC, -INFINITY, l[u]);
+        if (n.t != 0.0) probs4(a, n.probs, v + 128 * u, end, q[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      double y[4];
+      weights4(a, sm, n, v + 128 * u, l[u], q[u], y);
+      sum[u] += (y[0] + y[1]) + (y[2] + y[3]);
+    }
+  }
+  return warp_total(sum[0] + sum[1]);
+}
+
+__device__ __forceinline__ void take(Exchange& x, const Exchange& y) {
+  x.sum += y.sum;
+  if (y.top > x.top || (y.top == x.top && y.at < x.at)) {
+    x.top = y.top;
+    x.at = y.at;
+  }
+  x.bad |= y.bad;
+}
+
+// Every warp's x to all: those of this CTA into sm.warp, the CTAs' into sm.told[turn], and what they
+// come to.  By all threads of all CTAs.  Two slots in turn: a CTA writes a slot again when all
+// have passed the barrier after reading it.
+__device__ __noinline__ Exchange share_out(Smem& sm, int turn, const Exchange x, uint32_t rank,
+                                           uint32_t ctas) {
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm.warp[threadIdx.x >> 5] = x;
+  __syncthreads();
   if (threadIdx.x < ctas) {
+    Exchange mine = sm.warp[0];
+    for (int w = 1; w < kWarps; ++w) take(mine, sm.warp[w]);
     const uint32_t at = b200attn::ptx::mapa_shared(
         b200attn::ptx::smem_u32(&sm.told[turn][rank]), threadIdx.x);
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(mine.sum) : "memory");
@@ -185,6 +283,9 @@ __device__ __forceinline__ void tell(Smem& sm, int& turn, const Exchange& mine, 
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + 16), "r"(mine.bad) : "memory");
   }
   b200attn::ptx::cluster_sync();
+  Exchange all = sm.told[turn][0];
+  for (uint32_t c = 1; c < ctas; ++c) take(all, sm.told[turn][c]);
+  return all;
 }
 
 template <int DT, bool VEC>
@@ -202,6 +303,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
     if (tid == 0 && rank == 0) report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
     n = 0;
   }
+  if (tid < 64) sm.power[tid] = exp2(tid / 64.0);
   const uint8_t* logits = a.logits + b * a.l_seq;
   const uint8_t* probs = a.probs ? a.probs + b * a.q_seq : nullptr;
   for (int i = tid; i < n; i += kThreads) {
@@ -237,152 +339,77 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
   bool teller = rank == 0;  // this CTA writes the next token
   Node node{};
 
-  // Sums the weights that are left after `level` refusals: sm.warp_sum a warp of this CTA, told[turn] a
-  // CTA, and in all.
-  auto total_of = [&](int level) {
-    double s = 0.0;
-    for (int v = begin + 4 * lane; v < end; v += 128) {
-      double y[4];
-      weights4<DT>(a, sm, node, level, v, end, VEC, y);
-      s += (y[0] + y[1]) + (y[2] + y[3]);
-    }
-    s = warp_total(s);
-    __syncthreads();
-    if (lane == 0) sm.warp_sum[warp] = s;
-    __syncthreads();
-    Exchange mine{0.0, 0.f, 0, 0};
-    for (int w = 0; w < kWarps; ++w) mine.sum += sm.warp_sum[w];
-    tell(sm, turn, mine, rank, ctas);
-    double total = 0.0;
-    for (uint32_t c = 0; c < ctas; ++c) total += sm.told[turn][c].sum;
-    return total;
+  auto first_of = [&]() {
+    turn ^= 1;
+    return share_out(sm, turn, first_pass<DT, VEC>(a, sm, node.row, node.top, begin, end), rank, ctas);
+  };
+  auto sum_of = [&]() {
+    turn ^= 1;
+    return share_out(sm, turn, Exchange{sum_pass<DT, VEC>(a, sm, node, begin, end), 0.f, 0, 0}, rank,
+                     ctas).sum;
   };
 
   while (n > 0) {
-    // ------------------------------------- a node: its largest logit and its sum
+    // --------------------------------------------------- a node: its sum of weights
     if (tid == 0 && rank == 0) sm.path[length] = at;
     ++length;
-    node.row = logits + at * a.l_node;
-    node.probs = probs ? probs + at * a.q_node : nullptr;
-    node.exact = false;
-    node.refusals = 0;
-    float top = -INFINITY, sum = 0.f;
-    int where = 0;
-    bool bad = false;
-    const float to_log2 = static_cast<float>(a.inv_temp * 1.4426950408889634);
-    for (int v = begin + 4 * lane; v < end; v += 4 * 128) {
-      float l[4][4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (v + 128 * u < end) {
-          load4<DT>(node.row, v + 128 * u, end, VEC, -INFINITY, l[u]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) l[u][i] = -INFINITY;
-        }
-      }
-      float big = top;
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bad |= !(l[u][i] < INFINITY);
-          if (l[u][i] > big) {
-            big = l[u][i];
-            where = v + 128 * u + i;
-          }
-        }
-      if (big == -INFINITY) continue;
-      sum *= exp2f((top - big) * to_log2);
-      top = big;
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += exp2f((l[u][i] - big) * to_log2);
+    node = Node{logits + at * a.l_node, probs ? probs + at * a.q_node : nullptr, 0.0, 1.0, 0.0, 0};
+    Exchange all = first_of();
+    if (all.bad || all.top == -INFINITY) break;  // no distribution
+    if (fabs(static_cast<double>(all.top) * a.inv_temp) > 600.0) {
+      node.top = static_cast<double>(all.top) * a.inv_temp;
+      all = first_of();
     }
-    Exchange mine{sum, top, where, bad ? 1 : 0};
-    auto take = [&](Exchange& x, const Exchange& y) {  // y lies behind or before x
-      const float big = fmaxf(x.top, y.top);
-      if (y.top > x.top || (y.top == x.top && y.at < x.at)) x.at = y.at;
-      if (big > -INFINITY)
-        x.sum = x.sum * exp2f((x.top - big) * to_log2) + y.sum * exp2f((y.top - big) * to_log2);
-      x.top = big;
-      x.bad |= y.bad;
-    };
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Exchange y;
-      y.sum = __shfl_xor_sync(kAll, mine.sum, o);
-      y.top = __shfl_xor_sync(kAll, mine.top, o);
-      y.at = __shfl_xor_sync(kAll, mine.at, o);
-      y.bad = __shfl_xor_sync(kAll, mine.bad, o);
-      take(mine, y);
-    }
-    __syncthreads();
-    if (lane == 0) sm.warp[warp] = mine;
-    __syncthreads();
-    mine = sm.warp[0];
-    for (int w = 1; w < kWarps; ++w) take(mine, sm.warp[w]);
-    tell(sm, turn, mine, rank, ctas);
-    mine = sm.told[turn][0];
-    for (uint32_t c = 1; c < ctas; ++c) take(mine, sm.told[turn][c]);
-    node.top = mine.top;
-    node.sum = mine.sum;
-    const bool none = mine.bad || mine.top == -INFINITY;  // no distribution
-    if (none) break;
+    const double inv = 1.0 / all.sum;
 
     // --------------------------------------------------- its children in order
     int kept = -1;
-    double gone = 0.0;   // weight of the refused tokens, where drafts count as certain
-    bool summed = false; // warp_sum and told hold what is left now
-    double left = 0.0;   // its sum
+    double gone = 0.0;       // weight of the refused tokens, where drafts count as certain
+    bool summed = true;      // sm.warp and told hold the sums of the weights as they are now
+    double left = all.sum;   // in all
+    const int likeliest = all.at;
     for (int i0 = at + 1; i0 < n && kept < 0; i0 += 32) {
       uint32_t mask = __ballot_sync(kAll, i0 + lane < n && sm.parent[i0 + lane] == at);
       while (mask != 0u && kept < 0) {
         const int c = i0 + __ffs(mask) - 1;
         mask &= mask - 1;
         if (a.inv_temp == 0.0) {
-          if (sm.token[c] == mine.at && sm.uniform[c] < 1.f) kept = c;
+          if (sm.token[c] == likeliest && sm.uniform[c] < 1.f) kept = c;
           continue;
         }
-        const double e = sm.logit[c] == -INFINITY ? 0.0 : weight(a, sm.logit[c], node.top);
+        const double e = weight(a, sm, sm.logit[c], node.top);
         const double u = static_cast<double>(sm.uniform[c]);
         if (!probs) {
           bool again = false;
-          for (int j = 0; j < node.refusals; ++j) again |= sm.refused[j] == sm.token[c];
+          for (int j = 0; j < node.refused; ++j) again |= sm.refused[j] == sm.token[c];
           if (again) continue;
-          if (u * (node.sum - gone) < e) {
+          if (u * (all.sum - gone) < e) {
             kept = c;
-            continue;
-          }
-          if (node.sum - gone - e > 0.0) {  // something is left without it
+          } else if (all.sum - gone - e > 0.0) {  // something is left without it
             gone += e;
             __syncthreads();
-            if (tid == 0) sm.refused[node.refusals] = sm.token[c];
+            if (tid == 0) sm.refused[node.refused] = sm.token[c];
             __syncthreads();
-            ++node.refusals;
+            ++node.refused;
+            summed = false;
           }
           continue;
         }
         const double q = static_cast<double>(sm.prob[c]);
-        const double y = left_of(sm, node, node.refusals, e, q);
-        const double of = node.refusals > 0 ? sm.z[node.refusals - 1] : node.sum;
-        if (u * q * of < y) {
+        if (u * q * left < fmax(fma(e, node.scale, -node.t * q), 0.0)) {
           kept = c;
           continue;
         }
-        if (!node.exact) {
-          node.sum = total_of(0);
-          node.exact = true;
-        }
-        const double rest = total_of(node.refusals + 1);
+        // the weights so far were e, or max(p - t q, 0), which add up to `left`
+        const Node before = node;
+        node.t = node.t == 0.0 ? 1.0 : node.t + left;
+        node.scale = inv;
+        const double rest = sum_of();
         summed = rest > 0.0;
         if (summed) {
           left = rest;
-          __syncthreads();
-          if (tid == 0) sm.z[node.refusals] = rest;
-          __syncthreads();
-          ++node.refusals;
+        } else {
+          node = before;
         }
       }
     }
@@ -392,13 +419,12 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
     }
     // ------------------------------------------------------- the next token
     if (a.inv_temp == 0.0) {
-      next = mine.at;
+      next = likeliest;
       break;
     }
-    const int level = probs ? node.refusals : 0;
-    if (!summed) left = total_of(level);
-    if (!(left > 0.0)) {  // only by the rounding of the row's sum: refusals leave something
-      next = mine.at;
+    if (!summed) left = sum_of();
+    if (!(left > 0.0)) {  // only by the rounding of a sum: refusals leave something
+      next = likeliest;
       break;
     }
     const double goal = static_cast<double>(sm.uniform[0]) * left;
@@ -423,23 +449,15 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
     const int cta = find([&](int i) { return sm.told[turn][i].sum; }, static_cast<int>(ctas));
     teller = cta == static_cast<int>(rank);
     if (!teller) break;
-    const int owner = find([&](int i) { return sm.warp_sum[i]; }, kWarps);
+    const int owner = find([&](int i) { return sm.warp[i].sum; }, kWarps);
     const int part = (a.share / 4 + kWarps - 1) / kWarps * 4;
     const int from = min(static_cast<int64_t>(a.vocab),
                          static_cast<int64_t>(rank * kWarps + owner) * a.share);
     const int to = min(static_cast<int64_t>(a.vocab), from + static_cast<int64_t>(a.share));
-    {
-      double s = 0.0;
-      const int stop = min(to, from + (warp + 1) * part);
-      for (int v = from + warp * part + 4 * lane; v < stop; v += 128) {
-        double y[4];
-        weights4<DT>(a, sm, node, level, v, stop, VEC, y);
-        s += (y[0] + y[1]) + (y[2] + y[3]);
-      }
-      s = warp_total(s);
-      if (lane == 0) sm.part_sum[warp] = s;
-      __syncthreads();
-    }
+    const double mine = sum_pass<DT, VEC>(a, sm, node, min(to, from + warp * part),
+                                          min(to, from + (warp + 1) * part));
+    if (lane == 0) sm.part_sum[warp] = mine;
+    __syncthreads();
     const int which = find([&](int i) { return sm.part_sum[i]; }, kWarps);
     if (warp == 0) {
       const int stop = min(to, from + (which + 1) * part);
@@ -447,7 +465,12 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
       for (int v0 = from + which * part; v0 < stop && found < 0; v0 += 128) {
         const int v = v0 + 4 * lane;
         double y[4] = {0.0, 0.0, 0.0, 0.0};
-        if (v < stop) weights4<DT>(a, sm, node, level, v, stop, VEC, y);
+        if (v < stop) {
+          float l[4], q[4] = {0.f, 0.f, 0.f, 0.f};
+          load4<DT>(node.row, v, stop, VEC, -INFINITY, l);
+          if (node.t != 0.0) probs4(a, node.probs, v, stop, q);
+          weights4(a, sm, node, v, l, q, y);
+        }
         double mine4 = (y[0] + y[1]) + (y[2] + y[3]), cum = mine4;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {

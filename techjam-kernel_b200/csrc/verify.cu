@@ -20,6 +20,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <mutex>
 
 #include "b200_verify.h"
 #include "byte_range.h"
@@ -35,7 +36,7 @@ using b200tree::Elem;
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps, kMaxCluster = 8;
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kMaxCluster = 16;
 constexpr int kMaxNodes = B200_VERIFY_MAX_NODES;
 constexpr uint32_t kAll = 0xffffffffu;
 
@@ -58,6 +59,7 @@ struct Args {
   int32_t nodes, vocab, share;  // share: numbers of a warp, a multiple of 4
   int32_t probs_type, wide_tokens;
   bool probs_vec;
+  bool keep;  // a row's exponentials fit in shared memory
   int32_t* err;
 };
 
@@ -68,19 +70,34 @@ struct Exchange {  // what a CTA tells the others
   int32_t bad;
 };
 
+// Shared memory of a CTA: what the nodes need lies behind the fixed part, and the exponentials of
+// the CTA's share of the row behind that.
 struct Smem {
   Exchange told[2][kMaxCluster];
   Exchange warp[kWarps];
   double part_sum[kWarps];
-  double power[64];           // 2^(j / 64)
-  int32_t parent[kMaxNodes];
-  int32_t token[kMaxNodes];
-  float uniform[kMaxNodes];
-  float logit[kMaxNodes];     // the target's for the node's token, in its parent's row
-  float prob[kMaxNodes];      // the drafter's
-  int32_t refused[kMaxNodes]; // tokens refused at this node that have no weight any more
-  int32_t path[kMaxNodes];
+  double power[64];  // 2^(j / 64)
 };
+struct Views {
+  int32_t* parent;
+  int32_t* token;
+  float* uniform;
+  float* logit;      // the target's for the node's token, in its parent's row
+  float* prob;       // the drafter's
+  int32_t* refused;  // tokens refused at this node that have no weight any more
+  int32_t* path;
+  double* kept;
+};
+constexpr int kNodeArrays = 7;
+__host__ __device__ inline int nodes_padded(int nodes) { return (nodes + 3) & ~3; }
+
+__device__ __forceinline__ Views views_of(uint8_t* smem, int nodes) {
+  int32_t* p = reinterpret_cast<int32_t*>(smem + sizeof(Smem));
+  const int n = nodes_padded(nodes);
+  return Views{p, p + n, reinterpret_cast<float*>(p + 2 * n), reinterpret_cast<float*>(p + 3 * n),
+               reinterpret_cast<float*>(p + 4 * n), p + 5 * n, p + 6 * n,
+               reinterpret_cast<double*>(p + kNodeArrays * n)};
+}
 
 // Four numbers of a row from number v on; `vec`: by one load where all four are there.
 template <int DT, class T = typename Elem<DT>::T>
@@ -157,14 +174,36 @@ __device__ __forceinline__ double weight(const Args& a, const Smem& sm, float l,
   return exp_of(sm.power, fma(static_cast<double>(l), a.inv_temp, -top));
 }
 
-// The weights of four numbers from v on.
-__device__ __forceinline__ void weights4(const Args& a, const Smem& sm, const Node& n, int v,
-                                         const float (&l)[4], const float (&q)[4], double (&y)[4]) {
+// e^((l - top) / T) of four numbers, into or out of the CTA's kept ones (`kept`: the first's).
+__device__ __forceinline__ void keep4(double* kept, const double (&e)[4]) {
+  reinterpret_cast<double2*>(kept)[0] = make_double2(e[0], e[1]);
+  reinterpret_cast<double2*>(kept)[1] = make_double2(e[2], e[3]);
+}
+
+// The weights of four numbers from v on; `base`: the CTA's first number.
+template <int DT, bool VEC>
+__device__ __forceinline__ void weights4(const Args& a, const Smem& sm, const Views& vw,
+                                         const Node& n, int v, int base, int end, double (&y)[4]) {
+  float q[4] = {0.f, 0.f, 0.f, 0.f};
+  if (n.t != 0.0) probs4(a, n.probs, v, end, q);
+  if (a.keep) {
+    const double2* p = reinterpret_cast<const double2*>(vw.kept + (v - base));
+    const double2 e0 = p[0], e1 = p[1];
+    y[0] = e0.x, y[1] = e0.y, y[2] = e1.x, y[3] = e1.y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (v + i >= end) y[i] = 0.0;
+  } else {
+    float l[4];
+    load4<DT>(n.row, v, end, VEC, -INFINITY, l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = weight(a, sm, l[i], n.top);
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    y[i] = fmax(fma(weight(a, sm, l[i], n.top), n.scale, -n.t * static_cast<double>(q[i])), 0.0);
+    y[i] = fmax(fma(y[i], n.scale, -n.t * static_cast<double>(q[i])), 0.0);
   for (int j = 0; j < n.refused; ++j) {
-    const uint32_t x = static_cast<uint32_t>(sm.refused[j] - v);
+    const uint32_t x = static_cast<uint32_t>(vw.refused[j] - v);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (x == i) y[i] = 0.0;
@@ -178,15 +217,18 @@ __device__ __forceinline__ T warp_total(T x) {
   return x;
 }
 
-// A row's first pass, of numbers [begin, end) by a warp: the sum of e^((l - top) / T), the largest logit and
-// its place, and whether one is NaN or +infinity.
+// A row's first pass, of numbers [begin, end) by a warp: the sum of e^((l - top) / T), the largest
+// logit and whether one is NaN or +infinity; at temperature 0 the place of the largest instead of
+// the sum.
 template <int DT, bool VEC>
-__device__ __noinline__ Exchange first_pass(const Args& a, const Smem& sm, const uint8_t* row,
-                                            double top, int begin, int end) {
+__device__ __noinline__ Exchange first_pass(const Args& a, const Smem& sm, const Views& vw,
+                                            const uint8_t* row, double top, int base, int begin,
+                                            int end) {
   constexpr int kDeep = 4;  // loads in flight
   const int lane = threadIdx.x & 31;
   Exchange x{0.0, -INFINITY, 0x7fffffff, 0};
   double sum[2] = {0.0, 0.0};
+  bool bad = false;
   for (int v = begin + 4 * lane; v < end; v += 128 * kDeep) {
     float l[kDeep][4];
 #pragma unroll
@@ -200,18 +242,28 @@ __device__ __noinline__ Exchange first_pass(const Args& a, const Smem& sm, const
 #pragma unroll
     for (int u = 0; u < kDeep; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x.bad |= !(l[u][i] < INFINITY);
-        if (l[u][i] > x.top) {
-          x.top = l[u][i];
-          x.at = v + 128 * u + i;
-        }
-      }
-    if (a.inv_temp != 0.0) {
+      for (int i = 0; i < 4; ++i) bad |= !(l[u][i] < INFINITY);
+    if (a.inv_temp == 0.0) {
 #pragma unroll
       for (int u = 0; u < kDeep; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i & 1] += weight(a, sm, l[u][i], top);
+        for (int i = 0; i < 4; ++i)
+          if (l[u][i] > x.top) {
+            x.top = l[u][i];
+            x.at = v + 128 * u + i;
+          }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        double e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x.top = fmaxf(x.top, l[u][i]);
+          e[i] = weight(a, sm, l[u][i], top);
+          sum[i & 1] += e[i];
+        }
+        if (a.keep && v + 128 * u < end) keep4(vw.kept + (v + 128 * u - base), e);
+      }
     }
   }
   x.sum = warp_total(sum[0] + sum[1]);
@@ -224,35 +276,22 @@ __device__ __noinline__ Exchange first_pass(const Args& a, const Smem& sm, const
       x.at = at;
     }
   }
-  x.bad = __any_sync(kAll, x.bad);
+  x.bad = __any_sync(kAll, bad);
   return x;
 }
 
 // The sum of the weights of numbers [begin, end), by a warp.
 template <int DT, bool VEC>
-__device__ __noinline__ double sum_pass(const Args& a, const Smem& sm, const Node& n, int begin,
-                                        int end) {
-  constexpr int kDeep = 2;  // loads in flight
-  double sum[2] = {0.0, 0.0};
-  for (int v = begin + 4 * (threadIdx.x & 31); v < end; v += 128 * kDeep) {
-    float l[kDeep][4], q[kDeep][4];
-#pragma unroll
-    for (int u = 0; u < kDeep; ++u) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) l[u][i] = -INFINITY, q[u][i] = 0.f;
-      if (v + 128 * u < end) {
-        load4<DT>(n.row, v + 128 * u, end, VEC, -INFINITY, l[u]);
-        if (n.t != 0.0) probs4(a, n.probs, v + 128 * u, end, q[u]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kDeep; ++u) {
-      double y[4];
-      weights4(a, sm, n, v + 128 * u, l[u], q[u], y);
-      sum[u] += (y[0] + y[1]) + (y[2] + y[3]);
-    }
+__device__ __noinline__ double sum_pass(const Args& a, const Smem& sm, const Views& vw,
+                                        const Node& n, int base, int begin, int end) {
+  double sum = 0.0;
+#pragma unroll 2
+  for (int v = begin + 4 * (threadIdx.x & 31); v < end; v += 128) {
+    double y[4];
+    weights4<DT, VEC>(a, sm, vw, n, v, base, end, y);
+    sum += (y[0] + y[1]) + (y[2] + y[3]);
   }
-  return warp_total(sum[0] + sum[1]);
+  return warp_total(sum);
 }
 
 __device__ __forceinline__ void take(Exchange& x, const Exchange& y) {
@@ -274,6 +313,7 @@ __device__ __noinline__ Exchange share_out(Smem& sm, int turn, const Exchange x,
   __syncthreads();
   if (threadIdx.x < ctas) {
     Exchange mine = sm.warp[0];
+#pragma unroll
     for (int w = 1; w < kWarps; ++w) take(mine, sm.warp[w]);
     const uint32_t at = b200attn::ptx::mapa_shared(
         b200attn::ptx::smem_u32(&sm.told[turn][rank]), threadIdx.x);
@@ -284,7 +324,9 @@ __device__ __noinline__ Exchange share_out(Smem& sm, int turn, const Exchange x,
   }
   b200attn::ptx::cluster_sync();
   Exchange all = sm.told[turn][0];
-  for (uint32_t c = 1; c < ctas; ++c) take(all, sm.told[turn][c]);
+#pragma unroll
+  for (uint32_t c = 1; c < kMaxCluster; ++c)
+    if (c < ctas) take(all, sm.told[turn][c]);
   return all;
 }
 
@@ -292,6 +334,7 @@ template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_constant__ Args a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Smem& sm = *reinterpret_cast<Smem*>(raw);
+  const Views vw = views_of(raw, a.nodes);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ctas = gridDim.x, rank = blockIdx.x;  // one cluster a sequence
   const int64_t b = blockIdx.y;
@@ -308,9 +351,9 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
   const uint8_t* probs = a.probs ? a.probs + b * a.q_seq : nullptr;
   for (int i = tid; i < n; i += kThreads) {
     int parent = a.parents ? a.parents[b * a.p_seq + i] : i - 1;
-    sm.uniform[i] = a.uniforms[b * a.u_seq + i];
+    vw.uniform[i] = a.uniforms[b * a.u_seq + i];
     if (i == 0) {
-      sm.parent[0] = -1;
+      vw.parent[0] = -1;
       continue;
     }
     const int64_t t = a.wide_tokens ? reinterpret_cast<const int64_t*>(a.tokens)[b * a.t_seq + i]
@@ -320,17 +363,18 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
       if (rank == 0) report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
       parent = -1;
     }
-    sm.parent[i] = parent;
-    sm.token[i] = static_cast<int>(t);
+    vw.parent[i] = parent;
+    vw.token[i] = static_cast<int>(t);
     if (parent >= 0) {
       const uint8_t* row = logits + parent * a.l_node;
-      sm.logit[i] = Elem<DT>::widen(reinterpret_cast<const typename Elem<DT>::T*>(row)[t]);
-      if (probs) sm.prob[i] = one_prob(a, probs + parent * a.q_node, static_cast<int>(t));
+      vw.logit[i] = Elem<DT>::widen(reinterpret_cast<const typename Elem<DT>::T*>(row)[t]);
+      if (probs) vw.prob[i] = one_prob(a, probs + parent * a.q_node, static_cast<int>(t));
     }
   }
   // every CTA of the cluster runs: its shared memory may be written
   b200attn::ptx::cluster_sync();
 
+  const int base = min(static_cast<int64_t>(a.vocab), static_cast<int64_t>(rank * kWarps) * a.share);
   const int begin = min(static_cast<int64_t>(a.vocab),
                         static_cast<int64_t>(rank * kWarps + warp) * a.share);
   const int end = min(static_cast<int64_t>(a.vocab), begin + static_cast<int64_t>(a.share));
@@ -341,17 +385,17 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
 
   auto first_of = [&]() {
     turn ^= 1;
-    return share_out(sm, turn, first_pass<DT, VEC>(a, sm, node.row, node.top, begin, end), rank, ctas);
+    return share_out(sm, turn, first_pass<DT, VEC>(a, sm, vw, node.row, node.top, base, begin, end), rank, ctas);
   };
   auto sum_of = [&]() {
     turn ^= 1;
-    return share_out(sm, turn, Exchange{sum_pass<DT, VEC>(a, sm, node, begin, end), 0.f, 0, 0}, rank,
+    return share_out(sm, turn, Exchange{sum_pass<DT, VEC>(a, sm, vw, node, base, begin, end), 0.f, 0, 0}, rank,
                      ctas).sum;
   };
 
   while (n > 0) {
     // --------------------------------------------------- a node: its sum of weights
-    if (tid == 0 && rank == 0) sm.path[length] = at;
+    if (tid == 0 && rank == 0) vw.path[length] = at;
     ++length;
     node = Node{logits + at * a.l_node, probs ? probs + at * a.q_node : nullptr, 0.0, 1.0, 0.0, 0};
     Exchange all = first_of();
@@ -369,33 +413,33 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
     double left = all.sum;   // in all
     const int likeliest = all.at;
     for (int i0 = at + 1; i0 < n && kept < 0; i0 += 32) {
-      uint32_t mask = __ballot_sync(kAll, i0 + lane < n && sm.parent[i0 + lane] == at);
+      uint32_t mask = __ballot_sync(kAll, i0 + lane < n && vw.parent[i0 + lane] == at);
       while (mask != 0u && kept < 0) {
         const int c = i0 + __ffs(mask) - 1;
         mask &= mask - 1;
         if (a.inv_temp == 0.0) {
-          if (sm.token[c] == likeliest && sm.uniform[c] < 1.f) kept = c;
+          if (vw.token[c] == likeliest && vw.uniform[c] < 1.f) kept = c;
           continue;
         }
-        const double e = weight(a, sm, sm.logit[c], node.top);
-        const double u = static_cast<double>(sm.uniform[c]);
+        const double e = weight(a, sm, vw.logit[c], node.top);
+        const double u = static_cast<double>(vw.uniform[c]);
         if (!probs) {
           bool again = false;
-          for (int j = 0; j < node.refused; ++j) again |= sm.refused[j] == sm.token[c];
+          for (int j = 0; j < node.refused; ++j) again |= vw.refused[j] == vw.token[c];
           if (again) continue;
           if (u * (all.sum - gone) < e) {
             kept = c;
           } else if (all.sum - gone - e > 0.0) {  // something is left without it
             gone += e;
             __syncthreads();
-            if (tid == 0) sm.refused[node.refused] = sm.token[c];
+            if (tid == 0) vw.refused[node.refused] = vw.token[c];
             __syncthreads();
             ++node.refused;
             summed = false;
           }
           continue;
         }
-        const double q = static_cast<double>(sm.prob[c]);
+        const double q = static_cast<double>(vw.prob[c]);
         if (u * q * left < fmax(fma(e, node.scale, -node.t * q), 0.0)) {
           kept = c;
           continue;
@@ -423,11 +467,12 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
       break;
     }
     if (!summed) left = sum_of();
-    if (!(left > 0.0)) {  // only by the rounding of a sum: refusals leave something
-      next = likeliest;
-      break;
+    // (refusals leave something: only the rounding of a sum lets one too many through)
+    while (!(left > 0.0) && node.refused > 0) {
+      --node.refused;
+      left = sum_of();
     }
-    const double goal = static_cast<double>(sm.uniform[0]) * left;
+    const double goal = static_cast<double>(vw.uniform[0]) * left;
     // the CTA, then the warp, then the part of its share that the goal lies in: the first
     // whose end is past it, or else the last with any weight
     double before = 0.0;
@@ -454,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
     const int from = min(static_cast<int64_t>(a.vocab),
                          static_cast<int64_t>(rank * kWarps + owner) * a.share);
     const int to = min(static_cast<int64_t>(a.vocab), from + static_cast<int64_t>(a.share));
-    const double mine = sum_pass<DT, VEC>(a, sm, node, min(to, from + warp * part),
+    const double mine = sum_pass<DT, VEC>(a, sm, vw, node, base, min(to, from + warp * part),
                                           min(to, from + (warp + 1) * part));
     if (lane == 0) sm.part_sum[warp] = mine;
     __syncthreads();
@@ -465,12 +510,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
       for (int v0 = from + which * part; v0 < stop && found < 0; v0 += 128) {
         const int v = v0 + 4 * lane;
         double y[4] = {0.0, 0.0, 0.0, 0.0};
-        if (v < stop) {
-          float l[4], q[4] = {0.f, 0.f, 0.f, 0.f};
-          load4<DT>(node.row, v, stop, VEC, -INFINITY, l);
-          if (node.t != 0.0) probs4(a, node.probs, v, stop, q);
-          weights4(a, sm, node, v, l, q, y);
-        }
+        if (v < stop) weights4<DT, VEC>(a, sm, vw, node, v, base, stop, y);
         double mine4 = (y[0] + y[1]) + (y[2] + y[3]), cum = mine4;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -501,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
   if (rank == 0) {
     __syncthreads();
     for (int i = tid; i < a.nodes; i += kThreads)
-      a.paths[b * a.nodes + i] = i < length ? sm.path[i] : -1;
+      a.paths[b * a.nodes + i] = i < length ? vw.path[i] : -1;
     if (tid == 0) a.counts[b] = length;
   }
   if (teller && tid == 0) a.next[b] = next;
@@ -510,12 +550,28 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
 // -------------------------------------------------------------------- host
 using namespace b200paged;
 
-int32_t launch_cluster(void (*kernel)(Args), const Args& a, unsigned ctas, int64_t batch,
-                       cudaStream_t stream) {
+// Shared memory of a CTA, up to half an SM's.
+constexpr int64_t kMostSmem = 100 * 1024;
+int64_t fixed_bytes(int nodes) { return sizeof(Smem) + 4ll * kNodeArrays * nodes_padded(nodes); }
+int64_t kept_bytes(int64_t share) { return 8 * kWarps * share; }
+
+template <void (*kKernel)(Args)>
+int32_t launch_cluster(const Args& a, unsigned ctas, int64_t batch, int device, cudaStream_t stream) {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  std::call_once(once[device], [&] {
+    err[device] = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+    if (err[device] == cudaSuccess)
+      err[device] = cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
+  if (err[device] != cudaSuccess) {
+    set_error(cudaGetErrorString(err[device]));
+    return B200_ATTN_ERR_LAUNCH;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas, static_cast<unsigned>(batch));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Smem);
+  cfg.dynamicSmemBytes = fixed_bytes(a.nodes) + (a.keep ? kept_bytes(a.share) : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -526,7 +582,7 @@ int32_t launch_cluster(void (*kernel)(Args), const Args& a, unsigned ctas, int64
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kKernel, a);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     set_error(cudaGetErrorString(e));
@@ -535,8 +591,6 @@ int32_t launch_cluster(void (*kernel)(Args), const Args& a, unsigned ctas, int64
   count_launch();
   return B200_ATTN_OK;
 }
-static_assert(sizeof(Smem) <= 48 * 1024, "no opt-in needed");
-
 // Rows of four numbers can be read by one load.
 bool by_fours(const void* base, const int64_t* stride, const int64_t* extent, int64_t eb) {
   if (reinterpret_cast<uintptr_t>(base) % (4 * eb)) return false;
@@ -546,8 +600,9 @@ bool by_fours(const void* base, const int64_t* stride, const int64_t* extent, in
 }
 
 template <int DT>
-int32_t run(const Args& a, bool vec, unsigned ctas, int64_t batch, cudaStream_t s) {
-  return launch_cluster(vec ? verify_kernel<DT, true> : verify_kernel<DT, false>, a, ctas, batch, s);
+int32_t run(const Args& a, bool vec, unsigned ctas, int64_t batch, int device, cudaStream_t s) {
+  return vec ? launch_cluster<verify_kernel<DT, true>>(a, ctas, batch, device, s)
+             : launch_cluster<verify_kernel<DT, false>>(a, ctas, batch, device, s);
 }
 
 }  // namespace
@@ -640,14 +695,16 @@ extern "C" int32_t b200_verify_drafts(const b200_verify_params* p, void* stream)
   a.nodes = static_cast<int32_t>(p->nodes);
   a.vocab = static_cast<int32_t>(p->vocab);
   a.wide_tokens = p->wide_tokens;
-  const unsigned ctas = p->vocab > 16384 ? 8 : (p->vocab > 4096 ? 4 : 1);
+  // so many CTAs that four of them, with a row's exponentials, fit on an SM
+  const unsigned ctas = p->vocab > 53248 ? 16 : (p->vocab > 16384 ? 8 : (p->vocab > 4096 ? 4 : 1));
   const int64_t warps = static_cast<int64_t>(ctas) * kWarps;
   a.share = static_cast<int32_t>((p->vocab + 4 * warps - 1) / (4 * warps) * 4);
+  a.keep = a.inv_temp != 0.0 && fixed_bytes(a.nodes) + kept_bytes(a.share) <= kMostSmem;
   const bool vec = by_fours(p->logits, p->logits_stride, extent, eb);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (p->dtype) {
-    case B200_ATTN_DTYPE_BF16: return run<B200_ATTN_DTYPE_BF16>(a, vec, ctas, p->batch, s);
-    case B200_ATTN_DTYPE_FP16: return run<B200_ATTN_DTYPE_FP16>(a, vec, ctas, p->batch, s);
-    default: return run<B200_ATTN_DTYPE_FP32>(a, vec, ctas, p->batch, s);
+    case B200_ATTN_DTYPE_BF16: return run<B200_ATTN_DTYPE_BF16>(a, vec, ctas, p->batch, scope.device, s);
+    case B200_ATTN_DTYPE_FP16: return run<B200_ATTN_DTYPE_FP16>(a, vec, ctas, p->batch, scope.device, s);
+    default: return run<B200_ATTN_DTYPE_FP32>(a, vec, ctas, p->batch, scope.device, s);
   }
 }

@@ -1,9 +1,9 @@
 // cache4.cu — append to and read from the paged cache held in 4 bits
 // (format: b200_cache4.h).
 //
-// A thread takes 8 numbers of a key row and the same 8 of the value row; the 2 or 4 threads
-// of a group find its smallest and largest number by shuffles.  Bound by HBM for
-// large calls: a vector of D numbers is read once and D / 2 + 16 bytes are written.
+// A thread takes a group of a key or value vector, 16 or 32 numbers, so what is done once a group
+// (its ends, step and low) is shared by many numbers; the four threads of a vector exchange words to
+// write rows 8 or 16 bytes at a time.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -23,6 +23,7 @@ using b200tree::Elem;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kParts = 8;  // threads of a token's key and value of a head
 
 struct Call {
   uint8_t* k;  // pools
@@ -38,33 +39,40 @@ struct Call {
   int64_t vx_layer, vx_seq, vx_head, vx_tok;
   const int32_t* counts;
   int32_t batch, slots, pages, page_size, heads, tokens, head_dim;
+  uint32_t inv_tok, inv_size;  // for divisions by the threads of a token and by the page size
   int32_t* err;
 };
 
-// The thread's vector: sequence, token, head and eighth-of-numbers `x` of it.
+// x / d with inv = 2^32 / d rounded up (0 for d = 1): the product is the quotient or one more.
+__host__ __device__ inline uint32_t inverse_of(uint32_t d) { return 0xffffffffu / d + 1u; }
+__device__ __forceinline__ uint32_t divided(uint32_t x, uint32_t d, uint32_t inv) {
+  if (d == 1u) return x;
+  const uint32_t q = __umulhi(x, inv);
+  return q * d > x ? q - 1u : q;
+}
+
+// The thread's group: token, head, keys or values, group.  blockIdx: threads of a sequence, layers,
+// sequences.  The threads of a vector are lanes 4 n to 4 n + 3 of a warp.
 struct Place {
-  int b, j, h, x;
+  int j, h, g;
+  bool value;
 };
 
-template <int P>
 __device__ __forceinline__ bool place_of(const Call& c, Place* p) {
-  constexpr uint32_t kParts = P / 8;
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const uint32_t idx = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t per_tok = c.heads * kParts;
-  const int64_t per_seq = static_cast<int64_t>(c.tokens) * per_tok;
-  p->b = static_cast<int>(idx / per_seq);
-  const uint32_t rest = static_cast<uint32_t>(idx - p->b * per_seq);
-  p->j = static_cast<int>(rest / per_tok);
-  const uint32_t in = rest - p->j * per_tok;
+  const uint32_t j = divided(idx, per_tok, c.inv_tok), in = idx - j * per_tok;
+  p->j = static_cast<int>(j);
   p->h = static_cast<int>(in / kParts);
-  p->x = static_cast<int>(in % kParts);
-  return p->b < c.batch;
+  p->value = in % kParts >= 4;
+  p->g = static_cast<int>(in % 4);
+  return j < static_cast<uint32_t>(c.tokens);
 }
 
 // The page and row of token lens[b] + j; false where there is none (reported).
 __device__ __forceinline__ bool find_row(const Call& c, int b, int j, int* page, uint32_t* row) {
   const int len = c.lens[b];
-  const uint32_t at = static_cast<uint32_t>(len) + j, slot = at / static_cast<uint32_t>(c.page_size);
+  const uint32_t at = static_cast<uint32_t>(len) + j, slot = divided(at, c.page_size, c.inv_size);
   int p = -1;
   if (len >= 0 && slot < static_cast<uint32_t>(c.slots)) p = c.table[b * c.table_stride + slot];
   if (p < 0 || p >= c.pages) {
@@ -77,7 +85,7 @@ __device__ __forceinline__ bool find_row(const Call& c, int b, int j, int* page,
 }
 
 template <int DT>
-__device__ __forceinline__ void load8(const uint8_t* src, float (&x)[8]) {
+__device__ __forceinline__ void load8(const uint8_t* src, float* x) {
   using E = Elem<DT>;
   union {
     uint4 w[E::kBytes / 2];
@@ -110,94 +118,196 @@ __device__ __forceinline__ float step_of(float2 span) {
   };
   if (span.x == 0.f) return 0.f;
   if (!(span.x < INFINITY)) return INFINITY;
-  uint32_t u = __float_as_uint(span.x / 15.f) & 0xffff0000u;
+  uint32_t u = __float_as_uint(span.x * (1.f / 15.f)) & 0xffff0000u;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (!enough(u)) u += 0x10000u;
   return __uint_as_float(u);
 }
 
-struct Coded {
-  uint32_t code[8];
-  float step, low;
-};
+// The nearest whole number to (x - low) / step, ties to even, where `code` is it but for a rounding
+// of the quotient: x - low = d.x + d.y, and what is left of d.x after `code` steps is exact.
+__device__ __forceinline__ float settled(float x, float step, float low, float code) {
+  const float2 d = difference(x, low);
+  const float left = 2.f * fmaf(-code, step, d.x);
+  const bool odd = static_cast<int>(code) & 1;
+  const bool tie_up = d.y > 0.f || (d.y == 0.f && odd), tie_down = d.y < 0.f || (d.y == 0.f && odd);
+  if (left > step || (left == step && tie_up)) code += 1.f;
+  else if (left < -step || (left == -step && tie_down)) code -= 1.f;
+  return fmaxf(0.f, fminf(15.f, code));
+}
 
-// The codes of the thread's 8 numbers and its group's step and low.  `there`: the numbers
-// lie inside the vector.  By whole warps.
-template <int P>
-__device__ __forceinline__ Coded encode(const float (&x)[8], bool there) {
-  constexpr int kLanes = P / 32;  // of a group
-  Coded r;
-  float lo = INFINITY, hi = -INFINITY;
-  if (there) {
-    float odd = 0.f;  // NaN where a number is not finite
+// Codes in place of the group's first n numbers (a multiple of 8; 0 for the others), its step and its
+// low.
+template <int G>
+__device__ __forceinline__ float2 encode(float (&x)[G], int n) {
+  float lo = INFINITY, hi = -INFINITY, odd = 0.f;  // NaN where a number is not finite
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < G; ++i) {
+    if (i < n) {
       lo = fminf(lo, x[i]);
       hi = fmaxf(hi, x[i]);
       odd = fmaf(x[i], 0.f, odd);
     }
-    if (odd != 0.f) lo = -INFINITY;
   }
+  if (odd != 0.f) lo = -INFINITY;
+  if (n <= 0) lo = hi = 0.f;
+  float low = bf16_down(lo), step = step_of(difference(hi, low));
+  if (step > 0.f && step < 0x1p-100f) step = 0x1p-100f;
+  if (!(isfinite(low) && isfinite(step))) {
+    step = low = __uint_as_float(0x7fc00000u);
+    n = 0;
+  }
+  if (!(step > 0.f)) n = 0;
+  constexpr float kRound = 12582912.f;  // 1.5 2^23
+  const float inv = __frcp_rn(step);
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  for (int i = 0; i < G; ++i) {
+    const float f = (x[i] - low) * inv;
+    float code = (f + kRound) - kRound;
+    // next to a border the quotient's rounding could decide
+    if (i < n && fabsf(f - code) > 0.5f - 0x1p-14f) code = settled(x[i], step, low, code);
+    x[i] = i < n ? code : 0.f;
   }
-  if (lo == INFINITY) lo = hi = 0.f;  // a group past the vector
-  r.low = bf16_down(lo);
-  r.step = step_of(difference(hi, r.low));
-  if (r.step > 0.f && r.step < 0x1p-100f) r.step = 0x1p-100f;
-  const bool fine = isfinite(r.low) && isfinite(r.step);
-  const float inv = fine && r.step > 0.f ? 1.f / r.step : 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // x - low = d.x + d.y; what is left of d.x after t steps is exact, so the code is the
-    // nearest one, with ties to even
-    const float2 d = there && fine ? difference(x[i], r.low) : make_float2(0.f, 0.f);
-    int t = __float2int_rn(d.x * inv);
-    const float left = 2.f * fmaf(-static_cast<float>(t), r.step, d.x);
-    const bool tie_up = d.y > 0.f || (d.y == 0.f && (t & 1));
-    const bool tie_down = d.y < 0.f || (d.y == 0.f && (t & 1));
-    if (left > r.step || (left == r.step && tie_up)) ++t;
-    else if (left < -r.step || (left == -r.step && tie_down)) --t;
-    r.code[i] = static_cast<uint32_t>(max(0, min(15, t)));
-  }
-  if (!fine) r.step = r.low = __uint_as_float(0x7fc00000u);
-  return r;
+  return make_float2(step, low);
 }
 
-// Part x (8 numbers) of a row of codes, as keys or values lie: see the header.
+// a + 16 b + 256 c + 4096 d of codes, as a whole number.
+__device__ __forceinline__ uint32_t four(float a, float b, float c, float d) {
+  const float v = fmaf(fmaf(fmaf(d, 16.f, c), 16.f, b), 16.f, a);
+  return __float_as_uint(v + 8388608.f) & 0xffffu;
+}
+__device__ __forceinline__ uint32_t two(float a, float b) {
+  return __float_as_uint(fmaf(b, 16.f, a) + 8388608.f) & 0xffu;
+}
+
+// The 4 x 4 words of four lanes, transposed: word i of lane k becomes word k of lane i.  By whole
+// warps.
+__device__ __forceinline__ void transpose(uint32_t (&w)[4]) {
+  const bool one = threadIdx.x & 1, two = threadIdx.x & 2;
+  uint32_t a = __shfl_xor_sync(0xffffffffu, one ? w[0] : w[1], 1);
+  uint32_t b = __shfl_xor_sync(0xffffffffu, one ? w[2] : w[3], 1);
+  if (one) w[0] = a, w[2] = b;
+  else w[1] = a, w[3] = b;
+  a = __shfl_xor_sync(0xffffffffu, two ? w[0] : w[2], 2);
+  b = __shfl_xor_sync(0xffffffffu, two ? w[1] : w[3], 2);
+  if (two) w[0] = a, w[1] = b;
+  else w[2] = a, w[3] = b;
+}
+
+// The codes of group g of a row, as keys or values lie (see the header): lane g of the row's four
+// writes quarter g of the row's codes.  By whole warps; `mine`: there is a row.
 template <int P>
-__device__ __forceinline__ void put_key_codes(uint8_t* row, int x, const uint32_t (&c)[8]) {
+__device__ __forceinline__ void put_codes(uint8_t* row, int g, bool value, const float (&c)[P / 4],
+                                          bool mine) {
+  uint32_t w[4];
   if constexpr (P == 128) {
-    uint32_t w = 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= c[i] << (4 * (2 * (i / 4) + i % 4 / 2 + 4 * (i % 2)));
-    *reinterpret_cast<uint32_t*>(row + 16 * (x % 4) + 4 * (x / 4)) = w;
+    for (int i = 0; i < 4; ++i) {
+      const float* x = c + 8 * i;
+      w[i] = value ? four(x[0], x[1], x[2], x[3]) | four(x[4], x[5], x[6], x[7]) << 16
+                   : four(x[0], x[2], x[4], x[6]) | four(x[1], x[3], x[5], x[7]) << 16;
+    }
   } else {
-    const int g = x / 2;
 #pragma unroll
-    for (int y = 0; y < 8; y += 4) {
-      uint8_t* at = row + 8 * (2 * (x % 2) + y / 4) + 4 * (g / 2) + g % 2;
-      at[0] = static_cast<uint8_t>(c[y] | c[y + 2] << 4);
-      at[2] = static_cast<uint8_t>(c[y + 1] | c[y + 3] << 4);
+    for (int i = 0; i < 4; ++i) {
+      const float* x = c + 4 * i;
+      w[i] = value ? two(x[0], x[1]) | two(x[2], x[3]) << 8
+                   : (two(x[0], x[2]) | two(x[1], x[3]) << 16) << (8 * (g % 2));
     }
   }
-}
-template <int P>
-__device__ __forceinline__ void put_value_codes(uint8_t* row, int x, const uint32_t (&c)[8]) {
+  transpose(w);
+  if (!mine) return;
   if constexpr (P == 128) {
-#pragma unroll
-    for (int y = 0; y < 8; y += 4)
-      *reinterpret_cast<uint16_t*>(row + 8 * (2 * (x % 4) + y / 4) + 2 * (x / 4)) =
-          static_cast<uint16_t>(c[y] | c[y + 1] << 4 | c[y + 2] << 8 | c[y + 3] << 12);
+    uint4 o = make_uint4(w[0], w[1], w[2], w[3]);
+    if (value)
+      o = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410),
+                     __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+    reinterpret_cast<uint4*>(row)[g] = o;
   } else {
-#pragma unroll
-    for (int y = 0; y < 8; y += 2)
-      row[4 * (4 * (x % 2) + y / 2) + x / 2] = static_cast<uint8_t>(c[y] | c[y + 1] << 4);
+    uint2 o = make_uint2(w[0] | w[1], w[2] | w[3]);
+    if (value) {
+      const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
+      o = make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+    }
+    reinterpret_cast<uint2*>(row)[g] = o;
   }
 }
+
+__device__ __forceinline__ uint16_t bf16_bits(float x) {
+  return static_cast<uint16_t>(__float_as_uint(x) >> 16);
+}
+__device__ __forceinline__ float of_bf16(uint16_t x) {
+  return __uint_as_float(static_cast<uint32_t>(x) << 16);
+}
+
+// Rows in and out of a thread's pool and vectors.
+struct Sides {
+  uint8_t* row;  // of the pool
+  uint8_t* x;    // the group's first number in the vector
+};
+template <int P, int DT>
+__device__ __forceinline__ Sides sides_of(const Call& c, const Place& p, int page, uint32_t row) {
+  const int64_t b = blockIdx.z, l = blockIdx.y;
+  const int at = P / 4 * Elem<DT>::kBytes * p.g;
+  return p.value ? Sides{c.v + l * c.v_layer + page * c.v_page + p.h * c.v_head + row * c.v_row,
+                         c.vx + l * c.vx_layer + b * c.vx_seq + p.h * c.vx_head + p.j * c.vx_tok + at}
+                 : Sides{c.k + l * c.k_layer + page * c.k_page + p.h * c.k_head + row * c.k_row,
+                         c.kx + l * c.kx_layer + b * c.kx_seq + p.h * c.kx_head + p.j * c.kx_tok + at};
+}
+
+template <int P, int DT>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ Call c) {
+  constexpr int G = P / 4;
+  b200attn::ptx::launch_dependents();
+  b200attn::ptx::grid_dependency_wait();
+  Place p;
+  bool mine = place_of(c, &p);
+  int page = 0;
+  uint32_t row = 0;
+  if (mine) {
+    const int count = c.counts ? c.counts[blockIdx.z] : c.tokens;
+    if (count < 0 || count > c.tokens) {
+      report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
+      mine = false;
+    }
+    mine = mine && p.j < count && find_row(c, blockIdx.z, p.j, &page, &row);
+  }
+  if (!__any_sync(0xffffffffu, mine)) return;
+  const Sides to = sides_of<P, DT>(c, p, page, row);
+  const int n = mine ? min(G, c.head_dim - G * p.g) : 0;
+  float x[G];
+#pragma unroll
+  for (int i = 0; i < G; i += 8) {
+    if (i < n) {
+      load8<DT>(to.x + i * Elem<DT>::kBytes, x + i);
+    } else {
+#pragma unroll
+      for (int y = 0; y < 8; ++y) x[i + y] = 0.f;
+    }
+  }
+  const float2 meta = encode(x, n);
+  put_codes<P>(to.row, p.g, p.value, x, mine);
+  if (!mine) return;
+  uint16_t* m = reinterpret_cast<uint16_t*>(to.row + P / 2) + p.g;
+  m[0] = bf16_bits(meta.x);
+  m[4] = bf16_bits(meta.y);
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(uint8_t* dst, const float* x) {
+  using E = Elem<DT>;
+  union {
+    uint4 w[E::kBytes / 2];
+    typename E::T e[8];
+  } u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u.e[i] = E::round(x[i]);
+#pragma unroll
+  for (int i = 0; i < E::kBytes / 2; ++i) reinterpret_cast<uint4*>(dst)[i] = u.w[i];
+}
+
+// Part x (8 numbers) of a row's codes.
 template <int P>
 __device__ __forceinline__ void get_key_codes(const uint8_t* row, int x, uint32_t (&c)[8]) {
   if constexpr (P == 128) {
@@ -236,101 +346,45 @@ __device__ __forceinline__ void get_value_codes(const uint8_t* row, int x, uint3
   }
 }
 
-__device__ __forceinline__ uint16_t bf16_bits(float x) {
-  return static_cast<uint16_t>(__float_as_uint(x) >> 16);
-}
-__device__ __forceinline__ float of_bf16(uint16_t x) {
-  return __uint_as_float(static_cast<uint32_t>(x) << 16);
-}
-
-template <int P, int DT>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ Call c) {
-  b200attn::ptx::launch_dependents();
-  b200attn::ptx::grid_dependency_wait();
-  Place p;
-  bool mine = place_of<P>(c, &p);
-  int page = 0;
-  uint32_t row = 0;
-  if (mine) {
-    const int count = c.counts ? c.counts[p.b] : c.tokens;
-    if (count < 0 || count > c.tokens) {
-      report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
-      mine = false;
-    }
-    mine = mine && p.j < count && find_row(c, p.b, p.j, &page, &row);
-  }
-  const bool there = mine && 8 * p.x < c.head_dim;
-  const int64_t l = blockIdx.y;
-  float k[8], v[8];
-  if (there) {
-    const int at = 8 * Elem<DT>::kBytes * p.x;
-    load8<DT>(c.kx + l * c.kx_layer + p.b * c.kx_seq + p.h * c.kx_head + p.j * c.kx_tok + at, k);
-    load8<DT>(c.vx + l * c.vx_layer + p.b * c.vx_seq + p.h * c.vx_head + p.j * c.vx_tok + at, v);
-  }
-  const Coded kc = encode<P>(k, there), vc = encode<P>(v, there);
-  if (!mine) return;
-  uint8_t* kr = c.k + l * c.k_layer + page * c.k_page + p.h * c.k_head + row * c.k_row;
-  uint8_t* vr = c.v + l * c.v_layer + page * c.v_page + p.h * c.v_head + row * c.v_row;
-  put_key_codes<P>(kr, p.x, kc.code);
-  put_value_codes<P>(vr, p.x, vc.code);
-  if (p.x % (P / 32) == 0) {
-    const int g = p.x / (P / 32);
-    uint16_t* km = reinterpret_cast<uint16_t*>(kr + P / 2) + g;
-    uint16_t* vm = reinterpret_cast<uint16_t*>(vr + P / 2) + g;
-    km[0] = bf16_bits(kc.step);
-    km[4] = bf16_bits(kc.low);
-    vm[0] = bf16_bits(vc.step);
-    vm[4] = bf16_bits(vc.low);
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ void store8(uint8_t* dst, const float (&x)[8]) {
-  using E = Elem<DT>;
-  union {
-    uint4 w[E::kBytes / 2];
-    typename E::T e[8];
-  } u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) u.e[i] = E::round(x[i]);
-#pragma unroll
-  for (int i = 0; i < E::kBytes / 2; ++i) reinterpret_cast<uint4*>(dst)[i] = u.w[i];
-}
-
+// A thread gives 8 numbers of a key and the same 8 of the value, so that neighbours write side by
+// side (a group a thread as above: 46 us against 34 us for 33 thousand tokens of 8 heads).
 template <int P, int DT>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ Call c) {
   b200attn::ptx::launch_dependents();
   b200attn::ptx::grid_dependency_wait();
-  Place p;
-  if (!place_of<P>(c, &p) || 8 * p.x >= c.head_dim) return;
-  const int count = c.counts ? c.counts[p.b] : c.tokens;
+  const uint32_t idx = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t per_tok = c.heads * (P / 8);
+  const uint32_t tok = divided(idx, per_tok, c.inv_tok), in = idx - tok * per_tok;
+  const int j = static_cast<int>(tok), h = static_cast<int>(in / (P / 8)), x = static_cast<int>(in % (P / 8));
+  if (j >= c.tokens || 8 * x >= c.head_dim) return;
+  const int64_t b = blockIdx.z, l = blockIdx.y;
+  const int count = c.counts ? c.counts[b] : c.tokens;
   if (count < 0 || count > c.tokens) report_error(c.err, B200_ATTN_DEVERR_BOUNDS);
-  const int64_t l = blockIdx.y;
   float k[8], v[8];
   int page;
   uint32_t row;
-  if (count <= c.tokens && p.j < count && find_row(c, p.b, p.j, &page, &row)) {
-    const uint8_t* kr = c.k + l * c.k_layer + page * c.k_page + p.h * c.k_head + row * c.k_row;
-    const uint8_t* vr = c.v + l * c.v_layer + page * c.v_page + p.h * c.v_head + row * c.v_row;
-    const int g = p.x / (P / 32);
+  if (count <= c.tokens && j < count && find_row(c, b, j, &page, &row)) {
+    const uint8_t* kr = c.k + l * c.k_layer + page * c.k_page + h * c.k_head + row * c.k_row;
+    const uint8_t* vr = c.v + l * c.v_layer + page * c.v_page + h * c.v_head + row * c.v_row;
+    const int g = x / (P / 32);
     const uint16_t* km = reinterpret_cast<const uint16_t*>(kr + P / 2) + g;
     const uint16_t* vm = reinterpret_cast<const uint16_t*>(vr + P / 2) + g;
     uint32_t kc[8], vc[8];
-    get_key_codes<P>(kr, p.x, kc);
-    get_value_codes<P>(vr, p.x, vc);
+    get_key_codes<P>(kr, x, kc);
+    get_value_codes<P>(vr, x, vc);
     const float ks = of_bf16(km[0]), kl = of_bf16(km[4]), vs = of_bf16(vm[0]), vl = of_bf16(vm[4]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      k[i] = fmaf(ks, static_cast<float>(kc[i]), kl);
-      v[i] = fmaf(vs, static_cast<float>(vc[i]), vl);
+    for (int i = 0; i < 8; ++i) {  // (a code under the exponent of 2^23 is that number and the code)
+      k[i] = fmaf(ks, __uint_as_float(kc[i] | 0x4b000000u) - 8388608.f, kl);
+      v[i] = fmaf(vs, __uint_as_float(vc[i] | 0x4b000000u) - 8388608.f, vl);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
   }
-  const int at = 8 * Elem<DT>::kBytes * p.x;
-  store8<DT>(c.kx + l * c.kx_layer + p.b * c.kx_seq + p.h * c.kx_head + p.j * c.kx_tok + at, k);
-  store8<DT>(c.vx + l * c.vx_layer + p.b * c.vx_seq + p.h * c.vx_head + p.j * c.vx_tok + at, v);
+  const int at = 8 * Elem<DT>::kBytes * x;
+  store8<DT>(c.kx + l * c.kx_layer + b * c.kx_seq + h * c.kx_head + j * c.kx_tok + at, k);
+  store8<DT>(c.vx + l * c.vx_layer + b * c.vx_seq + h * c.vx_head + j * c.vx_tok + at, v);
 }
 
 // -------------------------------------------------------------------- host
@@ -339,6 +393,7 @@ using b200attn::may_overlap;
 using b200attn::stretches_of;
 
 // Checks both entry points' arguments and fills the call; `out`: the vectors are written.
+// threads: of a sequence.
 int32_t fill(const b200_cache* c, int64_t head_dim, int32_t dtype, const b200_cache_rows* rows,
              bool out, Call* a, int64_t* threads) {
   const int32_t rc = b200_cache_check(c);
@@ -354,11 +409,12 @@ int32_t fill(const b200_cache* c, int64_t head_dim, int32_t dtype, const b200_ca
       !vectors_aligned(rows->v, rows->v_stride, extent, 4, eb) ||
       (reinterpret_cast<uintptr_t>(rows->counts) & 3u))
     return B200_ATTN_ERR_ALIGNMENT;
-  const int64_t parts = (head_dim <= 64 ? 64 : 128) / 8;
-  if (rows->tokens > 0x3fffffff || rows->tokens * c->kv_heads * parts > 0x7fffffffll ||
-      c->batch * rows->tokens * c->kv_heads * parts > (1ll << 38))
+  const int64_t parts = out && head_dim > 64 ? 16 : kParts;  // threads of a token's heads, each
+  if (rows->tokens > 0x3fffffff || rows->tokens * c->kv_heads * parts > 0x7fffffffll - kThreads)
     return B200_ATTN_ERR_INVALID_ARGUMENT;
-  *threads = c->batch * rows->tokens * c->kv_heads * parts;
+  *threads = rows->tokens * c->kv_heads * parts;
+  a->inv_tok = inverse_of(static_cast<uint32_t>(c->kv_heads * parts));
+  a->inv_size = inverse_of(static_cast<uint32_t>(c->page_size));
   // what is written shares no byte with what is read, nor with itself
   const int64_t pool[4] = {c->layers, c->pages, c->kv_heads, c->page_size};
   const auto kp = stretches_of(c->k, c->k_stride, pool, 4, c->head_dim, 2);
@@ -426,10 +482,10 @@ int32_t run_call(const b200_cache* c, int64_t head_dim, int32_t dtype, const b20
   DeviceScope scope;
   if ((rc = scope.enter(c->k, "the pools are not device memory")) != B200_ATTN_OK) return rc;
   if ((rc = resolve_error_word(c->error_word, &a.err)) != B200_ATTN_OK) return rc;
-  const dim3 grid(static_cast<unsigned>((threads + kThreads - 1) / kThreads),
-                  static_cast<unsigned>(c->layers));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = head_dim > 64;
+  const dim3 grid(static_cast<unsigned>((threads + kThreads - 1) / kThreads),
+                  static_cast<unsigned>(c->layers), static_cast<unsigned>(c->batch));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case B200_ATTN_DTYPE_BF16:
       return wide ? run<128, B200_ATTN_DTYPE_BF16>(out, a, grid, s)

@@ -30,9 +30,9 @@ CHECKED_LIB_PATH = PACKAGE_DIR / "libb200_attention_checked.so"
 
 SOURCES = ("attn_fwd_sm100.cu", "linear_sm100.cu", "layernorm.cu", "softmax.cu",
            "paged_cache.cu", "tree_attn.cu", "tree_attn_sm100.cu", "cache4.cu", "tree_attn4.cu",
-           "verify.cu")
+           "tree_attn4_sm100.cu", "verify.cu")
 HEADERS = ("sm100_ptx.cuh", "error_word.cuh", "byte_range.h", "paged_host.h", "tree_attn.cuh",
-           "tree_attn_host.cuh", "tree_attn_rows.cuh")
+           "tree_attn_host.cuh", "tree_attn_rows.cuh", "tree_attn_tiles.cuh", "tree_attn4.cuh")
 
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -324,15 +324,6 @@ int64_t desc_bytes(const b200_tree_attn_params* p, const Choice& c) {
 }
 
 
-template <int RM, int DP, int DT>
-int32_t run_join_columns(const Args& a, int64_t units, cudaStream_t s) {
-  // few units: the blocks that share a unit's rows share its columns too
-  const bool spread = units * (RM / 32) < 300;
-  return launch(spread ? join_columns_kernel<RM, DP, DT, true> : join_columns_kernel<RM, DP, DT, false>,
-                dim3(static_cast<unsigned>(units), RM / 32, spread ? DP / kJoinCols : 1),
-                dim3(32 * kJoinWarps), 0, s, a);
-}
-
 // One kernel over the runs, and where it does not join the units that were cut, one that
 // does.
 template <int DP, int DT>

@@ -28,6 +28,7 @@
 #include "error_word.cuh"
 #include "paged_host.h"
 #include "tree_attn.cuh"
+#include "tree_attn4.cuh"
 #include "tree_attn_host.cuh"
 #include "tree_attn_rows.cuh"
 
@@ -107,14 +108,6 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// `bytes` (a multiple of 16) of global memory to shared memory; counted by barrier `bar`.
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const uint8_t* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
 // Waits for a block's copies, a second at most; false (reported) when they did not come.  By
 // whole warps.
 __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int32_t* err) {
@@ -129,33 +122,6 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int32_t* e
 }
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-
-// Adds NaN to the numbers of a finished row (`out`) or its partial sums (`part`) whose group
-// is NaN in a drafted token that the row's token sees: such steps and lows were left
-// out of the products, where a weight of zero would not hide them.
-template <int DP, int DT>
-__device__ __noinline__ void add_odd4(const Args& a, int b, int h, Seq s, int tok, int d0, int d1,
-                                      int col0, int col1, uint16_t* out, float* part) {
-  using E = Elem<DT>;
-  const uint32_t size = static_cast<uint32_t>(a.page_size);
-  for (int d = max(0, d0); d < min(s.drafts, d1); ++d) {
-    if (!sees(a, b, tok, d)) continue;
-    const uint32_t key = s.len + d, slot = key / size;
-    const int pg = a.table[b * a.table_stride + slot];
-    if (pg < 0 || pg >= a.pages) continue;
-    const uint16_t* meta = reinterpret_cast<const uint16_t*>(
-        a.v + pg * a.v_page + h * a.v_head + static_cast<int64_t>(key - slot * size) * a.v_row +
-        DP / 2);
-    for (int c = col0; c < col1; ++c) {
-      const int g = c / (DP / 4);
-      const float x = __uint_as_float(static_cast<uint32_t>(meta[g]) << 16) +
-                      __uint_as_float(static_cast<uint32_t>(meta[4 + g]) << 16);
-      if (isfinite(x)) continue;
-      if (out) reinterpret_cast<typename E::T*>(out)[c] = E::round(x - x);
-      else part[c] += x - x;
-    }
-  }
-}
 
 template <class S, int DT>
 __global__ void __launch_bounds__(S::kThreads, S::kCtas)
@@ -732,7 +698,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       for (int c0 = c; c0 < DP; c0 += kC)
         add_odd4<DP, DT>(a, done.b, done.h, done.s, tok, t0 * S::kTile - done.s.len,
                          (t0 + n) * S::kTile - done.s.len, c0, min(a.head_dim, c0 + kEach),
-                         finish ? reinterpret_cast<uint16_t*>(out) : nullptr, part + r * DP);
+                         finish ? reinterpret_cast<uint16_t*>(out) : nullptr, part + r * DP, 1);
     if (!finish && c == 0) {
       part[RM * DP + r] = top;
       part[RM * DP + RM + r] = total;
@@ -762,32 +728,60 @@ using AnyShape = Shape4<false, 128>;  // row and key tiles do not depend on the 
 static_assert(AnyShape::kTile == Shape4<true, 64>::kTile && AnyShape::RM == Shape4<true, 64>::RM,
               "one division of the work");
 
+// Up to so many rows a key head the kernel of matrix instructions of a warp.
+constexpr int64_t kFewRows4 = 16;
+
 int64_t rows_of(const b200_tree_attn_params* p) { return p->tokens * (p->heads / p->cache.kv_heads); }
 
-int64_t row_tiles(const b200_tree_attn_params* p) {
-  return (rows_of(p) + AnyShape::RM - 1) / AnyShape::RM;
-}
+// The kernel a call takes: its row tile (`rm` places, `rows` of them used), its key tile and the
+// CTAs of an SM.
+struct Choice4 {
+  bool many;  // the tcgen05 kernel
+  int rm, rows, tn, ctas;
+};
 
-int64_t units_of(const b200_tree_attn_params* p) {
-  return p->cache.batch * p->cache.kv_heads * row_tiles(p);
-}
-
-int64_t runs_of(const b200_tree_attn_params* p, int64_t sms) {
+Choice4 choose(const b200_tree_attn_params* p, int32_t dtype) {
+  const int64_t rows = rows_of(p), group = p->heads / p->cache.kv_heads;
+  // The tcgen05 kernel has bf16 values and weights, and masks of up to 64 tokens.
+  if (rows > kFewRows4 && dtype == B200_ATTN_DTYPE_BF16 && group <= 128 && (p->tokens <= 64 || !p->mask)) {
+    const int tile = static_cast<int>(128 / group * group);  // whole tokens to 128 places
+    if (rows <= tile) return Choice4{true, 128, tile, 128, 1};
+    return Choice4{true, 256, 2 * tile, 128, 1};
+  }
   const bool narrow = p->cache.head_dim == 24;  // rows of 48 bytes
+  return Choice4{false, AnyShape::RM, AnyShape::RM, AnyShape::kTile,
+                 rows > 8 ? AnyShape::kCtas : narrow ? Shape4<true, 64>::kCtas : Shape4<true, 128>::kCtas};
+}
+
+int64_t row_tiles(const b200_tree_attn_params* p, const Choice4& c) {
+  return (rows_of(p) + c.rows - 1) / c.rows;
+}
+
+int64_t units_of(const b200_tree_attn_params* p, const Choice4& c) {
+  return p->cache.batch * p->cache.kv_heads * row_tiles(p, c);
+}
+
+int64_t runs_of(const b200_tree_attn_params* p, const Choice4& c, int64_t sms) {
   const int64_t keys = p->cache.slots * p->cache.page_size;
-  const double tiles = static_cast<double>(units_of(p)) *
-                       static_cast<double>((keys + AnyShape::kTile - 1) / AnyShape::kTile);
-  const int64_t most = (sms < kMaxSms ? sms : kMaxSms) *
-                       (rows_of(p) > 8 ? AnyShape::kCtas
-                        : narrow      ? Shape4<true, 64>::kCtas
-                                      : Shape4<true, 128>::kCtas);
+  const double tiles =
+      static_cast<double>(units_of(p, c)) * static_cast<double>((keys + c.tn - 1) / c.tn);
+  const int64_t most = (sms < kMaxSms ? sms : kMaxSms) * c.ctas;
   return tiles < static_cast<double>(most) ? static_cast<int64_t>(tiles) : most;
 }
 
 template <int DP, int DT>
-int32_t run_width(const Args& a, int runs, int64_t units, bool spread, int device, cudaStream_t s) {
+int32_t run_width(const Choice4& c, const Args& a, int runs, int64_t units, bool spread, int device,
+                  cudaStream_t s) {
   using Few = Shape4<true, DP>;
   using One = Shape4<false, DP>;
+  if constexpr (DT == B200_ATTN_DTYPE_BF16) {
+    if (c.many) {
+      const int32_t rc = launch_coded(c.rm, DP, a, runs, device, s);
+      if (rc != B200_ATTN_OK) return rc;
+      return c.rm == 128 ? run_join_columns<128, DP, DT>(a, units, s)
+                         : run_join_columns<256, DP, DT>(a, units, s);
+    }
+  }
   const int32_t rc =
       a.tokens * a.group <= 8
           ? run_one<rows4_kernel<Few, DT>>(Few::kThreads, Few::kSmemBytes, a, runs, device, s)
@@ -825,8 +819,9 @@ extern "C" int32_t b200_cache4_attn_check(const b200_tree_attn_params* p, int64_
       ((reinterpret_cast<uintptr_t>(p->draft_lens) | reinterpret_cast<uintptr_t>(p->counters)) & 3u))
     return B200_ATTN_ERR_ALIGNMENT;
   // so are all key tiles of a call
-  if (static_cast<double>(units_of(p)) *
-          static_cast<double>(c.slots * c.page_size / AnyShape::kTile + 4) > 2e9)
+  const Choice4 ch = choose(p, dtype);
+  if (static_cast<double>(units_of(p, ch)) *
+          static_cast<double>(c.slots * c.page_size / ch.tn + 5) > 2e9)
     return B200_ATTN_ERR_INVALID_ARGUMENT;
   if (p->mask && (p->mask_stride[0] < 0 || p->mask_stride[1] < 0 || p->mask_stride[2] < 0))
     return B200_ATTN_ERR_INVALID_ARGUMENT;
@@ -838,7 +833,8 @@ extern "C" int64_t b200_cache4_attn_workspace_bytes(const b200_tree_attn_params*
                                                     int64_t head_dim, int32_t dtype) {
   if (b200_cache4_attn_check(p, head_dim, dtype) != B200_ATTN_OK) return 0;
   const int dp = head_dim <= 64 ? 64 : 128;
-  return round16(8 * units_of(p)) + 2 * runs_of(p, kMaxSms) * 4 * AnyShape::RM * (dp + 2);
+  const Choice4 ch = choose(p, dtype);
+  return round16(8 * units_of(p, ch)) + 2 * runs_of(p, ch, kMaxSms) * 4 * ch.rm * (dp + 2);
 }
 
 extern "C" int32_t b200_cache4_attn_fwd(const b200_tree_attn_params* p, int64_t head_dim,
@@ -853,23 +849,24 @@ extern "C" int32_t b200_cache4_attn_fwd(const b200_tree_attn_params* p, int64_t 
   Args a{};
   if ((rc = b200attn::resolve_error_word(p->cache.error_word, &a.err)) != B200_ATTN_OK) return rc;
   fill_args(p, 2, 2, head_dim, &a);
-  a.unit_rows = AnyShape::RM;
-  a.row_tiles = static_cast<int32_t>(row_tiles(p));
+  const Choice4 ch = choose(p, dtype);
+  a.unit_rows = ch.rows;
+  a.row_tiles = static_cast<int32_t>(row_tiles(p, ch));
   a.scale_log2 = p->scale * 1.4426950408889634f;
-  const int64_t units = units_of(p);
+  const int64_t units = units_of(p, ch);
   a.desc = static_cast<int2*>(p->workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + round16(8 * units));
-  const int runs = static_cast<int>(runs_of(p, b200paged::sm_count(scope.device)));
+  const int runs = static_cast<int>(runs_of(p, ch, b200paged::sm_count(scope.device)));
   a.runs = runs;
   // as for caches of 16 bits: long contexts of several rows are joined by a kernel of their own
-  const bool spread = rows_of(p) > 4 && p->cache.slots * p->cache.page_size >= 12 * AnyShape::kTile &&
+  const bool spread = rows_of(p) > 4 && p->cache.slots * p->cache.page_size >= 12 * ch.tn &&
                       runs >= 8 * units;
-  if (!spread && units <= B200_TREE_ATTN_COUNTERS) a.counters = p->counters;
+  if (!ch.many && !spread && units <= B200_TREE_ATTN_COUNTERS) a.counters = p->counters;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = head_dim > 64;
   if (dtype == B200_ATTN_DTYPE_BF16)
-    return wide ? run_width<128, B200_ATTN_DTYPE_BF16>(a, runs, units, spread, scope.device, s)
-                : run_width<64, B200_ATTN_DTYPE_BF16>(a, runs, units, spread, scope.device, s);
-  return wide ? run_width<128, B200_ATTN_DTYPE_FP16>(a, runs, units, spread, scope.device, s)
-              : run_width<64, B200_ATTN_DTYPE_FP16>(a, runs, units, spread, scope.device, s);
+    return wide ? run_width<128, B200_ATTN_DTYPE_BF16>(ch, a, runs, units, spread, scope.device, s)
+                : run_width<64, B200_ATTN_DTYPE_BF16>(ch, a, runs, units, spread, scope.device, s);
+  return wide ? run_width<128, B200_ATTN_DTYPE_FP16>(ch, a, runs, units, spread, scope.device, s)
+              : run_width<64, B200_ATTN_DTYPE_FP16>(ch, a, runs, units, spread, scope.device, s);
 }

@@ -1,0 +1,905 @@
+// tree_attn4_sm100.cu — drafted-token attention of many rows over a paged cache held in 4
+// bits, on the fifth-generation tensor cores: wide trees, and pieces of prompts.
+//
+// The kernel of 16-bit caches (tree_attn_sm100.cu has the roles, the tensor memory and the
+// order of the loads) with another producer: one warp copies coded rows to shared memory
+// in bulk, and four warps, a thread a row, turn them into the operands of the products
+// in the swizzled layout that the tensor cores read.  A row of the matrix instruction
+// kernel (tree_attn4.cu) would be decoded again for every 16 rows of queries; here it is once for
+// up to 256.
+// Keys become fp16 numbers, as the queries do, each times a power of two, of the row of the
+// queries and of 32 keys, that the scores are rid of again: rounded to 11 bits, they leave
+// the scores as exact as the weights' own rounding.  Values and weights are bf16: whatever
+// the size of a value, it fits.
+// Registers: a softmax thread holds a row of 128 scores; the others leave it theirs.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <mutex>
+
+#define B200_TREE_CALL __forceinline__
+#include "b200_cache4.h"
+#include "paged_host.h"
+#include "tree_attn.cuh"
+#include "tree_attn4.cuh"
+#include "tree_attn_tiles.cuh"
+
+namespace b200tree {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kSoftmaxThreads = 256;
+constexpr int kLoadWarp = 8, kQkWarp = 9, kPvWarp = 10, kPlanWarp = 11;
+constexpr int kCodeWarp = 12, kCodeWarps = 4;
+constexpr int kAhead = 4;        // segments that are planned ahead
+constexpr int kReaders = 15;     // warps that go through the segments
+
+// What is left of a unit in the CTA's run; tiles 0: the run's end.
+struct Segment {
+  int b, h, rt, t;  // sequence, key head, row tile, first key tile
+  int n, tiles;     // key tiles of the segment and of the unit
+  int len, drafts;
+};
+// Of the block's 512 x 128 registers: 256 threads take 176, 128 keep 64 and 128 keep 96.
+constexpr int kSoftmaxRegs = 176, kIssueRegs = 64, kCodeRegs = 96;
+static_assert(256 * kSoftmaxRegs + 128 * (kIssueRegs + kCodeRegs) <= kThreads * 128,
+              "more registers than the block has");
+
+template <int kRegs>
+__device__ __forceinline__ void keep_more() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void keep_fewer() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+template <int DP_, bool kTwo_>
+struct CodedShape {
+  static constexpr int DP = DP_;
+  static constexpr bool kTwo = kTwo_;
+  static constexpr int RM = kTwo ? 256 : 128;
+  static constexpr int kChunks = DP / 64;                  // 128-byte swizzle blocks of a row
+  static constexpr int kChunkBytes = kTile * 128;
+  static constexpr int kTileBytes = kChunks * kChunkBytes;  // a Q, K or V tile
+  static constexpr int kQTiles = kTwo ? 2 : 1;
+  static constexpr int kSlots = DP == 128 ? 4 : 6;
+  static constexpr int kRawRow = DP / 2 + 16, kRawBytes = kTile * kRawRow;  // coded
+  static constexpr int kRawSlots = DP == 64 ? 8 : (kTwo ? 2 : 6);
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffRing = kQTiles * kTileBytes;
+  static constexpr int kOffRaw = kOffRing + kSlots * kTileBytes;
+  static constexpr int kOffSums = kOffRaw + kRawSlots * kRawBytes;
+  static constexpr int kOffRun = kOffSums + 8 * 16;  // one sum a warp
+  static constexpr int kOffPlan = kOffRun + 64;  // [kAhead]
+  static constexpr int kOffSeen = kOffPlan + kAhead * 32;  // [kAhead][kSeen] masks of a unit's tokens
+  static constexpr int kOffRowScale = kOffSeen + kAhead * 8 * kSeen;  // [kAhead][RM]
+  static constexpr int kOffKeyScale = kOffRowScale + kAhead * 4 * RM;
+  static constexpr int kOffBar = kOffKeyScale + 8 * 4 * 4;
+  static_assert(sizeof(Segment) == 32, "eight numbers");
+  static_assert(sizeof(Run) <= 64, "a run's place");
+  using G = Grid<RM, kTile, 4>;
+  static constexpr int kBarQ = 0, kBarQRead = 1, kBarFull = 2, kBarEmpty = kBarFull + kSlots,
+                       kBarScores = kBarEmpty + kSlots, kBarRead = kBarScores + 2,
+                       kBarWeights = kBarRead + 2, kBarSums = kBarWeights + 2,
+                       kBarDrain = kBarSums + 2, kBarRawFull = kBarDrain + 1,
+                       kBarRawEmpty = kBarRawFull + kRawSlots, kBarPlan = kBarRawEmpty + kRawSlots,
+                       kBarDone = kBarPlan + kAhead, kBars = kBarDone + kAhead;
+  static constexpr int kOffMisc = kOffBar + 8 * kBars;
+  static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
+  static_assert(kSmemBytes <= 232448, "exceeds the shared memory of a block");
+  static constexpr uint32_t kColP = 128, kColO = 256;
+  // Numbers of the loads, in the order of their use: the scores lead the values by a
+  // tile, K0 K1 V0 K2 V1 ... (the place of the key tile past the last stays empty).
+  __device__ static uint32_t load_k(uint32_t t) { return t ? 2 * t - 1 : 0u; }
+  __device__ static uint32_t load_v(uint32_t t) { return 2 * t + 2; }
+  static_assert(kColO + 2 * DP <= kTmemCols, "exceeds the tensor memory");
+};
+
+// The lowest n bits.
+__device__ __forceinline__ uint32_t first_bits(int n) {
+  return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
+}
+
+__device__ __forceinline__ float half_of(uint32_t w, int high) {
+  return __uint_as_float(high ? w & 0xffff0000u : w << 16);
+}
+__device__ __forceinline__ uint32_t bits_of(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+__device__ __forceinline__ uint32_t bits_of(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
+
+// Half bytes n and n + 4 of w as fp16 numbers: under the exponent of 1024, less 1024.
+__device__ __forceinline__ __half2 codes_fp16(uint32_t w, int n) {
+  const uint32_t x = (w >> (4 * n) & 0x000f000fu) | 0x64006400u;
+  return __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1024.f));
+}
+// The same as bf16 numbers.
+__device__ __forceinline__ __nv_bfloat162 codes_bf16(uint32_t w, int n) {
+  const uint32_t x = (w >> (4 * n) & 0x000f000fu) | 0x43004300u;
+  return __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(128.f));
+}
+
+// A row of keys as fp16 numbers times `up`: put(piece of 8 numbers, its bits).  m: steps, lows.
+template <int DP, class Put>
+__device__ __forceinline__ void keys(const uint4 (&c)[DP / 32], const uint32_t (&m)[4], float up,
+                                     Put put) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&c[0]);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const __half2 step = __float2half2_rn(half_of(m[g / 2], g & 1) * up);
+    const __half2 low = __float2half2_rn(half_of(m[2 + g / 2], g & 1) * up);
+    auto pair = [&](uint32_t x, int n) { return bits_of(__hfma2(codes_fp16(x, n), step, low)); };
+    if constexpr (DP == 128) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // lane q's word of the group
+        const uint32_t x = w[4 * q + g];
+        put(4 * g + q, make_uint4(pair(x, 0), pair(x, 1), pair(x, 2), pair(x, 3)));
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {  // words g / 2 of lanes 2 q and 2 q + 1
+        const uint32_t x = w[4 * q + g / 2], y = w[4 * q + 2 + g / 2];
+        const int n = 2 * (g % 2);
+        put(2 * g + q, make_uint4(pair(x, n), pair(x, n + 1), pair(y, n), pair(y, n + 1)));
+      }
+    }
+  }
+}
+
+// A row of values as bf16 numbers.
+template <int DP, class Put>
+__device__ __forceinline__ void values(const uint4 (&c)[DP / 32], const uint32_t (&m)[4], Put put) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&c[0]);
+  auto as = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
+  if constexpr (DP == 128) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {  // groups 2 y and 2 y + 1 share words
+      const __nv_bfloat162 step = as(m[y]), low = as(m[2 + y]);
+      auto pair = [&](uint32_t x, int n) { return bits_of(__hfma2(codes_bf16(x, n), step, low)); };
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // columns 2 q and 2 q + 1 of the row
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int n = 0; n < 4; n += 2) {
+            const uint32_t word = w[4 * q + 2 * x + y], a = pair(word, n), b = pair(word, n + 1);
+            lo[2 * x + n / 2] = __byte_perm(a, b, 0x5410);
+            hi[2 * x + n / 2] = __byte_perm(a, b, 0x7632);
+          }
+        put(8 * y + q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        put(8 * y + 4 + q, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+      }
+    }
+  } else {
+    // half bytes 0, 1 of a word's halves are groups 0 and 2, half bytes 2, 3 groups 1 and 3
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int from = y ? 0x7632 : 0x5410;
+      const __nv_bfloat162 step = as(__byte_perm(m[0], m[1], from)), low = as(__byte_perm(m[2], m[3], from));
+      auto pair = [&](uint32_t x, int n) { return bits_of(__hfma2(codes_bf16(x, n), step, low)); };
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // column 4 q + x of the row
+          const uint32_t a = pair(w[4 * q + x], 2 * y), b = pair(w[4 * q + x], 2 * y + 1);
+          lo[x] = __byte_perm(a, b, 0x5410);
+          hi[x] = __byte_perm(a, b, 0x7632);
+        }
+        put(2 * y + q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        put(2 * (y + 2) + q, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+      }
+    }
+  }
+}
+
+template <class S>
+__global__ void __launch_bounds__(kThreads, 1)
+    coded_kernel(const __grid_constant__ Args a, const int32_t box_rows) {
+  constexpr int DP = S::DP, NS = S::kSlots, RM = S::RM, NR = S::kRawSlots, DT = B200_ATTN_DTYPE_BF16;
+  constexpr bool kTwo = S::kTwo;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = ptx::smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Run* found = reinterpret_cast<Run*>(smem + S::kOffRun);
+  // misc[0] tensor memory base, [1] abort flag, [2] last segment with a value that is not finite
+  uint64_t* seen = reinterpret_cast<uint64_t*>(smem + S::kOffSeen);
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem + S::kOffMisc);
+  volatile uint32_t* abort_flag = misc + 1;
+  auto bar = [&](int i) { return sbase + S::kOffBar + 8u * static_cast<uint32_t>(i); };
+
+  ptx::launch_dependents();
+  if (threadIdx.x == 0) {
+    misc[1] = 0u;
+    misc[2] = 0u;
+    ptx::mbar_init(bar(S::kBarQ), kCodeWarps);
+    ptx::mbar_init(bar(S::kBarQRead), 1);
+    for (int s = 0; s < NS; ++s) {
+      ptx::mbar_init(bar(S::kBarFull + s), kCodeWarps);
+      ptx::mbar_init(bar(S::kBarEmpty + s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(bar(S::kBarScores + i), 1);
+      ptx::mbar_init(bar(S::kBarRead + i), 4);
+      ptx::mbar_init(bar(S::kBarWeights + i), 4);
+      ptx::mbar_init(bar(S::kBarSums + i), 1);
+    }
+    for (int s = 0; s < kAhead; ++s) {
+      ptx::mbar_init(bar(S::kBarPlan + s), 1);
+      ptx::mbar_init(bar(S::kBarDone + s), kReaders);
+    }
+    for (int s = 0; s < NR; ++s) {
+      ptx::mbar_init(bar(S::kBarRawFull + s), 1);
+      ptx::mbar_init(bar(S::kBarRawEmpty + s), kCodeWarps);
+    }
+    ptx::mbar_init(bar(S::kBarDrain), 2);
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+  }
+  ptx::grid_dependency_wait();
+  if (threadIdx.x < kSoftmaxThreads) zero_unused_rows(a, 2, kSoftmaxThreads);
+  find_run<typename S::G>(a, blockIdx.x, gridDim.x, reinterpret_cast<uint32_t*>(smem + S::kOffSums),
+                          found);
+  const Run& run = *found;
+  if (run.done(run.p)) return;
+  if (warp == kQkWarp) {
+    ptx::tmem_alloc(sbase + S::kOffMisc, kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = misc[0];
+  // rows of a unit, and of those one group's share
+  auto unit_rows = [&](const Segment& p) {
+    return min(a.unit_rows, p.drafts * a.group - p.rt * a.unit_rows);
+  };
+  const int share = kTwo ? a.unit_rows >> 1 : a.unit_rows;
+  // group i takes tile j of a segment
+  auto takes = [&](int i, int j, int rows) {
+    return kTwo ? (i == 0 || rows > share) : (j & 1) == i;
+  };
+  // Segment `seg` of the run, by every reading warp; false: there is none, or a wait ran out.  A warp
+  // that is done with a segment says so.
+  volatile int* plan = reinterpret_cast<volatile int*>(smem + S::kOffPlan);
+  auto segment = [&](uint32_t seg, Segment* p) {
+    if (!warp_wait(bar(S::kBarPlan + seg % kAhead), (seg / kAhead) & 1u, abort_flag, a.err)) {
+      p->n = 0;
+      return false;
+    }
+    volatile int* x = plan + 8 * (seg % kAhead);
+    *p = Segment{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+    return p->n > 0;
+  };
+  auto segment_done = [&](uint32_t seg) {
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar(S::kBarDone + seg % kAhead));
+  };
+  float* row_scale = reinterpret_cast<float*>(smem + S::kOffRowScale);  // [kAhead][RM]
+  float* key_scale = reinterpret_cast<float*>(smem + S::kOffKeyScale);  // [8 tiles][4 warps]
+
+  // The softmax groups take the registers that the others leave.  (Nothing may lie behind the
+  // three branches: it would have to do with the fewest.)
+  if (warp >= kLoadWarp && warp < kCodeWarp) {
+    keep_fewer<kIssueRegs>();
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------ producer of coded rows
+    // A box of rows that lie side by side is one copy; a lane a box.
+    const int boxes = kTile / box_rows;
+    const uint32_t size = static_cast<uint32_t>(a.page_size);
+    auto load = [&](bool value, int b, int h, int k0, int total, uint32_t seq) {
+      const uint32_t r = seq % NR, full = bar(S::kBarRawFull + r);
+      if (!warp_wait(bar(S::kBarRawEmpty + r), ((seq / NR) & 1u) ^ 1u, abort_flag, a.err)) return false;
+      const int valid = min(kTile, total - k0);
+      const uint8_t* base = value ? a.v + h * a.v_head : a.k + h * a.k_head;
+      const int64_t page_stride = value ? a.v_page : a.k_page, row_stride = value ? a.v_row : a.k_row;
+      const uint32_t at = S::kOffRaw + r * S::kRawBytes;
+      const int32_t* table = a.table + b * a.table_stride;
+      int page[4];
+      uint32_t rows = 0;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int key = (lane + 32 * y) * box_rows, n = min(box_rows, valid - key);
+        page[y] = -1;
+        if (lane + 32 * y >= boxes || n <= 0) continue;
+        page[y] = __ldg(table + static_cast<uint32_t>(k0 + key) / size);
+        if (page[y] < 0 || page[y] >= a.pages) {
+          report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
+          page[y] = -1;
+          for (int x = 0; x < n * S::kRawRow; x += 16)  // rows without a page are zero
+            *reinterpret_cast<uint4*>(smem + at + key * S::kRawRow + x) = make_uint4(0u, 0u, 0u, 0u);
+          ptx::fence_proxy_async_smem();
+        } else {
+          rows += n;
+        }
+      }
+      rows = __reduce_add_sync(0xffffffffu, rows);
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_expect_tx(full, rows * S::kRawRow);
+      __syncwarp();
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        if (page[y] < 0) continue;
+        const int key = (lane + 32 * y) * box_rows, n = min(box_rows, valid - key);
+        const uint32_t in = static_cast<uint32_t>(k0 + key) % size;
+        bulk_copy(sbase + at + key * S::kRawRow, base + page[y] * page_stride + in * row_stride,
+                  n * S::kRawRow, full);
+      }
+      return true;
+    };
+    // the page numbers of the tile after, on their way to L1
+    auto warm = [&](int b, int k0, int total) {
+      const int key = k0 + kTile + 4 * lane;
+      if (key < total)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.table + b * a.table_stride +
+                                                      static_cast<uint32_t>(key) / size));
+    };
+    int old[2][4];  // sequence, key head, first key and keys of the tiles t - 2 and t - 1
+    uint32_t seq = 0, seg = 0;
+    Segment p;
+    bool ok = true, more = segment(0, &p);
+    int j = 0, rest = 2;  // rounds after the last keys, for the last values
+#pragma unroll 1
+    for (uint32_t t = 0; ok && rest > 0; ++t) {
+      if (t >= 2) {
+        ok = load(true, old[0][0], old[0][1], old[0][2], old[0][3], seq);
+        if (ok) ++seq;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) old[0][x] = old[1][x];
+      if (!more) {
+        --rest;
+        continue;
+      }
+      const int k0 = (p.t + j) * kTile, total = p.len + p.drafts;
+      ok = ok && load(false, p.b, p.h, k0, total, seq);
+      if (ok) ++seq;
+      warm(p.b, k0, total);
+      old[1][0] = p.b, old[1][1] = p.h, old[1][2] = k0, old[1][3] = total;
+      if (++j == p.n) {
+        segment_done(seg);
+        more = segment(++seg, &p);
+        j = 0;
+      }
+    }
+    if (!ok) {
+      // copies in flight land before the shared memory goes
+      for (uint32_t x = seq > NR ? seq - NR : 0u; x < seq; ++x)
+        settle(bar(S::kBarRawFull + x % NR), (x / NR) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == kQkWarp) {
+    // -------------------------------------------------- scores S = Q K^T
+    // By the whole warp, one lane of which issues: in control flow that is the same for the
+    // warp the operands' descriptors stay in uniform registers.
+    constexpr uint32_t id = ptx::idesc_f16(false, kTile, kTile, false);
+    uint32_t tile = 0, seg = 0;
+    uint32_t made = 0u;  // bit i: parity of the number of scores made for group i
+    int prev = -1;
+    bool ok = true;
+    Segment p;
+#pragma unroll 1
+    for (; ok && segment(seg, &p); ++seg) {
+      const int n = __shfl_sync(0xffffffffu, p.n, 0);
+      const bool second = !kTwo || __shfl_sync(0xffffffffu, unit_rows(p), 0) > share;
+      ok = warp_wait(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
+#pragma unroll 1
+      for (int j = 0; ok && j < n; ++j, ++tile) {
+        const uint32_t number = S::load_k(tile), s = number % NS;
+        ok = issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          if (!ok || (kTwo ? (i == 1 && !second) : (j & 1) != i)) continue;
+          // the scores before these have been copied to registers
+          ok = prev < 0 ||
+               issuer_wait(bar(S::kBarRead + prev), ((made >> prev) & 1u) ^ 1u, abort_flag, a.err);
+          if (!ok) continue;
+          ptx::tc_fence_after();
+          const uint64_t qd = ptx::smem_desc_sw128(
+              sbase + S::kOffQ + (kTwo ? i : 0) * S::kTileBytes, 16, 1024);
+          const uint64_t kd =
+              ptx::smem_desc_sw128(sbase + S::kOffRing + s * S::kTileBytes, 16, 1024);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * S::kChunkBytes + (kk & 3) * 32) >> 4;
+              ptx::tc_mma_ss(tmem, qd + off, kd + off, id, kk > 0 ? 1u : 0u);
+            }
+            ptx::tc_commit(bar(S::kBarScores + i));
+          }
+          __syncwarp();
+          made ^= 1u << i;
+          prev = i;
+        }
+        if (ok && elect_one()) ptx::tc_commit(bar(S::kBarEmpty + s));
+        __syncwarp();
+      }
+      if (elect_one()) ptx::tc_commit(bar(S::kBarQRead));
+      segment_done(seg);
+    }
+    if (elect_one()) {
+      ptx::tc_commit(bar(S::kBarDrain));
+      settle(bar(S::kBarDrain), 0);
+    }
+    __syncwarp();
+  } else if (warp == kPlanWarp) {
+    // ------------------------------------------------- segments and their masks
+    Place pl = run.p;
+    bool ok = true, more = true;
+#pragma unroll 1
+    for (uint32_t seg = 0; ok && more; ++seg) {
+      const uint32_t at = seg % kAhead;
+      ok = warp_wait(bar(S::kBarDone + at), ((seg / kAhead) & 1u) ^ 1u, abort_flag, a.err);
+      if (!ok) break;
+      more = !run.done(pl);
+      const int n = more ? run.tiles(pl) : 0;
+      if (more && a.tokens <= kSeen) {
+        // a bit for each drafted token that a token sees
+#pragma unroll 1
+        for (int x = lane; x < 2 * a.tokens; x += 32)
+          reinterpret_cast<uint32_t*>(seen)[at * 2 * kSeen + x] =
+              (x & 1) && a.tokens <= 32 ? 0u : seen_word(a, pl.b, x >> 1, 32 * (x & 1), pl.s.drafts);
+      }
+      if (lane == 0) {
+        volatile int* x = plan + 8 * at;
+        x[0] = pl.b, x[1] = pl.h, x[2] = pl.rt, x[3] = pl.t, x[4] = n, x[5] = pl.tiles;
+        x[6] = pl.s.len, x[7] = pl.s.drafts;
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(S::kBarPlan + at));
+      pl.t += n;
+      if (more && pl.t == pl.tiles) pl = next_unit<typename S::G>(a, pl);
+    }
+    __syncwarp();
+  } else if (warp == kPvWarp) {
+    // ------------------------------------------------------- O_i += P_i V
+    constexpr uint32_t id = ptx::idesc_f16(true, kTile, DP, true);
+    uint32_t tile = 0, seg = 0;
+    uint32_t made = 0u;  // bit i: parity of the number of products made for group i
+    bool ok = true;
+    Segment p;
+#pragma unroll 1
+    for (; ok && segment(seg, &p); ++seg) {
+      const int n = __shfl_sync(0xffffffffu, p.n, 0);
+      const int rows = __shfl_sync(0xffffffffu, unit_rows(p), 0);
+      uint32_t begun = 0u;  // bit i: O_i holds a product of this segment
+#pragma unroll 1
+      for (int j = 0; ok && j < n; ++j, ++tile) {
+        const uint32_t number = S::load_v(tile), s = number % NS;
+        ok = warp_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
+        const uint32_t va = sbase + S::kOffRing + s * S::kTileBytes;
+        const uint64_t vd = ptx::smem_desc_sw128(va, S::kChunkBytes, 1024);
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          if (!ok || !takes(i, j, rows)) continue;
+          ok = issuer_wait(bar(S::kBarWeights + i), (made >> i) & 1u, abort_flag, a.err);
+          if (!ok) continue;
+          ptx::tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + S::kColP + 64 * i + kk * 8,
+                             vd + kk * (2048 >> 4), id, (((begun >> i) & 1u) || kk > 0) ? 1u : 0u);
+            ptx::tc_commit(bar(S::kBarSums + i));
+          }
+          __syncwarp();
+          begun |= 1u << i;
+          made ^= 1u << i;
+        }
+        if (ok && elect_one()) ptx::tc_commit(bar(S::kBarEmpty + s));
+        __syncwarp();
+      }
+      segment_done(seg);
+    }
+    if (elect_one()) {
+      ptx::tc_commit(bar(S::kBarDrain));
+      settle(bar(S::kBarDrain), 0);
+    }
+    __syncwarp();
+  }
+  } else if (warp >= kCodeWarp) {
+    keep_fewer<kCodeRegs>();
+    // ------------------------------------------- operands from queries and codes
+    const int wq = warp - kCodeWarp, row = 32 * wq + lane;  // of a tile
+    auto put = [&](uint32_t at, int piece, uint4 v) {
+      *reinterpret_cast<uint4*>(smem + at + (piece >> 3) * S::kChunkBytes + row * 128 +
+                                (((piece & 7) ^ (row & 7)) << 4)) = v;
+    };
+    auto hand_over = [&](int b) {  // what the warp wrote, to the tensor cores
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(b));
+    };
+    // The queries of a segment: fp16, times the power of two that brings the row's largest
+    // number to 2^13..2^14.
+    auto queries = [&](const Segment& p, uint32_t seg) {
+      const int rows = unit_rows(p);
+#pragma unroll 1
+      for (int i = 0; i < (kTwo ? 2 : 1); ++i) {
+        if (row >= share || i * share + row >= rows) continue;
+        const int r = p.rt * a.unit_rows + i * share + row, tok = r / a.group;
+        const uint8_t* src = a.q + p.b * a.q_seq + (p.h * a.group + r - tok * a.group) * a.q_head +
+                             tok * a.q_tok;
+        float big = 0.f;
+#pragma unroll 4
+        for (int x = 0; x < a.head_dim / 8; ++x) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + x);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float2 f = unpack2<DT>(w[y]);
+            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        const int e = max(static_cast<int>(__float_as_uint(big) >> 23), 20);
+        const float up = __uint_as_float(static_cast<uint32_t>(267 - e) << 23);
+#pragma unroll 4
+        for (int x = 0; x < DP / 8; ++x) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (8 * x < a.head_dim) v = __ldg(reinterpret_cast<const uint4*>(src) + x);
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float2 f = unpack2<DT>(w[y]);
+            w[y] = pack2<B200_ATTN_DTYPE_FP16>(f.x * up, f.y * up);
+          }
+          put(S::kOffQ + i * S::kTileBytes, x, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+        row_scale[(seg % kAhead) * RM + i * kTile + row] =
+            a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
+      }
+      hand_over(S::kBarQ);
+    };
+    // A tile: each thread has a row of codes c[DP / 32], steps and lows.
+    auto tile_of = [&](bool value, int k0, int len, int total, uint32_t seg, uint32_t t, uint32_t seq,
+                       uint32_t number) {
+      const uint32_t r = seq % NR, s = number % NS;
+      if (!warp_wait(bar(S::kBarRawFull + r), (seq / NR) & 1u, abort_flag, a.err)) return false;
+      const uint4* raw_row = reinterpret_cast<const uint4*>(smem + S::kOffRaw + r * S::kRawBytes + row * S::kRawRow);
+      uint4 c[DP / 32], meta;
+#pragma unroll
+      for (int x = 0; x < DP / 32; ++x) c[x] = raw_row[x];
+      meta = raw_row[DP / 32];
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(S::kBarRawEmpty + r));
+      const int key = k0 + row;
+      if (key >= total) {
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x) c[x] = make_uint4(0u, 0u, 0u, 0u);
+        meta = make_uint4(0u, 0u, 0u, 0u);
+      }
+      uint32_t m[4] = {meta.x, meta.y, meta.z, meta.w};
+      if (value && key >= len) {
+        // a hidden value must not reach a row as 0 x NaN: added by the softmax groups
+        bool odd = false;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t f = not_finite<DT>(m[x]);
+          odd |= f != 0u;
+          m[x] &= ~f;
+        }
+        if (odd) misc[2] = seg + 1u;
+      }
+      const uint32_t at = S::kOffRing + s * S::kTileBytes;
+      if (value) {
+        if (!warp_wait(bar(S::kBarEmpty + s), ((number / NS) & 1u) ^ 1u, abort_flag, a.err)) return false;
+        values<DP>(c, m, [&](int piece, uint4 v) { put(at, piece, v); });
+      } else {
+        // fp16, times the power of two that brings the warp's largest number below 2^14
+        uint32_t e = 20u;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float step = half_of(m[g / 2], g & 1), low = half_of(m[2 + g / 2], g & 1);
+          const float most = fmaxf(fabsf(low), fabsf(fmaf(15.f, step, low)));
+          if (isfinite(step) && isfinite(low)) e = max(e, __float_as_uint(fminf(most, 0x1.fffffep127f)) >> 23);
+        }
+        e = __reduce_max_sync(0xffffffffu, e);
+        if (lane == 0) key_scale[(t & 7u) * 4 + wq] = __uint_as_float((e - 13u) << 23);
+        if (!warp_wait(bar(S::kBarEmpty + s), ((number / NS) & 1u) ^ 1u, abort_flag, a.err)) return false;
+        keys<DP>(c, m, __uint_as_float((267u - e) << 23), [&](int piece, uint4 v) { put(at, piece, v); });
+      }
+      hand_over(S::kBarFull + s);
+      return true;
+    };
+    int old[2][4];  // first key, committed tokens, keys and segment of the tiles t - 2 and t - 1
+    uint32_t seq = 0, seg = 0;
+    Segment p;
+    bool ok = true, more = segment(0, &p);
+    int j = 0, rest = 2;
+#pragma unroll 1
+    for (uint32_t t = 0; ok && rest > 0; ++t) {
+      if (t >= 2)
+        ok = tile_of(true, old[0][0], old[0][1], old[0][2], static_cast<uint32_t>(old[0][3]), t - 2,
+                     seq++, S::load_v(t - 2));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) old[0][x] = old[1][x];
+      if (!more) {
+        --rest;
+        continue;
+      }
+      if (ok && j == 0) {
+        ok = seg == 0 || warp_wait(bar(S::kBarQRead), (seg - 1u) & 1u, abort_flag, a.err);
+        if (ok) queries(p, seg);
+      }
+      const int k0 = (p.t + j) * kTile, total = p.len + p.drafts;
+      ok = ok && tile_of(false, k0, p.len, total, seg, t, seq++, S::load_k(t));
+      old[1][0] = k0, old[1][1] = p.len, old[1][2] = total, old[1][3] = static_cast<int>(seg);
+      if (++j == p.n) {
+        segment_done(seg);
+        more = segment(++seg, &p);
+        j = 0;
+      }
+    }
+    __syncwarp();
+  } else {
+    keep_more<kSoftmaxRegs>();
+    // ------------------------------------------------------------ softmax
+    const int i = warp >> 2, quad = warp & 3, rl = quad * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t tS = tmem + lanes, tP = tS + S::kColP + 64 * i, tO = tS + S::kColO;
+    const int row0 = i * (kTwo ? share : 0);  // first row of this group in the unit
+    uint32_t seg = 0, cnt = 0, tile0 = 0;  // segments of the run, tiles of this group, of all before the segment
+    bool ok = true;
+    // what is needed of the segment only at its ends stays in shared memory
+    volatile int* unit = plan;
+    Segment begin;
+#pragma unroll 1
+    for (; ok && segment(seg, &begin); ++seg) {
+      unit = plan + 8 * (seg % kAhead);
+      const int n = begin.n, rows = unit_rows(begin), t0 = begin.t, len = begin.len;
+      const bool idle = row0 + quad * 32 >= rows || quad * 32 >= share;  // padding rows only
+      float m_run = -INFINITY, l_run = 0.f;
+      int done = 0;
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        if (!takes(i, j, rows)) continue;
+        if (!warp_wait(bar(S::kBarScores + i), cnt & 1u, abort_flag, a.err)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const int k0 = (t0 + j) * kTile;
+        const bool partly = k0 + kTile > len;  // drafted tokens, or places past the last key
+        if (idle) {  // nothing to compute, but the barriers count this warp
+          warp_arrive(bar(S::kBarRead + i), lane);
+          ok = cnt == 0 || warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
+          if (!ok) break;
+          warp_arrive(bar(S::kBarWeights + i), lane);
+          ++cnt;
+          continue;
+        }
+        // a bit for each key that this row sees
+        uint32_t words[4] = {~0u, ~0u, ~0u, ~0u};
+        if (partly) {
+          const int tok = min((unit[2] * a.unit_rows + row0 + rl) / a.group, a.tokens - 1);
+          const uint64_t bits = a.tokens <= kSeen ? seen[(seg % kAhead) * kSeen + tok] : 0u;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int d = k0 + 32 * q - len;
+            if (d <= -32) continue;
+            if (a.tokens <= kSeen)
+              words[q] = d >= 64 ? 0u
+                                 : static_cast<uint32_t>(d < 0 ? bits << -d | ((1u << -d) - 1u) : bits >> d);
+            else
+              words[q] = first_bits(min(unit[7], tok + 1) - d);  // a chain
+          }
+        }
+        uint32_t sr[kTile];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          ptx::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * c]));
+        ptx::tmem_wait_ld();
+        warp_arrive(bar(S::kBarRead + i), lane);
+        if (partly) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            hide(*reinterpret_cast<uint32_t(*)[32]>(&sr[32 * q]), words[q]);
+        }
+        // from the products' unit to that of the exponents, for the keys of each of four warps
+        const float4 ks = *reinterpret_cast<const float4*>(key_scale + ((tile0 + j) & 7u) * 4);
+        const float rs = row_scale[(seg % kAhead) * RM + (kTwo ? i * kTile : 0) + rl];
+        const float to_log2[4] = {rs * ks.x, rs * ks.y, rs * ks.z, rs * ks.w};
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < kTile; k += 2)
+          top[k >> 5] = max3(top[k >> 5], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
+        const float mx = fmaxf(fmaxf(top[0] * to_log2[0], top[1] * to_log2[1]),
+                               fmaxf(top[2] * to_log2[2], top[3] * to_log2[3]));
+        const bool resc = mx > m_run + kRescale || (m_run == -INFINITY && mx > m_run);
+        const float m_new = resc ? mx : m_run;
+        const float alpha = resc ? ptx::ex2_approx(m_run - m_new) : 1.f;
+        m_run = m_new;
+        l_run *= alpha;
+        // P_i was last read by the product before this one, which also left O_i at rest
+        if (cnt > 0) {
+          if (!warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+        }
+        if (done > 0 && __any_sync(0xffffffffu, resc)) {
+#pragma unroll 1
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t o[16];
+            ld_x16(tO + DP * i + 16 * c, o);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            st_x16(tO + DP * i + 16 * c, o);
+          }
+        }
+        const float neg = m_run == -INFINITY ? 0.f : -m_run;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // pieces of 32 keys, so that few registers are new
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int k = 32 * c + 2 * e;
+            float x, y;
+            fma2(x, y, __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]), to_log2[c], neg);
+            x = ptx::ex2_approx(x);
+            y = ptx::ex2_approx(y);
+            pk[e] = pack2<DT>(x, y);
+            // the sum is taken of the rounded weights, which the product uses
+            const float2 r = unpack2<DT>(pk[e]);
+            add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], r.x, r.y);
+          }
+          st_x16(tP + 16 * c, pk);
+        }
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        ptx::tmem_wait_st();
+        warp_arrive(bar(S::kBarWeights + i), lane);
+        ++cnt;
+        ++done;
+      }
+      // while the last product runs: where the row's results go
+      const int ub = unit[0], uh = unit[1], urt = unit[2], tiles = unit[5];
+      const bool first = t0 == 0, last = t0 + n == tiles, finish = first && last;
+      const bool mine = rl < share && row0 + rl < rows;
+      const int row = urt * a.unit_rows + row0 + rl, tok = min(row / a.group, a.tokens - 1);
+      uint8_t* out = a.o + ub * a.o_seq + (uh * a.group + row % a.group) * a.o_head + tok * a.o_tok;
+      float* part = a.partial +
+                    static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * (RM * (DP + 2));
+      tile0 += n;
+      __syncwarp();
+      if (ok && cnt > 0) ok = warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
+      __syncwarp();
+      // ---------------------------------------------------- end of a segment
+      if (!kTwo && ok) {
+        // the other group reads this row's maximum and sum where P_i was
+        ptx::tc_fence_after();
+        st_pair(tP, __float_as_uint(m_run), __float_as_uint(l_run));
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+      }
+      if constexpr (!kTwo) ok = ptx::named_barrier_and(1, kSoftmaxThreads, ok);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      // (a later segment's may have been noted already: then add_odd looks, and finds none)
+      const bool any_odd = misc[2] > seg;
+      // weights of the groups' sums in this thread's row
+      float top = m_run, total = l_run, w[2] = {1.f, 1.f};
+      if constexpr (!kTwo) {
+        uint32_t om, ol;
+        ld_pair(tS + S::kColP + 64 * (1 - i), om, ol);
+        ptx::tmem_wait_ld();
+        const float m_other = __uint_as_float(om);
+        top = fmaxf(m_run, m_other);
+        const float mine_w = m_run == -INFINITY ? 0.f : ptx::ex2_approx(m_run - top);
+        const float other_w = m_other == -INFINITY ? 0.f : ptx::ex2_approx(m_other - top);
+        total = mine_w * l_run + other_w * __uint_as_float(ol);
+        w[0] = i == 0 ? mine_w : other_w;
+        w[1] = i == 0 ? other_w : mine_w;
+      }
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      if (!idle) {
+        // kTwo: all columns of the own rows; else half the columns of the shared ones
+        constexpr int kSpan = kTwo ? DP : DP / 2;
+#pragma unroll 1
+        for (int c = 0; c < kSpan / 32; ++c) {
+          const int col = (kTwo ? 0 : i * kSpan) + 32 * c;
+          uint32_t o[32];
+          float acc[32];
+          if constexpr (kTwo) {
+            ptx::tmem_ld_32x32b_x32(tO + DP * i + col, o);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[e] = __uint_as_float(o[e]);
+          } else {
+            ptx::tmem_ld_32x32b_x32(tO + col, o);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[e] = w[0] * __uint_as_float(o[e]);
+            if (n > 1) {
+              ptx::tmem_ld_32x32b_x32(tO + DP + col, o);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) acc[e] += w[1] * __uint_as_float(o[e]);
+            }
+          }
+          if (finish) {
+            if (mine) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (col + 8 * e < a.head_dim)
+                  *reinterpret_cast<uint4*>(out + 2 * (col + 8 * e)) = make_uint4(
+                      pack2<DT>(acc[8 * e] * inv, acc[8 * e + 1] * inv),
+                      pack2<DT>(acc[8 * e + 2] * inv, acc[8 * e + 3] * inv),
+                      pack2<DT>(acc[8 * e + 4] * inv, acc[8 * e + 5] * inv),
+                      pack2<DT>(acc[8 * e + 6] * inv, acc[8 * e + 7] * inv));
+            }
+          } else if (mine) {
+            // A column of rows at a time.  Own rows only: where the head group does not divide
+            // 128 a group's share is less than its 128 lanes, and the places of the lanes past
+            // it are the other group's first rows.
+#pragma unroll
+            for (int e = 0; e < 32; ++e) part[(col + e) * RM + row0 + rl] = acc[e];
+          }
+        }
+      }
+      if (!finish && mine && (kTwo || i == 0)) {
+        part[RM * DP + row0 + rl] = top;
+        part[RM * DP + RM + row0 + rl] = total;
+      }
+      if (any_odd && mine) {
+        const int col0 = kTwo ? 0 : i * (DP / 2), col1 = min(a.head_dim, kTwo ? DP : col0 + DP / 2);
+        add_odd4<DP, DT>(a, ub, uh, Seq{len, unit[7]}, tok, t0 * kTile - len, (t0 + n) * kTile - len,
+                         col0, col1, finish ? reinterpret_cast<uint16_t*>(out) : nullptr,
+                         part + row0 + rl, RM);
+      }
+      if (threadIdx.x == 0 && last)
+        a.desc[(ub * a.kv_heads + uh) * a.row_tiles + urt] =
+            make_int2(first ? static_cast<int>(blockIdx.x) : run.first_run,
+                      static_cast<int>(blockIdx.x));
+      // both groups' sums have been read by both
+      ptx::tc_fence_before();
+      if constexpr (!kTwo) ptx::named_barrier_sync(1, kSoftmaxThreads);
+      segment_done(seg);
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == kQkWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// -------------------------------------------------------------------- host
+template <class S>
+int32_t launch_coded_shape(const Args& a, int box_rows, int runs, int device, cudaStream_t s) {
+  using namespace b200paged;
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  std::call_once(once[device], [&] {
+    err[device] = cudaFuncSetAttribute(coded_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       S::kSmemBytes);
+  });
+  if (err[device] != cudaSuccess) {
+    set_error(cudaGetErrorString(err[device]));
+    return B200_ATTN_ERR_LAUNCH;
+  }
+  return launch(coded_kernel<S>, dim3(runs), dim3(kThreads), S::kSmemBytes, s, a, box_rows);
+}
+
+}  // namespace
+
+int32_t launch_coded(int rm, int dp, const Args& a, int runs, int device, cudaStream_t s) {
+  // rows that lie side by side and in one page, whatever the place of the first
+  const int row = dp / 2 + 16;
+  int box = 1;
+  if (a.k_row == row && a.v_row == row)
+    while (box < kTile && a.page_size % (2 * box) == 0) box *= 2;
+  if (rm == 256)
+    return dp == 64 ? launch_coded_shape<CodedShape<64, true>>(a, box, runs, device, s)
+                    : launch_coded_shape<CodedShape<128, true>>(a, box, runs, device, s);
+  return dp == 64 ? launch_coded_shape<CodedShape<64, false>>(a, box, runs, device, s)
+                  : launch_coded_shape<CodedShape<128, false>>(a, box, runs, device, s);
+}
+
+}  // namespace b200tree

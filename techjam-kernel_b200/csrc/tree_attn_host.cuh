@@ -113,4 +113,13 @@ int32_t run_join_rows(const Args& a, int64_t units, bool spread, cudaStream_t s)
                            dim3(32 * WARPS), 0, s, a);
 }
 
+template <int RM, int DP, int DT>
+int32_t run_join_columns(const Args& a, int64_t units, cudaStream_t s) {
+  // few units: the blocks that share a unit's rows share its columns too
+  const bool spread = units * (RM / 32) < 300;
+  return b200paged::launch(spread ? join_columns_kernel<RM, DP, DT, true> : join_columns_kernel<RM, DP, DT, false>,
+                dim3(static_cast<unsigned>(units), RM / 32, spread ? DP / kJoinCols : 1),
+                dim3(32 * kJoinWarps), 0, s, a);
+}
+
 }  // namespace b200tree

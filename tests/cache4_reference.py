@@ -104,14 +104,20 @@ def attention64(q, k, v, table, lens, mask=None, drafts=None, scale=None):
     return out, size, grow
 
 
-def attention_bound(dtype, out, size, grow, head_dim, keys):
+def attention_bound(dtype, out, size, grow, head_dim, keys, rows=1):
     """How far the kernel may be from the 64-bit result.  w = 2^-24.  A score is a sum of
     head_dim exact products and 4 steps and lows in fp32 (the queries' 16-bit form and the lows'
     three bf16 parts add less than w each): off by (head_dim + 12) w grow, a weight by that and a few w
     for the exponential, and normalising doubles it; sums over the keys add keys w.  A weight
-    times a step is rounded to fp16, 2^-11; so is the output to its type."""
+    times a step is rounded to fp16, 2^-11; so is the output to its type.
+
+    bf16 queries of more than 16 rows a key head take the kernel whose operands are rounded: keys to
+    fp16 (a score is off by 2^-11 grow more, a weight by that, and normalising doubles it), values
+    and weights to bf16, 2^-8 each (the sum is of the rounded weights)."""
     w = 2.0 ** -24
     weight = 2 * ((head_dim + 12) * w * grow + 16 * w) + 2 * keys * w + 2.0 ** -11
+    if dtype == torch.bfloat16 and rows > 16:
+        weight = weight + 2 * 2.0 ** -11 * grow + 3 * 2.0 ** -8
     rounding = torch.finfo(dtype).eps / 2
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
     return rounding * out.abs() + (1 + rounding) * weight * size + tiny

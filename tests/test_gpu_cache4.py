@@ -195,7 +195,8 @@ def check(out, q, k, v, table, lens, mask=None, drafts=None, scale=None):
     D = q.shape[-1]
     want, size, grow = attention64(q, decode(k, D, True), decode(v, D, False), table, lens, mask, drafts, scale)
     err = (out.cpu().double() - want).abs()
-    bound = attention_bound(q.dtype, want, size, grow, D, table.shape[1] * k.shape[2])
+    bound = attention_bound(q.dtype, want, size, grow, D, table.shape[1] * k.shape[2],
+                            q.shape[2] * q.shape[1] // k.shape[1])
     assert (err <= bound).all(), f"off by {float((err / bound.clamp(min=1e-30)).max()):.2f} of the bound"
 
 
@@ -212,6 +213,14 @@ CASES = [
     (2, 2, 5, 13, 128, 1, (5, 70), (13, 12), None),
     (2, 1, 4, 33, 72, 24, (90, 400), (33, 20), "tree"),
     (1, 2, 3, 70, 64, 16, (130,), None, "tree"),
+    # more than 16 rows: whole tokens to a row tile, one and two tiles of rows, small and large boxes
+    (2, 2, 4, 8, 128, 16, (0, 300), None, "tree"),
+    (3, 1, 1, 40, 64, 48, (127, 128, 5), (40, 0, 17), "tree"),
+    (1, 2, 3, 64, 96, 64, (777,), None, "shared"),
+    (2, 1, 5, 64, 128, 1, (40, 129), (64, 33), "tree"),
+    (1, 1, 2, 150, 128, 128, (260,), None, None),
+    (2, 1, 1, 300, 40, 32, (3, 0), (300, 1), None),
+    (1, 1, 100, 3, 64, 32, (500,), None, "tree"),
 ]
 
 
@@ -229,6 +238,9 @@ def test_long_context_split_over_the_gpu():
     check(b2.b200_tree_attention(*args), *args)
     args = case(1, 1, 1, 1, 64, 16, (9001,), None, FP16, None)
     check(b2.b200_tree_attention(*args), *args)
+    for T, D in ((10, 128), (40, 64)):
+        args = case(1, 1, 4, T, D, 64, (9001,), None, BF16, "tree")
+        check(b2.b200_tree_attention(*args), *args)
 
 
 def test_rows_that_see_nothing_and_layouts():
@@ -254,7 +266,7 @@ def test_rows_that_see_nothing_and_layouts():
 
 def test_nan_in_hidden_and_in_seen_rows():
     """Groups that are NaN reach the rows that see them, and no other."""
-    for T, group in ((6, 1), (6, 4)):
+    for T, group in ((6, 1), (6, 2), (6, 4), (6, 48)):
         q, k, v, table, lens, _, _ = case(2, 1, group, T, 64, 16, (30, 0), None, BF16, None)
         nan = torch.full((2, 1, T, 64), float("nan"), dtype=BF16, device=DEV)
         x = torch.randn(2, 1, T, 64, dtype=BF16, device=DEV)

@@ -11,13 +11,15 @@
 // queries and of 32 keys, that the scores are rid of again: rounded to 11 bits, they leave
 // the scores as exact as the weights' own rounding.  Values and weights are bf16: whatever
 // the size of a value, it fits.
-// Registers: a softmax thread holds a row of 128 scores; the others leave it theirs.
+// Each softmax group has scores of its own, over which its weights come to lie, and reads them
+// twice, 32 at a time: with a row of 128 scores in registers there were none for a second
+// warp of decoders on each scheduler, and code of four times the size kept all roles waiting
+// for instructions (16 sequences, 128 rows: 188 us).
 #include <cuda_runtime.h>
 
 #include <cstdint>
 #include <mutex>
 
-#define B200_TREE_CALL __forceinline__
 #include "b200_cache4.h"
 #include "paged_host.h"
 #include "tree_attn.cuh"
@@ -27,12 +29,12 @@
 namespace b200tree {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr int kSoftmaxThreads = 256;
 constexpr int kLoadWarp = 8, kQkWarp = 9, kPvWarp = 10, kPlanWarp = 11;
-constexpr int kCodeWarp = 12, kCodeWarps = 4;
+constexpr int kCodeWarp = 12, kCodeWarps = 8;
 constexpr int kAhead = 4;        // segments that are planned ahead
-constexpr int kReaders = 15;     // warps that go through the segments
+constexpr int kReaders = 19;     // warps that go through the segments
 
 // What is left of a unit in the CTA's run; tiles 0: the run's end.
 struct Segment {
@@ -40,20 +42,6 @@ struct Segment {
   int n, tiles;     // key tiles of the segment and of the unit
   int len, drafts;
 };
-// Of the block's 512 x 128 registers: 256 threads take 176, 128 keep 64 and 128 keep 96.
-constexpr int kSoftmaxRegs = 176, kIssueRegs = 64, kCodeRegs = 96;
-static_assert(256 * kSoftmaxRegs + 128 * (kIssueRegs + kCodeRegs) <= kThreads * 128,
-              "more registers than the block has");
-
-template <int kRegs>
-__device__ __forceinline__ void keep_more() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-template <int kRegs>
-__device__ __forceinline__ void keep_fewer() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-
 template <int DP_, bool kTwo_>
 struct CodedShape {
   static constexpr int DP = DP_;
@@ -65,30 +53,30 @@ struct CodedShape {
   static constexpr int kQTiles = kTwo ? 2 : 1;
   static constexpr int kSlots = DP == 128 ? 4 : 6;
   static constexpr int kRawRow = DP / 2 + 16, kRawBytes = kTile * kRawRow;  // coded
-  static constexpr int kRawSlots = DP == 64 ? 8 : (kTwo ? 2 : 6);
+  static constexpr int kRawSlots = DP == 64 ? 8 : (kTwo ? 2 : 5);
   static constexpr int kOffQ = 0;
   static constexpr int kOffRing = kQTiles * kTileBytes;
   static constexpr int kOffRaw = kOffRing + kSlots * kTileBytes;
   static constexpr int kOffSums = kOffRaw + kRawSlots * kRawBytes;
-  static constexpr int kOffRun = kOffSums + 8 * 16;  // one sum a warp
+  static constexpr int kOffRun = kOffSums + 8 * 24;  // one sum a warp
   static constexpr int kOffPlan = kOffRun + 64;  // [kAhead]
   static constexpr int kOffSeen = kOffPlan + kAhead * 32;  // [kAhead][kSeen] masks of a unit's tokens
   static constexpr int kOffRowScale = kOffSeen + kAhead * 8 * kSeen;  // [kAhead][RM]
   static constexpr int kOffKeyScale = kOffRowScale + kAhead * 4 * RM;
-  static constexpr int kOffBar = kOffKeyScale + 8 * 4 * 4;
+  static constexpr int kOffTold = kOffKeyScale + 8 * 4 * 4;  // [2][128] maximum and sum of a row
+  static constexpr int kOffBar = kOffTold + (kTwo ? 0 : 2 * 8 * kTile);
   static_assert(sizeof(Segment) == 32, "eight numbers");
   static_assert(sizeof(Run) <= 64, "a run's place");
   using G = Grid<RM, kTile, 4>;
   static constexpr int kBarQ = 0, kBarQRead = 1, kBarFull = 2, kBarEmpty = kBarFull + kSlots,
-                       kBarScores = kBarEmpty + kSlots, kBarRead = kBarScores + 2,
-                       kBarWeights = kBarRead + 2, kBarSums = kBarWeights + 2,
+                       kBarScores = kBarEmpty + kSlots, kBarWeights = kBarScores + 2, kBarSums = kBarWeights + 2,
                        kBarDrain = kBarSums + 2, kBarRawFull = kBarDrain + 1,
                        kBarRawEmpty = kBarRawFull + kRawSlots, kBarPlan = kBarRawEmpty + kRawSlots,
                        kBarDone = kBarPlan + kAhead, kBars = kBarDone + kAhead;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of a block");
-  static constexpr uint32_t kColP = 128, kColO = 256;
+  static constexpr uint32_t kColO = 256;
   // Numbers of the loads, in the order of their use: the scores lead the values by a
   // tile, K0 K1 V0 K2 V1 ... (the place of the key tile past the last stays empty).
   __device__ static uint32_t load_k(uint32_t t) { return t ? 2 * t - 1 : 0u; }
@@ -118,26 +106,23 @@ __device__ __forceinline__ __nv_bfloat162 codes_bf16(uint32_t w, int n) {
   return __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(128.f));
 }
 
-// A row of keys as fp16 numbers times `up`: put(piece of 8 numbers, its bits).  m: steps, lows.
+// A row of codes as operands, quarter q of them (16 or 8 bytes) at a time, so that the code is
+// small, half of them a side: put(piece of 8 numbers, its bits).  Keys as fp16 numbers; step,
+// low: of the groups.
 template <int DP, class Put>
-__device__ __forceinline__ void keys(const uint4 (&c)[DP / 32], const uint32_t (&m)[4], float up,
-                                     Put put) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&c[0]);
+__device__ __forceinline__ void keys(const uint8_t* row, int side, const __half2 (&step)[4],
+                                     const __half2 (&low)[4], Put put) {
+#pragma unroll 1
+  for (int q = DP / 64 * side; q < DP / 64 * (side + 1); ++q) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + 16 * q);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const __half2 step = __float2half2_rn(half_of(m[g / 2], g & 1) * up);
-    const __half2 low = __float2half2_rn(half_of(m[2 + g / 2], g & 1) * up);
-    auto pair = [&](uint32_t x, int n) { return bits_of(__hfma2(codes_fp16(x, n), step, low)); };
-    if constexpr (DP == 128) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {  // lane q's word of the group
-        const uint32_t x = w[4 * q + g];
-        put(4 * g + q, make_uint4(pair(x, 0), pair(x, 1), pair(x, 2), pair(x, 3)));
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {  // words g / 2 of lanes 2 q and 2 q + 1
-        const uint32_t x = w[4 * q + g / 2], y = w[4 * q + 2 + g / 2];
+    for (int g = 0; g < 4; ++g) {
+      auto pair = [&](uint32_t x, int n) { return bits_of(__hfma2(codes_fp16(x, n), step[g], low[g])); };
+      if constexpr (DP == 128) {  // lane q's word of the group
+        put(4 * g + q, make_uint4(pair(w[g], 0), pair(w[g], 1), pair(w[g], 2), pair(w[g], 3)));
+      } else {  // words g / 2 of lanes 2 q and 2 q + 1
+        const uint32_t x = w[g / 2], y = w[2 + g / 2];
         const int n = 2 * (g % 2);
         put(2 * g + q, make_uint4(pair(x, n), pair(x, n + 1), pair(y, n), pair(y, n + 1)));
       }
@@ -145,50 +130,32 @@ __device__ __forceinline__ void keys(const uint4 (&c)[DP / 32], const uint32_t (
   }
 }
 
-// A row of values as bf16 numbers.
+// Values as bf16 numbers; step, low: of the two groups that share a word's halves.
 template <int DP, class Put>
-__device__ __forceinline__ void values(const uint4 (&c)[DP / 32], const uint32_t (&m)[4], Put put) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&c[0]);
-  auto as = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
-  if constexpr (DP == 128) {
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {  // groups 2 y and 2 y + 1 share words
-      const __nv_bfloat162 step = as(m[y]), low = as(m[2 + y]);
-      auto pair = [&](uint32_t x, int n) { return bits_of(__hfma2(codes_bf16(x, n), step, low)); };
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {  // columns 2 q and 2 q + 1 of the row
-        uint32_t lo[4], hi[4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int n = 0; n < 4; n += 2) {
-            const uint32_t word = w[4 * q + 2 * x + y], a = pair(word, n), b = pair(word, n + 1);
-            lo[2 * x + n / 2] = __byte_perm(a, b, 0x5410);
-            hi[2 * x + n / 2] = __byte_perm(a, b, 0x7632);
-          }
-        put(8 * y + q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-        put(8 * y + 4 + q, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-      }
-    }
-  } else {
-    // half bytes 0, 1 of a word's halves are groups 0 and 2, half bytes 2, 3 groups 1 and 3
+__device__ __forceinline__ void values(const uint8_t* row, int side, const __nv_bfloat162 (&step)[2],
+                                       const __nv_bfloat162 (&low)[2], Put put) {
+#pragma unroll 1
+  for (int q = DP / 64 * side; q < DP / 64 * (side + 1); ++q) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + 16 * q);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-      const int from = y ? 0x7632 : 0x5410;
-      const __nv_bfloat162 step = as(__byte_perm(m[0], m[1], from)), low = as(__byte_perm(m[2], m[3], from));
-      auto pair = [&](uint32_t x, int n) { return bits_of(__hfma2(codes_bf16(x, n), step, low)); };
+      auto pair = [&](uint32_t x, int n) { return bits_of(__hfma2(codes_bf16(x, n), step[y], low[y])); };
+      uint32_t lo[4], hi[4];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t lo[4], hi[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {  // column 4 q + x of the row
-          const uint32_t a = pair(w[4 * q + x], 2 * y), b = pair(w[4 * q + x], 2 * y + 1);
-          lo[x] = __byte_perm(a, b, 0x5410);
-          hi[x] = __byte_perm(a, b, 0x7632);
+      for (int x = 0; x < 4; ++x) {
+        uint32_t a, b;
+        if constexpr (DP == 128) {  // columns 2 q and 2 q + 1 of the row, groups 2 y and 2 y + 1
+          const uint32_t word = w[2 * (x / 2) + y];
+          a = pair(word, 2 * (x % 2)), b = pair(word, 2 * (x % 2) + 1);
+        } else {  // column 4 q + x of the row, groups y and y + 2
+          a = pair(w[x], 2 * y), b = pair(w[x], 2 * y + 1);
         }
-        put(2 * y + q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-        put(2 * (y + 2) + q, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+        lo[x] = __byte_perm(a, b, 0x5410);
+        hi[x] = __byte_perm(a, b, 0x7632);
       }
+      put(DP == 128 ? 8 * y + q : 2 * y + q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+      put(DP == 128 ? 8 * y + 4 + q : 2 * (y + 2) + q, make_uint4(hi[0], hi[1], hi[2], hi[3]));
     }
   }
 }
@@ -222,7 +189,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(bar(S::kBarScores + i), 1);
-      ptx::mbar_init(bar(S::kBarRead + i), 4);
       ptx::mbar_init(bar(S::kBarWeights + i), 4);
       ptx::mbar_init(bar(S::kBarSums + i), 1);
     }
@@ -280,10 +246,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* row_scale = reinterpret_cast<float*>(smem + S::kOffRowScale);  // [kAhead][RM]
   float* key_scale = reinterpret_cast<float*>(smem + S::kOffKeyScale);  // [8 tiles][4 warps]
 
-  // The softmax groups take the registers that the others leave.  (Nothing may lie behind the
-  // three branches: it would have to do with the fewest.)
-  if (warp >= kLoadWarp && warp < kCodeWarp) {
-    keep_fewer<kIssueRegs>();
   if (warp == kLoadWarp) {
     // ------------------------------------------------ producer of coded rows
     // A box of rows that lie side by side is one copy; a lane a box.
@@ -376,8 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // warp the operands' descriptors stay in uniform registers.
     constexpr uint32_t id = ptx::idesc_f16(false, kTile, kTile, false);
     uint32_t tile = 0, seg = 0;
-    uint32_t made = 0u;  // bit i: parity of the number of scores made for group i
-    int prev = -1;
+    uint32_t made = 0u, any = 0u;  // bit i: parity of the number of scores made for group i, and any
     bool ok = true;
     Segment p;
 #pragma unroll 1
@@ -392,9 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (!ok || (kTwo ? (i == 1 && !second) : (j & 1) != i)) continue;
-          // the scores before these have been copied to registers
-          ok = prev < 0 ||
-               issuer_wait(bar(S::kBarRead + prev), ((made >> prev) & 1u) ^ 1u, abort_flag, a.err);
+          // the weights that lie over the group's last scores have been used
+          ok = !((any >> i) & 1u) ||
+               issuer_wait(bar(S::kBarSums + i), ((made >> i) & 1u) ^ 1u, abort_flag, a.err);
           if (!ok) continue;
           ptx::tc_fence_after();
           const uint64_t qd = ptx::smem_desc_sw128(
@@ -405,13 +366,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
               const uint32_t off = ((kk >> 2) * S::kChunkBytes + (kk & 3) * 32) >> 4;
-              ptx::tc_mma_ss(tmem, qd + off, kd + off, id, kk > 0 ? 1u : 0u);
+              ptx::tc_mma_ss(tmem + kTile * i, qd + off, kd + off, id, kk > 0 ? 1u : 0u);
             }
             ptx::tc_commit(bar(S::kBarScores + i));
           }
           __syncwarp();
           made ^= 1u << i;
-          prev = i;
+          any |= 1u << i;
         }
         if (ok && elect_one()) ptx::tc_commit(bar(S::kBarEmpty + s));
         __syncwarp();
@@ -480,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; ++kk)
-              ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + S::kColP + 64 * i + kk * 8,
+              ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + kTile * i + kk * 8,
                              vd + kk * (2048 >> 4), id, (((begun >> i) & 1u) || kk > 0) ? 1u : 0u);
             ptx::tc_commit(bar(S::kBarSums + i));
           }
@@ -498,11 +459,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       settle(bar(S::kBarDrain), 0);
     }
     __syncwarp();
-  }
   } else if (warp >= kCodeWarp) {
-    keep_fewer<kCodeRegs>();
     // ------------------------------------------- operands from queries and codes
-    const int wq = warp - kCodeWarp, row = 32 * wq + lane;  // of a tile
+    const int wq = (warp - kCodeWarp) & 3, row = 32 * wq + lane;  // of a tile
+    const int side = (warp - kCodeWarp) >> 2;                    // two threads a row
     auto put = [&](uint32_t at, int piece, uint4 v) {
       *reinterpret_cast<uint4*>(smem + at + (piece >> 3) * S::kChunkBytes + row * 128 +
                                 (((piece & 7) ^ (row & 7)) << 4)) = v;
@@ -536,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e = max(static_cast<int>(__float_as_uint(big) >> 23), 20);
         const float up = __uint_as_float(static_cast<uint32_t>(267 - e) << 23);
 #pragma unroll 4
-        for (int x = 0; x < DP / 8; ++x) {
+        for (int x = DP / 16 * side; x < DP / 16 * (side + 1); ++x) {
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
           if (8 * x < a.head_dim) v = __ldg(reinterpret_cast<const uint4*>(src) + x);
           uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -547,59 +507,70 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           put(S::kOffQ + i * S::kTileBytes, x, make_uint4(w[0], w[1], w[2], w[3]));
         }
-        row_scale[(seg % kAhead) * RM + i * kTile + row] =
+        if (side == 0) row_scale[(seg % kAhead) * RM + i * kTile + row] =
             a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
       }
       hand_over(S::kBarQ);
     };
-    // A tile: each thread has a row of codes c[DP / 32], steps and lows.
+    // A tile: a thread a row.
     auto tile_of = [&](bool value, int k0, int len, int total, uint32_t seg, uint32_t t, uint32_t seq,
                        uint32_t number) {
       const uint32_t r = seq % NR, s = number % NS;
       if (!warp_wait(bar(S::kBarRawFull + r), (seq / NR) & 1u, abort_flag, a.err)) return false;
-      const uint4* raw_row = reinterpret_cast<const uint4*>(smem + S::kOffRaw + r * S::kRawBytes + row * S::kRawRow);
-      uint4 c[DP / 32], meta;
-#pragma unroll
-      for (int x = 0; x < DP / 32; ++x) c[x] = raw_row[x];
-      meta = raw_row[DP / 32];
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(S::kBarRawEmpty + r));
+      const uint8_t* codes = smem + S::kOffRaw + r * S::kRawBytes + row * S::kRawRow;
       const int key = k0 + row;
-      if (key >= total) {
-#pragma unroll
-        for (int x = 0; x < DP / 32; ++x) c[x] = make_uint4(0u, 0u, 0u, 0u);
-        meta = make_uint4(0u, 0u, 0u, 0u);
-      }
+      uint4 meta = make_uint4(0u, 0u, 0u, 0u);  // what lies past the last key counts as 0
+      if (key < total) meta = *reinterpret_cast<const uint4*>(codes + DP / 2);
       uint32_t m[4] = {meta.x, meta.y, meta.z, meta.w};
-      if (value && key >= len) {
-        // a hidden value must not reach a row as 0 x NaN: added by the softmax groups
-        bool odd = false;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t f = not_finite<DT>(m[x]);
-          odd |= f != 0u;
-          m[x] &= ~f;
-        }
-        if (odd) misc[2] = seg + 1u;
-      }
       const uint32_t at = S::kOffRing + s * S::kTileBytes;
+      auto put_here = [&](int piece, uint4 v) { put(at, piece, v); };
       if (value) {
+        if (key >= len) {
+          // a hidden value must not reach a row as 0 x NaN: added by the softmax groups
+          bool odd = false;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t f = not_finite<DT>(m[x]);
+            odd |= f != 0u;
+            m[x] &= ~f;
+          }
+          if (odd) misc[2] = seg + 1u;
+        }
+        auto as = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
+        __nv_bfloat162 step[2], low[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int from = y ? 0x7632 : 0x5410;
+          step[y] = as(DP == 128 ? m[y] : __byte_perm(m[0], m[1], from));
+          low[y] = as(DP == 128 ? m[2 + y] : __byte_perm(m[2], m[3], from));
+        }
         if (!warp_wait(bar(S::kBarEmpty + s), ((number / NS) & 1u) ^ 1u, abort_flag, a.err)) return false;
-        values<DP>(c, m, [&](int piece, uint4 v) { put(at, piece, v); });
+        values<DP>(codes, side, step, low, put_here);
       } else {
         // fp16, times the power of two that brings the warp's largest number below 2^14
         uint32_t e = 20u;
+        float steps[4], lows[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float step = half_of(m[g / 2], g & 1), low = half_of(m[2 + g / 2], g & 1);
-          const float most = fmaxf(fabsf(low), fabsf(fmaf(15.f, step, low)));
-          if (isfinite(step) && isfinite(low)) e = max(e, __float_as_uint(fminf(most, 0x1.fffffep127f)) >> 23);
+          steps[g] = half_of(m[g / 2], g & 1), lows[g] = half_of(m[2 + g / 2], g & 1);
+          const float most = fmaxf(fabsf(lows[g]), fabsf(fmaf(15.f, steps[g], lows[g])));
+          if (isfinite(steps[g]) && isfinite(lows[g]))
+            e = max(e, __float_as_uint(fminf(most, 0x1.fffffep127f)) >> 23);
         }
         e = __reduce_max_sync(0xffffffffu, e);
-        if (lane == 0) key_scale[(t & 7u) * 4 + wq] = __uint_as_float((e - 13u) << 23);
+        if (lane == 0 && side == 0) key_scale[(t & 7u) * 4 + wq] = __uint_as_float((e - 13u) << 23);
+        const float up = __uint_as_float((267u - e) << 23);
+        __half2 step[4], low[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          step[g] = __float2half2_rn(steps[g] * up);
+          low[g] = __float2half2_rn(lows[g] * up);
+        }
         if (!warp_wait(bar(S::kBarEmpty + s), ((number / NS) & 1u) ^ 1u, abort_flag, a.err)) return false;
-        keys<DP>(c, m, __uint_as_float((267u - e) << 23), [&](int piece, uint4 v) { put(at, piece, v); });
+        keys<DP>(codes, side, step, low, put_here);
       }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(S::kBarRawEmpty + r));
       hand_over(S::kBarFull + s);
       return true;
     };
@@ -634,11 +605,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    keep_more<kSoftmaxRegs>();
     // ------------------------------------------------------------ softmax
     const int i = warp >> 2, quad = warp & 3, rl = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t tS = tmem + lanes, tP = tS + S::kColP + 64 * i, tO = tS + S::kColO;
+    // the weights take the place of the scores that have been read
+    const uint32_t tS = tmem + lanes + kTile * i, tO = tmem + lanes + S::kColO;
     const int row0 = i * (kTwo ? share : 0);  // first row of this group in the unit
     uint32_t seg = 0, cnt = 0, tile0 = 0;  // segments of the run, tiles of this group, of all before the segment
     bool ok = true;
@@ -663,56 +634,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int k0 = (t0 + j) * kTile;
         const bool partly = k0 + kTile > len;  // drafted tokens, or places past the last key
         if (idle) {  // nothing to compute, but the barriers count this warp
-          warp_arrive(bar(S::kBarRead + i), lane);
-          ok = cnt == 0 || warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
-          if (!ok) break;
           warp_arrive(bar(S::kBarWeights + i), lane);
           ++cnt;
           continue;
         }
-        // a bit for each key that this row sees
-        uint32_t words[4] = {~0u, ~0u, ~0u, ~0u};
-        if (partly) {
-          const int tok = min((unit[2] * a.unit_rows + row0 + rl) / a.group, a.tokens - 1);
-          const uint64_t bits = a.tokens <= kSeen ? seen[(seg % kAhead) * kSeen + tok] : 0u;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int d = k0 + 32 * q - len;
-            if (d <= -32) continue;
-            if (a.tokens <= kSeen)
-              words[q] = d >= 64 ? 0u
-                                 : static_cast<uint32_t>(d < 0 ? bits << -d | ((1u << -d) - 1u) : bits >> d);
-            else
-              words[q] = first_bits(min(unit[7], tok + 1) - d);  // a chain
-          }
-        }
-        uint32_t sr[kTile];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          ptx::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * c]));
-        ptx::tmem_wait_ld();
-        warp_arrive(bar(S::kBarRead + i), lane);
-        if (partly) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            hide(*reinterpret_cast<uint32_t(*)[32]>(&sr[32 * q]), words[q]);
-        }
         // from the products' unit to that of the exponents, for the keys of each of four warps
-        const float4 ks = *reinterpret_cast<const float4*>(key_scale + ((tile0 + j) & 7u) * 4);
+        const float* ks = key_scale + ((tile0 + j) & 7u) * 4;
         const float rs = row_scale[(seg % kAhead) * RM + (kTwo ? i * kTile : 0) + rl];
-        const float to_log2[4] = {rs * ks.x, rs * ks.y, rs * ks.z, rs * ks.w};
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // a bit for each of 32 keys that this row sees
+        uint64_t bits = 0u;
+        int tok = 0;
+        if (partly) {
+          tok = min((unit[2] * a.unit_rows + row0 + rl) / a.group, a.tokens - 1);
+          if (a.tokens <= kSeen) bits = seen[(seg % kAhead) * kSeen + tok];
+        }
+        auto visible = [&](int c) {
+          const int d = k0 + 32 * c - len;
+          if (d <= -32) return ~0u;
+          if (a.tokens > kSeen) return first_bits(min(unit[7], tok + 1) - d);  // a chain
+          return d >= 64 ? 0u
+                         : static_cast<uint32_t>(d < 0 ? bits << -d | ((1u << -d) - 1u) : bits >> d);
+        };
+        // Twice over the scores, 32 at a time: little code, few registers.
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t sr[32];
+          ptx::tmem_ld_32x32b_x32(tS + 32 * c, sr);
+          ptx::tmem_wait_ld();
+          if (partly) hide(sr, visible(c));
+          float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < kTile; k += 2)
-          top[k >> 5] = max3(top[k >> 5], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
-        const float mx = fmaxf(fmaxf(top[0] * to_log2[0], top[1] * to_log2[1]),
-                               fmaxf(top[2] * to_log2[2], top[3] * to_log2[3]));
+          for (int k = 0; k < 32; k += 2)
+            top[(k >> 1) & 1] =
+                max3(top[(k >> 1) & 1], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
+          mx = fmaxf(mx, fmaxf(top[0], top[1]) * (rs * ks[c]));
+        }
         const bool resc = mx > m_run + kRescale || (m_run == -INFINITY && mx > m_run);
         const float m_new = resc ? mx : m_run;
         const float alpha = resc ? ptx::ex2_approx(m_run - m_new) : 1.f;
         m_run = m_new;
         l_run *= alpha;
-        // P_i was last read by the product before this one, which also left O_i at rest
+        // (the scores were formed after the last product of the group, so O_i is at rest)
         if (cnt > 0) {
           if (!warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err)) {
             ok = false;
@@ -733,14 +696,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float neg = m_run == -INFINITY ? 0.f : -m_run;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {  // pieces of 32 keys, so that few registers are new
-          uint32_t pk[16];
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t sr[32], pk[16];
+          ptx::tmem_ld_32x32b_x32(tS + 32 * c, sr);
+          ptx::tmem_wait_ld();
+          if (partly) hide(sr, visible(c));
+          const float to_log2 = rs * ks[c];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int k = 32 * c + 2 * e;
             float x, y;
-            fma2(x, y, __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]), to_log2[c], neg);
+            fma2(x, y, __uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1]), to_log2, neg);
             x = ptx::ex2_approx(x);
             y = ptx::ex2_approx(y);
             pk[e] = pack2<DT>(x, y);
@@ -748,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float2 r = unpack2<DT>(pk[e]);
             add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], r.x, r.y);
           }
-          st_x16(tP + 16 * c, pk);
+          st_x16(tS + 16 * c, pk);
         }
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         ptx::tmem_wait_st();
@@ -769,13 +735,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && cnt > 0) ok = warp_wait(bar(S::kBarSums + i), (cnt - 1u) & 1u, abort_flag, a.err);
       __syncwarp();
       // ---------------------------------------------------- end of a segment
-      if (!kTwo && ok) {
-        // the other group reads this row's maximum and sum where P_i was
-        ptx::tc_fence_after();
-        st_pair(tP, __float_as_uint(m_run), __float_as_uint(l_run));
-        ptx::tmem_wait_st();
-        ptx::tc_fence_before();
-      }
+      float2* told = reinterpret_cast<float2*>(smem + S::kOffTold);  // for the other group
+      if (!kTwo) told[kTile * i + rl] = make_float2(m_run, l_run);
       if constexpr (!kTwo) ok = ptx::named_barrier_and(1, kSoftmaxThreads, ok);
       if (!ok) break;
       ptx::tc_fence_after();
@@ -784,14 +745,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       // weights of the groups' sums in this thread's row
       float top = m_run, total = l_run, w[2] = {1.f, 1.f};
       if constexpr (!kTwo) {
-        uint32_t om, ol;
-        ld_pair(tS + S::kColP + 64 * (1 - i), om, ol);
-        ptx::tmem_wait_ld();
-        const float m_other = __uint_as_float(om);
+        const float2 other = told[kTile * (1 - i) + rl];
+        const float m_other = other.x;
         top = fmaxf(m_run, m_other);
         const float mine_w = m_run == -INFINITY ? 0.f : ptx::ex2_approx(m_run - top);
         const float other_w = m_other == -INFINITY ? 0.f : ptx::ex2_approx(m_other - top);
-        total = mine_w * l_run + other_w * __uint_as_float(ol);
+        total = mine_w * l_run + other_w * other.y;
         w[0] = i == 0 ? mine_w : other_w;
         w[1] = i == 0 ? other_w : mine_w;
       }

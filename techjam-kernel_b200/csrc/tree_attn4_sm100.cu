@@ -51,13 +51,15 @@ struct CodedShape {
   static constexpr int kChunkBytes = kTile * 128;
   static constexpr int kTileBytes = kChunks * kChunkBytes;  // a Q, K or V tile
   static constexpr int kQTiles = kTwo ? 2 : 1;
-  static constexpr int kSlots = DP == 128 ? 4 : 6;
+  static constexpr int kSlots = DP == 128 ? 2 : 3;  // of K and of V
   static constexpr int kRawRow = DP / 2 + 16, kRawBytes = kTile * kRawRow;  // coded
-  static constexpr int kRawSlots = DP == 64 ? 8 : (kTwo ? 2 : 5);
+  static constexpr int kRawK = DP == 64 ? 4 : (kTwo ? 1 : 3), kRawV = DP == 64 ? 4 : (kTwo ? 1 : 2);
   static constexpr int kOffQ = 0;
   static constexpr int kOffRing = kQTiles * kTileBytes;
-  static constexpr int kOffRaw = kOffRing + kSlots * kTileBytes;
-  static constexpr int kOffSums = kOffRaw + kRawSlots * kRawBytes;
+  static constexpr int kOffV = kOffRing + kSlots * kTileBytes;
+  static constexpr int kOffRaw = kOffV + kSlots * kTileBytes;
+  static constexpr int kOffRawV = kOffRaw + kRawK * kRawBytes;
+  static constexpr int kOffSums = kOffRawV + kRawV * kRawBytes;
   static constexpr int kOffRun = kOffSums + 8 * 24;  // one sum a warp
   static constexpr int kOffPlan = kOffRun + 64;  // [kAhead]
   static constexpr int kOffSeen = kOffPlan + kAhead * 32;  // [kAhead][kSeen] masks of a unit's tokens
@@ -68,21 +70,25 @@ struct CodedShape {
   static_assert(sizeof(Segment) == 32, "eight numbers");
   static_assert(sizeof(Run) <= 64, "a run's place");
   using G = Grid<RM, kTile, 4>;
-  static constexpr int kBarQ = 0, kBarQRead = 1, kBarFull = 2, kBarEmpty = kBarFull + kSlots,
-                       kBarScores = kBarEmpty + kSlots, kBarWeights = kBarScores + 2, kBarSums = kBarWeights + 2,
-                       kBarDrain = kBarSums + 2, kBarRawFull = kBarDrain + 1,
-                       kBarRawEmpty = kBarRawFull + kRawSlots, kBarPlan = kBarRawEmpty + kRawSlots,
-                       kBarDone = kBarPlan + kAhead, kBars = kBarDone + kAhead;
+  // (those of the values lie kSlots, kRawK or kRawV behind those of the keys)
+  static constexpr int kBarQ = 0, kBarQRead = 1, kBarFull = 2, kBarEmpty = kBarFull + 2 * kSlots,
+                       kBarScores = kBarEmpty + 2 * kSlots, kBarWeights = kBarScores + 2,
+                       kBarSums = kBarWeights + 2, kBarDrain = kBarSums + 2,
+                       kBarRawFull = kBarDrain + 1, kBarRawEmpty = kBarRawFull + kRawK + kRawV,
+                       kBarPlan = kBarRawEmpty + kRawK + kRawV, kBarDone = kBarPlan + kAhead,
+                       kBars = kBarDone + kAhead;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of a block");
   static constexpr uint32_t kColO = 256;
-  // Numbers of the loads, in the order of their use: the scores lead the values by a
-  // tile, K0 K1 V0 K2 V1 ... (the place of the key tile past the last stays empty).
-  __device__ static uint32_t load_k(uint32_t t) { return t ? 2 * t - 1 : 0u; }
-  __device__ static uint32_t load_v(uint32_t t) { return 2 * t + 2; }
   static_assert(kColO + 2 * DP <= kTmemCols, "exceeds the tensor memory");
 };
+
+// So many bytes more are to come before the barrier's phase ends.
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
 
 // The lowest n bits.
 __device__ __forceinline__ uint32_t first_bits(int n) {
@@ -107,13 +113,12 @@ __device__ __forceinline__ __nv_bfloat162 codes_bf16(uint32_t w, int n) {
 }
 
 // A row of codes as operands, quarter q of them (16 or 8 bytes) at a time, so that the code is
-// small, half of them a side: put(piece of 8 numbers, its bits).  Keys as fp16 numbers; step,
-// low: of the groups.
+// small: put(piece of 8 numbers, its bits).  Keys as fp16 numbers; step, low: of the groups.
 template <int DP, class Put>
-__device__ __forceinline__ void keys(const uint8_t* row, int side, const __half2 (&step)[4],
+__device__ __forceinline__ void keys(const uint8_t* row, const __half2 (&step)[4],
                                      const __half2 (&low)[4], Put put) {
 #pragma unroll 1
-  for (int q = DP / 64 * side; q < DP / 64 * (side + 1); ++q) {
+  for (int q = 0; q < DP / 32; ++q) {
     const uint4 v = *reinterpret_cast<const uint4*>(row + 16 * q);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -132,10 +137,10 @@ __device__ __forceinline__ void keys(const uint8_t* row, int side, const __half2
 
 // Values as bf16 numbers; step, low: of the two groups that share a word's halves.
 template <int DP, class Put>
-__device__ __forceinline__ void values(const uint8_t* row, int side, const __nv_bfloat162 (&step)[2],
+__device__ __forceinline__ void values(const uint8_t* row, const __nv_bfloat162 (&step)[2],
                                        const __nv_bfloat162 (&low)[2], Put put) {
 #pragma unroll 1
-  for (int q = DP / 64 * side; q < DP / 64 * (side + 1); ++q) {
+  for (int q = 0; q < DP / 32; ++q) {
     const uint4 v = *reinterpret_cast<const uint4*>(row + 16 * q);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -163,7 +168,7 @@ __device__ __forceinline__ void values(const uint8_t* row, int side, const __nv_
 template <class S>
 __global__ void __launch_bounds__(kThreads, 1)
     coded_kernel(const __grid_constant__ Args a, const int32_t box_rows) {
-  constexpr int DP = S::DP, NS = S::kSlots, RM = S::RM, NR = S::kRawSlots, DT = B200_ATTN_DTYPE_BF16;
+  constexpr int DP = S::DP, NS = S::kSlots, RM = S::RM, DT = B200_ATTN_DTYPE_BF16;
   constexpr bool kTwo = S::kTwo;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
@@ -181,10 +186,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     misc[1] = 0u;
     misc[2] = 0u;
-    ptx::mbar_init(bar(S::kBarQ), kCodeWarps);
+    ptx::mbar_init(bar(S::kBarQ), kCodeWarps / 2);
     ptx::mbar_init(bar(S::kBarQRead), 1);
-    for (int s = 0; s < NS; ++s) {
-      ptx::mbar_init(bar(S::kBarFull + s), kCodeWarps);
+    for (int s = 0; s < 2 * NS; ++s) {
+      ptx::mbar_init(bar(S::kBarFull + s), kCodeWarps / 2);
       ptx::mbar_init(bar(S::kBarEmpty + s), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -196,9 +201,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(bar(S::kBarPlan + s), 1);
       ptx::mbar_init(bar(S::kBarDone + s), kReaders);
     }
-    for (int s = 0; s < NR; ++s) {
+    for (int s = 0; s < S::kRawK + S::kRawV; ++s) {
       ptx::mbar_init(bar(S::kBarRawFull + s), 1);
-      ptx::mbar_init(bar(S::kBarRawEmpty + s), kCodeWarps);
+      ptx::mbar_init(bar(S::kBarRawEmpty + s), kCodeWarps / 2);
     }
     ptx::mbar_init(bar(S::kBarDrain), 2);
     ptx::fence_mbar_init();
@@ -248,88 +253,79 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kLoadWarp) {
     // ------------------------------------------------ producer of coded rows
-    // A box of rows that lie side by side is one copy; a lane a box.
+    // A box of rows that lie side by side is one copy; a lane a box.  The page numbers of a
+    // tile are read while the tile before is copied.
     const int boxes = kTile / box_rows;
-    const uint32_t size = static_cast<uint32_t>(a.page_size);
-    auto load = [&](bool value, int b, int h, int k0, int total, uint32_t seq) {
-      const uint32_t r = seq % NR, full = bar(S::kBarRawFull + r);
-      if (!warp_wait(bar(S::kBarRawEmpty + r), ((seq / NR) & 1u) ^ 1u, abort_flag, a.err)) return false;
-      const int valid = min(kTile, total - k0);
-      const uint8_t* base = value ? a.v + h * a.v_head : a.k + h * a.k_head;
-      const int64_t page_stride = value ? a.v_page : a.k_page, row_stride = value ? a.v_row : a.k_row;
-      const uint32_t at = S::kOffRaw + r * S::kRawBytes;
-      const int32_t* table = a.table + b * a.table_stride;
-      int page[4];
-      uint32_t rows = 0;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int key = (lane + 32 * y) * box_rows, n = min(box_rows, valid - key);
-        page[y] = -1;
-        if (lane + 32 * y >= boxes || n <= 0) continue;
-        page[y] = __ldg(table + static_cast<uint32_t>(k0 + key) / size);
-        if (page[y] < 0 || page[y] >= a.pages) {
-          report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
-          page[y] = -1;
-          for (int x = 0; x < n * S::kRawRow; x += 16)  // rows without a page are zero
-            *reinterpret_cast<uint4*>(smem + at + key * S::kRawRow + x) = make_uint4(0u, 0u, 0u, 0u);
-          ptx::fence_proxy_async_smem();
-        } else {
-          rows += n;
-        }
-      }
-      rows = __reduce_add_sync(0xffffffffu, rows);
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_expect_tx(full, rows * S::kRawRow);
-      __syncwarp();
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        if (page[y] < 0) continue;
-        const int key = (lane + 32 * y) * box_rows, n = min(box_rows, valid - key);
-        const uint32_t in = static_cast<uint32_t>(k0 + key) % size;
-        bulk_copy(sbase + at + key * S::kRawRow, base + page[y] * page_stride + in * row_stride,
-                  n * S::kRawRow, full);
-      }
-      return true;
+    const uint32_t size = static_cast<uint32_t>(a.page_size), inv_size = 0xffffffffu / size + 1u;
+    auto slot_of = [&](uint32_t key) {  // key / size: the product is it or one more
+      if (size == 1u) return key;
+      const uint32_t q = __umulhi(key, inv_size);
+      return q * size > key ? q - 1u : q;
     };
-    // the page numbers of the tile after, on their way to L1
-    auto warm = [&](int b, int k0, int total) {
-      const int key = k0 + kTile + 4 * lane;
-      if (key < total)
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.table + b * a.table_stride +
-                                                      static_cast<uint32_t>(key) / size));
-    };
-    int old[2][4];  // sequence, key head, first key and keys of the tiles t - 2 and t - 1
-    uint32_t seq = 0, seg = 0;
+    uint32_t tiles = 0, seg = 0;
+    uint32_t rk = 0, rv = 0, pk = 1u, pv = 1u;  // raw slots, and parities of their release
     Segment p;
     bool ok = true, more = segment(0, &p);
-    int j = 0, rest = 2;  // rounds after the last keys, for the last values
+    int j = 0, next = -1;
+    auto look_up = [&]() {
+      const int key = (p.t + j) * kTile + lane * box_rows;
+      next = lane < boxes && key < p.len + p.drafts ? __ldg(a.table + p.b * a.table_stride + slot_of(key))
+                                                    : -1;
+    };
+    if (more) look_up();
 #pragma unroll 1
-    for (uint32_t t = 0; ok && rest > 0; ++t) {
-      if (t >= 2) {
-        ok = load(true, old[0][0], old[0][1], old[0][2], old[0][3], seq);
-        if (ok) ++seq;
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) old[0][x] = old[1][x];
-      if (!more) {
-        --rest;
-        continue;
-      }
-      const int k0 = (p.t + j) * kTile, total = p.len + p.drafts;
-      ok = ok && load(false, p.b, p.h, k0, total, seq);
-      if (ok) ++seq;
-      warm(p.b, k0, total);
-      old[1][0] = p.b, old[1][1] = p.h, old[1][2] = k0, old[1][3] = total;
+    for (; ok && more; ++tiles) {
+      const int k0 = (p.t + j) * kTile, valid = min(kTile, p.len + p.drafts - k0);
+      const int32_t* table = a.table + p.b * a.table_stride;
+      const uint8_t* kb = a.k + p.h * a.k_head;
+      const uint8_t* vb = a.v + p.h * a.v_head;
+      const int now = next;
       if (++j == p.n) {
         segment_done(seg);
         more = segment(++seg, &p);
         j = 0;
       }
+      if (more) look_up();
+      const uint32_t fk = bar(S::kBarRawFull + rk), fv = bar(S::kBarRawFull + S::kRawK + rv);
+      ok = warp_wait(bar(S::kBarRawEmpty + rk), pk, abort_flag, a.err) &&
+           warp_wait(bar(S::kBarRawEmpty + S::kRawK + rv), pv, abort_flag, a.err);
+      if (!ok) break;
+      const uint32_t at_k = S::kOffRaw + rk * S::kRawBytes, at_v = S::kOffRawV + rv * S::kRawBytes;
+#pragma unroll 1
+      for (int u = lane; u < boxes; u += 32) {
+        const int key = u * box_rows, n = min(box_rows, valid - key);
+        if (n <= 0) break;
+        const uint32_t slot = slot_of(k0 + key), in = k0 + key - slot * size;
+        const int page = u == lane ? now : __ldg(table + slot);
+        if (page < 0 || page >= a.pages) {
+          report_error(a.err, B200_ATTN_DEVERR_BOUNDS);
+          for (int x = 0; x < n * S::kRawRow; x += 16) {  // rows without a page are zero
+            *reinterpret_cast<uint4*>(smem + at_k + key * S::kRawRow + x) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(smem + at_v + key * S::kRawRow + x) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          ptx::fence_proxy_async_smem();
+          continue;
+        }
+        const uint32_t bytes = n * S::kRawRow;
+        expect_tx(fk, bytes);
+        expect_tx(fv, bytes);
+        bulk_copy(sbase + at_k + key * S::kRawRow, kb + page * a.k_page + in * a.k_row, bytes, fk);
+        bulk_copy(sbase + at_v + key * S::kRawRow, vb + page * a.v_page + in * a.v_row, bytes, fv);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        ptx::mbar_arrive(fk);
+        ptx::mbar_arrive(fv);
+      }
+      if (++rk == S::kRawK) rk = 0, pk ^= 1u;
+      if (++rv == S::kRawV) rv = 0, pv ^= 1u;
     }
     if (!ok) {
       // copies in flight land before the shared memory goes
-      for (uint32_t x = seq > NR ? seq - NR : 0u; x < seq; ++x)
-        settle(bar(S::kBarRawFull + x % NR), (x / NR) & 1u);
+      for (uint32_t x = tiles > S::kRawK ? tiles - S::kRawK : 0u; x < tiles; ++x)
+        settle(bar(S::kBarRawFull + x % S::kRawK), (x / S::kRawK) & 1u);
+      for (uint32_t x = tiles > S::kRawV ? tiles - S::kRawV : 0u; x < tiles; ++x)
+        settle(bar(S::kBarRawFull + S::kRawK + x % S::kRawV), (x / S::kRawV) & 1u);
     }
     __syncwarp();
   } else if (warp == kQkWarp) {
@@ -348,8 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = warp_wait(bar(S::kBarQ), seg & 1u, abort_flag, a.err);
 #pragma unroll 1
       for (int j = 0; ok && j < n; ++j, ++tile) {
-        const uint32_t number = S::load_k(tile), s = number % NS;
-        ok = issuer_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
+        const uint32_t s = tile % NS;
+        ok = issuer_wait(bar(S::kBarFull + s), (tile / NS) & 1u, abort_flag, a.err);
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (!ok || (kTwo ? (i == 1 && !second) : (j & 1) != i)) continue;
@@ -428,9 +424,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t begun = 0u;  // bit i: O_i holds a product of this segment
 #pragma unroll 1
       for (int j = 0; ok && j < n; ++j, ++tile) {
-        const uint32_t number = S::load_v(tile), s = number % NS;
-        ok = warp_wait(bar(S::kBarFull + s), (number / NS) & 1u, abort_flag, a.err);
-        const uint32_t va = sbase + S::kOffRing + s * S::kTileBytes;
+        const uint32_t s = tile % NS;
+        ok = warp_wait(bar(S::kBarFull + NS + s), (tile / NS) & 1u, abort_flag, a.err);
+        const uint32_t va = sbase + S::kOffV + s * S::kTileBytes;
         const uint64_t vd = ptx::smem_desc_sw128(va, S::kChunkBytes, 1024);
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
@@ -449,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           begun |= 1u << i;
           made ^= 1u << i;
         }
-        if (ok && elect_one()) ptx::tc_commit(bar(S::kBarEmpty + s));
+        if (ok && elect_one()) ptx::tc_commit(bar(S::kBarEmpty + NS + s));
         __syncwarp();
       }
       segment_done(seg);
@@ -461,8 +457,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= kCodeWarp) {
     // ------------------------------------------- operands from queries and codes
-    const int wq = (warp - kCodeWarp) & 3, row = 32 * wq + lane;  // of a tile
-    const int side = (warp - kCodeWarp) >> 2;                    // two threads a row
+    // Four warps for the keys, four for the queries and the values, a thread a row of a tile.
+    const int wq = (warp - kCodeWarp) & 3, row = 32 * wq + lane;
+    const bool value = warp >= kCodeWarp + 4;
     auto put = [&](uint32_t at, int piece, uint4 v) {
       *reinterpret_cast<uint4*>(smem + at + (piece >> 3) * S::kChunkBytes + row * 128 +
                                 (((piece & 7) ^ (row & 7)) << 4)) = v;
@@ -496,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e = max(static_cast<int>(__float_as_uint(big) >> 23), 20);
         const float up = __uint_as_float(static_cast<uint32_t>(267 - e) << 23);
 #pragma unroll 4
-        for (int x = DP / 16 * side; x < DP / 16 * (side + 1); ++x) {
+        for (int x = 0; x < DP / 8; ++x) {
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
           if (8 * x < a.head_dim) v = __ldg(reinterpret_cast<const uint4*>(src) + x);
           uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -507,17 +504,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           put(S::kOffQ + i * S::kTileBytes, x, make_uint4(w[0], w[1], w[2], w[3]));
         }
-        if (side == 0) row_scale[(seg % kAhead) * RM + i * kTile + row] =
+        row_scale[(seg % kAhead) * RM + i * kTile + row] =
             a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
       }
       hand_over(S::kBarQ);
     };
-    // A tile: a thread a row.
-    auto tile_of = [&](bool value, int k0, int len, int total, uint32_t seg, uint32_t t, uint32_t seq,
-                       uint32_t number) {
-      const uint32_t r = seq % NR, s = number % NS;
-      if (!warp_wait(bar(S::kBarRawFull + r), (seq / NR) & 1u, abort_flag, a.err)) return false;
-      const uint8_t* codes = smem + S::kOffRaw + r * S::kRawBytes + row * S::kRawRow;
+    uint32_t r = 0, rp = 0;  // raw slot and parity of its filling
+    uint32_t e0 = 0, ep = 1u;  // slot of the operand and parity of its release
+    const uint32_t raw_slots = value ? S::kRawV : S::kRawK;
+    auto tile_of = [&](int k0, int len, int total, uint32_t seg, uint32_t t) {
+      const uint32_t raw_bar = value ? S::kRawK + r : r, s = value ? NS + e0 : e0;
+      if (!warp_wait(bar(S::kBarRawFull + raw_bar), rp, abort_flag, a.err)) return false;
+      const uint8_t* codes = smem + S::kOffRaw + raw_bar * S::kRawBytes + row * S::kRawRow;
       const int key = k0 + row;
       uint4 meta = make_uint4(0u, 0u, 0u, 0u);  // what lies past the last key counts as 0
       if (key < total) meta = *reinterpret_cast<const uint4*>(codes + DP / 2);
@@ -544,8 +542,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           step[y] = as(DP == 128 ? m[y] : __byte_perm(m[0], m[1], from));
           low[y] = as(DP == 128 ? m[2 + y] : __byte_perm(m[2], m[3], from));
         }
-        if (!warp_wait(bar(S::kBarEmpty + s), ((number / NS) & 1u) ^ 1u, abort_flag, a.err)) return false;
-        values<DP>(codes, side, step, low, put_here);
+        if (!warp_wait(bar(S::kBarEmpty + s), ep, abort_flag, a.err)) return false;
+        values<DP>(codes, step, low, put_here);
       } else {
         // fp16, times the power of two that brings the warp's largest number below 2^14
         uint32_t e = 20u;
@@ -558,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             e = max(e, __float_as_uint(fminf(most, 0x1.fffffep127f)) >> 23);
         }
         e = __reduce_max_sync(0xffffffffu, e);
-        if (lane == 0 && side == 0) key_scale[(t & 7u) * 4 + wq] = __uint_as_float((e - 13u) << 23);
+        if (lane == 0) key_scale[(t & 7u) * 4 + wq] = __uint_as_float((e - 13u) << 23);
         const float up = __uint_as_float((267u - e) << 23);
         __half2 step[4], low[4];
 #pragma unroll
@@ -566,42 +564,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           step[g] = __float2half2_rn(steps[g] * up);
           low[g] = __float2half2_rn(lows[g] * up);
         }
-        if (!warp_wait(bar(S::kBarEmpty + s), ((number / NS) & 1u) ^ 1u, abort_flag, a.err)) return false;
-        keys<DP>(codes, side, step, low, put_here);
+        if (!warp_wait(bar(S::kBarEmpty + s), ep, abort_flag, a.err)) return false;
+        keys<DP>(codes, step, low, put_here);
       }
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(S::kBarRawEmpty + r));
+      if (lane == 0) ptx::mbar_arrive(bar(S::kBarRawEmpty + raw_bar));
       hand_over(S::kBarFull + s);
+      if (++r == raw_slots) r = 0, rp ^= 1u;
+      if (++e0 == NS) e0 = 0, ep ^= 1u;
       return true;
     };
-    int old[2][4];  // first key, committed tokens, keys and segment of the tiles t - 2 and t - 1
-    uint32_t seq = 0, seg = 0;
+    uint32_t t = 0;
+    bool ok = true;
     Segment p;
-    bool ok = true, more = segment(0, &p);
-    int j = 0, rest = 2;
 #pragma unroll 1
-    for (uint32_t t = 0; ok && rest > 0; ++t) {
-      if (t >= 2)
-        ok = tile_of(true, old[0][0], old[0][1], old[0][2], static_cast<uint32_t>(old[0][3]), t - 2,
-                     seq++, S::load_v(t - 2));
-#pragma unroll
-      for (int x = 0; x < 4; ++x) old[0][x] = old[1][x];
-      if (!more) {
-        --rest;
-        continue;
-      }
-      if (ok && j == 0) {
+    for (uint32_t seg = 0; ok && segment(seg, &p); ++seg) {
+      if (value) {
         ok = seg == 0 || warp_wait(bar(S::kBarQRead), (seg - 1u) & 1u, abort_flag, a.err);
         if (ok) queries(p, seg);
       }
-      const int k0 = (p.t + j) * kTile, total = p.len + p.drafts;
-      ok = ok && tile_of(false, k0, p.len, total, seg, t, seq++, S::load_k(t));
-      old[1][0] = k0, old[1][1] = p.len, old[1][2] = total, old[1][3] = static_cast<int>(seg);
-      if (++j == p.n) {
-        segment_done(seg);
-        more = segment(++seg, &p);
-        j = 0;
-      }
+#pragma unroll 1
+      for (int j = 0; ok && j < p.n; ++j, ++t)
+        ok = tile_of((p.t + j) * kTile, p.len, p.len + p.drafts, seg, t);
+      segment_done(seg);
     }
     __syncwarp();
   } else {

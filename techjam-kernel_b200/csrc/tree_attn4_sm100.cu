@@ -345,13 +345,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int j = 0; ok && j < n; ++j, ++tile) {
         const uint32_t s = tile % NS;
-        ok = issuer_wait(bar(S::kBarFull + s), (tile / NS) & 1u, abort_flag, a.err);
+        ok = warp_wait(bar(S::kBarFull + s), (tile / NS) & 1u, abort_flag, a.err);
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (!ok || (kTwo ? (i == 1 && !second) : (j & 1) != i)) continue;
           // the weights that lie over the group's last scores have been used
           ok = !((any >> i) & 1u) ||
-               issuer_wait(bar(S::kBarSums + i), ((made >> i) & 1u) ^ 1u, abort_flag, a.err);
+               warp_wait(bar(S::kBarSums + i), ((made >> i) & 1u) ^ 1u, abort_flag, a.err);
           if (!ok) continue;
           ptx::tc_fence_after();
           const uint64_t qd = ptx::smem_desc_sw128(
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (!ok || !takes(i, j, rows)) continue;
-          ok = issuer_wait(bar(S::kBarWeights + i), (made >> i) & 1u, abort_flag, a.err);
+          ok = warp_wait(bar(S::kBarWeights + i), (made >> i) & 1u, abort_flag, a.err);
           if (!ok) continue;
           ptx::tc_fence_after();
           if (elect_one()) {
@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             odd |= f != 0u;
             m[x] &= ~f;
           }
-          if (odd) misc[2] = seg + 1u;
+          // (a warp that is ahead may have noted a later segment)
+          if (odd) atomicMax(const_cast<uint32_t*>(&misc[2]), seg + 1u);
         }
         auto as = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
         __nv_bfloat162 step[2], low[2];

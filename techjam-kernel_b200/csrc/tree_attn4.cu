@@ -9,7 +9,10 @@
 // weights w = 2^(s - m),
 //   sum w v = sum_g (w step_g) code + w low_g:
 // w step_g is rounded to fp16 (relative to a power of two that follows the largest step), w low_g
-// and sum w are fp32.
+// and sum w are fp32.  For results of fp16 the codes of values are taken less 8 and the lows plus
+// 8 steps: of numbers on both sides of zero low and step code are each a multiple of the
+// sum, and so was the error of the rounded w step_g (24 sequences of 7 rows, head dim 64: 1.45
+// times that of weights and values rounded to fp16, now 1.1 times; 45.6 us without, 47.3 with).
 //
 // A half byte becomes an fp16 operand by one AND: bits 0..3 of a half word are the subnormal
 // number code 2^-24, bits 4..7 the number 16 code 2^-24 (the factors go into the queries and
@@ -123,10 +126,17 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int32_t* e
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 
+// Pairs of fp16 numbers, x - y: of codes exact.
+__device__ __forceinline__ uint32_t less(uint32_t x, uint32_t y) {
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
 template <class S, int DT>
 __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     rows4_kernel(const __grid_constant__ Args a) {
   constexpr int RM = S::RM, DP = S::DP, NS = S::kStages, NG = DP / 32, NT = S::kHalves;
+  constexpr bool kCentred = DT == B200_ATTN_DTYPE_FP16;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sbase = b200attn::ptx::smem_u32(smem);
   float* join = reinterpret_cast<float*>(smem + S::kOffJoin);
@@ -552,8 +562,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             const uint32_t lw0 = g < 2 ? m0.z : m0.w, lw1 = g < 2 ? m1.z : m1.w;
             const float st0 = g & 1 ? high_half(sw0) : low_half(sw0);
             const float st1 = g & 1 ? high_half(sw1) : low_half(sw1);
-            const float lo0 = g & 1 ? high_half(lw0) : low_half(lw0);
-            const float lo1 = g & 1 ? high_half(lw1) : low_half(lw1);
+            float lo0 = g & 1 ? high_half(lw0) : low_half(lw0);
+            float lo1 = g & 1 ? high_half(lw1) : low_half(lw1);
+            if constexpr (kCentred) lo0 = fmaf(8.f, st0, lo0), lo1 = fmaf(8.f, st1, lo1);
             uint32_t pf[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -572,8 +583,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             }
 #pragma unroll
             for (int y = 0; y < NG / 2; ++y) {
-              const uint32_t vf[4] = {(v0 >> 8 * y) & kLow, (v0 >> 8 * y) & kHigh,
-                                      (v1 >> 8 * y) & kLow, (v1 >> 8 * y) & kHigh};
+              uint32_t vf[4] = {(v0 >> 8 * y) & kLow, (v0 >> 8 * y) & kHigh,
+                                (v1 >> 8 * y) & kLow, (v1 >> 8 * y) & kHigh};
+              if constexpr (kCentred) {
+                vf[0] = less(vf[0], 0x00080008u), vf[1] = less(vf[1], 0x00800080u);
+                vf[2] = less(vf[2], 0x00080008u), vf[3] = less(vf[3], 0x00800080u);
+              }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 float(&d)[4] = o[nt][NG / 2 * g + y];

@@ -324,7 +324,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       const uint32_t mid = pack_pair<B200_ATTN_DTYPE_BF16>(rest, 0.f);
       qs[nt][0] = hi | mid << 16;
       qs[nt][1] = pack_pair<B200_ATTN_DTYPE_BF16>(rest - low_half(mid), 0.f);
-      const float f = a.scale_log2 * 0x1p24f * __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
+      // (neither 0, as a hidden score is -inf, nor infinite, as a score may be 0)
+      const float f = fminf(
+          fmaxf(a.scale_log2 * 0x1p24f * __uint_as_float(static_cast<uint32_t>(e - 13) << 23), 0x1p-149f),
+          0x1.fffffep127f);
       to_log2[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c4);
       to_log2[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
     }

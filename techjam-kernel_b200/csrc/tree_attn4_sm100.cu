@@ -641,6 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           return d >= 64 ? 0u
                          : static_cast<uint32_t>(d < 0 ? bits << -d | ((1u << -d) - 1u) : bits >> d);
         };
+        // neither 0, as a hidden score is -inf, nor infinite, as a score may be 0 (scores are
+        // below 2^36, so what the lower end adds to one is nothing)
+        auto to_log2 = [&](int c) { return fminf(fmaxf(rs * ks[c], 0x1p-126f), 0x1.fffffep127f); };
         // Twice over the scores, 32 at a time: little code, few registers.
         float mx = -INFINITY;
 #pragma unroll 1
@@ -654,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 32; k += 2)
             top[(k >> 1) & 1] =
                 max3(top[(k >> 1) & 1], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
-          mx = fmaxf(mx, fmaxf(top[0], top[1]) * (rs * ks[c]));
+          mx = fmaxf(mx, fmaxf(top[0], top[1]) * to_log2(c));
         }
         const bool resc = mx > m_run + kRescale || (m_run == -INFINITY && mx > m_run);
         const float m_new = resc ? mx : m_run;
@@ -688,11 +691,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::tmem_ld_32x32b_x32(tS + 32 * c, sr);
           ptx::tmem_wait_ld();
           if (partly) hide(sr, visible(c));
-          const float to_log2 = rs * ks[c];
+          const float up = to_log2(c);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x, y;
-            fma2(x, y, __uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1]), to_log2, neg);
+            fma2(x, y, __uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1]), up, neg);
             x = ptx::ex2_approx(x);
             y = ptx::ex2_approx(y);
             pk[e] = pack2<DT>(x, y);

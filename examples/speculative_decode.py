@@ -2,7 +2,8 @@
 
 A small decoder (random weights) answers a batch of prompts twice: token by token,
 and with a tree of drafted tokens per step, of which the longest path that greedy
-decoding would have taken is kept.  Both give the same tokens.  Run it on a B200:
+decoding would have taken is kept (``b200_verify_drafts`` at temperature 0).  Both give
+the same tokens.  Run it on a B200:
 
     python examples/speculative_decode.py
 """
@@ -14,7 +15,7 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "techjam-kernel_b200"))
 
-from b200_attention import check_device_errors  # noqa: E402
+from b200_attention import b200_verify_drafts, check_device_errors  # noqa: E402
 from b200_attention.transformer import Decoder, DecoderConfig, init_normal_  # noqa: E402
 
 
@@ -74,6 +75,8 @@ def speculate(model, prompts, new_tokens, draft, branches=3, depth=3):
     dev = prompts.device
     parent, _, mask = tree(branches, depth, dev)
     nodes = len(parent)
+    parents = torch.tensor(parent, dtype=torch.int32, device=dev)
+    uniforms = torch.zeros(batch, nodes, device=dev)  # nothing is drawn at temperature 0
     cache = model.new_cache(batch, length + new_tokens + nodes + depth + 1)
     token = feed_prompts(model, cache, prompts)
     answers = [[int(t)] for t in token]
@@ -83,25 +86,16 @@ def speculate(model, prompts, new_tokens, draft, branches=3, depth=3):
         if int(cache.reserve(nodes)) != 0:
             raise RuntimeError("no pages left")
         hidden = model.cached_forward(drafted, cache, mask)
-        best = logits(model, hidden).argmax(-1).tolist()
-        told = drafted.tolist()
-        paths = torch.zeros(batch, depth + 1, dtype=torch.int32)
-        counts = torch.zeros(batch, dtype=torch.int32)
-        for b in range(batch):
-            if len(answers[b]) >= new_tokens:
-                continue
-            path = [0]  # the root is the model's own last token
-            while True:
-                at = path[-1]
-                answers[b].append(best[b][at])
-                child = [i for i in range(nodes) if parent[i] == at and told[b][i] == best[b][at]]
-                if not child or len(answers[b]) >= new_tokens:
-                    break
-                path.append(child[0])
-            paths[b, :len(path)] = torch.tensor(path, dtype=torch.int32)
-            counts[b] = len(path)
-        cache.accept(paths.to(dev), counts.to(dev))
-        token = torch.tensor([a[-1] for a in answers], device=dev)
+        paths, counts, following = b200_verify_drafts(logits(model, hidden), drafted, uniforms,
+                                                      None, parents, temperature=0.0)
+        # a sequence that has its answer keeps nothing more
+        counts *= torch.tensor([len(a) < new_tokens for a in answers], device=dev)
+        cache.accept(paths, counts)
+        token = torch.where(counts > 0, following, token)
+        told, kept, nexts = drafted.tolist(), paths.tolist(), following.tolist()
+        for b, n in enumerate(counts.tolist()):
+            if n > 0:  # the root is the model's own last token
+                answers[b] += [told[b][at] for at in kept[b][1:n]] + [nexts[b]]
         steps += 1
     check_device_errors(dev)
     return torch.tensor([a[:new_tokens] for a in answers], device=dev), steps

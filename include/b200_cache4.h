@@ -51,11 +51,18 @@ B200_ATTN_API int32_t b200_cache4_read(const b200_cache* c, int64_t head_dim, in
 
 /*
  * b200_tree_attn_fwd over a 4-bit cache (p->cache as above); queries and output of `dtype`
- * (bf16 or fp16).  Products with the codes are exact in the tensor cores' fp32 sums; steps and
- * lows are applied in fp32.  The queries are taken as fp16 numbers times a power of two of
- * their row, which loses nothing of a bf16 or fp16 number that is no smaller than 2^-23 of
- * the row's largest.  A weight times the step of its value is rounded to fp16 for the product;
- * weights times lows, and the sum of weights, are fp32.
+ * (bf16 or fp16).  The queries are taken as fp16 numbers times a power of two of their row,
+ * which loses nothing of a bf16 or fp16 number that is no smaller than 2^-23 of the row's
+ * largest.  Scores, maxima, sums of weights and output sums are fp32, and the output is
+ * rounded once.  Up to 16 rows (tokens * heads / kv_heads), and all calls but those below:
+ * products with the codes are exact in the tensor cores' fp32 sums; steps and lows are applied
+ * in fp32; a weight times the step of its value is rounded to fp16 for the product (with fp16
+ * queries, for codes less 8), relative to the largest step that the row sees (what is below 2^-34
+ * of it is lost); weights times lows, and the sum of weights, are fp32.
+ * More rows with bf16 queries, heads / kv_heads up to 128, and no mask or up to 64 tokens: keys
+ * are rounded to fp16 numbers times a power of two of the 32 committed keys that they are among
+ * (what is below 2^-38 of their largest number is lost), or of a key alone where drafted ones
+ * are near, values and weights to bf16, and the sum is of the rounded weights.
  */
 B200_ATTN_API int32_t b200_cache4_attn_check(const b200_tree_attn_params* p, int64_t head_dim,
                                              int32_t dtype);

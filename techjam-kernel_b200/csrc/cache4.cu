@@ -4,6 +4,15 @@
 // A thread takes a group of a key or value vector, 16 or 32 numbers, so what is done once a group
 // (its ends, step and low) is shared by many numbers; the four threads of a vector exchange words to
 // write rows 8 or 16 bytes at a time.
+//
+// Bound by the issue of instructions: some ten a number where the bytes allow two.  33
+// thousand tokens of 8 heads of 128 bf16 numbers, keys and values: append 42 us, read 34 us, together
+// 37 us of bytes at the copy rate.  A thread a vector (80 us for append) kept 128 numbers in
+// registers, a warp a vector spent most of its time in shuffles.
+//
+// Bound by the issue of instructions.  33 thousand tokens of 8 heads of 128 bf16 numbers, keys and
+// values, in and back: 76 us (read 34 of them), 37 us of bytes at the copy rate; with a thread for 8
+// numbers, whose ends went through shuffles, and every code settled exactly: 177.
 #include <cuda_runtime.h>
 
 #include <cstdint>

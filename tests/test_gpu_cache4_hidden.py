@@ -44,3 +44,22 @@ def test_huge_numbers_in_hidden_tokens(T, group, D, dtype, what):
     assert torch.isfinite(second).all()
     bound = 2 * 2.0 ** -7 * (first.float().abs().amax(-1, keepdim=True) + 0.05)
     assert (first.float() - second.float()).abs().le(bound).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,group,D", [(4, 2, 64), (4, 4, 128), (9, 8, 128), (40, 5, 64)])
+def test_a_query_that_is_not_finite_stays_in_its_row(T, group, D, dtype):
+    q, k, v, table, lens, mask, _ = case(2, 2, group, T, D, 16, (50, 400), None, dtype, "tree")
+    q = q.contiguous()
+    want = b2.b200_tree_attention(q, k, v, table, lens, mask)
+    odd = q.clone()
+    odd[0, 1, 1, 3] = float("nan")
+    odd[1, 0, 2, 0] = float("inf")
+    out = b2.b200_tree_attention(odd, k, v, table, lens, mask)
+    check_device_errors(DEV)
+    assert torch.isnan(out[0, 1, 1]).all() and torch.isnan(out[1, 0, 2]).all()
+    out[0, 1, 1], out[1, 0, 2] = want[0, 1, 1], want[1, 0, 2]
+    if group * T <= 16:  # the order of a row's sums may follow its neighbours' steps
+        assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+    else:
+        assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -8)

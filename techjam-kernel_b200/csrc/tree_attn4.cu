@@ -297,12 +297,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             w[0] = v.x, w[1] = v.y;
           }
         }
-        sum[g] = 0.f;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
           const float2 f = unpack_pair<DT>(w[i]);
           big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-          sum[g] += f.x + f.y;
           float* dst = x[NG == 4 ? 2 * g + i / 2 : g];
           dst[2 * (i & 1)] = f.x;
           dst[2 * (i & 1) + 1] = f.y;
@@ -321,9 +319,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
       float mine = 0.f;  // the sum of group c4, in the unit of the products
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
+        sum[g] = 0.f;
+#pragma unroll
+        for (int i = DP / 64 * g; i < DP / 64 * (g + 1); ++i)
+          sum[g] += (x[i][0] * up + x[i][1] * up) + (x[i][2] * up + x[i][3] * up);
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
-        if (g == c4) mine = sum[g] * up * 0x1p-24f;
+        if (g == c4) mine = sum[g] * 0x1p-24f;
       }
       const uint32_t hi = pack_pair<B200_ATTN_DTYPE_BF16>(mine, 0.f);
       const float rest = mine - low_half(hi);
@@ -385,7 +387,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           const uint8_t* row1 = row0 + 8 * S::kRowBytes;
           uint32_t w0[NG], w1[NG];
           if constexpr (NG == 4) {
-            const uint4 u = lds<uint4>(row0 + c4 * (S::kCodes / 4)), v = lds<uint4>(row1 + c4 * (S::kCodes / 4));
+            const uint4 u = lds<uint4>(row0 + c4 * (S::kCodes / 4));
+            const uint4 v = lds<uint4>(row1 + c4 * (S::kCodes / 4));
             w0[0] = u.x, w0[1] = u.y, w0[2] = u.z, w0[3] = u.w;
             w1[0] = v.x, w1[1] = v.y, w1[2] = v.z, w1[3] = v.w;
           } else {
@@ -411,12 +414,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
               const uint32_t kf[4] = {u & kLow, v & kLow, u & kHigh, v & kHigh};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                {
                 const bool on = y > 0;
                 mma<B200_ATTN_DTYPE_FP16>(p[nt], kf, qf[nt][step][0], qf[nt][step][1],
                                           on ? p[nt][0] : 0.f, on ? p[nt][1] : 0.f,
                                           on ? p[nt][2] : 0.f, on ? p[nt][3] : 0.f);
-              }
               }
             }
             const uint32_t a0 = g < 2 ? s0.x : s0.y, a1 = g < 2 ? s1.x : s1.y;
@@ -472,9 +473,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
           __syncwarp();
         }
         // ------------------------------------------------------ softmax
-        // The maximum and the largest step that weights and steps are taken relative to follow the
-        // true ones only where a score is over 2^4 times, or a step is above them: of 18 blocks of
-        // random keys about two, where every new maximum would rescale the sums in ten.
+        // The maximum and the largest step that weights and steps are taken relative to, a row's own, follow
+        // the true ones only where a weight would pass 2^4, or a step is above the least of the rows'
+        // largest: of 18 blocks of random keys about two, where every new maximum would rescale the sums in
+        // ten.
         uint32_t big;  // steps of two keys' values
         bool grew = false;
         {

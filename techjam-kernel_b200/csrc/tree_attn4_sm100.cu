@@ -4,9 +4,9 @@
 // The kernel of 16-bit caches (tree_attn_sm100.cu has the roles, the tensor memory and the
 // order of the loads) with another producer: one warp copies coded rows to shared memory
 // in bulk, and of eight warps, a thread a row, four turn keys and four values into the operands of
-// the products in the swizzled layout that the tensor cores read, each through a ring of its own.  A row of the matrix instruction
-// kernel (tree_attn4.cu) would be decoded again for every 16 rows of queries; here it is once for
-// up to 256.
+// the products in the swizzled layout that the tensor cores read, each through a ring of its
+// own.  The matrix instruction kernel (tree_attn4.cu) would decode a row again for every 16 rows of
+// queries; here it is once for up to 256.
 // Keys become fp16 numbers, as the queries do, each times a power of two, of the row of the
 // queries and of 32 keys (of a key alone in tiles that hold drafted ones, which a row may not see),
 // that the scores are rid of again: rounded to 11 bits, they leave the scores as exact as the
@@ -613,7 +613,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the weights take the place of the scores that have been read
     const uint32_t tS = tmem + lanes + kTile * i, tO = tmem + lanes + S::kColO;
     const int row0 = i * (kTwo ? share : 0);  // first row of this group in the unit
-    uint32_t seg = 0, cnt = 0, tile0 = 0;  // segments of the run, tiles of this group, of all before the segment
+    uint32_t seg = 0, cnt = 0;  // segments of the run, tiles of this group
+    uint32_t tile0 = 0;         // tiles of both groups before the segment
     bool ok = true;
     // what is needed of the segment only at its ends stays in shared memory
     volatile int* unit = plan;

@@ -63,3 +63,17 @@ def test_a_query_that_is_not_finite_stays_in_its_row(T, group, D, dtype):
         assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
     else:
         assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -8)
+
+
+@pytest.mark.parametrize("T,group", [(4, 2), (24, 2)])
+def test_queries_and_keys_near_the_ends_of_the_type(T, group):
+    """Large queries with small keys and the other way round: ordinary scores."""
+    gen = torch.Generator().manual_seed(9)
+    for up in (100, -100, 110):
+        q, k, v, table, lens, mask, _ = case(2, 2, group, T, 64, 16, (0, 90), None, BF16, "tree")
+        x = torch.randn(2, 2, 2, T, 64, generator=gen)
+        lens = torch.zeros_like(lens)  # only these keys
+        b2.b200_cache_append((x[0] * 2.0 ** -up).to(DEV), x[1].to(DEV), k, v, table, lens)
+        args = ((q.float() * 2.0 ** up).to(BF16).contiguous(), k, v, table, lens, mask)
+        check(b2.b200_tree_attention(*args), *args)
+        check_device_errors(DEV)

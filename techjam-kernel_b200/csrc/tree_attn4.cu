@@ -497,8 +497,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
             grew |= top[nt][e] > m[nt][e] + 4.f;
           }
         if (__any_sync(0xffffffffu, grew)) {
-          // Largest steps of the lane's keys' values (16 h + 8 y + r8); a NaN counts as nothing.
-          uint32_t big_of[S::kParts][2];
+          // Largest steps among the lane's keys (16 h + 8 y + r8) that each of its rows sees: a value
+          // that a row does not see is not to cost it bits.  A NaN counts as nothing.
+          uint32_t step[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) step[nt][e] = 264u - (__float_as_uint(step_up[nt][e]) >> 23);
 #pragma unroll
           for (int h = 0; h < S::kParts; ++h)
 #pragma unroll
@@ -509,31 +514,28 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
                 const uint32_t one = (x < 2 ? u.x : u.y) >> 16 * (x & 1) & 0xffffu;
-                most = max(most, (one & 0x7fffu) > 0x7f80u ? 0u : one);
+                most = max(most, (one & 0x7fffu) > 0x7f80u ? 0u : one >> 7);
               }
-              big_of[h][y] = most >> 7;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (s[h][nt][2 * y + e] > -INFINITY) step[nt][e] = max(step[nt][e], most);
             }
           uint32_t least = 255u;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float f[2], d[2][2];
+            float f[2], d[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int z = 4; z < 32; z <<= 1)
+                step[nt][e] = max(step[nt][e], __shfl_xor_sync(0xffffffffu, step[nt][e], z));
+              // 2^(the step before - this one): by 2^-126 nothing is left of a sum either
+              const uint32_t less_by = step[nt][e] - (264u - (__float_as_uint(step_up[nt][e]) >> 23));
+              d[e] = __uint_as_float((127u - min(less_by, 126u)) << 23);
+              step_up[nt][e] = __uint_as_float((264u - step[nt][e]) << 23);
               float x = top[nt][e];
-              // of the keys that the row sees: a value that it does not see is not to cost it bits
-              const uint32_t was = 264u - (__float_as_uint(step_up[nt][e]) >> 23);
-              uint32_t step = was;
-#pragma unroll
-              for (int h = 0; h < S::kParts; ++h)
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-                  if (s[h][nt][2 * y + e] > -INFINITY) step = max(step, big_of[h][y]);
-#pragma unroll
-              for (int z = 4; z < 32; z <<= 1) step = max(step, __shfl_xor_sync(0xffffffffu, step, z));
-              step_up[nt][e] = __uint_as_float((264u - step) << 23);
-              // 2^(was - step), in two factors: they may lie 254 apart
-              d[e][0] = __uint_as_float((127u - (step - was) / 2) << 23);
-              d[e][1] = __uint_as_float((127u - (step - was + 1) / 2) << 23);
 #pragma unroll
               for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
               const float now = fmaxf(m[nt][e], x);
@@ -546,13 +548,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
               ol[nt][g].x *= f[0];
               ol[nt][g].y *= f[1];
             }
+            f[0] *= d[0];
+            f[1] *= d[1];
 #pragma unroll
             for (int x = 0; x < 2 * NG; ++x)
 #pragma unroll
-              for (int y = 0; y < 4; ++y) o[nt][x][y] = o[nt][x][y] * (f[y & 1] * d[y & 1][0]) * d[y & 1][1];
+              for (int y = 0; y < 4; ++y) o[nt][x][y] *= f[y & 1];
 #pragma unroll
             for (int e = 0; e < 2; ++e)  // a row that has seen no key takes its first later
-              if (m[nt][e] > -INFINITY) least = min(least, 264u - (__float_as_uint(step_up[nt][e]) >> 23));
+              if (m[nt][e] > -INFINITY) least = min(least, step[nt][e]);
           }
           most_step = __reduce_min_sync(0xffffffffu, least) << 7 | 0x7fu;
         }

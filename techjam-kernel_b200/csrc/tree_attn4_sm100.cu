@@ -42,6 +42,7 @@ constexpr int kThreads = 640;
 constexpr int kSoftmaxThreads = 256;
 constexpr int kLoadWarp = 8, kQkWarp = 9, kPvWarp = 10, kPlanWarp = 11;
 constexpr int kCodeWarp = 12, kCodeWarps = 8;
+constexpr float kGrowth = 8.f;   // a maximum is followed when a score is over 2^8 times its weight
 constexpr int kAhead = 4;        // segments that are planned ahead
 constexpr int kReaders = 19;     // warps that go through the segments
 
@@ -447,9 +448,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kTile / 16; ++kk)
-              ptx::tc_mma_ts(tmem + S::kColO + DP * i, tmem + kTile * i + kk * 8,
-                             vd + kk * (2048 >> 4), id, (((begun >> i) & 1u) || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < kTile / 16; ++kk) {
+              // 32 keys' weights lie over their scores: 16 columns rounded, 16 of what that left
+              const uint32_t w = tmem + kTile * i + 32 * (kk >> 1) + 8 * (kk & 1);
+              ptx::tc_mma_ts(tmem + S::kColO + DP * i, w, vd + kk * (2048 >> 4), id,
+                             (((begun >> i) & 1u) || kk > 0) ? 1u : 0u);
+              ptx::tc_mma_ts(tmem + S::kColO + DP * i, w + 16, vd + kk * (2048 >> 4), id, 1u);
+            }
             ptx::tc_commit(bar(S::kBarSums + i));
           }
           __syncwarp();
@@ -687,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 max3(top[(k >> 1) & 1], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
           mx = fmaxf(mx, fmaxf(top[0], top[1]) * to_log2(c));
         }
-        const bool resc = mx > m_run + kRescale || (m_run == -INFINITY && mx > m_run);
+        const bool resc = mx > m_run + kGrowth || (m_run == -INFINITY && mx > m_run);
         const float m_new = resc ? mx : m_run;
         const float alpha = resc ? ptx::ex2_approx(m_run - m_new) : 1.f;
         m_run = m_new;
@@ -715,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          uint32_t sr[32], pk[16];
+          uint32_t sr[32], hi[16], lo[16];
           ptx::tmem_ld_32x32b_x32(tS + 32 * c, sr);
           ptx::tmem_wait_ld();
           if (partly) drafted(sr, c);
@@ -726,12 +731,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             fma2(x, y, __uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1]), up, neg);
             x = ptx::ex2_approx(x);
             y = ptx::ex2_approx(y);
-            pk[e] = pack2<DT>(x, y);
-            // the sum is taken of the rounded weights, which the product uses
-            const float2 r = unpack2<DT>(pk[e]);
-            add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], r.x, r.y);
+            add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], x, y);
+            hi[e] = pack2<DT>(x, y);
+            const float2 r = unpack2<DT>(hi[e]);
+            lo[e] = pack2<DT>(x - r.x, y - r.y);
           }
-          st_x16(tS + 16 * c, pk);
+          st_x16(tS + 32 * c, hi);
+          st_x16(tS + 32 * c + 16, lo);
         }
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         ptx::tmem_wait_st();

@@ -62,7 +62,7 @@ B200_ATTN_API int32_t b200_cache4_read(const b200_cache* c, int64_t head_dim, in
  * More rows with bf16 queries, heads / kv_heads up to 128, and no mask or up to 64 tokens: keys
  * are rounded to fp16 numbers times a power of two of the 32 committed keys that they are among
  * (what is below 2^-38 of their largest number is lost), or of a key alone where drafted ones
- * are near, values and weights to bf16, and the sum is of the rounded weights.
+ * are near, and values to bf16; a weight is the sum of two bf16 numbers.
  */
 B200_ATTN_API int32_t b200_cache4_attn_check(const b200_tree_attn_params* p, int64_t head_dim,
                                              int32_t dtype);

@@ -172,7 +172,7 @@ def b200_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     applied in fp32; a weight times the step of its value is rounded to fp16 for the product
     with the codes (relative to the largest such step), the sum of weights is not.  With
     bfloat16 queries and more than 16 rows (``T * H / kv_heads``) keys are rounded to fp16
-    relative to the largest of 32, values and weights to bfloat16.  Returns
+    relative to the largest of 32, values to bfloat16.  Returns
     ``[B, H, T, D]``, or ``[B, T, H, D]`` with ``output_bshd``; ``out`` may supply it; it
     may be ``q`` itself, and shares no memory with another argument."""
     return _call("tree_attention", q.device, q, k_pages, v_pages, page_table, seq_lens, tree_mask,

@@ -26,7 +26,7 @@
 // lie in one page.  Bound by the issue of instructions and their latency, with HBM at half of its
 // rate: a block of 32 keys of 8 rows takes 690 instructions of a warp, of them 170 for the
 // scores, 260 for the values and 60 for its copies (64 sequences of up to 8191 keys, 8 key heads x 4, D
-// 128: 102 us, 51 us of bytes).  Four CTAs an SM where up to 8 rows leave the registers for it (64
+// 128: 104 us, 51 us of bytes).  Four CTAs an SM where up to 8 rows leave the registers for it (64
 // sequences of 250 keys: 22.3 us, with two 25.5).
 #include <cuda_runtime.h>
 
@@ -793,9 +793,9 @@ static_assert(AnyShape::kTile == Shape4<true, 64>::kTile && AnyShape::RM == Shap
 
 // Up to so many rows a key head the kernel of matrix instructions of a warp, whose time grows
 // with each 16 rows; the tcgen05 kernel takes as long for 16 as for 128.  Measured, this kernel
-// and that one (8 key heads x 4, D 128, pages of 64, us): 131001 keys, 16 rows 81 and 126, 20 rows 129 and
-// 131, 64 rows 230 and 133; 16 sequences of 1001 to 8100 keys 62 and 89, 93 and 91, 170 and 93; 64
-// sequences of 500 to 2000 keys 78 and 111, 126 and 113, 250 and 115.
+// and that one (8 key heads x 4, D 128, pages of 64, us): 131001 keys, 16 rows 82 and 136, 32 rows 130 and
+// 139, 64 rows 233 and 140; 16 sequences of 1001 to 8100 keys 63 and 95, 100 and 97, 175 and 97; 64
+// sequences of 500 to 2000 keys 79 and 118, 139 and 120, 261 and 124.
 constexpr int64_t kFewRows4 = 16;
 
 int64_t rows_of(const b200_tree_attn_params* p) { return p->tokens * (p->heads / p->cache.kv_heads); }

@@ -9,21 +9,22 @@
 // queries; here it is once for up to 256.
 // Keys become fp16 numbers, as the queries do, each times a power of two, of the row of the
 // queries and of 32 keys (of a key alone in tiles that hold drafted ones, which a row may not see),
-// that the scores are rid of again: rounded to 11 bits, they leave the scores as exact as the
-// weights' own rounding.  Values and weights are bf16: whatever
-// the size of a value, it fits.
+// that the scores are rid of again: rounded to 11 bits, they cost a weight less than the values'
+// rounding does.  Values are bf16: whatever the size of one, it fits.  A weight is two bf16 numbers, the
+// second what rounding left, over the scores of its keys: one alone made the error against 64 bits 1.48
+// times that of a rounded output instead of 1.36, for 4 % of the time.
 // Each softmax group has scores of its own, over which its weights come to lie, and reads them
 // twice, 32 at a time: with a row of 128 scores in registers there were none for a second
 // warp of decoders on each scheduler, and code of four times the size kept all roles waiting
 // for instructions (16 sequences, 128 rows: 188 us where this form took 140).
 //
 // Bound by latency along the chain codes -> operands -> scores -> weights -> sums, at half of the
-// issue rate and a fifth of the tensor pipe: 16 sequences of 1001 to 8100 keys, 128 rows, 8 key heads, D
-// 128: 95 us, 131001 keys and 64 rows 133 us (23 and 26 us of bytes).  Slower on the same two
-// cases: one pass over the scores with the maximum followed a quarter at a time (108 and 145), 16 scores
-// at a time with the next 16 on their way (109 and 154), a load warp more (80 registers a
-// thread: 105 and 146), decoding loops unrolled twice (104 and 141), keys and values
-// decoded on two schedulers each (101 and 139).
+// issue rate and a third of the tensor pipe: 16 sequences of 1001 to 8100 keys, 128 rows, 8 key heads, D
+// 128: 99 us, 131001 keys and 64 rows 140 us (23 and 26 us of bytes).  Slower, with one
+// number a weight, where this form took 95 and 133: one pass over the scores with the maximum followed a
+// quarter at a time (108 and 145), 16 scores at a time with the next 16 on their way (109 and
+// 154), a load warp more (80 registers a thread: 105 and 146), decoding loops unrolled twice (104 and
+// 141), keys and values decoded on two schedulers each (101 and 139).
 #include <cuda_runtime.h>
 
 #include <cstdint>

@@ -71,6 +71,16 @@ B200_ATTN_API int64_t b200_cache4_attn_workspace_bytes(const b200_tree_attn_para
 B200_ATTN_API int32_t b200_cache4_attn_fwd(const b200_tree_attn_params* p, int64_t head_dim,
                                            int32_t dtype, void* stream);
 
+/* Self-test of failure detection.  Launches the attention kernel of more than 16 rows like
+ * b200_cache4_attn_fwd (without the join of the units that were cut), except that in every CTA a copy
+ * of key tile number `skipped_tile` (0: its first) is announced to its barrier but never issued.
+ * The wait on it runs out after a second: the kernel ORs B200_ATTN_DEVERR_WAIT_TIMEOUT into the
+ * error word, waits (bounded) for its own copies and products, frees its tensor memory and returns,
+ * leaving the CUDA context usable.  For bf16, head_dim over 64, calls that take that kernel, and a
+ * non-null error_word (B200_ATTN_ERR_UNSUPPORTED otherwise).  The output is undefined. */
+B200_ATTN_API int32_t b200_cache4_selftest_stall(const b200_tree_attn_params* p, int64_t head_dim,
+                                                 int32_t dtype, int32_t skipped_tile, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

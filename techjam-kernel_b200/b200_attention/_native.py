@@ -91,6 +91,7 @@ CACHE4_SYMBOLS = (
     "b200_cache4_attn_check",
     "b200_cache4_attn_workspace_bytes",
     "b200_cache4_attn_fwd",
+    "b200_cache4_selftest_stall",
 )
 
 # Every symbol ``include/b200_verify.h`` declares.
@@ -370,6 +371,7 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
             ("b200_cache4_attn_check", i32, [tree, i64, i32]),
             ("b200_cache4_attn_workspace_bytes", i64, [tree, i64, i32]),
             ("b200_cache4_attn_fwd", i32, [tree, i64, i32, ptr]),
+            ("b200_cache4_selftest_stall", i32, [tree, i64, i32, i32, ptr]),
             ("b200_verify_check", i32, [ctypes.POINTER(VerifyParams)]),
             ("b200_verify_drafts", i32, [ctypes.POINTER(VerifyParams), ptr])):
         getattr(lib, name).restype = result

@@ -904,36 +904,70 @@ extern "C" int64_t b200_cache4_attn_workspace_bytes(const b200_tree_attn_params*
   return round16(8 * units_of(p, ch)) + 2 * runs_of(p, ch, kMaxSms) * 4 * ch.rm * (dp + 2);
 }
 
-extern "C" int32_t b200_cache4_attn_fwd(const b200_tree_attn_params* p, int64_t head_dim,
-                                        int32_t dtype, void* stream) {
+namespace {
+
+// What both entry points do: checks, and the arguments of the kernels.
+struct Prepared {
+  b200paged::DeviceScope scope;
+  Args a{};
+  Choice4 ch{};
+  int64_t units = 0;
+  int runs = 0;
+  bool spread = false;
+};
+
+int32_t prepare(const b200_tree_attn_params* p, int64_t head_dim, int32_t dtype, Prepared* r) {
   int32_t rc = b200_cache4_attn_check(p, head_dim, dtype);
   if (rc != B200_ATTN_OK) return rc;
   if (!p->workspace || p->workspace_bytes < b200_cache4_attn_workspace_bytes(p, head_dim, dtype))
     return B200_ATTN_ERR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(p->workspace) & 15u) return B200_ATTN_ERR_ALIGNMENT;
-  b200paged::DeviceScope scope;
-  if ((rc = scope.enter(p->q, "q is not a device pointer")) != B200_ATTN_OK) return rc;
-  Args a{};
+  if ((rc = r->scope.enter(p->q, "q is not a device pointer")) != B200_ATTN_OK) return rc;
+  Args& a = r->a;
   if ((rc = b200attn::resolve_error_word(p->cache.error_word, &a.err)) != B200_ATTN_OK) return rc;
   fill_args(p, 2, 2, head_dim, &a);
-  const Choice4 ch = choose(p, dtype);
+  const Choice4 ch = r->ch = choose(p, dtype);
   a.unit_rows = ch.rows;
   a.row_tiles = static_cast<int32_t>(row_tiles(p, ch));
   a.scale_log2 = p->scale * 1.4426950408889634f;
-  const int64_t units = units_of(p, ch);
+  r->units = units_of(p, ch);
   a.desc = static_cast<int2*>(p->workspace);
-  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + round16(8 * units));
-  const int runs = static_cast<int>(runs_of(p, ch, b200paged::sm_count(scope.device)));
-  a.runs = runs;
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + round16(8 * r->units));
+  r->runs = static_cast<int>(runs_of(p, ch, b200paged::sm_count(r->scope.device)));
+  a.runs = r->runs;
   // as for caches of 16 bits: long contexts of several rows are joined by a kernel of their own
-  const bool spread = rows_of(p) > 4 && p->cache.slots * p->cache.page_size >= 12 * ch.tn &&
-                      runs >= 8 * units;
-  if (!ch.many && !spread && units <= B200_TREE_ATTN_COUNTERS) a.counters = p->counters;
+  r->spread = rows_of(p) > 4 && p->cache.slots * p->cache.page_size >= 12 * ch.tn &&
+              r->runs >= 8 * r->units;
+  if (!ch.many && !r->spread && r->units <= B200_TREE_ATTN_COUNTERS) a.counters = p->counters;
+  return B200_ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t b200_cache4_attn_fwd(const b200_tree_attn_params* p, int64_t head_dim,
+                                        int32_t dtype, void* stream) {
+  Prepared r;
+  const int32_t rc = prepare(p, head_dim, dtype, &r);
+  if (rc != B200_ATTN_OK) return rc;
+  const int device = r.scope.device;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = head_dim > 64;
   if (dtype == B200_ATTN_DTYPE_BF16)
-    return wide ? run_width<128, B200_ATTN_DTYPE_BF16>(ch, a, runs, units, spread, scope.device, s)
-                : run_width<64, B200_ATTN_DTYPE_BF16>(ch, a, runs, units, spread, scope.device, s);
-  return wide ? run_width<128, B200_ATTN_DTYPE_FP16>(ch, a, runs, units, spread, scope.device, s)
-              : run_width<64, B200_ATTN_DTYPE_FP16>(ch, a, runs, units, spread, scope.device, s);
+    return wide ? run_width<128, B200_ATTN_DTYPE_BF16>(r.ch, r.a, r.runs, r.units, r.spread, device, s)
+                : run_width<64, B200_ATTN_DTYPE_BF16>(r.ch, r.a, r.runs, r.units, r.spread, device, s);
+  return wide ? run_width<128, B200_ATTN_DTYPE_FP16>(r.ch, r.a, r.runs, r.units, r.spread, device, s)
+              : run_width<64, B200_ATTN_DTYPE_FP16>(r.ch, r.a, r.runs, r.units, r.spread, device, s);
+}
+
+extern "C" int32_t b200_cache4_selftest_stall(const b200_tree_attn_params* p, int64_t head_dim,
+                                              int32_t dtype, int32_t skipped_tile, void* stream) {
+  if (!p || dtype != B200_ATTN_DTYPE_BF16 || head_dim <= 64 || head_dim > 128 ||
+      !p->cache.error_word || skipped_tile < 0)
+    return B200_ATTN_ERR_UNSUPPORTED;
+  Prepared r;
+  const int32_t rc = prepare(p, head_dim, dtype, &r);
+  if (rc != B200_ATTN_OK) return rc;
+  if (!r.ch.many) return B200_ATTN_ERR_UNSUPPORTED;
+  return launch_coded_stall(r.ch.rm, r.a, r.runs, r.scope.device, static_cast<cudaStream_t>(stream),
+                            skipped_tile);
 }

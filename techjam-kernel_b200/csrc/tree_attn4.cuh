@@ -49,5 +49,7 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const uint8_t* src, uint
 
 // Host side of tree_attn4_sm100.cu: row tiles of 128 or 256 rows, bf16 queries.
 int32_t launch_coded(int rm, int dp, const Args& a, int runs, int device, cudaStream_t s);
+// The same for the stall self-test, head dims over 64.
+int32_t launch_coded_stall(int rm, const Args& a, int runs, int device, cudaStream_t s, int32_t skip);
 
 }  // namespace b200tree

@@ -177,9 +177,10 @@ __device__ __forceinline__ void values(const uint8_t* row, const __nv_bfloat162 
   }
 }
 
-template <class S>
+// kStall: the stall self-test's instance, which leaves out a copy of tile number `skip` of each CTA.
+template <class S, bool kStall>
 __global__ void __launch_bounds__(kThreads, 1)
-    coded_kernel(const __grid_constant__ Args a, const int32_t box_rows) {
+    coded_kernel(const __grid_constant__ Args a, const int32_t box_rows, const int32_t skip) {
   constexpr int DP = S::DP, NS = S::kSlots, RM = S::RM, DT = B200_ATTN_DTYPE_BF16;
   constexpr bool kTwo = S::kTwo;
   extern __shared__ uint8_t raw[];
@@ -322,7 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t bytes = n * S::kRawRow;
         expect_tx(fk, bytes);
         expect_tx(fv, bytes);
-        bulk_copy(sbase + at_k + key * S::kRawRow, kb + page * a.k_page + in * a.k_row, bytes, fk);
+        if (!(kStall && u == 0 && static_cast<int>(tiles) == skip))
+          bulk_copy(sbase + at_k + key * S::kRawRow, kb + page * a.k_page + in * a.k_row, bytes, fk);
         bulk_copy(sbase + at_v + key * S::kRawRow, vb + page * a.v_page + in * a.v_row, bytes, fv);
       }
       __syncwarp();
@@ -333,13 +335,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (++rk == S::kRawK) rk = 0, pk ^= 1u;
       if (++rv == S::kRawV) rv = 0, pv ^= 1u;
     }
-    if (!ok) {
-      // copies in flight land before the shared memory goes
-      for (uint32_t x = tiles > S::kRawK ? tiles - S::kRawK : 0u; x < tiles; ++x)
-        settle(bar(S::kBarRawFull + x % S::kRawK), (x / S::kRawK) & 1u);
-      for (uint32_t x = tiles > S::kRawV ? tiles - S::kRawV : 0u; x < tiles; ++x)
-        settle(bar(S::kBarRawFull + S::kRawK + x % S::kRawV), (x / S::kRawV) & 1u);
-    }
+    // Copies in flight land before the shared memory goes, also where this warp had issued its last
+    // when another's wait ran out, or found no further segment because of it.
+    for (uint32_t x = tiles > S::kRawK ? tiles - S::kRawK : 0u; x < tiles; ++x)
+      settle(bar(S::kBarRawFull + x % S::kRawK), (x / S::kRawK) & 1u);
+    for (uint32_t x = tiles > S::kRawV ? tiles - S::kRawV : 0u; x < tiles; ++x)
+      settle(bar(S::kBarRawFull + S::kRawK + x % S::kRawV), (x / S::kRawV) & 1u);
     __syncwarp();
   } else if (warp == kQkWarp) {
     // -------------------------------------------------- scores S = Q K^T
@@ -626,7 +627,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int* unit = plan;
     Segment begin;
 #pragma unroll 1
-    for (; ok && segment(seg, &begin); ++seg) {
+    for (;; ++seg) {
+      if (!segment(seg, &begin)) {
+        // Where a wait ran out some of the warps can have the segment and others not: each comes to the
+        // barrier below once a segment, the one that none has included, or those that have it would wait
+        // for the others for good.
+        if constexpr (!kTwo) ptx::named_barrier_and(1, kSoftmaxThreads, false);
+        break;
+      }
       unit = plan + 8 * (seg % kAhead);
       const int n = begin.n, rows = unit_rows(begin), t0 = begin.t, len = begin.len;
       const bool idle = row0 + quad * 32 >= rows || quad * 32 >= share;  // padding rows only
@@ -854,35 +862,47 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // -------------------------------------------------------------------- host
-template <class S>
-int32_t launch_coded_shape(const Args& a, int box_rows, int runs, int device, cudaStream_t s) {
+template <class S, bool kStall = false>
+int32_t launch_coded_shape(const Args& a, int box_rows, int runs, int device, cudaStream_t s,
+                           int32_t skip = -1) {
   using namespace b200paged;
   static std::once_flag once[kMaxDevices];
   static cudaError_t err[kMaxDevices];
   std::call_once(once[device], [&] {
-    err[device] = cudaFuncSetAttribute(coded_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       S::kSmemBytes);
+    err[device] = cudaFuncSetAttribute(coded_kernel<S, kStall>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
   });
   if (err[device] != cudaSuccess) {
     set_error(cudaGetErrorString(err[device]));
     return B200_ATTN_ERR_LAUNCH;
   }
-  return launch(coded_kernel<S>, dim3(runs), dim3(kThreads), S::kSmemBytes, s, a, box_rows);
+  return launch(coded_kernel<S, kStall>, dim3(runs), dim3(kThreads), S::kSmemBytes, s, a, box_rows, skip);
+}
+
+// Rows that lie side by side and in one page, whatever the place of the first.
+int box_of(int dp, const Args& a) {
+  const int row = dp / 2 + 16;
+  int box = 1;
+  if (a.k_row == row && a.v_row == row)
+    while (box < kTile && a.page_size % (2 * box) == 0) box *= 2;
+  return box;
 }
 
 }  // namespace
 
 int32_t launch_coded(int rm, int dp, const Args& a, int runs, int device, cudaStream_t s) {
-  // rows that lie side by side and in one page, whatever the place of the first
-  const int row = dp / 2 + 16;
-  int box = 1;
-  if (a.k_row == row && a.v_row == row)
-    while (box < kTile && a.page_size % (2 * box) == 0) box *= 2;
+  const int box = box_of(dp, a);
   if (rm == 256)
     return dp == 64 ? launch_coded_shape<CodedShape<64, true>>(a, box, runs, device, s)
                     : launch_coded_shape<CodedShape<128, true>>(a, box, runs, device, s);
   return dp == 64 ? launch_coded_shape<CodedShape<64, false>>(a, box, runs, device, s)
                   : launch_coded_shape<CodedShape<128, false>>(a, box, runs, device, s);
+}
+
+int32_t launch_coded_stall(int rm, const Args& a, int runs, int device, cudaStream_t s, int32_t skip) {
+  const int box = box_of(128, a);
+  return rm == 256 ? launch_coded_shape<CodedShape<128, true>, true>(a, box, runs, device, s, skip)
+                   : launch_coded_shape<CodedShape<128, false>, true>(a, box, runs, device, s, skip);
 }
 
 }  // namespace b200tree

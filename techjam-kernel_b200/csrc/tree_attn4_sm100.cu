@@ -102,6 +102,15 @@ __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
                : "memory");
 }
 
+// (x, y) times (a, b) m, two lanes an instruction.
+__device__ __forceinline__ void scale2(uint32_t& x, uint32_t& y, float a, float b, float m) {
+  asm("{\n\t.reg .b64 p, q, r;\n\t"
+      "mov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %4};\n\tmov.b64 r, {%0, %1};\n\t"
+      "mul.rn.f32x2 p, p, q;\n\tmul.rn.f32x2 r, r, p;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "+r"(x), "+r"(y)
+      : "f"(a), "f"(b), "f"(m));
+}
+
 // The lowest n bits.
 __device__ __forceinline__ uint32_t first_bits(int n) {
   return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           put(S::kOffQ + i * S::kTileBytes, x, make_uint4(w[0], w[1], w[2], w[3]));
         }
         row_scale[(seg % kAhead) * RM + i * kTile + row] =
-            a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
+            __uint_as_float(static_cast<uint32_t>(e - 13) << 23);
       }
       hand_over(S::kBarQ);
     };
@@ -657,13 +666,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // from the products' unit to that of the exponents, for the keys of each of four warps
         const float* ks = key_scale + ((tile0 + j) & 7u) * 4;
-        const float rs = row_scale[(seg % kAhead) * RM + (kTwo ? i * kTile : 0) + rl];
+        const float* pow_r = row_scale + (seg % kAhead) * RM + (kTwo ? i * kTile : 0) + rl;
+        float rs = a.scale_log2 * *pow_r;
         // a bit for each of 32 keys that this row sees
         uint64_t bits = 0u;
         int tok = 0;
         if (partly) {
           tok = min((unit[2] * a.unit_rows + row0 + rl) / a.group, a.tokens - 1);
           if (a.tokens <= kSeen) bits = seen[(seg % kAhead) * kSeen + tok];
+          rs = a.scale_log2 * fmaxf(*pow_r * 0x1p-13f, 1.f);
         }
         auto visible = [&](int c) {
           const int d = k0 + 32 * c - len;
@@ -672,15 +683,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           return d >= 64 ? 0u
                          : static_cast<uint32_t>(d < 0 ? bits << -d | ((1u << -d) - 1u) : bits >> d);
         };
+        // A key's own power of two (up to 2^114) and the row's act as one factor: a score times the
+        // key's alone would pass the range where the row's numbers are next to nothing.  What of the
+        // row's is over 2^13 waits for the scale, so that the factor is finite.
         auto drafted = [&](uint32_t (&sr)[32], int c) {
+          const float near = fminf(*pow_r, 0x1p13f);
           const float4* f = reinterpret_cast<const float4*>(own_scale + ((tile0 + j) & 7u) * kTile + 32 * c);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float4 x = f[k];
-            sr[4 * k] = __float_as_uint(__uint_as_float(sr[4 * k]) * x.x);
-            sr[4 * k + 1] = __float_as_uint(__uint_as_float(sr[4 * k + 1]) * x.y);
-            sr[4 * k + 2] = __float_as_uint(__uint_as_float(sr[4 * k + 2]) * x.z);
-            sr[4 * k + 3] = __float_as_uint(__uint_as_float(sr[4 * k + 3]) * x.w);
+            scale2(sr[4 * k], sr[4 * k + 1], x.x, x.y, near);
+            scale2(sr[4 * k + 2], sr[4 * k + 3], x.z, x.w, near);
           }
           hide(sr, visible(c));
         };

@@ -196,9 +196,13 @@ class Decoder(nn.Module):
                   pages: Optional[int] = None, bits: Optional[int] = None) -> PagedKVCache:
         """An empty paged cache for ``batch`` sequences of up to ``max_tokens`` committed
         and drafted tokens (``pages`` in the pool; by default enough for all of them), of the
-        model's type, or with ``bits=4`` held in 4 bits."""
+        model's type, or with ``bits=4`` held in 4 bits (bfloat16 and float16 models: the attention
+        over such a cache takes no others)."""
         slots = -(-max_tokens // page_size)
         weight = self.final_norm.weight
+        if bits == 4 and weight.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError("attention over a 4-bit cache takes bfloat16 or float16 queries, the "
+                            f"model is {weight.dtype}")
         return PagedKVCache(self.config.num_layers, pages if pages is not None else batch * slots,
                             self.config.num_heads, page_size,
                             self.config.d_model // self.config.num_heads, batch, slots,

@@ -11,9 +11,10 @@
  *          where it is not 0,
  *   code = (x - low) / step rounded to the nearest whole number, ties to even, 0..15,
  * and the row stands for low + step * code: nothing is clipped, and a number is off by half
- * a step at most.  A group that holds an infinity or NaN, or whose step would not be
- * finite, stands for NaN (step and low NaN, codes 0); a group past head_dim has step, low
- * and codes 0.  The row is P / 2 bytes of codes, four bf16 steps, four bf16 lows: 48 or 80
+ * a step at most.  A group that holds an infinity or NaN stands for NaN (step and low NaN,
+ * codes 0), and so does one whose largest - low is past the largest fp32 number: fifteen of
+ * its steps would be no fp32 number, in which the attention adds them to low.  A group past
+ * head_dim has step, low and codes 0.  The row is P / 2 bytes of codes, four bf16 steps, four bf16 lows: 48 or 80
  * bytes.  Half bytes are counted from the low half of byte 0.  Number e of group g of a row
  * of keys lies in half byte
  *   P = 128:  32 (e / 8) + 8 g       + 2 (e % 8 / 4) + e % 4 / 2 + 4 (e % 2)

@@ -77,7 +77,8 @@ def b200_cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.T
     of a vector padded to 64 or 128 has a ``low``, the bfloat16 number at or below its smallest, a
     ``step``, that at or above a fifteenth of the way from it to the largest, and codes
     ``(x - low) / step`` rounded to nearest, ties to even.  A number is off by half a step at
-    most; a group that holds an infinity or NaN reads as NaN."""
+    most; a group that holds an infinity or NaN, or whose numbers lie further apart than the
+    largest float32, reads as NaN."""
     _call("cache_append", k_pages.device, k_new, v_new, k_pages, v_pages, page_table, seq_lens,
           draft_lens)
 

@@ -118,8 +118,8 @@ __device__ __forceinline__ float2 difference(float a, float b) {
   return make_float2(d, (x - b) + (a - (d + x)));
 }
 
-// The bf16 number at or above a fifteenth of span.x + span.y >= 0.  The quotient is rounded, so its
-// neighbours are looked at too: 15 times a bf16 number is exact.
+// The bf16 number at or above a fifteenth of span.x + span.y >= 0; infinity where the span passes fp32.
+// The quotient is rounded, so its neighbours are looked at too: 15 times a bf16 number is exact.
 __device__ __forceinline__ float step_of(float2 span) {
   auto enough = [&](uint32_t bits) {
     const float c = 15.f * __uint_as_float(bits);

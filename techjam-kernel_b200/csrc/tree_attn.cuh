@@ -24,12 +24,6 @@
 #include "error_word.cuh"
 #include "sm100_ptx.cuh"
 
-// Parts that run once a unit are calls, but in a kernel that moves registers between its warps,
-// which cannot have any.
-#ifndef B200_TREE_CALL
-#define B200_TREE_CALL __noinline__
-#endif
-
 namespace b200tree {
 
 using b200attn::report_error;
@@ -127,7 +121,7 @@ __device__ __forceinline__ void enter_seq(const Args& a, Place& p) {
 // once a unit: with them in line at each use the kernels were up to 188 KB of code, and
 // fetching the instructions of what runs seldom took longer than its work.
 template <class G>
-__device__ B200_TREE_CALL Place next_unit(const Args& a, Place p) {
+__device__ __noinline__ Place next_unit(const Args& a, Place p) {
   p.t = 0;
   if (++p.rt < p.rts) return p;
   p.rt = 0;
@@ -210,7 +204,7 @@ __device__ __forceinline__ void put_place(const Args& a, const Cuts& cuts, bool 
 // first place and the next run's walk to them.  `sums`: scratch of one value a warp.
 // Ends with a barrier; *out is in shared memory.
 template <class G>
-__device__ B200_TREE_CALL void find_run(const Args& a, uint32_t run, uint32_t ctas, uint32_t* sums,
+__device__ __noinline__ void find_run(const Args& a, uint32_t run, uint32_t ctas, uint32_t* sums,
                                       Run* out) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const bool one = a.batch <= 32;  // a lane a sequence: one warp finds the run by itself
@@ -271,7 +265,7 @@ __device__ B200_TREE_CALL void find_run(const Args& a, uint32_t run, uint32_t ct
 // The drafted tokens i >= n_b of the sequences that this CTA looks after get
 // zero rows (sequences without drafted tokens have no unit at all).
 // `threads`: the first threads of the CTA, which call this.
-static __device__ B200_TREE_CALL void zero_unused_rows(const Args& a, int elem_bytes, int threads) {
+static __device__ __noinline__ void zero_unused_rows(const Args& a, int elem_bytes, int threads) {
   const int heads = a.kv_heads * a.group;
   const int pieces = a.head_dim * elem_bytes / 16;
 #pragma unroll 1
@@ -297,7 +291,7 @@ __device__ __forceinline__ bool sees(const Args& a, int b, int i, int j) {
 // draft.  Places before the draft are committed tokens, which it sees.  A row of
 // mask bytes is read as the aligned words that hold it, all at once: a byte at a
 // time, each waiting for its load, these reads took longer than the tile's products.
-static __device__ B200_TREE_CALL uint32_t seen_word(const Args& a, int b, int i, int d0, int drafts) {
+static __device__ __noinline__ uint32_t seen_word(const Args& a, int b, int i, int d0, int drafts) {
   uint32_t word = 0u;
   int n = drafts - d0;  // bits of the word that lie in the draft or before it
   if (!a.mask) {
@@ -358,7 +352,7 @@ struct Elem<B200_ATTN_DTYPE_FP32> {
 // values of drafted tokens d0..d1 that are not finite and that the row's token sees.
 // They were left out of the product, where a weight of zero would not hide them.
 template <int DT>
-__device__ B200_TREE_CALL void add_odd(const Args& a, int b, int h, Seq s, int tok, int d0, int d1,
+__device__ __noinline__ void add_odd(const Args& a, int b, int h, Seq s, int tok, int d0, int d1,
                                      int col0, int col1, uint16_t* out, float* part, int pitch) {
   using E = Elem<DT>;
   const uint32_t size = static_cast<uint32_t>(a.page_size);
@@ -433,7 +427,7 @@ struct JoinSmem {
 };
 
 template <int RM, int DP, int DT, int WARPS>
-__device__ B200_TREE_CALL void join_four(const Args& a, Joint j, JoinSmem<DP, WARPS>* sm) {
+__device__ __noinline__ void join_four(const Args& a, Joint j, JoinSmem<DP, WARPS>* sm) {
   using E = Elem<DT>;
   constexpr int kCols = DP / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -499,7 +493,7 @@ __device__ B200_TREE_CALL void join_four(const Args& a, Joint j, JoinSmem<DP, WA
 
 // More rows: each warp takes RM / WARPS of them over all runs, without shared memory.
 template <int RM, int DP, int DT, int WARPS>
-__device__ B200_TREE_CALL void join_many(const Args& a, Joint j) {
+__device__ __noinline__ void join_many(const Args& a, Joint j) {
   using E = Elem<DT>;
   constexpr int kCols = DP / 32, kN = RM / WARPS;
   const int lane = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * kN;
@@ -577,7 +571,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 // The same within the kernel that left the partial results: the last of a unit's runs to
 // arrive joins them all.  By all threads of a CTA, after it has written its own.
 template <int RM, int DP, int DT, int WARPS>
-__device__ B200_TREE_CALL void join_if_last(const Args& a, int b, int h, int rt, int rows, int first,
+__device__ __noinline__ void join_if_last(const Args& a, int b, int h, int rt, int rows, int first,
                                           int last, JoinSmem<DP, WARPS>* sm) {
   __threadfence();
   __syncthreads();

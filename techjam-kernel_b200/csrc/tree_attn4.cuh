@@ -12,7 +12,7 @@ namespace {
 // `pitch` apart) whose group is NaN in a drafted token that the row's token sees: such steps and
 // lows were left out of the products, where a weight of zero would not hide them.
 template <int DP, int DT>
-__device__ B200_TREE_CALL void add_odd4(const Args& a, int b, int h, Seq s, int tok, int d0, int d1,
+__device__ __noinline__ void add_odd4(const Args& a, int b, int h, Seq s, int tok, int d0, int d1,
                                       int col0, int col1, uint16_t* out, float* part,
                                       int pitch) {
   using E = Elem<DT>;

@@ -22,7 +22,7 @@ constexpr float kRescale = 1.0f;
 constexpr int kSeen = 64;  // tokens of a draft whose masks fit a word of 64 bits each
 constexpr int kIssuerSpin = 4096;  // polls of an issuer before its suspending wait
 
-__device__ B200_TREE_CALL bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
                                        int32_t* err) {
   const uint64_t t0 = ptx::globaltimer_ns();
   while (true) {

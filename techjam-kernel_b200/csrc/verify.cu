@@ -42,7 +42,6 @@ using b200tree::Elem;
 namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps, kMaxCluster = 16;
-constexpr int kMaxNodes = B200_VERIFY_MAX_NODES;
 constexpr uint32_t kAll = 0xffffffffu;
 
 struct Args {

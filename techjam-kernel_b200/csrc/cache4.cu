@@ -1,18 +1,19 @@
 // cache4.cu — append to and read from the paged cache held in 4 bits
 // (format: b200_cache4.h).
 //
-// A thread takes a group of a key or value vector, 16 or 32 numbers, so what is done once a group
-// (its ends, step and low) is shared by many numbers; the four threads of a vector exchange words to
-// write rows 8 or 16 bytes at a time.
+// append: a thread takes a group of a key or value vector, 16 or 32 numbers, so what is done once a
+// group (its ends, step and low) is shared by many numbers; the four threads of a vector exchange
+// words to write rows 8 or 16 bytes at a time.  read: a thread takes 8 numbers of a key and the same
+// 8 of the value.
 //
-// Bound by the issue of instructions: some ten a number where the bytes allow two.  33
-// thousand tokens of 8 heads of 128 bf16 numbers, keys and values: append 42 us, read 34 us, together
-// 37 us of bytes at the copy rate.  A thread a vector (80 us for append) kept 128 numbers in
-// registers, a warp a vector spent most of its time in shuffles.
-//
-// Bound by the issue of instructions.  33 thousand tokens of 8 heads of 128 bf16 numbers, keys and
-// values, in and back: 76 us (read 34 of them), 37 us of bytes at the copy rate; with a thread for 8
-// numbers, whose ends went through shuffles, and every code settled exactly: 177.
+// Bound by the issue of instructions.  16 prompts of up to 2048 tokens, 16 thousand in all, of 8 heads of
+// 128 bf16 numbers, keys and values: append 42 us, where its bytes take 13 at the copy rate, with 34
+// instructions a number and 76 % of the issue slots used; read, which writes the rows behind the
+// counts too, 34 us, bytes 24, 12 instructions a number and 74 %.  A lane of append
+// reads 64 bytes that lie together, so each 32-byte sector is asked for twice, the second time from
+// L1.  A thread for 8 numbers, whose group's ends went through shuffles, and every code settled
+// exactly: 177 us for both.  A thread a vector (append 80 us) kept 128 numbers in registers, a
+// warp a vector spent most of its time in shuffles.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -393,7 +394,7 @@ __device__ __noinline__ void store_sums(const uint8_t* kr, const uint8_t* vr, in
 }
 
 // A thread gives 8 numbers of a key and the same 8 of the value, so that neighbours write side by
-// side (a group a thread as above: 46 us against 34 us for 33 thousand tokens of 8 heads).
+// side (a group a thread as above: 46 us against 34 us for 33 thousand rows of 8 heads).
 template <int P, int DT>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ Call c) {
   b200attn::ptx::launch_dependents();

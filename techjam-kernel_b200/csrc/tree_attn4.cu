@@ -795,7 +795,9 @@ static_assert(AnyShape::kTile == Shape4<true, 64>::kTile && AnyShape::RM == Shap
 // with each 16 rows; the tcgen05 kernel takes as long for 16 as for 128.  Measured, this kernel
 // and that one (8 key heads x 4, D 128, pages of 64, us): 131001 keys, 16 rows 82 and 136, 32 rows 130 and
 // 139, 64 rows 233 and 140; 16 sequences of 1001 to 8100 keys 63 and 95, 100 and 97, 175 and 97; 64
-// sequences of 500 to 2000 keys 79 and 118, 139 and 120, 261 and 124.
+// sequences of 500 to 2000 keys 79 and 118, 139 and 120, 261 and 124.  (32 rows over one long context
+// would be 7 % faster here; the rule goes by the rows alone.)  fp16 queries of more rows, and masks of
+// more than 64 tokens, take this kernel all the same: the other has neither.
 constexpr int64_t kFewRows4 = 16;
 
 int64_t rows_of(const b200_tree_attn_params* p) { return p->tokens * (p->heads / p->cache.kv_heads); }
@@ -809,7 +811,8 @@ struct Choice4 {
 
 Choice4 choose(const b200_tree_attn_params* p, int32_t dtype) {
   const int64_t rows = rows_of(p), group = p->heads / p->cache.kv_heads;
-  // The tcgen05 kernel has bf16 values and weights, and masks of up to 64 tokens.
+  // The tcgen05 kernel has bf16 values and weights, too few bits for fp16 results, and masks of up
+  // to 64 tokens.
   if (rows > kFewRows4 && dtype == B200_ATTN_DTYPE_BF16 && group <= 128 && (p->tokens <= 64 || !p->mask)) {
     const int tile = static_cast<int>(128 / group * group);  // whole tokens to 128 places
     if (rows <= tile) return Choice4{true, 128, tile, 128, 1};

@@ -17,8 +17,10 @@
 // beforehand: e^(l / T) does not leave the range of 64 bits unless |l / T| is over 600, and such
 // a row is summed again relative to its maximum.
 //
-// Bound by 64-bit arithmetic and the exchange of a pass's sums: 64 sequences with trees of 16 nodes,
-// vocabulary 100003, take 132 us where the rows on the paths are 12 us of bytes; 64 chains of 8
+// Bound by the latency of passes that follow one another, each a wait for its row, a barrier of the
+// cluster and the next decision: 64 sequences with trees of 16 nodes, vocabulary 100003, take 130 us
+// where the rows on the paths are 12 us of bytes, with the issue slots half used, the 64-bit pipe a
+// fifth and L1 half (of rows that do not start on four numbers each number is a load); 64 chains of 8
 // nodes, vocabulary 32000, 43 us.  With a pass over the row for each refusal before (what is left
 // taken again step by step) those trees took 412 us, and with a maximum first the chains 51.
 #include <cuda_runtime.h>
@@ -700,9 +702,22 @@ extern "C" int32_t b200_verify_drafts(const b200_verify_params* p, void* stream)
   a.nodes = static_cast<int32_t>(p->nodes);
   a.vocab = static_cast<int32_t>(p->vocab);
   a.wide_tokens = p->wide_tokens;
-  // So many CTAs that four of them, with a row's exponentials, fit on an SM.  Vocabulary 100003,
-  // trees of 16 nodes, 1 / 32 / 64 sequences: 27 / 75 / 132 us; 16 CTAs that compute the exponentials again
-  // 27 / 92 / 147, 8 such CTAs 37 / 109 / 124.
+  // So many CTAs that four of them, with a row's exponentials, fit on an SM up to a vocabulary of
+  // about 110 thousand (three up to 149 thousand, two up to 200 thousand; past that each pass computes
+  // them again).  Trees of 16 nodes with probabilities, us for 1 / 32 / 64 sequences; in brackets with
+  // exponentials that are computed again:
+  //   vocabulary    1 CTA             2               4               8               16
+  //     4096    29 / 33 / 33   24 / 27 / 25    21 / 23 / 25    23 / 27 / 31    27 / 37 / 65
+  //    16384                                   18 / 33 / 39    16 / 31 / 37    19 / 44 / 68
+  //    53248                                   64 / 98 / 107   37 / 55 / 62    31 / 49 / 88
+  //   100003                                   59 / 176 / 184  38 / 86 / 153   27 / 76 / 131
+  //                                                           [39 / 111 / 125 27 / 93 / 148]
+  //   128256                                   64 / 215 / 285  39 / 129 / 173  27 / 94 / 186
+  //                                                                           [27 / 96 / 173]
+  //   151936                                   76 / 268 / 321  45 / 152 / 185  33 / 133 / 255
+  //                                                                           [33 / 124 / 213]
+  // By the vocabulary alone: a row of 4096 numbers would be faster with 2 CTAs, and 64 sequences of
+  // wide ones with 8, where one sequence would take a third more.
   const unsigned ctas = p->vocab > 53248 ? 16 : (p->vocab > 16384 ? 8 : (p->vocab > 4096 ? 4 : 1));
   const int64_t warps = static_cast<int64_t>(ctas) * kWarps;
   a.share = static_cast<int32_t>((p->vocab + 4 * warps - 1) / (4 * warps) * 4);

@@ -54,7 +54,8 @@ B200_ATTN_API int32_t b200_cache4_read(const b200_cache* c, int64_t head_dim, in
  * b200_tree_attn_fwd over a 4-bit cache (p->cache as above); queries and output of `dtype`
  * (bf16 or fp16).  The queries are taken as fp16 numbers times a power of two of their row,
  * which loses nothing of a bf16 or fp16 number that is no smaller than 2^-23 of the row's
- * largest (rows whose largest number times the scale is between 2^-113 and 2^116).  Scores, maxima, sums of weights and output sums are fp32, and the output is
+ * largest.  Scores, maxima, sums of weights and output sums are fp32 (scores keep their bits where
+ * the row's largest number times the scale lies between 2^-113 and 2^116), and the output is
  * rounded once.  Up to 16 rows (tokens * heads / kv_heads), and all calls but those below:
  * products with the codes are exact in the tensor cores' fp32 sums; steps and lows are applied
  * in fp32; a weight times the step of its value is rounded to fp16 for the product (with fp16
